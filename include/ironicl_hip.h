@@ -331,6 +331,113 @@ int irx_regression_summary(irx_device *device, const float *decoded, size_t ense
                            size_t quantiles, const float *levels, size_t n_levels, float *mean,
                            float *variance, float *at_levels, float *raw);
 
+/* ---- The 4-bit ICL cache. No counterpart in the reference, whose caches hold
+ * FP32, FP16 or FP8 (cuda/cache.rs). Keys and values of 64-wide heads in 4
+ * bits, the attention over all of them, and attention over the blocks of 64
+ * rows that a cheap score picks for each query. All buffers but the structs
+ * are device memory of `device`; the work is enqueued on `stream` (a
+ * hipStream_t of that device, or NULL for its null stream) and the calls return
+ * without waiting; none allocates, so each may be captured into a HIP graph.
+ * The calling thread's current device is left as it was.
+ *
+ * What a cache holds. E2M1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6, then their
+ * negatives) times 2^e: one e per key and 32 dims, one per value dim and 32 rows,
+ * the smallest with max |x| <= 6 * 2^e, held to -13 .. 13. A number is rounded to
+ * the nearest such value, ties to the even code, larger ones to 6 * 2^13 = 49,152.
+ * Numbers that are not finite are held as 0 and counted. Rows past an
+ * estimator's length are held as 0 and touch no exponent. Every held number is
+ * exact in FP16.
+ *
+ * A cache of P = estimators * heads pairs of T = ceil(rows / 64) blocks is
+ * P * T * 4,480 + P * 256 bytes: per pair and block 4,352 bytes (2,048 of keys'
+ * codes, row 32 s + 16 a + 8 b + i, dim 16 g + 2 y + z at byte [s 2][g 4][a 2][i 8]
+ * [b 2][y 8], nibble z, lower nibble first; 2,048 of values' codes, row 32 s +
+ * 16 t + 8 b + 4 h + 2 y + z, dim 16 d + i at byte [s 2][t 2][h 2][i 16][d 4][b 2]
+ * [y 2], nibble z; 128 of keys' e + 127, dims 32 u .., at [u 2][a 2][i 8][s 2][b 2];
+ * 128 of values' e + 127 at [i 16][s 2][d 4]); then int8 bounds [P, T, 2, 64]; then
+ * their units, FP32 [P, 64]. The unit of a (pair, dim) is the smallest 2^x, x >=
+ * -20, with max |held key| <= 127 * 2^x; a block's bounds are floor(min / 2^x) and
+ * ceil(max / 2^x) over its rows inside the length (0 and 0 when none is). ---- */
+
+typedef enum irx_element { IRX_ELEMENT_F32 = 0, IRX_ELEMENT_F16 = 1 } irx_element;
+
+/* 1 to 65,536 pairs (estimators * heads), 1 to 2^27 rows, 2^40 bytes of cache at most. */
+typedef struct irx_icl4_shape {
+    size_t estimators;
+    size_t heads;
+    size_t rows;
+} irx_icl4_shape;
+
+/* Elements from one estimator, head and row to the next; a row's 64 numbers
+ * are adjacent. Multiples of 16 bytes, as the pointers are. Head-major [E, H,
+ * N, 64] is {H * N * 64, N * 64, 64}, token rows [E, N, H * 64] {N * H * 64, 64,
+ * H * 64}. An input's may be 0 (shared); an output's are at least 64 where there
+ * is more than one, and its rows must not overlap. */
+typedef struct irx_strides {
+    size_t estimator;
+    size_t head;
+    size_t row;
+} irx_strides;
+
+typedef struct irx_icl4_rows {
+    irx_icl4_shape shape;
+    int element;             /* irx_element of k and v */
+    void *k;
+    void *v;
+    irx_strides k_strides;
+    irx_strides v_strides;
+    const uint32_t *lengths; /* [estimators] rows of each (more than rows counts as rows), or NULL: all */
+} irx_icl4_rows;
+
+typedef struct irx_icl4_queries {
+    irx_icl4_shape shape;
+    size_t query_rows;       /* 1 to 2^24 */
+    int element;             /* irx_element of q, and of the attention's output */
+    const void *q;           /* [E, H, query_rows, 64], finite */
+    irx_strides q_strides;
+    const uint32_t *lengths; /* as above: later rows are not attended */
+    const uint64_t *keep;    /* [estimators, T]: row 64 t + r of an estimator is attended where
+                              * bit r of its word t is set, or NULL: every row */
+} irx_icl4_queries;
+
+/* Bytes of a cache (16-byte aligned); 0 for a shape out of range. */
+size_t irx_icl4_bytes(const irx_icl4_shape *shape);
+/* Bytes of workspace (16-byte aligned) with which irx_icl4_select and
+ * irx_icl4_attention run on `device` for query_rows queries and n_blocks chosen
+ * blocks (0: attention over every block); 0 for arguments out of range, or when
+ * none is needed. Calls that may run at once, in graphs too, need one each. */
+size_t irx_icl4_workspace_bytes(irx_device *device, const irx_icl4_shape *shape, size_t query_rows, size_t n_blocks);
+/* Writes `cache` from rows->k and rows->v. nonfinite, when not NULL, is a
+ * device counter to which the numbers that are not finite, inside the lengths,
+ * are added. */
+int irx_icl4_encode(irx_device *device, const irx_icl4_rows *rows, void *cache, uint32_t *nonfinite, void *stream);
+/* Reads what `cache` holds into rows->k and rows->v (either may be NULL; rows
+ * past the lengths are left as they were) and, when not NULL, the bounds times
+ * their units into bounds, FP32 [P, T, 2, 64]. Exact for either element. */
+int irx_icl4_decode(irx_device *device, const void *cache, const irx_icl4_rows *rows, float *bounds, void *stream);
+/* For each (estimator, head, query) the n_blocks (1 to 4,096) blocks with the
+ * highest scores among those with a row to attend to, ties to the lower block,
+ * into blocks [E, H, query_rows, n_blocks]: ascending, then -1 where there are
+ * fewer. A score bounds q k over the block's rows: with x = q * unit, f the
+ * smallest integer >= -100 with max |x| <= 127 * 2^f and c = x / 2^f rounded to
+ * the nearest integer (ties to even), it is sum over the dims of max(c low, c
+ * high), a whole number. */
+int irx_icl4_select(irx_device *device, const irx_icl4_queries *queries, const void *cache, size_t n_blocks,
+                    int32_t *blocks, void *workspace, size_t workspace_bytes, void *stream);
+/* softmax(scale q k^T) v over the attended rows, scale finite and positive, into
+ * out [E, H, query_rows, 64] at out_strides; a query that attends to no row gets
+ * 0. With blocks (n_blocks of them per query, as irx_icl4_select writes) only
+ * the listed blocks' rows are attended; entries that are no block of the cache
+ * are skipped, and a block that is listed twice counts twice. blocks NULL and
+ * n_blocks 0: every block. lse, when not NULL, [E, H, query_rows] FP32: the
+ * natural logarithm of the sum of exp(scale q k), -inf for a query that attends
+ * to none. FP32 queries and weights are multiplied as pairs of FP16 values (22
+ * bits), FP16 queries as they are with weights rounded once to FP16; sums are
+ * FP32. Results do not depend on other calls or on the workspace's contents. */
+int irx_icl4_attention(irx_device *device, const irx_icl4_queries *queries, const void *cache, float scale,
+                       const int32_t *blocks, size_t n_blocks, void *out, const irx_strides *out_strides, float *lse,
+                       void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- Kernel harness (cuda/testing.rs:27-207): one kernel family on host data ---- */
 
 /* softmax(q k^T / 8) v for `pairs` (estimator, head) pairs: q [pairs, query_rows, 64],

@@ -455,6 +455,55 @@ void pack_icl16(const void *k, const void *v, bool src_f16, long long rows, int 
 void unpack_icl16(const unsigned short *k16, const unsigned short *v16, long long rows, int pairs,
                   unsigned short *k, unsigned short *v, hipStream_t stream);
 
+// The 4-bit ICL cache (icl4.hip): rows in blocks of 64 per (estimator, head)
+// pair, then every block's bounds and their scales; the layout stands there.
+constexpr int kIcl4Block = 64;
+constexpr int kIcl4BlockBytes = 4352;
+struct Icl4Shape {
+    int estimators, heads, rows;
+    int pairs() const { return estimators * heads; }
+    int blocks() const { return (rows + kIcl4Block - 1) / kIcl4Block; }
+};
+// Keys and values [estimators, heads, rows, 64], FP32 or FP16 (half), at
+// strides in elements per estimator, head and row.
+struct Icl4Rows {
+    Icl4Shape shape;
+    bool half;
+    void *k, *v;
+    long long k_strides[3], v_strides[3];
+    const unsigned *lengths;  // [estimators] on the device, or null: every row
+};
+struct Icl4Queries {
+    Icl4Shape shape;
+    bool half;
+    const void *cache;
+    const void *q;
+    long long q_strides[3];
+    int q_rows;
+    const unsigned *lengths;
+    const unsigned long long *keep;  // [estimators, blocks]: bit r of a block's word, or null
+    int compute_units;
+};
+struct Icl4Attend {
+    float scale;
+    const int *list;  // [pairs, q_rows, n] blocks, or null: all
+    int n;
+    void *out;
+    long long o_strides[3];
+    float *lse;       // [pairs, q_rows] or null
+    void *workspace;
+};
+size_t icl4_bytes(const Icl4Shape &s);
+size_t icl4_attend_workspace(const Icl4Shape &s, int q_rows, int n_blocks, int compute_units);
+size_t icl4_select_workspace(const Icl4Shape &s, int q_rows);
+// Whether the attention's workgroups can be one launch.
+bool icl4_grid_fits(const Icl4Shape &s, int q_rows, int n_blocks, int compute_units);
+void icl4_encode(const Icl4Rows &a, void *cache, unsigned *nonfinite, hipStream_t stream);
+// a.k and a.v (either may be null) are written.
+void icl4_decode(const Icl4Rows &a, const void *cache, float *bounds, hipStream_t stream);
+void icl4_select(const Icl4Queries &a, int n, int *out, void *workspace, hipStream_t stream);
+void icl4_attend(const Icl4Queries &a, const Icl4Attend &b, hipStream_t stream);
+
 // TabICL preprocessing (preprocess.hip), in f64. Fit: statistics of every
 // kept feature, [groups, 9, kept_count] (mean, scale, minimum, maximum,
 // lower, upper, then lambda, mean, scale of the power transform), and a

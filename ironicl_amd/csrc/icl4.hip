@@ -1,0 +1,788 @@
+// The 4-bit ICL cache: its writer and reader, the attention over it, and the
+// choice of blocks for attention over a part of it.
+//
+// A cache holds keys and values of 64-wide heads, [pairs, rows, 64] with pair
+// = estimator * heads + head, as E2M1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and
+// their negatives) times powers of two 2^e: one e per key and 32 dims, one per
+// value dim and 32 rows, the smallest with max |x| <= 6 * 2^e, held to -13..13.
+// Every held number is then exact in FP16 (2^-14 at least, 49,152 at most, or
+// zero), so the FP16 matrix cores take it without another rounding. Rows go in
+// blocks of 64, each 4,352 contiguous bytes in the order in which the
+// 16x16x32 products read them:
+//   0     keys' codes [s 2][g 4][a 2][i 8][b 2][8 bytes]: row 32 s + 16 a +
+//         8 b + i, dims 16 g .. +15, the lower dim in the lower nibble
+//   2048  values' codes [s 2][t 2][h 2][i 16][d 4][b 2][2 bytes]: dim 16 d + i,
+//         rows 32 s + 16 t + 8 b + 4 h .. +3, the lower row in the lower nibble
+//   4096  keys' e + 127, bytes [32 dims 2][a 2][i 8][s 2][b 2]
+//   4224  values' e + 127, bytes [i 16][s 2][d 4]
+// Lane 16 g + (8 a + i) of a wave finds its operands of rows 32 s .. +31 in 16
+// contiguous bytes of keys and 16 of values (g = 2 t + h).
+// After the blocks of every pair come their bounds, int8 [pairs, blocks, low
+// and high, 64], and the bounds' scales, FP32 [pairs, 64] (powers of two).
+#include "common.hpp"
+
+#include <algorithm>
+#include <cmath>
+
+namespace irx {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kBlock = kIcl4Block;            // rows of a block
+constexpr int kBlockBytes = kIcl4BlockBytes;  // bytes of one pair's block
+constexpr int kValuesAt = 2048, kKeyExpsAt = 4096, kValueExpsAt = 4224;
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(_Float16 x) { return (float)x; }
+
+// 2^(byte - 127) of byte `i` of a word.
+template <int I>
+__device__ __forceinline__ float exp_byte(unsigned word) {
+    return __uint_as_float(((word >> (8 * I)) & 0xffu) << 23);
+}
+
+// Eight E2M1 codes times `scale` (a power of two) as FP16, exactly.
+__device__ __forceinline__ half8 codes8(unsigned word, float scale) {
+    const half2v a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, scale, 0);
+    const half2v b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, scale, 1);
+    const half2v c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, scale, 2);
+    const half2v d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, scale, 3);
+    return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// Rows that estimator e's queries may attend to.
+__device__ __forceinline__ int rows_of(const unsigned *lengths, int e, int rows) {
+    return lengths ? (int)min(lengths[e], (unsigned)rows) : rows;
+}
+
+// Bit r: row 64 block + r is attended.
+__device__ __forceinline__ unsigned long long block_mask(const unsigned long long *keep, int e, int blocks, int block,
+                                                         int rows) {
+    const int left = rows - block * kBlock;
+    if (left <= 0) return 0;
+    unsigned long long m = keep ? keep[(long long)e * blocks + block] : ~0ull;
+    if (left < kBlock) m &= (1ull << left) - 1;
+    return m;
+}
+
+// ---- writing ----
+
+// The smallest e with m <= 6 * 2^e, held to -13..13 (m finite).
+__device__ __forceinline__ int code_exponent(float m) {
+    if (m == 0.f) return -13;
+    const unsigned bits = __float_as_uint(m);
+    // m = f * 2^x with f in [0.5, 1); subnormal m ends at -13 whatever x is.
+    const int x = (int)(bits >> 23) - 126;
+    return min(13, max(-13, (bits & 0x7fffffu) <= 0x400000u ? x - 3 : x - 2));
+}
+
+// The E2M1 code of x / 2^e: to nearest, ties to the even code, saturated.
+__device__ __forceinline__ unsigned code_of(float x, float inv) {
+    const float m = fabsf(x) * inv;
+    const unsigned c = (m > 0.25f) + (m >= 0.75f) + (m > 1.25f) + (m >= 1.75f) + (m > 2.5f) + (m >= 3.5f) + (m > 5.0f);
+    return c | (x < 0.f ? 8u : 0u);
+}
+
+__device__ __forceinline__ float value_of(unsigned code, float scale) {
+    const unsigned c = code & 7u;
+    // 0, 0.5, then 1.m * 2^(c / 2 - 1) with m the low bit.
+    const float m = c < 2u ? 0.5f * (float)c : (1.0f + 0.5f * (float)(c & 1u)) * (float)(1u << ((c >> 1) - 1));
+    return (code & 8u ? -m : m) * scale;
+}
+
+// The smallest unit 2^x with m <= 127 * 2^x (m a held key; 2^-20 for zero).
+__device__ __forceinline__ float bound_unit(float m) {
+    if (m == 0.f) return pow2(-20);
+    const unsigned bits = __float_as_uint(m);
+    const int x = (int)(bits >> 23) - 126;  // m = f 2^x, f in [0.5, 1); f <= 127/128?
+    return pow2((bits & 0x7fffffu) <= 0x7e0000u ? x - 7 : x - 6);
+}
+
+struct StoreArgs {
+    const void *k, *v;
+    long long k_est, k_head, k_row, v_est, v_head, v_row;
+    const unsigned *lengths;
+    int heads, pairs, rows, blocks;
+    unsigned char *tiles;
+    signed char *bounds;
+    float *scales;
+    unsigned *nonfinite;
+};
+
+__global__ __launch_bounds__(256) void icl4_units_kernel(float *scales, int count) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < count) scales[i] = 9.5367431640625e-07f;  // 2^-20
+}
+
+// One workgroup per (block, pair): codes and exponents; the bounds' scales by
+// maxima of 2^x (as words, so their order does not matter).
+template <typename T>
+__global__ __launch_bounds__(256) void icl4_encode_kernel(StoreArgs p) {
+    __shared__ float held[64][65];
+    __shared__ float part_max[4][64];
+    const int tid = threadIdx.x;
+    const int block = (int)(blockIdx.x % (unsigned)p.blocks), pair = (int)(blockIdx.x / (unsigned)p.blocks);
+    const int e = pair / p.heads, head = pair - e * p.heads;
+    const int rows = rows_of(p.lengths, e, p.rows);
+    unsigned char *out = p.tiles + ((long long)pair * p.blocks + block) * kBlockBytes;
+    unsigned bad = 0;
+    {  // Keys: thread t takes dims 16 (t % 4) .. +15 of row t / 4.
+        const int r = tid >> 2, g = tid & 3;
+        const long long row = (long long)block * kBlock + r;
+        float x[16];
+        float m = 0.f;
+        const T *src = static_cast<const T *>(p.k) + e * p.k_est + head * p.k_head + row * p.k_row + 16 * g;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            x[i] = row < rows ? to_float(src[i]) : 0.f;
+            if (!(fabsf(x[i]) <= 3.4028235e38f)) x[i] = 0.f, ++bad;
+            m = fmaxf(m, fabsf(x[i]));
+        }
+        m = fmaxf(m, __shfl_xor(m, 1, 64));
+        const int ex = code_exponent(m);
+        const float inv = pow2(-ex), scale = pow2(ex);
+        unsigned w[2] = {0u, 0u};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const unsigned c = code_of(x[i], inv);
+            w[i >> 3] |= c << (4 * (i & 7));
+            held[r][16 * g + i] = fabsf(value_of(c, scale));
+        }
+        const int s = r >> 5, a = (r >> 4) & 1, b = (r >> 3) & 1, i8 = r & 7;
+        *reinterpret_cast<u32x2 *>(out + s * 1024 + (16 * g + 8 * a + i8) * 16 + b * 8) = u32x2{w[0], w[1]};
+        if (!(g & 1)) out[kKeyExpsAt + ((g >> 1) * 16 + 8 * a + i8) * 4 + 2 * s + b] = (unsigned char)(ex + 127);
+    }
+    __syncthreads();
+    {  // Largest held |key| of each dim, into the bounds' scales.
+        const int d = tid & 63, q = tid >> 6;
+        float m = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) m = fmaxf(m, held[16 * q + i][d]);
+        part_max[q][d] = m;
+    }
+    __syncthreads();
+    if (tid < 64) {
+        const float m = fmaxf(fmaxf(part_max[0][tid], part_max[1][tid]), fmaxf(part_max[2][tid], part_max[3][tid]));
+        atomicMax(reinterpret_cast<unsigned *>(p.scales) + pair * 64 + tid, __float_as_uint(bound_unit(m)));
+    }
+    __syncthreads();
+    {  // Values: thread t takes rows 16 (t / 64) .. +15 of dim t % 64.
+        const int d = tid & 63, q = tid >> 6;
+        float x[16];
+        float m = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const long long row = (long long)block * kBlock + 16 * q + i;
+            const T *src = static_cast<const T *>(p.v) + e * p.v_est + head * p.v_head + row * p.v_row + d;
+            x[i] = row < rows ? to_float(*src) : 0.f;
+            if (!(fabsf(x[i]) <= 3.4028235e38f)) x[i] = 0.f, ++bad;
+            m = fmaxf(m, fabsf(x[i]));
+        }
+        part_max[q][d] = m;
+        __syncthreads();
+        m = fmaxf(m, part_max[q ^ 1][d]);
+        const int ex = code_exponent(m);
+        const float inv = pow2(-ex);
+        const int s = q >> 1, t = q & 1;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            unsigned w = 0u;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w |= code_of(x[8 * b + 4 * h + j], inv) << (4 * (4 * b + j));
+            *reinterpret_cast<unsigned *>(out + kValuesAt + s * 1024 + (16 * (2 * t + h) + (d & 15)) * 16 +
+                                          (d >> 4) * 4) = w;
+        }
+        if (!t) out[kValueExpsAt + (d & 15) * 8 + s * 4 + (d >> 4)] = (unsigned char)(ex + 127);
+    }
+    if (bad && p.nonfinite) atomicAdd(p.nonfinite, bad);
+}
+
+// Bounds of one block per wave, from the codes: lane 16 g + i16 holds dims
+// 16 g .. +15 of four rows; the 16 lanes of a g join theirs.
+__global__ __launch_bounds__(256) void icl4_bounds_kernel(StoreArgs p) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, i16 = lane & 15;
+    const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (at >= (long long)p.pairs * p.blocks) return;
+    const int pair = (int)(at / p.blocks), block = (int)(at - (long long)pair * p.blocks);
+    const int rows = rows_of(p.lengths, pair / p.heads, p.rows);
+    const int left = rows - block * kBlock;
+    const unsigned char *in = p.tiles + at * kBlockBytes;
+    const unsigned exps = *reinterpret_cast<const unsigned *>(in + kKeyExpsAt + ((g >> 1) * 16 + i16) * 4);
+    float lo[16], hi[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) lo[i] = INFINITY, hi[i] = -INFINITY;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(in + s * 1024 + lane * 16);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const int r = 32 * s + 16 * (i16 >> 3) + 8 * b + (i16 & 7);
+            const float scale = __uint_as_float(((exps >> (8 * (2 * s + b))) & 0xffu) << 23);
+            if (r < left) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float x = value_of((w[2 * b + (i >> 3)] >> (4 * (i & 7))) & 15u, scale);
+                    lo[i] = fminf(lo[i], x), hi[i] = fmaxf(hi[i], x);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+#pragma unroll
+        for (int off = 1; off < 16; off *= 2) {
+            lo[i] = fminf(lo[i], __shfl_xor(lo[i], off, 64));
+            hi[i] = fmaxf(hi[i], __shfl_xor(hi[i], off, 64));
+        }
+    if (i16 == 0) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float inv = 1.0f / p.scales[pair * 64 + 16 * g + i];
+            p.bounds[at * 128 + 16 * g + i] = left > 0 ? (signed char)floorf(lo[i] * inv) : (signed char)0;
+            p.bounds[at * 128 + 64 + 16 * g + i] = left > 0 ? (signed char)ceilf(hi[i] * inv) : (signed char)0;
+        }
+    }
+}
+
+struct ReadArgs {
+    void *k, *v;
+    long long k_est, k_head, k_row, v_est, v_head, v_row;
+    const unsigned *lengths;
+    int heads, pairs, rows, blocks;
+    const unsigned char *tiles;
+    const signed char *bounds;
+    const float *scales;
+    float *bounds_out;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void icl4_decode_kernel(ReadArgs p) {
+    const int tid = threadIdx.x;
+    const int block = (int)(blockIdx.x % (unsigned)p.blocks), pair = (int)(blockIdx.x / (unsigned)p.blocks);
+    const int e = pair / p.heads, head = pair - e * p.heads;
+    const int rows = rows_of(p.lengths, e, p.rows);
+    const long long at = (long long)pair * p.blocks + block;
+    const unsigned char *in = p.tiles + at * kBlockBytes;
+    const int r = tid >> 2, g = tid & 3;
+    const long long row = (long long)block * kBlock + r;
+    const int s = r >> 5, a = (r >> 4) & 1, b = (r >> 3) & 1, i8 = r & 7;
+    if (row < rows) {
+        if (p.k) {
+            const unsigned *w = reinterpret_cast<const unsigned *>(in + s * 1024 + (16 * g + 8 * a + i8) * 16 + b * 8);
+            const float scale = pow2((int)in[kKeyExpsAt + ((g >> 1) * 16 + 8 * a + i8) * 4 + 2 * s + b] - 127);
+            T *dst = static_cast<T *>(p.k) + e * p.k_est + head * p.k_head + row * p.k_row + 16 * g;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dst[i] = (T)value_of((w[i >> 3] >> (4 * (i & 7))) & 15u, scale);
+        }
+        if (p.v) {
+            const int t = a, h = (r >> 2) & 1, j = r & 3;
+            T *dst = static_cast<T *>(p.v) + e * p.v_est + head * p.v_head + row * p.v_row + 16 * g;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const unsigned c = in[kValuesAt + s * 1024 + (16 * (2 * t + h) + i) * 16 + g * 4 + 2 * b + (j >> 1)];
+                const float scale = pow2((int)in[kValueExpsAt + i * 8 + s * 4 + g] - 127);
+                dst[i] = (T)value_of((c >> (4 * (j & 1))) & 15u, scale);
+            }
+        }
+    }
+    if (p.bounds_out && tid < 128)
+        p.bounds_out[at * 128 + tid] = (float)p.bounds[at * 128 + tid] * p.scales[pair * 64 + (tid & 63)];
+}
+
+// ---- choosing blocks ----
+
+struct SelectArgs {
+    const void *q;
+    long long q_est, q_head, q_row;
+    const unsigned *lengths;
+    const unsigned long long *keep;
+    int heads, pairs, q_rows, rows, blocks;
+    const signed char *bounds;
+    const float *scales;
+    int n;
+    int *out;
+    int *scores;         // [rows of this launch, blocks]
+    long long first;     // the first (pair, query) of this launch
+};
+
+constexpr int kNoScore = -(1 << 30);
+
+// One workgroup per (pair, query): every block's score, the n-th largest by
+// bisection, and the blocks above it in order.
+template <typename T>
+__global__ __launch_bounds__(256) void icl4_select_kernel(SelectArgs p) {
+    __shared__ unsigned pos[16], neg[16];
+    __shared__ int count, base, equal_base;
+    __shared__ int wave_above[4], wave_equal[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const long long pq = p.first + blockIdx.x;
+    const int pair = (int)(pq / p.q_rows), row = (int)(pq - (long long)pair * p.q_rows);
+    const int e = pair / p.heads, head = pair - e * p.heads;
+    const int rows = rows_of(p.lengths, e, p.rows);
+    int *scores = p.scores + (long long)blockIdx.x * p.blocks;
+    int *out = p.out + pq * p.n;
+    if (wave == 0) {
+        const T *src = static_cast<const T *>(p.q) + e * p.q_est + head * p.q_head + row * p.q_row;
+        const float x = to_float(src[lane]) * p.scales[pair * 64 + lane];
+        const float m = wave_max(fabsf(x));
+        int f = -100;
+        if (m > 0.f) {
+            const unsigned bits = __float_as_uint(m);
+            const int ex = (int)(bits >> 23) - 126;
+            f = min(120, max(-100, (bits & 0x7fffffu) <= 0x7e0000u ? ex - 7 : ex - 6));
+        }
+        const float c = rintf(fminf(fmaxf(x * pow2(-f), -127.f), 127.f));
+        reinterpret_cast<signed char *>(pos)[lane] = (signed char)fmaxf(c, 0.f);
+        reinterpret_cast<signed char *>(neg)[lane] = (signed char)fminf(c, 0.f);
+    }
+    if (tid == 0) count = 0;
+    __syncthreads();
+    int candidates = 0;
+    for (int b = tid; b < p.blocks; b += 256) {
+        int s = kNoScore;
+        if (block_mask(p.keep, e, p.blocks, b, rows)) {
+            const unsigned *w = reinterpret_cast<const unsigned *>(p.bounds + ((long long)pair * p.blocks + b) * 128);
+            s = 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s = __builtin_amdgcn_sdot4((int)neg[i], (int)w[i], s, false);
+                s = __builtin_amdgcn_sdot4((int)pos[i], (int)w[16 + i], s, false);
+            }
+            ++candidates;
+        }
+        scores[b] = s;
+    }
+    if (candidates) atomicAdd(&count, candidates);
+    __syncthreads();
+    const int total = count;
+    __syncthreads();
+    // The largest v that at least n scores reach (every candidate when there are no more than n).
+    int lo = -(1 << 21), hi = 1 << 21;  // count(>= lo) >= n > count(>= hi)
+    if (total > p.n) {
+        while (hi - lo > 1) {
+            const int mid = lo + (hi - lo) / 2;
+            if (tid == 0) count = 0;
+            __syncthreads();
+            int c = 0;
+            for (int b = tid; b < p.blocks; b += 256) c += scores[b] >= mid;
+            if (c) atomicAdd(&count, c);
+            __syncthreads();
+            if (count >= p.n)
+                lo = mid;
+            else
+                hi = mid;
+            __syncthreads();
+        }
+    }
+    // Blocks above lo, and the first of those at lo that there is room for.
+    if (tid == 0) count = 0;
+    __syncthreads();
+    int c = 0;
+    for (int b = tid; b < p.blocks; b += 256) c += scores[b] > lo;
+    if (c) atomicAdd(&count, c);
+    __syncthreads();
+    const int room = p.n - count;
+    if (tid == 0) base = 0, equal_base = 0;
+    __syncthreads();
+    for (int b0 = 0; b0 < p.blocks; b0 += 256) {
+        const int b = b0 + tid;
+        const int s = b < p.blocks ? scores[b] : kNoScore;
+        const bool above = s > lo, equal = s == lo;
+        const unsigned long long va = __ballot(above), ve = __ballot(equal);
+        const unsigned long long below = (1ull << lane) - 1;
+        if (lane == 0) wave_above[wave] = __popcll(va), wave_equal[wave] = __popcll(ve);
+        __syncthreads();
+        int before_above = base, before_equal = equal_base;
+        for (int w = 0; w < wave; ++w) before_above += wave_above[w], before_equal += wave_equal[w];
+        before_above += __popcll(va & below), before_equal += __popcll(ve & below);
+        const int at = before_above + min(before_equal, room);
+        if (above || (equal && before_equal < room)) out[at] = b;
+        __syncthreads();
+        if (tid == 0)
+            for (int w = 0; w < 4; ++w) base += wave_above[w], equal_base += wave_equal[w];
+        __syncthreads();
+    }
+    for (int i = min(total, p.n) + tid; i < p.n; i += 256) out[i] = -1;
+}
+
+// ---- attention ----
+
+struct AttendArgs {
+    const void *q;
+    long long q_est, q_head, q_row;
+    void *o;
+    long long o_est, o_head, o_row;
+    float *lse;
+    const unsigned char *tiles;
+    const unsigned *lengths;
+    const unsigned long long *keep;
+    const int *list;  // [pairs, q_rows, n] or null
+    int n;
+    int heads, pairs, q_rows, rows, blocks;
+    float scale;      // times log2 e
+    float *partial;   // outputs [splits, pairs * q_rows, 64], then log2-sum-exps [splits, pairs * q_rows]
+    int splits, per_split;  // blocks (or listed places) of a split
+    int qtiles;
+};
+
+constexpr float kLn2 = 0.69314718055994530942f;
+// Probabilities are held against a reference 2^8 below the largest so far, so
+// that FP16's smallest step, 2^-24, is 2^-32 of the largest.
+constexpr float kHeadroom = 8.0f;
+
+// The writer of one query's output: dims d .. +3.
+template <typename T>
+__device__ __forceinline__ void store_out(const AttendArgs &p, int pair, int row, int d, f32x4 v) {
+    const int e = pair / p.heads, head = pair - e * p.heads;
+    T *dst = static_cast<T *>(p.o) + e * p.o_est + head * p.o_head + row * p.o_row + d;
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<f32x4 *>(dst) = v;
+    } else {
+        typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<half4 *>(dst) = __builtin_convertvector(v, half4);
+    }
+}
+
+constexpr int kWaves = 4;
+
+// One workgroup per (16 queries, pair, split), or per (query, pair, split)
+// over listed blocks: wave w takes every fourth block of the split. FP32
+// queries and probabilities are pairs of FP16 values, two products each.
+template <typename T, bool LISTED, bool SPLIT>
+__global__ __launch_bounds__(kWaves * 64) void icl4_rows_kernel(AttendArgs p) {
+    constexpr bool PAIRS = sizeof(T) == 4;
+    __shared__ float red_o[kWaves][16 * 68];
+    __shared__ float red_m[kWaves][16], red_l[kWaves][16];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, i16 = lane & 15;
+    unsigned id = blockIdx.x;
+    const int split = (int)(id % (unsigned)p.splits);
+    id /= (unsigned)p.splits;
+    const int qt = (int)(id % (unsigned)p.qtiles), pair = (int)(id / (unsigned)p.qtiles);
+    const int e = pair / p.heads, head = pair - e * p.heads;
+    const int rows = rows_of(p.lengths, e, p.rows);
+    const int qrow = LISTED ? qt : min(16 * qt + i16, p.q_rows - 1);
+    half8 qh[2], ql[2];
+    float c = p.scale;
+    {
+        const T *src = static_cast<const T *>(p.q) + e * p.q_est + head * p.q_head + (long long)qrow * p.q_row + 16 * g;
+        if constexpr (PAIRS) {
+            float x[16];
+            float m = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x4 v = *reinterpret_cast<const f32x4 *>(src + 4 * i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[4 * i + j] = v[j], m = fmaxf(m, fabsf(v[j]));
+            }
+            m = fmaxf(m, __shfl_xor(m, 16, 64));
+            m = fmaxf(m, __shfl_xor(m, 32, 64));
+            const int ex = pair_exponent(m);
+            const float up = pow2(ex);
+            c *= pow2(-ex);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] *= up;
+            pair8(x, qh[0], ql[0]);
+            pair8(x + 8, qh[1], ql[1]);
+        } else {
+            qh[0] = *reinterpret_cast<const half8 *>(src);
+            qh[1] = *reinterpret_cast<const half8 *>(src + 8);
+        }
+    }
+    f32x4 o[4];
+#pragma unroll
+    for (int d = 0; d < 4; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m_run = -INFINITY, l_run = 0.f;  // m_run: the largest score less the headroom
+    const unsigned char *tiles = p.tiles + (long long)pair * p.blocks * kBlockBytes;
+    const int places = LISTED ? p.n : p.blocks;
+    const int end = min(places, (split + 1) * p.per_split);
+    for (int at = split * p.per_split + wave; at < end; at += kWaves) {
+        int block = at;
+        if constexpr (LISTED) {
+            block = p.list[((long long)pair * p.q_rows + qt) * p.n + at];
+            if ((unsigned)block >= (unsigned)p.blocks) continue;
+        }
+        const unsigned long long mask = block_mask(p.keep, e, p.blocks, block, rows);
+        if (mask == 0) continue;
+        const unsigned char *in = tiles + (long long)block * kBlockBytes;
+        const unsigned ke = *reinterpret_cast<const unsigned *>(in + kKeyExpsAt + ((g >> 1) * 16 + i16) * 4);
+        const u32x2 ve = *reinterpret_cast<const u32x2 *>(in + kValueExpsAt + i16 * 8);
+        f32x4 s[4];
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) {
+            const u32x2 w = *reinterpret_cast<const u32x2 *>(in + (kb >> 1) * 1024 + lane * 16 + (kb & 1) * 8);
+            const float scale = __uint_as_float(((ke >> (8 * kb)) & 0xffu) << 23);
+            s[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                const half8 a = codes8(w[m], scale);
+                if constexpr (PAIRS) s[kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[m], s[kb], 0, 0, 0);
+                s[kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[m], s[kb], 0, 0, 0);
+            }
+            s[kb] *= c;
+        }
+        // Register r of s[2 s + b]: row 32 s + 16 (g / 2) + 8 b + 4 (g % 2) + r.
+        if (mask != ~0ull) {
+            const unsigned long long mine = mask >> (16 * (g >> 1) + 4 * (g & 1));
+#pragma unroll
+            for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (!((mine >> (32 * (kb >> 1) + 8 * (kb & 1) + r)) & 1)) s[kb][r] = -INFINITY;
+        }
+        float mt = s[0][0];
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) mt = fmaxf(mt, s[kb][r]);
+        mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
+        mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+        const float m_new = fmaxf(m_run, mt - kHeadroom);  // finite: the block has an attended row
+        const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+        m_run = m_new;
+        l_run *= alpha;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) o[d] *= alpha;
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i] = __builtin_amdgcn_exp2f(s[2 * st + (i >> 2)][i & 3] - m_new);
+                l_run += x[i];
+            }
+            half8 ph, pl;
+            if constexpr (PAIRS) {
+                pair8(x, ph, pl);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) ph[i] = (_Float16)x[i];
+            }
+            const u32x4 w = *reinterpret_cast<const u32x4 *>(in + kValuesAt + st * 1024 + lane * 16);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                const half8 a = codes8(w[d], __uint_as_float(((ve[st] >> (8 * d)) & 0xffu) << 23));
+                if constexpr (PAIRS) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl, o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph, o[d], 0, 0, 0);
+            }
+        }
+    }
+    // The waves' parts: lane (g, i16) holds dims 16 d + 4 g + r of query i16.
+    l_run += __shfl_xor(l_run, 16, 64);
+    l_run += __shfl_xor(l_run, 32, 64);
+    if (g == 0) red_m[wave][i16] = m_run, red_l[wave][i16] = l_run;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) *reinterpret_cast<f32x4 *>(&red_o[wave][i16 * 68 + 16 * d + 4 * g]) = o[d];
+    __syncthreads();
+    const int qi = threadIdx.x >> 4, d = 4 * (threadIdx.x & 15);
+    const int out_row = LISTED ? qt : 16 * qt + qi;
+    if ((LISTED && qi) || out_row >= p.q_rows) return;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, red_m[w][qi]);
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    float den = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        // Nothing attended: every part is zero. (A query that is not finite gives NaN.)
+        const float a = mx > -INFINITY ? __builtin_amdgcn_exp2f(red_m[w][qi] - mx) : 1.0f;
+        acc += a * *reinterpret_cast<const f32x4 *>(&red_o[w][qi * 68 + d]);
+        den += a * red_l[w][qi];
+    }
+    if (den != 0.f) acc *= 1.0f / den;
+    const float lse2 = mx + log2f(den);  // -inf where nothing is attended
+    if constexpr (SPLIT) {
+        const long long all = (long long)p.pairs * p.q_rows;
+        const long long at = split * all + (long long)pair * p.q_rows + out_row;
+        *reinterpret_cast<f32x4 *>(p.partial + at * 64 + d) = acc;
+        if (d == 0) p.partial[p.splits * all * 64 + at] = lse2;
+    } else {
+        store_out<T>(p, pair, out_row, d, acc);
+        if (p.lse && d == 0) p.lse[(long long)pair * p.q_rows + out_row] = lse2 * kLn2;
+    }
+}
+
+// Splits' outputs weighted by their sums: 16 lanes per (pair, query).
+template <typename T>
+__global__ __launch_bounds__(256) void icl4_merge_kernel(AttendArgs p) {
+    const long long all = (long long)p.pairs * p.q_rows;
+    const long long pq = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+    if (pq >= all) return;
+    const int d = 4 * (threadIdx.x & 15);
+    const float *lse = p.partial + p.splits * all * 64 + pq;
+    float mx = -INFINITY;
+    for (int s = 0; s < p.splits; ++s) mx = fmaxf(mx, lse[s * all]);
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    float den = 0.f;
+    const float ref = mx > -INFINITY ? mx : 0.f;
+    for (int s = 0; s < p.splits; ++s) {
+        const float a = __builtin_amdgcn_exp2f(lse[s * all] - ref);
+        acc += a * *reinterpret_cast<const f32x4 *>(p.partial + (s * all + pq) * 64 + d);
+        den += a;
+    }
+    if (den != 0.f) acc *= 1.0f / den;
+    const int pair = (int)(pq / p.q_rows), row = (int)(pq - (long long)pair * p.q_rows);
+    store_out<T>(p, pair, row, d, acc);
+    if (p.lse && d == 0) p.lse[pq] = (ref + log2f(den)) * kLn2;
+}
+
+struct Plan {
+    int qtiles, splits, per_split;
+    long long rows;  // (pair, query) rows
+};
+
+// About two workgroups per compute unit, at least four blocks to a split (one to a wave).
+Plan plan_attend(const Icl4Shape &s, int q_rows, int n_blocks, int compute_units) {
+    Plan pl{};
+    const int places = n_blocks ? n_blocks : s.blocks();
+    pl.qtiles = n_blocks ? q_rows : (int)ceil_div(q_rows, 16);
+    pl.rows = (long long)s.pairs() * q_rows;
+    const long long base = (long long)s.pairs() * pl.qtiles;
+    const long long want = std::max<long long>(1, (2LL * compute_units + base - 1) / base);
+    const int splits = (int)std::min<long long>(want, std::max(1, places / kWaves));
+    pl.per_split = (int)ceil_div(ceil_div(places, splits), kWaves) * kWaves;
+    pl.splits = (int)ceil_div(places, pl.per_split);
+    return pl;
+}
+
+// Scores of one launch: at most 64 MiB of them.
+long long select_rows(const Icl4Shape &s, long long rows) {
+    return std::max<long long>(1, std::min<long long>(rows, (16LL << 20) / s.blocks()));
+}
+
+struct Parts {
+    unsigned char *tiles;
+    signed char *bounds;
+    float *scales;
+};
+Parts parts(const void *cache, const Icl4Shape &s) {
+    unsigned char *p = static_cast<unsigned char *>(const_cast<void *>(cache));
+    const size_t blocks = (size_t)s.pairs() * s.blocks();
+    return {p, reinterpret_cast<signed char *>(p + blocks * kBlockBytes),
+            reinterpret_cast<float *>(p + blocks * (kBlockBytes + 128))};
+}
+
+template <typename T>
+void attend(const Icl4Queries &a, const Icl4Attend &b, hipStream_t stream) {
+    const Icl4Shape &s = a.shape;
+    const Plan pl = plan_attend(s, a.q_rows, b.list ? b.n : 0, a.compute_units);
+    AttendArgs p{};
+    p.q = a.q, p.q_est = a.q_strides[0], p.q_head = a.q_strides[1], p.q_row = a.q_strides[2];
+    p.o = b.out, p.o_est = b.o_strides[0], p.o_head = b.o_strides[1], p.o_row = b.o_strides[2];
+    p.lse = b.lse, p.tiles = parts(a.cache, s).tiles, p.lengths = a.lengths, p.keep = a.keep;
+    p.list = b.list, p.n = b.n, p.heads = s.heads, p.pairs = s.pairs(), p.q_rows = a.q_rows, p.rows = s.rows;
+    p.blocks = s.blocks(), p.scale = b.scale * kLog2e, p.partial = static_cast<float *>(b.workspace);
+    p.splits = pl.splits, p.per_split = pl.per_split, p.qtiles = pl.qtiles;
+    const dim3 grid((unsigned)((long long)pl.splits * pl.qtiles * s.pairs())), wg(kWaves * 64);
+    {
+        const long long tiles = b.list ? (long long)pl.rows * b.n : (long long)s.pairs() * s.blocks();
+        const double work = 256.0 * kBlock * (b.list ? (double)tiles : (double)tiles * a.q_rows);
+        KernelTimer timer(kFamIcl, stream, work, (double)tiles * kBlockBytes + 2.0 * sizeof(T) * 64 * pl.rows);
+        if (b.list && pl.splits > 1)
+            hipLaunchKernelGGL((icl4_rows_kernel<T, true, true>), grid, wg, 0, stream, p);
+        else if (b.list)
+            hipLaunchKernelGGL((icl4_rows_kernel<T, true, false>), grid, wg, 0, stream, p);
+        else if (pl.splits > 1)
+            hipLaunchKernelGGL((icl4_rows_kernel<T, false, true>), grid, wg, 0, stream, p);
+        else
+            hipLaunchKernelGGL((icl4_rows_kernel<T, false, false>), grid, wg, 0, stream, p);
+        IRX_HIP(hipGetLastError());
+    }
+    if (pl.splits > 1) {
+        KernelTimer timer(kFamIclMerge, stream, 0.0, 4.0 * pl.rows * (65.0 * pl.splits + 64.0));
+        hipLaunchKernelGGL(icl4_merge_kernel<T>, dim3(ceil_div((size_t)pl.rows, 16)), dim3(256), 0, stream, p);
+        IRX_HIP(hipGetLastError());
+    }
+}
+
+}  // namespace
+
+size_t icl4_bytes(const Icl4Shape &s) {
+    return (size_t)s.pairs() * ((size_t)s.blocks() * (kBlockBytes + 128) + 64 * sizeof(float));
+}
+
+size_t icl4_attend_workspace(const Icl4Shape &s, int q_rows, int n_blocks, int compute_units) {
+    const Plan pl = plan_attend(s, q_rows, n_blocks, compute_units);
+    return pl.splits > 1 ? (size_t)pl.splits * (size_t)pl.rows * 65 * sizeof(float) : 0;
+}
+
+size_t icl4_select_workspace(const Icl4Shape &s, int q_rows) {
+    return (size_t)select_rows(s, (long long)s.pairs() * q_rows) * s.blocks() * sizeof(int);
+}
+
+bool icl4_grid_fits(const Icl4Shape &s, int q_rows, int n_blocks, int compute_units) {
+    const Plan pl = plan_attend(s, q_rows, n_blocks, compute_units);
+    return (double)pl.splits * pl.qtiles * s.pairs() < 8388608.0;
+}
+
+void icl4_encode(const Icl4Rows &a, void *cache, unsigned *nonfinite, hipStream_t stream) {
+    const Icl4Shape &s = a.shape;
+    const Parts c = parts(cache, s);
+    StoreArgs p{};
+    p.k = a.k, p.v = a.v, p.k_est = a.k_strides[0], p.k_head = a.k_strides[1], p.k_row = a.k_strides[2];
+    p.v_est = a.v_strides[0], p.v_head = a.v_strides[1], p.v_row = a.v_strides[2];
+    p.lengths = a.lengths, p.heads = s.heads, p.pairs = s.pairs(), p.rows = s.rows, p.blocks = s.blocks();
+    p.tiles = c.tiles, p.bounds = c.bounds, p.scales = c.scales, p.nonfinite = nonfinite;
+    const long long blocks = (long long)s.pairs() * s.blocks();
+    KernelTimer timer(kFamGlue, stream, 0.0, 2.0 * s.pairs() * s.rows * 64 * (a.half ? 2 : 4) + (double)icl4_bytes(s));
+    hipLaunchKernelGGL(icl4_units_kernel, dim3(ceil_div((size_t)s.pairs() * 64, 256)), dim3(256), 0, stream, c.scales,
+                       s.pairs() * 64);
+    IRX_HIP(hipGetLastError());
+    if (a.half)
+        hipLaunchKernelGGL(icl4_encode_kernel<_Float16>, dim3((unsigned)blocks), dim3(256), 0, stream, p);
+    else
+        hipLaunchKernelGGL(icl4_encode_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, stream, p);
+    IRX_HIP(hipGetLastError());
+    hipLaunchKernelGGL(icl4_bounds_kernel, dim3(ceil_div((size_t)blocks, 4)), dim3(256), 0, stream, p);
+    IRX_HIP(hipGetLastError());
+}
+
+void icl4_decode(const Icl4Rows &a, const void *cache, float *bounds, hipStream_t stream) {
+    const Icl4Shape &s = a.shape;
+    const Parts c = parts(cache, s);
+    ReadArgs p{};
+    p.k = a.k, p.v = a.v, p.k_est = a.k_strides[0], p.k_head = a.k_strides[1], p.k_row = a.k_strides[2];
+    p.v_est = a.v_strides[0], p.v_head = a.v_strides[1], p.v_row = a.v_strides[2];
+    p.lengths = a.lengths, p.heads = s.heads, p.pairs = s.pairs(), p.rows = s.rows, p.blocks = s.blocks();
+    p.tiles = c.tiles, p.bounds = c.bounds, p.scales = c.scales, p.bounds_out = bounds;
+    const long long blocks = (long long)s.pairs() * s.blocks();
+    KernelTimer timer(kFamGlue, stream, 0.0, 2.0 * s.pairs() * s.rows * 64 * (a.half ? 2 : 4) + (double)icl4_bytes(s));
+    if (a.half)
+        hipLaunchKernelGGL(icl4_decode_kernel<_Float16>, dim3((unsigned)blocks), dim3(256), 0, stream, p);
+    else
+        hipLaunchKernelGGL(icl4_decode_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, stream, p);
+    IRX_HIP(hipGetLastError());
+}
+
+void icl4_select(const Icl4Queries &a, int n, int *out, void *workspace, hipStream_t stream) {
+    const Icl4Shape &s = a.shape;
+    const Parts c = parts(a.cache, s);
+    SelectArgs p{};
+    p.q = a.q, p.q_est = a.q_strides[0], p.q_head = a.q_strides[1], p.q_row = a.q_strides[2];
+    p.lengths = a.lengths, p.keep = a.keep, p.heads = s.heads, p.pairs = s.pairs(), p.q_rows = a.q_rows;
+    p.rows = s.rows, p.blocks = s.blocks(), p.bounds = c.bounds, p.scales = c.scales, p.n = n, p.out = out;
+    p.scores = static_cast<int *>(workspace);
+    const long long rows = (long long)s.pairs() * a.q_rows, step = select_rows(s, rows);
+    for (p.first = 0; p.first < rows; p.first += step) {
+        const dim3 grid((unsigned)std::min(step, rows - p.first));
+        KernelTimer timer(kFamIcl, stream, 256.0 * grid.x * p.blocks, 128.0 * s.pairs() * p.blocks);
+        if (a.half)
+            hipLaunchKernelGGL(icl4_select_kernel<_Float16>, grid, dim3(256), 0, stream, p);
+        else
+            hipLaunchKernelGGL(icl4_select_kernel<float>, grid, dim3(256), 0, stream, p);
+        IRX_HIP(hipGetLastError());
+    }
+}
+
+void icl4_attend(const Icl4Queries &a, const Icl4Attend &b, hipStream_t stream) {
+    if (a.half)
+        attend<_Float16>(a, b, stream);
+    else
+        attend<float>(a, b, stream);
+}
+
+}  // namespace irx

@@ -1559,6 +1559,119 @@ int guarded(const char *where, auto &&fn) {
     }
 }
 
+// ---- the 4-bit ICL cache: argument checks ----
+
+constexpr size_t kIcl4MaxQueries = size_t(1) << 24, kIcl4MaxBlocks = 4096;
+
+// The calling thread's current device while a call is on `d`'s.
+class CurrentDevice {
+  public:
+    explicit CurrentDevice(const irx_device *d) {
+        IRX_HIP(hipGetDevice(&before_));
+        if (before_ != d->ordinal) IRX_HIP(hipSetDevice(d->ordinal));
+        moved_ = before_ != d->ordinal;
+    }
+    ~CurrentDevice() {
+        if (moved_) (void)hipSetDevice(before_);
+    }
+    CurrentDevice(const CurrentDevice &) = delete;
+    CurrentDevice &operator=(const CurrentDevice &) = delete;
+
+  private:
+    int before_ = 0;
+    bool moved_ = false;
+};
+
+Icl4Shape icl4_shape(const irx_icl4_shape &s) { return {(int)s.estimators, (int)s.heads, (int)s.rows}; }
+
+bool icl4_shape_ok(const irx_icl4_shape *s) {
+    if (!s || !s->estimators || !s->heads || !s->rows) return false;
+    if (s->estimators > 65536 || s->heads > 65536 || s->estimators * s->heads > 65536) return false;
+    if (s->rows > (size_t)1 << 27) return false;
+    return icl4_bytes(icl4_shape(*s)) <= (size_t)1 << 40;
+}
+
+void icl4_aligned(const void *p, size_t bytes, const char *what) {
+    if (reinterpret_cast<uintptr_t>(p) % bytes)
+        fail(IRX_INVALID_ARGUMENT, std::string(what) + " must be aligned to " + std::to_string(bytes) + " bytes");
+}
+
+// Strides of [estimators, heads, rows, 64], checked: whole 16 bytes, offsets within 2^60 elements.
+void icl4_strides(const irx_icl4_shape &s, size_t rows, bool half, const irx_strides &in, long long *out) {
+    const size_t unit = half ? 8 : 4, most = (size_t)1 << 40;
+    const size_t stride[3] = {in.estimator, in.head, in.row}, count[3] = {s.estimators, s.heads, rows};
+    for (int i = 0; i < 3; ++i) {
+        // A stride along which there is one element is not used.
+        if (count[i] > 1 && (stride[i] % unit || stride[i] > most / count[i]))
+            fail(IRX_INVALID_ARGUMENT, "strides must be multiples of 16 bytes and within range");
+        out[i] = count[i] > 1 ? (long long)stride[i] : 0;
+    }
+}
+
+// An output's strides: no two rows may share a number.
+void icl4_output(const irx_icl4_shape &s, size_t rows, const irx_strides &in) {
+    size_t stride[3] = {in.estimator, in.head, in.row}, count[3] = {s.estimators, s.heads, rows};
+    // From the smallest stride up, each steps over all that the smaller ones reach.
+    size_t reach = 64;
+    bool done[3] = {count[0] < 2, count[1] < 2, count[2] < 2};
+    for (int step = 0; step < 3; ++step) {
+        int least = -1;
+        for (int i = 0; i < 3; ++i)
+            if (!done[i] && (least < 0 || stride[i] < stride[least])) least = i;
+        if (least < 0) break;
+        if (stride[least] < reach) fail(IRX_INVALID_ARGUMENT, "an output's rows must not overlap");
+        reach += stride[least] * (count[least] - 1);
+        done[least] = true;
+    }
+}
+
+bool icl4_half(int element) {
+    if (element != IRX_ELEMENT_F32 && element != IRX_ELEMENT_F16)
+        fail(IRX_INVALID_ARGUMENT, "elements are FP32 or FP16");
+    return element == IRX_ELEMENT_F16;
+}
+
+Icl4Rows icl4_rows(const irx_icl4_rows &r) {
+    if (!icl4_shape_ok(&r.shape)) fail(IRX_INVALID_ARGUMENT, "the 4-bit cache's shape is out of range");
+    Icl4Rows a{};
+    a.shape = icl4_shape(r.shape), a.half = icl4_half(r.element), a.k = r.k, a.v = r.v, a.lengths = r.lengths;
+    if (r.k) icl4_strides(r.shape, r.shape.rows, a.half, r.k_strides, a.k_strides);
+    if (r.v) icl4_strides(r.shape, r.shape.rows, a.half, r.v_strides, a.v_strides);
+    icl4_aligned(r.k, 16, "keys");
+    icl4_aligned(r.v, 16, "values");
+    icl4_aligned(r.lengths, 4, "lengths");
+    return a;
+}
+
+Icl4Queries icl4_queries(const irx_icl4_queries &q, const void *cache) {
+    if (!icl4_shape_ok(&q.shape)) fail(IRX_INVALID_ARGUMENT, "the 4-bit cache's shape is out of range");
+    if (!q.q || !q.query_rows || q.query_rows > kIcl4MaxQueries)
+        fail(IRX_INVALID_ARGUMENT, "1 to 2^24 queries are answered");
+    if (q.query_rows > (size_t)0x7fffffff / (q.shape.estimators * q.shape.heads))
+        fail(IRX_INVALID_ARGUMENT, "too many queries for one call");
+    Icl4Queries a{};
+    a.shape = icl4_shape(q.shape), a.half = icl4_half(q.element), a.cache = cache, a.q = q.q;
+    icl4_strides(q.shape, q.query_rows, a.half, q.q_strides, a.q_strides);
+    a.q_rows = (int)q.query_rows, a.lengths = q.lengths;
+    a.keep = reinterpret_cast<const unsigned long long *>(q.keep);
+    icl4_aligned(q.q, 16, "queries");
+    icl4_aligned(cache, 16, "the cache");
+    icl4_aligned(q.lengths, 4, "lengths");
+    icl4_aligned(q.keep, 8, "keep");
+    return a;
+}
+
+// After the checks that need none, so that they hold without a GPU too.
+void icl4_device(const irx_device *device) {
+    if (!device) fail(IRX_INVALID_ARGUMENT, "the call needs a device");
+}
+
+void icl4_workspace(const void *workspace, size_t bytes, size_t needed) {
+    icl4_aligned(workspace, 16, "the workspace");
+    if (needed && (!workspace || bytes < needed))
+        fail(IRX_INVALID_ARGUMENT, "the workspace must hold " + std::to_string(needed) + " bytes");
+}
+
 void device_release(irx_device *d) {
     if (d && d->refs.fetch_sub(1) == 1) delete d;
 }
@@ -2153,6 +2266,93 @@ int irx_icl_attention_noalloc(irx_device *device, const float *q, const float *k
         a.pairs = (int)pairs, a.q_rows = (int)query_rows, a.kv_rows = (int)rows;
         a.partial = pf ? device->scratch : nullptr, a.partial_floats = pf, a.compute_units = device->compute_units;
         icl_attention(a, static_cast<hipStream_t>(stream));
+    });
+}
+
+// ---- the 4-bit ICL cache ----
+
+size_t irx_icl4_bytes(const irx_icl4_shape *shape) {
+    return icl4_shape_ok(shape) ? icl4_bytes(icl4_shape(*shape)) : 0;
+}
+
+size_t irx_icl4_workspace_bytes(irx_device *device, const irx_icl4_shape *shape, size_t query_rows, size_t n_blocks) {
+    if (!device || !icl4_shape_ok(shape) || !query_rows || query_rows > kIcl4MaxQueries || n_blocks > kIcl4MaxBlocks)
+        return 0;
+    const Icl4Shape s = icl4_shape(*shape);
+    const size_t attend = icl4_attend_workspace(s, (int)query_rows, (int)n_blocks, device->compute_units);
+    return n_blocks ? std::max(attend, icl4_select_workspace(s, (int)query_rows)) : attend;
+}
+
+int irx_icl4_encode(irx_device *device, const irx_icl4_rows *rows, void *cache, uint32_t *nonfinite, void *stream) {
+    return guarded("irx_icl4_encode", [&] {
+        if (!rows || !rows->k || !rows->v || !cache)
+            fail(IRX_INVALID_ARGUMENT, "the 4-bit cache is written from keys and values");
+        const Icl4Rows a = icl4_rows(*rows);
+        icl4_aligned(cache, 16, "the cache");
+        icl4_aligned(nonfinite, 4, "the counter");
+        icl4_device(device);
+        CurrentDevice here(device);
+        icl4_encode(a, cache, nonfinite, static_cast<hipStream_t>(stream));
+    });
+}
+
+int irx_icl4_decode(irx_device *device, const void *cache, const irx_icl4_rows *rows, float *bounds, void *stream) {
+    return guarded("irx_icl4_decode", [&] {
+        if (!rows || !cache || (!rows->k && !rows->v && !bounds))
+            fail(IRX_INVALID_ARGUMENT, "nothing to read the 4-bit cache into");
+        const Icl4Rows a = icl4_rows(*rows);
+        if (rows->k) icl4_output(rows->shape, rows->shape.rows, rows->k_strides);
+        if (rows->v) icl4_output(rows->shape, rows->shape.rows, rows->v_strides);
+        icl4_aligned(cache, 16, "the cache");
+        icl4_aligned(bounds, 4, "bounds");
+        icl4_device(device);
+        CurrentDevice here(device);
+        icl4_decode(a, cache, bounds, static_cast<hipStream_t>(stream));
+    });
+}
+
+int irx_icl4_select(irx_device *device, const irx_icl4_queries *queries, const void *cache, size_t n_blocks,
+                    int32_t *blocks, void *workspace, size_t workspace_bytes, void *stream) {
+    return guarded("irx_icl4_select", [&] {
+        if (!queries || !cache || !blocks)
+            fail(IRX_INVALID_ARGUMENT, "a choice of blocks needs queries, a cache and its output");
+        if (!n_blocks || n_blocks > kIcl4MaxBlocks)
+            fail(IRX_INVALID_ARGUMENT, "1 to " + std::to_string(kIcl4MaxBlocks) + " blocks are chosen");
+        Icl4Queries a = icl4_queries(*queries, cache);
+        icl4_aligned(blocks, 4, "blocks");
+        icl4_device(device);
+        a.compute_units = device->compute_units;
+        icl4_workspace(workspace, workspace_bytes, icl4_select_workspace(a.shape, a.q_rows));
+        CurrentDevice here(device);
+        icl4_select(a, (int)n_blocks, blocks, workspace, static_cast<hipStream_t>(stream));
+    });
+}
+
+int irx_icl4_attention(irx_device *device, const irx_icl4_queries *queries, const void *cache, float scale,
+                       const int32_t *blocks, size_t n_blocks, void *out, const irx_strides *out_strides, float *lse,
+                       void *workspace, size_t workspace_bytes, void *stream) {
+    return guarded("irx_icl4_attention", [&] {
+        if (!queries || !cache || !out || !out_strides)
+            fail(IRX_INVALID_ARGUMENT, "attention needs queries, a cache and its output");
+        if (!(scale > 0.f) || !std::isfinite(scale)) fail(IRX_INVALID_ARGUMENT, "the scale must be positive and finite");
+        if (!blocks != !n_blocks || n_blocks > kIcl4MaxBlocks)
+            fail(IRX_INVALID_ARGUMENT, "blocks and n_blocks name 1 to " + std::to_string(kIcl4MaxBlocks) +
+                                           " blocks per query, or are NULL and 0");
+        Icl4Queries a = icl4_queries(*queries, cache);
+        Icl4Attend b{};
+        b.scale = scale, b.list = blocks, b.n = (int)n_blocks, b.out = out, b.lse = lse, b.workspace = workspace;
+        icl4_strides(queries->shape, queries->query_rows, a.half, *out_strides, b.o_strides);
+        icl4_output(queries->shape, queries->query_rows, *out_strides);
+        icl4_aligned(out, 16, "the output");
+        icl4_aligned(blocks, 4, "blocks");
+        icl4_aligned(lse, 4, "lse");
+        icl4_device(device);
+        a.compute_units = device->compute_units;
+        if (!icl4_grid_fits(a.shape, a.q_rows, b.n, a.compute_units))
+            fail(IRX_INVALID_ARGUMENT, "too many queries for one call");
+        icl4_workspace(workspace, workspace_bytes, icl4_attend_workspace(a.shape, a.q_rows, b.n, a.compute_units));
+        CurrentDevice here(device);
+        icl4_attend(a, b, static_cast<hipStream_t>(stream));
     });
 }
 

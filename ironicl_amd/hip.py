@@ -59,6 +59,27 @@ class KernelStats(ctypes.Structure):
                 ("bytes", ctypes.c_double), ("busy_milliseconds", ctypes.c_double)]
 
 
+ELEMENT_F32, ELEMENT_F16 = 0, 1
+
+
+class Icl4Shape(ctypes.Structure):
+    _fields_ = [("estimators", _sz), ("heads", _sz), ("rows", _sz)]
+
+
+class Strides(ctypes.Structure):
+    _fields_ = [("estimator", _sz), ("head", _sz), ("row", _sz)]
+
+
+class Icl4Rows(ctypes.Structure):
+    _fields_ = [("shape", Icl4Shape), ("element", ctypes.c_int), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("k_strides", Strides), ("v_strides", Strides), ("lengths", ctypes.c_void_p)]
+
+
+class Icl4Queries(ctypes.Structure):
+    _fields_ = [("shape", Icl4Shape), ("query_rows", _sz), ("element", ctypes.c_int), ("q", ctypes.c_void_p),
+                ("q_strides", Strides), ("lengths", ctypes.c_void_p), ("keep", ctypes.c_void_p)]
+
+
 # Every entry point include/ironicl_hip.h declares, with its ctypes signature.
 SIGNATURES = {
     "irx_last_error": (ctypes.c_char_p, []),
@@ -108,6 +129,17 @@ SIGNATURES = {
     "irx_test_icl_attention": (ctypes.c_int, [ctypes.c_void_p, _CF, _CF, _CF, _sz, _sz, _sz, _F]),
     "irx_icl_attention_noalloc": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                                  _sz, _sz, _sz, ctypes.c_void_p, ctypes.c_void_p]),
+    "irx_icl4_bytes": (_sz, [ctypes.POINTER(Icl4Shape)]),
+    "irx_icl4_workspace_bytes": (_sz, [ctypes.c_void_p, ctypes.POINTER(Icl4Shape), _sz, _sz]),
+    "irx_icl4_encode": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Icl4Rows), ctypes.c_void_p, ctypes.c_void_p,
+                                       ctypes.c_void_p]),
+    "irx_icl4_decode": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.POINTER(Icl4Rows), ctypes.c_void_p,
+                                       ctypes.c_void_p]),
+    "irx_icl4_select": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Icl4Queries), ctypes.c_void_p, _sz,
+                                       ctypes.c_void_p, ctypes.c_void_p, _sz, ctypes.c_void_p]),
+    "irx_icl4_attention": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Icl4Queries), ctypes.c_void_p, ctypes.c_float,
+                                          ctypes.c_void_p, _sz, ctypes.c_void_p, ctypes.POINTER(Strides),
+                                          ctypes.c_void_p, ctypes.c_void_p, _sz, ctypes.c_void_p]),
     "irx_test_icl_attention_precision": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, _CF, _CF, _CF, _sz, _sz,
                                                         _sz, _F]),
     "irx_test_encode_icl8": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, _sz, _sz,

@@ -1,0 +1,103 @@
+"""The 4-bit ICL cache on device buffers (irx_icl4_*, include/ironicl_hip.h).
+
+Keys and values of 64-wide heads in 4 bits, attention over all of them, and
+attention over the blocks of 64 rows that a cheap score picks for each query.
+
+A buffer is an integer address, a ``hipmem.DeviceArray`` or anything with
+``data_ptr()`` (a torch tensor on the device), or None where the call allows
+it. Buffers are the caller's: they must be of the stated type and size, and
+live until the work on ``stream`` (an address, or None for the null stream)
+is done. ``shape`` is (estimators, heads, rows); strides are (estimator, head,
+row) in elements, by default those of [estimators, heads, rows, 64]. Calls
+enqueue their work and return; invalid ones raise ``hip.HipError``.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+from . import hip
+
+ELEMENTS = {"f32": hip.ELEMENT_F32, "f16": hip.ELEMENT_F16}
+BLOCK = 64  # rows of a block
+
+
+def _address(buffer):
+    if buffer is None or isinstance(buffer, int):
+        return buffer
+    if hasattr(buffer, "data_ptr"):
+        return buffer.data_ptr()
+    return buffer.ptr
+
+
+def _element(element: str) -> int:
+    if element not in ELEMENTS:
+        raise ValueError(f"element must be one of {sorted(ELEMENTS)}, not {element!r}")
+    return ELEMENTS[element]
+
+
+def _strides(strides, heads: int, rows: int) -> hip.Strides:
+    if strides is None:
+        return hip.Strides(heads * rows * 64, rows * 64, 64)
+    return hip.Strides(*strides)
+
+
+def _rows(shape, k, v, element, k_strides, v_strides, lengths) -> hip.Icl4Rows:
+    _, heads, rows = shape
+    return hip.Icl4Rows(hip.Icl4Shape(*shape), _element(element), _address(k), _address(v),
+                        _strides(k_strides, heads, rows), _strides(v_strides, heads, rows), _address(lengths))
+
+
+def _queries(shape, q, query_rows, element, q_strides, lengths, keep) -> hip.Icl4Queries:
+    return hip.Icl4Queries(hip.Icl4Shape(*shape), query_rows, _element(element), _address(q),
+                           _strides(q_strides, shape[1], query_rows), _address(lengths), _address(keep))
+
+
+def cache_bytes(shape) -> int:
+    """Bytes of a cache of `shape` (0: out of range)."""
+    return hip.lib().irx_icl4_bytes(ctypes.byref(hip.Icl4Shape(*shape)))
+
+
+def workspace_bytes(device: hip.Device, shape, query_rows: int, n_blocks: int = 0) -> int:
+    """Bytes of workspace for `select` and `attention` of `query_rows` queries."""
+    return hip.lib().irx_icl4_workspace_bytes(device.handle, ctypes.byref(hip.Icl4Shape(*shape)), query_rows, n_blocks)
+
+
+def encode(device: hip.Device, shape, k, v, cache, *, element: str = "f32", k_strides=None, v_strides=None,
+           lengths=None, nonfinite=None, stream=None) -> None:
+    """Writes `cache` (cache_bytes) from keys and values [estimators, heads, rows, 64];
+    numbers that are not finite are held as 0 and added to the uint32 `nonfinite`."""
+    rows = _rows(shape, k, v, element, k_strides, v_strides, lengths)
+    hip.check(hip.lib().irx_icl4_encode(device.handle, ctypes.byref(rows), _address(cache), _address(nonfinite),
+                                        _address(stream)))
+
+
+def decode(device: hip.Device, shape, cache, k=None, v=None, *, element: str = "f32", k_strides=None,
+           v_strides=None, lengths=None, bounds=None, stream=None) -> None:
+    """Reads what `cache` holds into k and v, and its bounds into FP32 [estimators *
+    heads, blocks, 2, 64]. Rows past an estimator's length are left as they were."""
+    rows = _rows(shape, k, v, element, k_strides, v_strides, lengths)
+    hip.check(hip.lib().irx_icl4_decode(device.handle, _address(cache), ctypes.byref(rows), _address(bounds),
+                                        _address(stream)))
+
+
+def select(device: hip.Device, shape, cache, q, query_rows: int, n_blocks: int, blocks, *, element: str = "f32",
+           q_strides=None, lengths=None, keep=None, workspace=None, workspace_bytes: int = 0, stream=None) -> None:
+    """The `n_blocks` best blocks of each query into int32 `blocks` [estimators,
+    heads, query_rows, n_blocks], ascending, -1 where there are fewer."""
+    queries = _queries(shape, q, query_rows, element, q_strides, lengths, keep)
+    hip.check(hip.lib().irx_icl4_select(device.handle, ctypes.byref(queries), _address(cache), n_blocks,
+                                        _address(blocks), _address(workspace), workspace_bytes, _address(stream)))
+
+
+def attention(device: hip.Device, shape, cache, q, query_rows: int, out, *, element: str = "f32", scale: float = 0.125,
+              q_strides=None, out_strides=None, lengths=None, keep=None, blocks=None, n_blocks: int = 0, lse=None,
+              workspace=None, workspace_bytes: int = 0, stream=None) -> None:
+    """softmax(scale q k^T) v over the attended rows (those of `blocks`, when
+    given) into `out`, and the log-sum-exp into FP32 `lse` [estimators, heads,
+    query_rows]; 0 and -inf where a query attends to nothing."""
+    queries = _queries(shape, q, query_rows, element, q_strides, lengths, keep)
+    strides = _strides(out_strides, shape[1], query_rows)
+    hip.check(hip.lib().irx_icl4_attention(device.handle, ctypes.byref(queries), _address(cache), scale,
+                                           _address(blocks), n_blocks, _address(out), ctypes.byref(strides),
+                                           _address(lse), _address(workspace), workspace_bytes, _address(stream)))

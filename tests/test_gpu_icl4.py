@@ -1,0 +1,513 @@
+"""The 4-bit ICL cache on the GPU against its definition in float64
+(icl4_np.py): what it holds bit for bit, the choice of blocks exactly, the
+attention within bounds worked out beforehand.
+
+Bounds. A score is a sum of 64 products: FP32 queries as pairs of FP16 values
+are off by at most 2^-22 relative each, a 64-term FP32 sum by 2^-18 of the sum
+of magnitudes A, and FP32's scaling by less: |ds| <= 2^-17 A. A weight exp(s) is
+then off by 2 ds relative, and so is a weighted mean of values up to V by at
+most 4 ds V (numerator and denominator). FP32 weights are pairs (2^-22); FP16
+ones are off by half a step, 2^-11, and below FP16's smallest step by at most
+2^-33 of the largest, N of them. FP32 sums of N / 8 addends (two keys' worth of
+products in one) add N 2^-27 V at most. FP16 outputs round by 2^-11 of
+themselves. The log-sum-exp is off by 2 ds, N 2^-27 and 2^-22 of itself."""
+
+import ctypes
+
+import numpy as np
+import pytest
+
+import icl4_np
+from ironicl_amd import hip, hipmem, icl4
+
+pytestmark = pytest.mark.gpu
+DTYPES = {"f32": np.float32, "f16": np.float16}
+
+
+@pytest.fixture(scope="module")
+def device():
+    return hip.Device(0)
+
+
+def put(a):
+    return None if a is None else hipmem.DeviceArray.from_host(np.ascontiguousarray(a))
+
+
+class Tensor:
+    """[E, H, N, 64] on the device, head-major or as token rows [E, N, H * 64 + gap]."""
+
+    def __init__(self, shape, element, layout="heads", host=None):
+        e, h, n, _ = shape
+        self.shape, self.layout, self.element = shape, layout, element
+        self.width = h * 64 + 16  # token rows with a gap
+        if layout == "heads":
+            self.strides, full = (h * n * 64, n * 64, 64), (e, h, n, 64)
+        else:
+            self.strides, full = (n * self.width, 64, self.width), (e, n, self.width)
+        self.host = np.full(full, 77, DTYPES[element])
+        if host is not None:
+            self.view(self.host)[:] = host
+        self.array = put(self.host)
+
+    def view(self, a):
+        if self.layout == "heads":
+            return a
+        e, h, n, _ = self.shape
+        return a[:, :, : h * 64].reshape(e, n, h, 64).transpose(0, 2, 1, 3) if a is not self.host else \
+            np.lib.stride_tricks.as_strided(a, self.shape, [s * a.itemsize for s in self.strides] + [a.itemsize])
+
+    def get(self):
+        a = self.array.to_host()
+        if self.layout != "heads":
+            assert np.all(a[:, :, self.shape[1] * 64:] == 77), "written past the heads"
+        return np.ascontiguousarray(self.view(a))
+
+
+def draw(shape, element, seed, scale=1.0):
+    return (np.random.default_rng(seed).standard_normal(shape) * scale).astype(DTYPES[element])
+
+
+def make(device, e, h, n, element="f32", layout="heads", lengths=None, seed=0, k=None, v=None):
+    """A cache on the device and its definition, from random (or the given) keys and values."""
+    k = draw((e, h, n, 64), element, seed, 1.3) if k is None else k
+    v = draw((e, h, n, 64), element, seed + 1) if v is None else v
+    want = icl4_np.Cache(k, v, lengths)
+    dk, dv = (Tensor(x.shape, element, layout, x) for x in (k, v))
+    cache = hipmem.DeviceArray((icl4.cache_bytes((e, h, n)),), np.uint8)
+    bad = put(np.array([5], np.uint32))
+    icl4.encode(device, (e, h, n), dk.array, dv.array, cache, element=element, k_strides=dk.strides,
+                v_strides=dv.strides, lengths=put_lengths(lengths), nonfinite=bad)
+    hipmem.synchronize()
+    assert int(bad.to_host()[0]) == 5 + want.nonfinite
+    return cache, want
+
+
+KEPT = []  # small device arrays of calls whose work may still run
+
+
+def put_lengths(lengths):
+    if lengths is None:
+        return None
+    KEPT.append(put(np.asarray(lengths, np.uint32)))
+    return KEPT[-1]
+
+
+def workspace(device, shape, q_rows, n_blocks=0):
+    size = icl4.workspace_bytes(device, shape, q_rows, n_blocks)
+    return {"workspace": hipmem.DeviceArray((max(size, 16),), np.uint8), "workspace_bytes": size}
+
+
+def attend(device, cache, shape, q, element="f32", layout="heads", keep=None, lengths=None, blocks=None, scale=0.125):
+    rows = q.shape[2]
+    dq, out = Tensor(q.shape, element, layout, q), Tensor(q.shape, element, layout)
+    lse = put(np.full(q.shape[:3], 77, np.float32))
+    n = 0 if blocks is None else blocks.shape[-1]
+    words = None if keep is None else put(icl4_np.bits(keep))
+    space, listed, rows_of = workspace(device, shape, rows, n), put(blocks), put_lengths(lengths)
+    icl4.attention(device, shape, cache, dq.array, rows, out.array, element=element, scale=scale, q_strides=dq.strides,
+                   out_strides=out.strides, lengths=rows_of, keep=words, blocks=listed, n_blocks=n, lse=lse, **space)
+    hipmem.synchronize()
+    return out.get(), lse.to_host()
+
+
+def select(device, cache, shape, q, n, element="f32", layout="heads", keep=None, lengths=None):
+    dq = Tensor(q.shape, element, layout, q)
+    out = put(np.full(q.shape[:3] + (n,), 77, np.int32))
+    words, rows_of = None if keep is None else put(icl4_np.bits(keep)), put_lengths(lengths)
+    space = workspace(device, shape, q.shape[2], n)
+    icl4.select(device, shape, cache, dq.array, q.shape[2], n, out, element=element, q_strides=dq.strides,
+                lengths=rows_of, keep=words, **space)
+    hipmem.synchronize()
+    return out.to_host()
+
+
+def check(got, want, element, cache):
+    (out, lse), (out64, lse64, magnitude) = got, want
+    ds = 2.0 ** -17 * magnitude
+    n, v = cache.k.shape[2], np.abs(cache.v).max()
+    weight = 2.0 ** -21 if element == "f32" else 2.0 ** -10
+    bound = v * (4 * ds + weight + n * 2.0 ** -27 + n * 2.0 ** -32)
+    if element == "f16":
+        bound = bound + np.abs(out64) * 2.0 ** -11 + 2.0 ** -25
+    assert np.isfinite(out).all()
+    off = np.abs(out.astype(np.float64) - out64) - bound
+    assert off.max() <= 0, f"{off.max():.3e} past the bound"
+    empty = np.isneginf(lse64)
+    assert np.array_equal(np.isneginf(lse), empty)
+    assert np.all(out[empty] == 0)
+    off = np.abs(lse[~empty] - lse64[~empty]) - (2 * ds + n * 2.0 ** -26 + 2.0 ** -21 * np.abs(lse64[~empty]) + 1e-6)
+    assert empty.all() or off.max() <= 0, f"lse {off.max():.3e} past the bound"
+
+
+# ---- what the cache holds ----
+
+@pytest.mark.parametrize("e,h,n,element,layout,lengths", [
+    (1, 1, 1, "f32", "heads", None),
+    (1, 8, 63, "f32", "heads", None),
+    (1, 8, 64, "f16", "tokens", None),
+    (2, 3, 65, "f32", "tokens", (65, 2)),
+    (3, 8, 200, "f16", "heads", (0, 200, 129)),
+    (2, 5, 130, "f32", "heads", (1000, 64)),
+])
+def test_cache_holds_what_it_says(device, e, h, n, element, layout, lengths):
+    print(f"encode {e} x {h} x {n} {element} {layout} {lengths}", flush=True)
+    cache, want = make(device, e, h, n, element, layout, lengths)
+    np.testing.assert_array_equal(cache.to_host(), want.bytes())
+    outs = [Tensor((e, h, n, 64), element, layout) for _ in range(2)]
+    bounds = put(np.full((e * h, -(-n // 64), 2, 64), 77, np.float32))
+    icl4.decode(device, (e, h, n), cache, outs[0].array, outs[1].array, element=element, k_strides=outs[0].strides,
+                v_strides=outs[1].strides, lengths=put_lengths(lengths), bounds=bounds)
+    hipmem.synchronize()
+    rows = icl4_np.inside((e, h, n), lengths)[:, None, :, None]
+    for out, held in zip(outs, (want.k, want.v)):
+        np.testing.assert_array_equal(out.get(), np.where(rows, held[:, :, :n], 77))  # rows past the length stay
+    np.testing.assert_array_equal(bounds.to_host(),
+                                  (want.bounds * want.units[:, :, None, None]).reshape(e * h, -1, 2, 64))
+
+
+@pytest.mark.parametrize("element", ["f32", "f16"])
+def test_cache_of_odd_numbers(device, element):
+    """Ties, both zeros, subnormals, the largest numbers, infinities and NaN, and rows of zeros."""
+    levels = np.array([0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, -0.25, -0.75, -5.0, -0.0, 0.2501, 4.999, 5.001])
+    rng = np.random.default_rng(3)
+    k, v = (levels[rng.integers(0, 16, (1, 2, 150, 64))] * 2.0 ** rng.integers(-18, 13, (1, 2, 150, 1))
+            for _ in range(2))
+    k[0, 0, 3] = 0.0
+    k[0, 0, 4, :5] = (np.inf, -np.inf, np.nan, 3.0, 65504.0)
+    k[0, 1, 7, 40] = 1e-7
+    v[0, 0, 64:96, 7] = 0.0
+    v[0, 1, 100, :4] = (np.nan, np.inf, -65504.0, 65504.0)
+    k, v = k.astype(DTYPES[element]), v.astype(DTYPES[element])
+    if element == "f32":
+        k[0, 1, 9, :3] = (3e38, -1e30, 1e-40)
+        v[0, 0, 20, 9] = -3.4e38
+    cache, want = make(device, 1, 2, 150, element, k=k, v=v)
+    assert want.nonfinite == 5
+    got = cache.to_host()
+    # A negative number that rounds to zero may be held as either zero: compared by value below.
+    outs = [Tensor((1, 2, 150, 64), "f32") for _ in range(2)]
+    icl4.decode(device, (1, 2, 150), cache, outs[0].array, outs[1].array)
+    hipmem.synchronize()
+    for out, held in zip(outs, (want.k, want.v)):
+        np.testing.assert_array_equal(out.get(), held[:, :, :150])
+    np.testing.assert_array_equal(got[2 * 3 * 4352:], want.bytes()[2 * 3 * 4352:])
+
+
+def test_one_side_is_read_alone(device):
+    cache, want = make(device, 1, 2, 70)
+    out = Tensor((1, 2, 70, 64), "f16", "tokens")
+    icl4.decode(device, (1, 2, 70), cache, v=out.array, element="f16", v_strides=out.strides)
+    hipmem.synchronize()
+    np.testing.assert_array_equal(out.get(), want.v[:, :, :70])
+
+
+# ---- attention ----
+
+@pytest.mark.parametrize("element,layout", [("f32", "heads"), ("f16", "tokens"), ("f32", "tokens"), ("f16", "heads")])
+@pytest.mark.parametrize("e,h,n,rows", [(1, 8, 1, 1), (1, 8, 63, 3), (2, 4, 64, 16), (1, 8, 65, 17), (1, 3, 1000, 1),
+                                        (2, 8, 777, 33), (1, 8, 2049, 65), (1, 2, 640, 130), (1, 1, 5000, 300),
+                                        (1, 2, 20011, 5)])
+def test_attention(device, e, h, n, rows, element, layout):
+    print(f"attention {e} x {h} x {n}, {rows} queries, {element} {layout}", flush=True)
+    cache, want = make(device, e, h, n, element, layout, seed=n)
+    q = draw((e, h, rows, 64), element, n + 7, 1.5)
+    check(attend(device, cache, (e, h, n), q, element, layout), want.attend(q), element, want)
+
+
+@pytest.mark.parametrize("element", ["f32", "f16"])
+@pytest.mark.parametrize("rows", [1, 20, 150, 600])
+def test_attention_of_ragged_and_masked_estimators(device, element, rows):
+    """Lengths 0, 1, odd, past the rows; masks that leave blocks, single rows and nothing."""
+    e, h, n = 6, 2, 700
+    lengths = (0, 1, 333, 9999, 700, 700)
+    keep = np.random.default_rng(rows).random((e, n)) < 0.5
+    keep[3, 128:512] = False
+    keep[4] = False
+    keep[5] = False
+    keep[5, 130] = True
+    cache, want = make(device, e, h, n, element, lengths=lengths, seed=5)
+    q = draw((e, h, rows, 64), element, 11, 1.5)
+    got = attend(device, cache, (e, h, n), q, element, keep=keep, lengths=lengths)
+    check(got, want.attend(q, keep=keep), element, want)
+    assert np.all(got[0][0] == 0) and np.all(got[0][4] == 0)
+    # One attended row: its held value, whatever its score.
+    bound = np.abs(want.v[5, :, None, 130]) * (2.0 ** -20 if element == "f32" else 2.0 ** -11)
+    assert np.all(np.abs(got[0][5] - want.v[5, :, None, 130]) <= bound)
+
+
+def test_keep_bits_past_the_rows_are_not_read_as_rows(device):
+    cache, want = make(device, 1, 2, 70)
+    q = draw((1, 2, 4, 64), "f32", 1)
+    words = put(np.full((1, 2), 2 ** 64 - 1, np.uint64))
+    out = Tensor(q.shape, "f32")
+    dq, space = put(q), workspace(device, (1, 2, 70), 4)
+    icl4.attention(device, (1, 2, 70), cache, dq, 4, out.array, keep=words, **space)
+    hipmem.synchronize()
+    np.testing.assert_allclose(out.get(), want.attend(q)[0], atol=1e-4)
+
+
+@pytest.mark.parametrize("rows", [2, 70])
+@pytest.mark.parametrize("element", ["f32", "f16"])
+def test_attention_of_peaked_and_extreme_scores(device, element, rows):
+    """A later key far above the first ones, keys and values of the largest and smallest held sizes, large and zero
+    queries, and a scale that is not 1 / 8."""
+    n = 900
+    k, v = draw((1, 2, n, 64), element, 1), draw((1, 2, n, 64), element, 2)
+    k[0, 0, 500:] *= 8
+    k[0, 1, 700] *= 40
+    v[0, :, 100:140] *= 2.0 ** 14
+    v[0, :, 140:180] *= 2.0 ** -12
+    cache, want = make(device, 1, 2, n, element, k=k, v=v)
+    q = draw((1, 2, rows, 64), element, 3)
+    q[0, 0, 0] = 0.0
+    q[0, 1, 1] *= 30
+    if element == "f32":
+        q[0, 0, 1] *= 1e-30
+    check(attend(device, cache, (1, 2, n), q, element, scale=0.3), want.attend(q, scale=0.3), element, want)
+
+
+def test_large_fp32_queries(device):
+    """Queries past FP16's range, with a scale that brings their scores back."""
+    cache, want = make(device, 1, 8, 300)
+    q = draw((1, 8, 40, 64), "f32", 4) * np.float32(1e6)
+    for rows in (3, 40):
+        got = attend(device, cache, (1, 8, 300), q[:, :, :rows], scale=1e-7)
+        check(got, want.attend(q[:, :, :rows], scale=1e-7), "f32", want)
+
+
+def test_a_query_that_is_not_finite_leaves_the_others(device):
+    cache, _ = make(device, 1, 8, 300)
+    q = draw((1, 8, 70, 64), "f32", 4)
+    whole, _ = attend(device, cache, (1, 8, 300), q)
+    q[0, 3, 5, 9] = np.nan
+    got, _ = attend(device, cache, (1, 8, 300), q)
+    others = np.ones((1, 8, 70), bool)
+    others[0, 3, 5] = False
+    np.testing.assert_array_equal(got[others], whole[others])
+    assert np.isnan(got[0, 3, 5]).all()
+
+
+# ---- the choice of blocks, and attention over it ----
+
+@pytest.mark.parametrize("element,layout", [("f32", "heads"), ("f16", "tokens")])
+@pytest.mark.parametrize("e,h,n,rows,count", [(1, 8, 1, 1, 1), (1, 8, 640, 3, 4), (2, 3, 1000, 20, 16), (1, 2, 130, 5, 9),
+                                              (1, 2, 20011, 3, 100), (1, 1, 70000, 2, 700), (2, 8, 777, 150, 1)])
+def test_select(device, e, h, n, rows, count, element, layout):
+    print(f"select {count} of {e} x {h} x {n}, {rows} queries, {element} {layout}", flush=True)
+    cache, want = make(device, e, h, n, element, layout, seed=n)
+    q = draw((e, h, rows, 64), element, n + 3, 1.5)
+    np.testing.assert_array_equal(select(device, cache, (e, h, n), q, count, element, layout), want.select(q, count))
+
+
+def test_select_of_equal_scores_takes_the_lower_blocks(device):
+    """Every block the same rows, and queries of zeros."""
+    k = np.tile(draw((1, 2, 64, 64), "f32", 1), (1, 1, 40, 1))
+    cache, want = make(device, 1, 2, 2560, k=k, v=k)
+    q = draw((1, 2, 6, 64), "f32", 2)
+    q[0, :, 3:] = 0.0
+    got = select(device, cache, (1, 2, 2560), q, 7)
+    np.testing.assert_array_equal(got, want.select(q, 7))
+    assert np.all(got == np.arange(7))
+
+
+def test_select_of_masked_and_empty_blocks(device):
+    e, h, n = 4, 2, 900
+    lengths = (0, 65, 900, 500)
+    keep = np.random.default_rng(1).random((e, n)) < 0.3
+    keep[2, 64:640] = False
+    keep[3, 1:] = False
+    cache, want = make(device, e, h, n, lengths=lengths)
+    q = draw((e, h, 5, 64), "f32", 2)
+    for count in (1, 6, 15, 40):
+        got = select(device, cache, (e, h, n), q, count, keep=keep, lengths=lengths)
+        np.testing.assert_array_equal(got, want.select(q, count, keep=keep))
+    assert np.all(got[0] == -1) and np.all(got[3, :, :, 1:] == -1)
+
+
+def test_select_of_queries_of_any_size(device):
+    cache, want = make(device, 1, 2, 900)
+    q = draw((1, 2, 8, 64), "f32", 2)
+    q *= np.float32(10.0) ** np.array([-36, -31, -20, -3, 0, 5, 20, 30], np.float32)[None, None, :, None]
+    q[0, 0, 4, 5] = 127.0 * 2.0 ** 4  # the largest of its row, exactly at the edge of a step
+    np.testing.assert_array_equal(select(device, cache, (1, 2, 900), q, 5), want.select(q, 5))
+
+
+@pytest.mark.parametrize("element,layout", [("f32", "heads"), ("f16", "tokens")])
+@pytest.mark.parametrize("e,h,n,rows,count", [(1, 8, 1, 1, 1), (1, 8, 640, 3, 4), (2, 3, 1000, 20, 16), (1, 1, 9000, 2, 100),
+                                              (1, 2, 777, 300, 3)])
+def test_attention_over_listed_blocks(device, e, h, n, rows, count, element, layout):
+    """Listed in any order, some twice, some that are no blocks."""
+    print(f"{count} listed blocks of {e} x {h} x {n}, {rows} queries, {element} {layout}", flush=True)
+    rng = np.random.default_rng(n)
+    cache, want = make(device, e, h, n, element, layout, seed=n)
+    q = draw((e, h, rows, 64), element, n + 3, 1.5)
+    tiles = -(-n // 64)
+    blocks = rng.integers(0, tiles, (e, h, rows, count)).astype(np.int32)
+    odd = rng.random(blocks.shape)
+    blocks[odd < 0.1] = -1
+    blocks[odd > 0.95] = tiles
+    blocks[odd > 0.97] = 2 ** 31 - 1
+    blocks[odd > 0.98] = -2 ** 31
+    keep = rng.random((e, n)) < 0.7
+    got = attend(device, cache, (e, h, n), q, element, layout, keep=keep, blocks=blocks)
+    check(got, want.attend(q, keep=keep, blocks=blocks), element, want)
+
+
+def test_every_block_listed_is_attention_over_all(device):
+    e, h, n, rows = 1, 8, 1500, 9
+    cache, want = make(device, e, h, n)
+    q = draw((e, h, rows, 64), "f32", 2)
+    blocks = np.broadcast_to(np.arange(24, dtype=np.int32), (e, h, rows, 24))
+    check(attend(device, cache, (e, h, n), q, blocks=blocks), want.attend(q), "f32", want)
+
+
+# ---- the calls together ----
+
+class Runtime:
+    """Streams and graphs of the HIP runtime that the library uses."""
+
+    def __init__(self):
+        self.rt = hipmem.runtime()
+        self.stream = ctypes.c_void_p()
+        self.ok(self.rt.hipStreamCreateWithFlags(ctypes.byref(self.stream), ctypes.c_uint(1)))
+
+    def ok(self, code):
+        assert code == 0, f"HIP error {code}"
+
+    def wait(self):
+        self.ok(self.rt.hipStreamSynchronize(self.stream))
+
+    def capture(self, fn):
+        graph, self.exec = ctypes.c_void_p(), ctypes.c_void_p()
+        self.ok(self.rt.hipStreamBeginCapture(self.stream, ctypes.c_int(1)))
+        fn()
+        self.ok(self.rt.hipStreamEndCapture(self.stream, ctypes.byref(graph)))
+        self.ok(self.rt.hipGraphInstantiate(ctypes.byref(self.exec), graph, None, None, ctypes.c_size_t(0)))
+        self.ok(self.rt.hipGraphDestroy(graph))
+
+    def launch(self):
+        self.ok(self.rt.hipGraphLaunch(self.exec, self.stream))
+
+
+class Run:
+    """Encode, select, attend over the chosen blocks and over all: buffers of one run."""
+
+    def __init__(self, device, e, h, n, rows, count, element, seed):
+        self.device, self.shape, self.rows, self.count, self.element = device, (e, h, n), rows, count, element
+        dtype = DTYPES[element]
+        self.k, self.v, self.q = (hipmem.DeviceArray((e, h, r, 64), dtype) for r in (n, n, rows))
+        self.cache = hipmem.DeviceArray((icl4.cache_bytes(self.shape),), np.uint8)
+        self.blocks = hipmem.DeviceArray((e, h, rows, count), np.int32)
+        self.outs = [hipmem.DeviceArray((e, h, rows, 64), dtype) for _ in range(2)]
+        self.lse = [hipmem.DeviceArray((e, h, rows), np.float32) for _ in range(2)]
+        self.space = workspace(device, self.shape, rows, count)
+        self.dense = workspace(device, self.shape, rows)
+        self.fill(seed)
+
+    def fill(self, seed):
+        e, h, n = self.shape
+        k, v, q = (draw((e, h, r, 64), self.element, seed + i, 1.2) for i, r in enumerate((n, n, self.rows)))
+        for d, a in ((self.k, k), (self.v, v), (self.q, q)):
+            assert hipmem.runtime().hipMemcpy(d.ptr, a.ctypes.data, d.nbytes, hipmem.H2D) == 0
+
+    def enqueue(self, stream):
+        kind = {"element": self.element, "stream": stream}
+        icl4.encode(self.device, self.shape, self.k, self.v, self.cache, **kind)
+        icl4.select(self.device, self.shape, self.cache, self.q, self.rows, self.count, self.blocks, **self.space, **kind)
+        icl4.attention(self.device, self.shape, self.cache, self.q, self.rows, self.outs[0], blocks=self.blocks,
+                       n_blocks=self.count, lse=self.lse[0], **self.space, **kind)
+        icl4.attention(self.device, self.shape, self.cache, self.q, self.rows, self.outs[1], lse=self.lse[1],
+                       **self.dense, **kind)
+
+    def results(self):
+        return [a.to_host() for a in (self.blocks, *self.outs, *self.lse)]
+
+
+@pytest.mark.parametrize("element", ["f32", "f16"])
+def test_a_run_is_captured_and_replayed(device, element):
+    """The whole run in a graph, replayed on new inputs with eager work between: bitwise the eager results."""
+    runtime = Runtime()
+    runs = [Run(device, 2, 4, 1300, 70, 5, element, 1), Run(device, 1, 8, 5000, 2, 9, element, 2)]
+    eager = [Run(device, 2, 4, 1300, 70, 5, element, 1), Run(device, 1, 8, 5000, 2, 9, element, 2)]
+    for run, other in zip(runs, eager):
+        runtime.capture(lambda: run.enqueue(runtime.stream.value))
+        for replay in range(4):
+            print(f"replay {replay}", flush=True)
+            run.fill(10 * replay), other.fill(10 * replay)
+            hipmem.synchronize()
+            runtime.launch()
+            runtime.wait()
+            got = run.results()
+            other.enqueue(None)
+            hipmem.synchronize()
+            for a, b in zip(got, other.results()):
+                np.testing.assert_array_equal(a, b)
+        want = icl4_np.Cache(run.k.to_host(), run.v.to_host())
+        q = run.q.to_host()
+        np.testing.assert_array_equal(got[0], want.select(q, run.count))
+        check((got[1], got[3]), want.attend(q, blocks=got[0]), element, want)
+        check((got[2], got[4]), want.attend(q), element, want)
+
+
+def test_two_streams_at_once(device):
+    """Runs on two streams with workspaces of their own: each bitwise its run alone."""
+    streams = [Runtime(), Runtime()]
+    runs = [Run(device, 1, 8, 4000, 40, 6, "f32", 1), Run(device, 1, 8, 6000, 1, 20, "f32", 2)]
+    alone = []
+    for run in runs:
+        run.enqueue(None)
+        hipmem.synchronize()
+        alone.append(run.results())
+    for _ in range(5):
+        for stream, run in zip(streams, runs):
+            run.enqueue(stream.stream.value)
+    for stream in streams:
+        stream.wait()
+    for run, want in zip(runs, alone):
+        for a, b in zip(run.results(), want):
+            np.testing.assert_array_equal(a, b)
+
+
+def test_shared_sources_and_a_cache_past_32_bits(device):
+    """One estimator's rows shared by 64 pairs (strides of 0): a 4.8 GB cache whose last pair answers as its first."""
+    e, h, n = 8, 8, 1_060_000
+    rng = np.random.default_rng(0)
+    k, v = (put(rng.standard_normal((n, 64), dtype=np.float32).astype(np.float16)) for _ in range(2))
+    cache = hipmem.DeviceArray((icl4.cache_bytes((e, h, n)),), np.uint8)
+    assert cache.nbytes > 2 ** 32
+    icl4.encode(device, (e, h, n), k, v, cache, element="f16", k_strides=(0, 0, 64), v_strides=(0, 0, 64))
+    q = put(rng.standard_normal((1, 64), dtype=np.float32).astype(np.float16))
+    out, lse = hipmem.DeviceArray((e, h, 1, 64), np.float16), hipmem.DeviceArray((e, h, 1), np.float32)
+    blocks = hipmem.DeviceArray((e, h, 1, 30), np.int32)
+    space = workspace(device, (e, h, n), 1, 30)
+    dense = workspace(device, (e, h, n), 1)
+    icl4.attention(device, (e, h, n), cache, q, 1, out, element="f16", q_strides=(0, 0, 0), lse=lse, **dense)
+    icl4.select(device, (e, h, n), cache, q, 1, 30, blocks, element="f16", q_strides=(0, 0, 0), **space)
+    hipmem.synchronize()
+    a, s, b = out.to_host().reshape(64, 64), lse.to_host().ravel(), blocks.to_host().reshape(64, 30)
+    assert np.all(a == a[0]) and np.all(s == s[0]) and np.all(b == b[0]) and np.all(np.diff(b[0]) > 0)
+    # log of the sum over n keys of exp(s), s of mean 0: log n at least, and finite.
+    assert np.log(n) - 0.1 < s[0] < np.log(n) + 40
+    icl4.attention(device, (e, h, n), cache, q, 1, out, element="f16", q_strides=(0, 0, 0), lse=lse, blocks=blocks,
+                   n_blocks=30, **space)
+    hipmem.synchronize()
+    a, s = out.to_host().reshape(64, 64), lse.to_host().ravel()
+    assert np.all(a == a[0]) and np.all(s == s[0])
+
+
+def test_small_workspaces_are_refused(device):
+    cache, _ = make(device, 1, 8, 5000)
+    q = put(draw((1, 8, 1, 64), "f32", 1))
+    out = hipmem.DeviceArray((1, 8, 1, 64))
+    need = icl4.workspace_bytes(device, (1, 8, 5000), 1)
+    assert need > 0
+    space = hipmem.DeviceArray((need,), np.uint8)
+    for kw in ({}, {"workspace": space, "workspace_bytes": need - 1}, {"workspace": None, "workspace_bytes": need}):
+        with pytest.raises(hip.HipError, match="workspace must hold") as info:
+            icl4.attention(device, (1, 8, 5000), cache, q, 1, out, **kw)
+        assert info.value.status == hip.INVALID_ARGUMENT
+    blocks = hipmem.DeviceArray((1, 8, 1, 4), np.int32)
+    with pytest.raises(hip.HipError, match="workspace must hold"):
+        icl4.select(device, (1, 8, 5000), cache, q, 1, 4, blocks)
+    with pytest.raises(hip.HipError, match="too many queries"):
+        icl4.attention(device, (8192, 8, 64), cache, q, 30000, out, out_strides=(30000 * 512, 64, 512))
