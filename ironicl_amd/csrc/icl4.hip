@@ -306,108 +306,157 @@ struct SelectArgs {
     const float *scales;
     int n;
     int *out;
-    int *scores;         // [rows of this launch, blocks]
-    long long first;     // the first (pair, query) of this launch
+    int *scores;            // [pair rows, padded]
+    long long padded;       // blocks rounded up to 64
+    int pair0, row0, rows_here;  // this launch's pairs and queries: scores row (pair - pair0) * rows_here + row - row0
+    int qtiles, chunks, chunk;   // chunk: blocks of one wave
 };
 
 constexpr int kNoScore = -(1 << 30);
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-// One workgroup per (pair, query): every block's score, the n-th largest by
-// bisection, and the blocks above it in order.
+// Scores of 16 queries against `chunk` blocks per wave: per 16 blocks and
+// sign one 16x16x64 product of whole numbers, [blocks, 64] lower bounds by the
+// negative parts of the queries' codes, upper bounds by the positive ones.
 template <typename T>
-__global__ __launch_bounds__(256) void icl4_select_kernel(SelectArgs p) {
-    __shared__ unsigned pos[16], neg[16];
-    __shared__ int count, base, equal_base;
-    __shared__ int wave_above[4], wave_equal[4];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const long long pq = p.first + blockIdx.x;
-    const int pair = (int)(pq / p.q_rows), row = (int)(pq - (long long)pair * p.q_rows);
+__global__ __launch_bounds__(256) void icl4_scores_kernel(SelectArgs p) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, i16 = lane & 15;
+    unsigned id = blockIdx.x;
+    const int part = (int)(id % (unsigned)p.chunks);
+    id /= (unsigned)p.chunks;
+    const int qt = (int)(id % (unsigned)p.qtiles), pair = p.pair0 + (int)(id / (unsigned)p.qtiles);
+    const int b0 = (part * 4 + wave) * p.chunk;
+    if (b0 >= p.blocks) return;
     const int e = pair / p.heads, head = pair - e * p.heads;
-    const int rows = rows_of(p.lengths, e, p.rows);
-    int *scores = p.scores + (long long)blockIdx.x * p.blocks;
-    int *out = p.out + pq * p.n;
-    if (wave == 0) {
-        const T *src = static_cast<const T *>(p.q) + e * p.q_est + head * p.q_head + row * p.q_row;
-        const float x = to_float(src[lane]) * p.scales[pair * 64 + lane];
-        const float m = wave_max(fabsf(x));
+    const int here = 16 * qt + i16, row = p.row0 + min(here, p.rows_here - 1);
+    i32x4 pos, neg;
+    {
+        const T *src = static_cast<const T *>(p.q) + e * p.q_est + head * p.q_head + row * p.q_row + 16 * g;
+        float x[16];
+        float m = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            x[i] = to_float(src[i]) * p.scales[pair * 64 + 16 * g + i];
+            m = fmaxf(m, fabsf(x[i]));
+        }
+        m = fmaxf(m, __shfl_xor(m, 16, 64));
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
         int f = -100;
         if (m > 0.f) {
             const unsigned bits = __float_as_uint(m);
             const int ex = (int)(bits >> 23) - 126;
             f = min(120, max(-100, (bits & 0x7fffffu) <= 0x7e0000u ? ex - 7 : ex - 6));
         }
-        const float c = rintf(fminf(fmaxf(x * pow2(-f), -127.f), 127.f));
-        reinterpret_cast<signed char *>(pos)[lane] = (signed char)fmaxf(c, 0.f);
-        reinterpret_cast<signed char *>(neg)[lane] = (signed char)fminf(c, 0.f);
-    }
-    if (tid == 0) count = 0;
-    __syncthreads();
-    int candidates = 0;
-    for (int b = tid; b < p.blocks; b += 256) {
-        int s = kNoScore;
-        if (block_mask(p.keep, e, p.blocks, b, rows)) {
-            const unsigned *w = reinterpret_cast<const unsigned *>(p.bounds + ((long long)pair * p.blocks + b) * 128);
-            s = 0;
+        const float inv = pow2(-f);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s = __builtin_amdgcn_sdot4((int)neg[i], (int)w[i], s, false);
-                s = __builtin_amdgcn_sdot4((int)pos[i], (int)w[16 + i], s, false);
+        for (int w = 0; w < 4; ++w) {
+            unsigned a = 0u, b = 0u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int c = (int)rintf(fminf(fmaxf(x[4 * w + i] * inv, -127.f), 127.f));
+                a |= (unsigned)max(c, 0) << (8 * i);
+                b |= ((unsigned)min(c, 0) & 0xffu) << (8 * i);
             }
-            ++candidates;
+            pos[w] = (int)a, neg[w] = (int)b;
         }
-        scores[b] = s;
     }
-    if (candidates) atomicAdd(&count, candidates);
-    __syncthreads();
-    const int total = count;
-    __syncthreads();
-    // The largest v that at least n scores reach (every candidate when there are no more than n).
-    int lo = -(1 << 21), hi = 1 << 21;  // count(>= lo) >= n > count(>= hi)
+    const signed char *bounds = p.bounds + (long long)pair * p.blocks * 128 + 16 * g;
+    int *out = p.scores + ((long long)(pair - p.pair0) * p.rows_here + here) * p.padded + 4 * g;
+    const int end = min(p.blocks, b0 + p.chunk);
+    for (int b = b0; b < end; b += 16) {
+        const signed char *src = bounds + (long long)min(b + i16, p.blocks - 1) * 128;
+        const i32x4 low = *reinterpret_cast<const i32x4 *>(src), high = *reinterpret_cast<const i32x4 *>(src + 64);
+        i32x4 s = {0, 0, 0, 0};
+        s = __builtin_amdgcn_mfma_i32_16x16x64_i8(low, neg, s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_i32_16x16x64_i8(high, pos, s, 0, 0, 0);
+        // Register r: block b + 4 g + r of query i16; blocks past the last lie in the row's padding.
+        if (here < p.rows_here) *reinterpret_cast<i32x4 *>(out + b) = s;
+    }
+}
+
+// The n best of one query's scores: WAVES waves hold up to REGS * 64 scores
+// each, a contiguous share, and find the n-th largest by bisection over the
+// scores' 21 bits, counting by ballots. (REGS 0: any number of blocks, scores
+// read again for every step.)
+template <int WAVES, int REGS>
+__global__ __launch_bounds__(WAVES * 64) void icl4_pick_kernel(SelectArgs p) {
+    __shared__ int counts[2][WAVES];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int at = (int)(blockIdx.x / (unsigned)p.rows_here);
+    const int pair = p.pair0 + at, row = p.row0 + (int)(blockIdx.x - (unsigned)at * p.rows_here);
+    const int e = pair / p.heads;
+    const int rows = rows_of(p.lengths, e, p.rows);
+    const int *scores = p.scores + (long long)blockIdx.x * p.padded;
+    int *out = p.out + ((long long)pair * p.q_rows + row) * p.n;
+    const int share = (int)(p.padded / 64 + WAVES - 1) / WAVES;  // 64-block steps of a wave
+    const int first = wave * share * 64;
+    auto score = [&](int i) {
+        const int b = first + 64 * i + lane;
+        return i < share && b < p.blocks && block_mask(p.keep, e, p.blocks, b, rows) ? scores[b] : kNoScore;
+    };
+    int held[REGS > 0 ? REGS : 1];
+    if constexpr (REGS > 0) {
+#pragma unroll
+        for (int i = 0; i < REGS; ++i) held[i] = score(i);
+    }
+    auto each = [&](auto &&fn) {
+        if constexpr (REGS > 0) {
+#pragma unroll
+            for (int i = 0; i < REGS; ++i)
+                if (i < share) fn(held[i], i);
+        } else {
+            for (int i = 0; i < share; ++i) fn(score(i), i);
+        }
+    };
+    int phase = 0;
+    // Scores of the query that are at least v.
+    auto reach = [&](int v) {
+        int c = 0;
+        each([&](int s, int) { c += __popcll(__ballot(s >= v)); });
+        if constexpr (WAVES == 1) return c;
+        if (lane == 0) counts[phase][wave] = c;
+        __syncthreads();
+        int total = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) total += counts[phase][w];
+        phase ^= 1;  // the next count's writes pass this one's reads
+        return total;
+    };
+    const int total = reach(kNoScore + 1);
+    int lo = -(1 << 20), hi = 1 << 20;  // reach(lo) >= n > reach(hi), where there are more than n
     if (total > p.n) {
         while (hi - lo > 1) {
-            const int mid = lo + (hi - lo) / 2;
-            if (tid == 0) count = 0;
-            __syncthreads();
-            int c = 0;
-            for (int b = tid; b < p.blocks; b += 256) c += scores[b] >= mid;
-            if (c) atomicAdd(&count, c);
-            __syncthreads();
-            if (count >= p.n)
+            const int mid = (lo + hi) >> 1;
+            if (reach(mid) >= p.n)
                 lo = mid;
             else
                 hi = mid;
-            __syncthreads();
         }
     }
-    // Blocks above lo, and the first of those at lo that there is room for.
-    if (tid == 0) count = 0;
-    __syncthreads();
-    int c = 0;
-    for (int b = tid; b < p.blocks; b += 256) c += scores[b] > lo;
-    if (c) atomicAdd(&count, c);
-    __syncthreads();
-    const int room = p.n - count;
-    if (tid == 0) base = 0, equal_base = 0;
-    __syncthreads();
-    for (int b0 = 0; b0 < p.blocks; b0 += 256) {
-        const int b = b0 + tid;
-        const int s = b < p.blocks ? scores[b] : kNoScore;
-        const bool above = s > lo, equal = s == lo;
-        const unsigned long long va = __ballot(above), ve = __ballot(equal);
-        const unsigned long long below = (1ull << lane) - 1;
-        if (lane == 0) wave_above[wave] = __popcll(va), wave_equal[wave] = __popcll(ve);
+    // Blocks above lo, and the first of those at lo that there is room for, in order.
+    int above = 0, equal = 0;
+    each([&](int s, int) { above += __popcll(__ballot(s > lo)), equal += __popcll(__ballot(s == lo)); });
+    int before_above = 0, before_equal = 0, all_above = above;
+    if constexpr (WAVES > 1) {
         __syncthreads();
-        int before_above = base, before_equal = equal_base;
-        for (int w = 0; w < wave; ++w) before_above += wave_above[w], before_equal += wave_equal[w];
-        before_above += __popcll(va & below), before_equal += __popcll(ve & below);
-        const int at = before_above + min(before_equal, room);
-        if (above || (equal && before_equal < room)) out[at] = b;
+        if (lane == 0) counts[0][wave] = above, counts[1][wave] = equal;
         __syncthreads();
-        if (tid == 0)
-            for (int w = 0; w < 4; ++w) base += wave_above[w], equal_base += wave_equal[w];
-        __syncthreads();
+        all_above = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            if (w < wave) before_above += counts[0][w], before_equal += counts[1][w];
+            all_above += counts[0][w];
+        }
     }
-    for (int i = min(total, p.n) + tid; i < p.n; i += 256) out[i] = -1;
+    const int room = p.n - all_above;
+    const unsigned long long below = (1ull << lane) - 1;
+    each([&](int s, int i) {
+        const unsigned long long va = __ballot(s > lo), ve = __ballot(s == lo);
+        const int a = before_above + __popcll(va & below), q = before_equal + __popcll(ve & below);
+        if (s > lo || (s == lo && q < room)) out[a + min(q, room)] = first + 64 * i + lane;
+        before_above += __popcll(va), before_equal += __popcll(ve);
+    });
+    for (int i = min(total, p.n) + (int)threadIdx.x; i < p.n; i += WAVES * 64) out[i] = -1;
 }
 
 // ---- attention ----
@@ -606,28 +655,70 @@ __global__ __launch_bounds__(kWaves * 64) void icl4_rows_kernel(AttendArgs p) {
     }
 }
 
-// Splits' outputs weighted by their sums: 16 lanes per (pair, query).
-template <typename T>
+// Splits' outputs weighted by their sums. 16 lanes of four dims each take a
+// (pair, query) and every GROUPS-th split; a workgroup holds 16 / GROUPS rows.
+template <typename T, int GROUPS>
 __global__ __launch_bounds__(256) void icl4_merge_kernel(AttendArgs p) {
+    __shared__ float sums[GROUPS > 1 ? 16 * 66 : 1];
     const long long all = (long long)p.pairs * p.q_rows;
-    const long long pq = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
-    if (pq >= all) return;
-    const int d = 4 * (threadIdx.x & 15);
+    const int tid = threadIdx.x, slot = tid >> 4, group = slot % GROUPS, d = 4 * (tid & 15);
+    const long long mine = (long long)blockIdx.x * (16 / GROUPS) + slot / GROUPS;
+    const long long pq = min(mine, all - 1);
     const float *lse = p.partial + p.splits * all * 64 + pq;
-    float mx = -INFINITY;
-    for (int s = 0; s < p.splits; ++s) mx = fmaxf(mx, lse[s * all]);
+    const float *part = p.partial + pq * 64 + d;
+    // Eight splits' loads at once; slots past the last read it again and weigh nothing.
+    float ref = -INFINITY, den = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    float den = 0.f;
-    const float ref = mx > -INFINITY ? mx : 0.f;
-    for (int s = 0; s < p.splits; ++s) {
-        const float a = __builtin_amdgcn_exp2f(lse[s * all] - ref);
-        acc += a * *reinterpret_cast<const f32x4 *>(p.partial + (s * all + pq) * 64 + d);
-        den += a;
+    for (int s0 = group; s0 < p.splits; s0 += 8 * GROUPS) {
+        float l[8];
+        f32x4 v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int s = s0 + i * GROUPS, at = min(s, p.splits - 1);
+            l[i] = lse[at * all];
+            v[i] = *reinterpret_cast<const f32x4 *>(part + at * all * 64);
+            if (s >= p.splits) l[i] = -INFINITY, v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        float top = ref;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, l[i]);
+        const float base = top > -INFINITY ? top : 0.f;
+        const float a = __builtin_amdgcn_exp2f(ref - base);
+        acc *= a, den *= a;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float w = __builtin_amdgcn_exp2f(l[i] - base);
+            acc += w * v[i];
+            den += w;
+        }
+        ref = top;
     }
+    if constexpr (GROUPS > 1) {
+        *reinterpret_cast<f32x2 *>(&sums[slot * 66 + d]) = f32x2{acc[0], acc[1]};
+        *reinterpret_cast<f32x2 *>(&sums[slot * 66 + d + 2]) = f32x2{acc[2], acc[3]};
+        if (d == 0) sums[slot * 66 + 64] = ref, sums[slot * 66 + 65] = den;
+        __syncthreads();
+        if (group) return;
+        float top = ref;
+#pragma unroll
+        for (int i = 1; i < GROUPS; ++i) top = fmaxf(top, sums[(slot + i) * 66 + 64]);
+        const float base = top > -INFINITY ? top : 0.f;
+        acc = f32x4{0.f, 0.f, 0.f, 0.f}, den = 0.f;
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) {
+            const float *of = sums + (slot + i) * 66;
+            const float a = __builtin_amdgcn_exp2f(of[64] - base);
+            acc += a * f32x4{of[d], of[d + 1], of[d + 2], of[d + 3]};
+            den += a * of[65];
+        }
+        ref = top;
+    }
+    if (mine >= all) return;
     if (den != 0.f) acc *= 1.0f / den;
     const int pair = (int)(pq / p.q_rows), row = (int)(pq - (long long)pair * p.q_rows);
     store_out<T>(p, pair, row, d, acc);
-    if (p.lse && d == 0) p.lse[pq] = (ref + log2f(den)) * kLn2;
+    // Nothing attended: log 0.
+    if (p.lse && d == 0) p.lse[pq] = ((ref > -INFINITY ? ref : 0.f) + log2f(den)) * kLn2;
 }
 
 struct Plan {
@@ -649,9 +740,19 @@ Plan plan_attend(const Icl4Shape &s, int q_rows, int n_blocks, int compute_units
     return pl;
 }
 
-// Scores of one launch: at most 64 MiB of them.
-long long select_rows(const Icl4Shape &s, long long rows) {
-    return std::max<long long>(1, std::min<long long>(rows, (16LL << 20) / s.blocks()));
+// Scores are made and picked from in turns of at most 64 MiB (or one query's):
+// whole pairs, or a part of one pair's queries.
+struct SelectTurns {
+    long long padded;
+    int pairs, rows;
+};
+SelectTurns select_turns(const Icl4Shape &s, int q_rows) {
+    SelectTurns t{};
+    t.padded = (s.blocks() + 63) / 64 * 64;
+    const long long most = std::max<long long>(1, (16LL << 20) / t.padded);  // queries of a turn
+    t.rows = (int)std::min<long long>(q_rows, most);
+    t.pairs = t.rows < q_rows ? 1 : (int)std::min<long long>(s.pairs(), std::max<long long>(1, most / q_rows));
+    return t;
 }
 
 struct Parts {
@@ -694,7 +795,13 @@ void attend(const Icl4Queries &a, const Icl4Attend &b, hipStream_t stream) {
     }
     if (pl.splits > 1) {
         KernelTimer timer(kFamIclMerge, stream, 0.0, 4.0 * pl.rows * (65.0 * pl.splits + 64.0));
-        hipLaunchKernelGGL(icl4_merge_kernel<T>, dim3(ceil_div((size_t)pl.rows, 16)), dim3(256), 0, stream, p);
+        // A lane's splits come eight at a time: more groups where there are more splits.
+        if (pl.splits <= 8)
+            hipLaunchKernelGGL((icl4_merge_kernel<T, 1>), dim3(ceil_div((size_t)pl.rows, 16)), dim3(256), 0, stream, p);
+        else if (pl.splits <= 32)
+            hipLaunchKernelGGL((icl4_merge_kernel<T, 4>), dim3(ceil_div((size_t)pl.rows, 4)), dim3(256), 0, stream, p);
+        else
+            hipLaunchKernelGGL((icl4_merge_kernel<T, 16>), dim3((unsigned)pl.rows), dim3(256), 0, stream, p);
         IRX_HIP(hipGetLastError());
     }
 }
@@ -711,7 +818,8 @@ size_t icl4_attend_workspace(const Icl4Shape &s, int q_rows, int n_blocks, int c
 }
 
 size_t icl4_select_workspace(const Icl4Shape &s, int q_rows) {
-    return (size_t)select_rows(s, (long long)s.pairs() * q_rows) * s.blocks() * sizeof(int);
+    const SelectTurns t = select_turns(s, q_rows);
+    return (size_t)t.pairs * t.rows * t.padded * sizeof(int);
 }
 
 bool icl4_grid_fits(const Icl4Shape &s, int q_rows, int n_blocks, int compute_units) {
@@ -766,16 +874,37 @@ void icl4_select(const Icl4Queries &a, int n, int *out, void *workspace, hipStre
     p.lengths = a.lengths, p.keep = a.keep, p.heads = s.heads, p.pairs = s.pairs(), p.q_rows = a.q_rows;
     p.rows = s.rows, p.blocks = s.blocks(), p.bounds = c.bounds, p.scales = c.scales, p.n = n, p.out = out;
     p.scores = static_cast<int *>(workspace);
-    const long long rows = (long long)s.pairs() * a.q_rows, step = select_rows(s, rows);
-    for (p.first = 0; p.first < rows; p.first += step) {
-        const dim3 grid((unsigned)std::min(step, rows - p.first));
-        KernelTimer timer(kFamIcl, stream, 256.0 * grid.x * p.blocks, 128.0 * s.pairs() * p.blocks);
-        if (a.half)
-            hipLaunchKernelGGL(icl4_select_kernel<_Float16>, grid, dim3(256), 0, stream, p);
-        else
-            hipLaunchKernelGGL(icl4_select_kernel<float>, grid, dim3(256), 0, stream, p);
-        IRX_HIP(hipGetLastError());
-    }
+    const SelectTurns t = select_turns(s, a.q_rows);
+    p.padded = t.padded;
+    for (p.pair0 = 0; p.pair0 < p.pairs; p.pair0 += t.pairs)
+        for (p.row0 = 0; p.row0 < p.q_rows; p.row0 += t.rows) {
+            const int pairs = std::min(t.pairs, p.pairs - p.pair0);
+            p.rows_here = std::min(t.rows, p.q_rows - p.row0);
+            p.qtiles = (int)ceil_div(p.rows_here, 16);
+            // A wave takes 16 to 256 blocks: fewer where that leaves compute units idle.
+            const long long tiles = (long long)pairs * p.qtiles;
+            p.chunk = 256;
+            while (p.chunk > 16 && tiles * ceil_div(p.blocks, 4 * p.chunk) < 2LL * a.compute_units) p.chunk /= 2;
+            p.chunks = (int)ceil_div(p.blocks, 4 * p.chunk);
+            const dim3 grid((unsigned)(tiles * p.chunks)), rows((unsigned)(pairs * p.rows_here));
+            KernelTimer timer(kFamIcl, stream, 256.0 * rows.x * p.blocks, 128.0 * pairs * p.blocks);
+            if (a.half)
+                hipLaunchKernelGGL(icl4_scores_kernel<_Float16>, grid, dim3(256), 0, stream, p);
+            else
+                hipLaunchKernelGGL(icl4_scores_kernel<float>, grid, dim3(256), 0, stream, p);
+            IRX_HIP(hipGetLastError());
+            if (p.blocks <= 512)
+                hipLaunchKernelGGL((icl4_pick_kernel<1, 8>), rows, dim3(64), 0, stream, p);
+            else if (p.blocks <= 1024)
+                hipLaunchKernelGGL((icl4_pick_kernel<1, 16>), rows, dim3(64), 0, stream, p);
+            else if (p.blocks <= 4096)
+                hipLaunchKernelGGL((icl4_pick_kernel<4, 16>), rows, dim3(256), 0, stream, p);
+            else if (p.blocks <= 16384)
+                hipLaunchKernelGGL((icl4_pick_kernel<16, 16>), rows, dim3(1024), 0, stream, p);
+            else
+                hipLaunchKernelGGL((icl4_pick_kernel<16, 0>), rows, dim3(1024), 0, stream, p);
+            IRX_HIP(hipGetLastError());
+        }
 }
 
 void icl4_attend(const Icl4Queries &a, const Icl4Attend &b, hipStream_t stream) {
