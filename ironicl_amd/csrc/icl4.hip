@@ -476,7 +476,7 @@ struct AttendArgs {
     float scale;      // times log2 e
     float *partial;   // outputs [splits, pairs * q_rows, 64], then log2-sum-exps [splits, pairs * q_rows]
     int splits, per_split;  // blocks (or listed places) of a split
-    int qtiles;
+    int qtiles, count, per_xcd;
 };
 
 constexpr float kLn2 = 0.69314718055994530942f;
@@ -499,10 +499,10 @@ __device__ __forceinline__ void store_out(const AttendArgs &p, int pair, int row
 
 constexpr int kWaves = 4;
 
-// One workgroup per (16 queries, pair, split), or per (query, pair, split)
-// over listed blocks: wave w takes every fourth block of the split. FP32
-// queries and probabilities are pairs of FP16 values, two products each.
-template <typename T, bool LISTED, bool SPLIT>
+// One workgroup per (16 queries, pair, split): wave w takes every fourth block
+// of the split. FP32 queries and probabilities are pairs of FP16 values, two
+// products each.
+template <typename T, bool SPLIT>
 __global__ __launch_bounds__(kWaves * 64) void icl4_rows_kernel(AttendArgs p) {
     constexpr bool PAIRS = sizeof(T) == 4;
     __shared__ float red_o[kWaves][16 * 68];
@@ -514,7 +514,7 @@ __global__ __launch_bounds__(kWaves * 64) void icl4_rows_kernel(AttendArgs p) {
     const int qt = (int)(id % (unsigned)p.qtiles), pair = (int)(id / (unsigned)p.qtiles);
     const int e = pair / p.heads, head = pair - e * p.heads;
     const int rows = rows_of(p.lengths, e, p.rows);
-    const int qrow = LISTED ? qt : min(16 * qt + i16, p.q_rows - 1);
+    const int qrow = min(16 * qt + i16, p.q_rows - 1);
     half8 qh[2], ql[2];
     float c = p.scale;
     {
@@ -547,14 +547,8 @@ __global__ __launch_bounds__(kWaves * 64) void icl4_rows_kernel(AttendArgs p) {
     for (int d = 0; d < 4; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m_run = -INFINITY, l_run = 0.f;  // m_run: the largest score less the headroom
     const unsigned char *tiles = p.tiles + (long long)pair * p.blocks * kBlockBytes;
-    const int places = LISTED ? p.n : p.blocks;
-    const int end = min(places, (split + 1) * p.per_split);
-    for (int at = split * p.per_split + wave; at < end; at += kWaves) {
-        int block = at;
-        if constexpr (LISTED) {
-            block = p.list[((long long)pair * p.q_rows + qt) * p.n + at];
-            if ((unsigned)block >= (unsigned)p.blocks) continue;
-        }
+    const int end = min(p.blocks, (split + 1) * p.per_split);
+    for (int block = split * p.per_split + wave; block < end; block += kWaves) {
         const unsigned long long mask = block_mask(p.keep, e, p.blocks, block, rows);
         if (mask == 0) continue;
         const unsigned char *in = tiles + (long long)block * kBlockBytes;
@@ -628,8 +622,8 @@ __global__ __launch_bounds__(kWaves * 64) void icl4_rows_kernel(AttendArgs p) {
     for (int d = 0; d < 4; ++d) *reinterpret_cast<f32x4 *>(&red_o[wave][i16 * 68 + 16 * d + 4 * g]) = o[d];
     __syncthreads();
     const int qi = threadIdx.x >> 4, d = 4 * (threadIdx.x & 15);
-    const int out_row = LISTED ? qt : 16 * qt + qi;
-    if ((LISTED && qi) || out_row >= p.q_rows) return;
+    const int out_row = 16 * qt + qi;
+    if (out_row >= p.q_rows) return;
     float mx = -INFINITY;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, red_m[w][qi]);
@@ -652,6 +646,219 @@ __global__ __launch_bounds__(kWaves * 64) void icl4_rows_kernel(AttendArgs p) {
     } else {
         store_out<T>(p, pair, out_row, d, acc);
         if (p.lse && d == 0) p.lse[(long long)pair * p.q_rows + out_row] = lse2 * kLn2;
+    }
+}
+
+// Four consecutive lanes' neighbour: lane ^ 1.
+__device__ __forceinline__ float next_lane(float x) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0xb1, 0xf, 0xf, true));
+}
+
+// Lane N of each row of 16, in all of the row's lanes.
+template <int N>
+__device__ __forceinline__ unsigned row_lane(unsigned x) {
+    return __builtin_amdgcn_update_dpp(0, x, 0x150 + N, 0xf, 0xf, true);
+}
+
+// One block's operands of a wave as they lie in the cache.
+struct BlockWords {
+    u32x4 k[2], v[2];
+    unsigned ke;
+    u32x2 ve;
+};
+__device__ __forceinline__ void load_block(const unsigned char *in, int lane, BlockWords &w) {
+    const int g = lane >> 4, i16 = lane & 15;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        w.k[s] = *reinterpret_cast<const u32x4 *>(in + s * 1024 + lane * 16);
+        w.v[s] = *reinterpret_cast<const u32x4 *>(in + kValuesAt + s * 1024 + lane * 16);
+    }
+    w.ke = *reinterpret_cast<const unsigned *>(in + kKeyExpsAt + ((g >> 1) * 16 + i16) * 4);
+    w.ve = *reinterpret_cast<const u32x2 *>(in + kValueExpsAt + i16 * 8);
+}
+
+// One query per workgroup, its blocks (listed, or all) in turn over the waves.
+// All sixteen columns of the products hold the one query, so that a lane can
+// take one row's score out of its sixteen and the softmax costs one
+// exponential per row; FP32 operands' high and low parts stand in even and odd
+// columns, one product each, and neighbouring lanes add theirs.
+template <typename T, bool LISTED, bool SPLIT>
+__global__ __launch_bounds__(kWaves * 64) void icl4_one_kernel(AttendArgs p) {
+    constexpr bool PAIRS = sizeof(T) == 4;
+    __shared__ float red_o[kWaves][64];
+    __shared__ float red_m[kWaves], red_l[kWaves];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int g = lane >> 4, i16 = lane & 15;
+    // Workgroups of one XCD (every eighth) take consecutive queries of a pair, whose blocks then share its L2.
+    const unsigned id = (blockIdx.x & 7u) * (unsigned)p.per_xcd + (blockIdx.x >> 3);
+    if (id >= (unsigned)p.count) return;
+    const int split = (int)(id % (unsigned)p.splits);
+    const int pq = (int)(id / (unsigned)p.splits);
+    const int pair = pq / p.q_rows, row = pq - pair * p.q_rows;
+    const int e = pair / p.heads, head = pair - e * p.heads;
+    const int rows = rows_of(p.lengths, e, p.rows);
+    half8 q[2];
+    float c = p.scale;
+    {
+        const T *src = static_cast<const T *>(p.q) + e * p.q_est + head * p.q_head + (long long)row * p.q_row + 16 * g;
+        if constexpr (PAIRS) {
+            float x[16];
+            float m = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x4 v = *reinterpret_cast<const f32x4 *>(src + 4 * i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[4 * i + j] = v[j], m = fmaxf(m, fabsf(v[j]));
+            }
+            m = fmaxf(m, __shfl_xor(m, 16, 64));
+            m = fmaxf(m, __shfl_xor(m, 32, 64));
+            const int ex = pair_exponent(m);
+            const float up = pow2(ex);
+            c *= pow2(-ex);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] *= up;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                half8 hi, lo;
+                pair8(x + 8 * i, hi, lo);
+                q[i] = i16 & 1 ? lo : hi;
+            }
+        } else {
+            q[0] = *reinterpret_cast<const half8 *>(src);
+            q[1] = *reinterpret_cast<const half8 *>(src + 8);
+        }
+    }
+    f32x4 o[4];
+#pragma unroll
+    for (int d = 0; d < 4; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float ref = -INFINITY, l_run = 0.f;
+    const unsigned char *tiles = p.tiles + (long long)pair * p.blocks * kBlockBytes;
+    const int *list = LISTED ? p.list + (long long)pq * p.n : nullptr;
+    const int places = LISTED ? p.n : p.blocks;
+    const int end = min(places, (split + 1) * p.per_split);
+    // The lane's row of a block: result register i16 of its 16.
+    const int mine = 32 * (i16 >> 3) + 16 * (g >> 1) + 8 * ((i16 >> 2) & 1) + 4 * (g & 1) + (i16 & 3);
+    const unsigned parts = i16 & 1 ? 0x07060302u : 0x05040100u;  // low or high halves of two words
+
+    // The next place at or after `at` with a block to attend to: its block, or -1.
+    auto find = [&](int &at, unsigned long long &mask) {
+        for (; at < end; at += kWaves) {
+            const int block = LISTED ? __builtin_amdgcn_readfirstlane(list[at]) : at;
+            if (LISTED && (unsigned)block >= (unsigned)p.blocks) continue;
+            mask = block_mask(p.keep, e, p.blocks, block, rows);
+            if (mask) return block;
+        }
+        return -1;
+    };
+    auto process = [&](const BlockWords &w, unsigned long long mask) {
+        f32x4 s[4];
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) {
+            const float scale = __uint_as_float(((w.ke >> (8 * kb)) & 0xffu) << 23);
+            s[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+                s[kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(w.k[kb >> 1][2 * (kb & 1) + m], scale), q[m], s[kb],
+                                                               0, 0, 0);
+        }
+        // Register i16 and, for the neighbour, register i16 ^ 1.
+        float a[8], b[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a[i] = s[i >> 1][2 * (i & 1)], b[i] = s[i >> 1][2 * (i & 1) + 1];
+#pragma unroll
+        for (int half = 4; half >= 1; half /= 2)
+#pragma unroll
+            for (int i = 0; i < half; ++i) {
+                const bool up = i16 & (2 * half);
+                a[i] = up ? a[i + half] : a[i], b[i] = up ? b[i + half] : b[i];
+            }
+        const bool odd = i16 & 1;
+        float x = odd ? b[0] : a[0];
+        if constexpr (PAIRS) x += next_lane(odd ? a[0] : b[0]);
+        x *= c;
+        if (mask != ~0ull && !((mask >> mine) & 1)) x = -INFINITY;
+        float weight = __builtin_amdgcn_exp2f(x - ref);
+        if (__any(!(weight <= 32768.0f))) {
+            const float ref_new = fmaxf(ref, wave_max(x) - kHeadroom);
+            const float alpha = __builtin_amdgcn_exp2f(ref - ref_new);
+            l_run *= alpha;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) o[d] *= alpha;
+            ref = ref_new;
+            weight = __builtin_amdgcn_exp2f(x - ref);
+        }
+        l_run += weight;
+        const _Float16 hi = (_Float16)weight;
+        unsigned packed = __builtin_bit_cast(unsigned short, hi);
+        if constexpr (PAIRS)
+            packed |= (unsigned)__builtin_bit_cast(unsigned short, (_Float16)(weight - (float)hi)) << 16;
+        const unsigned all[16] = {row_lane<0>(packed),  row_lane<1>(packed),  row_lane<2>(packed),  row_lane<3>(packed),
+                                  row_lane<4>(packed),  row_lane<5>(packed),  row_lane<6>(packed),  row_lane<7>(packed),
+                                  row_lane<8>(packed),  row_lane<9>(packed),  row_lane<10>(packed), row_lane<11>(packed),
+                                  row_lane<12>(packed), row_lane<13>(packed), row_lane<14>(packed), row_lane<15>(packed)};
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+            u32x4 pw;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                pw[j] = __builtin_amdgcn_perm(all[8 * st + 2 * j + 1], all[8 * st + 2 * j], PAIRS ? parts : 0x05040100u);
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                    codes8(w.v[st][d], __uint_as_float(((w.ve[st] >> (8 * d)) & 0xffu) << 23)), as_half8(pw), o[d], 0, 0, 0);
+        }
+    };
+    // Two sets of operands in turn: the next block's loads are issued before this one's products.
+    BlockWords wa, wb;
+    unsigned long long mask_a = 0, mask_b = 0;
+    int at = split * p.per_split + wave;
+    int block = find(at, mask_a);
+    if (block >= 0) load_block(tiles + (long long)block * kBlockBytes, lane, wa);
+    while (block >= 0) {
+        at += kWaves;
+        block = find(at, mask_b);
+        if (block >= 0) load_block(tiles + (long long)block * kBlockBytes, lane, wb);
+        process(wa, mask_a);
+        if (block < 0) break;
+        at += kWaves;
+        block = find(at, mask_a);
+        if (block >= 0) load_block(tiles + (long long)block * kBlockBytes, lane, wa);
+        process(wb, mask_b);
+    }
+    // Register r of o[d]: dim 16 d + 4 g + r, in every column (pair of columns).
+    l_run = wave_sum(l_run);
+    if (lane == 0) red_m[wave] = ref, red_l[wave] = l_run;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+        f32x4 v = o[d];
+        if constexpr (PAIRS)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] += next_lane(v[r]);
+        if (i16 == 0) *reinterpret_cast<f32x4 *>(&red_o[wave][16 * d + 4 * g]) = v;
+    }
+    __syncthreads();
+    if (threadIdx.x >= 16) return;
+    const int d = 4 * threadIdx.x;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, red_m[w]);
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    float den = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        const float a = mx > -INFINITY ? __builtin_amdgcn_exp2f(red_m[w] - mx) : 1.0f;
+        acc += a * *reinterpret_cast<const f32x4 *>(&red_o[w][d]);
+        den += a * red_l[w];
+    }
+    if (den != 0.f) acc *= 1.0f / den;
+    const float lse2 = mx + log2f(den);
+    if constexpr (SPLIT) {
+        const long long all = (long long)p.pairs * p.q_rows, to = split * all + pq;
+        *reinterpret_cast<f32x4 *>(p.partial + to * 64 + d) = acc;
+        if (d == 0) p.partial[p.splits * all * 64 + to] = lse2;
+    } else {
+        store_out<T>(p, pair, row, d, acc);
+        if (p.lse && d == 0) p.lse[pq] = lse2 * kLn2;
     }
 }
 
@@ -722,15 +929,20 @@ __global__ __launch_bounds__(256) void icl4_merge_kernel(AttendArgs p) {
 }
 
 struct Plan {
+    bool one;  // a query per workgroup (icl4_one_kernel)
     int qtiles, splits, per_split;
     long long rows;  // (pair, query) rows
 };
+
+// Queries up to which attention over every block takes a workgroup per query.
+constexpr int kOneQueries = 1;
 
 // About two workgroups per compute unit, at least four blocks to a split (one to a wave).
 Plan plan_attend(const Icl4Shape &s, int q_rows, int n_blocks, int compute_units) {
     Plan pl{};
     const int places = n_blocks ? n_blocks : s.blocks();
-    pl.qtiles = n_blocks ? q_rows : (int)ceil_div(q_rows, 16);
+    pl.one = n_blocks || q_rows <= kOneQueries;
+    pl.qtiles = pl.one ? q_rows : (int)ceil_div(q_rows, 16);
     pl.rows = (long long)s.pairs() * q_rows;
     const long long base = (long long)s.pairs() * pl.qtiles;
     const long long want = std::max<long long>(1, (2LL * compute_units + base - 1) / base);
@@ -778,19 +990,26 @@ void attend(const Icl4Queries &a, const Icl4Attend &b, hipStream_t stream) {
     p.list = b.list, p.n = b.n, p.heads = s.heads, p.pairs = s.pairs(), p.q_rows = a.q_rows, p.rows = s.rows;
     p.blocks = s.blocks(), p.scale = b.scale * kLog2e, p.partial = static_cast<float *>(b.workspace);
     p.splits = pl.splits, p.per_split = pl.per_split, p.qtiles = pl.qtiles;
-    const dim3 grid((unsigned)((long long)pl.splits * pl.qtiles * s.pairs())), wg(kWaves * 64);
+    const long long count = (long long)pl.splits * pl.qtiles * s.pairs();
+    p.count = (int)count, p.per_xcd = (int)ceil_div((size_t)count, 8);
+    const dim3 grid((unsigned)(pl.one ? 8LL * p.per_xcd : count)), wg(kWaves * 64);
     {
         const long long tiles = b.list ? (long long)pl.rows * b.n : (long long)s.pairs() * s.blocks();
         const double work = 256.0 * kBlock * (b.list ? (double)tiles : (double)tiles * a.q_rows);
         KernelTimer timer(kFamIcl, stream, work, (double)tiles * kBlockBytes + 2.0 * sizeof(T) * 64 * pl.rows);
-        if (b.list && pl.splits > 1)
-            hipLaunchKernelGGL((icl4_rows_kernel<T, true, true>), grid, wg, 0, stream, p);
+        const bool split = pl.splits > 1;
+        if (b.list && split)
+            hipLaunchKernelGGL((icl4_one_kernel<T, true, true>), grid, wg, 0, stream, p);
         else if (b.list)
-            hipLaunchKernelGGL((icl4_rows_kernel<T, true, false>), grid, wg, 0, stream, p);
-        else if (pl.splits > 1)
-            hipLaunchKernelGGL((icl4_rows_kernel<T, false, true>), grid, wg, 0, stream, p);
+            hipLaunchKernelGGL((icl4_one_kernel<T, true, false>), grid, wg, 0, stream, p);
+        else if (pl.one && split)
+            hipLaunchKernelGGL((icl4_one_kernel<T, false, true>), grid, wg, 0, stream, p);
+        else if (pl.one)
+            hipLaunchKernelGGL((icl4_one_kernel<T, false, false>), grid, wg, 0, stream, p);
+        else if (split)
+            hipLaunchKernelGGL((icl4_rows_kernel<T, true>), grid, wg, 0, stream, p);
         else
-            hipLaunchKernelGGL((icl4_rows_kernel<T, false, false>), grid, wg, 0, stream, p);
+            hipLaunchKernelGGL((icl4_rows_kernel<T, false>), grid, wg, 0, stream, p);
         IRX_HIP(hipGetLastError());
     }
     if (pl.splits > 1) {
