@@ -649,6 +649,243 @@ __global__ __launch_bounds__(kWaves * 64) void icl4_rows_kernel(AttendArgs p) {
     }
 }
 
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+constexpr int kWideStride = 68;  // floats of one query's row in LDS
+
+// Larger of, or sum of, a lane's value and lane ^ 32's.
+__device__ __forceinline__ float halves_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float halves_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// 32 NJ queries per workgroup, every fourth block of its share to a wave, on
+// 32x32x16 products. A wave reads its blocks straight into registers and
+// decodes them there: 4 bits a number are few enough that neither LDS nor a
+// barrier stands between the cache and the products. Lane (r = lane % 32, h =
+// lane / 32), r = 16 s + 8 a + i:
+//   S^T, b = 0, 1: A = rows 32 s + 16 a + 8 b + i, dims 32 h + 8 m ..; B = query r, the same
+//     dims; result register 8 s + 4 a + j is row 32 s + 16 a + 8 b + 4 h + j, query r;
+//   O^T, D = 0, 1, step (s, a): A = dim 32 x + 16 D + i (r = 16 x + i), rows 32 s + 16 a + 8 b
+//     + 4 h + j; B = those probabilities, where they are; result register 8 x + 4 y + j is
+//     dim 32 x + 16 D + 8 y + 4 h + j, query r.
+template <typename T, int NJ, bool SPLIT>
+__global__ __launch_bounds__(kWaves * 64, 2) void icl4_wide_kernel(AttendArgs p) {
+    constexpr bool PAIRS = sizeof(T) == 4;
+    __shared__ float red_o[kWaves][32 * NJ * kWideStride];
+    __shared__ float red_m[kWaves][32 * NJ], red_l[kWaves][32 * NJ];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int h = lane >> 5, r32 = lane & 31, i16 = lane & 15, x16 = (lane >> 4) & 1;
+    // Workgroups of one XCD take consecutive query tiles of one share of the blocks, read into one L2.
+    unsigned id = (blockIdx.x & 7u) * (unsigned)p.per_xcd + (blockIdx.x >> 3);
+    if (id >= (unsigned)p.count) return;
+    const int qt = (int)(id % (unsigned)p.qtiles);
+    id /= (unsigned)p.qtiles;
+    const int split = (int)(id % (unsigned)p.splits), pair = (int)(id / (unsigned)p.splits);
+    const int e = pair / p.heads, head = pair - e * p.heads;
+    const int rows = rows_of(p.lengths, e, p.rows);
+    half8 qh[NJ][4], ql[PAIRS ? NJ : 1][4];
+    float c[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        const int row = min(32 * (NJ * qt + j) + r32, p.q_rows - 1);
+        const T *src = static_cast<const T *>(p.q) + e * p.q_est + head * p.q_head + (long long)row * p.q_row + 32 * h;
+        c[j] = p.scale;
+        if constexpr (PAIRS) {
+            float x[32];
+            float m = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const f32x4 v = *reinterpret_cast<const f32x4 *>(src + 4 * i);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[4 * i + k] = v[k], m = fmaxf(m, fabsf(v[k]));
+            }
+            const int ex = pair_exponent(halves_max(m));
+            const float up = pow2(ex);
+            c[j] *= pow2(-ex);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[i] *= up;
+#pragma unroll
+            for (int m4 = 0; m4 < 4; ++m4) pair8(x + 8 * m4, qh[j][m4], ql[j][m4]);
+        } else {
+#pragma unroll
+            for (int m4 = 0; m4 < 4; ++m4) qh[j][m4] = *reinterpret_cast<const half8 *>(src + 8 * m4);
+        }
+    }
+    f32x16 o[NJ][2];
+    float ref[NJ], l_run[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        ref[j] = -INFINITY, l_run[j] = 0.f;
+#pragma unroll
+        for (int d = 0; d < 2; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[j][d][r] = 0.f;
+    }
+    struct Words {
+        u32x4 k[2];
+        u32x2 v[4];
+        unsigned ke;
+        u32x2 ve;
+    };
+    const unsigned char *tiles = p.tiles + (long long)pair * p.blocks * kBlockBytes;
+    const int k_at = x16 * 1024 + (32 * h + i16) * 16, v_at = kValuesAt + (16 * h + i16) * 16 + 8 * x16;
+    const int ke_at = kKeyExpsAt + (16 * h + i16) * 4, ve_at = kValueExpsAt + i16 * 8;
+    auto load = [&](int block, Words &w) {
+        const unsigned char *in = tiles + (long long)block * kBlockBytes;
+        w.k[0] = *reinterpret_cast<const u32x4 *>(in + k_at);
+        w.k[1] = *reinterpret_cast<const u32x4 *>(in + k_at + 256);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) w.v[t] = *reinterpret_cast<const u32x2 *>(in + v_at + 512 * t);
+        w.ke = *reinterpret_cast<const unsigned *>(in + ke_at);
+        w.ve = *reinterpret_cast<const u32x2 *>(in + ve_at);
+    };
+    const int end = min(p.blocks, (split + 1) * p.per_split);
+    auto find = [&](int &at, unsigned long long &mask) {
+        for (; at < end; at += kWaves) {
+            mask = block_mask(p.keep, e, p.blocks, at, rows);
+            if (mask) return true;
+        }
+        return false;
+    };
+    auto process = [&](const Words &w, unsigned long long mask) {
+        const unsigned ke = w.ke >> (16 * x16);
+        const float ks[2] = {__uint_as_float((ke & 0xffu) << 23), __uint_as_float((ke >> 8 & 0xffu) << 23)};
+        f32x16 s[NJ][2];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[j][b][r] = 0.f;
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const half8 a = codes8(w.k[m >> 1][2 * b + (m & 1)], ks[b]);
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    if constexpr (PAIRS) s[j][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[j][m], s[j][b], 0, 0, 0);
+                    s[j][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[j][m], s[j][b], 0, 0, 0);
+                }
+            }
+        if (mask != ~0ull) {
+            const unsigned long long mine = mask >> (4 * h);
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (!((mine >> (32 * (r >> 3) + 16 * ((r >> 2) & 1) + 8 * b + (r & 3))) & 1))
+#pragma unroll
+                        for (int j = 0; j < NJ; ++j) s[j][b][r] = -INFINITY;
+        }
+        half8 ph[NJ][4], pl[PAIRS ? NJ : 1][4];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            float mt = s[j][0][0];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mt = fmaxf(mt, fmaxf(s[j][0][r], s[j][1][r]));
+            // The reference is raised when a probability could pass 2^15: each query's by
+            // its own scores alone, whatever the others of its wave do.
+            if (__any(!(mt * c[j] - ref[j] <= 15.0f))) {
+                const float top = halves_max(mt) * c[j];
+                const float ref_new = top - ref[j] <= 15.0f ? ref[j] : fmaxf(ref[j], top - kHeadroom);
+                const float alpha = __builtin_amdgcn_exp2f(ref[j] - ref_new);
+                ref[j] = ref_new;
+                l_run[j] *= alpha;
+#pragma unroll
+                for (int d = 0; d < 2; ++d) o[j][d] *= alpha;
+            }
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    x[i] = __builtin_amdgcn_exp2f(fmaf(s[j][i >> 2][4 * t + (i & 3)], c[j], -ref[j]));
+                    l_run[j] += x[i];
+                }
+                if constexpr (PAIRS) {
+                    pair8(x, ph[j][t], pl[j][t]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) ph[j][t][i] = (_Float16)x[i];
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {  // t = 2 s + a
+            const unsigned ve = w.ve[t >> 1] >> (16 * x16);
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+                const half8 a = codes8(w.v[t][d], __uint_as_float((ve >> (8 * d) & 0xffu) << 23));
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    if constexpr (PAIRS) o[j][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[j][t], o[j][d], 0, 0, 0);
+                    o[j][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[j][t], o[j][d], 0, 0, 0);
+                }
+            }
+        }
+    };
+    Words wa, wb;
+    unsigned long long mask_a = 0, mask_b = 0;
+    int at = split * p.per_split + wave;
+    bool more = find(at, mask_a);
+    if (more) load(at, wa);
+    while (more) {
+        at += kWaves;
+        more = find(at, mask_b);
+        if (more) load(at, wb);
+        process(wa, mask_a);
+        if (!more) break;
+        at += kWaves;
+        more = find(at, mask_a);
+        if (more) load(at, wa);
+        process(wb, mask_b);
+    }
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        const int q = 32 * j + r32;
+        const float l = halves_sum(l_run[j]);
+        if (h == 0) red_m[wave][q] = ref[j], red_l[wave][q] = l;
+#pragma unroll
+        for (int d = 0; d < 2; ++d)
+#pragma unroll
+            for (int a = 0; a < 4; ++a)
+                *reinterpret_cast<f32x4 *>(&red_o[wave][q * kWideStride + 32 * (a >> 1) + 16 * d + 8 * (a & 1) + 4 * h]) =
+                    f32x4{o[j][d][4 * a], o[j][d][4 * a + 1], o[j][d][4 * a + 2], o[j][d][4 * a + 3]};
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2 * NJ; ++i) {
+        const int q = 16 * i + (threadIdx.x >> 4), d = 4 * (threadIdx.x & 15), row = 32 * NJ * qt + q;
+        if (row >= p.q_rows) continue;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, red_m[w][q]);
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        float den = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float a = mx > -INFINITY ? __builtin_amdgcn_exp2f(red_m[w][q] - mx) : 1.0f;
+            acc += a * *reinterpret_cast<const f32x4 *>(&red_o[w][q * kWideStride + d]);
+            den += a * red_l[w][q];
+        }
+        if (den != 0.f) acc *= 1.0f / den;
+        const float lse2 = mx + log2f(den);
+        const long long all = (long long)p.pairs * p.q_rows, pq = (long long)pair * p.q_rows + row;
+        if constexpr (SPLIT) {
+            *reinterpret_cast<f32x4 *>(p.partial + (split * all + pq) * 64 + d) = acc;
+            if (d == 0) p.partial[p.splits * all * 64 + split * all + pq] = lse2;
+        } else {
+            store_out<T>(p, pair, row, d, acc);
+            if (p.lse && d == 0) p.lse[pq] = lse2 * kLn2;
+        }
+    }
+}
+
 // Four consecutive lanes' neighbour: lane ^ 1.
 __device__ __forceinline__ float next_lane(float x) {
     return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0xb1, 0xf, 0xf, true));
@@ -929,7 +1166,7 @@ __global__ __launch_bounds__(256) void icl4_merge_kernel(AttendArgs p) {
 }
 
 struct Plan {
-    bool one;  // a query per workgroup (icl4_one_kernel)
+    int queries;  // of a workgroup: 1, 16, 32 or 64
     int qtiles, splits, per_split;
     long long rows;  // (pair, query) rows
 };
@@ -941,13 +1178,25 @@ constexpr int kOneQueries = 1;
 Plan plan_attend(const Icl4Shape &s, int q_rows, int n_blocks, int compute_units) {
     Plan pl{};
     const int places = n_blocks ? n_blocks : s.blocks();
-    pl.one = n_blocks || q_rows <= kOneQueries;
-    pl.qtiles = pl.one ? q_rows : (int)ceil_div(q_rows, 16);
+    pl.queries = n_blocks || q_rows <= kOneQueries ? 1 : q_rows <= 16 ? 16 : q_rows <= 32 ? 32 : 64;
+    pl.qtiles = (int)ceil_div(q_rows, pl.queries);
     pl.rows = (long long)s.pairs() * q_rows;
     const long long base = (long long)s.pairs() * pl.qtiles;
-    const long long want = std::max<long long>(1, (2LL * compute_units + base - 1) / base);
-    const int splits = (int)std::min<long long>(want, std::max(1, places / kWaves));
-    pl.per_split = (int)ceil_div(ceil_div(places, splits), kWaves) * kWaves;
+    const long long slots = 2LL * compute_units, tiles = ceil_div(places, kWaves);
+    long long splits = 1;
+    if (pl.queries <= 16) {
+        splits = std::min(std::max(1LL, (slots + base - 1) / base), tiles);
+    } else {
+        // Microseconds: a workgroup's start and end, each round of its waves' blocks, the merge.
+        double best = 1e30;
+        for (long long n = 1; n <= std::min(tiles, std::max(8LL, 2 * slots / base)); ++n) {
+            const double rounds = (double)((base * n + slots - 1) / slots);
+            const double merge = n > 1 ? 4.0 + (double)pl.rows * (double)n * (520.0 / 4e6) : 0.0;
+            const double cost = rounds * (6.0 + 1.5 * (double)((tiles + n - 1) / n)) + merge;
+            if (cost < best) best = cost, splits = n;
+        }
+    }
+    pl.per_split = (int)((tiles + splits - 1) / splits) * kWaves;
     pl.splits = (int)ceil_div(places, pl.per_split);
     return pl;
 }
@@ -992,7 +1241,7 @@ void attend(const Icl4Queries &a, const Icl4Attend &b, hipStream_t stream) {
     p.splits = pl.splits, p.per_split = pl.per_split, p.qtiles = pl.qtiles;
     const long long count = (long long)pl.splits * pl.qtiles * s.pairs();
     p.count = (int)count, p.per_xcd = (int)ceil_div((size_t)count, 8);
-    const dim3 grid((unsigned)(pl.one ? 8LL * p.per_xcd : count)), wg(kWaves * 64);
+    const dim3 grid((unsigned)(pl.queries == 16 ? count : 8LL * p.per_xcd)), wg(kWaves * 64);
     {
         const long long tiles = b.list ? (long long)pl.rows * b.n : (long long)s.pairs() * s.blocks();
         const double work = 256.0 * kBlock * (b.list ? (double)tiles : (double)tiles * a.q_rows);
@@ -1002,14 +1251,22 @@ void attend(const Icl4Queries &a, const Icl4Attend &b, hipStream_t stream) {
             hipLaunchKernelGGL((icl4_one_kernel<T, true, true>), grid, wg, 0, stream, p);
         else if (b.list)
             hipLaunchKernelGGL((icl4_one_kernel<T, true, false>), grid, wg, 0, stream, p);
-        else if (pl.one && split)
+        else if (pl.queries == 1 && split)
             hipLaunchKernelGGL((icl4_one_kernel<T, false, true>), grid, wg, 0, stream, p);
-        else if (pl.one)
+        else if (pl.queries == 1)
             hipLaunchKernelGGL((icl4_one_kernel<T, false, false>), grid, wg, 0, stream, p);
-        else if (split)
+        else if (pl.queries == 16 && split)
             hipLaunchKernelGGL((icl4_rows_kernel<T, true>), grid, wg, 0, stream, p);
-        else
+        else if (pl.queries == 16)
             hipLaunchKernelGGL((icl4_rows_kernel<T, false>), grid, wg, 0, stream, p);
+        else if (pl.queries == 32 && split)
+            hipLaunchKernelGGL((icl4_wide_kernel<T, 1, true>), grid, wg, 0, stream, p);
+        else if (pl.queries == 32)
+            hipLaunchKernelGGL((icl4_wide_kernel<T, 1, false>), grid, wg, 0, stream, p);
+        else if (split)
+            hipLaunchKernelGGL((icl4_wide_kernel<T, 2, true>), grid, wg, 0, stream, p);
+        else
+            hipLaunchKernelGGL((icl4_wide_kernel<T, 2, false>), grid, wg, 0, stream, p);
         IRX_HIP(hipGetLastError());
     }
     if (pl.splits > 1) {
