@@ -23,6 +23,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace irx {
 namespace {
@@ -79,18 +80,13 @@ __device__ __forceinline__ int code_exponent(float m) {
     return min(13, max(-13, (bits & 0x7fffffu) <= 0x400000u ? x - 3 : x - 2));
 }
 
-// The E2M1 code of x / 2^e: to nearest, ties to the even code, saturated.
-__device__ __forceinline__ unsigned code_of(float x, float inv) {
-    const float m = fabsf(x) * inv;
-    const unsigned c = (m > 0.25f) + (m >= 0.75f) + (m > 1.25f) + (m >= 1.75f) + (m > 2.5f) + (m >= 3.5f) + (m > 5.0f);
-    return c | (x < 0.f ? 8u : 0u);
-}
-
-__device__ __forceinline__ float value_of(unsigned code, float scale) {
-    const unsigned c = code & 7u;
-    // 0, 0.5, then 1.m * 2^(c / 2 - 1) with m the low bit.
-    const float m = c < 2u ? 0.5f * (float)c : (1.0f + 0.5f * (float)(c & 1u)) * (float)(1u << ((c >> 1) - 1));
-    return (code & 8u ? -m : m) * scale;
+// Eight numbers as E2M1 codes of x / 2^e: to nearest, ties to the even code, saturated.
+__device__ __forceinline__ unsigned coded8(const float *x, float scale) {
+    unsigned w = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], scale, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], scale, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], scale, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], scale, 3);
 }
 
 // The smallest unit 2^x with m <= 127 * 2^x (m a held key; 2^-20 for zero).
@@ -117,105 +113,178 @@ __global__ __launch_bounds__(256) void icl4_units_kernel(float *scales, int coun
     if (i < count) scales[i] = 9.5367431640625e-07f;  // 2^-20
 }
 
+// The value of the lane eight, or sixteen, away (lane ^ 8 and lane ^ 16).
+__device__ __forceinline__ unsigned other_eight(unsigned x) {
+    return __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, true);
+}
+__device__ __forceinline__ float rows_max(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+// Lane ^ N of a row of 16, N a power of two below 16.
+template <int N>
+__device__ __forceinline__ unsigned row_xor(unsigned x) {
+    if constexpr (N == 1) return __builtin_amdgcn_update_dpp(0, x, 0xb1, 0xf, 0xf, true);  // 1, 0, 3, 2
+    if constexpr (N == 2) return __builtin_amdgcn_update_dpp(0, x, 0x4e, 0xf, 0xf, true);  // 2, 3, 0, 1
+    if constexpr (N == 4) {  // the halves of each eight swapped: mirrored, then each four mirrored
+        const unsigned m = __builtin_amdgcn_update_dpp(0, x, 0x141, 0xf, 0xf, true);
+        return __builtin_amdgcn_update_dpp(0, m, 0x1b, 0xf, 0xf, true);
+    }
+    if constexpr (N == 8) return other_eight(x);
+}
+typedef short short2v __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ unsigned pk_max(unsigned a, unsigned b) {  // of positive FP16 pairs
+    return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(short2v, a), __builtin_bit_cast(short2v, b)));
+}
+
+__device__ __forceinline__ void load16(const float *src, float *x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const f32x4 v = *reinterpret_cast<const f32x4 *>(src + 4 * i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[4 * i + j] = v[j];
+    }
+}
+__device__ __forceinline__ void load16(const _Float16 *src, float *x) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const half8 v = *reinterpret_cast<const half8 *>(src + 8 * i);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[8 * i + j] = (float)v[j];
+    }
+}
+
 // One workgroup per (block, pair): codes and exponents; the bounds' scales by
-// maxima of 2^x (as words, so their order does not matter).
+// maxima of 2^x (as words, so their order does not matter). Bound by its
+// reads: every load of the block is issued first, and the codes are the
+// conversion instructions' own. The block is put together in LDS and written in
+// whole lines: from registers, in words of several waves each, 50,000 rows took
+// 315 us. Keys: wave 2 s + b, lane (g, 8 a + i) takes
+// dims 16 g .. of row 32 s + 16 a + 8 b + i. Values: wave d, lane 8 (4 s + 2 t
+// + b) + i takes dims 16 d + 2 i and + 1 of rows 32 s + 16 t + 8 b .. +7.
 template <typename T>
 __global__ __launch_bounds__(256) void icl4_encode_kernel(StoreArgs p) {
-    __shared__ float held[64][65];
-    __shared__ float part_max[4][64];
-    const int tid = threadIdx.x;
+    typedef T T2 __attribute__((ext_vector_type(2)));
+    __shared__ unsigned peaks[4][32];
+    __shared__ __attribute__((aligned(16))) unsigned char out[kBlockBytes];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, i16 = lane & 15;
     const int block = (int)(blockIdx.x % (unsigned)p.blocks), pair = (int)(blockIdx.x / (unsigned)p.blocks);
     const int e = pair / p.heads, head = pair - e * p.heads;
-    const int rows = rows_of(p.lengths, e, p.rows);
-    unsigned char *out = p.tiles + ((long long)pair * p.blocks + block) * kBlockBytes;
+    const int left = rows_of(p.lengths, e, p.rows) - block * kBlock;  // rows of the block inside the length
+    const int key_row = 32 * (wave >> 1) + 16 * (i16 >> 3) + 8 * (wave & 1) + (i16 & 7);
+    const int value_row = 8 * (lane >> 3), value_dim = 16 * wave + 2 * (lane & 7);
+    float x[16];
+    T2 v[8];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = T2{(T)0.f, (T)0.f};
+    {
+        const long long row0 = (long long)block * kBlock;
+        const T *k = static_cast<const T *>(p.k) + e * p.k_est + head * p.k_head + (row0 + key_row) * p.k_row + 16 * g;
+        const T *vs = static_cast<const T *>(p.v) + e * p.v_est + head * p.v_head + (row0 + value_row) * p.v_row + value_dim;
+        if (key_row < left) load16(k, x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (value_row + i < left) v[i] = *reinterpret_cast<const T2 *>(vs + i * p.v_row);
+    }
     unsigned bad = 0;
-    {  // Keys: thread t takes dims 16 (t % 4) .. +15 of row t / 4.
-        const int r = tid >> 2, g = tid & 3;
-        const long long row = (long long)block * kBlock + r;
-        float x[16];
+    auto fix = [&](float &y) {
+        if (!(fabsf(y) <= 3.4028235e38f)) y = 0.f, ++bad;
+    };
+    {
         float m = 0.f;
-        const T *src = static_cast<const T *>(p.k) + e * p.k_est + head * p.k_head + row * p.k_row + 16 * g;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            x[i] = row < rows ? to_float(src[i]) : 0.f;
-            if (!(fabsf(x[i]) <= 3.4028235e38f)) x[i] = 0.f, ++bad;
+            fix(x[i]);
             m = fmaxf(m, fabsf(x[i]));
         }
-        m = fmaxf(m, __shfl_xor(m, 1, 64));
-        const int ex = code_exponent(m);
-        const float inv = pow2(-ex), scale = pow2(ex);
-        unsigned w[2] = {0u, 0u};
+        const int ex = code_exponent(rows_max(m));  // lanes of dims 32 u and + 16
+        const float scale = pow2(ex);
+        const u32x2 w = {coded8(x, scale), coded8(x + 8, scale)};
+        const int s = wave >> 1, b = wave & 1;
+        *reinterpret_cast<u32x2 *>(out + s * 1024 + lane * 16 + b * 8) = w;
+        if (!(g & 1)) out[kKeyExpsAt + ((g >> 1) * 16 + i16) * 4 + 2 * s + b] = (unsigned char)(ex + 127);
+        // Largest held |key| of each dim over the wave's rows: FP16 pairs, exact, in every lane of a row of 16.
+        u32x4 held[2];
+        held[0] = __builtin_bit_cast(u32x4, codes8(w[0], scale)), held[1] = __builtin_bit_cast(u32x4, codes8(w[1], scale));
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const unsigned c = code_of(x[i], inv);
-            w[i >> 3] |= c << (4 * (i & 7));
-            held[r][16 * g + i] = fabsf(value_of(c, scale));
+        for (int i = 0; i < 8; ++i) {
+            unsigned y = held[i >> 2][i & 3] & 0x7fff7fffu;
+            y = pk_max(y, row_xor<1>(y));
+            y = pk_max(y, row_xor<2>(y));
+            y = pk_max(y, row_xor<4>(y));
+            y = pk_max(y, row_xor<8>(y));
+            if (i16 == i) peaks[wave][8 * g + i] = y;
         }
-        const int s = r >> 5, a = (r >> 4) & 1, b = (r >> 3) & 1, i8 = r & 7;
-        *reinterpret_cast<u32x2 *>(out + s * 1024 + (16 * g + 8 * a + i8) * 16 + b * 8) = u32x2{w[0], w[1]};
-        if (!(g & 1)) out[kKeyExpsAt + ((g >> 1) * 16 + 8 * a + i8) * 4 + 2 * s + b] = (unsigned char)(ex + 127);
     }
     __syncthreads();
-    {  // Largest held |key| of each dim, into the bounds' scales.
-        const int d = tid & 63, q = tid >> 6;
-        float m = 0.f;
+    if (tid < 32) {
+        const unsigned m = pk_max(pk_max(peaks[0][tid], peaks[1][tid]), pk_max(peaks[2][tid], peaks[3][tid]));
+        const half2v pair2 = __builtin_bit_cast(half2v, m);
+        unsigned *unit = reinterpret_cast<unsigned *>(p.scales) + pair * 64 + 2 * tid;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) m = fmaxf(m, held[16 * q + i][d]);
-        part_max[q][d] = m;
+        for (int i = 0; i < 2; ++i) {
+            const unsigned u = __float_as_uint(bound_unit((float)pair2[i]));
+            // Few blocks raise a unit: one that is seen to be as large needs no atomic.
+            if (unit[i] < u) atomicMax(unit + i, u);
+        }
+    }
+    {
+        float m[2] = {0.f, 0.f}, y[2][8];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                y[c][i] = (float)v[i][c];
+                fix(y[c][i]);
+                m[c] = fmaxf(m[c], fabsf(y[c][i]));
+            }
+            // The 32 rows of a group: lanes ^ 8 and ^ 16.
+            m[c] = fmaxf(m[c], __uint_as_float(other_eight(__float_as_uint(m[c]))));
+            m[c] = rows_max(m[c]);
+        }
+        const int s = lane >> 5, t = (lane >> 4) & 1, b = (lane >> 3) & 1;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int i = 2 * (lane & 7) + c, ex = code_exponent(m[c]);
+            const unsigned w = coded8(y[c], pow2(ex));  // rows 4 h + j of h = 0 in the low half
+            // The lane of b = 0 writes the word of h = 0, that of b = 1 the other.
+            const unsigned far = other_eight(w);
+            const unsigned word = b ? (far >> 16) | (w & 0xffff0000u) : (w & 0xffffu) | (far << 16);
+            *reinterpret_cast<unsigned *>(out + kValuesAt + s * 1024 + (16 * (2 * t + b) + i) * 16 + wave * 4) = word;
+            if (!(lane & 24)) out[kValueExpsAt + i * 8 + s * 4 + wave] = (unsigned char)(ex + 127);
+        }
     }
     __syncthreads();
-    if (tid < 64) {
-        const float m = fmaxf(fmaxf(part_max[0][tid], part_max[1][tid]), fmaxf(part_max[2][tid], part_max[3][tid]));
-        atomicMax(reinterpret_cast<unsigned *>(p.scales) + pair * 64 + tid, __float_as_uint(bound_unit(m)));
-    }
-    __syncthreads();
-    {  // Values: thread t takes rows 16 (t / 64) .. +15 of dim t % 64.
-        const int d = tid & 63, q = tid >> 6;
-        float x[16];
-        float m = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const long long row = (long long)block * kBlock + 16 * q + i;
-            const T *src = static_cast<const T *>(p.v) + e * p.v_est + head * p.v_head + row * p.v_row + d;
-            x[i] = row < rows ? to_float(*src) : 0.f;
-            if (!(fabsf(x[i]) <= 3.4028235e38f)) x[i] = 0.f, ++bad;
-            m = fmaxf(m, fabsf(x[i]));
-        }
-        part_max[q][d] = m;
-        __syncthreads();
-        m = fmaxf(m, part_max[q ^ 1][d]);
-        const int ex = code_exponent(m);
-        const float inv = pow2(-ex);
-        const int s = q >> 1, t = q & 1;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            unsigned w = 0u;
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) w |= code_of(x[8 * b + 4 * h + j], inv) << (4 * (4 * b + j));
-            *reinterpret_cast<unsigned *>(out + kValuesAt + s * 1024 + (16 * (2 * t + h) + (d & 15)) * 16 +
-                                          (d >> 4) * 4) = w;
-        }
-        if (!t) out[kValueExpsAt + (d & 15) * 8 + s * 4 + (d >> 4)] = (unsigned char)(ex + 127);
-    }
+    u32x4 *to = reinterpret_cast<u32x4 *>(p.tiles + ((long long)pair * p.blocks + block) * kBlockBytes);
+    to[tid] = reinterpret_cast<const u32x4 *>(out)[tid];
+    if (tid < kBlockBytes / 16 - 256) to[256 + tid] = reinterpret_cast<const u32x4 *>(out)[256 + tid];
     if (bad && p.nonfinite) atomicAdd(p.nonfinite, bad);
 }
 
-// Bounds of one block per wave, from the codes: lane 16 g + i16 holds dims
-// 16 g .. +15 of four rows; the 16 lanes of a g join theirs.
+__device__ __forceinline__ unsigned pk_least(unsigned a, unsigned b) {
+    return __builtin_bit_cast(unsigned, __builtin_elementwise_min(__builtin_bit_cast(half2v, a), __builtin_bit_cast(half2v, b)));
+}
+__device__ __forceinline__ unsigned pk_most(unsigned a, unsigned b) {
+    return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(half2v, a), __builtin_bit_cast(half2v, b)));
+}
+
+// Bounds of one block per wave, from the codes as FP16 pairs (exact): lane
+// (g, i16) holds dims 16 g .. +15 of four rows; in four steps each lane hands
+// half of its dims to another and keeps the least and most of the rest, so
+// that lane i16 ends with dim 16 g + i16's.
 __global__ __launch_bounds__(256) void icl4_bounds_kernel(StoreArgs p) {
     const int lane = threadIdx.x & 63, g = lane >> 4, i16 = lane & 15;
     const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (at >= (long long)p.pairs * p.blocks) return;
     const int pair = (int)(at / p.blocks), block = (int)(at - (long long)pair * p.blocks);
-    const int rows = rows_of(p.lengths, pair / p.heads, p.rows);
-    const int left = rows - block * kBlock;
+    const int left = rows_of(p.lengths, pair / p.heads, p.rows) - block * kBlock;
     const unsigned char *in = p.tiles + at * kBlockBytes;
     const unsigned exps = *reinterpret_cast<const unsigned *>(in + kKeyExpsAt + ((g >> 1) * 16 + i16) * 4);
-    float lo[16], hi[16];
+    unsigned lo[8], hi[8];  // dims 2 i, 2 i + 1
 #pragma unroll
-    for (int i = 0; i < 16; ++i) lo[i] = INFINITY, hi[i] = -INFINITY;
+    for (int i = 0; i < 8; ++i) lo[i] = 0x7c007c00u, hi[i] = 0xfc00fc00u;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
         const u32x4 w = *reinterpret_cast<const u32x4 *>(in + s * 1024 + lane * 16);
@@ -223,30 +292,33 @@ __global__ __launch_bounds__(256) void icl4_bounds_kernel(StoreArgs p) {
         for (int b = 0; b < 2; ++b) {
             const int r = 32 * s + 16 * (i16 >> 3) + 8 * b + (i16 & 7);
             const float scale = __uint_as_float(((exps >> (8 * (2 * s + b))) & 0xffu) << 23);
-            if (r < left) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float x = value_of((w[2 * b + (i >> 3)] >> (4 * (i & 7))) & 15u, scale);
-                    lo[i] = fminf(lo[i], x), hi[i] = fmaxf(hi[i], x);
-                }
+            for (int c = 0; c < 2; ++c) {
+                const u32x4 y = __builtin_bit_cast(u32x4, codes8(w[2 * b + c], scale));
+                if (r < left)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) lo[4 * c + i] = pk_least(lo[4 * c + i], y[i]), hi[4 * c + i] = pk_most(hi[4 * c + i], y[i]);
             }
         }
     }
+    // Bits 3, 2 and 1 of the lane pick the pair of dims, bit 0 the dim of the pair.
+    auto step = [&](auto lanes, int keep, bool upper) {
+        constexpr int N = decltype(lanes)::value;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-#pragma unroll
-        for (int off = 1; off < 16; off *= 2) {
-            lo[i] = fminf(lo[i], __shfl_xor(lo[i], off, 64));
-            hi[i] = fmaxf(hi[i], __shfl_xor(hi[i], off, 64));
+        for (int i = 0; i < keep; ++i) {
+            const unsigned give_lo = upper ? lo[i] : lo[i + keep], give_hi = upper ? hi[i] : hi[i + keep];
+            const unsigned own_lo = upper ? lo[i + keep] : lo[i], own_hi = upper ? hi[i + keep] : hi[i];
+            lo[i] = pk_least(own_lo, row_xor<N>(give_lo)), hi[i] = pk_most(own_hi, row_xor<N>(give_hi));
         }
-    if (i16 == 0) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float inv = 1.0f / p.scales[pair * 64 + 16 * g + i];
-            p.bounds[at * 128 + 16 * g + i] = left > 0 ? (signed char)floorf(lo[i] * inv) : (signed char)0;
-            p.bounds[at * 128 + 64 + 16 * g + i] = left > 0 ? (signed char)ceilf(hi[i] * inv) : (signed char)0;
-        }
-    }
+    };
+    step(std::integral_constant<int, 8>{}, 4, i16 & 8);
+    step(std::integral_constant<int, 4>{}, 2, i16 & 4);
+    step(std::integral_constant<int, 2>{}, 1, i16 & 2);
+    const unsigned low2 = pk_least(lo[0], row_xor<1>(lo[0])), high2 = pk_most(hi[0], row_xor<1>(hi[0]));
+    const float low = (float)__builtin_bit_cast(half2v, low2)[i16 & 1], high = (float)__builtin_bit_cast(half2v, high2)[i16 & 1];
+    const float inv = 1.0f / p.scales[pair * 64 + lane];  // of a power of two: exact
+    p.bounds[at * 128 + lane] = left > 0 ? (signed char)floorf(low * inv) : (signed char)0;
+    p.bounds[at * 128 + 64 + lane] = left > 0 ? (signed char)ceilf(high * inv) : (signed char)0;
 }
 
 struct ReadArgs {
@@ -260,35 +332,55 @@ struct ReadArgs {
     float *bounds_out;
 };
 
+// The encoder's lanes and rows, the other way.
 template <typename T>
 __global__ __launch_bounds__(256) void icl4_decode_kernel(ReadArgs p) {
-    const int tid = threadIdx.x;
+    typedef T T2 __attribute__((ext_vector_type(2)));
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, i16 = lane & 15;
     const int block = (int)(blockIdx.x % (unsigned)p.blocks), pair = (int)(blockIdx.x / (unsigned)p.blocks);
     const int e = pair / p.heads, head = pair - e * p.heads;
-    const int rows = rows_of(p.lengths, e, p.rows);
-    const long long at = (long long)pair * p.blocks + block;
+    const int left = rows_of(p.lengths, e, p.rows) - block * kBlock;
+    const long long at = (long long)pair * p.blocks + block, row0 = (long long)block * kBlock;
     const unsigned char *in = p.tiles + at * kBlockBytes;
-    const int r = tid >> 2, g = tid & 3;
-    const long long row = (long long)block * kBlock + r;
-    const int s = r >> 5, a = (r >> 4) & 1, b = (r >> 3) & 1, i8 = r & 7;
-    if (row < rows) {
-        if (p.k) {
-            const unsigned *w = reinterpret_cast<const unsigned *>(in + s * 1024 + (16 * g + 8 * a + i8) * 16 + b * 8);
-            const float scale = pow2((int)in[kKeyExpsAt + ((g >> 1) * 16 + 8 * a + i8) * 4 + 2 * s + b] - 127);
-            T *dst = static_cast<T *>(p.k) + e * p.k_est + head * p.k_head + row * p.k_row + 16 * g;
+    if (p.k) {
+        const int s = wave >> 1, b = wave & 1, r = 32 * s + 16 * (i16 >> 3) + 8 * b + (i16 & 7);
+        const u32x2 w = *reinterpret_cast<const u32x2 *>(in + s * 1024 + lane * 16 + b * 8);
+        const float scale = pow2((int)in[kKeyExpsAt + ((g >> 1) * 16 + i16) * 4 + 2 * s + b] - 127);
+        if (r < left) {
+            T *dst = static_cast<T *>(p.k) + e * p.k_est + head * p.k_head + (row0 + r) * p.k_row + 16 * g;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) dst[i] = (T)value_of((w[i >> 3] >> (4 * (i & 7))) & 15u, scale);
-        }
-        if (p.v) {
-            const int t = a, h = (r >> 2) & 1, j = r & 3;
-            T *dst = static_cast<T *>(p.v) + e * p.v_est + head * p.v_head + row * p.v_row + 16 * g;
+            for (int c = 0; c < 2; ++c) {
+                const half8 y = codes8(w[c], scale);
+                if constexpr (sizeof(T) == 2) {
+                    *reinterpret_cast<half8 *>(dst + 8 * c) = y;
+                } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const unsigned c = in[kValuesAt + s * 1024 + (16 * (2 * t + h) + i) * 16 + g * 4 + 2 * b + (j >> 1)];
-                const float scale = pow2((int)in[kValueExpsAt + i * 8 + s * 4 + g] - 127);
-                dst[i] = (T)value_of((c >> (4 * (j & 1))) & 15u, scale);
+                    for (int i = 0; i < 2; ++i)
+                        *reinterpret_cast<f32x4 *>(dst + 8 * c + 4 * i) =
+                            f32x4{(float)y[4 * i], (float)y[4 * i + 1], (float)y[4 * i + 2], (float)y[4 * i + 3]};
+                }
             }
         }
+    }
+    if (p.v) {
+        const int s = lane >> 5, t = (lane >> 4) & 1, b = (lane >> 3) & 1, r = 8 * (lane >> 3);
+        half8 y[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int i = 2 * (lane & 7) + c;
+            unsigned w = 0u;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const unsigned both = *reinterpret_cast<const unsigned *>(in + kValuesAt + s * 1024 +
+                                                                          (16 * (2 * t + h) + i) * 16 + wave * 4);
+                w |= (b ? both >> 16 : both & 0xffffu) << (16 * h);
+            }
+            y[c] = codes8(w, pow2((int)in[kValueExpsAt + i * 8 + s * 4 + wave] - 127));
+        }
+        T *dst = static_cast<T *>(p.v) + e * p.v_est + head * p.v_head + (row0 + r) * p.v_row + 16 * wave + 2 * (lane & 7);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (r + i < left) *reinterpret_cast<T2 *>(dst + i * p.v_row) = T2{(T)y[0][i], (T)y[1][i]};
     }
     if (p.bounds_out && tid < 128)
         p.bounds_out[at * 128 + tid] = (float)p.bounds[at * 128 + tid] * p.scales[pair * 64 + (tid & 63)];
