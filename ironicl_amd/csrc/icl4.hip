@@ -89,12 +89,12 @@ __device__ __forceinline__ unsigned coded8(const float *x, float scale) {
     return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], scale, 3);
 }
 
-// The smallest unit 2^x with m <= 127 * 2^x (m a held key; 2^-20 for zero).
-__device__ __forceinline__ float bound_unit(float m) {
-    if (m == 0.f) return pow2(-20);
+// The smallest x >= -20 with m <= 127 * 2^x (m a held key's size).
+__device__ __forceinline__ int unit_exponent(float m) {
+    if (m == 0.f) return -20;
     const unsigned bits = __float_as_uint(m);
     const int x = (int)(bits >> 23) - 126;  // m = f 2^x, f in [0.5, 1); f <= 127/128?
-    return pow2((bits & 0x7fffffu) <= 0x7e0000u ? x - 7 : x - 6);
+    return (bits & 0x7fffffu) <= 0x7e0000u ? x - 7 : x - 6;
 }
 
 struct StoreArgs {
@@ -107,11 +107,6 @@ struct StoreArgs {
     float *scales;
     unsigned *nonfinite;
 };
-
-__global__ __launch_bounds__(256) void icl4_units_kernel(float *scales, int count) {
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i < count) scales[i] = 9.5367431640625e-07f;  // 2^-20
-}
 
 // The value of the lane eight, or sixteen, away (lane ^ 8 and lane ^ 16).
 __device__ __forceinline__ unsigned other_eight(unsigned x) {
@@ -154,9 +149,10 @@ __device__ __forceinline__ void load16(const _Float16 *src, float *x) {
     }
 }
 
-// One workgroup per (block, pair): codes and exponents; the bounds' scales by
-// maxima of 2^x (as words, so their order does not matter). Bound by its
-// reads: every load of the block is issued first, and the codes are the
+// One workgroup per (block, pair): codes and exponents, and the exponents that
+// the block's own bounds would take (icl4_units_kernel takes the largest of a
+// pair's; by atomics into one word per dim the kernel took 97 instead of 52 us
+// at 50,000 rows). Bound by its reads: every load of the block is issued first, and the codes are the
 // conversion instructions' own. The block is put together in LDS and written in
 // whole lines: from registers, in words of several waves each, 50,000 rows took
 // 315 us. Keys: wave 2 s + b, lane (g, 8 a + i) takes
@@ -221,14 +217,11 @@ __global__ __launch_bounds__(256) void icl4_encode_kernel(StoreArgs p) {
     __syncthreads();
     if (tid < 32) {
         const unsigned m = pk_max(pk_max(peaks[0][tid], peaks[1][tid]), pk_max(peaks[2][tid], peaks[3][tid]));
-        const half2v pair2 = __builtin_bit_cast(half2v, m);
-        unsigned *unit = reinterpret_cast<unsigned *>(p.scales) + pair * 64 + 2 * tid;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const unsigned u = __float_as_uint(bound_unit((float)pair2[i]));
-            // Few blocks raise a unit: one that is seen to be as large needs no atomic.
-            if (unit[i] < u) atomicMax(unit + i, u);
-        }
+        // The block's own exponents (plus 64, as bytes), where its bounds will stand.
+        const half2v both = __builtin_bit_cast(half2v, m);
+        const int x0 = unit_exponent((float)both[0]) + 64, x1 = unit_exponent((float)both[1]) + 64;
+        reinterpret_cast<unsigned short *>(p.bounds + ((long long)pair * p.blocks + block) * 128)[tid] =
+            (unsigned short)(x0 | x1 << 8);
     }
     {
         float m[2] = {0.f, 0.f}, y[2][8];
@@ -261,6 +254,37 @@ __global__ __launch_bounds__(256) void icl4_encode_kernel(StoreArgs p) {
     to[tid] = reinterpret_cast<const u32x4 *>(out)[tid];
     if (tid < kBlockBytes / 16 - 256) to[256 + tid] = reinterpret_cast<const u32x4 *>(out)[256 + tid];
     if (bad && p.nonfinite) atomicAdd(p.nonfinite, bad);
+}
+
+// A pair's units: the largest of its blocks' exponents, 16 dims to a workgroup.
+__global__ __launch_bounds__(1024) void icl4_units_kernel(StoreArgs p) {
+    __shared__ unsigned part[16][8];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, pair = blockIdx.x >> 2, g = blockIdx.x & 3;
+    const signed char *src = p.bounds + (long long)pair * p.blocks * 128 + 16 * g;
+    unsigned m[8];  // bytes 0 and 2, then 1 and 3, of the four words
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m[i] = 0u;
+    for (int t = tid; t < p.blocks; t += 1024) {
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(src + (long long)t * 128);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            m[2 * i] = pk_max(m[2 * i], w[i] & 0xff00ffu);
+            m[2 * i + 1] = pk_max(m[2 * i + 1], w[i] >> 8 & 0xff00ffu);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) m[i] = pk_max(m[i], (unsigned)__shfl_xor((int)m[i], off, 64));
+        if (lane == 0) part[wave][i] = m[i];
+    }
+    __syncthreads();
+    if (tid >= 16) return;
+    const int i = 2 * (tid >> 2) + (tid & 1), shift = 16 * ((tid >> 1) & 1);
+    int x = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) x = max(x, (int)(part[w][i] >> shift & 0xffffu));
+    p.scales[pair * 64 + 16 * g + tid] = pow2(x - 64);
 }
 
 __device__ __forceinline__ unsigned pk_least(unsigned a, unsigned b) {
@@ -1405,13 +1429,12 @@ void icl4_encode(const Icl4Rows &a, void *cache, unsigned *nonfinite, hipStream_
     p.tiles = c.tiles, p.bounds = c.bounds, p.scales = c.scales, p.nonfinite = nonfinite;
     const long long blocks = (long long)s.pairs() * s.blocks();
     KernelTimer timer(kFamGlue, stream, 0.0, 2.0 * s.pairs() * s.rows * 64 * (a.half ? 2 : 4) + (double)icl4_bytes(s));
-    hipLaunchKernelGGL(icl4_units_kernel, dim3(ceil_div((size_t)s.pairs() * 64, 256)), dim3(256), 0, stream, c.scales,
-                       s.pairs() * 64);
-    IRX_HIP(hipGetLastError());
     if (a.half)
         hipLaunchKernelGGL(icl4_encode_kernel<_Float16>, dim3((unsigned)blocks), dim3(256), 0, stream, p);
     else
         hipLaunchKernelGGL(icl4_encode_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, stream, p);
+    IRX_HIP(hipGetLastError());
+    hipLaunchKernelGGL(icl4_units_kernel, dim3(4 * s.pairs()), dim3(1024), 0, stream, p);
     IRX_HIP(hipGetLastError());
     hipLaunchKernelGGL(icl4_bounds_kernel, dim3(ceil_div((size_t)blocks, 4)), dim3(256), 0, stream, p);
     IRX_HIP(hipGetLastError());
