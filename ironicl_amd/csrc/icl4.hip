@@ -490,89 +490,213 @@ __global__ __launch_bounds__(256) void icl4_scores_kernel(SelectArgs p) {
     }
 }
 
-// The n best of one query's scores: WAVES waves hold up to REGS * 64 scores
-// each, a contiguous share, and find the n-th largest by bisection over the
-// scores' 21 bits, counting by ballots. (REGS 0: any number of blocks, scores
-// read again for every step.)
-template <int WAVES, int REGS>
-__global__ __launch_bounds__(WAVES * 64) void icl4_pick_kernel(SelectArgs p) {
-    __shared__ int counts[2][WAVES];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+// Sums, and largest, over a wave, in every lane: quads, eights and rows of 16
+// by DPP, then the rows.
+template <class Op>
+__device__ __forceinline__ int wave_join(int x, Op op) {
+    x = op(x, (int)row_xor<1>(x));
+    x = op(x, (int)row_xor<2>(x));
+    x = op(x, (int)__builtin_amdgcn_update_dpp(0, x, 0x141, 0xf, 0xf, true));  // mirrored eights
+    x = op(x, (int)__builtin_amdgcn_update_dpp(0, x, 0x140, 0xf, 0xf, true));  // mirrored rows
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = op((int)r[0], (int)r[1]);
+    const auto h = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return op((int)h[0], (int)h[1]);
+}
+
+// Scores b .. +3 of a query, those of blocks without an attended row replaced.
+__device__ __forceinline__ i32x4 attended_scores(const SelectArgs &p, const int *scores, int e, int rows, int b) {
+    i32x4 s = *reinterpret_cast<const i32x4 *>(scores + b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = rows > (b + i) * kBlock ? s[i] : kNoScore;
+    if (p.keep) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            // Past the last block the score is gone already.
+            const unsigned long long word = p.keep[(long long)e * p.blocks + min(b + i, p.blocks - 1)];
+            s[i] = word << max(0, kBlock - (rows - (b + i) * kBlock)) ? s[i] : kNoScore;
+        }
+    }
+    return s;
+}
+
+// The n best of one query's scores, for up to 1,024 blocks one wave with every
+// score in a register: bisection between the least and the largest for a value
+// that exactly n scores reach, or else the n-th largest. (Lane l holds blocks
+// 256 i + 4 l + j.)
+constexpr int kWavePicks = 1024;
+__global__ __launch_bounds__(64) void icl4_pick_wave_kernel(SelectArgs p) {
+    const int lane = threadIdx.x;
     const int at = (int)(blockIdx.x / (unsigned)p.rows_here);
     const int pair = p.pair0 + at, row = p.row0 + (int)(blockIdx.x - (unsigned)at * p.rows_here);
     const int e = pair / p.heads;
-    const int rows = rows_of(p.lengths, e, p.rows);
-    const int *scores = p.scores + (long long)blockIdx.x * p.padded;
+    const int rows = rows_of(p.lengths, e, p.rows), padded = (int)p.padded;
+    const int *scores = p.scores + (long long)blockIdx.x * padded;
     int *out = p.out + ((long long)pair * p.q_rows + row) * p.n;
-    const int share = (int)(p.padded / 64 + WAVES - 1) / WAVES;  // 64-block steps of a wave
-    const int first = wave * share * 64;
-    auto score = [&](int i) {
-        const int b = first + 64 * i + lane;
-        return i < share && b < p.blocks && block_mask(p.keep, e, p.blocks, b, rows) ? scores[b] : kNoScore;
-    };
-    int held[REGS > 0 ? REGS : 1];
-    if constexpr (REGS > 0) {
+    i32x4 held[kWavePicks / 256];
+    int least = 1 << 30, most = kNoScore, total = 0;
 #pragma unroll
-        for (int i = 0; i < REGS; ++i) held[i] = score(i);
-    }
-    auto each = [&](auto &&fn) {
-        if constexpr (REGS > 0) {
+    for (int i = 0; i < kWavePicks / 256; ++i) {
+        const int b = 256 * i + 4 * lane;
+        held[i] = b < padded ? attended_scores(p, scores, e, rows, b) : i32x4{kNoScore, kNoScore, kNoScore, kNoScore};
 #pragma unroll
-            for (int i = 0; i < REGS; ++i)
-                if (i < share) fn(held[i], i);
-        } else {
-            for (int i = 0; i < share; ++i) fn(score(i), i);
+        for (int j = 0; j < 4; ++j) {
+            most = max(most, held[i][j]);
+            least = held[i][j] == kNoScore ? least : min(least, held[i][j]);
+            total += held[i][j] != kNoScore;
         }
-    };
-    int phase = 0;
-    // Scores of the query that are at least v.
-    auto reach = [&](int v) {
+    }
+    const auto add = [](int a, int b) { return a + b; };
+    total = __builtin_amdgcn_readfirstlane(wave_join(total, add));
+    least = __builtin_amdgcn_readfirstlane(wave_join(least, [](int a, int b) { return min(a, b); }));
+    most = __builtin_amdgcn_readfirstlane(wave_join(most, [](int a, int b) { return max(a, b); }));
+    // More than n scores reach lo, fewer lo + gap.
+    int lo = least, gap = most + 1 - least;
+    bool exact = total <= p.n;
+    if (exact) lo = kNoScore;  // every candidate lies above
+    while (!exact && gap > 1) {
+        const int cut = lo + (gap >> 1);
         int c = 0;
-        each([&](int s, int) { c += __popcll(__ballot(s >= v)); });
-        if constexpr (WAVES == 1) return c;
-        if (lane == 0) counts[phase][wave] = c;
-        __syncthreads();
-        int total = 0;
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) total += counts[phase][w];
-        phase ^= 1;  // the next count's writes pass this one's reads
-        return total;
-    };
-    const int total = reach(kNoScore + 1);
-    int lo = -(1 << 20), hi = 1 << 20;  // reach(lo) >= n > reach(hi), where there are more than n
-    if (total > p.n) {
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (reach(mid) >= p.n)
-                lo = mid;
-            else
-                hi = mid;
-        }
-    }
-    // Blocks above lo, and the first of those at lo that there is room for, in order.
-    int above = 0, equal = 0;
-    each([&](int s, int) { above += __popcll(__ballot(s > lo)), equal += __popcll(__ballot(s == lo)); });
-    int before_above = 0, before_equal = 0, all_above = above;
-    if constexpr (WAVES > 1) {
-        __syncthreads();
-        if (lane == 0) counts[0][wave] = above, counts[1][wave] = equal;
-        __syncthreads();
-        all_above = 0;
+        for (int i = 0; i < kWavePicks / 256; ++i)
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
-            if (w < wave) before_above += counts[0][w], before_equal += counts[1][w];
-            all_above += counts[0][w];
-        }
+            for (int j = 0; j < 4; ++j) c += held[i][j] >= cut;
+        c = __builtin_amdgcn_readfirstlane(wave_join(c, add));
+        exact = c == p.n;
+        if (exact)
+            lo = cut - 1;  // the scores above are the n best
+        else if (c > p.n)
+            gap -= cut - lo, lo = cut;
+        else
+            gap = cut - lo;
     }
-    const int room = p.n - all_above;
+    // Scores above lo, and where no value parts n of them the first at it that there is room for. A lane's place
+    // among the lanes before it by a prefix sum of (above, equal), 10 bits each and more.
+    int all = 0;
+#pragma unroll
+    for (int i = 0; i < kWavePicks / 256; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) all += held[i][j] > lo;
+    const int room = exact ? 0 : p.n - __builtin_amdgcn_readfirstlane(wave_join(all, add));
     const unsigned long long below = (1ull << lane) - 1;
-    each([&](int s, int i) {
+    int before_above = 0, before_equal = 0;
+#pragma unroll
+    for (int i = 0; i < kWavePicks / 256; ++i) {
+        if (256 * i >= padded) break;
+        unsigned long long va[4], ve[4];
+        int a = before_above, q = before_equal;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            va[j] = __ballot(held[i][j] > lo), ve[j] = room > 0 ? __ballot(held[i][j] == lo) : 0ull;
+            a += __popcll(va[j] & below), q += __popcll(ve[j] & below);
+            before_above += __popcll(va[j]), before_equal += __popcll(ve[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const bool above = held[i][j] > lo, equal = room > 0 && held[i][j] == lo;
+            if (above || (equal && q < room)) out[a + min(q, room)] = 256 * i + 4 * lane + j;
+            a += above, q += equal;
+        }
+    }
+    for (int i = min(total, p.n) + lane; i < p.n; i += 64) out[i] = -1;
+}
+
+// The same for more blocks: sixteen waves, cuts at quarters (a barrier costs
+// more than three counts), scores staged in LDS (STAGED) or, where there are more
+// than fit, kept where they are.
+constexpr int kStagedPicks = 14336;
+template <bool STAGED>
+__global__ __launch_bounds__(1024) void icl4_pick_kernel(SelectArgs p) {
+    constexpr int CUTS = 3, WAVES = 16;
+    extern __shared__ __attribute__((aligned(16))) int staged[];
+    __shared__ int counts[3][4];
+    __shared__ int sides[2][WAVES];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int at = (int)(blockIdx.x / (unsigned)p.rows_here);
+    const int pair = p.pair0 + at, row = p.row0 + (int)(blockIdx.x - (unsigned)at * p.rows_here);
+    const int e = pair / p.heads;
+    const int rows = rows_of(p.lengths, e, p.rows), padded = (int)p.padded;
+    int *scores = p.scores + (long long)blockIdx.x * padded;
+    int *held = STAGED ? staged : scores;
+    int *out = p.out + ((long long)pair * p.q_rows + row) * p.n;
+    if (tid < 12) counts[tid >> 2][tid & 3] = 0;
+    int total = 0;
+    for (int b = 4 * tid; b < padded; b += 4 * WAVES * 64) {
+        const i32x4 s = attended_scores(p, scores, e, rows, b);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) total += s[j] != kNoScore;
+        *reinterpret_cast<i32x4 *>(held + b) = s;
+    }
+    const auto add = [](int a, int b) { return a + b; };
+    // Counts summed over the workgroup, cut i in lane i. A step's stand in one of three rows in turn, cleared after
+    // the barrier of the step before the last.
+    int phase = 0;
+    auto sum = [&](const int (&c)[CUTS]) {
+        int mine = 0;
+#pragma unroll
+        for (int i = 0; i < CUTS; ++i) {
+            const int x = wave_join(c[i], add);
+            mine = lane == i ? x : mine;
+        }
+        if (lane < CUTS) atomicAdd(&counts[phase][lane], mine);
+        __syncthreads();
+        mine = counts[phase][lane & 3];
+        phase = phase == 2 ? 0 : phase + 1;
+        if (tid < 4) counts[phase == 2 ? 0 : phase + 1][tid] = 0;
+        return mine;
+    };
+    __syncthreads();
+    {
+        const int c[CUTS] = {total, 0, 0};
+        total = __builtin_amdgcn_readfirstlane(sum(c));
+    }
+    // More than n scores reach lo, fewer lo + gap.
+    int lo = -(1 << 20) - 1, gap = 1 << 21;
+    bool exact = total <= p.n;  // every candidate lies above lo
+    while (!exact && gap > 1) {
+        const int step = (gap + CUTS) / (CUTS + 1);
+        int c[CUTS] = {};
+        for (int b = 4 * tid; b < padded; b += 4 * WAVES * 64) {
+            const i32x4 s = *reinterpret_cast<const i32x4 *>(held + b);
+#pragma unroll
+            for (int i = 0; i < CUTS; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) c[i] += s[j] >= lo + (i + 1) * step;
+        }
+        const int got = sum(c);
+        const unsigned cuts = (1u << CUTS) - 1u;
+        const unsigned reached = (unsigned)__ballot(got >= p.n) & cuts, hit = (unsigned)__ballot(got == p.n) & cuts;
+        if (hit) {
+            lo += (__builtin_ctz(hit) + 1) * step - 1;  // the scores above this are the n best
+            exact = true;
+        } else {
+            lo += __builtin_popcount(reached) * step;
+            gap = step;
+        }
+    }
+    // Each wave a contiguous share, in order.
+    const int share = (padded / 64 + WAVES - 1) / WAVES * 64;
+    const int first = wave * share, end = min(padded, first + share);
+    int above = 0, equal = 0;
+    for (int b = first + lane; b < end; b += 64) above += held[b] > lo, equal += held[b] == lo;
+    above = wave_join(above, add), equal = wave_join(equal, add);
+    if (lane == 0) sides[0][wave] = above, sides[1][wave] = equal;
+    __syncthreads();
+    int before_above = 0, before_equal = 0, all = 0;
+    for (int w = 0; w < WAVES; ++w) {
+        if (w < wave) before_above += sides[0][w], before_equal += sides[1][w];
+        all += sides[0][w];
+    }
+    const int room = exact ? 0 : p.n - all;
+    const unsigned long long below = (1ull << lane) - 1;
+    for (int b = first + lane; b < end; b += 64) {
+        const int s = held[b];
         const unsigned long long va = __ballot(s > lo), ve = __ballot(s == lo);
         const int a = before_above + __popcll(va & below), q = before_equal + __popcll(ve & below);
-        if (s > lo || (s == lo && q < room)) out[a + min(q, room)] = first + 64 * i + lane;
+        if (s > lo || (s == lo && q < room)) out[a + min(q, room)] = b;
         before_above += __popcll(va), before_equal += __popcll(ve);
-    });
-    for (int i = min(total, p.n) + (int)threadIdx.x; i < p.n; i += WAVES * 64) out[i] = -1;
+    }
+    for (int i = min(total, p.n) + tid; i < p.n; i += WAVES * 64) out[i] = -1;
 }
 
 // ---- attention ----
@@ -1484,16 +1608,12 @@ void icl4_select(const Icl4Queries &a, int n, int *out, void *workspace, hipStre
             else
                 hipLaunchKernelGGL(icl4_scores_kernel<float>, grid, dim3(256), 0, stream, p);
             IRX_HIP(hipGetLastError());
-            if (p.blocks <= 512)
-                hipLaunchKernelGGL((icl4_pick_kernel<1, 8>), rows, dim3(64), 0, stream, p);
-            else if (p.blocks <= 1024)
-                hipLaunchKernelGGL((icl4_pick_kernel<1, 16>), rows, dim3(64), 0, stream, p);
-            else if (p.blocks <= 4096)
-                hipLaunchKernelGGL((icl4_pick_kernel<4, 16>), rows, dim3(256), 0, stream, p);
-            else if (p.blocks <= 16384)
-                hipLaunchKernelGGL((icl4_pick_kernel<16, 16>), rows, dim3(1024), 0, stream, p);
+            if (p.blocks <= kWavePicks)
+                hipLaunchKernelGGL(icl4_pick_wave_kernel, rows, dim3(64), 0, stream, p);
+            else if (p.blocks <= kStagedPicks)
+                hipLaunchKernelGGL(icl4_pick_kernel<true>, rows, dim3(1024), (unsigned)p.padded * sizeof(int), stream, p);
             else
-                hipLaunchKernelGGL((icl4_pick_kernel<16, 0>), rows, dim3(1024), 0, stream, p);
+                hipLaunchKernelGGL(icl4_pick_kernel<false>, rows, dim3(1024), 0, stream, p);
             IRX_HIP(hipGetLastError());
         }
 }

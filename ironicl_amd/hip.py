@@ -129,17 +129,18 @@ SIGNATURES = {
     "irx_test_icl_attention": (ctypes.c_int, [ctypes.c_void_p, _CF, _CF, _CF, _sz, _sz, _sz, _F]),
     "irx_icl_attention_noalloc": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                                  _sz, _sz, _sz, ctypes.c_void_p, ctypes.c_void_p]),
-    "irx_icl4_bytes": (_sz, [ctypes.POINTER(Icl4Shape)]),
-    "irx_icl4_workspace_bytes": (_sz, [ctypes.c_void_p, ctypes.POINTER(Icl4Shape), _sz, _sz]),
-    "irx_icl4_encode": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Icl4Rows), ctypes.c_void_p, ctypes.c_void_p,
+    # The icl4 calls take their structures by address or as packed bytes (icl4.py).
+    "irx_icl4_bytes": (_sz, [ctypes.c_void_p]),
+    "irx_icl4_workspace_bytes": (_sz, [ctypes.c_void_p, ctypes.c_void_p, _sz, _sz]),
+    "irx_icl4_encode": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                        ctypes.c_void_p]),
-    "irx_icl4_decode": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.POINTER(Icl4Rows), ctypes.c_void_p,
+    "irx_icl4_decode": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                        ctypes.c_void_p]),
-    "irx_icl4_select": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Icl4Queries), ctypes.c_void_p, _sz,
-                                       ctypes.c_void_p, ctypes.c_void_p, _sz, ctypes.c_void_p]),
-    "irx_icl4_attention": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(Icl4Queries), ctypes.c_void_p, ctypes.c_float,
-                                          ctypes.c_void_p, _sz, ctypes.c_void_p, ctypes.POINTER(Strides),
-                                          ctypes.c_void_p, ctypes.c_void_p, _sz, ctypes.c_void_p]),
+    "irx_icl4_select": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, _sz, ctypes.c_void_p,
+                                       ctypes.c_void_p, _sz, ctypes.c_void_p]),
+    "irx_icl4_attention": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_float,
+                                          ctypes.c_void_p, _sz, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                          ctypes.c_void_p, _sz, ctypes.c_void_p]),
     "irx_test_icl_attention_precision": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, _CF, _CF, _CF, _sz, _sz,
                                                         _sz, _F]),
     "irx_test_encode_icl8": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, _sz, _sz,

@@ -14,12 +14,19 @@ enqueue their work and return; invalid ones raise ``hip.HipError``.
 
 from __future__ import annotations
 
-import ctypes
+import functools
+import struct
 
 from . import hip
 
 ELEMENTS = {"f32": hip.ELEMENT_F32, "f16": hip.ELEMENT_F16}
 BLOCK = 64  # rows of a block
+
+# hip.Icl4Rows and hip.Icl4Queries as bytes: packing them costs a call a few
+# microseconds less than building the structures field by field.
+_ROWS = struct.Struct("@NNNiPPNNNNNNP")
+_QUERIES = struct.Struct("@NNNNiPNNNPP")
+_THREE = struct.Struct("@NNN")
 
 
 def _address(buffer):
@@ -36,31 +43,39 @@ def _element(element: str) -> int:
     return ELEMENTS[element]
 
 
-def _strides(strides, heads: int, rows: int) -> hip.Strides:
-    if strides is None:
-        return hip.Strides(heads * rows * 64, rows * 64, 64)
-    return hip.Strides(*strides)
+def _strides(strides, heads: int, rows: int):
+    return (heads * rows * 64, rows * 64, 64) if strides is None else strides
 
 
-def _rows(shape, k, v, element, k_strides, v_strides, lengths) -> hip.Icl4Rows:
-    _, heads, rows = shape
-    return hip.Icl4Rows(hip.Icl4Shape(*shape), _element(element), _address(k), _address(v),
-                        _strides(k_strides, heads, rows), _strides(v_strides, heads, rows), _address(lengths))
+def _rows(shape, k, v, element, k_strides, v_strides, lengths) -> bytes:
+    estimators, heads, rows = shape
+    return _ROWS.pack(estimators, heads, rows, _element(element), _address(k) or 0, _address(v) or 0,
+                      *_strides(k_strides, heads, rows), *_strides(v_strides, heads, rows), _address(lengths) or 0)
 
 
-def _queries(shape, q, query_rows, element, q_strides, lengths, keep) -> hip.Icl4Queries:
-    return hip.Icl4Queries(hip.Icl4Shape(*shape), query_rows, _element(element), _address(q),
-                           _strides(q_strides, shape[1], query_rows), _address(lengths), _address(keep))
+def _queries(shape, q, query_rows, element, q_strides, lengths, keep) -> bytes:
+    estimators, heads, rows = shape
+    return _QUERIES.pack(estimators, heads, rows, query_rows, _element(element), _address(q) or 0,
+                         *_strides(q_strides, heads, query_rows), _address(lengths) or 0, _address(keep) or 0)
+
+
+@functools.lru_cache(maxsize=None)
+def _call(name: str):
+    return getattr(hip.lib(), name)
+
+
+def _shape(shape) -> bytes:  # hip.Icl4Shape, or hip.Strides
+    return _THREE.pack(*shape)
 
 
 def cache_bytes(shape) -> int:
     """Bytes of a cache of `shape` (0: out of range)."""
-    return hip.lib().irx_icl4_bytes(ctypes.byref(hip.Icl4Shape(*shape)))
+    return _call("irx_icl4_bytes")(_shape(shape))
 
 
 def workspace_bytes(device: hip.Device, shape, query_rows: int, n_blocks: int = 0) -> int:
     """Bytes of workspace for `select` and `attention` of `query_rows` queries."""
-    return hip.lib().irx_icl4_workspace_bytes(device.handle, ctypes.byref(hip.Icl4Shape(*shape)), query_rows, n_blocks)
+    return _call("irx_icl4_workspace_bytes")(device.handle, _shape(shape), query_rows, n_blocks)
 
 
 def encode(device: hip.Device, shape, k, v, cache, *, element: str = "f32", k_strides=None, v_strides=None,
@@ -68,8 +83,7 @@ def encode(device: hip.Device, shape, k, v, cache, *, element: str = "f32", k_st
     """Writes `cache` (cache_bytes) from keys and values [estimators, heads, rows, 64];
     numbers that are not finite are held as 0 and added to the uint32 `nonfinite`."""
     rows = _rows(shape, k, v, element, k_strides, v_strides, lengths)
-    hip.check(hip.lib().irx_icl4_encode(device.handle, ctypes.byref(rows), _address(cache), _address(nonfinite),
-                                        _address(stream)))
+    hip.check(_call("irx_icl4_encode")(device.handle, rows, _address(cache), _address(nonfinite), _address(stream)))
 
 
 def decode(device: hip.Device, shape, cache, k=None, v=None, *, element: str = "f32", k_strides=None,
@@ -77,8 +91,7 @@ def decode(device: hip.Device, shape, cache, k=None, v=None, *, element: str = "
     """Reads what `cache` holds into k and v, and its bounds into FP32 [estimators *
     heads, blocks, 2, 64]. Rows past an estimator's length are left as they were."""
     rows = _rows(shape, k, v, element, k_strides, v_strides, lengths)
-    hip.check(hip.lib().irx_icl4_decode(device.handle, _address(cache), ctypes.byref(rows), _address(bounds),
-                                        _address(stream)))
+    hip.check(_call("irx_icl4_decode")(device.handle, _address(cache), rows, _address(bounds), _address(stream)))
 
 
 def select(device: hip.Device, shape, cache, q, query_rows: int, n_blocks: int, blocks, *, element: str = "f32",
@@ -86,8 +99,8 @@ def select(device: hip.Device, shape, cache, q, query_rows: int, n_blocks: int, 
     """The `n_blocks` best blocks of each query into int32 `blocks` [estimators,
     heads, query_rows, n_blocks], ascending, -1 where there are fewer."""
     queries = _queries(shape, q, query_rows, element, q_strides, lengths, keep)
-    hip.check(hip.lib().irx_icl4_select(device.handle, ctypes.byref(queries), _address(cache), n_blocks,
-                                        _address(blocks), _address(workspace), workspace_bytes, _address(stream)))
+    hip.check(_call("irx_icl4_select")(device.handle, queries, _address(cache), n_blocks, _address(blocks),
+                                       _address(workspace), workspace_bytes, _address(stream)))
 
 
 def attention(device: hip.Device, shape, cache, q, query_rows: int, out, *, element: str = "f32", scale: float = 0.125,
@@ -97,7 +110,7 @@ def attention(device: hip.Device, shape, cache, q, query_rows: int, out, *, elem
     given) into `out`, and the log-sum-exp into FP32 `lse` [estimators, heads,
     query_rows]; 0 and -inf where a query attends to nothing."""
     queries = _queries(shape, q, query_rows, element, q_strides, lengths, keep)
-    strides = _strides(out_strides, shape[1], query_rows)
-    hip.check(hip.lib().irx_icl4_attention(device.handle, ctypes.byref(queries), _address(cache), scale,
-                                           _address(blocks), n_blocks, _address(out), ctypes.byref(strides),
-                                           _address(lse), _address(workspace), workspace_bytes, _address(stream)))
+    strides = _shape(_strides(out_strides, shape[1], query_rows))
+    hip.check(_call("irx_icl4_attention")(device.handle, queries, _address(cache), scale, _address(blocks), n_blocks,
+                                          _address(out), strides, _address(lse), _address(workspace), workspace_bytes,
+                                          _address(stream)))
