@@ -36,9 +36,6 @@ constexpr int kBlock = kIcl4Block;            // rows of a block
 constexpr int kBlockBytes = kIcl4BlockBytes;  // bytes of one pair's block
 constexpr int kValuesAt = 2048, kKeyExpsAt = 4096, kValueExpsAt = 4224;
 
-__device__ __forceinline__ float to_float(float x) { return x; }
-__device__ __forceinline__ float to_float(_Float16 x) { return (float)x; }
-
 // 2^(byte - 127) of byte `i` of a word.
 template <int I>
 __device__ __forceinline__ float exp_byte(unsigned word) {
@@ -431,9 +428,63 @@ struct SelectArgs {
 constexpr int kNoScore = -(1 << 30);
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-// Scores of 16 queries against `chunk` blocks per wave: per 16 blocks and
-// sign one 16x16x64 product of whole numbers, [blocks, 64] lower bounds by the
-// negative parts of the queries' codes, upper bounds by the positive ones.
+// A query's codes as operands: lane (g, i16) dims 16 g .. of query i16,
+// positive and negative parts as bytes.
+struct QueryCodes {
+    i32x4 pos, neg;
+};
+template <typename T>
+__device__ __forceinline__ QueryCodes query_codes(const SelectArgs &p, int pair, int row, int g) {
+    const int e = pair / p.heads, head = pair - e * p.heads;
+    const T *src = static_cast<const T *>(p.q) + e * p.q_est + head * p.q_head + row * p.q_row + 16 * g;
+    float x[16];
+    load16(src, x);
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        x[i] *= p.scales[pair * 64 + 16 * g + i];
+        m = fmaxf(m, fabsf(x[i]));
+    }
+    m = fmaxf(m, __shfl_xor(m, 16, 64));
+    m = fmaxf(m, __shfl_xor(m, 32, 64));
+    int f = -100;
+    if (m > 0.f) {
+        const unsigned bits = __float_as_uint(m);
+        const int ex = (int)(bits >> 23) - 126;
+        f = min(120, max(-100, (bits & 0x7fffffu) <= 0x7e0000u ? ex - 7 : ex - 6));
+    }
+    const float inv = pow2(-f);
+    QueryCodes c;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        unsigned a = 0u, b = 0u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int v = (int)rintf(fminf(fmaxf(x[4 * w + i] * inv, -127.f), 127.f));
+            a |= (unsigned)max(v, 0) << (8 * i);
+            b |= ((unsigned)min(v, 0) & 0xffu) << (8 * i);
+        }
+        c.pos[w] = (int)a, c.neg[w] = (int)b;
+    }
+    return c;
+}
+
+// The bounds of blocks b .. +15 as operands (`bounds`: the pair's, at dims 16
+// g); past the last block it stands in.
+__device__ __forceinline__ void load_bounds(const signed char *bounds, int b, int blocks, int i16, i32x4 &low, i32x4 &high) {
+    const signed char *src = bounds + (long long)min(b + i16, blocks - 1) * 128;
+    low = *reinterpret_cast<const i32x4 *>(src), high = *reinterpret_cast<const i32x4 *>(src + 64);
+}
+// Scores of 16 queries against them: per sign one 16x16x64 product of whole
+// numbers, lower bounds by the codes' negative parts, upper bounds by the
+// positive ones. Register r: block b + 4 g + r of query i16.
+__device__ __forceinline__ i32x4 block_scores(const i32x4 &low, const i32x4 &high, const QueryCodes &c) {
+    i32x4 s = {0, 0, 0, 0};
+    s = __builtin_amdgcn_mfma_i32_16x16x64_i8(low, c.neg, s, 0, 0, 0);
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(high, c.pos, s, 0, 0, 0);
+}
+
+// Scores of 16 queries against `chunk` blocks per wave.
 template <typename T>
 __global__ __launch_bounds__(256) void icl4_scores_kernel(SelectArgs p) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, i16 = lane & 15;
@@ -443,49 +494,16 @@ __global__ __launch_bounds__(256) void icl4_scores_kernel(SelectArgs p) {
     const int qt = (int)(id % (unsigned)p.qtiles), pair = p.pair0 + (int)(id / (unsigned)p.qtiles);
     const int b0 = (part * 4 + wave) * p.chunk;
     if (b0 >= p.blocks) return;
-    const int e = pair / p.heads, head = pair - e * p.heads;
-    const int here = 16 * qt + i16, row = p.row0 + min(here, p.rows_here - 1);
-    i32x4 pos, neg;
-    {
-        const T *src = static_cast<const T *>(p.q) + e * p.q_est + head * p.q_head + row * p.q_row + 16 * g;
-        float x[16];
-        float m = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            x[i] = to_float(src[i]) * p.scales[pair * 64 + 16 * g + i];
-            m = fmaxf(m, fabsf(x[i]));
-        }
-        m = fmaxf(m, __shfl_xor(m, 16, 64));
-        m = fmaxf(m, __shfl_xor(m, 32, 64));
-        int f = -100;
-        if (m > 0.f) {
-            const unsigned bits = __float_as_uint(m);
-            const int ex = (int)(bits >> 23) - 126;
-            f = min(120, max(-100, (bits & 0x7fffffu) <= 0x7e0000u ? ex - 7 : ex - 6));
-        }
-        const float inv = pow2(-f);
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            unsigned a = 0u, b = 0u;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int c = (int)rintf(fminf(fmaxf(x[4 * w + i] * inv, -127.f), 127.f));
-                a |= (unsigned)max(c, 0) << (8 * i);
-                b |= ((unsigned)min(c, 0) & 0xffu) << (8 * i);
-            }
-            pos[w] = (int)a, neg[w] = (int)b;
-        }
-    }
+    const int here = 16 * qt + i16;
+    const QueryCodes c = query_codes<T>(p, pair, p.row0 + min(here, p.rows_here - 1), g);
     const signed char *bounds = p.bounds + (long long)pair * p.blocks * 128 + 16 * g;
     int *out = p.scores + ((long long)(pair - p.pair0) * p.rows_here + here) * p.padded + 4 * g;
     const int end = min(p.blocks, b0 + p.chunk);
     for (int b = b0; b < end; b += 16) {
-        const signed char *src = bounds + (long long)min(b + i16, p.blocks - 1) * 128;
-        const i32x4 low = *reinterpret_cast<const i32x4 *>(src), high = *reinterpret_cast<const i32x4 *>(src + 64);
-        i32x4 s = {0, 0, 0, 0};
-        s = __builtin_amdgcn_mfma_i32_16x16x64_i8(low, neg, s, 0, 0, 0);
-        s = __builtin_amdgcn_mfma_i32_16x16x64_i8(high, pos, s, 0, 0, 0);
-        // Register r: block b + 4 g + r of query i16; blocks past the last lie in the row's padding.
+        i32x4 low, high;
+        load_bounds(bounds, b, p.blocks, i16, low, high);
+        const i32x4 s = block_scores(low, high, c);
+        // Blocks past the last lie in the row's padding.
         if (here < p.rows_here) *reinterpret_cast<i32x4 *>(out + b) = s;
     }
 }
@@ -520,23 +538,17 @@ __device__ __forceinline__ i32x4 attended_scores(const SelectArgs &p, const int 
     return s;
 }
 
-// The n best of one query's scores, for up to 1,024 blocks one wave with every
-// score in a register: bisection between the least and the largest for a value
-// that exactly n scores reach, or else the n-th largest. (Lane l holds blocks
-// 256 i + 4 l + j.)
-constexpr int kWavePicks = 1024;
-__global__ __launch_bounds__(64) void icl4_pick_wave_kernel(SelectArgs p) {
-    const int lane = threadIdx.x;
-    const int at = (int)(blockIdx.x / (unsigned)p.rows_here);
-    const int pair = p.pair0 + at, row = p.row0 + (int)(blockIdx.x - (unsigned)at * p.rows_here);
-    const int e = pair / p.heads;
-    const int rows = rows_of(p.lengths, e, p.rows), padded = (int)p.padded;
-    const int *scores = p.scores + (long long)blockIdx.x * padded;
-    int *out = p.out + ((long long)pair * p.q_rows + row) * p.n;
-    i32x4 held[kWavePicks / 256];
+// The n best of one query's scores by one wave with every score in a register
+// (up to 1,024): bisection between the least and the largest for a value
+// that exactly n scores reach, or else the n-th largest. Lane l holds blocks
+// 256 i + 4 l + j.
+constexpr int kWavePicks = 960;  // sixteen queries' scores in 64 KB of LDS
+__device__ __forceinline__ void pick_by_wave(const SelectArgs &p, const int *scores, int e, int rows, int *out) {
+    const int lane = threadIdx.x & 63, padded = (int)p.padded;
+    i32x4 held[4];
     int least = 1 << 30, most = kNoScore, total = 0;
 #pragma unroll
-    for (int i = 0; i < kWavePicks / 256; ++i) {
+    for (int i = 0; i < 4; ++i) {
         const int b = 256 * i + 4 * lane;
         held[i] = b < padded ? attended_scores(p, scores, e, rows, b) : i32x4{kNoScore, kNoScore, kNoScore, kNoScore};
 #pragma unroll
@@ -558,7 +570,7 @@ __global__ __launch_bounds__(64) void icl4_pick_wave_kernel(SelectArgs p) {
         const int cut = lo + (gap >> 1);
         int c = 0;
 #pragma unroll
-        for (int i = 0; i < kWavePicks / 256; ++i)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) c += held[i][j] >= cut;
         c = __builtin_amdgcn_readfirstlane(wave_join(c, add));
@@ -570,26 +582,24 @@ __global__ __launch_bounds__(64) void icl4_pick_wave_kernel(SelectArgs p) {
         else
             gap = cut - lo;
     }
-    // Scores above lo, and where no value parts n of them the first at it that there is room for. A lane's place
-    // among the lanes before it by a prefix sum of (above, equal), 10 bits each and more.
+    // Scores above lo and, where no value parts n of them, the first at it that there is room for, in order.
     int all = 0;
 #pragma unroll
-    for (int i = 0; i < kWavePicks / 256; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) all += held[i][j] > lo;
     const int room = exact ? 0 : p.n - __builtin_amdgcn_readfirstlane(wave_join(all, add));
     const unsigned long long below = (1ull << lane) - 1;
     int before_above = 0, before_equal = 0;
 #pragma unroll
-    for (int i = 0; i < kWavePicks / 256; ++i) {
+    for (int i = 0; i < 4; ++i) {
         if (256 * i >= padded) break;
-        unsigned long long va[4], ve[4];
         int a = before_above, q = before_equal;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            va[j] = __ballot(held[i][j] > lo), ve[j] = room > 0 ? __ballot(held[i][j] == lo) : 0ull;
-            a += __popcll(va[j] & below), q += __popcll(ve[j] & below);
-            before_above += __popcll(va[j]), before_equal += __popcll(ve[j]);
+            const unsigned long long va = __ballot(held[i][j] > lo), ve = room > 0 ? __ballot(held[i][j] == lo) : 0ull;
+            a += __popcll(va & below), q += __popcll(ve & below);
+            before_above += __popcll(va), before_equal += __popcll(ve);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -601,102 +611,166 @@ __global__ __launch_bounds__(64) void icl4_pick_wave_kernel(SelectArgs p) {
     for (int i = min(total, p.n) + lane; i < p.n; i += 64) out[i] = -1;
 }
 
-// The same for more blocks: sixteen waves, cuts at quarters (a barrier costs
-// more than three counts), scores staged in LDS (STAGED) or, where there are more
-// than fit, kept where they are.
-constexpr int kStagedPicks = 14336;
+// Sum over the lanes up to this one.
+__device__ __forceinline__ int wave_prefix(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // one lane up in each row of 16
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row 0's last to row 1, 2's to 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row 1's last to rows 2 and 3
+    return x;
+}
+
+// The n best of one query's scores by a workgroup, for any number of blocks:
+// the n-th largest by a histogram of 1,024 steps of 2^sh over the scores'
+// range, then over the step that holds it, until a step ends at exactly n or is
+// one value wide (two rounds as a rule). Bisection by the sixteen waves took
+// 1,550 cycles a step and 11 steps for 3,125 scores. Scores stand in `held`, LDS
+// (STAGED) or where they are.
+constexpr int kPickWaves = 8;
+constexpr int kStagedPicks = 12288;  // scores that fit a workgroup's LDS beside the histogram
 template <bool STAGED>
-__global__ __launch_bounds__(1024) void icl4_pick_kernel(SelectArgs p) {
-    constexpr int CUTS = 3, WAVES = 16;
+__global__ __launch_bounds__(kPickWaves * 64) void icl4_pick_kernel(SelectArgs p) {
+    constexpr int THREADS = kPickWaves * 64, BINS = 2 * THREADS;
     extern __shared__ __attribute__((aligned(16))) int staged[];
-    __shared__ int counts[3][4];
-    __shared__ int sides[2][WAVES];
+    __shared__ int bins[BINS];  // from the highest down
+    __shared__ int joint[3][kPickWaves];
+    __shared__ int found[3];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int at = (int)(blockIdx.x / (unsigned)p.rows_here);
     const int pair = p.pair0 + at, row = p.row0 + (int)(blockIdx.x - (unsigned)at * p.rows_here);
-    const int e = pair / p.heads;
-    const int rows = rows_of(p.lengths, e, p.rows), padded = (int)p.padded;
-    int *scores = p.scores + (long long)blockIdx.x * padded;
+    const int e = pair / p.heads, rows = rows_of(p.lengths, e, p.rows), padded = (int)p.padded;
+    int *scores = p.scores + (long long)blockIdx.x * p.padded;
     int *held = STAGED ? staged : scores;
     int *out = p.out + ((long long)pair * p.q_rows + row) * p.n;
-    if (tid < 12) counts[tid >> 2][tid & 3] = 0;
-    int total = 0;
-    for (int b = 4 * tid; b < padded; b += 4 * WAVES * 64) {
+    int total = 0, least = 1 << 30, most = kNoScore;
+    for (int b = 4 * tid; b < padded; b += 4 * THREADS) {
         const i32x4 s = attended_scores(p, scores, e, rows, b);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) total += s[j] != kNoScore;
+        for (int j = 0; j < 4; ++j) {
+            total += s[j] != kNoScore;
+            most = max(most, s[j]);
+            least = s[j] == kNoScore ? least : min(least, s[j]);
+        }
         *reinterpret_cast<i32x4 *>(held + b) = s;
     }
     const auto add = [](int a, int b) { return a + b; };
-    // Counts summed over the workgroup, cut i in lane i. A step's stand in one of three rows in turn, cleared after
-    // the barrier of the step before the last.
-    int phase = 0;
-    auto sum = [&](const int (&c)[CUTS]) {
-        int mine = 0;
-#pragma unroll
-        for (int i = 0; i < CUTS; ++i) {
-            const int x = wave_join(c[i], add);
-            mine = lane == i ? x : mine;
-        }
-        if (lane < CUTS) atomicAdd(&counts[phase][lane], mine);
-        __syncthreads();
-        mine = counts[phase][lane & 3];
-        phase = phase == 2 ? 0 : phase + 1;
-        if (tid < 4) counts[phase == 2 ? 0 : phase + 1][tid] = 0;
-        return mine;
-    };
+    total = wave_join(total, add);
+    least = wave_join(least, [](int a, int b) { return min(a, b); });
+    most = wave_join(most, [](int a, int b) { return max(a, b); });
+    if (lane == 0) joint[0][wave] = total, joint[1][wave] = least, joint[2][wave] = most;
     __syncthreads();
-    {
-        const int c[CUTS] = {total, 0, 0};
-        total = __builtin_amdgcn_readfirstlane(sum(c));
-    }
-    // More than n scores reach lo, fewer lo + gap.
-    int lo = -(1 << 20) - 1, gap = 1 << 21;
-    bool exact = total <= p.n;  // every candidate lies above lo
-    while (!exact && gap > 1) {
-        const int step = (gap + CUTS) / (CUTS + 1);
-        int c[CUTS] = {};
-        for (int b = 4 * tid; b < padded; b += 4 * WAVES * 64) {
-            const i32x4 s = *reinterpret_cast<const i32x4 *>(held + b);
+    total = 0;
 #pragma unroll
-            for (int i = 0; i < CUTS; ++i)
+    for (int w = 0; w < kPickWaves; ++w)
+        total += joint[0][w], least = min(least, joint[1][w]), most = max(most, joint[2][w]);
+    int lo = kNoScore, room = 0;  // chosen: the scores above lo and `room` of those at it
+    if (total > p.n) {
+        int base = __builtin_amdgcn_readfirstlane(least), sh = 0, above = 0, limit = BINS;
+        const int range = __builtin_amdgcn_readfirstlane(most) - base;
+        while (range >> sh >= BINS) ++sh;
+        for (;;) {
+            bins[tid] = 0, bins[tid + THREADS] = 0;
+            __syncthreads();
+            for (int b = 4 * tid; b < padded; b += 4 * THREADS) {
+                const i32x4 s = *reinterpret_cast<const i32x4 *>(held + b);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) c[i] += s[j] >= lo + (i + 1) * step;
-        }
-        const int got = sum(c);
-        const unsigned cuts = (1u << CUTS) - 1u;
-        const unsigned reached = (unsigned)__ballot(got >= p.n) & cuts, hit = (unsigned)__ballot(got == p.n) & cuts;
-        if (hit) {
-            lo += (__builtin_ctz(hit) + 1) * step - 1;  // the scores above this are the n best
-            exact = true;
-        } else {
-            lo += __builtin_popcount(reached) * step;
-            gap = step;
+                for (int j = 0; j < 4; ++j) {
+                    const unsigned bin = (unsigned)(s[j] - base) >> sh;
+                    if (bin < (unsigned)limit) atomicAdd(&bins[BINS - 1 - bin], 1);
+                }
+            }
+            __syncthreads();
+            const int c0 = bins[2 * tid], c1 = bins[2 * tid + 1];
+            int upto = wave_prefix(c0 + c1);
+            if (lane == 63) joint[0][wave] = upto;
+            __syncthreads();
+            upto += above;
+#pragma unroll
+            for (int w = 0; w < kPickWaves; ++w) upto += w < wave ? joint[0][w] : 0;
+            // The step where the count from the top reaches n: its thread tells the others.
+            const int to0 = upto - c1, before = to0 - c0;
+            if (before < p.n && upto >= p.n) {
+                const bool first = to0 >= p.n;
+                found[0] = BINS - 1 - (2 * tid + (first ? 0 : 1));
+                found[1] = first ? before : to0;
+                found[2] = first ? to0 : upto;
+            }
+            __syncthreads();
+            const int bin = found[0];
+            above = found[1];
+            lo = base + (bin << sh);
+            if (found[2] == p.n) {
+                --lo;  // the whole step is chosen
+                break;
+            }
+            if (sh == 0) {
+                room = p.n - above;
+                break;
+            }
+            // The step's 2^sh values alone: what lies above it is counted already.
+            static_assert(BINS == 1024, "a step's values fit the next histogram");
+            base = lo;
+            limit = 1 << min(sh, 10);
+            sh = max(0, sh - 10);
         }
     }
-    // Each wave a contiguous share, in order.
-    const int share = (padded / 64 + WAVES - 1) / WAVES * 64;
+    // In order: each wave a contiguous share.
+    const int share = (padded / 64 + kPickWaves - 1) / kPickWaves * 64;
     const int first = wave * share, end = min(padded, first + share);
-    int above = 0, equal = 0;
-    for (int b = first + lane; b < end; b += 64) above += held[b] > lo, equal += held[b] == lo;
-    above = wave_join(above, add), equal = wave_join(equal, add);
-    if (lane == 0) sides[0][wave] = above, sides[1][wave] = equal;
+    int more = 0, equal = 0;
+    for (int b = first + lane; b < end; b += 64) more += held[b] > lo, equal += held[b] == lo;
+    more = wave_join(more, add), equal = wave_join(equal, add);
+    if (lane == 0) joint[1][wave] = more, joint[2][wave] = equal;
     __syncthreads();
-    int before_above = 0, before_equal = 0, all = 0;
-    for (int w = 0; w < WAVES; ++w) {
-        if (w < wave) before_above += sides[0][w], before_equal += sides[1][w];
-        all += sides[0][w];
-    }
-    const int room = exact ? 0 : p.n - all;
+    int before_more = 0, before_equal = 0;
+#pragma unroll
+    for (int w = 0; w < kPickWaves; ++w)
+        before_more += w < wave ? joint[1][w] : 0, before_equal += w < wave ? joint[2][w] : 0;
     const unsigned long long below = (1ull << lane) - 1;
     for (int b = first + lane; b < end; b += 64) {
         const int s = held[b];
         const unsigned long long va = __ballot(s > lo), ve = __ballot(s == lo);
-        const int a = before_above + __popcll(va & below), q = before_equal + __popcll(ve & below);
+        const int a = before_more + __popcll(va & below), q = before_equal + __popcll(ve & below);
         if (s > lo || (s == lo && q < room)) out[a + min(q, room)] = b;
-        before_above += __popcll(va), before_equal += __popcll(ve);
+        before_more += __popcll(va), before_equal += __popcll(ve);
     }
-    for (int i = min(total, p.n) + tid; i < p.n; i += WAVES * 64) out[i] = -1;
+    for (int i = min(total, p.n) + tid; i < p.n; i += THREADS) out[i] = -1;
+}
+
+// Scores and choice in one launch, no scores in memory, up to 960 blocks:
+// sixteen queries to a workgroup, scored together, then each chosen for by a
+// wave of its own.
+constexpr int kChooseWaves = 16;
+template <typename T>
+__global__ __launch_bounds__(kChooseWaves * 64) void icl4_choose_kernel(SelectArgs p) {
+    extern __shared__ __attribute__((aligned(16))) int staged[];  // [queries][padded + 4]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, i16 = lane & 15;
+    const int pair = (int)(blockIdx.x / (unsigned)p.qtiles), qt = (int)(blockIdx.x - (unsigned)pair * p.qtiles);
+    const int e = pair / p.heads, rows = rows_of(p.lengths, e, p.rows);
+    const signed char *bounds = p.bounds + (long long)pair * p.blocks * 128 + 16 * g;
+    const int stride = (int)p.padded + 4;  // four banks on from one query to the next
+    // At most four steps of sixteen blocks to a wave, all loaded at once, the queries' codes beneath them.
+    constexpr int STEPS = 4, STEP = 16 * kChooseWaves;
+    static_assert(STEPS * STEP >= kWavePicks, "every block is scored");
+    i32x4 low[STEPS], high[STEPS];
+#pragma unroll
+    for (int u = 0; u < STEPS; ++u) load_bounds(bounds, 16 * wave + u * STEP, p.blocks, i16, low[u], high[u]);
+    const QueryCodes c = query_codes<T>(p, pair, min(16 * qt + i16, p.q_rows - 1), g);
+#pragma unroll
+    for (int u = 0; u < STEPS; ++u) {
+        const int b = 16 * wave + u * STEP;
+        const i32x4 s = block_scores(low[u], high[u], c);
+        // Only queries that there are have a row.
+        if (b < p.padded && 16 * qt + i16 < p.q_rows)
+            *reinterpret_cast<i32x4 *>(staged + i16 * stride + b + 4 * g) = s;
+    }
+    __syncthreads();
+    const int mine = 16 * qt + wave;
+    if (mine < p.q_rows)
+        pick_by_wave(p, staged + wave * stride, e, rows, p.out + ((long long)pair * p.q_rows + mine) * p.n);
 }
 
 // ---- attention ----
@@ -1441,15 +1515,21 @@ Plan plan_attend(const Icl4Shape &s, int q_rows, int n_blocks, int compute_units
     return pl;
 }
 
-// Scores are made and picked from in turns of at most 64 MiB (or one query's):
-// whole pairs, or a part of one pair's queries.
-struct SelectTurns {
+// How blocks are chosen: in one launch up to 960 blocks; else scores first, then
+// choices, in turns of at most 64 MiB of scores (or one query's): whole pairs,
+// or a part of one pair's queries. (One launch with a workgroup to a query took
+// 24 us for 8 queries of 3,125 blocks, a compute unit alone being slow to read
+// 400 KB, where scores and choice apart take 4 and CHOICE.)
+struct SelectPlan {
+    bool fused;
     long long padded;
-    int pairs, rows;
+    int pairs, rows;  // of a turn
 };
-SelectTurns select_turns(const Icl4Shape &s, int q_rows) {
-    SelectTurns t{};
+SelectPlan plan_select(const Icl4Shape &s, int q_rows) {
+    SelectPlan t{};
     t.padded = (s.blocks() + 63) / 64 * 64;
+    t.fused = s.blocks() <= kWavePicks;
+    if (t.fused) return t;
     const long long most = std::max<long long>(1, (16LL << 20) / t.padded);  // queries of a turn
     t.rows = (int)std::min<long long>(q_rows, most);
     t.pairs = t.rows < q_rows ? 1 : (int)std::min<long long>(s.pairs(), std::max<long long>(1, most / q_rows));
@@ -1534,8 +1614,12 @@ size_t icl4_attend_workspace(const Icl4Shape &s, int q_rows, int n_blocks, int c
 }
 
 size_t icl4_select_workspace(const Icl4Shape &s, int q_rows) {
-    const SelectTurns t = select_turns(s, q_rows);
-    return (size_t)t.pairs * t.rows * t.padded * sizeof(int);
+    const SelectPlan t = plan_select(s, q_rows);
+    return t.fused ? 0 : (size_t)t.pairs * t.rows * t.padded * sizeof(int);
+}
+
+bool icl4_select_fits(const Icl4Shape &s, int q_rows) {
+    return (double)s.pairs() * ceil_div(q_rows, 16) * (kChooseWaves * 64) < 4294967296.0;
 }
 
 bool icl4_grid_fits(const Icl4Shape &s, int q_rows, int n_blocks, int compute_units) {
@@ -1581,7 +1665,8 @@ void icl4_decode(const Icl4Rows &a, const void *cache, float *bounds, hipStream_
     IRX_HIP(hipGetLastError());
 }
 
-void icl4_select(const Icl4Queries &a, int n, int *out, void *workspace, hipStream_t stream) {
+template <typename T>
+void choose(const Icl4Queries &a, int n, int *out, void *workspace, hipStream_t stream) {
     const Icl4Shape &s = a.shape;
     const Parts c = parts(a.cache, s);
     SelectArgs p{};
@@ -1589,8 +1674,18 @@ void icl4_select(const Icl4Queries &a, int n, int *out, void *workspace, hipStre
     p.lengths = a.lengths, p.keep = a.keep, p.heads = s.heads, p.pairs = s.pairs(), p.q_rows = a.q_rows;
     p.rows = s.rows, p.blocks = s.blocks(), p.bounds = c.bounds, p.scales = c.scales, p.n = n, p.out = out;
     p.scores = static_cast<int *>(workspace);
-    const SelectTurns t = select_turns(s, a.q_rows);
+    const SelectPlan t = plan_select(s, a.q_rows);
     p.padded = t.padded;
+    KernelTimer timer(kFamIcl, stream, 256.0 * p.pairs * p.q_rows * p.blocks, 128.0 * p.pairs * p.blocks);
+    const dim3 wg(kPickWaves * 64);
+    if (t.fused) {
+        p.qtiles = (int)ceil_div(p.q_rows, 16);
+        const dim3 grid((unsigned)((long long)p.pairs * p.qtiles));
+        const unsigned lds = (unsigned)(std::min(16, p.q_rows) * (t.padded + 4) * sizeof(int));
+        hipLaunchKernelGGL(icl4_choose_kernel<T>, grid, dim3(kChooseWaves * 64), lds, stream, p);
+        IRX_HIP(hipGetLastError());
+        return;
+    }
     for (p.pair0 = 0; p.pair0 < p.pairs; p.pair0 += t.pairs)
         for (p.row0 = 0; p.row0 < p.q_rows; p.row0 += t.rows) {
             const int pairs = std::min(t.pairs, p.pairs - p.pair0);
@@ -1602,20 +1697,21 @@ void icl4_select(const Icl4Queries &a, int n, int *out, void *workspace, hipStre
             while (p.chunk > 16 && tiles * ceil_div(p.blocks, 4 * p.chunk) < 2LL * a.compute_units) p.chunk /= 2;
             p.chunks = (int)ceil_div(p.blocks, 4 * p.chunk);
             const dim3 grid((unsigned)(tiles * p.chunks)), rows((unsigned)(pairs * p.rows_here));
-            KernelTimer timer(kFamIcl, stream, 256.0 * rows.x * p.blocks, 128.0 * pairs * p.blocks);
-            if (a.half)
-                hipLaunchKernelGGL(icl4_scores_kernel<_Float16>, grid, dim3(256), 0, stream, p);
-            else
-                hipLaunchKernelGGL(icl4_scores_kernel<float>, grid, dim3(256), 0, stream, p);
+            hipLaunchKernelGGL(icl4_scores_kernel<T>, grid, dim3(256), 0, stream, p);
             IRX_HIP(hipGetLastError());
-            if (p.blocks <= kWavePicks)
-                hipLaunchKernelGGL(icl4_pick_wave_kernel, rows, dim3(64), 0, stream, p);
-            else if (p.blocks <= kStagedPicks)
-                hipLaunchKernelGGL(icl4_pick_kernel<true>, rows, dim3(1024), (unsigned)p.padded * sizeof(int), stream, p);
+            if (p.blocks <= kStagedPicks)
+                hipLaunchKernelGGL(icl4_pick_kernel<true>, rows, wg, (unsigned)p.padded * sizeof(int), stream, p);
             else
-                hipLaunchKernelGGL(icl4_pick_kernel<false>, rows, dim3(1024), 0, stream, p);
+                hipLaunchKernelGGL(icl4_pick_kernel<false>, rows, wg, 0, stream, p);
             IRX_HIP(hipGetLastError());
         }
+}
+
+void icl4_select(const Icl4Queries &a, int n, int *out, void *workspace, hipStream_t stream) {
+    if (a.half)
+        choose<_Float16>(a, n, out, workspace, stream);
+    else
+        choose<float>(a, n, out, workspace, stream);
 }
 
 void icl4_attend(const Icl4Queries &a, const Icl4Attend &b, hipStream_t stream) {

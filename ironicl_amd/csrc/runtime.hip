@@ -1588,7 +1588,8 @@ bool icl4_shape_ok(const irx_icl4_shape *s) {
     if (!s || !s->estimators || !s->heads || !s->rows) return false;
     if (s->estimators > 65536 || s->heads > 65536 || s->estimators * s->heads > 65536) return false;
     if (s->rows > (size_t)1 << 27) return false;
-    return icl4_bytes(icl4_shape(*s)) <= (size_t)1 << 40;
+    // A workgroup of 256 to a block: one launch of less than 2^32 work-items.
+    return s->estimators * s->heads * ((s->rows + kIcl4Block - 1) / kIcl4Block) < (size_t)1 << 24;
 }
 
 void icl4_aligned(const void *p, size_t bytes, const char *what) {
@@ -2320,6 +2321,7 @@ int irx_icl4_select(irx_device *device, const irx_icl4_queries *queries, const v
             fail(IRX_INVALID_ARGUMENT, "1 to " + std::to_string(kIcl4MaxBlocks) + " blocks are chosen");
         Icl4Queries a = icl4_queries(*queries, cache);
         icl4_aligned(blocks, 4, "blocks");
+        if (!icl4_select_fits(a.shape, a.q_rows)) fail(IRX_INVALID_ARGUMENT, "too many queries for one call");
         icl4_device(device);
         a.compute_units = device->compute_units;
         icl4_workspace(workspace, workspace_bytes, icl4_select_workspace(a.shape, a.q_rows));

@@ -30,11 +30,12 @@ _THREE = struct.Struct("@NNN")
 
 
 def _address(buffer):
-    if buffer is None or isinstance(buffer, int):
+    if buffer is None or buffer.__class__ is int:
         return buffer
-    if hasattr(buffer, "data_ptr"):
+    try:
         return buffer.data_ptr()
-    return buffer.ptr
+    except AttributeError:
+        return buffer.ptr
 
 
 def _element(element: str) -> int:

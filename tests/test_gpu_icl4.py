@@ -310,6 +310,25 @@ def test_select_of_equal_scores_takes_the_lower_blocks(device):
     assert np.all(got == np.arange(7))
 
 
+@pytest.mark.parametrize("times,rows", [(3, 70), (30, 2), (30, 40)])
+def test_select_of_many_blocks(device, times, rows):
+    """500 blocks over and over: 1,500 for many queries and 15,000, in the forms that keep scores in memory. Equal
+    scores are many, and the lowest of them are taken."""
+    k = draw((1, 2, 32000, 64), "f32", 5)
+    want = icl4_np.Cache(k, k)
+    whole, shape = np.tile(k, (1, 1, times, 1)), (1, 2, 32000 * times)
+    cache = hipmem.DeviceArray((icl4.cache_bytes(shape),), np.uint8)
+    dk = put(whole)
+    icl4.encode(device, shape, dk, dk, cache)
+    hipmem.synchronize()
+    q = draw((1, 2, 300 if times == 3 else rows, 64), "f32", 6)
+    keep = np.random.default_rng(7).random((1, shape[2] // 64)) < 0.8
+    scores = np.where(keep[:, None, None], np.tile(want.scores(q), (1, 1, 1, times)), -np.inf)
+    order = np.sort(np.argsort(-scores, axis=-1, kind="stable")[..., :rows], axis=-1)
+    got = select(device, cache, shape, q, rows, keep=np.repeat(keep, 64, axis=1))
+    np.testing.assert_array_equal(got, order)
+
+
 def test_select_of_masked_and_empty_blocks(device):
     e, h, n = 4, 2, 900
     lengths = (0, 65, 900, 500)
@@ -506,8 +525,10 @@ def test_small_workspaces_are_refused(device):
         with pytest.raises(hip.HipError, match="workspace must hold") as info:
             icl4.attention(device, (1, 8, 5000), cache, q, 1, out, **kw)
         assert info.value.status == hip.INVALID_ARGUMENT
-    blocks = hipmem.DeviceArray((1, 8, 1, 4), np.int32)
-    with pytest.raises(hip.HipError, match="workspace must hold"):
-        icl4.select(device, (1, 8, 5000), cache, q, 1, 4, blocks)
+    blocks = hipmem.DeviceArray((1, 8, 200, 4), np.int32)
+    with pytest.raises(hip.HipError, match="workspace must hold"):  # its scores do not fit one launch
+        icl4.select(device, (1, 8, 70000), cache, q, 200, 4, blocks)
+    with pytest.raises(hip.HipError, match="too many queries"):
+        icl4.select(device, (8192, 8, 64), cache, q, 30000, 4, blocks)
     with pytest.raises(hip.HipError, match="too many queries"):
         icl4.attention(device, (8192, 8, 64), cache, q, 30000, out, out_strides=(30000 * 512, 64, 512))
