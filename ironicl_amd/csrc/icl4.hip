@@ -440,9 +440,11 @@ __device__ __forceinline__ QueryCodes query_codes(const SelectArgs &p, int pair,
     float x[16];
     load16(src, x);
     float m = 0.f;
+    float unit[16];
+    load16(p.scales + pair * 64 + 16 * g, unit);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        x[i] *= p.scales[pair * 64 + 16 * g + i];
+        x[i] *= unit[i];
         m = fmaxf(m, fabsf(x[i]));
     }
     m = fmaxf(m, __shfl_xor(m, 16, 64));
@@ -543,16 +545,18 @@ __device__ __forceinline__ i32x4 attended_scores(const SelectArgs &p, const int 
 // that exactly n scores reach, or else the n-th largest. Lane l holds blocks
 // 256 i + 4 l + j.
 constexpr int kWavePicks = 960;  // sixteen queries' scores in 64 KB of LDS
-__device__ __forceinline__ void pick_by_wave(const SelectArgs &p, const int *scores, int e, int rows, int *out) {
+__device__ __forceinline__ void pick_by_wave(const SelectArgs &p, const int *scores, const unsigned *attended, int *out) {
     const int lane = threadIdx.x & 63, padded = (int)p.padded;
     i32x4 held[4];
     int least = 1 << 30, most = kNoScore, total = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int b = 256 * i + 4 * lane;
-        held[i] = b < padded ? attended_scores(p, scores, e, rows, b) : i32x4{kNoScore, kNoScore, kNoScore, kNoScore};
+        held[i] = *reinterpret_cast<const i32x4 *>(scores + min(b, padded - 4));
+        const unsigned some = attended[64 * i + lane];  // a byte to a block, 0 past the last
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+            held[i][j] = some >> (8 * j) & 0xffu ? held[i][j] : kNoScore;
             most = max(most, held[i][j]);
             least = held[i][j] == kNoScore ? least : min(least, held[i][j]);
             total += held[i][j] != kNoScore;
@@ -746,6 +750,7 @@ constexpr int kChooseWaves = 16;
 template <typename T>
 __global__ __launch_bounds__(kChooseWaves * 64) void icl4_choose_kernel(SelectArgs p) {
     extern __shared__ __attribute__((aligned(16))) int staged[];  // [queries][padded + 4]
+    __shared__ __attribute__((aligned(16))) unsigned char attended[kChooseWaves * 64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, i16 = lane & 15;
     const int pair = (int)(blockIdx.x / (unsigned)p.qtiles), qt = (int)(blockIdx.x - (unsigned)pair * p.qtiles);
@@ -758,6 +763,11 @@ __global__ __launch_bounds__(kChooseWaves * 64) void icl4_choose_kernel(SelectAr
     i32x4 low[STEPS], high[STEPS];
 #pragma unroll
     for (int u = 0; u < STEPS; ++u) load_bounds(bounds, 16 * wave + u * STEP, p.blocks, i16, low[u], high[u]);
+    {
+        static_assert(kChooseWaves * 64 >= kWavePicks, "a thread to a block");
+        const int b = threadIdx.x;
+        attended[b] = b < p.blocks && block_mask(p.keep, e, p.blocks, b, rows) != 0;
+    }
     const QueryCodes c = query_codes<T>(p, pair, min(16 * qt + i16, p.q_rows - 1), g);
 #pragma unroll
     for (int u = 0; u < STEPS; ++u) {
@@ -770,7 +780,8 @@ __global__ __launch_bounds__(kChooseWaves * 64) void icl4_choose_kernel(SelectAr
     __syncthreads();
     const int mine = 16 * qt + wave;
     if (mine < p.q_rows)
-        pick_by_wave(p, staged + wave * stride, e, rows, p.out + ((long long)pair * p.q_rows + mine) * p.n);
+        pick_by_wave(p, staged + wave * stride, reinterpret_cast<const unsigned *>(attended),
+                     p.out + ((long long)pair * p.q_rows + mine) * p.n);
 }
 
 // ---- attention ----
@@ -1233,11 +1244,11 @@ __device__ __forceinline__ void load_block(const unsigned char *in, int lane, Bl
 // take one row's score out of its sixteen and the softmax costs one
 // exponential per row; FP32 operands' high and low parts stand in even and odd
 // columns, one product each, and neighbouring lanes add theirs.
-template <typename T, bool LISTED, bool SPLIT>
-__global__ __launch_bounds__(kWaves * 64) void icl4_one_kernel(AttendArgs p) {
+template <typename T, bool LISTED, bool SPLIT, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, 4) void icl4_one_kernel(AttendArgs p) {
     constexpr bool PAIRS = sizeof(T) == 4;
-    __shared__ float red_o[kWaves][64];
-    __shared__ float red_m[kWaves], red_l[kWaves];
+    __shared__ float red_o[WAVES][64];
+    __shared__ float red_m[WAVES], red_l[WAVES];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int g = lane >> 4, i16 = lane & 15;
     // Workgroups of one XCD (every eighth) take consecutive queries of a pair, whose blocks then share its L2.
@@ -1291,16 +1302,6 @@ __global__ __launch_bounds__(kWaves * 64) void icl4_one_kernel(AttendArgs p) {
     const int mine = 32 * (i16 >> 3) + 16 * (g >> 1) + 8 * ((i16 >> 2) & 1) + 4 * (g & 1) + (i16 & 3);
     const unsigned parts = i16 & 1 ? 0x07060302u : 0x05040100u;  // low or high halves of two words
 
-    // The next place at or after `at` with a block to attend to: its block, or -1.
-    auto find = [&](int &at, unsigned long long &mask) {
-        for (; at < end; at += kWaves) {
-            const int block = LISTED ? __builtin_amdgcn_readfirstlane(list[at]) : at;
-            if (LISTED && (unsigned)block >= (unsigned)p.blocks) continue;
-            mask = block_mask(p.keep, e, p.blocks, block, rows);
-            if (mask) return block;
-        }
-        return -1;
-    };
     auto process = [&](const BlockWords &w, unsigned long long mask) {
         f32x4 s[4];
 #pragma unroll
@@ -1359,22 +1360,36 @@ __global__ __launch_bounds__(kWaves * 64) void icl4_one_kernel(AttendArgs p) {
                     codes8(w.v[st][d], __uint_as_float(((w.ve[st] >> (8 * d)) & 0xffu) << 23)), as_half8(pw), o[d], 0, 0, 0);
         }
     };
-    // Two sets of operands in turn: the next block's loads are issued before this one's products.
+    // 64 of the wave's places at a time, one to a lane; two sets of operands in turn, the next block's loads issued
+    // before this one's products.
     BlockWords wa, wb;
-    unsigned long long mask_a = 0, mask_b = 0;
-    int at = split * p.per_split + wave;
-    int block = find(at, mask_a);
-    if (block >= 0) load_block(tiles + (long long)block * kBlockBytes, lane, wa);
-    while (block >= 0) {
-        at += kWaves;
-        block = find(at, mask_b);
-        if (block >= 0) load_block(tiles + (long long)block * kBlockBytes, lane, wb);
-        process(wa, mask_a);
-        if (block < 0) break;
-        at += kWaves;
-        block = find(at, mask_a);
-        if (block >= 0) load_block(tiles + (long long)block * kBlockBytes, lane, wa);
-        process(wb, mask_b);
+    for (int at0 = split * p.per_split + wave; at0 < end; at0 += 64 * WAVES) {
+        int block = at0 + WAVES * lane;
+        unsigned long long mask = 0;
+        if (block < end) {
+            if (LISTED) block = list[block];
+            if ((unsigned)block < (unsigned)p.blocks) mask = block_mask(p.keep, e, p.blocks, block, rows);
+        }
+        unsigned long long live = __ballot(mask != 0);
+        const int low = (int)(unsigned)mask, high = (int)(unsigned)(mask >> 32);
+        auto take = [&](BlockWords &w, unsigned long long &m) {
+            const int i = __builtin_ctzll(live);
+            live &= live - 1;
+            m = (unsigned long long)(unsigned)__builtin_amdgcn_readlane(high, i) << 32 | (unsigned)__builtin_amdgcn_readlane(low, i);
+            load_block(tiles + (long long)__builtin_amdgcn_readlane(block, i) * kBlockBytes, lane, w);
+        };
+        unsigned long long mask_a = 0, mask_b = 0;
+        bool more = live != 0;
+        if (more) take(wa, mask_a);
+        while (more) {
+            more = live != 0;
+            if (more) take(wb, mask_b);
+            process(wa, mask_a);
+            if (!more) break;
+            more = live != 0;
+            if (more) take(wa, mask_a);
+            process(wb, mask_b);
+        }
     }
     // Register r of o[d]: dim 16 d + 4 g + r, in every column (pair of columns).
     l_run = wave_sum(l_run);
@@ -1392,11 +1407,11 @@ __global__ __launch_bounds__(kWaves * 64) void icl4_one_kernel(AttendArgs p) {
     const int d = 4 * threadIdx.x;
     float mx = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, red_m[w]);
+    for (int w = 0; w < WAVES; ++w) mx = fmaxf(mx, red_m[w]);
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     float den = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
         const float a = mx > -INFINITY ? __builtin_amdgcn_exp2f(red_m[w] - mx) : 1.0f;
         acc += a * *reinterpret_cast<const f32x4 *>(&red_o[w][d]);
         den += a * red_l[w];
@@ -1481,9 +1496,13 @@ __global__ __launch_bounds__(256) void icl4_merge_kernel(AttendArgs p) {
 
 struct Plan {
     int queries;  // of a workgroup: 1, 16, 32 or 64
+    int waves;    // of a workgroup of one query: 4 or 16
     int qtiles, splits, per_split;
     long long rows;  // (pair, query) rows
 };
+
+// Listed blocks up to which few queries take sixteen waves each rather than splits of four and a merge.
+constexpr int kManyWaves = 16, kUnsplitBlocks = 256;
 
 // Queries up to which attention over every block takes a workgroup per query.
 constexpr int kOneQueries = 1;
@@ -1495,7 +1514,12 @@ Plan plan_attend(const Icl4Shape &s, int q_rows, int n_blocks, int compute_units
     pl.queries = n_blocks || q_rows <= kOneQueries ? 1 : q_rows <= 16 ? 16 : q_rows <= 32 ? 32 : 64;
     pl.qtiles = (int)ceil_div(q_rows, pl.queries);
     pl.rows = (long long)s.pairs() * q_rows;
+    pl.waves = kWaves;
     const long long base = (long long)s.pairs() * pl.qtiles;
+    if (n_blocks && n_blocks <= kUnsplitBlocks && n_blocks > kWaves && base < 2LL * compute_units) {
+        pl.waves = kManyWaves, pl.splits = 1, pl.per_split = n_blocks;
+        return pl;
+    }
     const long long slots = 2LL * compute_units, tiles = ceil_div(places, kWaves);
     long long splits = 1;
     if (pl.queries <= 16) {
@@ -1567,14 +1591,16 @@ void attend(const Icl4Queries &a, const Icl4Attend &b, hipStream_t stream) {
         const double work = 256.0 * kBlock * (b.list ? (double)tiles : (double)tiles * a.q_rows);
         KernelTimer timer(kFamIcl, stream, work, (double)tiles * kBlockBytes + 2.0 * sizeof(T) * 64 * pl.rows);
         const bool split = pl.splits > 1;
-        if (b.list && split)
-            hipLaunchKernelGGL((icl4_one_kernel<T, true, true>), grid, wg, 0, stream, p);
+        if (b.list && pl.waves == kManyWaves)
+            hipLaunchKernelGGL((icl4_one_kernel<T, true, false, kManyWaves>), grid, dim3(kManyWaves * 64), 0, stream, p);
+        else if (b.list && split)
+            hipLaunchKernelGGL((icl4_one_kernel<T, true, true, kWaves>), grid, wg, 0, stream, p);
         else if (b.list)
-            hipLaunchKernelGGL((icl4_one_kernel<T, true, false>), grid, wg, 0, stream, p);
+            hipLaunchKernelGGL((icl4_one_kernel<T, true, false, kWaves>), grid, wg, 0, stream, p);
         else if (pl.queries == 1 && split)
-            hipLaunchKernelGGL((icl4_one_kernel<T, false, true>), grid, wg, 0, stream, p);
+            hipLaunchKernelGGL((icl4_one_kernel<T, false, true, kWaves>), grid, wg, 0, stream, p);
         else if (pl.queries == 1)
-            hipLaunchKernelGGL((icl4_one_kernel<T, false, false>), grid, wg, 0, stream, p);
+            hipLaunchKernelGGL((icl4_one_kernel<T, false, false, kWaves>), grid, wg, 0, stream, p);
         else if (pl.queries == 16 && split)
             hipLaunchKernelGGL((icl4_rows_kernel<T, true>), grid, wg, 0, stream, p);
         else if (pl.queries == 16)
