@@ -66,6 +66,22 @@ __device__ __forceinline__ unsigned long long block_mask(const unsigned long lon
     return m;
 }
 
+// Whole division of 0 <= n < 2^31 by a constant of the launch: with 2^(l - 1) < d
+// <= 2^l and m = floor(2^(31 + l) / d) + 1, n m / 2^(31 + l) is past n / d by less
+// than 1 / d. (A division by a variable is some 25 scalar instructions, before
+// a workgroup's first load.)
+struct Division {
+    unsigned d, m, shift;
+};
+Division division(long long d) {
+    unsigned l = 0;
+    while ((1ll << l) < d) ++l;
+    return {(unsigned)d, (unsigned)((1ull << (31 + l)) / (unsigned long long)d + 1), 31 + l};
+}
+__device__ __forceinline__ unsigned divide(unsigned n, const Division &by) {
+    return (unsigned)(((unsigned long long)n * by.m) >> by.shift);
+}
+
 // ---- writing ----
 
 // The smallest e with m <= 6 * 2^e, held to -13..13 (m finite).
@@ -802,6 +818,7 @@ struct AttendArgs {
     float *partial;   // outputs [splits, pairs * q_rows, 64], then log2-sum-exps [splits, pairs * q_rows]
     int splits, per_split;  // blocks (or listed places) of a split
     int qtiles, count, per_xcd;
+    Division by_qtiles, by_splits, by_queries, by_heads;
 };
 
 constexpr float kLn2 = 0.69314718055994530942f;
@@ -833,11 +850,10 @@ __global__ __launch_bounds__(kWaves * 64) void icl4_rows_kernel(AttendArgs p) {
     __shared__ float red_o[kWaves][16 * 68];
     __shared__ float red_m[kWaves][16], red_l[kWaves][16];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, i16 = lane & 15;
-    unsigned id = blockIdx.x;
-    const int split = (int)(id % (unsigned)p.splits);
-    id /= (unsigned)p.splits;
-    const int qt = (int)(id % (unsigned)p.qtiles), pair = (int)(id / (unsigned)p.qtiles);
-    const int e = pair / p.heads, head = pair - e * p.heads;
+    const unsigned tile = SPLIT ? divide(blockIdx.x, p.by_splits) : blockIdx.x;
+    const int split = SPLIT ? (int)(blockIdx.x - tile * p.by_splits.d) : 0;
+    const int pair = (int)divide(tile, p.by_qtiles), qt = (int)(tile - pair * p.by_qtiles.d);
+    const int e = (int)divide(pair, p.by_heads), head = pair - e * p.heads;
     const int rows = rows_of(p.lengths, e, p.rows);
     const int qrow = min(16 * qt + i16, p.q_rows - 1);
     half8 qh[2], ql[2];
@@ -1005,12 +1021,12 @@ __global__ __launch_bounds__(kWaves * 64, 2) void icl4_wide_kernel(AttendArgs p)
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int h = lane >> 5, r32 = lane & 31, i16 = lane & 15, x16 = (lane >> 4) & 1;
     // Workgroups of one XCD take consecutive query tiles of one share of the blocks, read into one L2.
-    unsigned id = (blockIdx.x & 7u) * (unsigned)p.per_xcd + (blockIdx.x >> 3);
+    const unsigned id = (blockIdx.x & 7u) * (unsigned)p.per_xcd + (blockIdx.x >> 3);
     if (id >= (unsigned)p.count) return;
-    const int qt = (int)(id % (unsigned)p.qtiles);
-    id /= (unsigned)p.qtiles;
-    const int split = (int)(id % (unsigned)p.splits), pair = (int)(id / (unsigned)p.splits);
-    const int e = pair / p.heads, head = pair - e * p.heads;
+    const unsigned share = divide(id, p.by_qtiles);
+    const int qt = (int)(id - share * p.by_qtiles.d), pair = SPLIT ? (int)divide(share, p.by_splits) : (int)share;
+    const int split = SPLIT ? (int)(share - pair * p.by_splits.d) : 0;
+    const int e = (int)divide(pair, p.by_heads), head = pair - e * p.heads;
     const int rows = rows_of(p.lengths, e, p.rows);
     half8 qh[NJ][4], ql[PAIRS ? NJ : 1][4];
     float c[NJ];
@@ -1222,74 +1238,88 @@ __device__ __forceinline__ unsigned row_lane(unsigned x) {
     return __builtin_amdgcn_update_dpp(0, x, 0x150 + N, 0xf, 0xf, true);
 }
 
-// One block's operands of a wave as they lie in the cache.
-struct BlockWords {
-    u32x4 k[2], v[2];
-    unsigned ke;
-    u32x2 ve;
-};
-__device__ __forceinline__ void load_block(const unsigned char *in, int lane, BlockWords &w) {
-    const int g = lane >> 4, i16 = lane & 15;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        w.k[s] = *reinterpret_cast<const u32x4 *>(in + s * 1024 + lane * 16);
-        w.v[s] = *reinterpret_cast<const u32x4 *>(in + kValuesAt + s * 1024 + lane * 16);
-    }
-    w.ke = *reinterpret_cast<const unsigned *>(in + kKeyExpsAt + ((g >> 1) * 16 + i16) * 4);
-    w.ve = *reinterpret_cast<const u32x2 *>(in + kValueExpsAt + i16 * 8);
-}
+typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 // One query per workgroup, its blocks (listed, or all) in turn over the waves.
-// All sixteen columns of the products hold the one query, so that a lane can
-// take one row's score out of its sixteen and the softmax costs one
-// exponential per row; FP32 operands' high and low parts stand in even and odd
-// columns, one product each, and neighbouring lanes add theirs.
+//
+// Scores come from the codes as they lie in the cache: 16x16x128 products of the
+// query, in whole numbers, by E2M1 rows with their exponents, which take no
+// conversion. The query, scaled by a power of two to 31-bit integers, is eight
+// digits to the base 16 (the first signed), exact in E4M3. Row 4 n + r of the
+// query's operand holds digits 2 r (times 16) and 2 r + 1: the 128 terms are the
+// 64 dims by the two; terms 32 g .. +15 are dims 16 g .. by the first, the next 16
+// the same dims by the second, so a lane's 16 dims of a key stand twice. The
+// exponent of row 4 n + r is that of its digits in the product of the n-th 16
+// rows of the block and 2^-127 in the others, so that the four products add up
+// in one accumulator: lane (g, i16) ends with the four digit pairs of the i16-th
+// row of the g-th sixteen, and adds them. The softmax so costs one exponential
+// per row. (With keys converted to FP16 and every column the query, a block
+// took 190 vector instructions instead of 100.) Weights go through LDS to where
+// the second product wants them: FP32's as high FP16 parts in even and low ones
+// in odd columns.
 template <typename T, bool LISTED, bool SPLIT, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 4) void icl4_one_kernel(AttendArgs p) {
     constexpr bool PAIRS = sizeof(T) == 4;
     __shared__ float red_o[WAVES][64];
     __shared__ float red_m[WAVES], red_l[WAVES];
+    __shared__ __attribute__((aligned(16))) _Float16 shared_weights[WAVES][2][64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int g = lane >> 4, i16 = lane & 15;
     // Workgroups of one XCD (every eighth) take consecutive queries of a pair, whose blocks then share its L2.
     const unsigned id = (blockIdx.x & 7u) * (unsigned)p.per_xcd + (blockIdx.x >> 3);
     if (id >= (unsigned)p.count) return;
-    const int split = (int)(id % (unsigned)p.splits);
-    const int pq = (int)(id / (unsigned)p.splits);
-    const int pair = pq / p.q_rows, row = pq - pair * p.q_rows;
-    const int e = pair / p.heads, head = pair - e * p.heads;
+    const int pq = SPLIT ? (int)divide(id, p.by_splits) : (int)id, split = SPLIT ? (int)(id - pq * p.by_splits.d) : 0;
+    const int pair = (int)divide(pq, p.by_queries), row = pq - pair * p.q_rows;
+    const int e = (int)divide(pair, p.by_heads), head = pair - e * p.heads;
     const int rows = rows_of(p.lengths, e, p.rows);
-    half8 q[2];
+    _Float16 *weights = shared_weights[wave][0];
+    i32x8 digits;
     float c = p.scale;
     {
-        const T *src = static_cast<const T *>(p.q) + e * p.q_est + head * p.q_head + (long long)row * p.q_row + 16 * g;
-        if constexpr (PAIRS) {
-            float x[16];
-            float m = 0.f;
+        // Terms 16 g .. and 64 + 16 g .. stand in lane (g, .): dims 16 (g / 2) .. and 32 more, digit 2 (i16 % 4) + g % 2.
+        // Every fourth lane of a row makes a part: dims 4 (i16 / 4) .. +3 of both.
+        const T *src = static_cast<const T *>(p.q) + e * p.q_est + head * p.q_head + (long long)row * p.q_row +
+                       16 * (g >> 1) + 4 * (i16 >> 2);
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        const T4 v[2] = {*reinterpret_cast<const T4 *>(src), *reinterpret_cast<const T4 *>(src + 32)};
+        float x[8];
+        float m = 0.f;
+        bool finite = true;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            x[i] = (float)v[i >> 2][i & 3];
+            m = fmaxf(m, fabsf(x[i]));
+            finite = finite && fabsf(x[i]) <= 3.4028235e38f;
+        }
+        m = fmaxf(m, __uint_as_float(row_xor<4>(__float_as_uint(m))));
+        m = fmaxf(m, __uint_as_float(row_xor<8>(__float_as_uint(m))));
+        m = halves_max(m);
+        // The largest into [2^29, 2^30).
+        const int ex = min(126, 29 - ((int)(__float_as_uint(m) >> 23) - 127));
+        c *= pow2(-ex);
+        if (!__all(finite)) c = NAN;
+        const float up = pow2(ex);
+        const int digit = 2 * (i16 & 3) + (g & 1), sh = 28 - 4 * digit;
+        const float first = g & 1 ? 1.0f : 16.0f;
+        unsigned *words = reinterpret_cast<unsigned *>(weights);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            float y[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const f32x4 v = *reinterpret_cast<const f32x4 *>(src + 4 * i);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[4 * i + j] = v[j], m = fmaxf(m, fabsf(v[j]));
+                const int whole = (int)fminf(fmaxf(rintf(x[4 * n + i] * up), -1073741824.f), 1073741824.f);
+                y[i] = (float)(digit ? (whole >> sh) & 15 : whole >> 28) * first;
             }
-            m = fmaxf(m, __shfl_xor(m, 16, 64));
-            m = fmaxf(m, __shfl_xor(m, 32, 64));
-            const int ex = pair_exponent(m);
-            const float up = pow2(ex);
-            c *= pow2(-ex);
+            int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+            w = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
+            words[(4 * g + (i16 & 3)) * 4 + (i16 >> 2)] = (unsigned)w;
+            const u32x4 all = *reinterpret_cast<const u32x4 *>(words + (4 * g + (i16 & 3)) * 4);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] *= up;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                half8 hi, lo;
-                pair8(x + 8 * i, hi, lo);
-                q[i] = i16 & 1 ? lo : hi;
-            }
-        } else {
-            q[0] = *reinterpret_cast<const half8 *>(src);
-            q[1] = *reinterpret_cast<const half8 *>(src + 8);
+            for (int i = 0; i < 4; ++i) digits[4 * n + i] = (int)all[i];
         }
     }
+    // Exponent bytes of row i16 in the products of the four sixteens: 16^(6 - 2 (i16 % 4)) in its own.
+    const int digit_exps = (127 + 24 - 8 * (i16 & 3)) << (8 * (i16 >> 2));
     f32x4 o[4];
 #pragma unroll
     for (int d = 0; d < 4; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1298,71 +1328,27 @@ __global__ __launch_bounds__(WAVES * 64, 4) void icl4_one_kernel(AttendArgs p) {
     const int *list = LISTED ? p.list + (long long)pq * p.n : nullptr;
     const int places = LISTED ? p.n : p.blocks;
     const int end = min(places, (split + 1) * p.per_split);
-    // The lane's row of a block: result register i16 of its 16.
-    const int mine = 32 * (i16 >> 3) + 16 * (g >> 1) + 8 * ((i16 >> 2) & 1) + 4 * (g & 1) + (i16 & 3);
-    const unsigned parts = i16 & 1 ? 0x07060302u : 0x05040100u;  // low or high halves of two words
+    // The lane's row of a block, and its weight's place: [step s][lanes g = 2 t + h][4 b + j].
+    const int mine = 32 * (g >> 1) + 16 * (i16 >> 3) + 8 * (g & 1) + (i16 & 7);
+    _Float16 *give = weights + 32 * (g >> 1) + 8 * (i16 >> 2) + 4 * (g & 1) + (i16 & 3);
+    const _Float16 *get = weights + (PAIRS ? 64 * (i16 & 1) : 0) + 8 * g;
+    const unsigned chunk_at = 16u * lane, ke_at = kKeyExpsAt + ((g >> 1) * 16 + i16) * 4, ve_at = kValueExpsAt + i16 * 8;
 
-    auto process = [&](const BlockWords &w, unsigned long long mask) {
-        f32x4 s[4];
-#pragma unroll
-        for (int kb = 0; kb < 4; ++kb) {
-            const float scale = __uint_as_float(((w.ke >> (8 * kb)) & 0xffu) << 23);
-            s[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-                s[kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(w.k[kb >> 1][2 * (kb & 1) + m], scale), q[m], s[kb],
-                                                               0, 0, 0);
-        }
-        // Register i16 and, for the neighbour, register i16 ^ 1.
-        float a[8], b[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) a[i] = s[i >> 1][2 * (i & 1)], b[i] = s[i >> 1][2 * (i & 1) + 1];
-#pragma unroll
-        for (int half = 4; half >= 1; half /= 2)
-#pragma unroll
-            for (int i = 0; i < half; ++i) {
-                const bool up = i16 & (2 * half);
-                a[i] = up ? a[i + half] : a[i], b[i] = up ? b[i + half] : b[i];
-            }
-        const bool odd = i16 & 1;
-        float x = odd ? b[0] : a[0];
-        if constexpr (PAIRS) x += next_lane(odd ? a[0] : b[0]);
-        x *= c;
-        if (mask != ~0ull && !((mask >> mine) & 1)) x = -INFINITY;
-        float weight = __builtin_amdgcn_exp2f(x - ref);
-        if (__any(!(weight <= 32768.0f))) {
-            const float ref_new = fmaxf(ref, wave_max(x) - kHeadroom);
-            const float alpha = __builtin_amdgcn_exp2f(ref - ref_new);
-            l_run *= alpha;
-#pragma unroll
-            for (int d = 0; d < 4; ++d) o[d] *= alpha;
-            ref = ref_new;
-            weight = __builtin_amdgcn_exp2f(x - ref);
-        }
-        l_run += weight;
-        const _Float16 hi = (_Float16)weight;
-        unsigned packed = __builtin_bit_cast(unsigned short, hi);
-        if constexpr (PAIRS)
-            packed |= (unsigned)__builtin_bit_cast(unsigned short, (_Float16)(weight - (float)hi)) << 16;
-        const unsigned all[16] = {row_lane<0>(packed),  row_lane<1>(packed),  row_lane<2>(packed),  row_lane<3>(packed),
-                                  row_lane<4>(packed),  row_lane<5>(packed),  row_lane<6>(packed),  row_lane<7>(packed),
-                                  row_lane<8>(packed),  row_lane<9>(packed),  row_lane<10>(packed), row_lane<11>(packed),
-                                  row_lane<12>(packed), row_lane<13>(packed), row_lane<14>(packed), row_lane<15>(packed)};
-#pragma unroll
-        for (int st = 0; st < 2; ++st) {
-            u32x4 pw;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                pw[j] = __builtin_amdgcn_perm(all[8 * st + 2 * j + 1], all[8 * st + 2 * j], PAIRS ? parts : 0x05040100u);
-#pragma unroll
-            for (int d = 0; d < 4; ++d)
-                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                    codes8(w.v[st][d], __uint_as_float(((w.ve[st] >> (8 * d)) & 0xffu) << 23)), as_half8(pw), o[d], 0, 0, 0);
-        }
+    u32x4 kw[2], vw[2];
+    unsigned ke;
+    u32x2 ve;
+    auto load_keys = [&](const unsigned char *in) {
+        kw[0] = *reinterpret_cast<const u32x4 *>(in + chunk_at);
+        kw[1] = *reinterpret_cast<const u32x4 *>(in + 1024 + chunk_at);
+        ke = *reinterpret_cast<const unsigned *>(in + ke_at);
     };
-    // 64 of the wave's places at a time, one to a lane; two sets of operands in turn, the next block's loads issued
-    // before this one's products.
-    BlockWords wa, wb;
+    auto load_values = [&](const unsigned char *in) {
+        vw[0] = *reinterpret_cast<const u32x4 *>(in + kValuesAt + chunk_at);
+        vw[1] = *reinterpret_cast<const u32x4 *>(in + kValuesAt + 1024 + chunk_at);
+        ve = *reinterpret_cast<const u32x2 *>(in + ve_at);
+    };
+    // 64 of the wave's places at a time, one to a lane. A block's keys are loaded as soon as the one before has its
+    // scores, its values once that one has its output.
     for (int at0 = split * p.per_split + wave; at0 < end; at0 += 64 * WAVES) {
         int block = at0 + WAVES * lane;
         unsigned long long mask = 0;
@@ -1371,24 +1357,64 @@ __global__ __launch_bounds__(WAVES * 64, 4) void icl4_one_kernel(AttendArgs p) {
             if ((unsigned)block < (unsigned)p.blocks) mask = block_mask(p.keep, e, p.blocks, block, rows);
         }
         unsigned long long live = __ballot(mask != 0);
+        if (!live) continue;
+        const unsigned long long whole = __ballot(mask == ~0ull);
         const int low = (int)(unsigned)mask, high = (int)(unsigned)(mask >> 32);
-        auto take = [&](BlockWords &w, unsigned long long &m) {
-            const int i = __builtin_ctzll(live);
+        int i = __builtin_ctzll(live);
+        const unsigned char *in = tiles + (long long)__builtin_amdgcn_readlane(block, i) * kBlockBytes;
+        load_keys(in);
+        load_values(in);
+        for (;;) {
+            const int now = i;
             live &= live - 1;
-            m = (unsigned long long)(unsigned)__builtin_amdgcn_readlane(high, i) << 32 | (unsigned)__builtin_amdgcn_readlane(low, i);
-            load_block(tiles + (long long)__builtin_amdgcn_readlane(block, i) * kBlockBytes, lane, w);
-        };
-        unsigned long long mask_a = 0, mask_b = 0;
-        bool more = live != 0;
-        if (more) take(wa, mask_a);
-        while (more) {
-            more = live != 0;
-            if (more) take(wb, mask_b);
-            process(wa, mask_a);
-            if (!more) break;
-            more = live != 0;
-            if (more) take(wa, mask_a);
-            process(wb, mask_b);
+            if (live) {
+                i = __builtin_ctzll(live);
+                in = tiles + (long long)__builtin_amdgcn_readlane(block, i) * kBlockBytes;
+            }
+            f32x4 s = {0.f, 0.f, 0.f, 0.f};
+            // Formats 0 (E4M3) and 4 (E2M1); the exponents are byte n of their words.
+#define IRX_SCORES(n)                                                                                                       \
+    {                                                                                                                       \
+        const int w0 = (int)kw[n / 2][2 * (n % 2)], w1 = (int)kw[n / 2][2 * (n % 2) + 1];                                   \
+        s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(digits, (i32x8{w0, w1, w0, w1, 0, 0, 0, 0}), s, 0, 4, n,       \
+                                                             digit_exps, n, (int)ke);                                       \
+    }
+            IRX_SCORES(0)
+            IRX_SCORES(1)
+            IRX_SCORES(2)
+            IRX_SCORES(3)
+#undef IRX_SCORES
+            if (live) load_keys(in);
+            float x = ((s[0] + s[1]) + (s[2] + s[3])) * c;
+            if (!(whole >> now & 1)) {
+                const unsigned long long m = (unsigned long long)(unsigned)__builtin_amdgcn_readlane(high, now) << 32 |
+                                             (unsigned)__builtin_amdgcn_readlane(low, now);
+                if (!((m >> mine) & 1)) x = -INFINITY;
+            }
+            float weight = __builtin_amdgcn_exp2f(x - ref);
+            if (__any(!(weight <= 32768.0f))) {
+                const float ref_new = fmaxf(ref, wave_max(x) - kHeadroom);
+                const float alpha = __builtin_amdgcn_exp2f(ref - ref_new);
+                l_run *= alpha;
+#pragma unroll
+                for (int d = 0; d < 4; ++d) o[d] *= alpha;
+                ref = ref_new;
+                weight = __builtin_amdgcn_exp2f(x - ref);
+            }
+            l_run += weight;
+            const _Float16 hi = (_Float16)weight;
+            give[0] = hi;
+            if constexpr (PAIRS) give[64] = (_Float16)(weight - (float)hi);
+#pragma unroll
+            for (int st = 0; st < 2; ++st) {
+                const half8 w = *reinterpret_cast<const half8 *>(get + 32 * st);
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                        codes8(vw[st][d], __uint_as_float(((ve[st] >> (8 * d)) & 0xffu) << 23)), w, o[d], 0, 0, 0);
+            }
+            if (!live) break;
+            load_values(in);
         }
     }
     // Register r of o[d]: dim 16 d + 4 g + r, in every column (pair of columns).
@@ -1585,6 +1611,8 @@ void attend(const Icl4Queries &a, const Icl4Attend &b, hipStream_t stream) {
     p.splits = pl.splits, p.per_split = pl.per_split, p.qtiles = pl.qtiles;
     const long long count = (long long)pl.splits * pl.qtiles * s.pairs();
     p.count = (int)count, p.per_xcd = (int)ceil_div((size_t)count, 8);
+    p.by_qtiles = division(pl.qtiles), p.by_splits = division(pl.splits), p.by_queries = division(a.q_rows);
+    p.by_heads = division(s.heads);
     const dim3 grid((unsigned)(pl.queries == 16 ? count : 8LL * p.per_xcd)), wg(kWaves * 64);
     {
         const long long tiles = b.list ? (long long)pl.rows * b.n : (long long)s.pairs() * s.blocks();
