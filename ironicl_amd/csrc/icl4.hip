@@ -1313,7 +1313,9 @@ __global__ __launch_bounds__(WAVES * 64, 4) void icl4_one_kernel(AttendArgs p) {
             int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
             w = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
             words[(4 * g + (i16 & 3)) * 4 + (i16 >> 2)] = (unsigned)w;
+            __builtin_amdgcn_wave_barrier();  // the wave's own LDS operations run in order
             const u32x4 all = *reinterpret_cast<const u32x4 *>(words + (4 * g + (i16 & 3)) * 4);
+            __builtin_amdgcn_wave_barrier();
 #pragma unroll
             for (int i = 0; i < 4; ++i) digits[4 * n + i] = (int)all[i];
         }
@@ -1405,6 +1407,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void icl4_one_kernel(AttendArgs p) {
             const _Float16 hi = (_Float16)weight;
             give[0] = hi;
             if constexpr (PAIRS) give[64] = (_Float16)(weight - (float)hi);
+            __builtin_amdgcn_wave_barrier();  // the wave's own LDS operations run in order
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
                 const half8 w = *reinterpret_cast<const half8 *>(get + 32 * st);
@@ -1522,13 +1525,15 @@ __global__ __launch_bounds__(256) void icl4_merge_kernel(AttendArgs p) {
 
 struct Plan {
     int queries;  // of a workgroup: 1, 16, 32 or 64
-    int waves;    // of a workgroup of one query: 4 or 16
+    int waves;    // of a workgroup of one query: 1, 4 or 16
     int qtiles, splits, per_split;
     long long rows;  // (pair, query) rows
 };
 
 // Listed blocks up to which few queries take sixteen waves each rather than splits of four and a merge.
 constexpr int kManyWaves = 16, kUnsplitBlocks = 256;
+// Queries per compute unit from which a query with listed blocks takes one wave.
+constexpr int kManyQueries = 16;
 
 // Queries up to which attention over every block takes a workgroup per query.
 constexpr int kOneQueries = 1;
@@ -1544,6 +1549,10 @@ Plan plan_attend(const Icl4Shape &s, int q_rows, int n_blocks, int compute_units
     const long long base = (long long)s.pairs() * pl.qtiles;
     if (n_blocks && n_blocks <= kUnsplitBlocks && n_blocks > kWaves && base < 2LL * compute_units) {
         pl.waves = kManyWaves, pl.splits = 1, pl.per_split = n_blocks;
+        return pl;
+    }
+    if (n_blocks && base >= (long long)kManyQueries * compute_units) {
+        pl.waves = 1, pl.splits = 1, pl.per_split = n_blocks;
         return pl;
     }
     const long long slots = 2LL * compute_units, tiles = ceil_div(places, kWaves);
@@ -1621,6 +1630,8 @@ void attend(const Icl4Queries &a, const Icl4Attend &b, hipStream_t stream) {
         const bool split = pl.splits > 1;
         if (b.list && pl.waves == kManyWaves)
             hipLaunchKernelGGL((icl4_one_kernel<T, true, false, kManyWaves>), grid, dim3(kManyWaves * 64), 0, stream, p);
+        else if (b.list && pl.waves == 1)
+            hipLaunchKernelGGL((icl4_one_kernel<T, true, false, 1>), grid, dim3(64), 0, stream, p);
         else if (b.list && split)
             hipLaunchKernelGGL((icl4_one_kernel<T, true, true, kWaves>), grid, wg, 0, stream, p);
         else if (b.list)
