@@ -361,7 +361,7 @@ int irx_regression_summary(irx_device *device, const float *decoded, size_t ense
 
 typedef enum irx_element { IRX_ELEMENT_F32 = 0, IRX_ELEMENT_F16 = 1 } irx_element;
 
-/* 1 to 65,536 pairs (estimators * heads), 1 to 2^27 rows, less than 2^24 blocks (75 GB) in all. */
+/* 1 to 65,535 pairs (estimators * heads), 1 to 2^27 rows, less than 2^24 blocks (75 GB) in all. */
 typedef struct irx_icl4_shape {
     size_t estimators;
     size_t heads;

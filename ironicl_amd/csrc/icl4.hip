@@ -36,10 +36,11 @@ constexpr int kBlock = kIcl4Block;            // rows of a block
 constexpr int kBlockBytes = kIcl4BlockBytes;  // bytes of one pair's block
 constexpr int kValuesAt = 2048, kKeyExpsAt = 4096, kValueExpsAt = 4224;
 
-// 2^(byte - 127) of byte `i` of a word.
+// The exponent byte I of a word as the scale of a conversion, which reads
+// nothing but the scale's exponent bits: the bits beside them are left in.
 template <int I>
-__device__ __forceinline__ float exp_byte(unsigned word) {
-    return __uint_as_float(((word >> (8 * I)) & 0xffu) << 23);
+__device__ __forceinline__ float scale_byte(unsigned word) {
+    return __uint_as_float(I == 0 ? word << 23 : I == 1 ? word << 15 : I == 2 ? word << 7 : word >> 1);
 }
 
 // Eight E2M1 codes times `scale` (a power of two) as FP16, exactly.
@@ -444,6 +445,13 @@ struct SelectArgs {
 constexpr int kNoScore = -(1 << 30);
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
+// The smallest f >= -100 with m <= 127 * 2^f.
+__device__ __forceinline__ int code_power(float m) {
+    const unsigned bits = __float_as_uint(m);
+    const int x = (int)(bits >> 23) - 126;  // zero and subnormal m end at -100
+    return min(120, max(-100, (bits & 0x7fffffu) <= 0x7e0000u ? x - 7 : x - 6));
+}
+
 // A query's codes as operands: lane (g, i16) dims 16 g .. of query i16,
 // positive and negative parts as bytes.
 struct QueryCodes {
@@ -465,13 +473,7 @@ __device__ __forceinline__ QueryCodes query_codes(const SelectArgs &p, int pair,
     }
     m = fmaxf(m, __shfl_xor(m, 16, 64));
     m = fmaxf(m, __shfl_xor(m, 32, 64));
-    int f = -100;
-    if (m > 0.f) {
-        const unsigned bits = __float_as_uint(m);
-        const int ex = (int)(bits >> 23) - 126;
-        f = min(120, max(-100, (bits & 0x7fffffu) <= 0x7e0000u ? ex - 7 : ex - 6));
-    }
-    const float inv = pow2(-f);
+    const float inv = pow2(-code_power(m));
     QueryCodes c;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
@@ -559,14 +561,15 @@ __device__ __forceinline__ i32x4 attended_scores(const SelectArgs &p, const int 
 // The n best of one query's scores by one wave with every score in a register
 // (up to 1,024): bisection between the least and the largest for a value
 // that exactly n scores reach, or else the n-th largest. Lane l holds blocks
-// 256 i + 4 l + j.
+// 256 i + 4 l + j of GROUPS 256s.
 constexpr int kWavePicks = 960;  // sixteen queries' scores in 64 KB of LDS
+template <int GROUPS>
 __device__ __forceinline__ void pick_by_wave(const SelectArgs &p, const int *scores, const unsigned *attended, int *out) {
     const int lane = threadIdx.x & 63, padded = (int)p.padded;
-    i32x4 held[4];
+    i32x4 held[GROUPS];
     int least = 1 << 30, most = kNoScore, total = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < GROUPS; ++i) {
         const int b = 256 * i + 4 * lane;
         held[i] = *reinterpret_cast<const i32x4 *>(scores + min(b, padded - 4));
         const unsigned some = attended[64 * i + lane];  // a byte to a block, 0 past the last
@@ -590,7 +593,7 @@ __device__ __forceinline__ void pick_by_wave(const SelectArgs &p, const int *sco
         const int cut = lo + (gap >> 1);
         int c = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < GROUPS; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) c += held[i][j] >= cut;
         c = __builtin_amdgcn_readfirstlane(wave_join(c, add));
@@ -605,14 +608,14 @@ __device__ __forceinline__ void pick_by_wave(const SelectArgs &p, const int *sco
     // Scores above lo and, where no value parts n of them, the first at it that there is room for, in order.
     int all = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < GROUPS; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) all += held[i][j] > lo;
     const int room = exact ? 0 : p.n - __builtin_amdgcn_readfirstlane(wave_join(all, add));
     const unsigned long long below = (1ull << lane) - 1;
     int before_above = 0, before_equal = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < GROUPS; ++i) {
         if (256 * i >= padded) break;
         int a = before_above, q = before_equal;
 #pragma unroll
@@ -761,32 +764,42 @@ __global__ __launch_bounds__(kPickWaves * 64) void icl4_pick_kernel(SelectArgs p
 
 // Scores and choice in one launch, no scores in memory, up to 960 blocks:
 // sixteen queries to a workgroup, scored together, then each chosen for by a
-// wave of its own.
+// wave of its own. Every load is issued first; each wave makes one query's
+// codes (the sixteen by every wave cost more than the scores).
 constexpr int kChooseWaves = 16;
-template <typename T>
+template <typename T, int GROUPS>
 __global__ __launch_bounds__(kChooseWaves * 64) void icl4_choose_kernel(SelectArgs p) {
     extern __shared__ __attribute__((aligned(16))) int staged[];  // [queries][padded + 4]
     __shared__ __attribute__((aligned(16))) unsigned char attended[kChooseWaves * 64];
+    __shared__ __attribute__((aligned(16))) signed char codes[2][kChooseWaves][64 + 16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, i16 = lane & 15;
-    const int pair = (int)(blockIdx.x / (unsigned)p.qtiles), qt = (int)(blockIdx.x - (unsigned)pair * p.qtiles);
-    const int e = pair / p.heads, rows = rows_of(p.lengths, e, p.rows);
+    const int qt = blockIdx.x, head = blockIdx.y, e = blockIdx.z, pair = e * p.heads + head;
+    const int rows = rows_of(p.lengths, e, p.rows), row = min(16 * qt + wave, p.q_rows - 1);
+    const float x0 = (float)static_cast<const T *>(p.q)[e * p.q_est + head * p.q_head + row * p.q_row + lane];
+    const float unit = p.scales[pair * 64 + lane];
     const signed char *bounds = p.bounds + (long long)pair * p.blocks * 128 + 16 * g;
     const int stride = (int)p.padded + 4;  // four banks on from one query to the next
-    // At most four steps of sixteen blocks to a wave, all loaded at once, the queries' codes beneath them.
-    constexpr int STEPS = 4, STEP = 16 * kChooseWaves;
-    static_assert(STEPS * STEP >= kWavePicks, "every block is scored");
-    i32x4 low[STEPS], high[STEPS];
+    // At most GROUPS steps of sixteen blocks to a wave.
+    constexpr int STEP = 16 * kChooseWaves;
+    i32x4 low[GROUPS], high[GROUPS];
 #pragma unroll
-    for (int u = 0; u < STEPS; ++u) load_bounds(bounds, 16 * wave + u * STEP, p.blocks, i16, low[u], high[u]);
+    for (int u = 0; u < GROUPS; ++u) load_bounds(bounds, 16 * wave + u * STEP, p.blocks, i16, low[u], high[u]);
+    const int mine = threadIdx.x;  // a thread to a block
+    const unsigned long long word = p.keep ? p.keep[(long long)e * p.blocks + min(mine, p.blocks - 1)] : ~0ull;
     {
-        static_assert(kChooseWaves * 64 >= kWavePicks, "a thread to a block");
-        const int b = threadIdx.x;
-        attended[b] = b < p.blocks && block_mask(p.keep, e, p.blocks, b, rows) != 0;
+        const float x = x0 * unit;
+        const float inv = pow2(-code_power(wave_max(fabsf(x))));
+        const int c = (int)rintf(fminf(fmaxf(x * inv, -127.f), 127.f));
+        codes[0][wave][lane] = (signed char)max(c, 0), codes[1][wave][lane] = (signed char)min(c, 0);
     }
-    const QueryCodes c = query_codes<T>(p, pair, min(16 * qt + i16, p.q_rows - 1), g);
+    const int left = rows - mine * kBlock;
+    attended[mine] = mine < p.blocks && left > 0 && word << max(0, kBlock - left) != 0;
+    __syncthreads();
+    const QueryCodes c = {*reinterpret_cast<const i32x4 *>(&codes[0][i16][16 * g]),
+                          *reinterpret_cast<const i32x4 *>(&codes[1][i16][16 * g])};
 #pragma unroll
-    for (int u = 0; u < STEPS; ++u) {
+    for (int u = 0; u < GROUPS; ++u) {
         const int b = 16 * wave + u * STEP;
         const i32x4 s = block_scores(low[u], high[u], c);
         // Only queries that there are have a row.
@@ -794,10 +807,10 @@ __global__ __launch_bounds__(kChooseWaves * 64) void icl4_choose_kernel(SelectAr
             *reinterpret_cast<i32x4 *>(staged + i16 * stride + b + 4 * g) = s;
     }
     __syncthreads();
-    const int mine = 16 * qt + wave;
-    if (mine < p.q_rows)
-        pick_by_wave(p, staged + wave * stride, reinterpret_cast<const unsigned *>(attended),
-                     p.out + ((long long)pair * p.q_rows + mine) * p.n);
+    const int query = 16 * qt + wave;
+    if (query < p.q_rows)
+        pick_by_wave<GROUPS>(p, staged + wave * stride, reinterpret_cast<const unsigned *>(attended),
+                             p.out + ((long long)pair * p.q_rows + query) * p.n);
 }
 
 // ---- attention ----
@@ -1094,7 +1107,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void icl4_wide_kernel(AttendArgs p)
     };
     auto process = [&](const Words &w, unsigned long long mask) {
         const unsigned ke = w.ke >> (16 * x16);
-        const float ks[2] = {__uint_as_float((ke & 0xffu) << 23), __uint_as_float((ke >> 8 & 0xffu) << 23)};
+        const float ks[2] = {scale_byte<0>(ke), scale_byte<1>(ke)};
         f32x16 s[NJ][2];
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
@@ -1161,7 +1174,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void icl4_wide_kernel(AttendArgs p)
             const unsigned ve = w.ve[t >> 1] >> (16 * x16);
 #pragma unroll
             for (int d = 0; d < 2; ++d) {
-                const half8 a = codes8(w.v[t][d], __uint_as_float((ve >> (8 * d) & 0xffu) << 23));
+                const half8 a = codes8(w.v[t][d], d ? scale_byte<1>(ve) : scale_byte<0>(ve));
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
                     if constexpr (PAIRS) o[j][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[j][t], o[j][d], 0, 0, 0);
@@ -1411,10 +1424,10 @@ __global__ __launch_bounds__(WAVES * 64, 4) void icl4_one_kernel(AttendArgs p) {
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
                 const half8 w = *reinterpret_cast<const half8 *>(get + 32 * st);
-#pragma unroll
-                for (int d = 0; d < 4; ++d)
-                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                        codes8(vw[st][d], __uint_as_float(((ve[st] >> (8 * d)) & 0xffu) << 23)), w, o[d], 0, 0, 0);
+                o[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(vw[st][0], scale_byte<0>(ve[st])), w, o[0], 0, 0, 0);
+                o[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(vw[st][1], scale_byte<1>(ve[st])), w, o[1], 0, 0, 0);
+                o[2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(vw[st][2], scale_byte<2>(ve[st])), w, o[2], 0, 0, 0);
+                o[3] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes8(vw[st][3], scale_byte<3>(ve[st])), w, o[3], 0, 0, 0);
             }
             if (!live) break;
             load_values(in);
@@ -1744,10 +1757,14 @@ void choose(const Icl4Queries &a, int n, int *out, void *workspace, hipStream_t 
     KernelTimer timer(kFamIcl, stream, 256.0 * p.pairs * p.q_rows * p.blocks, 128.0 * p.pairs * p.blocks);
     const dim3 wg(kPickWaves * 64);
     if (t.fused) {
-        p.qtiles = (int)ceil_div(p.q_rows, 16);
-        const dim3 grid((unsigned)((long long)p.pairs * p.qtiles));
+        const dim3 grid(ceil_div(p.q_rows, 16), (unsigned)s.heads, (unsigned)s.estimators), many(kChooseWaves * 64);
         const unsigned lds = (unsigned)(std::min(16, p.q_rows) * (t.padded + 4) * sizeof(int));
-        hipLaunchKernelGGL(icl4_choose_kernel<T>, grid, dim3(kChooseWaves * 64), lds, stream, p);
+        if (t.padded <= 256)
+            hipLaunchKernelGGL((icl4_choose_kernel<T, 1>), grid, many, lds, stream, p);
+        else if (t.padded <= 512)
+            hipLaunchKernelGGL((icl4_choose_kernel<T, 2>), grid, many, lds, stream, p);
+        else
+            hipLaunchKernelGGL((icl4_choose_kernel<T, 4>), grid, many, lds, stream, p);
         IRX_HIP(hipGetLastError());
         return;
     }

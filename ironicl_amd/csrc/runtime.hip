@@ -1586,7 +1586,7 @@ Icl4Shape icl4_shape(const irx_icl4_shape &s) { return {(int)s.estimators, (int)
 
 bool icl4_shape_ok(const irx_icl4_shape *s) {
     if (!s || !s->estimators || !s->heads || !s->rows) return false;
-    if (s->estimators > 65536 || s->heads > 65536 || s->estimators * s->heads > 65536) return false;
+    if (s->estimators > 65535 || s->heads > 65535 || s->estimators * s->heads > 65535) return false;
     if (s->rows > (size_t)1 << 27) return false;
     // A workgroup of 256 to a block: one launch of less than 2^32 work-items.
     return s->estimators * s->heads * ((s->rows + kIcl4Block - 1) / kIcl4Block) < (size_t)1 << 24;

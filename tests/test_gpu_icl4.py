@@ -529,6 +529,6 @@ def test_small_workspaces_are_refused(device):
     with pytest.raises(hip.HipError, match="workspace must hold"):  # its scores do not fit one launch
         icl4.select(device, (1, 8, 70000), cache, q, 200, 4, blocks)
     with pytest.raises(hip.HipError, match="too many queries"):
-        icl4.select(device, (8192, 8, 64), cache, q, 30000, 4, blocks)
+        icl4.select(device, (8190, 8, 64), cache, q, 30000, 4, blocks)
     with pytest.raises(hip.HipError, match="too many queries"):
-        icl4.attention(device, (8192, 8, 64), cache, q, 30000, out, out_strides=(30000 * 512, 64, 512))
+        icl4.attention(device, (8190, 8, 64), cache, q, 30000, out, out_strides=(30000 * 512, 64, 512))
