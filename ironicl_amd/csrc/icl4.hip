@@ -1016,19 +1016,50 @@ __device__ __forceinline__ float halves_sum(float x) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// 32 NJ queries per workgroup, every fourth block of its share to a wave, on
-// 32x32x16 products. A wave reads its blocks straight into registers and
-// decodes them there: 4 bits a number are few enough that neither LDS nor a
-// barrier stands between the cache and the products. Lane (r = lane % 32, h =
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x6 __attribute__((ext_vector_type(6)));
+typedef float f32x32 __attribute__((ext_vector_type(32)));
+
+// 32 numbers, scaled by a power of two so that the largest of the row is in [2,
+// 4), as PARTS operands in E2M3 (multiples of 1/8 below 2, of 1/4 below 4): x = p0
+// + p1 / 2^4 + p2 / 2^9 + ..., each part the nearest to what is left, which is at
+// most 1/8 (then 1/16) and is scaled up to 2 again: five bits a part, 2^-20 of
+// the largest after four and 2^-25 after five. The exponent bytes of parts 0
+// to 3 and of part 4: 16^-1, then 32^-1 each.
+constexpr int kPartExps = 127 | (127 - 4) << 8 | (127 - 9) << 16 | (127 - 14) << 24, kPartExps4 = 127 - 19;
+template <int PARTS>
+__device__ __forceinline__ void query_parts(f32x16 &even, f32x16 &odd, u32x6 (&parts)[PARTS]) {
+#pragma unroll
+    for (int n = 0; n < PARTS; ++n) {
+        parts[n] = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, 1.0f);
+        if (n == PARTS - 1) break;
+        const f32x32 held = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(parts[n], 1.0f);
+        const float up = n == 0 ? 16.f : 32.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            even[i] = (even[i] - held[2 * i]) * up, odd[i] = (odd[i] - held[2 * i + 1]) * up;
+    }
+}
+
+// 32 NJ queries per workgroup, every fourth block of its share to a wave. A wave
+// reads its blocks straight into registers: 4 bits a number are few enough that
+// neither LDS nor a barrier stands between the cache and the products. Scores
+// are scaled 32x32x64 products of the E2M1 keys as they lie in the cache by the
+// queries' E2M3 parts (33 cycles for what two 32x32x16 ones take 66 for, and no
+// conversion of keys, 7.4 cycles a pair of numbers); values are converted to
+// FP16 and multiplied by FP16 weights (FP32: pairs). What bounds it is the vector
+// unit: per 64 x 64 scores 64 exponentials (9.3 cycles), 64 multiply-adds, 32
+// conversions of values and 32 of weights, and the sums. Lane (r = lane % 32, h =
 // lane / 32), r = 16 s + 8 a + i:
-//   S^T, b = 0, 1: A = rows 32 s + 16 a + 8 b + i, dims 32 h + 8 m ..; B = query r, the same
-//     dims; result register 8 s + 4 a + j is row 32 s + 16 a + 8 b + 4 h + j, query r;
+//   S^T, b = 0, 1: A = rows 32 s + 16 a + 8 b + i, dims 32 h ..; B = query r, the same dims;
+//     result register 8 s + 4 a + j is row 32 s + 16 a + 8 b + 4 h + j, query r;
 //   O^T, D = 0, 1, step (s, a): A = dim 32 x + 16 D + i (r = 16 x + i), rows 32 s + 16 a + 8 b
-//     + 4 h + j; B = those probabilities, where they are; result register 8 x + 4 y + j is
+//     + 4 h + j; B = those weights, where they are; result register 8 x + 4 y + j is
 //     dim 32 x + 16 D + 8 y + 4 h + j, query r.
 template <typename T, int NJ, bool SPLIT>
 __global__ __launch_bounds__(kWaves * 64, 2) void icl4_wide_kernel(AttendArgs p) {
     constexpr bool PAIRS = sizeof(T) == 4;
+    constexpr int PARTS = PAIRS ? 5 : 4;
     __shared__ float red_o[kWaves][32 * NJ * kWideStride];
     __shared__ float red_m[kWaves][32 * NJ], red_l[kWaves][32 * NJ];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -1041,34 +1072,35 @@ __global__ __launch_bounds__(kWaves * 64, 2) void icl4_wide_kernel(AttendArgs p)
     const int split = SPLIT ? (int)(share - pair * p.by_splits.d) : 0;
     const int e = (int)divide(pair, p.by_heads), head = pair - e * p.heads;
     const int rows = rows_of(p.lengths, e, p.rows);
-    half8 qh[NJ][4], ql[PAIRS ? NJ : 1][4];
+    u32x6 parts[NJ][PARTS];
     float c[NJ];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
         const int row = min(32 * (NJ * qt + j) + r32, p.q_rows - 1);
         const T *src = static_cast<const T *>(p.q) + e * p.q_est + head * p.q_head + (long long)row * p.q_row + 32 * h;
-        c[j] = p.scale;
-        if constexpr (PAIRS) {
-            float x[32];
-            float m = 0.f;
+        float x[32];
+        load16(src, x);
+        load16(src + 16, x + 16);
+        float m = 0.f;
+        bool finite = true;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const f32x4 v = *reinterpret_cast<const f32x4 *>(src + 4 * i);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) x[4 * i + k] = v[k], m = fmaxf(m, fabsf(v[k]));
-            }
-            const int ex = pair_exponent(halves_max(m));
-            const float up = pow2(ex);
-            c[j] *= pow2(-ex);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] *= up;
-#pragma unroll
-            for (int m4 = 0; m4 < 4; ++m4) pair8(x + 8 * m4, qh[j][m4], ql[j][m4]);
-        } else {
-#pragma unroll
-            for (int m4 = 0; m4 < 4; ++m4) qh[j][m4] = *reinterpret_cast<const half8 *>(src + 8 * m4);
+        for (int i = 0; i < 32; ++i) {
+            m = fmaxf(m, fabsf(x[i]));
+            finite = finite && fabsf(x[i]) <= 3.4028235e38f;
         }
+        m = halves_max(m);
+        const int ex = min(126, 1 - ((int)(__float_as_uint(m) >> 23) - 127));
+        const float up = pow2(ex);
+        f32x16 even, odd;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) even[i] = x[2 * i] * up, odd[i] = x[2 * i + 1] * up;
+        query_parts<PARTS>(even, odd, parts[j]);
+        // A query that is not finite makes NaN of its own scores alone.
+        c[j] = halves_max(finite ? 0.f : 1.f) > 0.f ? NAN : p.scale * pow2(-ex);
     }
+    // The products take exponents from vector registers only.
+    int part_exps = kPartExps, part_exps4 = kPartExps4, one_exp = 127, most_exp = 254;
+    asm volatile("" : "+v"(part_exps), "+v"(part_exps4), "+v"(one_exp), "+v"(most_exp));
     f32x16 o[NJ][2];
     float ref[NJ], l_run[NJ];
 #pragma unroll
@@ -1079,23 +1111,23 @@ __global__ __launch_bounds__(kWaves * 64, 2) void icl4_wide_kernel(AttendArgs p)
 #pragma unroll
             for (int r = 0; r < 16; ++r) o[j][d][r] = 0.f;
     }
-    struct Words {
-        u32x4 k[2];
-        u32x2 v[4];
-        unsigned ke;
-        u32x2 ve;
-    };
     const unsigned char *tiles = p.tiles + (long long)pair * p.blocks * kBlockBytes;
-    const int k_at = x16 * 1024 + (32 * h + i16) * 16, v_at = kValuesAt + (16 * h + i16) * 16 + 8 * x16;
-    const int ke_at = kKeyExpsAt + (16 * h + i16) * 4, ve_at = kValueExpsAt + i16 * 8;
-    auto load = [&](int block, Words &w) {
-        const unsigned char *in = tiles + (long long)block * kBlockBytes;
-        w.k[0] = *reinterpret_cast<const u32x4 *>(in + k_at);
-        w.k[1] = *reinterpret_cast<const u32x4 *>(in + k_at + 256);
+    const unsigned k_at = x16 * 1024 + (32 * h + i16) * 16, v_at = kValuesAt + (16 * h + i16) * 16 + 8 * x16;
+    const unsigned ke_at = kKeyExpsAt + (16 * h + i16) * 4, ve_at = kValueExpsAt + i16 * 8;
+    u32x2 kw[2][2], vw[4];
+    unsigned ke;
+    u32x2 ve;
+    auto load_keys = [&](const unsigned char *in) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) w.v[t] = *reinterpret_cast<const u32x2 *>(in + v_at + 512 * t);
-        w.ke = *reinterpret_cast<const unsigned *>(in + ke_at);
-        w.ve = *reinterpret_cast<const u32x2 *>(in + ve_at);
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) kw[b][n] = *reinterpret_cast<const u32x2 *>(in + k_at + 256 * n + 8 * b);
+        ke = *reinterpret_cast<const unsigned *>(in + ke_at);
+    };
+    auto load_values = [&](const unsigned char *in) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) vw[t] = *reinterpret_cast<const u32x2 *>(in + v_at + 512 * t);
+        ve = *reinterpret_cast<const u32x2 *>(in + ve_at);
     };
     const int end = min(p.blocks, (split + 1) * p.per_split);
     auto find = [&](int &at, unsigned long long &mask) {
@@ -1105,76 +1137,130 @@ __global__ __launch_bounds__(kWaves * 64, 2) void icl4_wide_kernel(AttendArgs p)
         }
         return false;
     };
-    auto process = [&](const Words &w, unsigned long long mask) {
-        const unsigned ke = w.ke >> (16 * x16);
-        const float ks[2] = {scale_byte<0>(ke), scale_byte<1>(ke)};
+    unsigned long long mask = 0;
+    int at = split * p.per_split + wave;
+    bool more = find(at, mask);
+    if (more) load_keys(tiles + (long long)at * kBlockBytes), load_values(tiles + (long long)at * kBlockBytes);
+    // A block's keys are loaded as soon as the one before has its scores, its values once that one has its output.
+    while (more) {
+        const unsigned long long now = mask;
+        at += kWaves;
+        more = find(at, mask);
+        const unsigned char *next = tiles + (long long)at * kBlockBytes;
         f32x16 s[NJ][2];
+        {
+            const int ks = (int)(ke >> (16 * x16));
+            const i32x8 a[2] = {{(int)kw[0][0][0], (int)kw[0][0][1], (int)kw[0][1][0], (int)kw[0][1][1], 0, 0, 0, 0},
+                                {(int)kw[1][0][0], (int)kw[1][0][1], (int)kw[1][1][0], (int)kw[1][1][1], 0, 0, 0, 0}};
+            // Formats 4 (E2M1) and 2 (E2M3); bytes b and n of the exponents.
+#define IRX_PART(j, b, n, exps, byte)                                                                                    \
+    s[j][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[b],                                                      \
+                                                              (i32x8{(int)parts[j][n][0], (int)parts[j][n][1],           \
+                                                                     (int)parts[j][n][2], (int)parts[j][n][3],           \
+                                                                     (int)parts[j][n][4], (int)parts[j][n][5], 0, 0}),   \
+                                                              s[j][b], 4, 2, b, ks, byte, exps)
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
+            for (int j = 0; j < NJ; ++j) {
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
+                for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[j][b][r] = 0.f;
-#pragma unroll
-        for (int m = 0; m < 4; ++m)
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const half8 a = codes8(w.k[m >> 1][2 * b + (m & 1)], ks[b]);
-#pragma unroll
-                for (int j = 0; j < NJ; ++j) {
-                    if constexpr (PAIRS) s[j][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[j][m], s[j][b], 0, 0, 0);
-                    s[j][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[j][m], s[j][b], 0, 0, 0);
+                    for (int r = 0; r < 16; ++r) s[j][b][r] = 0.f;
+                if constexpr (PAIRS) {
+                    IRX_PART(j, 0, 4, part_exps4, 0);
+                    IRX_PART(j, 1, 4, part_exps4, 0);
                 }
+                IRX_PART(j, 0, 3, part_exps, 3);
+                IRX_PART(j, 1, 3, part_exps, 3);
+                IRX_PART(j, 0, 2, part_exps, 2);
+                IRX_PART(j, 1, 2, part_exps, 2);
+                IRX_PART(j, 0, 1, part_exps, 1);
+                IRX_PART(j, 1, 1, part_exps, 1);
+                IRX_PART(j, 0, 0, part_exps, 0);
+                IRX_PART(j, 1, 0, part_exps, 0);
             }
-        if (mask != ~0ull) {
-            const unsigned long long mine = mask >> (4 * h);
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (!((mine >> (32 * (r >> 3) + 16 * ((r >> 2) & 1) + 8 * b + (r & 3))) & 1))
-#pragma unroll
-                        for (int j = 0; j < NJ; ++j) s[j][b][r] = -INFINITY;
+#undef IRX_PART
         }
+        if (now != ~0ull) {
+            // Rows that are not attended: one more product, of -6 * 2^127 in their first term by 1, makes -inf of
+            // their scores.
+            const unsigned bits = x16 ? (unsigned)(now >> 32) : (unsigned)now;
+            const int r = r32 & 15, first = r + (r & 8);  // 16 a + i
+            const i32x8 one = {h ? 0 : 8, 0, 0, 0, 0, 0, 0, 0};
+            const i32x8 a0 = {h || (bits >> first & 1) ? 0 : 15, 0, 0, 0, 0, 0, 0, 0};
+            const i32x8 a1 = {h || (bits >> (first + 8) & 1) ? 0 : 15, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                s[j][0] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a0, one, s[j][0], 4, 2, 0, most_exp, 0, one_exp);
+                s[j][1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a1, one, s[j][1], 4, 2, 0, most_exp, 0, one_exp);
+            }
+        }
+        if (more) load_keys(next);
         half8 ph[NJ][4], pl[PAIRS ? NJ : 1][4];
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            float mt = s[j][0][0];
+            // The query's weights against its reference, and the lane's sum of them.
+            auto weigh = [&] {
+                float l = 0.f;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) mt = fmaxf(mt, fmaxf(s[j][0][r], s[j][1][r]));
-            // The reference is raised when a probability could pass 2^15: each query's by
-            // its own scores alone, whatever the others of its wave do.
-            if (__any(!(mt * c[j] - ref[j] <= 15.0f))) {
-                const float top = halves_max(mt) * c[j];
-                const float ref_new = top - ref[j] <= 15.0f ? ref[j] : fmaxf(ref[j], top - kHeadroom);
+                for (int t = 0; t < 4; ++t) {
+                    float x[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        x[i] = __builtin_amdgcn_exp2f(fmaf(s[j][i >> 2][4 * t + (i & 3)], c[j], -ref[j]));
+                        l += x[i];
+                    }
+                    if constexpr (PAIRS)
+                        pair8(x, ph[j][t], pl[j][t]);
+                    else
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const half2v w = __builtin_convertvector((f32x2{x[2 * i], x[2 * i + 1]}), half2v);
+                            ph[j][t][2 * i] = w[0], ph[j][t][2 * i + 1] = w[1];
+                        }
+                }
+                return l;
+            };
+            auto largest = [&] {
+                float mt = s[j][0][0];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) mt = fmaxf(mt, fmaxf(s[j][0][r], s[j][1][r]));
+                return mt;
+            };
+            // Raises the reference of the queries of which `past` says so, each by its own scores alone, whatever the
+            // others of its wave do.
+            auto raise = [&](bool past, float mt) {
+                const bool fits = halves_max(past ? 1.f : 0.f) == 0.f;
+                const float ref_new = fits ? ref[j] : fmaxf(ref[j], halves_max(mt) * c[j] - kHeadroom);
                 const float alpha = __builtin_amdgcn_exp2f(ref[j] - ref_new);
                 ref[j] = ref_new;
                 l_run[j] *= alpha;
 #pragma unroll
                 for (int d = 0; d < 2; ++d) o[j][d] *= alpha;
-            }
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                float x[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    x[i] = __builtin_amdgcn_exp2f(fmaf(s[j][i >> 2][4 * t + (i & 3)], c[j], -ref[j]));
-                    l_run[j] += x[i];
+            };
+            // A weight must not pass FP16. FP16 weights leave registers for the scores, so the sum of the weights, at
+            // most 2^15, tells; FP32's pairs take their place, so the largest score is looked for first.
+            float l;
+            if constexpr (PAIRS) {
+                const float mt = largest();
+                const bool past = !(mt * c[j] - ref[j] <= 15.0f);
+                if (__any(past)) raise(past, mt);
+                l = weigh();
+            } else {
+                l = weigh();
+                const bool past = !(l <= 32768.0f);
+                if (__any(past)) {
+                    raise(past, largest());
+                    l = weigh();
                 }
-                if constexpr (PAIRS) {
-                    pair8(x, ph[j][t], pl[j][t]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) ph[j][t][i] = (_Float16)x[i];
-                }
             }
+            l_run[j] += l;
         }
 #pragma unroll
         for (int t = 0; t < 4; ++t) {  // t = 2 s + a
-            const unsigned ve = w.ve[t >> 1] >> (16 * x16);
+            const unsigned v = ve[t >> 1] >> (16 * x16);
 #pragma unroll
             for (int d = 0; d < 2; ++d) {
-                const half8 a = codes8(w.v[t][d], d ? scale_byte<1>(ve) : scale_byte<0>(ve));
+                const half8 a = codes8(vw[t][d], d ? scale_byte<1>(v) : scale_byte<0>(v));
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
                     if constexpr (PAIRS) o[j][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[j][t], o[j][d], 0, 0, 0);
@@ -1182,22 +1268,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void icl4_wide_kernel(AttendArgs p)
                 }
             }
         }
-    };
-    Words wa, wb;
-    unsigned long long mask_a = 0, mask_b = 0;
-    int at = split * p.per_split + wave;
-    bool more = find(at, mask_a);
-    if (more) load(at, wa);
-    while (more) {
-        at += kWaves;
-        more = find(at, mask_b);
-        if (more) load(at, wb);
-        process(wa, mask_a);
-        if (!more) break;
-        at += kWaves;
-        more = find(at, mask_a);
-        if (more) load(at, wa);
-        process(wb, mask_b);
+        if (more) load_values(next);
     }
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
@@ -1250,8 +1321,6 @@ template <int N>
 __device__ __forceinline__ unsigned row_lane(unsigned x) {
     return __builtin_amdgcn_update_dpp(0, x, 0x150 + N, 0xf, 0xf, true);
 }
-
-typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 // One query per workgroup, its blocks (listed, or all) in turn over the waves.
 //
