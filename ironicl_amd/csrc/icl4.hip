@@ -832,6 +832,9 @@ struct AttendArgs {
     int splits, per_split;  // blocks (or listed places) of a split
     int qtiles, count, per_xcd;
     Division by_qtiles, by_splits, by_queries, by_heads;
+    int whole, unit_rows;  // units that are not split; rows of a split unit (0: partials of every row)
+    Division by_rest;      // units that are
+    long long part_rows;   // rows of a split's partials
 };
 
 constexpr float kLn2 = 0.69314718055994530942f;
@@ -841,8 +844,7 @@ constexpr float kHeadroom = 8.0f;
 
 // The writer of one query's output: dims d .. +3.
 template <typename T>
-__device__ __forceinline__ void store_out(const AttendArgs &p, int pair, int row, int d, f32x4 v) {
-    const int e = pair / p.heads, head = pair - e * p.heads;
+__device__ __forceinline__ void store_out(const AttendArgs &p, int e, int head, int row, int d, f32x4 v) {
     T *dst = static_cast<T *>(p.o) + e * p.o_est + head * p.o_head + row * p.o_row + d;
     if constexpr (sizeof(T) == 4) {
         *reinterpret_cast<f32x4 *>(dst) = v;
@@ -998,7 +1000,7 @@ __global__ __launch_bounds__(kWaves * 64) void icl4_rows_kernel(AttendArgs p) {
         *reinterpret_cast<f32x4 *>(p.partial + at * 64 + d) = acc;
         if (d == 0) p.partial[p.splits * all * 64 + at] = lse2;
     } else {
-        store_out<T>(p, pair, out_row, d, acc);
+        store_out<T>(p, e, head, out_row, d, acc);
         if (p.lse && d == 0) p.lse[(long long)pair * p.q_rows + out_row] = lse2 * kLn2;
     }
 }
@@ -1020,24 +1022,23 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef unsigned u32x6 __attribute__((ext_vector_type(6)));
 typedef float f32x32 __attribute__((ext_vector_type(32)));
 
-// 32 numbers, scaled by a power of two so that the largest of the row is in [2,
-// 4), as PARTS operands in E2M3 (multiples of 1/8 below 2, of 1/4 below 4): x = p0
-// + p1 / 2^4 + p2 / 2^9 + ..., each part the nearest to what is left, which is at
-// most 1/8 (then 1/16) and is scaled up to 2 again: five bits a part, 2^-20 of
-// the largest after four and 2^-25 after five. The exponent bytes of parts 0
-// to 3 and of part 4: 16^-1, then 32^-1 each.
+// 32 numbers as PARTS operands in E2M3 (multiples of 1/8 below 2, of 1/4 below
+// 4): x = unit (p0 + p1 / 2^4 + p2 / 2^9 + ...), the unit a power of two that
+// brings the largest of the row into [2, 4), each part the nearest to what is
+// left, at most 1/8 (then 1/16) of its own unit's 2: five bits a part, 2^-20 of
+// the largest after four and 2^-25 after five. The exponent bytes of parts 0 to
+// 3 and of part 4: 16^-1, then 32^-1 each.
 constexpr int kPartExps = 127 | (127 - 4) << 8 | (127 - 9) << 16 | (127 - 14) << 24, kPartExps4 = 127 - 19;
 template <int PARTS>
-__device__ __forceinline__ void query_parts(f32x16 &even, f32x16 &odd, u32x6 (&parts)[PARTS]) {
+__device__ __forceinline__ void query_parts(f32x16 &even, f32x16 &odd, float unit, u32x6 (&parts)[PARTS]) {
 #pragma unroll
     for (int n = 0; n < PARTS; ++n) {
-        parts[n] = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, 1.0f);
+        parts[n] = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, unit);
         if (n == PARTS - 1) break;
-        const f32x32 held = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(parts[n], 1.0f);
-        const float up = n == 0 ? 16.f : 32.f;
+        const f32x32 held = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(parts[n], unit);
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-            even[i] = (even[i] - held[2 * i]) * up, odd[i] = (odd[i] - held[2 * i + 1]) * up;
+        for (int i = 0; i < 16; ++i) even[i] -= held[2 * i], odd[i] -= held[2 * i + 1];
+        unit *= n == 0 ? 0.0625f : 0.03125f;
     }
 }
 
@@ -1056,7 +1057,9 @@ __device__ __forceinline__ void query_parts(f32x16 &even, f32x16 &odd, u32x6 (&p
 //   O^T, D = 0, 1, step (s, a): A = dim 32 x + 16 D + i (r = 16 x + i), rows 32 s + 16 a + 8 b
 //     + 4 h + j; B = those weights, where they are; result register 8 x + 4 y + j is
 //     dim 32 x + 16 D + 8 y + 4 h + j, query r.
-template <typename T, int NJ, bool SPLIT>
+// Workgroups 0 .. whole - 1 take every block for a (query tile, pair) and write
+// its output; the later ones take a split each of the units left over.
+template <typename T, int NJ>
 __global__ __launch_bounds__(kWaves * 64, 2) void icl4_wide_kernel(AttendArgs p) {
     constexpr bool PAIRS = sizeof(T) == 4;
     constexpr int PARTS = PAIRS ? 5 : 4;
@@ -1064,12 +1067,15 @@ __global__ __launch_bounds__(kWaves * 64, 2) void icl4_wide_kernel(AttendArgs p)
     __shared__ float red_m[kWaves][32 * NJ], red_l[kWaves][32 * NJ];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int h = lane >> 5, r32 = lane & 31, i16 = lane & 15, x16 = (lane >> 4) & 1;
-    // Workgroups of one XCD take consecutive query tiles of one share of the blocks, read into one L2.
-    const unsigned id = (blockIdx.x & 7u) * (unsigned)p.per_xcd + (blockIdx.x >> 3);
-    if (id >= (unsigned)p.count) return;
-    const unsigned share = divide(id, p.by_qtiles);
-    const int qt = (int)(id - share * p.by_qtiles.d), pair = SPLIT ? (int)divide(share, p.by_splits) : (int)share;
-    const int split = SPLIT ? (int)(share - pair * p.by_splits.d) : 0;
+    // Workgroups of one XCD take consecutive query tiles of one pair (or share of its blocks), read into one L2.
+    const bool tail = blockIdx.x >= (unsigned)p.whole;
+    const unsigned bid = tail ? blockIdx.x - p.whole : blockIdx.x, per_xcd = tail ? p.per_xcd : p.whole >> 3;
+    const unsigned id = (bid & 7u) * per_xcd + (bid >> 3);
+    if (tail && id >= (unsigned)p.count) return;
+    // A tail's order is pair, split, query tile, as far as its units go: unit = whole + id % rest.
+    const int split = tail ? (int)divide(id, p.by_rest) : 0;
+    const int unit = tail ? p.whole + (int)(id - split * p.by_rest.d) : (int)id;
+    const int pair = (int)divide(unit, p.by_qtiles), qt = unit - pair * p.by_qtiles.d;
     const int e = (int)divide(pair, p.by_heads), head = pair - e * p.heads;
     const int rows = rows_of(p.lengths, e, p.rows);
     u32x6 parts[NJ][PARTS];
@@ -1081,22 +1087,19 @@ __global__ __launch_bounds__(kWaves * 64, 2) void icl4_wide_kernel(AttendArgs p)
         float x[32];
         load16(src, x);
         load16(src + 16, x + 16);
-        float m = 0.f;
-        bool finite = true;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            m = fmaxf(m, fabsf(x[i]));
-            finite = finite && fabsf(x[i]) <= 3.4028235e38f;
-        }
-        m = halves_max(m);
-        const int ex = min(126, 1 - ((int)(__float_as_uint(m) >> 23) - 127));
-        const float up = pow2(ex);
+        float m = 0.f, nan = 0.f;
         f32x16 even, odd;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) even[i] = x[2 * i] * up, odd[i] = x[2 * i + 1] * up;
-        query_parts<PARTS>(even, odd, parts[j]);
+        for (int i = 0; i < 16; ++i) {
+            even[i] = x[2 * i], odd[i] = x[2 * i + 1];
+            m = fmaxf(m, fmaxf(fabsf(even[i]), fabsf(odd[i])));
+            nan = fmaf(odd[i], 0.f, fmaf(even[i], 0.f, nan));
+        }
+        // The least unit leaves 2^-19 of it normal.
+        const int ex = max(-100, (int)(__float_as_uint(halves_max(m)) >> 23) - 128);
+        query_parts<PARTS>(even, odd, pow2(ex), parts[j]);
         // A query that is not finite makes NaN of its own scores alone.
-        c[j] = halves_max(finite ? 0.f : 1.f) > 0.f ? NAN : p.scale * pow2(-ex);
+        c[j] = p.scale * pow2(ex) + halves_sum(nan);
     }
     // The products take exponents from vector registers only.
     int part_exps = kPartExps, part_exps4 = kPartExps4, one_exp = 127, most_exp = 254;
@@ -1129,7 +1132,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void icl4_wide_kernel(AttendArgs p)
         for (int t = 0; t < 4; ++t) vw[t] = *reinterpret_cast<const u32x2 *>(in + v_at + 512 * t);
         ve = *reinterpret_cast<const u32x2 *>(in + ve_at);
     };
-    const int end = min(p.blocks, (split + 1) * p.per_split);
+    const int end = tail ? min(p.blocks, (split + 1) * p.per_split) : p.blocks;
     auto find = [&](int &at, unsigned long long &mask) {
         for (; at < end; at += kWaves) {
             mask = block_mask(p.keep, e, p.blocks, at, rows);
@@ -1300,13 +1303,13 @@ __global__ __launch_bounds__(kWaves * 64, 2) void icl4_wide_kernel(AttendArgs p)
         }
         if (den != 0.f) acc *= 1.0f / den;
         const float lse2 = mx + log2f(den);
-        const long long all = (long long)p.pairs * p.q_rows, pq = (long long)pair * p.q_rows + row;
-        if constexpr (SPLIT) {
-            *reinterpret_cast<f32x4 *>(p.partial + (split * all + pq) * 64 + d) = acc;
-            if (d == 0) p.partial[p.splits * all * 64 + split * all + pq] = lse2;
+        if (tail && p.splits > 1) {
+            const long long all = (long long)p.by_rest.d * (32 * NJ), to = split * all + (long long)(unit - p.whole) * (32 * NJ) + q;
+            *reinterpret_cast<f32x4 *>(p.partial + to * 64 + d) = acc;
+            if (d == 0) p.partial[p.splits * all * 64 + to] = lse2;
         } else {
-            store_out<T>(p, pair, row, d, acc);
-            if (p.lse && d == 0) p.lse[pq] = lse2 * kLn2;
+            store_out<T>(p, e, head, row, d, acc);
+            if (p.lse && d == 0) p.lse[(long long)pair * p.q_rows + row] = lse2 * kLn2;
         }
     }
 }
@@ -1534,7 +1537,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void icl4_one_kernel(AttendArgs p) {
         *reinterpret_cast<f32x4 *>(p.partial + to * 64 + d) = acc;
         if (d == 0) p.partial[p.splits * all * 64 + to] = lse2;
     } else {
-        store_out<T>(p, pair, row, d, acc);
+        store_out<T>(p, e, head, row, d, acc);
         if (p.lse && d == 0) p.lse[pq] = lse2 * kLn2;
     }
 }
@@ -1544,12 +1547,12 @@ __global__ __launch_bounds__(WAVES * 64, 4) void icl4_one_kernel(AttendArgs p) {
 template <typename T, int GROUPS>
 __global__ __launch_bounds__(256) void icl4_merge_kernel(AttendArgs p) {
     __shared__ float sums[GROUPS > 1 ? 16 * 66 : 1];
-    const long long all = (long long)p.pairs * p.q_rows;
+    const long long all = p.part_rows;
     const int tid = threadIdx.x, slot = tid >> 4, group = slot % GROUPS, d = 4 * (tid & 15);
     const long long mine = (long long)blockIdx.x * (16 / GROUPS) + slot / GROUPS;
-    const long long pq = min(mine, all - 1);
-    const float *lse = p.partial + p.splits * all * 64 + pq;
-    const float *part = p.partial + pq * 64 + d;
+    const long long at_row = min(mine, all - 1);
+    const float *lse = p.partial + p.splits * all * 64 + at_row;
+    const float *part = p.partial + at_row * 64 + d;
     // Eight splits' loads at once; slots past the last read it again and weigh nothing.
     float ref = -INFINITY, den = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -1598,18 +1601,33 @@ __global__ __launch_bounds__(256) void icl4_merge_kernel(AttendArgs p) {
         ref = top;
     }
     if (mine >= all) return;
+    int pair, row;
+    if (p.unit_rows) {
+        // A unit's rows, some past the last query.
+        const unsigned of = (unsigned)mine, shift = p.unit_rows == 64 ? 6 : 5;
+        const int unit = p.whole + (int)(of >> shift);
+        pair = (int)divide(unit, p.by_qtiles);
+        row = (unit - pair * (int)p.by_qtiles.d) * p.unit_rows + (int)(of & (p.unit_rows - 1u));
+        if (row >= p.q_rows) return;
+    } else {
+        pair = (int)divide((unsigned)mine, p.by_queries), row = (int)mine - pair * p.q_rows;
+    }
     if (den != 0.f) acc *= 1.0f / den;
-    const int pair = (int)(pq / p.q_rows), row = (int)(pq - (long long)pair * p.q_rows);
-    store_out<T>(p, pair, row, d, acc);
+    const int e = (int)divide(pair, p.by_heads);
+    store_out<T>(p, e, pair - e * p.heads, row, d, acc);
     // Nothing attended: log 0.
-    if (p.lse && d == 0) p.lse[pq] = ((ref > -INFINITY ? ref : 0.f) + log2f(den)) * kLn2;
+    if (p.lse && d == 0)
+        p.lse[(long long)pair * p.q_rows + row] = ((ref > -INFINITY ? ref : 0.f) + log2f(den)) * kLn2;
 }
 
 struct Plan {
     int queries;  // of a workgroup: 1, 16, 32 or 64
     int waves;    // of a workgroup of one query: 1, 4 or 16
     int qtiles, splits, per_split;
-    long long rows;  // (pair, query) rows
+    long long rows;       // (pair, query) rows
+    long long whole;      // 32 or 64 queries: units (query tile, pair) that are not split
+    long long rest;       // and those that are
+    long long part_rows;  // rows of a split's partials
 };
 
 // Listed blocks up to which few queries take sixteen waves each rather than splits of four and a merge.
@@ -1626,7 +1644,7 @@ Plan plan_attend(const Icl4Shape &s, int q_rows, int n_blocks, int compute_units
     const int places = n_blocks ? n_blocks : s.blocks();
     pl.queries = n_blocks || q_rows <= kOneQueries ? 1 : q_rows <= 16 ? 16 : q_rows <= 32 ? 32 : 64;
     pl.qtiles = (int)ceil_div(q_rows, pl.queries);
-    pl.rows = (long long)s.pairs() * q_rows;
+    pl.rows = pl.part_rows = (long long)s.pairs() * q_rows;
     pl.waves = kWaves;
     const long long base = (long long)s.pairs() * pl.qtiles;
     if (n_blocks && n_blocks <= kUnsplitBlocks && n_blocks > kWaves && base < 2LL * compute_units) {
@@ -1642,14 +1660,17 @@ Plan plan_attend(const Icl4Shape &s, int q_rows, int n_blocks, int compute_units
     if (pl.queries <= 16) {
         splits = std::min(std::max(1LL, (slots + base - 1) / base), tiles);
     } else {
+        // Whole rounds of workgroups take every block; the units left over are split where that is quicker.
         // Microseconds: a workgroup's start and end, each round of its waves' blocks, the merge.
+        pl.whole = base / slots * slots / 8 * 8, pl.rest = base - pl.whole;
         double best = 1e30;
-        for (long long n = 1; n <= std::min(tiles, std::max(8LL, 2 * slots / base)); ++n) {
-            const double rounds = (double)((base * n + slots - 1) / slots);
-            const double merge = n > 1 ? 4.0 + (double)pl.rows * (double)n * (520.0 / 4e6) : 0.0;
-            const double cost = rounds * (6.0 + 1.5 * (double)((tiles + n - 1) / n)) + merge;
+        for (long long n = 1; pl.rest && n <= std::min(tiles, std::max(8LL, 2 * slots / pl.rest)); ++n) {
+            const double rounds = (double)((pl.rest * n + slots - 1) / slots);
+            const double merge = n > 1 ? 4.0 + (double)pl.rest * pl.queries * (double)n * (520.0 / 4e6) : 0.0;
+            const double cost = rounds * (6.0 + 2.0 * (double)((tiles + n - 1) / n)) + merge;
             if (cost < best) best = cost, splits = n;
         }
+        pl.part_rows = pl.rest * pl.queries;
     }
     pl.per_split = (int)((tiles + splits - 1) / splits) * kWaves;
     pl.splits = (int)ceil_div(places, pl.per_split);
@@ -1700,11 +1721,13 @@ void attend(const Icl4Queries &a, const Icl4Attend &b, hipStream_t stream) {
     p.list = b.list, p.n = b.n, p.heads = s.heads, p.pairs = s.pairs(), p.q_rows = a.q_rows, p.rows = s.rows;
     p.blocks = s.blocks(), p.scale = b.scale * kLog2e, p.partial = static_cast<float *>(b.workspace);
     p.splits = pl.splits, p.per_split = pl.per_split, p.qtiles = pl.qtiles;
-    const long long count = (long long)pl.splits * pl.qtiles * s.pairs();
+    const bool wide = pl.queries > 16;
+    const long long count = (wide ? pl.rest : (long long)pl.qtiles * s.pairs()) * pl.splits;
     p.count = (int)count, p.per_xcd = (int)ceil_div((size_t)count, 8);
     p.by_qtiles = division(pl.qtiles), p.by_splits = division(pl.splits), p.by_queries = division(a.q_rows);
-    p.by_heads = division(s.heads);
-    const dim3 grid((unsigned)(pl.queries == 16 ? count : 8LL * p.per_xcd)), wg(kWaves * 64);
+    p.by_heads = division(s.heads), p.by_rest = division(std::max(1LL, pl.rest));
+    p.whole = (int)pl.whole, p.unit_rows = wide ? pl.queries : 0, p.part_rows = pl.part_rows;
+    const dim3 grid((unsigned)(pl.queries == 16 ? count : pl.whole + 8LL * p.per_xcd)), wg(kWaves * 64);
     {
         const long long tiles = b.list ? (long long)pl.rows * b.n : (long long)s.pairs() * s.blocks();
         const double work = 256.0 * kBlock * (b.list ? (double)tiles : (double)tiles * a.q_rows);
@@ -1726,25 +1749,21 @@ void attend(const Icl4Queries &a, const Icl4Attend &b, hipStream_t stream) {
             hipLaunchKernelGGL((icl4_rows_kernel<T, true>), grid, wg, 0, stream, p);
         else if (pl.queries == 16)
             hipLaunchKernelGGL((icl4_rows_kernel<T, false>), grid, wg, 0, stream, p);
-        else if (pl.queries == 32 && split)
-            hipLaunchKernelGGL((icl4_wide_kernel<T, 1, true>), grid, wg, 0, stream, p);
         else if (pl.queries == 32)
-            hipLaunchKernelGGL((icl4_wide_kernel<T, 1, false>), grid, wg, 0, stream, p);
-        else if (split)
-            hipLaunchKernelGGL((icl4_wide_kernel<T, 2, true>), grid, wg, 0, stream, p);
+            hipLaunchKernelGGL((icl4_wide_kernel<T, 1>), grid, wg, 0, stream, p);
         else
-            hipLaunchKernelGGL((icl4_wide_kernel<T, 2, false>), grid, wg, 0, stream, p);
+            hipLaunchKernelGGL((icl4_wide_kernel<T, 2>), grid, wg, 0, stream, p);
         IRX_HIP(hipGetLastError());
     }
     if (pl.splits > 1) {
-        KernelTimer timer(kFamIclMerge, stream, 0.0, 4.0 * pl.rows * (65.0 * pl.splits + 64.0));
+        KernelTimer timer(kFamIclMerge, stream, 0.0, 4.0 * pl.part_rows * (65.0 * pl.splits + 64.0));
         // A lane's splits come eight at a time: more groups where there are more splits.
         if (pl.splits <= 8)
-            hipLaunchKernelGGL((icl4_merge_kernel<T, 1>), dim3(ceil_div((size_t)pl.rows, 16)), dim3(256), 0, stream, p);
+            hipLaunchKernelGGL((icl4_merge_kernel<T, 1>), dim3(ceil_div((size_t)pl.part_rows, 16)), dim3(256), 0, stream, p);
         else if (pl.splits <= 32)
-            hipLaunchKernelGGL((icl4_merge_kernel<T, 4>), dim3(ceil_div((size_t)pl.rows, 4)), dim3(256), 0, stream, p);
+            hipLaunchKernelGGL((icl4_merge_kernel<T, 4>), dim3(ceil_div((size_t)pl.part_rows, 4)), dim3(256), 0, stream, p);
         else
-            hipLaunchKernelGGL((icl4_merge_kernel<T, 16>), dim3((unsigned)pl.rows), dim3(256), 0, stream, p);
+            hipLaunchKernelGGL((icl4_merge_kernel<T, 16>), dim3((unsigned)pl.part_rows), dim3(256), 0, stream, p);
         IRX_HIP(hipGetLastError());
     }
 }
@@ -1757,7 +1776,7 @@ size_t icl4_bytes(const Icl4Shape &s) {
 
 size_t icl4_attend_workspace(const Icl4Shape &s, int q_rows, int n_blocks, int compute_units) {
     const Plan pl = plan_attend(s, q_rows, n_blocks, compute_units);
-    return pl.splits > 1 ? (size_t)pl.splits * (size_t)pl.rows * 65 * sizeof(float) : 0;
+    return pl.splits > 1 ? (size_t)pl.splits * (size_t)pl.part_rows * 65 * sizeof(float) : 0;
 }
 
 size_t icl4_select_workspace(const Icl4Shape &s, int q_rows) {
@@ -1771,7 +1790,8 @@ bool icl4_select_fits(const Icl4Shape &s, int q_rows) {
 
 bool icl4_grid_fits(const Icl4Shape &s, int q_rows, int n_blocks, int compute_units) {
     const Plan pl = plan_attend(s, q_rows, n_blocks, compute_units);
-    return (double)pl.splits * pl.qtiles * s.pairs() < 8388608.0;
+    const double units = pl.queries > 16 ? (double)pl.whole + (double)pl.rest * pl.splits : (double)pl.splits * pl.qtiles * s.pairs();
+    return (units + 8) * pl.waves * 64 < 4294967296.0 && (double)pl.part_rows < 2147483648.0;
 }
 
 void icl4_encode(const Icl4Rows &a, void *cache, unsigned *nonfinite, hipStream_t stream) {
