@@ -494,11 +494,11 @@ struct Icl4Attend {
     void *workspace;
 };
 size_t icl4_bytes(const Icl4Shape &s);
-size_t icl4_attend_workspace(const Icl4Shape &s, int q_rows, int n_blocks, int compute_units);
+size_t icl4_attend_workspace(const Icl4Shape &s, bool half, int q_rows, int n_blocks, int compute_units);
 size_t icl4_select_workspace(const Icl4Shape &s, int q_rows);
 // Whether the choice's, and the attention's, workgroups can be one launch.
 bool icl4_select_fits(const Icl4Shape &s, int q_rows);
-bool icl4_grid_fits(const Icl4Shape &s, int q_rows, int n_blocks, int compute_units);
+bool icl4_grid_fits(const Icl4Shape &s, bool half, int q_rows, int n_blocks, int compute_units);
 void icl4_encode(const Icl4Rows &a, void *cache, unsigned *nonfinite, hipStream_t stream);
 // a.k and a.v (either may be null) are written.
 void icl4_decode(const Icl4Rows &a, const void *cache, float *bounds, hipStream_t stream);

@@ -838,9 +838,13 @@ struct AttendArgs {
 };
 
 constexpr float kLn2 = 0.69314718055994530942f;
-// Probabilities are held against a reference 2^8 below the largest so far, so
-// that FP16's smallest step, 2^-24, is 2^-32 of the largest.
-constexpr float kHeadroom = 8.0f;
+// Weights are held against a reference below the largest so far, so that FP16's
+// smallest step, 2^-24, is small beside the largest weight: 2^-32 of it where a
+// reference is cheap to raise. The wide kernels raise theirs when weights pass
+// 2^15 or so, which costs them most of a block's work: with 2^5 (FP16) and 2^6
+// (FP32) 1.2 and 1.7 times in a wave's 40 blocks of 10,007 rows, with 2^8 4.9
+// times; a weight is then off by at most 2^-30 and 2^-31 of the largest.
+constexpr float kHeadroom = 8.0f, kWideHeadroom16 = 5.0f, kWideHeadroom32 = 6.0f;
 
 // The writer of one query's output: dims d .. +3.
 template <typename T>
@@ -1060,7 +1064,7 @@ __device__ __forceinline__ void query_parts(f32x16 &even, f32x16 &odd, float uni
 // Workgroups 0 .. whole - 1 take every block for a (query tile, pair) and write
 // its output; the later ones take a split each of the units left over.
 template <typename T, int NJ>
-__global__ __launch_bounds__(kWaves * 64, 2) void icl4_wide_kernel(AttendArgs p) {
+__global__ __launch_bounds__(kWaves * 64, NJ == 1 ? 3 : 2) void icl4_wide_kernel(AttendArgs p) {
     constexpr bool PAIRS = sizeof(T) == 4;
     constexpr int PARTS = PAIRS ? 5 : 4;
     __shared__ float red_o[kWaves][32 * NJ * kWideStride];
@@ -1233,7 +1237,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void icl4_wide_kernel(AttendArgs p)
             // others of its wave do.
             auto raise = [&](bool past, float mt) {
                 const bool fits = halves_max(past ? 1.f : 0.f) == 0.f;
-                const float ref_new = fits ? ref[j] : fmaxf(ref[j], halves_max(mt) * c[j] - kHeadroom);
+                const float ref_new = fits ? ref[j] : fmaxf(ref[j], halves_max(mt) * c[j] - (PAIRS ? kWideHeadroom32 : kWideHeadroom16));
                 const float alpha = __builtin_amdgcn_exp2f(ref[j] - ref_new);
                 ref[j] = ref_new;
                 l_run[j] *= alpha;
@@ -1638,11 +1642,18 @@ constexpr int kManyQueries = 16;
 // Queries up to which attention over every block takes a workgroup per query.
 constexpr int kOneQueries = 1;
 
-// About two workgroups per compute unit, at least four blocks to a split (one to a wave).
-Plan plan_attend(const Icl4Shape &s, int q_rows, int n_blocks, int compute_units) {
+// About two workgroups per compute unit, at least four blocks to a split (one to
+// a wave). Above 16 queries a workgroup takes 32, three to a compute unit (168
+// registers), or 64, two (256): FP16 queries 64 where that makes a whole round
+// of workgroups (10,007 queries x 10,007 rows 237 against 248 us; 777 x 12,345 x
+// 2 estimators, 208 workgroups, 70.3 against 68.2), FP32 ones, whose pairs do not
+// fit 256 registers beside 64 queries' scores, never (512 x 50,000 111 against
+// 106.6 us).
+Plan plan_attend(const Icl4Shape &s, bool half, int q_rows, int n_blocks, int compute_units) {
     Plan pl{};
     const int places = n_blocks ? n_blocks : s.blocks();
-    pl.queries = n_blocks || q_rows <= kOneQueries ? 1 : q_rows <= 16 ? 16 : q_rows <= 32 ? 32 : 64;
+    const bool full = half && (long long)s.pairs() * ceil_div(q_rows, 64) >= 2LL * compute_units;
+    pl.queries = n_blocks || q_rows <= kOneQueries ? 1 : q_rows <= 16 ? 16 : full ? 64 : 32;
     pl.qtiles = (int)ceil_div(q_rows, pl.queries);
     pl.rows = pl.part_rows = (long long)s.pairs() * q_rows;
     pl.waves = kWaves;
@@ -1655,7 +1666,7 @@ Plan plan_attend(const Icl4Shape &s, int q_rows, int n_blocks, int compute_units
         pl.waves = 1, pl.splits = 1, pl.per_split = n_blocks;
         return pl;
     }
-    const long long slots = 2LL * compute_units, tiles = ceil_div(places, kWaves);
+    const long long slots = (pl.queries == 32 ? 3LL : 2LL) * compute_units, tiles = ceil_div(places, kWaves);
     long long splits = 1;
     if (pl.queries <= 16) {
         splits = std::min(std::max(1LL, (slots + base - 1) / base), tiles);
@@ -1667,7 +1678,7 @@ Plan plan_attend(const Icl4Shape &s, int q_rows, int n_blocks, int compute_units
         for (long long n = 1; pl.rest && n <= std::min(tiles, std::max(8LL, 2 * slots / pl.rest)); ++n) {
             const double rounds = (double)((pl.rest * n + slots - 1) / slots);
             const double merge = n > 1 ? 4.0 + (double)pl.rest * pl.queries * (double)n * (520.0 / 4e6) : 0.0;
-            const double cost = rounds * (6.0 + 2.0 * (double)((tiles + n - 1) / n)) + merge;
+            const double cost = rounds * (6.0 + (pl.queries == 32 ? 1.8 : 2.2) * (double)((tiles + n - 1) / n)) + merge;
             if (cost < best) best = cost, splits = n;
         }
         pl.part_rows = pl.rest * pl.queries;
@@ -1713,7 +1724,7 @@ Parts parts(const void *cache, const Icl4Shape &s) {
 template <typename T>
 void attend(const Icl4Queries &a, const Icl4Attend &b, hipStream_t stream) {
     const Icl4Shape &s = a.shape;
-    const Plan pl = plan_attend(s, a.q_rows, b.list ? b.n : 0, a.compute_units);
+    const Plan pl = plan_attend(s, a.half, a.q_rows, b.list ? b.n : 0, a.compute_units);
     AttendArgs p{};
     p.q = a.q, p.q_est = a.q_strides[0], p.q_head = a.q_strides[1], p.q_row = a.q_strides[2];
     p.o = b.out, p.o_est = b.o_strides[0], p.o_head = b.o_strides[1], p.o_row = b.o_strides[2];
@@ -1774,8 +1785,8 @@ size_t icl4_bytes(const Icl4Shape &s) {
     return (size_t)s.pairs() * ((size_t)s.blocks() * (kBlockBytes + 128) + 64 * sizeof(float));
 }
 
-size_t icl4_attend_workspace(const Icl4Shape &s, int q_rows, int n_blocks, int compute_units) {
-    const Plan pl = plan_attend(s, q_rows, n_blocks, compute_units);
+size_t icl4_attend_workspace(const Icl4Shape &s, bool half, int q_rows, int n_blocks, int compute_units) {
+    const Plan pl = plan_attend(s, half, q_rows, n_blocks, compute_units);
     return pl.splits > 1 ? (size_t)pl.splits * (size_t)pl.part_rows * 65 * sizeof(float) : 0;
 }
 
@@ -1788,8 +1799,8 @@ bool icl4_select_fits(const Icl4Shape &s, int q_rows) {
     return (double)s.pairs() * ceil_div(q_rows, 16) * (kChooseWaves * 64) < 4294967296.0;
 }
 
-bool icl4_grid_fits(const Icl4Shape &s, int q_rows, int n_blocks, int compute_units) {
-    const Plan pl = plan_attend(s, q_rows, n_blocks, compute_units);
+bool icl4_grid_fits(const Icl4Shape &s, bool half, int q_rows, int n_blocks, int compute_units) {
+    const Plan pl = plan_attend(s, half, q_rows, n_blocks, compute_units);
     const double units = pl.queries > 16 ? (double)pl.whole + (double)pl.rest * pl.splits : (double)pl.splits * pl.qtiles * s.pairs();
     return (units + 8) * pl.waves * 64 < 4294967296.0 && (double)pl.part_rows < 2147483648.0;
 }

@@ -2280,7 +2280,9 @@ size_t irx_icl4_workspace_bytes(irx_device *device, const irx_icl4_shape *shape,
     if (!device || !icl4_shape_ok(shape) || !query_rows || query_rows > kIcl4MaxQueries || n_blocks > kIcl4MaxBlocks)
         return 0;
     const Icl4Shape s = icl4_shape(*shape);
-    const size_t attend = icl4_attend_workspace(s, (int)query_rows, (int)n_blocks, device->compute_units);
+    size_t attend = 0;
+    for (const bool half : {false, true})
+        attend = std::max(attend, icl4_attend_workspace(s, half, (int)query_rows, (int)n_blocks, device->compute_units));
     return n_blocks ? std::max(attend, icl4_select_workspace(s, (int)query_rows)) : attend;
 }
 
@@ -2350,9 +2352,9 @@ int irx_icl4_attention(irx_device *device, const irx_icl4_queries *queries, cons
         icl4_aligned(lse, 4, "lse");
         icl4_device(device);
         a.compute_units = device->compute_units;
-        if (!icl4_grid_fits(a.shape, a.q_rows, b.n, a.compute_units))
+        if (!icl4_grid_fits(a.shape, a.half, a.q_rows, b.n, a.compute_units))
             fail(IRX_INVALID_ARGUMENT, "too many queries for one call");
-        icl4_workspace(workspace, workspace_bytes, icl4_attend_workspace(a.shape, a.q_rows, b.n, a.compute_units));
+        icl4_workspace(workspace, workspace_bytes, icl4_attend_workspace(a.shape, a.half, a.q_rows, b.n, a.compute_units));
         CurrentDevice here(device);
         icl4_attend(a, b, static_cast<hipStream_t>(stream));
     });

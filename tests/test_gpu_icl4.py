@@ -7,8 +7,9 @@ are off by at most 2^-22 relative each, a 64-term FP32 sum by 2^-18 of the sum
 of magnitudes A, and FP32's scaling by less: |ds| <= 2^-17 A. A weight exp(s) is
 then off by 2 ds relative, and so is a weighted mean of values up to V by at
 most 4 ds V (numerator and denominator). FP32 weights are pairs (2^-22); FP16
-ones are off by half a step, 2^-11, and below FP16's smallest step by at most
-2^-33 of the largest, N of them. FP32 sums of N / 8 addends (two keys' worth of
+ones are off by half a step, 2^-11, and below FP16's smallest step (half of it
+2^-25, where the largest weight is at least 2^5) by at most 2^-30 of the
+largest, N of them. FP32 sums of N / 8 addends (two keys' worth of
 products in one) add N 2^-27 V at most. FP16 outputs round by 2^-11 of
 themselves. The log-sum-exp is off by 2 ds, N 2^-27 and 2^-22 of itself."""
 
@@ -126,7 +127,7 @@ def check(got, want, element, cache):
     ds = 2.0 ** -17 * magnitude
     n, v = cache.k.shape[2], np.abs(cache.v).max()
     weight = 2.0 ** -21 if element == "f32" else 2.0 ** -10
-    bound = v * (4 * ds + weight + n * 2.0 ** -27 + n * 2.0 ** -32)
+    bound = v * (4 * ds + weight + n * 2.0 ** -27 + n * 2.0 ** -30)
     if element == "f16":
         bound = bound + np.abs(out64) * 2.0 ** -11 + 2.0 ** -25
     assert np.isfinite(out).all()
