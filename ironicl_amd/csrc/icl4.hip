@@ -875,6 +875,35 @@ __global__ __launch_bounds__(kWaves * 64) void icl4_rows_kernel(AttendArgs p) {
     const int e = (int)divide(pair, p.by_heads), head = pair - e * p.heads;
     const int rows = rows_of(p.lengths, e, p.rows);
     const int qrow = min(16 * qt + i16, p.q_rows - 1);
+    // The first block's operands, beneath the queries' setup; then a block's keys are loaded as soon as the one before
+    // has its scores, its values once that one has its output.
+    const unsigned char *tiles = p.tiles + (long long)pair * p.blocks * kBlockBytes;
+    const int end = min(p.blocks, (split + 1) * p.per_split);
+    const unsigned chunk_at = 16u * lane, ke_at = kKeyExpsAt + ((g >> 1) * 16 + i16) * 4, ve_at = kValueExpsAt + i16 * 8;
+    u32x4 kw[2], vw[2];
+    unsigned ke;
+    u32x2 ve;
+    auto load_keys = [&](const unsigned char *in) {
+        kw[0] = *reinterpret_cast<const u32x4 *>(in + chunk_at);
+        kw[1] = *reinterpret_cast<const u32x4 *>(in + 1024 + chunk_at);
+        ke = *reinterpret_cast<const unsigned *>(in + ke_at);
+    };
+    auto load_values = [&](const unsigned char *in) {
+        vw[0] = *reinterpret_cast<const u32x4 *>(in + kValuesAt + chunk_at);
+        vw[1] = *reinterpret_cast<const u32x4 *>(in + kValuesAt + 1024 + chunk_at);
+        ve = *reinterpret_cast<const u32x2 *>(in + ve_at);
+    };
+    auto find = [&](int &at, unsigned long long &mask) {
+        for (; at < end; at += kWaves) {
+            mask = block_mask(p.keep, e, p.blocks, at, rows);
+            if (mask) return true;
+        }
+        return false;
+    };
+    unsigned long long next_mask = 0;
+    int at = split * p.per_split + wave;
+    bool more = find(at, next_mask);
+    if (more) load_keys(tiles + (long long)at * kBlockBytes), load_values(tiles + (long long)at * kBlockBytes);
     half8 qh[2], ql[2];
     float c = p.scale;
     {
@@ -906,19 +935,16 @@ __global__ __launch_bounds__(kWaves * 64) void icl4_rows_kernel(AttendArgs p) {
 #pragma unroll
     for (int d = 0; d < 4; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m_run = -INFINITY, l_run = 0.f;  // m_run: the largest score less the headroom
-    const unsigned char *tiles = p.tiles + (long long)pair * p.blocks * kBlockBytes;
-    const int end = min(p.blocks, (split + 1) * p.per_split);
-    for (int block = split * p.per_split + wave; block < end; block += kWaves) {
-        const unsigned long long mask = block_mask(p.keep, e, p.blocks, block, rows);
-        if (mask == 0) continue;
-        const unsigned char *in = tiles + (long long)block * kBlockBytes;
-        const unsigned ke = *reinterpret_cast<const unsigned *>(in + kKeyExpsAt + ((g >> 1) * 16 + i16) * 4);
-        const u32x2 ve = *reinterpret_cast<const u32x2 *>(in + kValueExpsAt + i16 * 8);
+    while (more) {
+        const unsigned long long mask = next_mask;
+        at += kWaves;
+        more = find(at, next_mask);
+        const unsigned char *next = tiles + (long long)at * kBlockBytes;
         f32x4 s[4];
 #pragma unroll
         for (int kb = 0; kb < 4; ++kb) {
-            const u32x2 w = *reinterpret_cast<const u32x2 *>(in + (kb >> 1) * 1024 + lane * 16 + (kb & 1) * 8);
-            const float scale = __uint_as_float(((ke >> (8 * kb)) & 0xffu) << 23);
+            const unsigned w[2] = {kw[kb >> 1][2 * (kb & 1)], kw[kb >> 1][2 * (kb & 1) + 1]};
+            const float scale = kb == 0 ? scale_byte<0>(ke) : kb == 1 ? scale_byte<1>(ke) : kb == 2 ? scale_byte<2>(ke) : scale_byte<3>(ke);
             s[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
@@ -928,6 +954,7 @@ __global__ __launch_bounds__(kWaves * 64) void icl4_rows_kernel(AttendArgs p) {
             }
             s[kb] *= c;
         }
+        if (more) load_keys(next);
         // Register r of s[2 s + b]: row 32 s + 16 (g / 2) + 8 b + 4 (g % 2) + r.
         if (mask != ~0ull) {
             const unsigned long long mine = mask >> (16 * (g >> 1) + 4 * (g & 1));
@@ -965,14 +992,15 @@ __global__ __launch_bounds__(kWaves * 64) void icl4_rows_kernel(AttendArgs p) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) ph[i] = (_Float16)x[i];
             }
-            const u32x4 w = *reinterpret_cast<const u32x4 *>(in + kValuesAt + st * 1024 + lane * 16);
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
-                const half8 a = codes8(w[d], __uint_as_float(((ve[st] >> (8 * d)) & 0xffu) << 23));
+                const float scale = d == 0 ? scale_byte<0>(ve[st]) : d == 1 ? scale_byte<1>(ve[st]) : d == 2 ? scale_byte<2>(ve[st]) : scale_byte<3>(ve[st]);
+                const half8 a = codes8(vw[st][d], scale);
                 if constexpr (PAIRS) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl, o[d], 0, 0, 0);
                 o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph, o[d], 0, 0, 0);
             }
         }
+        if (more) load_values(next);
     }
     // The waves' parts: lane (g, i16) holds dims 16 d + 4 g + r of query i16.
     l_run += __shfl_xor(l_run, 16, 64);
@@ -1082,6 +1110,36 @@ __global__ __launch_bounds__(kWaves * 64, NJ == 1 ? 3 : 2) void icl4_wide_kernel
     const int pair = (int)divide(unit, p.by_qtiles), qt = unit - pair * p.by_qtiles.d;
     const int e = (int)divide(pair, p.by_heads), head = pair - e * p.heads;
     const int rows = rows_of(p.lengths, e, p.rows);
+    const unsigned char *tiles = p.tiles + (long long)pair * p.blocks * kBlockBytes;
+    const unsigned k_at = x16 * 1024 + (32 * h + i16) * 16, v_at = kValuesAt + (16 * h + i16) * 16 + 8 * x16;
+    const unsigned ke_at = kKeyExpsAt + (16 * h + i16) * 4, ve_at = kValueExpsAt + i16 * 8;
+    u32x2 kw[2][2], vw[4];
+    unsigned ke;
+    u32x2 ve;
+    auto load_keys = [&](const unsigned char *in) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) kw[b][n] = *reinterpret_cast<const u32x2 *>(in + k_at + 256 * n + 8 * b);
+        ke = *reinterpret_cast<const unsigned *>(in + ke_at);
+    };
+    auto load_values = [&](const unsigned char *in) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) vw[t] = *reinterpret_cast<const u32x2 *>(in + v_at + 512 * t);
+        ve = *reinterpret_cast<const u32x2 *>(in + ve_at);
+    };
+    const int end = tail ? min(p.blocks, (split + 1) * p.per_split) : p.blocks;
+    auto find = [&](int &at, unsigned long long &mask) {
+        for (; at < end; at += kWaves) {
+            mask = block_mask(p.keep, e, p.blocks, at, rows);
+            if (mask) return true;
+        }
+        return false;
+    };
+    unsigned long long mask = 0;
+    int at = split * p.per_split + wave;
+    bool more = find(at, mask);
+    if (more) load_keys(tiles + (long long)at * kBlockBytes), load_values(tiles + (long long)at * kBlockBytes);
     u32x6 parts[NJ][PARTS];
     float c[NJ];
 #pragma unroll
@@ -1118,36 +1176,6 @@ __global__ __launch_bounds__(kWaves * 64, NJ == 1 ? 3 : 2) void icl4_wide_kernel
 #pragma unroll
             for (int r = 0; r < 16; ++r) o[j][d][r] = 0.f;
     }
-    const unsigned char *tiles = p.tiles + (long long)pair * p.blocks * kBlockBytes;
-    const unsigned k_at = x16 * 1024 + (32 * h + i16) * 16, v_at = kValuesAt + (16 * h + i16) * 16 + 8 * x16;
-    const unsigned ke_at = kKeyExpsAt + (16 * h + i16) * 4, ve_at = kValueExpsAt + i16 * 8;
-    u32x2 kw[2][2], vw[4];
-    unsigned ke;
-    u32x2 ve;
-    auto load_keys = [&](const unsigned char *in) {
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int n = 0; n < 2; ++n) kw[b][n] = *reinterpret_cast<const u32x2 *>(in + k_at + 256 * n + 8 * b);
-        ke = *reinterpret_cast<const unsigned *>(in + ke_at);
-    };
-    auto load_values = [&](const unsigned char *in) {
-#pragma unroll
-        for (int t = 0; t < 4; ++t) vw[t] = *reinterpret_cast<const u32x2 *>(in + v_at + 512 * t);
-        ve = *reinterpret_cast<const u32x2 *>(in + ve_at);
-    };
-    const int end = tail ? min(p.blocks, (split + 1) * p.per_split) : p.blocks;
-    auto find = [&](int &at, unsigned long long &mask) {
-        for (; at < end; at += kWaves) {
-            mask = block_mask(p.keep, e, p.blocks, at, rows);
-            if (mask) return true;
-        }
-        return false;
-    };
-    unsigned long long mask = 0;
-    int at = split * p.per_split + wave;
-    bool more = find(at, mask);
-    if (more) load_keys(tiles + (long long)at * kBlockBytes), load_values(tiles + (long long)at * kBlockBytes);
     // A block's keys are loaded as soon as the one before has its scores, its values once that one has its output.
     while (more) {
         const unsigned long long now = mask;
@@ -1762,7 +1790,7 @@ void attend(const Icl4Queries &a, const Icl4Attend &b, hipStream_t stream) {
             hipLaunchKernelGGL((icl4_rows_kernel<T, false>), grid, wg, 0, stream, p);
         else if (pl.queries == 32)
             hipLaunchKernelGGL((icl4_wide_kernel<T, 1>), grid, wg, 0, stream, p);
-        else
+        else if constexpr (sizeof(T) == 2)
             hipLaunchKernelGGL((icl4_wide_kernel<T, 2>), grid, wg, 0, stream, p);
         IRX_HIP(hipGetLastError());
     }
