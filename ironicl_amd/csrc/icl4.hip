@@ -1700,12 +1700,13 @@ Plan plan_attend(const Icl4Shape &s, bool half, int q_rows, int n_blocks, int co
         splits = std::min(std::max(1LL, (slots + base - 1) / base), tiles);
     } else {
         // Whole rounds of workgroups take every block; the units left over are split where that is quicker.
-        // Microseconds: a workgroup's start and end, each round of its waves' blocks, the merge.
+        // Microseconds: a workgroup's start and end, each round of its waves' blocks, the merge with its launch. (16
+        // units of 16 blocks, 33 queries: 15.1 us unsplit, 18.0 in four.)
         pl.whole = base / slots * slots / 8 * 8, pl.rest = base - pl.whole;
         double best = 1e30;
         for (long long n = 1; pl.rest && n <= std::min(tiles, std::max(8LL, 2 * slots / pl.rest)); ++n) {
             const double rounds = (double)((pl.rest * n + slots - 1) / slots);
-            const double merge = n > 1 ? 4.0 + (double)pl.rest * pl.queries * (double)n * (520.0 / 4e6) : 0.0;
+            const double merge = n > 1 ? 7.0 + (double)pl.rest * pl.queries * (double)n * (520.0 / 4e6) : 0.0;
             const double cost = rounds * (6.0 + (pl.queries == 32 ? 1.8 : 2.2) * (double)((tiles + n - 1) / n)) + merge;
             if (cost < best) best = cost, splits = n;
         }
@@ -1720,7 +1721,7 @@ Plan plan_attend(const Icl4Shape &s, bool half, int q_rows, int n_blocks, int co
 // choices, in turns of at most 64 MiB of scores (or one query's): whole pairs,
 // or a part of one pair's queries. (One launch with a workgroup to a query took
 // 24 us for 8 queries of 3,125 blocks, a compute unit alone being slow to read
-// 400 KB, where scores and choice apart take 4 and CHOICE.)
+// 400 KB, where scores and choice apart take 3.8 and 6.5.)
 struct SelectPlan {
     bool fused;
     long long padded;
