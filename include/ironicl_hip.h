@@ -337,7 +337,8 @@ int irx_regression_summary(irx_device *device, const float *decoded, size_t ense
  * rows that a cheap score picks for each query. All buffers but the structs
  * are device memory of `device`; the work is enqueued on `stream` (a
  * hipStream_t of that device, or NULL for its null stream) and the calls return
- * without waiting; none allocates, so each may be captured into a HIP graph.
+ * without waiting; none allocates, so each may be captured into a HIP graph. An
+ * output overlaps no input and no other output.
  * The calling thread's current device is left as it was.
  *
  * What a cache holds. E2M1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6, then their
@@ -431,9 +432,13 @@ int irx_icl4_select(irx_device *device, const irx_icl4_queries *queries, const v
  * are skipped, and a block that is listed twice counts twice. blocks NULL and
  * n_blocks 0: every block. lse, when not NULL, [E, H, query_rows] FP32: the
  * natural logarithm of the sum of exp(scale q k), -inf for a query that attends
- * to none. FP32 queries and weights are multiplied as pairs of FP16 values (22
- * bits), FP16 queries as they are with weights rounded once to FP16; sums are
- * FP32. Results do not depend on other calls or on the workspace's contents. */
+ * to none. Results do not depend on other calls or on the workspace's contents.
+ * Scores must lie within FP32's range. What is rounded: an FP32 query of up to
+ * 16 a call is a pair of FP16 values (22 bits), of one a call or with blocks a
+ * 31-bit integer times a power of two, of more to 2^-24 of its largest number;
+ * an FP16 query is exact, but of more than 16 a call numbers below 2^-9 of its
+ * largest are rounded to 2^-18 of it. Weights are pairs of FP16 values for FP32
+ * queries, else FP16 (rounded once); sums are FP32. */
 int irx_icl4_attention(irx_device *device, const irx_icl4_queries *queries, const void *cache, float scale,
                        const int32_t *blocks, size_t n_blocks, void *out, const irx_strides *out_strides, float *lse,
                        void *workspace, size_t workspace_bytes, void *stream);

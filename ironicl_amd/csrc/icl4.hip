@@ -550,9 +550,10 @@ __device__ __forceinline__ i32x4 attended_scores(const SelectArgs &p, const int 
     if (p.keep) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            // Past the last block the score is gone already.
+            // Past the length, and past the last block, the score is gone already.
             const unsigned long long word = p.keep[(long long)e * p.blocks + min(b + i, p.blocks - 1)];
-            s[i] = word << max(0, kBlock - (rows - (b + i) * kBlock)) ? s[i] : kNoScore;
+            const int past = kBlock - (rows - (b + i) * kBlock);  // of the block's rows
+            s[i] = word << min(max(past, 0), kBlock - 1) ? s[i] : kNoScore;
         }
     }
     return s;
@@ -658,7 +659,7 @@ __global__ __launch_bounds__(kPickWaves * 64) void icl4_pick_kernel(SelectArgs p
     constexpr int THREADS = kPickWaves * 64, BINS = 2 * THREADS;
     extern __shared__ __attribute__((aligned(16))) int staged[];
     __shared__ int bins[BINS];  // from the highest down
-    __shared__ int joint[3][kPickWaves];
+    __shared__ int joint[5][kPickWaves];
     __shared__ int found[3];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int at = (int)(blockIdx.x / (unsigned)p.rows_here);
@@ -745,12 +746,12 @@ __global__ __launch_bounds__(kPickWaves * 64) void icl4_pick_kernel(SelectArgs p
     int more = 0, equal = 0;
     for (int b = first + lane; b < end; b += 64) more += held[b] > lo, equal += held[b] == lo;
     more = wave_join(more, add), equal = wave_join(equal, add);
-    if (lane == 0) joint[1][wave] = more, joint[2][wave] = equal;
+    if (lane == 0) joint[3][wave] = more, joint[4][wave] = equal;
     __syncthreads();
     int before_more = 0, before_equal = 0;
 #pragma unroll
     for (int w = 0; w < kPickWaves; ++w)
-        before_more += w < wave ? joint[1][w] : 0, before_equal += w < wave ? joint[2][w] : 0;
+        before_more += w < wave ? joint[3][w] : 0, before_equal += w < wave ? joint[4][w] : 0;
     const unsigned long long below = (1ull << lane) - 1;
     for (int b = first + lane; b < end; b += 64) {
         const int s = held[b];
@@ -1057,9 +1058,11 @@ typedef float f32x32 __attribute__((ext_vector_type(32)));
 // 32 numbers as PARTS operands in E2M3 (multiples of 1/8 below 2, of 1/4 below
 // 4): x = unit (p0 + p1 / 2^4 + p2 / 2^9 + ...), the unit a power of two that
 // brings the largest of the row into [2, 4), each part the nearest to what is
-// left, at most 1/8 (then 1/16) of its own unit's 2: five bits a part, 2^-20 of
-// the largest after four and 2^-25 after five. The exponent bytes of parts 0 to
-// 3 and of part 4: 16^-1, then 32^-1 each.
+// left: the first is off by at most 1/8, the next, in a unit 2^-4 and then 2^-5
+// as large, by at most 1/16. What four leave is at most 2^-18 unit, 2^-19 of the
+// row's largest, what five leave 2^-24 of it. (FP16 numbers down to 2^-9 of the
+// largest are whole multiples of that step: exact.) The exponent bytes of parts
+// 0 to 3 and of part 4.
 constexpr int kPartExps = 127 | (127 - 4) << 8 | (127 - 9) << 16 | (127 - 14) << 24, kPartExps4 = 127 - 19;
 template <int PARTS>
 __device__ __forceinline__ void query_parts(f32x16 &even, f32x16 &odd, float unit, u32x6 (&parts)[PARTS]) {

@@ -1562,6 +1562,7 @@ int guarded(const char *where, auto &&fn) {
 // ---- the 4-bit ICL cache: argument checks ----
 
 constexpr size_t kIcl4MaxQueries = size_t(1) << 24, kIcl4MaxBlocks = 4096;
+constexpr size_t kIcl4MaxRows = 0x7fffffff;  // (estimator, head, query) rows of a call
 
 // The calling thread's current device while a call is on `d`'s.
 class CurrentDevice {
@@ -1648,7 +1649,7 @@ Icl4Queries icl4_queries(const irx_icl4_queries &q, const void *cache) {
     if (!icl4_shape_ok(&q.shape)) fail(IRX_INVALID_ARGUMENT, "the 4-bit cache's shape is out of range");
     if (!q.q || !q.query_rows || q.query_rows > kIcl4MaxQueries)
         fail(IRX_INVALID_ARGUMENT, "1 to 2^24 queries are answered");
-    if (q.query_rows > (size_t)0x7fffffff / (q.shape.estimators * q.shape.heads))
+    if (q.query_rows > kIcl4MaxRows / (q.shape.estimators * q.shape.heads))
         fail(IRX_INVALID_ARGUMENT, "too many queries for one call");
     Icl4Queries a{};
     a.shape = icl4_shape(q.shape), a.half = icl4_half(q.element), a.cache = cache, a.q = q.q;
@@ -2279,6 +2280,7 @@ size_t irx_icl4_bytes(const irx_icl4_shape *shape) {
 size_t irx_icl4_workspace_bytes(irx_device *device, const irx_icl4_shape *shape, size_t query_rows, size_t n_blocks) {
     if (!device || !icl4_shape_ok(shape) || !query_rows || query_rows > kIcl4MaxQueries || n_blocks > kIcl4MaxBlocks)
         return 0;
+    if (query_rows > kIcl4MaxRows / (shape->estimators * shape->heads)) return 0;
     const Icl4Shape s = icl4_shape(*shape);
     size_t attend = 0;
     for (const bool half : {false, true})

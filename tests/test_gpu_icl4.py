@@ -4,7 +4,12 @@ attention within bounds worked out beforehand.
 
 Bounds. A score is a sum of 64 products: FP32 queries as pairs of FP16 values
 are off by at most 2^-22 relative each, a 64-term FP32 sum by 2^-18 of the sum
-of magnitudes A, and FP32's scaling by less: |ds| <= 2^-17 A. A weight exp(s) is
+of magnitudes A, and FP32's scaling by less: |ds| <= 2^-17 A. (One query's
+31-bit integers are off by 2^-31 of its largest number, those of more than 16
+by 2^-24 of it, or for FP16 by 2^-19 where they are below 2^-9 of it. The
+largest of 64 normal numbers is at most 6 times the mean of their sizes, and
+some one in a hundred is that small: 2^-21 and 2^-22 of A, inside the half of
+the bound that the sum leaves.) A weight exp(s) is
 then off by 2 ds relative, and so is a weighted mean of values up to V by at
 most 4 ds V (numerator and denominator). FP32 weights are pairs (2^-22); FP16
 ones are off by half a step, 2^-11, and below FP16's smallest step (half of it
@@ -95,7 +100,8 @@ def put_lengths(lengths):
 
 def workspace(device, shape, q_rows, n_blocks=0):
     size = icl4.workspace_bytes(device, shape, q_rows, n_blocks)
-    return {"workspace": hipmem.DeviceArray((max(size, 16),), np.uint8), "workspace_bytes": size}
+    # Full of NaN: nothing may hang on what it held.
+    return {"workspace": put(np.full(max(size, 16), 255, np.uint8)), "workspace_bytes": size}
 
 
 def attend(device, cache, shape, q, element="f32", layout="heads", keep=None, lengths=None, blocks=None, scale=0.125):
@@ -288,6 +294,36 @@ def test_a_query_that_is_not_finite_leaves_the_others(device):
     assert np.isnan(got[0, 3, 5]).all()
 
 
+@pytest.mark.parametrize("element", ["f32", "f16"])
+@pytest.mark.parametrize("rows,listed", [(1, False), (5, False), (70, False), (5, True)])
+def test_a_query_that_is_not_a_number_stays_alone(device, element, rows, listed):
+    cache, _ = make(device, 2, 4, 700, element)
+    q = draw((2, 4, rows, 64), element, 4)
+    blocks = np.broadcast_to(np.arange(0, 10, 2, dtype=np.int32), (2, 4, rows, 5)) if listed else None
+    whole, whole_lse = attend(device, cache, (2, 4, 700), q, element, blocks=blocks)
+    q[1, 2, rows - 1, 9] = np.nan
+    got, lse = attend(device, cache, (2, 4, 700), q, element, blocks=blocks)
+    others = np.ones((2, 4, rows), bool)
+    others[1, 2, rows - 1] = False
+    np.testing.assert_array_equal(got[others], whole[others])
+    np.testing.assert_array_equal(lse[others], whole_lse[others])
+    assert np.isnan(got[1, 2, rows - 1]).all() and np.isnan(lse[1, 2, rows - 1])
+
+
+@pytest.mark.parametrize("element,rows", [("f32", 1568), ("f16", 2109), ("f16", 1570)])
+def test_attention_of_more_queries_than_the_gpu_takes_at_once(device, element, rows):
+    """Units of work past a whole round of workgroups, of which the last ones are split; every 37th query is checked."""
+    e, h, n = 2, 8, 2500
+    lengths = (2500, 2203)
+    keep = np.random.default_rng(rows).random((e, n)) < 0.9
+    cache, want = make(device, e, h, n, element, lengths=lengths, seed=8)
+    q = draw((e, h, rows, 64), element, 9, 1.5)
+    out, lse = attend(device, cache, (e, h, n), q, element, keep=keep, lengths=lengths)
+    some = np.r_[0:rows:37, rows - 2:rows]
+    check((out[:, :, some], lse[:, :, some]), want.attend(q[:, :, some], keep=keep), element, want)
+    assert np.isfinite(out).all() and np.isfinite(lse).all()
+
+
 # ---- the choice of blocks, and attention over it ----
 
 @pytest.mark.parametrize("element,layout", [("f32", "heads"), ("f16", "tokens")])
@@ -344,6 +380,18 @@ def test_select_of_masked_and_empty_blocks(device):
     assert np.all(got[0] == -1) and np.all(got[3, :, :, 1:] == -1)
 
 
+@pytest.mark.parametrize("e,h,tiles,rows,count", [(1, 2, 256, 40, 9), (2, 1, 257, 33, 17), (1, 1, 700, 17, 100),
+                                                  (1, 1, 960, 16, 960), (1, 1, 961, 17, 100)])
+def test_select_on_both_sides_of_its_forms(device, e, h, tiles, rows, count):
+    n = 64 * tiles - 5
+    lengths = (n, n - 1000)[:e]
+    keep = np.random.default_rng(tiles).random((e, n)) < 0.02
+    cache, want = make(device, e, h, n, "f16", lengths=lengths, seed=tiles)
+    q = draw((e, h, rows, 64), "f16", 2)
+    got = select(device, cache, (e, h, n), q, count, "f16", keep=keep, lengths=lengths)
+    np.testing.assert_array_equal(got, want.select(q, count, keep=keep))
+
+
 def test_select_of_queries_of_any_size(device):
     cache, want = make(device, 1, 2, 900)
     q = draw((1, 2, 8, 64), "f32", 2)
@@ -354,7 +402,7 @@ def test_select_of_queries_of_any_size(device):
 
 @pytest.mark.parametrize("element,layout", [("f32", "heads"), ("f16", "tokens")])
 @pytest.mark.parametrize("e,h,n,rows,count", [(1, 8, 1, 1, 1), (1, 8, 640, 3, 4), (2, 3, 1000, 20, 16), (1, 1, 9000, 2, 100),
-                                              (1, 2, 777, 300, 3)])
+                                              (1, 2, 777, 300, 3), (1, 8, 640, 600, 70), (1, 2, 640, 300, 300)])
 def test_attention_over_listed_blocks(device, e, h, n, rows, count, element, layout):
     """Listed in any order, some twice, some that are no blocks."""
     print(f"{count} listed blocks of {e} x {h} x {n}, {rows} queries, {element} {layout}", flush=True)
