@@ -166,12 +166,13 @@ __device__ __forceinline__ void load16(const _Float16 *src, float *x) {
 // One workgroup per (block, pair): codes and exponents, and the exponents that
 // the block's own bounds would take (icl4_units_kernel takes the largest of a
 // pair's; by atomics into one word per dim the kernel took 97 instead of 52 us
-// at 50,000 rows). Bound by its reads: every load of the block is issued first, and the codes are the
-// conversion instructions' own. The block is put together in LDS and written in
-// whole lines: from registers, in words of several waves each, 50,000 rows took
-// 315 us. Keys: wave 2 s + b, lane (g, 8 a + i) takes
-// dims 16 g .. of row 32 s + 16 a + 8 b + i. Values: wave d, lane 8 (4 s + 2 t
-// + b) + i takes dims 16 d + 2 i and + 1 of rows 32 s + 16 t + 8 b .. +7.
+// at 50,000 rows). Bound by its reads: every load of the block is issued first,
+// and the codes are the conversion instructions' own. The block is put together
+// in LDS and written in whole lines: from registers, in words of several waves
+// each, 50,000 rows took 315 us. 8 heads x 50,000 FP32 rows, 232 MB: 57 us, 4.1
+// TB/s (a large copy: 4.9). Keys: wave 2 s + b, lane (g, 8 a + i) takes dims
+// 16 g .. of row 32 s + 16 a + 8 b + i. Values: wave d, lane 8 (4 s + 2 t + b) + i
+// takes dims 16 d + 2 i and + 1 of rows 32 s + 16 t + 8 b .. +7.
 template <typename T>
 __global__ __launch_bounds__(256) void icl4_encode_kernel(StoreArgs p) {
     typedef T T2 __attribute__((ext_vector_type(2)));
@@ -271,6 +272,7 @@ __global__ __launch_bounds__(256) void icl4_encode_kernel(StoreArgs p) {
 }
 
 // A pair's units: the largest of its blocks' exponents, 16 dims to a workgroup.
+// Latency: 4.8 us for 782 blocks.
 __global__ __launch_bounds__(1024) void icl4_units_kernel(StoreArgs p) {
     __shared__ unsigned part[16][8];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, pair = blockIdx.x >> 2, g = blockIdx.x & 3;
@@ -311,7 +313,8 @@ __device__ __forceinline__ unsigned pk_most(unsigned a, unsigned b) {
 // Bounds of one block per wave, from the codes as FP16 pairs (exact): lane
 // (g, i16) holds dims 16 g .. +15 of four rows; in four steps each lane hands
 // half of its dims to another and keeps the least and most of the rest, so
-// that lane i16 ends with dim 16 g + i16's.
+// that lane i16 ends with dim 16 g + i16's. Reads the keys' codes, which the
+// encoder has left in the caches: 7.0 us for 8 x 782 blocks.
 __global__ __launch_bounds__(256) void icl4_bounds_kernel(StoreArgs p) {
     const int lane = threadIdx.x & 63, g = lane >> 4, i16 = lane & 15;
     const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -370,7 +373,8 @@ struct ReadArgs {
     float *bounds_out;
 };
 
-// The encoder's lanes and rows, the other way.
+// The encoder's lanes and rows, the other way. Bound by its writes: 8 heads x
+// 50,000 FP32 rows, 232 MB, 45 us, 5.1 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void icl4_decode_kernel(ReadArgs p) {
     typedef T T2 __attribute__((ext_vector_type(2)));
@@ -504,7 +508,8 @@ __device__ __forceinline__ i32x4 block_scores(const i32x4 &low, const i32x4 &hig
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(high, c.pos, s, 0, 0, 0);
 }
 
-// Scores of 16 queries against `chunk` blocks per wave.
+// Scores of 16 queries against `chunk` blocks per wave: one query, 8 heads, 3,125
+// blocks (3.2 MB of bounds) 3.8 us, most of it a workgroup's start and one trip to memory.
 template <typename T>
 __global__ __launch_bounds__(256) void icl4_scores_kernel(SelectArgs p) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, i16 = lane & 15;
@@ -650,8 +655,9 @@ __device__ __forceinline__ int wave_prefix(int x) {
 // the n-th largest by a histogram of 1,024 steps of 2^sh over the scores'
 // range, then over the step that holds it, until a step ends at exactly n or is
 // one value wide (two rounds as a rule). Bisection by the sixteen waves took
-// 1,550 cycles a step and 11 steps for 3,125 scores. Scores stand in `held`, LDS
-// (STAGED) or where they are.
+// 1,550 cycles a step and 11 steps for 3,125 scores; this takes 6.6 us for 8 of
+// them, its barriers one after another. Scores stand in `held`, LDS (STAGED) or
+// where they are.
 constexpr int kPickWaves = 8;
 constexpr int kStagedPicks = 12288;  // scores that fit a workgroup's LDS beside the histogram
 template <bool STAGED>
@@ -766,7 +772,9 @@ __global__ __launch_bounds__(kPickWaves * 64) void icl4_pick_kernel(SelectArgs p
 // Scores and choice in one launch, no scores in memory, up to 960 blocks:
 // sixteen queries to a workgroup, scored together, then each chosen for by a
 // wave of its own. Every load is issued first; each wave makes one query's
-// codes (the sixteen by every wave cost more than the scores).
+// codes (the sixteen by every wave cost more than the scores). 512 queries x 8
+// heads x 782 blocks 15.1 us (8.7 and 20.0 in two launches with the scores in
+// memory); 154 x 8 of 193 blocks 7.7, most of it latency.
 constexpr int kChooseWaves = 16;
 template <typename T, int GROUPS>
 __global__ __launch_bounds__(kChooseWaves * 64) void icl4_choose_kernel(SelectArgs p) {
@@ -863,7 +871,9 @@ constexpr int kWaves = 4;
 
 // One workgroup per (16 queries, pair, split): wave w takes every fourth block
 // of the split. FP32 queries and probabilities are pairs of FP16 values, two
-// products each.
+// products each. Bound by its reads of the cache: 8 FP16 queries x 16 pairs x
+// 200,000 rows, 218 MB, 41 us, 5.3 TB/s; with a block's loads all issued before
+// its work, and none beside it, 47.
 template <typename T, bool SPLIT>
 __global__ __launch_bounds__(kWaves * 64) void icl4_rows_kernel(AttendArgs p) {
     constexpr bool PAIRS = sizeof(T) == 4;
@@ -1085,8 +1095,11 @@ __device__ __forceinline__ void query_parts(f32x16 &even, f32x16 &odd, float uni
 // conversion of keys, 7.4 cycles a pair of numbers); values are converted to
 // FP16 and multiplied by FP16 weights (FP32: pairs). What bounds it is the vector
 // unit: per 64 x 64 scores 64 exponentials (9.3 cycles), 64 multiply-adds, 32
-// conversions of values and 32 of weights, and the sums. Lane (r = lane % 32, h =
-// lane / 32), r = 16 s + 8 a + i:
+// conversions of values and 32 of weights, and the sums: at 10,007 FP16 queries
+// and rows it is busy for 71% of the time, the matrix cores for 37%, one or the
+// other for 95%. 8 heads: 512 FP32 queries x 50,000 rows 102 us with the merge,
+// 513 TFLOP/s (a pair's two products counted once); 10,007 x 10,007 FP16 239, 858.
+// Lane (r = lane % 32, h = lane / 32), r = 16 s + 8 a + i:
 //   S^T, b = 0, 1: A = rows 32 s + 16 a + 8 b + i, dims 32 h ..; B = query r, the same dims;
 //     result register 8 s + 4 a + j is row 32 s + 16 a + 8 b + 4 h + j, query r;
 //   O^T, D = 0, 1, step (s, a): A = dim 32 x + 16 D + i (r = 16 x + i), rows 32 s + 16 a + 8 b
@@ -1376,7 +1389,10 @@ __device__ __forceinline__ unsigned row_lane(unsigned x) {
 // per row. (With keys converted to FP16 and every column the query, a block
 // took 190 vector instructions instead of 100.) Weights go through LDS to where
 // the second product wants them: FP32's as high FP16 parts in even and low ones
-// in odd columns.
+// in odd columns. One FP32 query, 8 heads x 50,000 rows (27 MB) 8.8 us, latency:
+// a third of it before a block is there. 4,096 queries x 32 listed blocks, 570 MB
+// through the L2s, 39 us, 14.6 TB/s, one wave to a query; 8 queries x 64 listed
+// blocks 8.8 us in sixteen.
 template <typename T, bool LISTED, bool SPLIT, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 4) void icl4_one_kernel(AttendArgs p) {
     constexpr bool PAIRS = sizeof(T) == 4;
@@ -1579,6 +1595,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void icl4_one_kernel(AttendArgs p) {
 
 // Splits' outputs weighted by their sums. 16 lanes of four dims each take a
 // (pair, query) and every GROUPS-th split; a workgroup holds 16 / GROUPS rows.
+// 3.4 to 5 us, the latency of one trip to memory and of a launch.
 template <typename T, int GROUPS>
 __global__ __launch_bounds__(256) void icl4_merge_kernel(AttendArgs p) {
     __shared__ float sums[GROUPS > 1 ? 16 * 66 : 1];
@@ -1665,42 +1682,52 @@ struct Plan {
     long long part_rows;  // rows of a split's partials
 };
 
-// Listed blocks up to which few queries take sixteen waves each rather than splits of four and a merge.
-constexpr int kManyWaves = 16, kUnsplitBlocks = 256;
-// Queries per compute unit from which a query with listed blocks takes one wave.
+// Queries up to which FP32 attention over every block takes a workgroup per query
+// (1 x 200,000 rows x 8 heads 22.1 us against 27.0 with 16 to a workgroup, 2
+// 25.9 against 27.4, 3 36.4 against 27.1; FP16, which takes one product where
+// FP32 takes two, 48.5 against 46.2 at 1 x 200,000 x 16).
+constexpr int kOneQueries = 2;
+// Queries per compute unit from which a query with listed blocks takes one wave,
+// up to the 64 blocks that its lanes hold at once (4,096 queries of 8 blocks 28.5
+// against 33.8 us with four waves, of 32 52.0 against 55.2, of 64 85.7 against
+// 87.0; of 128 151 against 148; 2,048 of 32 blocks 39.4 against 38.0).
 constexpr int kManyQueries = 16;
-
-// Queries up to which attention over every block takes a workgroup per query.
-constexpr int kOneQueries = 1;
+// Waves that take a query's listed blocks unsplit where queries are few.
+constexpr int kManyWaves = 16;
 
 // About two workgroups per compute unit, at least four blocks to a split (one to
-// a wave). Above 16 queries a workgroup takes 32, three to a compute unit (168
-// registers), or 64, two (256): FP16 queries 64 where that makes a whole round
-// of workgroups (10,007 queries x 10,007 rows 237 against 248 us; 777 x 12,345 x
-// 2 estimators, 208 workgroups, 70.3 against 68.2), FP32 ones, whose pairs do not
-// fit 256 registers beside 64 queries' scores, never (512 x 50,000 111 against
-// 106.6 us).
+// a wave). Listed blocks of queries that do not fill the compute units: a
+// compute unit reads a block in about 1/16 us whatever its waves, so sixteen
+// waves to a query and no merge where its busiest unit has at most 64 blocks (4
+// us, a merge with its launch) more than in splits of four waves: 8 queries of
+// 64 blocks of 3,125 17.7 against 16.2 us in a graph and two launches against
+// one, of 256 30.0 against 17.9; 256 of 256 34.9 against 43.3, 304 of 256 53.8
+// against 46.9. Attention over every block: above 16 queries a workgroup takes
+// 32, three to a compute unit (168 registers), or 64, two (256): FP16 queries 64
+// where that makes a whole round of workgroups (10,007 queries x 10,007 rows 237
+// against 248 us; 777 x 12,345 x 2 estimators, 208 workgroups, 70.3 against
+// 68.2), FP32 ones, whose pairs do not fit 256 registers beside 64 queries'
+// scores, never (512 x 50,000 111 against 106.6 us).
 Plan plan_attend(const Icl4Shape &s, bool half, int q_rows, int n_blocks, int compute_units) {
     Plan pl{};
     const int places = n_blocks ? n_blocks : s.blocks();
     const bool full = half && (long long)s.pairs() * ceil_div(q_rows, 64) >= 2LL * compute_units;
-    pl.queries = n_blocks || q_rows <= kOneQueries ? 1 : q_rows <= 16 ? 16 : full ? 64 : 32;
+    pl.queries = n_blocks || (!half && q_rows <= kOneQueries) ? 1 : q_rows <= 16 ? 16 : full ? 64 : 32;
     pl.qtiles = (int)ceil_div(q_rows, pl.queries);
     pl.rows = pl.part_rows = (long long)s.pairs() * q_rows;
     pl.waves = kWaves;
     const long long base = (long long)s.pairs() * pl.qtiles;
-    if (n_blocks && n_blocks <= kUnsplitBlocks && n_blocks > kWaves && base < 2LL * compute_units) {
-        pl.waves = kManyWaves, pl.splits = 1, pl.per_split = n_blocks;
-        return pl;
-    }
-    if (n_blocks && base >= (long long)kManyQueries * compute_units) {
-        pl.waves = 1, pl.splits = 1, pl.per_split = n_blocks;
-        return pl;
-    }
     const long long slots = (pl.queries == 32 ? 3LL : 2LL) * compute_units, tiles = ceil_div(places, kWaves);
     long long splits = 1;
     if (pl.queries <= 16) {
         splits = std::min(std::max(1LL, (slots + base - 1) / base), tiles);
+        if (n_blocks && base >= (long long)kManyQueries * compute_units && n_blocks <= 64) {
+            pl.waves = 1;
+        } else if (n_blocks && splits > 1) {
+            const auto of_unit = [&](long long workgroups) { return (workgroups + compute_units - 1) / compute_units; };
+            const long long share = (tiles + splits - 1) / splits * kWaves;
+            if (of_unit(base) * n_blocks <= of_unit(base * splits) * share + 64) pl.waves = kManyWaves, splits = 1;
+        }
     } else {
         // Whole rounds of workgroups take every block; the units left over are split where that is quicker.
         // Microseconds: a workgroup's start and end, each round of its waves' blocks, the merge with its launch. (16
@@ -1720,11 +1747,15 @@ Plan plan_attend(const Icl4Shape &s, bool half, int q_rows, int n_blocks, int co
     return pl;
 }
 
-// How blocks are chosen: in one launch up to 960 blocks; else scores first, then
-// choices, in turns of at most 64 MiB of scores (or one query's): whole pairs,
-// or a part of one pair's queries. (One launch with a workgroup to a query took
-// 24 us for 8 queries of 3,125 blocks, a compute unit alone being slow to read
-// 400 KB, where scores and choice apart take 3.8 and 6.5.)
+// How blocks are chosen: in one launch up to 512 blocks, and up to 960 where 16
+// queries to a workgroup come to 128 workgroups (512 blocks, 256 queries 15.8 us
+// in one launch, with attention over 16 of them, 14.3 in two, 1,024 19.5 and
+// 20.6; 782 blocks, 512 queries 21.8 and 17.5, 1,024 24.4 and 22.3, 2,048 30.4
+// and 33.0: few workgroups are slow to read so many bounds); else scores first,
+// then choices, in turns of at most 64 MiB of scores (or one query's): whole
+// pairs, or a part of one pair's queries. (One launch with a workgroup to a
+// query took 24 us for 8 queries of 3,125 blocks, a compute unit alone being
+// slow to read 400 KB, where scores and choice apart take 3.8 and 6.5.)
 struct SelectPlan {
     bool fused;
     long long padded;
@@ -1733,7 +1764,7 @@ struct SelectPlan {
 SelectPlan plan_select(const Icl4Shape &s, int q_rows) {
     SelectPlan t{};
     t.padded = (s.blocks() + 63) / 64 * 64;
-    t.fused = s.blocks() <= kWavePicks;
+    t.fused = s.blocks() <= 512 || (s.blocks() <= kWavePicks && (long long)s.pairs() * ceil_div(q_rows, 16) >= 128);
     if (t.fused) return t;
     const long long most = std::max<long long>(1, (16LL << 20) / t.padded);  // queries of a turn
     t.rows = (int)std::min<long long>(q_rows, most);
@@ -1751,6 +1782,17 @@ Parts parts(const void *cache, const Icl4Shape &s) {
     const size_t blocks = (size_t)s.pairs() * s.blocks();
     return {p, reinterpret_cast<signed char *>(p + blocks * kBlockBytes),
             reinterpret_cast<float *>(p + blocks * (kBlockBytes + 128))};
+}
+
+// FP16 queries never ask for it.
+template <typename T>
+void launch_one_over_all(bool split, dim3 grid, dim3 wg, hipStream_t stream, const AttendArgs &p) {
+    if constexpr (sizeof(T) == 4) {
+        if (split)
+            hipLaunchKernelGGL((icl4_one_kernel<T, false, true, kWaves>), grid, wg, 0, stream, p);
+        else
+            hipLaunchKernelGGL((icl4_one_kernel<T, false, false, kWaves>), grid, wg, 0, stream, p);
+    }
 }
 
 template <typename T>
@@ -1784,10 +1826,8 @@ void attend(const Icl4Queries &a, const Icl4Attend &b, hipStream_t stream) {
             hipLaunchKernelGGL((icl4_one_kernel<T, true, true, kWaves>), grid, wg, 0, stream, p);
         else if (b.list)
             hipLaunchKernelGGL((icl4_one_kernel<T, true, false, kWaves>), grid, wg, 0, stream, p);
-        else if (pl.queries == 1 && split)
-            hipLaunchKernelGGL((icl4_one_kernel<T, false, true, kWaves>), grid, wg, 0, stream, p);
         else if (pl.queries == 1)
-            hipLaunchKernelGGL((icl4_one_kernel<T, false, false, kWaves>), grid, wg, 0, stream, p);
+            launch_one_over_all<T>(split, grid, wg, stream, p);
         else if (pl.queries == 16 && split)
             hipLaunchKernelGGL((icl4_rows_kernel<T, true>), grid, wg, 0, stream, p);
         else if (pl.queries == 16)

@@ -381,7 +381,9 @@ def test_select_of_masked_and_empty_blocks(device):
 
 
 @pytest.mark.parametrize("e,h,tiles,rows,count", [(1, 2, 256, 40, 9), (2, 1, 257, 33, 17), (1, 1, 700, 17, 100),
-                                                  (1, 1, 960, 16, 960), (1, 1, 961, 17, 100)])
+                                                  (1, 1, 960, 16, 960), (1, 1, 961, 17, 100), (1, 1, 512, 16, 512),
+                                                  (1, 1, 513, 17, 100), (1, 2, 600, 1024, 9), (1, 2, 960, 1009, 960),
+                                                  (1, 2, 961, 1009, 100)])
 def test_select_on_both_sides_of_its_forms(device, e, h, tiles, rows, count):
     n = 64 * tiles - 5
     lengths = (n, n - 1000)[:e]
