@@ -433,12 +433,13 @@ int irx_icl4_select(irx_device *device, const irx_icl4_queries *queries, const v
  * n_blocks 0: every block. lse, when not NULL, [E, H, query_rows] FP32: the
  * natural logarithm of the sum of exp(scale q k), -inf for a query that attends
  * to none. Results do not depend on other calls or on the workspace's contents.
- * Scores must lie within FP32's range. What is rounded: an FP32 query of up to
- * 16 a call is a pair of FP16 values (22 bits), of one a call or with blocks a
- * 31-bit integer times a power of two, of more to 2^-24 of its largest number;
- * an FP16 query is exact, but of more than 16 a call numbers below 2^-9 of its
- * largest are rounded to 2^-18 of it. Weights are pairs of FP16 values for FP32
- * queries, else FP16 (rounded once); sums are FP32. */
+ * Scores must lie within FP32's range. What is rounded: an FP32 query with
+ * blocks, or of one or two a call, to 31 bits of its largest number, of up to 16
+ * to a pair of FP16 values (22 bits a number), of more to 2^-24 of its largest;
+ * an FP16 query is exact, but with blocks numbers are rounded to 2^-30 of its
+ * largest, and of more than 16 a call those below 2^-9 of it to 2^-18. Weights
+ * are pairs of FP16 values for FP32 queries, else FP16 (rounded once); sums are
+ * FP32. */
 int irx_icl4_attention(irx_device *device, const irx_icl4_queries *queries, const void *cache, float scale,
                        const int32_t *blocks, size_t n_blocks, void *out, const irx_strides *out_strides, float *lse,
                        void *workspace, size_t workspace_bytes, void *stream);

@@ -1687,6 +1687,14 @@ struct Plan {
 // 25.9 against 27.4, 3 36.4 against 27.1; FP16, which takes one product where
 // FP32 takes two, 48.5 against 46.2 at 1 x 200,000 x 16).
 constexpr int kOneQueries = 2;
+// Up to 16, FP32 or FP16, take the 16-query form in splits: 16 x 50,000 x 8 14.5
+// against 19.1 us in the wide one. (32 queries as two such tiles 18.9 against
+// 20.6, but 73.6 against 57.5 at 200,000 x 16; 33 x 1,024 x 16 7.2 against 8.9,
+// with a second launch.)
+constexpr int kRowQueries = 16;
+// Blocks, four to a tile, that they take without splits and a merge: 1 x 1,024
+// rows 5.4 against 6.7 us, 16 x 1,024 6.8 against 6.9; 16 x 2,000 10.4 against 7.0.
+constexpr int kWholeTiles = 4;
 // Queries per compute unit from which a query with listed blocks takes one wave,
 // up to the 64 blocks that its lanes hold at once (4,096 queries of 8 blocks 28.5
 // against 33.8 us with four waves, of 32 52.0 against 55.2, of 64 85.7 against
@@ -1712,7 +1720,7 @@ Plan plan_attend(const Icl4Shape &s, bool half, int q_rows, int n_blocks, int co
     Plan pl{};
     const int places = n_blocks ? n_blocks : s.blocks();
     const bool full = half && (long long)s.pairs() * ceil_div(q_rows, 64) >= 2LL * compute_units;
-    pl.queries = n_blocks || (!half && q_rows <= kOneQueries) ? 1 : q_rows <= 16 ? 16 : full ? 64 : 32;
+    pl.queries = n_blocks || (!half && q_rows <= kOneQueries) ? 1 : q_rows <= kRowQueries ? 16 : full ? 64 : 32;
     pl.qtiles = (int)ceil_div(q_rows, pl.queries);
     pl.rows = pl.part_rows = (long long)s.pairs() * q_rows;
     pl.waves = kWaves;
@@ -1720,7 +1728,7 @@ Plan plan_attend(const Icl4Shape &s, bool half, int q_rows, int n_blocks, int co
     const long long slots = (pl.queries == 32 ? 3LL : 2LL) * compute_units, tiles = ceil_div(places, kWaves);
     long long splits = 1;
     if (pl.queries <= 16) {
-        splits = std::min(std::max(1LL, (slots + base - 1) / base), tiles);
+        if (n_blocks || tiles > kWholeTiles) splits = std::min(std::max(1LL, (slots + base - 1) / base), tiles);
         if (n_blocks && base >= (long long)kManyQueries * compute_units && n_blocks <= 64) {
             pl.waves = 1;
         } else if (n_blocks && splits > 1) {
@@ -1840,7 +1848,8 @@ void attend(const Icl4Queries &a, const Icl4Attend &b, hipStream_t stream) {
     }
     if (pl.splits > 1) {
         KernelTimer timer(kFamIclMerge, stream, 0.0, 4.0 * pl.part_rows * (65.0 * pl.splits + 64.0));
-        // A lane's splits come eight at a time: more groups where there are more splits.
+        // A lane's splits come eight at a time: more groups where there are more splits (one group for 49 splits of 8
+        // rows 4 us more than sixteen, for 32 of 128 rows 2.3 more than four).
         if (pl.splits <= 8)
             hipLaunchKernelGGL((icl4_merge_kernel<T, 1>), dim3(ceil_div((size_t)pl.part_rows, 16)), dim3(256), 0, stream, p);
         else if (pl.splits <= 32)
@@ -1945,7 +1954,8 @@ void choose(const Icl4Queries &a, int n, int *out, void *workspace, hipStream_t 
             const int pairs = std::min(t.pairs, p.pairs - p.pair0);
             p.rows_here = std::min(t.rows, p.q_rows - p.row0);
             p.qtiles = (int)ceil_div(p.rows_here, 16);
-            // A wave takes 16 to 256 blocks: fewer where that leaves compute units idle.
+            // A wave takes 16 to 256 blocks: fewer where that leaves compute units idle (1 x 3,125 x 8: 16 each 3 us less
+            // than 256; 512 x 3,125 x 8 19 us more).
             const long long tiles = (long long)pairs * p.qtiles;
             p.chunk = 256;
             while (p.chunk > 16 && tiles * ceil_div(p.blocks, 4 * p.chunk) < 2LL * a.compute_units) p.chunk /= 2;

@@ -4,7 +4,7 @@ attention within bounds worked out beforehand.
 
 Bounds. A score is a sum of 64 products: FP32 queries as pairs of FP16 values
 are off by at most 2^-22 relative each, a 64-term FP32 sum by 2^-18 of the sum
-of magnitudes A, and FP32's scaling by less: |ds| <= 2^-17 A. (One query's
+of magnitudes A, and FP32's scaling by less: |ds| <= 2^-17 A. (One or two queries'
 31-bit integers are off by 2^-31 of its largest number, those of more than 16
 by 2^-24 of it, or for FP16 by 2^-19 where they are below 2^-9 of it. The
 largest of 64 normal numbers is at most 6 times the mean of their sizes, and
@@ -213,7 +213,7 @@ def test_one_side_is_read_alone(device):
 @pytest.mark.parametrize("element,layout", [("f32", "heads"), ("f16", "tokens"), ("f32", "tokens"), ("f16", "heads")])
 @pytest.mark.parametrize("e,h,n,rows", [(1, 8, 1, 1), (1, 8, 63, 3), (2, 4, 64, 16), (1, 8, 65, 17), (1, 3, 1000, 1),
                                         (2, 8, 777, 33), (1, 8, 2049, 65), (1, 2, 640, 130), (1, 1, 5000, 300),
-                                        (1, 2, 20011, 5)])
+                                        (1, 2, 20011, 5), (1, 8, 1025, 2), (1, 3, 20011, 1)])
 def test_attention(device, e, h, n, rows, element, layout):
     print(f"attention {e} x {h} x {n}, {rows} queries, {element} {layout}", flush=True)
     cache, want = make(device, e, h, n, element, layout, seed=n)
@@ -240,6 +240,20 @@ def test_attention_of_ragged_and_masked_estimators(device, element, rows):
     # One attended row: its held value, whatever its score.
     bound = np.abs(want.v[5, :, None, 130]) * (2.0 ** -20 if element == "f32" else 2.0 ** -11)
     assert np.all(np.abs(got[0][5] - want.v[5, :, None, 130]) <= bound)
+
+
+@pytest.mark.parametrize("element", ["f32", "f16"])
+@pytest.mark.parametrize("rows", [1, 2, 3, 16])
+def test_few_queries_of_ragged_and_masked_estimators(device, element, rows):
+    """Splits of long contexts, some of them past an estimator's length or masked whole."""
+    e, h, n = 4, 2, 9001
+    lengths = (9001, 0, 1500, 9000)
+    keep = np.random.default_rng(rows).random((e, n)) < 0.5
+    keep[0, 640:5000] = False
+    keep[3, :8990] = False
+    cache, want = make(device, e, h, n, element, lengths=lengths, seed=6)
+    q = draw((e, h, rows, 64), element, 12, 1.5)
+    check(attend(device, cache, (e, h, n), q, element, keep=keep, lengths=lengths), want.attend(q, keep=keep), element, want)
 
 
 def test_keep_bits_past_the_rows_are_not_read_as_rows(device):
