@@ -155,6 +155,9 @@ def check(got, want, element, cache):
     (2, 3, 65, "f32", "tokens", (65, 2)),
     (3, 8, 200, "f16", "heads", (0, 200, 129)),
     (2, 5, 130, "f32", "heads", (1000, 64)),
+    (2, 2, 2047, "f32", "heads", (2047, 700)),
+    (2, 2, 2049, "f16", "tokens", (2049, 700)),
+    (1, 1, 70001, "f32", "heads", None),
 ])
 def test_cache_holds_what_it_says(device, e, h, n, element, layout, lengths):
     print(f"encode {e} x {h} x {n} {element} {layout} {lengths}", flush=True)
