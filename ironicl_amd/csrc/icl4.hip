@@ -1134,9 +1134,10 @@ __device__ __forceinline__ void query_parts(f32x16 &even, f32x16 &odd, float uni
 // FP16 and multiplied by FP16 weights (FP32: pairs). What bounds it is the vector
 // unit: per 64 x 64 scores 64 exponentials (9.3 cycles), 64 multiply-adds, 32
 // conversions of values and 32 of weights, and the sums: at 10,007 FP16 queries
-// and rows it is busy for 71% of the time, the matrix cores for 37%, one or the
-// other for 95%. 8 heads: 512 FP32 queries x 50,000 rows 102 us with the merge,
-// 513 TFLOP/s (a pair's two products counted once); 10,007 x 10,007 FP16 239, 858.
+// and rows it is busy for 62% of the time, the matrix cores for 36%, one or the
+// other for 85% (three or two waves to a SIMD hide the rest no further). 8 heads:
+// 512 FP32 queries x 50,000 rows 100 us with the merge, 526 TFLOP/s (a pair's two
+// products counted once); 10,007 x 10,007 FP16 234, 877.
 // Lane (r = lane % 32, h = lane / 32), r = 16 s + 8 a + i:
 //   S^T, b = 0, 1: A = rows 32 s + 16 a + 8 b + i, dims 32 h ..; B = query r, the same dims;
 //     result register 8 s + 4 a + j is row 32 s + 16 a + 8 b + 4 h + j, query r;
@@ -1429,8 +1430,9 @@ __device__ __forceinline__ unsigned row_lane(unsigned x) {
 // the second product wants them: FP32's as high FP16 parts in even and low ones
 // in odd columns. One FP32 query, 8 heads x 50,000 rows (27 MB) 8.8 us, latency:
 // a third of it before a block is there. 4,096 queries x 32 listed blocks, 570 MB
-// through the L2s, 39 us, 14.6 TB/s, one wave to a query; 8 queries x 64 listed
-// blocks 8.8 us in sixteen.
+// through the L2s, 39 us, 14.6 TB/s, one wave to a query (vector unit 57% busy,
+// matrix cores 33%, one or the other 75%); 8 queries x 64 listed blocks 8.8 us in
+// sixteen.
 template <typename T, bool LISTED, bool SPLIT, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 4) void icl4_one_kernel(AttendArgs p) {
     constexpr bool PAIRS = sizeof(T) == 4;
