@@ -1778,14 +1778,22 @@ Plan plan_attend(const Icl4Shape &s, bool half, int q_rows, int n_blocks, int co
         }
     } else {
         // Whole rounds of workgroups take every block; the units left over are split where that is quicker.
-        // Microseconds: a workgroup's start and end, each round of its waves' blocks, the merge with its launch. (16
-        // units of 16 blocks, 33 queries: 15.1 us unsplit, 18.0 in four.)
+        // Microseconds: a workgroup's start and end, each round of its waves' blocks with one, two or three
+        // workgroups on a compute unit, the merge with its launch. (16 units of 16 blocks, 33 queries: 15.1 us unsplit,
+        // 18.0 in four; 400 units of 193 blocks, FP16 and masked, 63.2 unsplit, 77.0, 67.9 and 73.9 in two to four;
+        // 128 of 782 blocks, FP32, 252, 132, 121, 102, 114, 101 and, in eight, 103.)
+        static const double round32[2][3] = {{1.3, 1.85, 2.65}, {1.05, 1.2, 1.75}}, round64[2] = {1.6, 2.2};
+        const auto round = [&](long long groups) {  // of up to `slots` workgroups
+            const int k = (int)((groups + compute_units - 1) / compute_units) - 1;
+            return pl.queries == 32 ? round32[half][k] : round64[k];
+        };
         pl.whole = base / slots * slots / 8 * 8, pl.rest = base - pl.whole;
         double best = 1e30;
         for (long long n = 1; pl.rest && n <= std::min(tiles, std::max(8LL, 2 * slots / pl.rest)); ++n) {
-            const double rounds = (double)((pl.rest * n + slots - 1) / slots);
-            const double merge = n > 1 ? 7.0 + (double)pl.rest * pl.queries * (double)n * (520.0 / 4e6) : 0.0;
-            const double cost = rounds * (6.0 + (pl.queries == 32 ? 1.8 : 2.2) * (double)((tiles + n - 1) / n)) + merge;
+            const long long rounds = pl.rest * n / slots, last = pl.rest * n - rounds * slots;
+            const double share = (double)((tiles + n - 1) / n);
+            double cost = (double)rounds * (6.0 + round(slots) * share) + (last ? 6.0 + round(last) * share : 0.0);
+            if (n > 1) cost += 7.0 + (double)pl.rest * pl.queries * (double)n * (520.0 / 4e6);
             if (cost < best) best = cost, splits = n;
         }
         pl.part_rows = pl.rest * pl.queries;
