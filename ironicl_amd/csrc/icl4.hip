@@ -163,6 +163,28 @@ __device__ __forceinline__ void load16(const _Float16 *src, float *x) {
     }
 }
 
+// The largest magnitude; numbers that are not finite become 0 and are counted.
+template <int N>
+__device__ __forceinline__ float finite_peak(float *x, unsigned &bad) {
+    constexpr float kLargest = 3.4028235e38f;
+    float m = 0.f;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        m = fmaxf(m, fmaxf(fabsf(x[i]), fabsf(x[i + 1])));  // a NaN beside a number is passed over
+        odd |= __builtin_isunordered(x[i], x[i + 1]);
+    }
+    if (odd || m > kLargest) {
+        m = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (!(fabsf(x[i]) <= kLargest)) x[i] = 0.f, ++bad;
+            m = fmaxf(m, fabsf(x[i]));
+        }
+    }
+    return m;
+}
+
 // One workgroup per (block, pair): codes and exponents, and the exponents that
 // the block's own bounds would take (icl4_units_kernel takes the largest of a
 // pair's; by atomics into one word per dim the kernel took 97 instead of 52 us
@@ -170,7 +192,9 @@ __device__ __forceinline__ void load16(const _Float16 *src, float *x) {
 // and the codes are the conversion instructions' own. The block is put together
 // in LDS and written in whole lines: from registers, in words of several waves
 // each, 50,000 rows took 315 us. 8 heads x 50,000 FP32 rows, 232 MB: 57 us, 4.1
-// TB/s (a large copy: 4.9). Keys: wave 2 s + b, lane (g, 8 a + i) takes dims
+// TB/s (a large copy: 4.9); whole 256-byte rows to a load, or two blocks to a
+// workgroup, the second's loads beneath the first's work, are no quicker. 2 x 8 x
+// 12,345 FP16 rows 13.4 us, 4.8 TB/s. Keys: wave 2 s + b, lane (g, 8 a + i) takes dims
 // 16 g .. of row 32 s + 16 a + 8 b + i. Values: wave d, lane 8 (4 s + 2 t + b) + i
 // takes dims 16 d + 2 i and + 1 of rows 32 s + 16 t + 8 b .. +7.
 template <typename T>
@@ -186,48 +210,54 @@ __global__ __launch_bounds__(256) void icl4_encode_kernel(StoreArgs p) {
     const int value_row = 8 * (lane >> 3), value_dim = 16 * wave + 2 * (lane & 7);
     float x[16];
     T2 v[8];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = T2{(T)0.f, (T)0.f};
     {
         const long long row0 = (long long)block * kBlock;
         const T *k = static_cast<const T *>(p.k) + e * p.k_est + head * p.k_head + (row0 + key_row) * p.k_row + 16 * g;
         const T *vs = static_cast<const T *>(p.v) + e * p.v_est + head * p.v_head + (row0 + value_row) * p.v_row + value_dim;
-        if (key_row < left) load16(k, x);
+        if (left >= kBlock) {
+            load16(k, x);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (value_row + i < left) v[i] = *reinterpret_cast<const T2 *>(vs + i * p.v_row);
+            for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const T2 *>(vs + i * p.v_row);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = 0.f;
+            if (key_row < left) load16(k, x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                v[i] = T2{(T)0.f, (T)0.f};
+                if (value_row + i < left) v[i] = *reinterpret_cast<const T2 *>(vs + i * p.v_row);
+            }
+        }
     }
     unsigned bad = 0;
-    auto fix = [&](float &y) {
-        if (!(fabsf(y) <= 3.4028235e38f)) y = 0.f, ++bad;
-    };
     {
-        float m = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            fix(x[i]);
-            m = fmaxf(m, fabsf(x[i]));
-        }
+        const float m = finite_peak<16>(x, bad);
         const int ex = code_exponent(rows_max(m));  // lanes of dims 32 u and + 16
         const float scale = pow2(ex);
         const u32x2 w = {coded8(x, scale), coded8(x + 8, scale)};
         const int s = wave >> 1, b = wave & 1;
         *reinterpret_cast<u32x2 *>(out + s * 1024 + lane * 16 + b * 8) = w;
         if (!(g & 1)) out[kKeyExpsAt + ((g >> 1) * 16 + i16) * 4 + 2 * s + b] = (unsigned char)(ex + 127);
-        // Largest held |key| of each dim over the wave's rows: FP16 pairs, exact, in every lane of a row of 16.
+        // Largest held |key| of each dim over the wave's rows, FP16 pairs, exact: in three steps a lane hands half of its
+        // pairs to another, so that lanes 2 i and 2 i + 1 of a row of 16 end with pair i.
         u32x4 held[2];
         held[0] = __builtin_bit_cast(u32x4, codes8(w[0], scale)), held[1] = __builtin_bit_cast(u32x4, codes8(w[1], scale));
+        unsigned y[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            unsigned y = held[i >> 2][i & 3] & 0x7fff7fffu;
-            y = pk_max(y, row_xor<1>(y));
-            y = pk_max(y, row_xor<2>(y));
-            y = pk_max(y, row_xor<4>(y));
-            y = pk_max(y, row_xor<8>(y));
-            if (i16 == i) peaks[wave][8 * g + i] = y;
-        }
+        for (int i = 0; i < 8; ++i) y[i] = held[i >> 2][i & 3] & 0x7fff7fffu;
+        auto step = [&](auto lanes, int keep, bool upper) {
+            constexpr int N = decltype(lanes)::value;
+#pragma unroll
+            for (int i = 0; i < keep; ++i) {
+                const unsigned give = upper ? y[i] : y[i + keep], own = upper ? y[i + keep] : y[i];
+                y[i] = pk_max(own, row_xor<N>(give));
+            }
+        };
+        step(std::integral_constant<int, 8>{}, 4, i16 & 8);
+        step(std::integral_constant<int, 4>{}, 2, i16 & 4);
+        step(std::integral_constant<int, 2>{}, 1, i16 & 2);
+        y[0] = pk_max(y[0], row_xor<1>(y[0]));
+        if (!(i16 & 1)) peaks[wave][8 * g + (i16 >> 1)] = y[0];
     }
     __syncthreads();
     if (tid < 32) {
@@ -239,15 +269,12 @@ __global__ __launch_bounds__(256) void icl4_encode_kernel(StoreArgs p) {
             (unsigned short)(x0 | x1 << 8);
     }
     {
-        float m[2] = {0.f, 0.f}, y[2][8];
+        float m[2], y[2][8];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                y[c][i] = (float)v[i][c];
-                fix(y[c][i]);
-                m[c] = fmaxf(m[c], fabsf(y[c][i]));
-            }
+            for (int i = 0; i < 8; ++i) y[c][i] = (float)v[i][c];
+            m[c] = finite_peak<8>(y[c], bad);
             // The 32 rows of a group: lanes ^ 8 and ^ 16.
             m[c] = fmaxf(m[c], __uint_as_float(other_eight(__float_as_uint(m[c]))));
             m[c] = rows_max(m[c]);
