@@ -649,11 +649,9 @@ __device__ __forceinline__ void pick_by_wave(const SelectArgs &p, const int *sco
             held[i][j] = some >> (8 * j) & 0xffu ? held[i][j] : kNoScore;
             most = max(most, held[i][j]);
             least = held[i][j] == kNoScore ? least : min(least, held[i][j]);
-            total += held[i][j] != kNoScore;
+            total += __popcll(__ballot(held[i][j] != kNoScore));
         }
     }
-    const auto add = [](int a, int b) { return a + b; };
-    total = __builtin_amdgcn_readfirstlane(wave_join(total, add));
     least = __builtin_amdgcn_readfirstlane(wave_join(least, [](int a, int b) { return min(a, b); }));
     most = __builtin_amdgcn_readfirstlane(wave_join(most, [](int a, int b) { return max(a, b); }));
     // More than n scores reach lo, fewer lo + gap.
@@ -666,8 +664,7 @@ __device__ __forceinline__ void pick_by_wave(const SelectArgs &p, const int *sco
 #pragma unroll
         for (int i = 0; i < GROUPS; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) c += held[i][j] >= cut;
-        c = __builtin_amdgcn_readfirstlane(wave_join(c, add));
+            for (int j = 0; j < 4; ++j) c += __popcll(__ballot(held[i][j] >= cut));
         exact = c == p.n;
         if (exact)
             lo = cut - 1;  // the scores above are the n best
@@ -681,8 +678,8 @@ __device__ __forceinline__ void pick_by_wave(const SelectArgs &p, const int *sco
 #pragma unroll
     for (int i = 0; i < GROUPS; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) all += held[i][j] > lo;
-    const int room = exact ? 0 : p.n - __builtin_amdgcn_readfirstlane(wave_join(all, add));
+        for (int j = 0; j < 4; ++j) all += __popcll(__ballot(held[i][j] > lo));
+    const int room = exact ? 0 : p.n - all;
     const unsigned long long below = (1ull << lane) - 1;
     int before_above = 0, before_equal = 0;
 #pragma unroll
