@@ -406,7 +406,7 @@ size_t irx_icl4_bytes(const irx_icl4_shape *shape);
 /* Bytes of workspace (16-byte aligned) with which irx_icl4_select and
  * irx_icl4_attention run on `device` for query_rows queries and n_blocks chosen
  * blocks (0: attention over every block); 0 for arguments out of range, or when
- * none is needed. Calls that may run at once, in graphs too, need one each. */
+ * none is needed. Fewer queries can need more: they are split further. Calls that may run at once, in graphs too, need one each. */
 size_t irx_icl4_workspace_bytes(irx_device *device, const irx_icl4_shape *shape, size_t query_rows, size_t n_blocks);
 /* Writes `cache` from rows->k and rows->v. nonfinite, when not NULL, is a
  * device counter to which the numbers that are not finite, inside the lengths,

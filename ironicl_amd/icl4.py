@@ -75,7 +75,8 @@ def cache_bytes(shape) -> int:
 
 
 def workspace_bytes(device: hip.Device, shape, query_rows: int, n_blocks: int = 0) -> int:
-    """Bytes of workspace for `select` and `attention` of `query_rows` queries."""
+    """Bytes of workspace for `select` and `attention` of exactly `query_rows` queries
+    (fewer can need more: they are split further) over `n_blocks` blocks each, or all."""
     return _call("irx_icl4_workspace_bytes")(device.handle, _shape(shape), query_rows, n_blocks)
 
 
