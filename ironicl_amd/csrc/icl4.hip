@@ -893,6 +893,7 @@ struct AttendArgs {
     long long o_est, o_head, o_row;
     float *lse;
     const unsigned char *tiles;
+    const float *units;  // [pairs, 64], of the cache
     const unsigned *lengths;
     const unsigned long long *keep;
     const int *list;  // [pairs, q_rows, n] or null
@@ -916,6 +917,20 @@ constexpr float kLn2 = 0.69314718055994530942f;
 // (FP32) 1.2 and 1.7 times in a wave's 40 blocks of 10,007 rows, with 2^8 4.9
 // times; a weight is then off by at most 2^-30 and 2^-31 of the largest.
 constexpr float kHeadroom = 8.0f, kWideHeadroom16 = 5.0f, kWideHeadroom32 = 6.0f;
+
+// A product that is rounded by itself, whatever is added to it.
+__device__ __forceinline__ float product(float a, float b) {
+#pragma clang fp contract(off)
+    return a * b;
+}
+
+// The reference of weights whose largest score is `top`: `headroom` below it, or
+// `top` itself where FP32's step there is so large that more than 15 lie between
+// (a weight must not pass FP16's 65,504).
+__device__ __forceinline__ float reference(float top, float headroom) {
+    const float r = top - headroom;
+    return top - r > 15.0f ? top : r;
+}
 
 // The writer of one query's output: dims d .. +3.
 template <typename T>
@@ -1025,7 +1040,8 @@ __global__ __launch_bounds__(kWaves * 64) void icl4_rows_kernel(AttendArgs p) {
                 if constexpr (PAIRS) s[kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[m], s[kb], 0, 0, 0);
                 s[kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[m], s[kb], 0, 0, 0);
             }
-            s[kb] *= c;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[kb][r] = product(s[kb][r], c);
         }
         if (more) load_keys(next);
         // Register r of s[2 s + b]: row 32 s + 16 (g / 2) + 8 b + 4 (g % 2) + r.
@@ -1044,7 +1060,7 @@ __global__ __launch_bounds__(kWaves * 64) void icl4_rows_kernel(AttendArgs p) {
             for (int r = 0; r < 4; ++r) mt = fmaxf(mt, s[kb][r]);
         mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
         mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-        const float m_new = fmaxf(m_run, mt - kHeadroom);  // finite: the block has an attended row
+        const float m_new = fmaxf(m_run, reference(mt, kHeadroom));  // finite: the block has an attended row
         const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
         m_run = m_new;
         l_run *= alpha;
@@ -1221,6 +1237,10 @@ __global__ __launch_bounds__(kWaves * 64, NJ == 1 ? 3 : 2) void icl4_wide_kernel
     if (more) load_keys(tiles + (long long)at * kBlockBytes), load_values(tiles + (long long)at * kBlockBytes);
     u32x6 parts[NJ][PARTS];
     float c[NJ];
+    bool far = false;
+    float units[32];  // of the lane's dims of keys
+    load16(p.units + pair * 64 + 32 * h, units);
+    load16(p.units + pair * 64 + 32 * h + 16, units + 16);
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
         const int row = min(32 * (NJ * qt + j) + r32, p.q_rows - 1);
@@ -1228,8 +1248,10 @@ __global__ __launch_bounds__(kWaves * 64, NJ == 1 ? 3 : 2) void icl4_wide_kernel
         float x[32];
         load16(src, x);
         load16(src + 16, x + 16);
-        float m = 0.f, nan = 0.f;
+        float m = 0.f, nan = 0.f, reach = 0.f;
         f32x16 even, odd;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) reach = fmaf(fabsf(x[i]), units[i], reach);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             even[i] = x[2 * i], odd[i] = x[2 * i + 1];
@@ -1241,6 +1263,12 @@ __global__ __launch_bounds__(kWaves * 64, NJ == 1 ? 3 : 2) void icl4_wide_kernel
         query_parts<PARTS>(even, odd, pow2(ex), parts[j]);
         // A query that is not finite makes NaN of its own scores alone.
         c[j] = p.scale * pow2(ex) + halves_sum(nan);
+        // Scores that may reach 2^22 (no key's size passes 127 units) are products rounded by themselves, against which
+        // a reference can be held; weights take the others as they are multiplied. The factor waits in LDS, a lane's own.
+        const bool is_far = !(halves_sum(reach) * (127.0f * p.scale) < 4194304.0f);
+        (h ? red_m : red_l)[wave][32 * j + r32] = is_far ? c[j] : 1.0f;
+        c[j] = is_far ? 1.0f : c[j];
+        far = far || __any(is_far);
     }
     // The products take exponents from vector registers only.
     int part_exps = kPartExps, part_exps4 = kPartExps4, one_exp = 127, most_exp = 254;
@@ -1308,6 +1336,14 @@ __global__ __launch_bounds__(kWaves * 64, NJ == 1 ? 3 : 2) void icl4_wide_kernel
                 s[j][1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a1, one, s[j][1], 4, 2, 0, most_exp, 0, one_exp);
             }
         }
+        if (far) {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const float f = (h ? red_m : red_l)[wave][32 * j + r32];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[j][0][r] = product(s[j][0][r], f), s[j][1][r] = product(s[j][1][r], f);
+            }
+        }
         if (more) load_keys(next);
         half8 ph[NJ][4], pl[PAIRS ? NJ : 1][4];
 #pragma unroll
@@ -1344,7 +1380,8 @@ __global__ __launch_bounds__(kWaves * 64, NJ == 1 ? 3 : 2) void icl4_wide_kernel
             // others of its wave do.
             auto raise = [&](bool past, float mt) {
                 const bool fits = halves_max(past ? 1.f : 0.f) == 0.f;
-                const float ref_new = fits ? ref[j] : fmaxf(ref[j], halves_max(mt) * c[j] - (PAIRS ? kWideHeadroom32 : kWideHeadroom16));
+                const float top = product(halves_max(mt), c[j]);
+                const float ref_new = fits ? ref[j] : fmaxf(ref[j], reference(top, PAIRS ? kWideHeadroom32 : kWideHeadroom16));
                 const float alpha = __builtin_amdgcn_exp2f(ref[j] - ref_new);
                 ref[j] = ref_new;
                 l_run[j] *= alpha;
@@ -1356,7 +1393,7 @@ __global__ __launch_bounds__(kWaves * 64, NJ == 1 ? 3 : 2) void icl4_wide_kernel
             float l;
             if constexpr (PAIRS) {
                 const float mt = largest();
-                const bool past = !(mt * c[j] - ref[j] <= 15.0f);
+                const bool past = !(fmaf(mt, c[j], -ref[j]) <= 15.0f);
                 if (__any(past)) raise(past, mt);
                 l = weigh();
             } else {
@@ -1587,7 +1624,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void icl4_one_kernel(AttendArgs p) {
             IRX_SCORES(3)
 #undef IRX_SCORES
             if (live) load_keys(in);
-            float x = ((s[0] + s[1]) + (s[2] + s[3])) * c;
+            float x = product((s[0] + s[1]) + (s[2] + s[3]), c);
             if (!(whole >> now & 1)) {
                 const unsigned long long m = (unsigned long long)(unsigned)__builtin_amdgcn_readlane(high, now) << 32 |
                                              (unsigned)__builtin_amdgcn_readlane(low, now);
@@ -1595,7 +1632,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void icl4_one_kernel(AttendArgs p) {
             }
             float weight = __builtin_amdgcn_exp2f(x - ref);
             if (__any(!(weight <= 32768.0f))) {
-                const float ref_new = fmaxf(ref, wave_max(x) - kHeadroom);
+                const float ref_new = fmaxf(ref, reference(wave_max(x), kHeadroom));
                 const float alpha = __builtin_amdgcn_exp2f(ref - ref_new);
                 l_run *= alpha;
 #pragma unroll
@@ -1882,7 +1919,7 @@ void attend(const Icl4Queries &a, const Icl4Attend &b, hipStream_t stream) {
     AttendArgs p{};
     p.q = a.q, p.q_est = a.q_strides[0], p.q_head = a.q_strides[1], p.q_row = a.q_strides[2];
     p.o = b.out, p.o_est = b.o_strides[0], p.o_head = b.o_strides[1], p.o_row = b.o_strides[2];
-    p.lse = b.lse, p.tiles = parts(a.cache, s).tiles, p.lengths = a.lengths, p.keep = a.keep;
+    p.lse = b.lse, p.tiles = parts(a.cache, s).tiles, p.units = parts(a.cache, s).scales, p.lengths = a.lengths, p.keep = a.keep;
     p.list = b.list, p.n = b.n, p.heads = s.heads, p.pairs = s.pairs(), p.q_rows = a.q_rows, p.rows = s.rows;
     p.blocks = s.blocks(), p.scale = b.scale * kLog2e, p.partial = static_cast<float *>(b.workspace);
     p.splits = pl.splits, p.per_split = pl.per_split, p.qtiles = pl.qtiles;

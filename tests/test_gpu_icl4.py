@@ -290,6 +290,36 @@ def test_attention_of_peaked_and_extreme_scores(device, element, rows):
     check(attend(device, cache, (1, 2, n), q, element, scale=0.3), want.attend(q, scale=0.3), element, want)
 
 
+@pytest.mark.parametrize("element", ["f32", "f16"])
+@pytest.mark.parametrize("rows,listed", [(1, False), (2, False), (5, False), (70, False), (2100, False), (5, True)])
+def test_scores_past_what_fp32_tells_apart(device, element, rows, listed):
+    """Scores of 2^18 to 2^40, where FP32's step is 2^-5 to 2^17. Two equal keys lie far above the others (8 times their
+    scores and more), so each query gets the mean of their values, with two equal weights w. As pairs they and their
+    products are off by 2^-20 of the values. Rounded to FP16 both are off by the same 2^-11 at most, and the sum of
+    weights that divides them is not rounded: 2^-11 of the mean, and the output's rounding as much again. The
+    log-sum-exp is the score and log 2, off by 2^-19 of it."""
+    e, h, n = 2, 8, 900
+    rng = np.random.default_rng(rows)
+    k = rng.choice([-0.5, 0.5, 1.0], (e, h, n, 64)).astype(DTYPES[element])
+    k[:, :, 333] = k[:, :, 800] = 8.0
+    v = draw((e, h, n, 64), element, 3)
+    cache, want = make(device, e, h, n, element, k=k, v=v)
+    expected = (want.v[:, :, None, 333] + want.v[:, :, None, 800]) / 2
+    bound = np.abs(expected) * 2.0 ** -19 + np.abs(want.v).max() * 2.0 ** -20
+    if element == "f16":
+        bound = bound + np.abs(expected) * 2.0 ** -10 + 2.0 ** -25
+    size = 2.0 ** rng.uniform(0, 8, (e, h, rows, 1))
+    q = np.broadcast_to(size, (e, h, rows, 64)).astype(DTYPES[element])
+    tiles = -(-n // 64)
+    blocks = np.broadcast_to(np.arange(tiles, dtype=np.int32), (e, h, rows, tiles)) if listed else None
+    for power in (9, 16, 23, 31):
+        scale = 2.0 ** power
+        out, lse = attend(device, cache, (e, h, n), q, element, blocks=blocks, scale=scale)
+        assert np.all(np.abs(out - expected) <= bound), power
+        total = q[..., 0].astype(np.float64) * 512 * scale + np.log(2.0)
+        assert np.all(np.abs(lse - total) <= total * 2.0 ** -19), power
+
+
 def test_large_fp32_queries(device):
     """Queries past FP16's range, with a scale that brings their scores back."""
     cache, want = make(device, 1, 8, 300)
