@@ -419,10 +419,10 @@ int irx_icl4_decode(irx_device *device, const void *cache, const irx_icl4_rows *
 /* For each (estimator, head, query) the n_blocks (1 to 4,096) blocks with the
  * highest scores among those with a row to attend to, ties to the lower block,
  * into blocks [E, H, query_rows, n_blocks]: ascending, then -1 where there are
- * fewer. A score bounds q k over the block's rows: with x = q * unit, f the
- * smallest integer >= -100 with max |x| <= 127 * 2^f and c = x / 2^f rounded to
- * the nearest integer (ties to even), it is sum over the dims of max(c low, c
- * high), a whole number. */
+ * fewer. A score bounds q k over the block's rows: with x = q * unit (within
+ * FP32's range), f the smallest integer >= -100 with max |x| <= 127 * 2^f and c =
+ * x / 2^f rounded to the nearest integer (ties to even), it is sum over the dims
+ * of max(c low, c high), a whole number. */
 int irx_icl4_select(irx_device *device, const irx_icl4_queries *queries, const void *cache, size_t n_blocks,
                     int32_t *blocks, void *workspace, size_t workspace_bytes, void *stream);
 /* softmax(scale q k^T) v over the attended rows, scale finite and positive, into
@@ -433,7 +433,7 @@ int irx_icl4_select(irx_device *device, const irx_icl4_queries *queries, const v
  * n_blocks 0: every block. lse, when not NULL, [E, H, query_rows] FP32: the
  * natural logarithm of the sum of exp(scale q k), -inf for a query that attends
  * to none. Results do not depend on other calls or on the workspace's contents.
- * Scores must lie within FP32's range. What is rounded: an FP32 query with
+ * scale q and scores must lie within FP32's range. What is rounded: an FP32 query with
  * blocks, or of one or two a call, to 31 bits of its largest number, of up to 16
  * to a pair of FP16 values (22 bits a number), of more to 2^-24 of its largest;
  * an FP16 query is exact, but with blocks numbers are rounded to 2^-30 of its

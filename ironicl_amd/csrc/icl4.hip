@@ -518,7 +518,7 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ int code_power(float m) {
     const unsigned bits = __float_as_uint(m);
     const int x = (int)(bits >> 23) - 126;  // zero and subnormal m end at -100
-    return min(120, max(-100, (bits & 0x7fffffu) <= 0x7e0000u ? x - 7 : x - 6));
+    return min(122, max(-100, (bits & 0x7fffffu) <= 0x7e0000u ? x - 7 : x - 6));  // 122: the largest finite m's
 }
 
 // A query's codes as operands: lane (g, i16) dims 16 g .. of query i16,

@@ -449,6 +449,19 @@ def test_select_of_queries_of_any_size(device):
     np.testing.assert_array_equal(select(device, cache, (1, 2, 900), q, 5), want.select(q, 5))
 
 
+def test_select_of_the_largest_products(device):
+    """Units of 2^9, and products with them up to FP32's largest number, whose codes take the largest power of two."""
+    for tiles in (15, 600):
+        k = draw((1, 1, 64 * tiles, 64), "f32", 3, 10000.0)
+        k[0, 0, 0] = 49152.0
+        cache, want = make(device, 1, 1, 64 * tiles, k=k, v=k)
+        assert np.all(want.units == 512.0)
+        q = draw((1, 1, 6, 64), "f32", 2)
+        largest = np.array([3.4e38, 3.0e38, 1.8e38, 1.6e38, 8e37, 1e37]) / 512
+        q *= (largest / np.abs(q[0, 0]).max(-1)).astype(np.float32)[None, None, :, None]
+        np.testing.assert_array_equal(select(device, cache, (1, 1, 64 * tiles), q, 5), want.select(q, 5))
+
+
 @pytest.mark.parametrize("element,layout", [("f32", "heads"), ("f16", "tokens")])
 @pytest.mark.parametrize("e,h,n,rows,count", [(1, 8, 1, 1, 1), (1, 8, 640, 3, 4), (2, 3, 1000, 20, 16), (1, 1, 9000, 2, 100),
                                               (1, 2, 777, 300, 3), (1, 8, 640, 600, 70), (1, 2, 640, 300, 300)])
