@@ -900,7 +900,9 @@ struct AttendArgs {
     int n;
     int heads, pairs, q_rows, rows, blocks;
     float scale;      // times log2 e
-    float *partial;   // outputs [splits, pairs * q_rows, 64], then log2-sum-exps [splits, pairs * q_rows]
+    // Outputs [splits, part_rows, 64], then [splits, part_rows, 2]: their softmax's reference (log2) and the sum of weights
+    // against it. Apart, not as one logarithm: next to a reference of 2^20 that would keep a sum to three bits.
+    float *partial;
     int splits, per_split;  // blocks (or listed places) of a split
     int qtiles, count, per_xcd;
     Division by_qtiles, by_splits, by_queries, by_heads;
@@ -942,6 +944,13 @@ __device__ __forceinline__ void store_out(const AttendArgs &p, int e, int head, 
         typedef _Float16 half4 __attribute__((ext_vector_type(4)));
         *reinterpret_cast<half4 *>(dst) = __builtin_convertvector(v, half4);
     }
+}
+
+// The same of a split's row `at` of all splits' (`all` rows each).
+__device__ __forceinline__ void store_part(const AttendArgs &p, long long all, long long at, int d, f32x4 v, float reference,
+                                           float sum) {
+    *reinterpret_cast<f32x4 *>(p.partial + at * 64 + d) = v;
+    if (d == 0) *reinterpret_cast<f32x2 *>(p.partial + p.splits * all * 64 + 2 * at) = f32x2{reference, sum};
 }
 
 constexpr int kWaves = 4;
@@ -1114,15 +1123,13 @@ __global__ __launch_bounds__(kWaves * 64) void icl4_rows_kernel(AttendArgs p) {
         den += a * red_l[w][qi];
     }
     if (den != 0.f) acc *= 1.0f / den;
-    const float lse2 = mx + log2f(den);  // -inf where nothing is attended
     if constexpr (SPLIT) {
         const long long all = (long long)p.pairs * p.q_rows;
-        const long long at = split * all + (long long)pair * p.q_rows + out_row;
-        *reinterpret_cast<f32x4 *>(p.partial + at * 64 + d) = acc;
-        if (d == 0) p.partial[p.splits * all * 64 + at] = lse2;
+        store_part(p, all, split * all + (long long)pair * p.q_rows + out_row, d, acc, mx, den);
     } else {
         store_out<T>(p, e, head, out_row, d, acc);
-        if (p.lse && d == 0) p.lse[(long long)pair * p.q_rows + out_row] = lse2 * kLn2;
+        // -inf where nothing is attended.
+        if (p.lse && d == 0) p.lse[(long long)pair * p.q_rows + out_row] = (mx + log2f(den)) * kLn2;
     }
 }
 
@@ -1450,14 +1457,12 @@ __global__ __launch_bounds__(kWaves * 64, NJ == 1 ? 3 : 2) void icl4_wide_kernel
             den += a * red_l[w][q];
         }
         if (den != 0.f) acc *= 1.0f / den;
-        const float lse2 = mx + log2f(den);
         if (tail && p.splits > 1) {
-            const long long all = (long long)p.by_rest.d * (32 * NJ), to = split * all + (long long)(unit - p.whole) * (32 * NJ) + q;
-            *reinterpret_cast<f32x4 *>(p.partial + to * 64 + d) = acc;
-            if (d == 0) p.partial[p.splits * all * 64 + to] = lse2;
+            const long long all = (long long)p.by_rest.d * (32 * NJ);
+            store_part(p, all, split * all + (long long)(unit - p.whole) * (32 * NJ) + q, d, acc, mx, den);
         } else {
             store_out<T>(p, e, head, row, d, acc);
-            if (p.lse && d == 0) p.lse[(long long)pair * p.q_rows + row] = lse2 * kLn2;
+            if (p.lse && d == 0) p.lse[(long long)pair * p.q_rows + row] = (mx + log2f(den)) * kLn2;
         }
     }
 }
@@ -1683,14 +1688,12 @@ __global__ __launch_bounds__(WAVES * 64, 4) void icl4_one_kernel(AttendArgs p) {
         den += a * red_l[w];
     }
     if (den != 0.f) acc *= 1.0f / den;
-    const float lse2 = mx + log2f(den);
     if constexpr (SPLIT) {
-        const long long all = (long long)p.pairs * p.q_rows, to = split * all + pq;
-        *reinterpret_cast<f32x4 *>(p.partial + to * 64 + d) = acc;
-        if (d == 0) p.partial[p.splits * all * 64 + to] = lse2;
+        const long long all = (long long)p.pairs * p.q_rows;
+        store_part(p, all, split * all + pq, d, acc, mx, den);
     } else {
         store_out<T>(p, e, head, row, d, acc);
-        if (p.lse && d == 0) p.lse[pq] = lse2 * kLn2;
+        if (p.lse && d == 0) p.lse[pq] = (mx + log2f(den)) * kLn2;
     }
 }
 
@@ -1704,30 +1707,30 @@ __global__ __launch_bounds__(256) void icl4_merge_kernel(AttendArgs p) {
     const int tid = threadIdx.x, slot = tid >> 4, group = slot % GROUPS, d = 4 * (tid & 15);
     const long long mine = (long long)blockIdx.x * (16 / GROUPS) + slot / GROUPS;
     const long long at_row = min(mine, all - 1);
-    const float *lse = p.partial + p.splits * all * 64 + at_row;
+    const float *sum_of = p.partial + p.splits * all * 64 + 2 * at_row;  // reference and sum
     const float *part = p.partial + at_row * 64 + d;
     // Eight splits' loads at once; slots past the last read it again and weigh nothing.
     float ref = -INFINITY, den = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     for (int s0 = group; s0 < p.splits; s0 += 8 * GROUPS) {
-        float l[8];
+        f32x2 l[8];
         f32x4 v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int s = s0 + i * GROUPS, at = min(s, p.splits - 1);
-            l[i] = lse[at * all];
+            l[i] = *reinterpret_cast<const f32x2 *>(sum_of + 2 * at * all);
             v[i] = *reinterpret_cast<const f32x4 *>(part + at * all * 64);
-            if (s >= p.splits) l[i] = -INFINITY, v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (s >= p.splits) l[i] = f32x2{-INFINITY, 0.f}, v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
         float top = ref;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, l[i]);
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, l[i][0]);
         const float base = top > -INFINITY ? top : 0.f;
         const float a = __builtin_amdgcn_exp2f(ref - base);
         acc *= a, den *= a;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float w = __builtin_amdgcn_exp2f(l[i] - base);
+            const float w = __builtin_amdgcn_exp2f(l[i][0] - base) * l[i][1];
             acc += w * v[i];
             den += w;
         }
@@ -1956,7 +1959,7 @@ void attend(const Icl4Queries &a, const Icl4Attend &b, hipStream_t stream) {
         IRX_HIP(hipGetLastError());
     }
     if (pl.splits > 1) {
-        KernelTimer timer(kFamIclMerge, stream, 0.0, 4.0 * pl.part_rows * (65.0 * pl.splits + 64.0));
+        KernelTimer timer(kFamIclMerge, stream, 0.0, 4.0 * pl.part_rows * (66.0 * pl.splits + 64.0));
         // A lane's splits come eight at a time: more groups where there are more splits (one group for 49 splits of 8
         // rows 4 us more than sixteen, for 32 of 128 rows 2.3 more than four).
         if (pl.splits <= 8)
@@ -1977,7 +1980,7 @@ size_t icl4_bytes(const Icl4Shape &s) {
 
 size_t icl4_attend_workspace(const Icl4Shape &s, bool half, int q_rows, int n_blocks, int compute_units) {
     const Plan pl = plan_attend(s, half, q_rows, n_blocks, compute_units);
-    return pl.splits > 1 ? (size_t)pl.splits * (size_t)pl.part_rows * 65 * sizeof(float) : 0;
+    return pl.splits > 1 ? (size_t)pl.splits * (size_t)pl.part_rows * 66 * sizeof(float) : 0;
 }
 
 size_t icl4_select_workspace(const Icl4Shape &s, int q_rows) {

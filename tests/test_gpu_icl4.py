@@ -320,6 +320,56 @@ def test_scores_past_what_fp32_tells_apart(device, element, rows, listed):
         assert np.all(np.abs(lse - total) <= total * 2.0 ** -19), power
 
 
+@pytest.mark.parametrize("element", ["f32", "f16"])
+@pytest.mark.parametrize("e,h,n,rows,listed", [(1, 2, 20011, 1, 0), (1, 2, 20011, 2, 0), (1, 2, 20011, 5, 0),
+                                               (2, 1, 20011, 16, 0), (1, 2, 20011, 70, 0), (2, 8, 9001, 2100, 0),
+                                               (1, 2, 70000, 3, 1000)])
+def test_large_equal_scores_in_different_splits(device, e, h, n, rows, listed, element):
+    """Seven equal keys in the first block and one in the last, which another split takes, at scores of 2^16 to 2^31:
+    eight equal weights, whatever plan the sizes get. Bounds as for two of them: pairs and eight FP32 sums of products
+    are off by 2^-20 of the values, FP16 weights all by the same 2^-11, and the output's rounding by as much again."""
+    assert icl4.workspace_bytes(device, (e, h, n), rows, listed) > 0
+    rng = np.random.default_rng(rows)
+    k = rng.choice([-0.5, 0.5, 1.0], (e, h, n, 64)).astype(DTYPES[element])
+    tied = np.r_[2:63:10, n - 3]
+    k[:, :, tied] = 8.0
+    v = draw((e, h, n, 64), element, 3)
+    cache, want = make(device, e, h, n, element, k=k, v=v)
+    expected = want.v[:, :, None, tied].mean(3)
+    bound = np.abs(expected) * 2.0 ** -19 + np.abs(want.v).max() * 2.0 ** -20
+    if element == "f16":
+        bound = bound + np.abs(expected) * 2.0 ** -10 + 2.0 ** -25
+    q = np.broadcast_to(rng.uniform(1, 2, (e, h, rows, 1)), (e, h, rows, 64)).astype(DTYPES[element])
+    blocks = None
+    if listed:
+        tiles = -(-n // 64)
+        blocks = np.broadcast_to(np.r_[0:listed - 1, tiles - 1].astype(np.int32), (e, h, rows, listed))
+    for power in (7, 12, 17, 21):
+        scale = 2.0 ** power
+        out, lse = attend(device, cache, (e, h, n), q, element, blocks=blocks, scale=scale)
+        assert np.all(np.abs(out - expected) <= bound), power
+        total = q[..., 0].astype(np.float64) * 512 * scale + np.log(8.0)
+        assert np.all(np.abs(lse - total) <= total * 2.0 ** -19), power
+
+
+@pytest.mark.parametrize("element", ["f32", "f16"])
+@pytest.mark.parametrize("n,rows,listed", [(20011, 1, 0), (20011, 5, 0), (20011, 70, 0), (70000, 3, 1000)])
+def test_a_query_that_is_not_a_number_stays_alone_in_splits(device, n, rows, listed, element):
+    assert icl4.workspace_bytes(device, (1, 2, n), rows, listed) > 0
+    cache, _ = make(device, 1, 2, n, element)
+    q = draw((1, 2, rows, 64), element, 4)
+    blocks = np.broadcast_to(np.arange(listed, dtype=np.int32), (1, 2, rows, listed)) if listed else None
+    whole, whole_lse = attend(device, cache, (1, 2, n), q, element, blocks=blocks)
+    for bad in (np.nan, np.inf):
+        q[0, 1, rows - 1, 9] = bad
+        got, lse = attend(device, cache, (1, 2, n), q, element, blocks=blocks)
+        others = np.ones((1, 2, rows), bool)
+        others[0, 1, rows - 1] = False
+        np.testing.assert_array_equal(got[others], whole[others])
+        np.testing.assert_array_equal(lse[others], whole_lse[others])
+        assert np.isnan(got[0, 1, rows - 1]).all() and np.isnan(lse[0, 1, rows - 1])
+
+
 def test_large_fp32_queries(device):
     """Queries past FP16's range, with a scale that brings their scores back."""
     cache, want = make(device, 1, 8, 300)
