@@ -1268,8 +1268,9 @@ __global__ __launch_bounds__(kWaves * 64, NJ == 1 ? 3 : 2) void icl4_wide_kernel
         // The least unit leaves 2^-19 of it normal.
         const int ex = max(-100, (int)(__float_as_uint(halves_max(m)) >> 23) - 128);
         query_parts<PARTS>(even, odd, pow2(ex), parts[j]);
-        // A query that is not finite makes NaN of its own scores alone.
-        c[j] = p.scale * pow2(ex) + halves_sum(nan);
+        // A query that is not finite makes NaN of its own scores alone. The factor is normal, for -inf, a masked score,
+        // times 0 is no score; one that is less makes nothing of any score either way (they are below 2^25).
+        c[j] = fmaxf(p.scale * pow2(ex), 1.17549435e-38f) + halves_sum(nan);
         // Scores that may reach 2^22 (no key's size passes 127 units) are products rounded by themselves, against which
         // a reference can be held; weights take the others as they are multiplied. The factor waits in LDS, a lane's own.
         const bool is_far = !(halves_sum(reach) * (127.0f * p.scale) < 4194304.0f);

@@ -370,6 +370,25 @@ def test_a_query_that_is_not_a_number_stays_alone_in_splits(device, n, rows, lis
         assert np.isnan(got[0, 1, rows - 1]).all() and np.isnan(lse[0, 1, rows - 1])
 
 
+@pytest.mark.parametrize("element", ["f32", "f16"])
+@pytest.mark.parametrize("e,rows,listed", [(2, 1, False), (2, 16, False), (2, 20, False), (2, 70, False),
+                                           (16, 2100, False), (2, 5, True)])
+def test_zero_queries_at_the_smallest_scales(device, e, rows, listed, element):
+    """The mean of the attended values and the logarithm of their number, beside masked rows, rows past the last and a
+    query that is not zero."""
+    h, n = 1 if e == 16 else 2, 900
+    keep = np.random.default_rng(1).random((e, n)) < 0.7
+    keep[:, 640:768] = True
+    cache, want = make(device, e, h, n, element)
+    tiles = -(-n // 64)
+    blocks = np.broadcast_to(np.arange(tiles, dtype=np.int32), (e, h, rows, tiles)) if listed else None
+    q = np.zeros((e, h, rows, 64), DTYPES[element])
+    q[:, :, 1::7] = 0.5
+    for scale in (1e-13, 1e-16, 1e-30, 1e-38, 1e-45):
+        got = attend(device, cache, (e, h, n), q, element, keep=keep, blocks=blocks, scale=scale)
+        check(got, want.attend(q, scale=scale, keep=keep, blocks=blocks), element, want)
+
+
 def test_large_fp32_queries(device):
     """Queries past FP16's range, with a scale that brings their scores back."""
     cache, want = make(device, 1, 8, 300)
