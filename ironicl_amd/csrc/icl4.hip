@@ -934,6 +934,12 @@ __device__ __forceinline__ float reference(float top, float headroom) {
     return top - r > 15.0f ? top : r;
 }
 
+// The smallest e with |m| < 2^e of a finite m, subnormal or not (0 and infinity: 0).
+__device__ __forceinline__ int binade(float m) { return __builtin_amdgcn_frexp_expf(m); }
+
+// What a product of 2^-e q and k is multiplied by for its score times log2 e.
+__device__ __forceinline__ float factor(const AttendArgs &p, int e) { return __builtin_ldexpf(p.scale, e); }
+
 // The writer of one query's output: dims d .. +3.
 template <typename T>
 __device__ __forceinline__ void store_out(const AttendArgs &p, int e, int head, int row, int d, f32x4 v) {
@@ -1002,7 +1008,7 @@ __global__ __launch_bounds__(kWaves * 64) void icl4_rows_kernel(AttendArgs p) {
     bool more = find(at, next_mask);
     if (more) load_keys(tiles + (long long)at * kBlockBytes), load_values(tiles + (long long)at * kBlockBytes);
     half8 qh[2], ql[2];
-    float c = p.scale;
+    float c;
     {
         const T *src = static_cast<const T *>(p.q) + e * p.q_est + head * p.q_head + (long long)qrow * p.q_row + 16 * g;
         if constexpr (PAIRS) {
@@ -1018,12 +1024,13 @@ __global__ __launch_bounds__(kWaves * 64) void icl4_rows_kernel(AttendArgs p) {
             m = fmaxf(m, __shfl_xor(m, 32, 64));
             const int ex = pair_exponent(m);
             const float up = pow2(ex);
-            c *= pow2(-ex);
+            c = factor(p, -ex);
 #pragma unroll
             for (int i = 0; i < 16; ++i) x[i] *= up;
             pair8(x, qh[0], ql[0]);
             pair8(x + 8, qh[1], ql[1]);
         } else {
+            c = factor(p, 0);
             qh[0] = *reinterpret_cast<const half8 *>(src);
             qh[1] = *reinterpret_cast<const half8 *>(src + 8);
         }
@@ -1151,16 +1158,16 @@ typedef unsigned u32x6 __attribute__((ext_vector_type(6)));
 typedef float f32x32 __attribute__((ext_vector_type(32)));
 
 // 32 numbers as PARTS operands in E2M3 (multiples of 1/8 below 2, of 1/4 below
-// 4): x = unit (p0 + p1 / 2^4 + p2 / 2^9 + ...), the unit a power of two that
-// brings the largest of the row into [2, 4), each part the nearest to what is
-// left: the first is off by at most 1/8, the next, in a unit 2^-4 and then 2^-5
-// as large, by at most 1/16. What four leave is at most 2^-18 unit, 2^-19 of the
-// row's largest, what five leave 2^-24 of it. (FP16 numbers down to 2^-9 of the
-// largest are whole multiples of that step: exact.) The exponent bytes of parts
-// 0 to 3 and of part 4.
+// 4): x = p0 + p1 / 2^4 + p2 / 2^9 + ..., the largest of a row scaled into [2,
+// 4), each part the nearest to what is left: the first is off by at most 1/8,
+// the next, in a unit 2^-4 and then 2^-5 as large, by at most 1/16. What four
+// leave is at most 2^-18, 2^-19 of the row's largest, what five leave 2^-24 of
+// it. (FP16 numbers down to 2^-9 of the largest are whole multiples of that
+// step: exact.) The exponent bytes of parts 0 to 3 and of part 4.
 constexpr int kPartExps = 127 | (127 - 4) << 8 | (127 - 9) << 16 | (127 - 14) << 24, kPartExps4 = 127 - 19;
 template <int PARTS>
-__device__ __forceinline__ void query_parts(f32x16 &even, f32x16 &odd, float unit, u32x6 (&parts)[PARTS]) {
+__device__ __forceinline__ void query_parts(f32x16 &even, f32x16 &odd, u32x6 (&parts)[PARTS]) {
+    float unit = 1.0f;
 #pragma unroll
     for (int n = 0; n < PARTS; ++n) {
         parts[n] = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, unit);
@@ -1258,22 +1265,25 @@ __global__ __launch_bounds__(kWaves * 64, NJ == 1 ? 3 : 2) void icl4_wide_kernel
         float m = 0.f, nan = 0.f, reach = 0.f;
         f32x16 even, odd;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) reach = fmaf(fabsf(x[i]), units[i], reach);
-#pragma unroll
         for (int i = 0; i < 16; ++i) {
             even[i] = x[2 * i], odd[i] = x[2 * i + 1];
             m = fmaxf(m, fmaxf(fabsf(even[i]), fabsf(odd[i])));
             nan = fmaf(odd[i], 0.f, fmaf(even[i], 0.f, nan));
         }
-        // The least unit leaves 2^-19 of it normal.
-        const int ex = max(-100, (int)(__float_as_uint(halves_max(m)) >> 23) - 128);
-        query_parts<PARTS>(even, odd, pow2(ex), parts[j]);
+        // The largest into [2, 4).
+        const int ex = binade(halves_max(m)) - 2;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            even[i] = __builtin_ldexpf(even[i], -ex), odd[i] = __builtin_ldexpf(odd[i], -ex);
+            reach = fmaf(fabsf(even[i]), units[2 * i], fmaf(fabsf(odd[i]), units[2 * i + 1], reach));
+        }
+        query_parts<PARTS>(even, odd, parts[j]);
         // A query that is not finite makes NaN of its own scores alone. The factor is normal, for -inf, a masked score,
         // times 0 is no score; one that is less makes nothing of any score either way (they are below 2^25).
-        c[j] = fmaxf(p.scale * pow2(ex), 1.17549435e-38f) + halves_sum(nan);
+        c[j] = fmaxf(factor(p, ex), 1.17549435e-38f) + halves_sum(nan);
         // Scores that may reach 2^22 (no key's size passes 127 units) are products rounded by themselves, against which
         // a reference can be held; weights take the others as they are multiplied. The factor waits in LDS, a lane's own.
-        const bool is_far = !(halves_sum(reach) * (127.0f * p.scale) < 4194304.0f);
+        const bool is_far = !(halves_sum(reach) * (127.0f * c[j]) < 4194304.0f);
         (h ? red_m : red_l)[wave][32 * j + r32] = is_far ? c[j] : 1.0f;
         c[j] = is_far ? 1.0f : c[j];
         far = far || __any(is_far);
@@ -1517,7 +1527,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void icl4_one_kernel(AttendArgs p) {
     const int rows = rows_of(p.lengths, e, p.rows);
     _Float16 *weights = shared_weights[wave][0];
     i32x8 digits;
-    float c = p.scale;
+    float c;
     {
         // Terms 16 g .. and 64 + 16 g .. stand in lane (g, .): dims 16 (g / 2) .. and 32 more, digit 2 (i16 % 4) + g % 2.
         // Every fourth lane of a row makes a part: dims 4 (i16 / 4) .. +3 of both.
@@ -1538,10 +1548,8 @@ __global__ __launch_bounds__(WAVES * 64, 4) void icl4_one_kernel(AttendArgs p) {
         m = fmaxf(m, __uint_as_float(row_xor<8>(__float_as_uint(m))));
         m = halves_max(m);
         // The largest into [2^29, 2^30).
-        const int ex = min(126, 29 - ((int)(__float_as_uint(m) >> 23) - 127));
-        c *= pow2(-ex);
-        if (!__all(finite)) c = NAN;
-        const float up = pow2(ex);
+        const int ex = 30 - binade(m);
+        c = __all(finite) ? factor(p, -ex) : NAN;
         const int digit = 2 * (i16 & 3) + (g & 1), sh = 28 - 4 * digit;
         const float first = g & 1 ? 1.0f : 16.0f;
         unsigned *words = reinterpret_cast<unsigned *>(weights);
@@ -1550,7 +1558,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void icl4_one_kernel(AttendArgs p) {
             float y[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int whole = (int)fminf(fmaxf(rintf(x[4 * n + i] * up), -1073741824.f), 1073741824.f);
+                const int whole = (int)fminf(fmaxf(rintf(__builtin_ldexpf(x[4 * n + i], ex)), -1073741824.f), 1073741824.f);
                 y[i] = (float)(digit ? (whole >> sh) & 15 : whole >> 28) * first;
             }
             int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);

@@ -389,6 +389,25 @@ def test_zero_queries_at_the_smallest_scales(device, e, rows, listed, element):
         check(got, want.attend(q, scale=scale, keep=keep, blocks=blocks), element, want)
 
 
+@pytest.mark.parametrize("rows,listed", [(1, 0), (3, 0), (16, 0), (40, 0), (600, 0), (5, 13), (9000, 3)])
+@pytest.mark.parametrize("power", [90, 99, 105, 112, 120, 126])
+def test_tiny_fp32_queries(device, rows, listed, power):
+    """Queries near FP32's smallest numbers (their smaller ones below its smallest normal number), with a scale that
+    brings their scores back: bit for bit what the same queries times 2^power give at a scale of 1/8."""
+    cache, want = make(device, 1, 2, 900)
+    q = np.ldexp(draw((1, 2, rows, 64), "f32", 4, 1.5).astype(np.float64), -power).astype(np.float32)
+    blocks = np.random.default_rng(5).integers(0, 15, (1, 2, rows, listed)).astype(np.int32) if listed else None
+    scale = 0.125 * 2.0 ** power
+    got = attend(device, cache, (1, 2, 900), q, blocks=blocks, scale=scale)
+    back = np.ldexp(q.astype(np.float64), power).astype(np.float32)
+    whole = attend(device, cache, (1, 2, 900), back, blocks=blocks)
+    np.testing.assert_array_equal(got[0], whole[0])
+    np.testing.assert_array_equal(got[1], whole[1])
+    some = np.r_[0:rows:37, rows - 1]
+    check((got[0][:, :, some], got[1][:, :, some]),
+          want.attend(q[:, :, some], scale=scale, blocks=None if blocks is None else blocks[:, :, some]), "f32", want)
+
+
 def test_large_fp32_queries(device):
     """Queries past FP16's range, with a scale that brings their scores back."""
     cache, want = make(device, 1, 8, 300)
