@@ -899,7 +899,7 @@ struct AttendArgs {
     const int *list;  // [pairs, q_rows, n] or null
     int n;
     int heads, pairs, q_rows, rows, blocks;
-    float scale;      // times log2 e
+    float scale;
     // Outputs [splits, part_rows, 64], then [splits, part_rows, 2]: their softmax's reference (log2) and the sum of weights
     // against it. Apart, not as one logarithm: next to a reference of 2^20 that would keep a sum to three bits.
     float *partial;
@@ -938,7 +938,7 @@ __device__ __forceinline__ float reference(float top, float headroom) {
 __device__ __forceinline__ int binade(float m) { return __builtin_amdgcn_frexp_expf(m); }
 
 // What a product of 2^-e q and k is multiplied by for its score times log2 e.
-__device__ __forceinline__ float factor(const AttendArgs &p, int e) { return __builtin_ldexpf(p.scale, e); }
+__device__ __forceinline__ float factor(const AttendArgs &p, int e) { return __builtin_ldexpf(p.scale, e) * kLog2e; }
 
 // The writer of one query's output: dims d .. +3.
 template <typename T>
@@ -1933,7 +1933,7 @@ void attend(const Icl4Queries &a, const Icl4Attend &b, hipStream_t stream) {
     p.o = b.out, p.o_est = b.o_strides[0], p.o_head = b.o_strides[1], p.o_row = b.o_strides[2];
     p.lse = b.lse, p.tiles = parts(a.cache, s).tiles, p.units = parts(a.cache, s).scales, p.lengths = a.lengths, p.keep = a.keep;
     p.list = b.list, p.n = b.n, p.heads = s.heads, p.pairs = s.pairs(), p.q_rows = a.q_rows, p.rows = s.rows;
-    p.blocks = s.blocks(), p.scale = b.scale * kLog2e, p.partial = static_cast<float *>(b.workspace);
+    p.blocks = s.blocks(), p.scale = b.scale, p.partial = static_cast<float *>(b.workspace);
     p.splits = pl.splits, p.per_split = pl.per_split, p.qtiles = pl.qtiles;
     const bool wide = pl.queries > 16;
     const long long count = (wide ? pl.rest : (long long)pl.qtiles * s.pairs()) * pl.splits;

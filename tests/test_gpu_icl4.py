@@ -408,6 +408,17 @@ def test_tiny_fp32_queries(device, rows, listed, power):
           want.attend(q[:, :, some], scale=scale, blocks=None if blocks is None else blocks[:, :, some]), "f32", want)
 
 
+@pytest.mark.parametrize("rows,listed", [(1, 0), (3, 0), (40, 0), (5, 13)])
+def test_the_largest_fp32_queries_at_scales_below_the_smallest_normal_number(device, rows, listed):
+    """A scale of two bits, whose product with log2 e has more."""
+    cache, want = make(device, 1, 2, 900, k=draw((1, 2, 900, 64), "f32", 3, 4096.0))
+    q = np.ldexp(draw((1, 2, rows, 64), "f32", 4, 1.5).astype(np.float64), 124).astype(np.float32)
+    blocks = np.random.default_rng(5).integers(0, 15, (1, 2, rows, listed)).astype(np.int32) if listed else None
+    scale = 3 * 2.0 ** -149
+    got = attend(device, cache, (1, 2, 900), q, blocks=blocks, scale=scale)
+    check(got, want.attend(q, scale=scale, blocks=blocks), "f32", want)
+
+
 def test_large_fp32_queries(device):
     """Queries past FP16's range, with a scale that brings their scores back."""
     cache, want = make(device, 1, 8, 300)
