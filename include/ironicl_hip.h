@@ -425,7 +425,7 @@ int irx_icl4_decode(irx_device *device, const void *cache, const irx_icl4_rows *
  * of max(c low, c high), a whole number. */
 int irx_icl4_select(irx_device *device, const irx_icl4_queries *queries, const void *cache, size_t n_blocks,
                     int32_t *blocks, void *workspace, size_t workspace_bytes, void *stream);
-/* softmax(scale q k^T) v over the attended rows, scale finite and positive, into
+/* softmax(scale q k^T) v over the attended rows, scale positive and at most 2^127, into
  * out [E, H, query_rows, 64] at out_strides; a query that attends to no row gets
  * 0. With blocks (n_blocks of them per query, as irx_icl4_select writes) only
  * the listed blocks' rows are attended; entries that are no block of the cache

@@ -2340,7 +2340,9 @@ int irx_icl4_attention(irx_device *device, const irx_icl4_queries *queries, cons
     return guarded("irx_icl4_attention", [&] {
         if (!queries || !cache || !out || !out_strides)
             fail(IRX_INVALID_ARGUMENT, "attention needs queries, a cache and its output");
-        if (!(scale > 0.f) || !std::isfinite(scale)) fail(IRX_INVALID_ARGUMENT, "the scale must be positive and finite");
+        // Its product with log2 e is finite, too.
+        if (!(scale > 0.f && scale <= 0x1p127f))
+            fail(IRX_INVALID_ARGUMENT, "the scale must be positive and finite, at most 2^127");
         if (!blocks != !n_blocks || n_blocks > kIcl4MaxBlocks)
             fail(IRX_INVALID_ARGUMENT, "blocks and n_blocks name 1 to " + std::to_string(kIcl4MaxBlocks) +
                                            " blocks per query, or are NULL and 0");

@@ -419,6 +419,16 @@ def test_the_largest_fp32_queries_at_scales_below_the_smallest_normal_number(dev
     check(got, want.attend(q, scale=scale, blocks=blocks), "f32", want)
 
 
+@pytest.mark.parametrize("element", ["f32", "f16"])
+@pytest.mark.parametrize("rows,listed", [(1, 0), (3, 0), (40, 0), (5, 13)])
+def test_zero_queries_at_the_largest_scale(device, rows, listed, element):
+    cache, want = make(device, 1, 2, 900, element)
+    q = np.zeros((1, 2, rows, 64), DTYPES[element])
+    blocks = np.random.default_rng(5).integers(0, 15, (1, 2, rows, listed)).astype(np.int32) if listed else None
+    got = attend(device, cache, (1, 2, 900), q, element, blocks=blocks, scale=2.0 ** 127)
+    check(got, want.attend(q, blocks=blocks), element, want)
+
+
 def test_large_fp32_queries(device):
     """Queries past FP16's range, with a scale that brings their scores back."""
     cache, want = make(device, 1, 8, 300)

@@ -78,6 +78,12 @@ def test_queries_are_checked():
     refused("needs a device", icl4.attention, SHAPE, Q, Q, 2, Q, out_strides=(0, 64, 512))
 
 
+def test_scales_past_the_largest_are_refused():
+    for scale in (float.fromhex("0x1.000002p127"), 2.4e38, 3.4e38):
+        refused("positive and finite, at most 2\\^127", icl4.attention, SHAPE, Q, Q, 1, Q, scale=scale)
+    refused("needs a device", icl4.attention, SHAPE, Q, Q, 1, Q, scale=2.0 ** 127)
+
+
 def test_unknown_elements_are_refused():
     queries = hip.Icl4Queries(hip.Icl4Shape(*SHAPE), 1, 7, Q, hip.Strides(0, 64, 64), None, None)
     out = hip.Strides(0, 64, 64)
