@@ -969,7 +969,8 @@ constexpr int kWaves = 4;
 template <typename T, bool SPLIT>
 __global__ __launch_bounds__(kWaves * 64) void icl4_rows_kernel(AttendArgs p) {
     constexpr bool PAIRS = sizeof(T) == 4;
-    __shared__ float red_o[kWaves][16 * 68];
+    __shared__ __attribute__((aligned(16))) float red_o[kWaves][16 * 68];
+    static_assert(__alignof__(red_o) >= alignof(f32x4), "read and written in fours");
     __shared__ float red_m[kWaves][16], red_l[kWaves][16];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, i16 = lane & 15;
     const unsigned tile = SPLIT ? divide(blockIdx.x, p.by_splits) : blockIdx.x;
@@ -1204,7 +1205,8 @@ template <typename T, int NJ>
 __global__ __launch_bounds__(kWaves * 64, NJ == 1 ? 3 : 2) void icl4_wide_kernel(AttendArgs p) {
     constexpr bool PAIRS = sizeof(T) == 4;
     constexpr int PARTS = PAIRS ? 5 : 4;
-    __shared__ float red_o[kWaves][32 * NJ * kWideStride];
+    __shared__ __attribute__((aligned(16))) float red_o[kWaves][32 * NJ * kWideStride];
+    static_assert(__alignof__(red_o) >= alignof(f32x4), "read and written in fours");
     __shared__ float red_m[kWaves][32 * NJ], red_l[kWaves][32 * NJ];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int h = lane >> 5, r32 = lane & 31, i16 = lane & 15, x16 = (lane >> 4) & 1;
@@ -1513,7 +1515,8 @@ __device__ __forceinline__ unsigned row_lane(unsigned x) {
 template <typename T, bool LISTED, bool SPLIT, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 4) void icl4_one_kernel(AttendArgs p) {
     constexpr bool PAIRS = sizeof(T) == 4;
-    __shared__ float red_o[WAVES][64];
+    __shared__ __attribute__((aligned(16))) float red_o[WAVES][64];
+    static_assert(__alignof__(red_o) >= alignof(f32x4), "read and written in fours");
     __shared__ float red_m[WAVES], red_l[WAVES];
     __shared__ __attribute__((aligned(16))) _Float16 shared_weights[WAVES][2][64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -1711,7 +1714,8 @@ __global__ __launch_bounds__(WAVES * 64, 4) void icl4_one_kernel(AttendArgs p) {
 // 3.4 to 5 us, the latency of one trip to memory and of a launch.
 template <typename T, int GROUPS>
 __global__ __launch_bounds__(256) void icl4_merge_kernel(AttendArgs p) {
-    __shared__ float sums[GROUPS > 1 ? 16 * 66 : 1];
+    __shared__ __attribute__((aligned(16))) float sums[GROUPS > 1 ? 16 * 66 : 1];
+    static_assert(__alignof__(sums) >= alignof(f32x2), "read and written in pairs");
     const long long all = p.part_rows;
     const int tid = threadIdx.x, slot = tid >> 4, group = slot % GROUPS, d = 4 * (tid & 15);
     const long long mine = (long long)blockIdx.x * (16 / GROUPS) + slot / GROUPS;
