@@ -437,7 +437,10 @@ int irx_icl4_select(irx_device *device, const irx_icl4_queries *queries, const v
  * blocks, or of one or two a call, to 31 bits of its largest number, of up to 16
  * to a pair of FP16 values (22 bits a number), of more to 2^-24 of its largest;
  * an FP16 query is exact, but with blocks numbers are rounded to 2^-30 of its
- * largest, and of more than 16 a call those below 2^-9 of it to 2^-18. Weights
+ * largest, and of more than 16 a call those below 2^-8 of it to 2^-19 of it. Of more
+ * than 16 a call a query is rounded more finely (an FP16 one at last not at all)
+ * while that could move a score by more than 2^-14 and by more than 2^-20 of the
+ * sum over the dims of |scale q| times the largest |k|. Weights
  * are pairs of FP16 values for FP32 queries, else FP16 (rounded once); sums are
  * FP32. */
 int irx_icl4_attention(irx_device *device, const irx_icl4_queries *queries, const void *cache, float scale,

@@ -1163,8 +1163,11 @@ typedef float f32x32 __attribute__((ext_vector_type(32)));
 // 4), each part the nearest to what is left: the first is off by at most 1/8,
 // the next, in a unit 2^-4 and then 2^-5 as large, by at most 1/16. What four
 // leave is at most 2^-18, 2^-19 of the row's largest, what five leave 2^-24 of
-// it. (FP16 numbers down to 2^-9 of the largest are whole multiples of that
-// step: exact.) The exponent bytes of parts 0 to 3 and of part 4.
+// it. (FP16 numbers down to 2^-8 of the largest are whole multiples of the last
+// one's step, 2^-17: exact.) Fixed steps are coarse for a row whose largest
+// number, times small keys, does not make its scores: see kMoreParts. The
+// exponent bytes of parts 0 to 3 and of part 4; `even` and `odd` become what is
+// left.
 constexpr int kPartExps = 127 | (127 - 4) << 8 | (127 - 9) << 16 | (127 - 14) << 24, kPartExps4 = 127 - 19;
 template <int PARTS>
 __device__ __forceinline__ void query_parts(f32x16 &even, f32x16 &odd, u32x6 (&parts)[PARTS]) {
@@ -1172,13 +1175,26 @@ __device__ __forceinline__ void query_parts(f32x16 &even, f32x16 &odd, u32x6 (&p
 #pragma unroll
     for (int n = 0; n < PARTS; ++n) {
         parts[n] = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, unit);
-        if (n == PARTS - 1) break;
         const f32x32 held = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(parts[n], unit);
 #pragma unroll
         for (int i = 0; i < 16; ++i) even[i] -= held[2 * i], odd[i] -= held[2 * i + 1];
         unit *= n == 0 ? 0.0625f : 0.03125f;
     }
 }
+
+// Parts that a query takes beyond the kernel's own, as many as it needs, from
+// LDS: while what is left of its numbers, times the largest keys that the cache's
+// units allow, may move a score (times log2 e) by more than 2^-14 and more than
+// 2^-21 of the sum of its terms' sizes. Nine parts hold every FP16 row exactly
+// (2^-38 of [2, 4) is its last bit), ten an FP32 one to 2^-49 of its largest.
+// Queries that need none multiply zeros in their neighbours' extra parts, which
+// changes no bit of theirs. Normal queries take none. With one number of 200, 2,000
+// or 30,000 beside normal ones, on keys of zero, in every query: 10,007 x 10,007
+// FP16 258 us without it and 273, 278 and 291 with, off by 2.8e-4 each; 512 x
+// 50,000 FP32 106 and 119, 125 and 123, off by 1.0e-6 at most. (Four parts alone are
+// off by 2e-2 at 30,000, and five by 6e-4.)
+constexpr int kMoreParts = 5;
+constexpr float kScoreLeft = 0x1p-14f, kScoreShare = 0x1p-21f;
 
 // 32 NJ queries per workgroup, every fourth block of its share to a wave. A wave
 // reads its blocks straight into registers: 4 bits a number are few enough that
@@ -1253,6 +1269,8 @@ __global__ __launch_bounds__(kWaves * 64, NJ == 1 ? 3 : 2) void icl4_wide_kernel
     if (more) load_keys(tiles + (long long)at * kBlockBytes), load_values(tiles + (long long)at * kBlockBytes);
     u32x6 parts[NJ][PARTS];
     float c[NJ];
+    int more_parts[NJ];
+    static_assert(kMoreParts * 6 * 64 <= 32 * kWideStride, "a wave's outputs have room for them");
     bool far = false;
     float units[32];  // of the lane's dims of keys
     load16(p.units + pair * 64 + 32 * h, units);
@@ -1285,7 +1303,34 @@ __global__ __launch_bounds__(kWaves * 64, NJ == 1 ? 3 : 2) void icl4_wide_kernel
         c[j] = fmaxf(factor(p, ex), 1.17549435e-38f) + halves_sum(nan);
         // Scores that may reach 2^22 (no key's size passes 127 units) are products rounded by themselves, against which
         // a reference can be held; weights take the others as they are multiplied. The factor waits in LDS, a lane's own.
-        const bool is_far = !(halves_sum(reach) * (127.0f * c[j]) < 4194304.0f);
+        const float most = halves_sum(reach) * (127.0f * c[j]);
+        const bool is_far = !(most < 4194304.0f);
+        more_parts[j] = 0;
+        float step = PAIRS ? 0x1p-24f : 0x1p-19f;
+        for (;;) {
+            float left = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                asm volatile("" ::: "memory");  // read again, four at a time: held, they would cost the loop registers
+                const f32x4 u = *reinterpret_cast<const f32x4 *>(p.units + pair * 64 + 32 * h + 4 * i);
+                left = fmaf(fabsf(even[2 * i]), u[0], fmaf(fabsf(odd[2 * i]), u[1], left));
+                left = fmaf(fabsf(even[2 * i + 1]), u[2], fmaf(fabsf(odd[2 * i + 1]), u[3], left));
+            }
+            // (Of a query that is not finite: no.)
+            const bool needs = halves_sum(left) * (127.0f * c[j]) > fmaxf(kScoreLeft, most * kScoreShare);
+            if (!__any(needs)) break;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) even[i] = needs ? even[i] : 0.f, odd[i] = needs ? odd[i] : 0.f;
+            const u32x6 part = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, step);
+            u32x2 *to = reinterpret_cast<u32x2 *>(&red_o[wave][32 * kWideStride * j]) + 192 * more_parts[j] + lane;
+#pragma unroll
+            for (int i = 0; i < 3; ++i) to[64 * i] = u32x2{part[2 * i], part[2 * i + 1]};
+            if (++more_parts[j] == kMoreParts) break;
+            const f32x32 held = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(part, step);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) even[i] -= held[2 * i], odd[i] -= held[2 * i + 1];
+            step *= 0.03125f;
+        }
         (h ? red_m : red_l)[wave][32 * j + r32] = is_far ? c[j] : 1.0f;
         c[j] = is_far ? 1.0f : c[j];
         far = far || __any(is_far);
@@ -1341,6 +1386,17 @@ __global__ __launch_bounds__(kWaves * 64, NJ == 1 ? 3 : 2) void icl4_wide_kernel
                 IRX_PART(j, 1, 0, part_exps, 0);
             }
 #undef IRX_PART
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+                for (int n = 0; n < more_parts[j]; ++n) {  // last, so that the others begin at 0 without registers that hold it
+                    const u32x2 *from = reinterpret_cast<const u32x2 *>(&red_o[wave][32 * kWideStride * j]) + 192 * n + lane;
+                    const u32x2 part[3] = {from[0], from[64], from[128]};
+                    const i32x8 x = {(int)part[0][0], (int)part[0][1], (int)part[1][0], (int)part[1][1],
+                                     (int)part[2][0], (int)part[2][1], 0, 0};
+                    const int exps = 127 - (5 * (PARTS + n) - 1);
+                    s[j][0] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[0], x, s[j][0], 4, 2, 0, ks, 0, exps);
+                    s[j][1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[1], x, s[j][1], 4, 2, 1, ks, 0, exps);
+                }
         }
         if (now != ~0ull) {
             // Rows that are not attended: one more product, of -6 * 2^127 in their first term by 1, makes -inf of

@@ -429,6 +429,51 @@ def test_zero_queries_at_the_largest_scale(device, rows, listed, element):
     check(got, want.attend(q, blocks=blocks), element, want)
 
 
+@pytest.mark.parametrize("element", ["f32", "f16"])
+@pytest.mark.parametrize("e,h,n,rows,listed", [(1, 2, 900, 1, 0), (1, 2, 900, 16, 0), (1, 2, 900, 17, 0),
+                                               (1, 3, 5000, 70, 0), (16, 1, 900, 2100, 0), (1, 2, 900, 20, 14)])
+@pytest.mark.parametrize("outlier", [2000.0, 8000.0, 30000.0])
+def test_queries_with_one_large_channel(device, e, h, n, rows, listed, element, outlier):
+    """A number 1,000 to 20,000 times the others, whose keys are zero: scores are the others' sums, and neither they nor
+    their bound may lose bits to it. Some queries have none, and one has a second number between."""
+    k = draw((e, h, n, 64), element, 1, 1.3)
+    k[..., 40] = 0.0
+    cache, want = make(device, e, h, n, element, k=k)
+    q = draw((e, h, rows, 64), element, 2, 1.5)
+    q[:, :, ::3, 40] = outlier
+    q[:, :, rows // 2, 40] = -outlier / 3
+    q[:, :, rows // 2, 7] = 31.0
+    blocks = np.broadcast_to(np.arange(listed, dtype=np.int32), (e, h, rows, listed)) if listed else None
+    out, lse = attend(device, cache, (e, h, n), q, element, blocks=blocks)
+    some = np.r_[0:rows:37, rows // 2, rows - 1]
+    check((out[:, :, some], lse[:, :, some]),
+          want.attend(q[:, :, some], blocks=None if blocks is None else blocks[:, :, some]), element, want)
+
+
+@pytest.mark.parametrize("rows", [16, 17, 40])
+def test_the_last_bit_of_a_small_fp16_number(device, rows):
+    """2^-8 (1 + 2^-10) beside 2, on a key of 49,152: a score of 192.1875 against one of 192."""
+    k, v = np.zeros((1, 1, 70, 64), np.float16), draw((1, 1, 70, 64), "f16", 3)
+    k[0, 0, 0, 5], k[0, 0, 69, 40] = 49152, 192
+    cache, want = make(device, 1, 1, 70, "f16", k=k, v=v)
+    q = np.zeros((1, 1, rows, 64), np.float16)
+    q[..., 1], q[..., 5], q[..., 40] = 2, 2.0 ** -8 + 2.0 ** -18, 1
+    check(attend(device, cache, (1, 1, 70), q, "f16", scale=1.0), want.attend(q, scale=1.0), "f16", want)
+
+
+@pytest.mark.parametrize("element,rows", [("f32", 70), ("f16", 70), ("f16", 2100)])
+def test_a_query_with_one_large_channel_leaves_the_others(device, element, rows):
+    """Bit for bit, whatever the form does for it."""
+    cache, _ = make(device, 2, 8, 900, element)
+    q = draw((2, 8, rows, 64), element, 2, 1.5)
+    whole, whole_lse = attend(device, cache, (2, 8, 900), q, element)
+    q[:, :, 5::32, 40] = 30000.0
+    got, lse = attend(device, cache, (2, 8, 900), q, element)
+    others = np.arange(rows) % 32 != 5
+    np.testing.assert_array_equal(got[:, :, others], whole[:, :, others])
+    np.testing.assert_array_equal(lse[:, :, others], whole_lse[:, :, others])
+
+
 def test_large_fp32_queries(device):
     """Queries past FP16's range, with a scale that brings their scores back."""
     cache, want = make(device, 1, 8, 300)
