@@ -441,8 +441,8 @@ int irx_icl4_select(irx_device *device, const irx_icl4_queries *queries, const v
  * than 16 a call a query is rounded more finely (an FP16 one at last not at all)
  * while that could move a score by more than 2^-14 and by more than 2^-20 of the
  * sum over the dims of |scale q| times the largest |k|. Weights
- * are pairs of FP16 values for FP32 queries, else FP16 (rounded once); sums are
- * FP32. */
+ * are pairs of FP16 values for FP32 queries and over listed blocks, else FP16
+ * (rounded once); sums are FP32. */
 int irx_icl4_attention(irx_device *device, const irx_icl4_queries *queries, const void *cache, float scale,
                        const int32_t *blocks, size_t n_blocks, void *out, const irx_strides *out_strides, float *lse,
                        void *workspace, size_t workspace_bytes, void *stream);

@@ -1562,15 +1562,15 @@ __device__ __forceinline__ unsigned row_lane(unsigned x) {
 // row of the g-th sixteen, and adds them. The softmax so costs one exponential
 // per row. (With keys converted to FP16 and every column the query, a block
 // took 190 vector instructions instead of 100.) Weights go through LDS to where
-// the second product wants them: FP32's as high FP16 parts in even and low ones
-// in odd columns. One FP32 query, 8 heads x 50,000 rows (27 MB) 8.8 us, latency:
+// the second product wants them, as high FP16 parts in even and low ones in odd
+// columns: pairs cost FP16 queries nothing here (77 x 2 of 17 blocks 22.7 us, 22.9
+// with one part). One FP32 query, 8 heads x 50,000 rows (27 MB) 8.8 us, latency:
 // a third of it before a block is there. 4,096 queries x 32 listed blocks, 570 MB
 // through the L2s, 39 us, 14.6 TB/s, one wave to a query (vector unit 57% busy,
 // matrix cores 33%, one or the other 75%); 8 queries x 64 listed blocks 8.8 us in
 // sixteen.
 template <typename T, bool LISTED, bool SPLIT, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 4) void icl4_one_kernel(AttendArgs p) {
-    constexpr bool PAIRS = sizeof(T) == 4;
     __shared__ __attribute__((aligned(16))) float red_o[WAVES][64];
     static_assert(__alignof__(red_o) >= alignof(f32x4), "read and written in fours");
     __shared__ float red_m[WAVES], red_l[WAVES];
@@ -1643,7 +1643,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void icl4_one_kernel(AttendArgs p) {
     // The lane's row of a block, and its weight's place: [step s][lanes g = 2 t + h][4 b + j].
     const int mine = 32 * (g >> 1) + 16 * (i16 >> 3) + 8 * (g & 1) + (i16 & 7);
     _Float16 *give = weights + 32 * (g >> 1) + 8 * (i16 >> 2) + 4 * (g & 1) + (i16 & 3);
-    const _Float16 *get = weights + (PAIRS ? 64 * (i16 & 1) : 0) + 8 * g;
+    const _Float16 *get = weights + 64 * (i16 & 1) + 8 * g;
     const unsigned chunk_at = 16u * lane, ke_at = kKeyExpsAt + ((g >> 1) * 16 + i16) * 4, ve_at = kValueExpsAt + i16 * 8;
 
     u32x4 kw[2], vw[2];
@@ -1716,7 +1716,7 @@ __global__ __launch_bounds__(WAVES * 64, 4) void icl4_one_kernel(AttendArgs p) {
             l_run += weight;
             const _Float16 hi = (_Float16)weight;
             give[0] = hi;
-            if constexpr (PAIRS) give[64] = (_Float16)(weight - (float)hi);
+            give[64] = (_Float16)(weight - (float)hi);
             __builtin_amdgcn_wave_barrier();  // the wave's own LDS operations run in order
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
@@ -1736,9 +1736,8 @@ __global__ __launch_bounds__(WAVES * 64, 4) void icl4_one_kernel(AttendArgs p) {
 #pragma unroll
     for (int d = 0; d < 4; ++d) {
         f32x4 v = o[d];
-        if constexpr (PAIRS)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] += next_lane(v[r]);
+        for (int r = 0; r < 4; ++r) v[r] += next_lane(v[r]);
         if (i16 == 0) *reinterpret_cast<f32x4 *>(&red_o[wave][16 * d + 4 * g]) = v;
     }
     __syncthreads();

@@ -637,6 +637,27 @@ def test_attention_over_listed_blocks(device, e, h, n, rows, count, element, lay
     check(got, want.attend(q, keep=keep, blocks=blocks), element, want)
 
 
+@pytest.mark.parametrize("e,h,n,rows,count", [(2, 3, 1000, 20, 16), (1, 1, 70000, 40, 1000), (1, 8, 640, 600, 10),
+                                              (1, 2, 777, 300, 3)])
+def test_fp16_weights_of_listed_blocks_are_pairs(device, e, h, n, rows, count):
+    """check()'s bound of FP32 weights (pairs, 2^-21 of the values), and the output's rounding."""
+    rng = np.random.default_rng(n)
+    cache, want = make(device, e, h, n, "f16", seed=n)
+    q = draw((e, h, rows, 64), "f16", n + 3, 1.5)
+    blocks = rng.integers(0, -(-n // 64), (e, h, rows, count)).astype(np.int32)
+    out, lse = attend(device, cache, (e, h, n), q, "f16", blocks=blocks)
+    exact, lse64, magnitude = want.attend(q, blocks=blocks)
+    check((out, lse), (exact, lse64, magnitude), "f16", want)
+    ds, v = 2.0 ** -17 * magnitude, np.abs(want.v).max()
+    bound = v * (4 * ds + 2.0 ** -21 + want.k.shape[2] * (2.0 ** -27 + 2.0 ** -30)) + np.abs(exact) * 2.0 ** -11 + 2.0 ** -25
+    off = np.abs(out.astype(np.float64) - exact)
+    assert np.all(off <= bound), f"{(off - bound).max():.3e} past the bound"
+    # Errors of scores are random and far below that bound; one rounding of the weights would add as much again as the
+    # output's own, whose mean square is a twelfth of a step's: of 2,560 outputs or more to some 4%.
+    step = np.maximum(2.0 ** (np.floor(np.log2(np.abs(exact) + 1e-300)) - 10), 2.0 ** -24)
+    assert np.mean(off ** 2) <= 1.1 * np.mean(step ** 2) / 12
+
+
 def test_every_block_listed_is_attention_over_all(device):
     e, h, n, rows = 1, 8, 1500, 9
     cache, want = make(device, e, h, n)
