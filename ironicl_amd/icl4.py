@@ -48,16 +48,37 @@ def _strides(strides, heads: int, rows: int):
     return (heads * rows * 64, rows * 64, 64) if strides is None else strides
 
 
+def _refused() -> hip.HipError:
+    return hip.HipError(hip.INVALID_ARGUMENT, "sizes and strides are whole numbers from 0 to 2^64 - 1")
+
+
+def _size(n) -> int:
+    # A size_t argument would take what lies outside modulo 2^64.
+    try:
+        n = n.__index__()
+    except AttributeError:
+        raise _refused() from None
+    if not 0 <= n < 1 << 64:
+        raise _refused()
+    return n
+
+
 def _rows(shape, k, v, element, k_strides, v_strides, lengths) -> bytes:
     estimators, heads, rows = shape
-    return _ROWS.pack(estimators, heads, rows, _element(element), _address(k) or 0, _address(v) or 0,
-                      *_strides(k_strides, heads, rows), *_strides(v_strides, heads, rows), _address(lengths) or 0)
+    try:
+        return _ROWS.pack(estimators, heads, rows, _element(element), _address(k) or 0, _address(v) or 0,
+                          *_strides(k_strides, heads, rows), *_strides(v_strides, heads, rows), _address(lengths) or 0)
+    except struct.error:
+        raise _refused() from None
 
 
 def _queries(shape, q, query_rows, element, q_strides, lengths, keep) -> bytes:
     estimators, heads, rows = shape
-    return _QUERIES.pack(estimators, heads, rows, query_rows, _element(element), _address(q) or 0,
-                         *_strides(q_strides, heads, query_rows), _address(lengths) or 0, _address(keep) or 0)
+    try:
+        return _QUERIES.pack(estimators, heads, rows, query_rows, _element(element), _address(q) or 0,
+                             *_strides(q_strides, heads, query_rows), _address(lengths) or 0, _address(keep) or 0)
+    except struct.error:
+        raise _refused() from None
 
 
 @functools.lru_cache(maxsize=None)
@@ -66,18 +87,28 @@ def _call(name: str):
 
 
 def _shape(shape) -> bytes:  # hip.Icl4Shape, or hip.Strides
-    return _THREE.pack(*shape)
+    try:
+        return _THREE.pack(*shape)
+    except struct.error:
+        raise _refused() from None
 
 
 def cache_bytes(shape) -> int:
     """Bytes of a cache of `shape` (0: out of range)."""
-    return _call("irx_icl4_bytes")(_shape(shape))
+    try:
+        return _call("irx_icl4_bytes")(_shape(shape))
+    except hip.HipError:
+        return 0
 
 
 def workspace_bytes(device: hip.Device, shape, query_rows: int, n_blocks: int = 0) -> int:
     """Bytes of workspace for `select` and `attention` of exactly `query_rows` queries
-    (fewer can need more: they are split further) over `n_blocks` blocks each, or all."""
-    return _call("irx_icl4_workspace_bytes")(device.handle, _shape(shape), query_rows, n_blocks)
+    (fewer can need more: they are split further) over `n_blocks` blocks each, or all.
+    0 where none is needed, and for arguments out of range, which the calls refuse."""
+    try:
+        return _call("irx_icl4_workspace_bytes")(device.handle, _shape(shape), _size(query_rows), _size(n_blocks))
+    except hip.HipError:
+        return 0
 
 
 def encode(device: hip.Device, shape, k, v, cache, *, element: str = "f32", k_strides=None, v_strides=None,
@@ -101,8 +132,8 @@ def select(device: hip.Device, shape, cache, q, query_rows: int, n_blocks: int, 
     """The `n_blocks` best blocks of each query into int32 `blocks` [estimators,
     heads, query_rows, n_blocks], ascending, -1 where there are fewer."""
     queries = _queries(shape, q, query_rows, element, q_strides, lengths, keep)
-    hip.check(_call("irx_icl4_select")(device.handle, queries, _address(cache), n_blocks, _address(blocks),
-                                       _address(workspace), workspace_bytes, _address(stream)))
+    hip.check(_call("irx_icl4_select")(device.handle, queries, _address(cache), _size(n_blocks), _address(blocks),
+                                       _address(workspace), _size(workspace_bytes), _address(stream)))
 
 
 def attention(device: hip.Device, shape, cache, q, query_rows: int, out, *, element: str = "f32", scale: float = 0.125,
@@ -113,6 +144,6 @@ def attention(device: hip.Device, shape, cache, q, query_rows: int, out, *, elem
     query_rows]; 0 and -inf where a query attends to nothing."""
     queries = _queries(shape, q, query_rows, element, q_strides, lengths, keep)
     strides = _shape(_strides(out_strides, shape[1], query_rows))
-    hip.check(_call("irx_icl4_attention")(device.handle, queries, _address(cache), scale, _address(blocks), n_blocks,
-                                          _address(out), strides, _address(lse), _address(workspace), workspace_bytes,
-                                          _address(stream)))
+    hip.check(_call("irx_icl4_attention")(device.handle, queries, _address(cache), scale, _address(blocks),
+                                          _size(n_blocks), _address(out), strides, _address(lse), _address(workspace),
+                                          _size(workspace_bytes), _address(stream)))

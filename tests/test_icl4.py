@@ -84,6 +84,35 @@ def test_scales_past_the_largest_are_refused():
     refused("needs a device", icl4.attention, SHAPE, Q, Q, 1, Q, scale=2.0 ** 127)
 
 
+def test_numbers_that_are_no_sizes_are_refused():
+    """Not passed on as the sizes that they would wrap to."""
+    device = None_device()
+    calls = [
+        lambda: icl4.encode(device, (1, 8, -100), Q, Q, Q),
+        lambda: icl4.encode(device, (1, 8, 1 << 64), Q, Q, Q),
+        lambda: icl4.encode(device, SHAPE, Q, Q, Q, k_strides=(0, -64, 64)),
+        lambda: icl4.decode(device, (-1, 8, 100), Q, k=Q),
+        lambda: icl4.select(device, SHAPE, Q, Q, -1, 1, Q),
+        lambda: icl4.select(device, SHAPE, Q, Q, 1, -1, Q),
+        lambda: icl4.select(device, SHAPE, Q, Q, 1, (1 << 64) + 1, Q),
+        lambda: icl4.select(device, SHAPE, Q, Q, 1, 1, Q, workspace=Q, workspace_bytes=-1),
+        lambda: icl4.attention(device, SHAPE, Q, Q, 1.5, Q),
+        lambda: icl4.attention(device, SHAPE, Q, Q, 2, Q, out_strides=(0, 64, -512)),
+        lambda: icl4.attention(device, SHAPE, Q, Q, 1, Q, blocks=Q, n_blocks=-1),
+        lambda: icl4.attention(device, SHAPE, Q, Q, 1, Q, workspace=Q, workspace_bytes=-1),
+        lambda: icl4.attention(device, SHAPE, Q, Q, 1, Q, workspace=Q, workspace_bytes=1 << 64),
+    ]
+    for i, call in enumerate(calls):
+        with pytest.raises(hip.HipError, match="sizes and strides are whole numbers") as info:
+            call()
+        assert info.value.status == hip.INVALID_ARGUMENT, i
+    for shape in ((1, 8, -64), (1, 8, 1 << 64), (1.5, 8, 64)):
+        assert icl4.cache_bytes(shape) == 0
+        assert icl4.workspace_bytes(device, shape, 1) == 0
+    for rows, blocks in ((-1, 0), (1, -1), (1 << 64, 0), ((1 << 64) + 1, 0), (1, 1 << 64)):
+        assert icl4.workspace_bytes(device, SHAPE, rows, blocks) == 0
+
+
 def test_unknown_elements_are_refused():
     queries = hip.Icl4Queries(hip.Icl4Shape(*SHAPE), 1, 7, Q, hip.Strides(0, 64, 64), None, None)
     out = hip.Strides(0, 64, 64)
