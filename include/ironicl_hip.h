@@ -392,7 +392,7 @@ typedef struct irx_icl4_rows {
 
 typedef struct irx_icl4_queries {
     irx_icl4_shape shape;
-    size_t query_rows;       /* 1 to 2^24 */
+    size_t query_rows;       /* 1 to 2^24, and what a call's launches hold: below */
     int element;             /* irx_element of q, and of the attention's output */
     const void *q;           /* [E, H, query_rows, 64], finite */
     irx_strides q_strides;
@@ -406,7 +406,13 @@ size_t irx_icl4_bytes(const irx_icl4_shape *shape);
 /* Bytes of workspace (16-byte aligned) with which irx_icl4_select and
  * irx_icl4_attention run on `device` for query_rows queries and n_blocks chosen
  * blocks (0: attention over every block); 0 for arguments out of range, or when
- * none is needed. Fewer queries can need more: they are split further. Calls that may run at once, in graphs too, need one each. */
+ * none is needed. Fewer queries can need more: they are split further. Calls that
+ * may run at once, in graphs too, need one each.
+ * Calls are refused (IRX_INVALID_ARGUMENT) from 2^31 (estimator, head, query) rows
+ * on, and where a launch would pass 2^32 work-items: irx_icl4_select from 2^22 groups
+ * of 16 queries of one (estimator, head), irx_icl4_attention from about 2^24 rows
+ * with more than 64 blocks listed each, 2^26 with up to 64, and 2^24 groups of 32
+ * queries over every block. */
 size_t irx_icl4_workspace_bytes(irx_device *device, const irx_icl4_shape *shape, size_t query_rows, size_t n_blocks);
 /* Writes `cache` from rows->k and rows->v. nonfinite, when not NULL, is a
  * device counter to which the numbers that are not finite, inside the lengths,
@@ -419,10 +425,11 @@ int irx_icl4_decode(irx_device *device, const void *cache, const irx_icl4_rows *
 /* For each (estimator, head, query) the n_blocks (1 to 4,096) blocks with the
  * highest scores among those with a row to attend to, ties to the lower block,
  * into blocks [E, H, query_rows, n_blocks]: ascending, then -1 where there are
- * fewer. A score bounds q k over the block's rows: with x = q * unit (within
- * FP32's range), f the smallest integer >= -100 with max |x| <= 127 * 2^f and c =
- * x / 2^f rounded to the nearest integer (ties to even), it is sum over the dims
- * of max(c low, c high), a whole number. */
+ * fewer. A score stands for the largest q k that the block's bounds allow: with x =
+ * q * unit (within FP32's range), f the smallest integer >= -100 with max |x| <=
+ * 127 * 2^f and c = x / 2^f rounded to the nearest integer (ties to even), it is sum
+ * over the dims of max(c low, c high), a whole number. (It would bound q k 2^-f but
+ * for c's rounding: a block's largest product can lie above its score.) */
 int irx_icl4_select(irx_device *device, const irx_icl4_queries *queries, const void *cache, size_t n_blocks,
                     int32_t *blocks, void *workspace, size_t workspace_bytes, void *stream);
 /* softmax(scale q k^T) v over the attended rows, scale positive and at most 2^127, into
@@ -438,11 +445,11 @@ int irx_icl4_select(irx_device *device, const irx_icl4_queries *queries, const v
  * to a pair of FP16 values (22 bits a number), of more to 2^-24 of its largest;
  * an FP16 query is exact, but with blocks numbers are rounded to 2^-30 of its
  * largest, and of more than 16 a call those below 2^-8 of it to 2^-19 of it. Of more
- * than 16 a call a query is rounded more finely (an FP16 one at last not at all)
- * while that could move a score by more than 2^-14 and by more than 2^-20 of the
- * sum over the dims of |scale q| times the largest |k|. Weights
- * are pairs of FP16 values for FP32 queries and over listed blocks, else FP16
- * (rounded once); sums are FP32. */
+ * than 16 a call a query is rounded more finely (an FP16 one at last not at all, an
+ * FP32 one to 2^-49 of its largest) while that could move a score by more than 2^-14
+ * and by more than 2^-20 of the sum over the dims of |scale q| times the largest |k|.
+ * Weights are pairs of FP16 values for FP32 queries and over listed blocks, else
+ * FP16 (rounded once); sums are FP32. */
 int irx_icl4_attention(irx_device *device, const irx_icl4_queries *queries, const void *cache, float scale,
                        const int32_t *blocks, size_t n_blocks, void *out, const irx_strides *out_strides, float *lse,
                        void *workspace, size_t workspace_bytes, void *stream);

@@ -922,7 +922,7 @@ constexpr float kLn2 = 0.69314718055994530942f;
 // outputs are off by 2.8e-4 (2-norm; 8 x 200,000 x 2 by 2.2e-4), where the rounding
 // of the output alone leaves 2.1e-4 and pairs would too, but take 342 us instead
 // of 242 at 10,007 x 10,007, 84 instead of 70 at 777 x 12,345 x 2 masked, 54.4
-// instead of 50.3 at 8 x 200,000 x 2. Over listed blocks pairs cost nothing.
+// instead of 50.3 at 8 x 200,000 x 2. Over listed blocks pairs cost 1%.
 constexpr float kHeadroom = 8.0f, kWideHeadroom16 = 5.0f, kWideHeadroom32 = 6.0f;
 
 // A product that is rounded by itself, whatever is added to it.
@@ -1212,8 +1212,8 @@ constexpr float kScoreLeft = 0x1p-14f, kScoreShare = 0x1p-21f;
 // conversions of values and 32 of weights, and the sums: at 10,007 FP16 queries
 // and rows it is busy for 62% of the time, the matrix cores for 36%, one or the
 // other for 85% (three or two waves to a SIMD hide the rest no further). 8 heads:
-// 512 FP32 queries x 50,000 rows 100 us with the merge, 526 TFLOP/s (a pair's two
-// products counted once); 10,007 x 10,007 FP16 234, 877.
+// 512 FP32 queries x 50,000 rows 102 us with the merge, 514 TFLOP/s (a pair's two
+// products counted once); 10,007 x 10,007 FP16 239, 859.
 // Lane (r = lane % 32, h = lane / 32), r = 16 s + 8 a + i:
 //   S^T, b = 0, 1: A = rows 32 s + 16 a + 8 b + i, dims 32 h ..; B = query r, the same dims;
 //     result register 8 s + 4 a + j is row 32 s + 16 a + 8 b + 4 h + j, query r;
@@ -1393,7 +1393,9 @@ __global__ __launch_bounds__(kWaves * 64, NJ == 1 ? 3 : 2) void icl4_wide_kernel
 #undef IRX_PART
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
-                for (int n = 0; n < more_parts[j]; ++n) {  // last, so that the others begin at 0 without registers that hold it
+                // Last, so that the others begin at 0 without registers that hold it (before them: 252 us instead of 241
+                // for 10,007 x 10,007 FP16 queries that take none).
+                for (int n = 0; n < more_parts[j]; ++n) {
                     const u32x2 *from = reinterpret_cast<const u32x2 *>(&red_o[wave][32 * kWideStride * j]) + 192 * n + lane;
                     const u32x2 part[3] = {from[0], from[64], from[128]};
                     const i32x8 x = {(int)part[0][0], (int)part[0][1], (int)part[1][0], (int)part[1][1],
@@ -1568,10 +1570,10 @@ __device__ __forceinline__ unsigned row_lane(unsigned x) {
 // per row. (With keys converted to FP16 and every column the query, a block
 // took 190 vector instructions instead of 100.) Weights go through LDS to where
 // the second product wants them, as high FP16 parts in even and low ones in odd
-// columns: pairs cost FP16 queries nothing here (77 x 2 of 17 blocks 22.7 us, 22.9
-// with one part). One FP32 query, 8 heads x 50,000 rows (27 MB) 8.8 us, latency:
+// columns: pairs cost FP16 queries next to nothing here (512 of 32 blocks of 782,
+// choice included, 54.0 us, 53.5 with one part). One FP32 query, 8 heads x 50,000 rows (27 MB) 9.0 us, latency:
 // a third of it before a block is there. 4,096 queries x 32 listed blocks, 570 MB
-// through the L2s, 39 us, 14.6 TB/s, one wave to a query (vector unit 57% busy,
+// through the L2s, 40 us, 14.3 TB/s, one wave to a query (vector unit 57% busy,
 // matrix cores 33%, one or the other 75%); 8 queries x 64 listed blocks 8.8 us in
 // sixteen.
 template <typename T, bool LISTED, bool SPLIT, int WAVES>

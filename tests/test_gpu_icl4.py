@@ -16,7 +16,11 @@ ones are off by half a step, 2^-11, and below FP16's smallest step (half of it
 2^-25, where the largest weight is at least 2^5) by at most 2^-30 of the
 largest, N of them. FP32 sums of N / 8 addends (two keys' worth of
 products in one) add N 2^-27 V at most. FP16 outputs round by 2^-11 of
-themselves. The log-sum-exp is off by 2 ds, N 2^-27 and 2^-22 of itself."""
+themselves. The log-sum-exp is off by 2 ds, N 2^-27 and 2^-22 of itself.
+
+FP16 numbers of more than 16 queries a call are rounded from 2^-8 of the largest down, not from 2^-9: two in a hundred
+normal ones, 2^-21 of A, inside the same half. A query that this, or FP32's 2^-24, could cost 2^-14 of a score and 2^-20
+of the sum of the sizes of |scale q| times the largest |k| is rounded more finely."""
 
 import ctypes
 
