@@ -478,6 +478,74 @@ def test_a_query_with_one_large_channel_leaves_the_others(device, element, rows)
     np.testing.assert_array_equal(lse[:, :, others], whole_lse[:, :, others])
 
 
+@pytest.mark.parametrize("e,rows,listed", [(2, 1, 0), (2, 16, 0), (2, 20, 0), (2, 70, 0), (16, 2100, 0), (2, 5, 13),
+                                           (2, 6000, 3)])
+@pytest.mark.parametrize("power", [12, 20])
+def test_subnormal_fp16_queries(device, e, rows, listed, power):
+    """Bit for bit what the same queries times 2^power give at a scale of 1/8."""
+    h, n = 1 if e == 16 else 2, 900
+    keep = np.random.default_rng(1).random((e, n)) < 0.8
+    cache, want = make(device, e, h, n, "f16")
+    q = np.ldexp(draw((e, h, rows, 64), "f32", 4, 1.5).astype(np.float64), -power).astype(np.float16)
+    blocks = np.random.default_rng(5).integers(0, 15, (e, h, rows, listed)).astype(np.int32) if listed else None
+    scale = 0.125 * 2.0 ** power
+    got = attend(device, cache, (e, h, n), q, "f16", keep=keep, blocks=blocks, scale=scale)
+    back = np.ldexp(q.astype(np.float64), power).astype(np.float16)
+    whole = attend(device, cache, (e, h, n), back, "f16", keep=keep, blocks=blocks)
+    np.testing.assert_array_equal(got[0], whole[0])
+    np.testing.assert_array_equal(got[1], whole[1])
+    some = np.r_[0:rows:37, rows - 1]
+    check((got[0][:, :, some], got[1][:, :, some]),
+          want.attend(q[:, :, some], scale=scale, keep=keep, blocks=None if blocks is None else blocks[:, :, some]),
+          "f16", want)
+
+
+@pytest.mark.parametrize("element", ["f32", "f16"])
+@pytest.mark.parametrize("rows,blocks", [(1, 0), (16, 0), (70, 0), (3, 900)])
+def test_splits_of_any_lengths(device, rows, blocks, element):
+    """Lengths around the splits' ends, one at 1 and one at 0: splits that hold nothing, and those that hold one row."""
+    n, e = 20011, 6
+    lengths = (0, 1, 63, 64, 65, 19969)
+    keep = np.ones((e, n), bool)
+    keep[5, ::2] = False
+    cache, want = make(device, e, 1, n, element, lengths=lengths, seed=3)
+    assert icl4.workspace_bytes(device, (e, 1, n), rows, blocks) > 0
+    q = draw((e, 1, rows, 64), element, 4, 1.5)
+    listed = None
+    if blocks:
+        listed = np.random.default_rng(2).integers(-3, 330, (e, 1, rows, blocks)).astype(np.int32)
+        listed[..., 0] = 0
+    got = attend(device, cache, (e, 1, n), q, element, keep=keep, lengths=lengths, blocks=listed)
+    check(got, want.attend(q, keep=keep, blocks=listed), element, want)
+    assert np.all(got[0][0] == 0) and np.all(np.isneginf(got[1][0]))
+
+
+@pytest.mark.parametrize("element", ["f32", "f16"])
+@pytest.mark.parametrize("e,h,n,rows", [(1, 2, 900, 20), (1, 2, 20011, 70), (16, 1, 900, 2100)])
+def test_large_scores_of_queries_with_one_large_channel(device, e, h, n, rows, element):
+    """Scores of 2^16 to 2^31 by 63 channels, and a number of 30,000 on keys of zero in every other query. Bounds as for
+    equal scores in different splits."""
+    rng = np.random.default_rng(rows)
+    k = rng.choice([-0.5, 0.5, 1.0], (e, h, n, 64)).astype(DTYPES[element])
+    tied = np.r_[2:63:10, n - 3]
+    k[:, :, tied] = 8.0
+    k[..., 40] = 0.0
+    v = draw((e, h, n, 64), element, 3)
+    cache, want = make(device, e, h, n, element, k=k, v=v)
+    expected = want.v[:, :, None, tied].mean(3)
+    bound = np.abs(expected) * 2.0 ** -19 + np.abs(want.v).max() * 2.0 ** -20
+    if element == "f16":
+        bound = bound + np.abs(expected) * 2.0 ** -10 + 2.0 ** -25
+    q = np.broadcast_to(rng.uniform(1, 2, (e, h, rows, 1)), (e, h, rows, 64)).astype(DTYPES[element])
+    q[:, :, ::2, 40] = 30000.0
+    for power in (7, 12, 17, 21):
+        scale = 2.0 ** power
+        out, lse = attend(device, cache, (e, h, n), q, element, scale=scale)
+        assert np.all(np.abs(out - expected) <= bound), power
+        total = q[..., 0].astype(np.float64) * 504 * scale + np.log(8.0)
+        assert np.all(np.abs(lse - total) <= total * 2.0 ** -19), power
+
+
 def test_large_fp32_queries(device):
     """Queries past FP16's range, with a scale that brings their scores back."""
     cache, want = make(device, 1, 8, 300)
