@@ -360,7 +360,8 @@ int irx_regression_summary(irx_device *device, const float *decoded, size_t ense
  * -20, with max |held key| <= 127 * 2^x; a block's bounds are floor(min / 2^x) and
  * ceil(max / 2^x) over its rows inside the length (0 and 0 when none is). ---- */
 
-typedef enum irx_element { IRX_ELEMENT_F32 = 0, IRX_ELEMENT_F16 = 1 } irx_element;
+/* BF16: the training calls alone (below). */
+typedef enum irx_element { IRX_ELEMENT_F32 = 0, IRX_ELEMENT_F16 = 1, IRX_ELEMENT_BF16 = 2 } irx_element;
 
 /* 1 to 65,535 pairs (estimators * heads), 1 to 2^27 rows, less than 2^24 blocks (75 GB) in all. */
 typedef struct irx_icl4_shape {
@@ -453,6 +454,124 @@ int irx_icl4_select(irx_device *device, const irx_icl4_queries *queries, const v
 int irx_icl4_attention(irx_device *device, const irx_icl4_queries *queries, const void *cache, float scale,
                        const int32_t *blocks, size_t n_blocks, void *out, const irx_strides *out_strides, float *lse,
                        void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---- Attention for training, and dropout. No counterpart in the reference, which
+ * predicts only. For a host that tunes an ICL stage, or a context's keys and values
+ * themselves: attention of 64-wide heads that keeps what its backward pass needs, that
+ * pass, and dropout onto a residual. All buffers but the structs are device memory of
+ * `device`; the work is enqueued on `stream` (a hipStream_t of that device, or NULL
+ * for its null stream) and the calls return without waiting; none allocates, so each
+ * may be captured into a HIP graph (the seed is read when the work runs). An output
+ * overlaps no input and no other output, but where stated. Results do not depend on
+ * other calls, on the workspace's contents or on the order in which work is scheduled.
+ * The calling thread's current device is left as it was. ---- */
+
+/* Query heads h of an estimator share the keys and values of head h / (heads /
+ * kv_heads). 1 to 65,535 (estimator, head) pairs, kv_heads a divisor of heads, 1 to
+ * 2^24 query rows and rows; less than 2^27 rows of all queries, of all keys and
+ * values, and less than 2^24 workgroups of 128 rows (32 in a few forms) in a call. */
+typedef struct irx_train_shape {
+    size_t estimators;
+    size_t heads;
+    size_t kv_heads;
+    size_t query_rows;
+    size_t rows;
+} irx_train_shape;
+
+/* Dropout: a number is dropped (becomes 0) with probability dropped / 65,536, and
+ * what stays is multiplied by w = 65,536 / (65,536 - dropped). dropped is 0 (no
+ * dropout; seed may be NULL) to 65,535. Which numbers are dropped follows from the
+ * seed alone, and no mask is stored: word i of Philox4x32 with seven rounds (Salmon,
+ * Moraes, Dror and Shaw, SC 2011), key (lower, upper half of *seed), holds the 16-bit
+ * values 2 i (its lower half) and 2 i + 1, and a value below `dropped` drops its
+ * number. Attention's weight of query i and key j of pair p = estimator * heads +
+ * head has counter (2 (j / 16) + (j / 4) % 2, i, p, site) and value 4 ((j / 8) % 2) +
+ * j % 4; column j of row i of irx_train_dropout has counter (j / 8, i, 2^32 - 1,
+ * site) and value j % 8. Calls of one step take a site each, steps a seed each. */
+typedef struct irx_train_drop {
+    const uint64_t *seed; /* device memory: one number */
+    uint32_t site;
+    uint32_t dropped;
+} irx_train_drop;
+
+/* Strides as irx_strides, in elements, multiples of 16 bytes, as the pointers are.
+ * Inputs' may be 0. */
+typedef struct irx_train_inputs {
+    irx_train_shape shape;
+    int element;                   /* irx_element of q, k, v, the output and all gradients */
+    float scale;                   /* 2^-64 to 2^64 */
+    const void *q;                 /* [E, heads, query_rows, 64] */
+    const void *k;                 /* [E, kv_heads, rows, 64] */
+    const void *v;
+    irx_strides q_strides;
+    irx_strides k_strides;
+    irx_strides v_strides;
+    const uint32_t *query_lengths; /* [E] queries of each (more than query_rows counts as query_rows), or NULL: all.
+                                    * Nothing of later queries is read or written */
+    const uint32_t *lengths;       /* [E] rows of each, alike. Nothing of later rows is read or written */
+    const uint64_t *keep;          /* [E, ceil(rows / 64)]: row 64 t + r of an estimator is attended where bit r of its
+                                    * word t is set, or NULL: every row. What other rows hold does not matter (NaN too);
+                                    * their gradients are 0 */
+    irx_train_drop drop;           /* of the weights, after the softmax */
+} irx_train_inputs;
+
+/* What the backward pass reads besides, and the gradients that it writes. */
+typedef struct irx_train_gradients {
+    const void *out;    /* as irx_train_attention wrote it, with the same inputs, seed and site */
+    const float *stats; /* likewise */
+    const void *dout;   /* [E, heads, query_rows, 64] */
+    irx_strides out_strides;
+    irx_strides dout_strides;
+    void *dq;           /* [E, heads, query_rows, 64], or NULL */
+    void *dk;           /* [E, kv_heads, rows, 64], or NULL: with dv alone; one of the two sides is wanted */
+    void *dv;
+    irx_strides dq_strides;
+    irx_strides dk_strides; /* every (estimator, key head) has gradients of its own, also where inputs' strides are 0 */
+    irx_strides dv_strides;
+} irx_train_gradients;
+
+/* Bytes of workspace (16-byte aligned) with which irx_train_attention (backward 0)
+ * or irx_train_attention_backward (1) runs on `device` for exactly this shape
+ * and element; 0 for arguments out of range, or when none is needed. Calls that may run at once, in
+ * graphs too, need one each. */
+size_t irx_train_workspace_bytes(irx_device *device, const irx_train_shape *shape, int element, int backward);
+/* out = w D(softmax(scale q k^T)) v over the attended rows into [E, heads, query_rows,
+ * 64]; a query that attends to no row gets 0. lse, when not NULL, [E, heads,
+ * query_rows] FP32: the natural logarithm of the sum of exp(scale q k), -inf for a
+ * query that attends to none. stats, when not NULL, [E, heads, query_rows, 2] FP32,
+ * 8-byte aligned: what the backward pass needs, a whole number r and s = the sum of 2^(log2(e) scale q k - r)
+ * (0 and 0 where there is none).
+ * Inputs that are read must be finite, at most 2^127, and scale q and the scores
+ * within FP32's range. What is rounded: FP32 operands of a product to 24 bits
+ * (products of the lowest parts, below 2^-23, left out), FP16's operands of weights
+ * to 16, BF16's to 8; sums and statistics are FP32. Weights below 2^-126, and parts
+ * of operands below that, may be taken as 0. */
+int irx_train_attention(irx_device *device, const irx_train_inputs *inputs, void *out, const irx_strides *out_strides,
+                        float *stats, float *lse, void *workspace, size_t workspace_bytes, void *stream);
+/* The gradients of q, k and v from the output's. Probabilities are computed anew
+ * from stats. */
+int irx_train_attention_backward(irx_device *device, const irx_train_inputs *inputs,
+                                 const irx_train_gradients *gradients, void *workspace, size_t workspace_bytes,
+                                 void *stream);
+
+/* out = residual + w D(x), rounded once; with residual NULL, w D(x), which is also
+ * the gradient of x from that of out. Rows start `stride` elements apart (multiples of
+ * 16 bytes, as the pointers are; at least the width, where there is more than one
+ * row). out may be x or residual, at its stride. 1 to 2^31 - 1 columns, rows with less
+ * than 2^31 groups of 8 columns in all. */
+typedef struct irx_train_rows {
+    size_t rows;
+    size_t width;
+    int element;
+    const void *x;
+    const void *residual;
+    void *out;
+    size_t x_stride;
+    size_t residual_stride;
+    size_t out_stride;
+    irx_train_drop drop;
+} irx_train_rows;
+int irx_train_dropout(irx_device *device, const irx_train_rows *rows, void *stream);
 
 /* ---- Kernel harness (cuda/testing.rs:27-207): one kernel family on host data ---- */
 

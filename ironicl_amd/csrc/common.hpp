@@ -505,6 +505,54 @@ void icl4_decode(const Icl4Rows &a, const void *cache, float *bounds, hipStream_
 void icl4_select(const Icl4Queries &a, int n, int *out, void *workspace, hipStream_t stream);
 void icl4_attend(const Icl4Queries &a, const Icl4Attend &b, hipStream_t stream);
 
+// Attention for training, its backward pass and dropout (training.hip). Strides are {estimator, head, row} in elements.
+constexpr int kTrainF32 = 0, kTrainF16 = 1, kTrainBF16 = 2;
+struct TrainShape {
+    int estimators, heads, kv_heads, q_rows, rows;
+};
+struct TrainDrop {
+    const unsigned long long *seed;
+    unsigned site, dropped;  // dropped < 65,536
+};
+struct TrainInputs {
+    TrainShape shape;
+    int element;
+    float scale;
+    const void *q, *k, *v;
+    long long qs[3], ks[3], vs[3];
+    const unsigned *q_lengths, *lengths;
+    const unsigned long long *keep;
+    TrainDrop drop;
+};
+struct TrainForward {
+    void *out;
+    long long os[3];
+    float *stats, *lse;  // [estimators, heads, q_rows, 2] and [estimators, heads, q_rows], or null
+    void *workspace;
+};
+struct TrainBackward {
+    const void *out, *dout;
+    const float *stats;
+    long long os[3], gs[3];
+    void *dq, *dk, *dv;  // dq may be null, or dk and dv
+    long long dqs[3], dks[3], dvs[3];
+    void *workspace;
+};
+struct TrainRows {
+    size_t rows, width;
+    int element;
+    const void *x, *residual;
+    void *out;
+    long long xs, rs, os;
+    TrainDrop drop;
+};
+size_t train_workspace(const TrainShape &s, int element, bool backward, int compute_units);
+// Whether a call's launches hold it.
+bool train_fits(const TrainShape &s, int element, bool backward, int compute_units);
+void train_attention(const TrainInputs &a, const TrainForward &f, int compute_units, hipStream_t stream);
+void train_backward(const TrainInputs &a, const TrainBackward &b, int compute_units, hipStream_t stream);
+void train_dropout(const TrainRows &a, hipStream_t stream);
+
 // TabICL preprocessing (preprocess.hip), in f64. Fit: statistics of every
 // kept feature, [groups, 9, kept_count] (mean, scale, minimum, maximum,
 // lower, upper, then lambda, mean, scale of the power transform), and a

@@ -1674,6 +1674,60 @@ void icl4_workspace(const void *workspace, size_t bytes, size_t needed) {
         fail(IRX_INVALID_ARGUMENT, "the workspace must hold " + std::to_string(needed) + " bytes");
 }
 
+// ---- attention for training: argument checks ----
+
+bool train_shape_ok(const irx_train_shape *s) {
+    const size_t most = (size_t)1 << 24;
+    if (!s || !s->estimators || !s->heads || !s->kv_heads || !s->query_rows || !s->rows) return false;
+    if (s->estimators > 65535 || s->heads > 65535 || s->estimators * s->heads > 65535 || s->heads % s->kv_heads) return false;
+    return s->query_rows <= most && s->rows <= most;
+}
+
+TrainShape train_shape(const irx_train_shape &s) {
+    return {(int)s.estimators, (int)s.heads, (int)s.kv_heads, (int)s.query_rows, (int)s.rows};
+}
+
+int train_element(int element) {
+    if (element != IRX_ELEMENT_F32 && element != IRX_ELEMENT_F16 && element != IRX_ELEMENT_BF16)
+        fail(IRX_INVALID_ARGUMENT, "elements are FP32, FP16 or BF16");
+    return element;
+}
+
+TrainDrop train_drop(const irx_train_drop &d) {
+    if (d.dropped > 65535) fail(IRX_INVALID_ARGUMENT, "0 to 65,535 of 65,536 numbers are dropped");
+    if (d.dropped && !d.seed) fail(IRX_INVALID_ARGUMENT, "dropout needs a seed");
+    icl4_aligned(d.seed, 8, "the seed");
+    return {reinterpret_cast<const unsigned long long *>(d.seed), d.site, d.dropped};
+}
+
+// One tensor of the calls: its address and strides, and an output's rows apart.
+void train_tensor(const irx_train_shape &s, size_t heads, size_t rows, int element, const void *p, const char *what,
+                  const irx_strides &in, long long *strides, bool output) {
+    const irx_icl4_shape shape = {s.estimators, heads, rows};
+    icl4_aligned(p, 16, what);
+    icl4_strides(shape, rows, element != IRX_ELEMENT_F32, in, strides);
+    if (output) icl4_output(shape, rows, in);
+}
+
+TrainInputs train_inputs(const irx_train_inputs &in) {
+    if (!train_shape_ok(&in.shape)) fail(IRX_INVALID_ARGUMENT, "the attention's shape is out of range");
+    if (!in.q || !in.k || !in.v) fail(IRX_INVALID_ARGUMENT, "attention needs queries, keys and values");
+    if (!(in.scale >= 0x1p-64f && in.scale <= 0x1p64f)) fail(IRX_INVALID_ARGUMENT, "the scale is 2^-64 to 2^64");
+    TrainInputs a{};
+    a.shape = train_shape(in.shape), a.element = train_element(in.element), a.scale = in.scale;
+    a.q = in.q, a.k = in.k, a.v = in.v;
+    train_tensor(in.shape, in.shape.heads, in.shape.query_rows, in.element, in.q, "queries", in.q_strides, a.qs, false);
+    train_tensor(in.shape, in.shape.kv_heads, in.shape.rows, in.element, in.k, "keys", in.k_strides, a.ks, false);
+    train_tensor(in.shape, in.shape.kv_heads, in.shape.rows, in.element, in.v, "values", in.v_strides, a.vs, false);
+    icl4_aligned(in.query_lengths, 4, "query lengths");
+    icl4_aligned(in.lengths, 4, "lengths");
+    icl4_aligned(in.keep, 8, "keep");
+    a.q_lengths = in.query_lengths, a.lengths = in.lengths;
+    a.keep = reinterpret_cast<const unsigned long long *>(in.keep);
+    a.drop = train_drop(in.drop);
+    return a;
+}
+
 void device_release(irx_device *d) {
     if (d && d->refs.fetch_sub(1) == 1) delete d;
 }
@@ -2361,6 +2415,86 @@ int irx_icl4_attention(irx_device *device, const irx_icl4_queries *queries, cons
         icl4_workspace(workspace, workspace_bytes, icl4_attend_workspace(a.shape, a.half, a.q_rows, b.n, a.compute_units));
         CurrentDevice here(device);
         icl4_attend(a, b, static_cast<hipStream_t>(stream));
+    });
+}
+
+size_t irx_train_workspace_bytes(irx_device *device, const irx_train_shape *shape, int element, int backward) {
+    if (!device || !train_shape_ok(shape) || element < IRX_ELEMENT_F32 || element > IRX_ELEMENT_BF16) return 0;
+    const TrainShape s = train_shape(*shape);
+    if (!train_fits(s, element, backward, device->compute_units)) return 0;
+    return train_workspace(s, element, backward, device->compute_units);
+}
+
+int irx_train_attention(irx_device *device, const irx_train_inputs *inputs, void *out, const irx_strides *out_strides,
+                        float *stats, float *lse, void *workspace, size_t workspace_bytes, void *stream) {
+    return guarded("irx_train_attention", [&] {
+        if (!inputs || !out || !out_strides) fail(IRX_INVALID_ARGUMENT, "attention needs its inputs and its output");
+        const TrainInputs a = train_inputs(*inputs);
+        const irx_train_shape &s = inputs->shape;
+        TrainForward f{};
+        f.out = out, f.stats = stats, f.lse = lse, f.workspace = workspace;
+        train_tensor(s, s.heads, s.query_rows, a.element, out, "the output", *out_strides, f.os, true);
+        icl4_aligned(stats, 8, "stats");
+        icl4_aligned(lse, 4, "lse");
+        icl4_device(device);
+        if (!train_fits(a.shape, a.element, false, device->compute_units)) fail(IRX_INVALID_ARGUMENT, "too many rows for one call");
+        icl4_workspace(workspace, workspace_bytes, train_workspace(a.shape, a.element, false, device->compute_units));
+        CurrentDevice here(device);
+        train_attention(a, f, device->compute_units, static_cast<hipStream_t>(stream));
+    });
+}
+
+int irx_train_attention_backward(irx_device *device, const irx_train_inputs *inputs,
+                                 const irx_train_gradients *gradients, void *workspace, size_t workspace_bytes,
+                                 void *stream) {
+    return guarded("irx_train_attention_backward", [&] {
+        if (!inputs || !gradients || !gradients->out || !gradients->stats || !gradients->dout)
+            fail(IRX_INVALID_ARGUMENT, "the backward pass needs its inputs, the output, its statistics and its gradient");
+        const irx_train_gradients &g = *gradients;
+        if (!g.dk != !g.dv || (!g.dq && !g.dk))
+            fail(IRX_INVALID_ARGUMENT, "gradients are of the queries, of keys and values, or of both");
+        const TrainInputs a = train_inputs(*inputs);
+        const irx_train_shape &s = inputs->shape;
+        TrainBackward b{};
+        b.out = g.out, b.stats = g.stats, b.dout = g.dout, b.dq = g.dq, b.dk = g.dk, b.dv = g.dv, b.workspace = workspace;
+        train_tensor(s, s.heads, s.query_rows, a.element, g.out, "the output", g.out_strides, b.os, false);
+        train_tensor(s, s.heads, s.query_rows, a.element, g.dout, "the output's gradient", g.dout_strides, b.gs, false);
+        icl4_aligned(g.stats, 8, "stats");
+        if (g.dq) train_tensor(s, s.heads, s.query_rows, a.element, g.dq, "the queries' gradient", g.dq_strides, b.dqs, true);
+        if (g.dk) {
+            train_tensor(s, s.kv_heads, s.rows, a.element, g.dk, "the keys' gradient", g.dk_strides, b.dks, true);
+            train_tensor(s, s.kv_heads, s.rows, a.element, g.dv, "the values' gradient", g.dv_strides, b.dvs, true);
+        }
+        icl4_device(device);
+        if (!train_fits(a.shape, a.element, true, device->compute_units)) fail(IRX_INVALID_ARGUMENT, "too many rows for one call");
+        icl4_workspace(workspace, workspace_bytes, train_workspace(a.shape, a.element, true, device->compute_units));
+        CurrentDevice here(device);
+        train_backward(a, b, device->compute_units, static_cast<hipStream_t>(stream));
+    });
+}
+
+int irx_train_dropout(irx_device *device, const irx_train_rows *rows, void *stream) {
+    return guarded("irx_train_dropout", [&] {
+        if (!rows || !rows->x || !rows->out) fail(IRX_INVALID_ARGUMENT, "dropout needs its input and its output");
+        const irx_train_rows &r = *rows;
+        if (!r.rows || !r.width || r.width > 0x7fffffff || r.rows > 0x7fffffff / ((r.width + 7) / 8))
+            fail(IRX_INVALID_ARGUMENT, "rows and columns are out of range");
+        TrainRows a{};
+        a.rows = r.rows, a.width = r.width, a.element = train_element(r.element);
+        a.x = r.x, a.residual = r.residual, a.out = r.out, a.drop = train_drop(r.drop);
+        const size_t unit = r.element == IRX_ELEMENT_F32 ? 4 : 8, strides[3] = {r.x_stride, r.residual_stride, r.out_stride};
+        const void *const tensors[3] = {r.x, r.residual, r.out};
+        long long *const to[3] = {&a.xs, &a.rs, &a.os};
+        for (int i = 0; i < 3; ++i) {
+            icl4_aligned(tensors[i], 16, "a tensor");
+            if (!tensors[i] || r.rows == 1) continue;
+            if (strides[i] % unit || strides[i] < r.width || strides[i] > ((size_t)1 << 40) / r.rows)
+                fail(IRX_INVALID_ARGUMENT, "strides must be multiples of 16 bytes, the width at least, and within range");
+            *to[i] = (long long)strides[i];
+        }
+        icl4_device(device);
+        CurrentDevice here(device);
+        train_dropout(a, static_cast<hipStream_t>(stream));
     });
 }
 

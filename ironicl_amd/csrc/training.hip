@@ -1,0 +1,1016 @@
+// Attention for training, its backward pass, and dropout.
+//
+// With x_ij = scale log2(e) q_i.k_j over the keys that a query attends to:
+//   r_i = ceil(max_j x_ij), s_i = sum_j 2^(x_ij - r_i), P_ij = 2^(x_ij - r_i) / s_i
+//   out_i = w sum_j P_ij Z_ij v_j, Z_ij in {0, 1} the weights' dropout, w = 65,536 / (65,536 - dropped)
+// and, from dout and delta_i = dout_i.out_i:
+//   dS_ij = P_ij (w Z_ij dout_i.v_j - delta_i)
+//   dv_j = w sum_i P_ij Z_ij dout_i, dk_j = scale sum_i dS_ij q_i, dq_i = scale sum_j dS_ij k_j.
+// The reference r is a whole number: FP32 holds it exactly at any size, and what was summed under another
+// reference comes to it by an exact power of two. (One FP32 logarithm r + log2 s in place of the two
+// would put 2^-24 of itself into every weight of its row: 1e-5 at scores of 300.)
+//
+// Products run on the BF16 matrix cores with FP32 sums. BF16 operands are taken as they are; FP16 ones are
+// held as two BF16 parts (8 + 3 of 11 bits, exact) in three products, FP32 ones as three (8 + 8 + 8 of 24)
+// in six: lo.hi and hi.lo down to 2^-16 of hi.hi, what is left out is below 2^-23 of it (2^-17 with two
+// parts). BF16 has FP32's exponents, so gradients of any size need no scale. The probabilities and dS are
+// rounded to as many parts: BF16's eight bits, 2^-17, 2^-25.
+#include "common.hpp"
+
+#include <algorithm>
+#include <cmath>
+
+// LLVM's intrinsic, for which this compiler has no builtin: `old` with `value` in the named lane.
+extern "C" __device__ unsigned irx_writelane(unsigned value, unsigned lane, unsigned old) __asm("llvm.amdgcn.writelane.i32");
+
+namespace irx {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kTile = 64;   // rows of a streamed tile
+constexpr int kPitch = 72;  // BF16 numbers from one row of a tile to the next: 36 banks, so 16 rows' 16 bytes meet no bank twice
+constexpr float kLn2 = 0.69314718055994530942f;
+
+constexpr int parts_of(int element) { return element == kTrainF32 ? 3 : element == kTrainF16 ? 2 : 1; }
+
+// ---- elements ----
+
+// Eight adjacent numbers as they lie in memory.
+template <int EL>
+struct Raw {
+    u32x4 w[EL == kTrainF32 ? 2 : 1];
+};
+
+template <int EL>
+__device__ __forceinline__ Raw<EL> load8(const void *base, long long at) {
+    Raw<EL> r;
+    const u32x4 *p = reinterpret_cast<const u32x4 *>(static_cast<const char *>(base) + at * (EL == kTrainF32 ? 4 : 2));
+#pragma unroll
+    for (int i = 0; i < (EL == kTrainF32 ? 2 : 1); ++i) r.w[i] = p[i];
+    return r;
+}
+
+template <int EL>
+__device__ __forceinline__ void to_floats(const Raw<EL> &r, float *x) {
+    if constexpr (EL == kTrainF32) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(r.w[i / 4][i % 4]);
+    } else if constexpr (EL == kTrainF16) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned w = r.w[0][i];
+            const half2v h = __builtin_bit_cast(half2v, w);
+            x[2 * i] = (float)h[0], x[2 * i + 1] = (float)h[1];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __uint_as_float(r.w[0][i] << 16);
+            x[2 * i + 1] = __uint_as_float(r.w[0][i] & 0xffff0000u);
+        }
+    }
+}
+
+// Two numbers rounded to BF16 (nearest, ties to even), the first in the lower half.
+__device__ __forceinline__ unsigned bf16_pair(float a, float b) {
+    return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{a, b}), bf16x2));
+}
+
+// Eight numbers as P BF16 parts: each the rounded rest of those before.
+template <int P>
+__device__ __forceinline__ void split8(const float *x, bf16x8 (&out)[P]) {
+    u32x4 w[P];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float a = x[2 * i], b = x[2 * i + 1];
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            w[p][i] = bf16_pair(a, b);
+            if (p + 1 < P) {
+                a -= __uint_as_float(w[p][i] << 16);
+                b -= __uint_as_float(w[p][i] & 0xffff0000u);
+            }
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < P; ++p) out[p] = __builtin_bit_cast(bf16x8, w[p]);
+}
+
+template <int EL>
+__device__ __forceinline__ void split_raw(const Raw<EL> &r, bf16x8 (&out)[parts_of(EL)]) {
+    if constexpr (EL == kTrainBF16) {
+        out[0] = __builtin_bit_cast(bf16x8, r.w[0]);
+    } else {
+        float x[8];
+        to_floats<EL>(r, x);
+        split8<parts_of(EL)>(x, out);
+    }
+}
+
+// Four numbers rounded to the element type and stored.
+template <int EL>
+__device__ __forceinline__ void store4(void *base, long long at, f32x4 x) {
+    if constexpr (EL == kTrainF32) {
+        *reinterpret_cast<f32x4 *>(static_cast<float *>(base) + at) = x;
+    } else if constexpr (EL == kTrainF16) {
+        const half2v a = __builtin_convertvector((f32x2{x[0], x[1]}), half2v);
+        const half2v b = __builtin_convertvector((f32x2{x[2], x[3]}), half2v);
+        *reinterpret_cast<u32x2 *>(static_cast<unsigned short *>(base) + at) =
+            u32x2{__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b)};
+    } else {
+        *reinterpret_cast<u32x2 *>(static_cast<unsigned short *>(base) + at) =
+            u32x2{bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3])};
+    }
+}
+
+template <int EL>
+__device__ __forceinline__ f32x4 load4(const void *base, long long at) {
+    if constexpr (EL == kTrainF32) {
+        return *reinterpret_cast<const f32x4 *>(static_cast<const float *>(base) + at);
+    } else {
+        const u32x2 w = *reinterpret_cast<const u32x2 *>(static_cast<const unsigned short *>(base) + at);
+        if constexpr (EL == kTrainF16) {
+            const unsigned low = w[0], high = w[1];
+            const half2v a = __builtin_bit_cast(half2v, low), b = __builtin_bit_cast(half2v, high);
+            return f32x4{(float)a[0], (float)a[1], (float)b[0], (float)b[1]};
+        } else {
+            return f32x4{__uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xffff0000u), __uint_as_float(w[1] << 16),
+                         __uint_as_float(w[1] & 0xffff0000u)};
+        }
+    }
+}
+
+// ---- products ----
+
+// acc += A B on parts, the small terms first.
+template <int P>
+__device__ __forceinline__ void mma(f32x16 &acc, const bf16x8 (&a)[P], const bf16x8 (&b)[P]) {
+#pragma unroll
+    for (int order = P - 1; order >= 0; --order)
+#pragma unroll
+        for (int i = 0; i <= order; ++i)
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[order - i], b[i], acc, 0, 0, 0);
+}
+
+// A tile in LDS: P planes of 64 rows of 64 BF16 numbers.
+template <int P>
+struct Tile {
+    alignas(16) __bf16 p[P][kTile * kPitch];
+};
+
+// The A operand of rows `row0` .. + 31, dims 16 c .. + 15: lane (row l % 32, half h) holds dims 16 c + 8 h .. + 7.
+template <int P>
+__device__ __forceinline__ void rows_operand(const Tile<P> &t, int row0, int c, int lane, bf16x8 (&a)[P]) {
+    const int at = (row0 + (lane & 31)) * kPitch + 16 * c + 8 * (lane >> 5);
+#pragma unroll
+    for (int p = 0; p < P; ++p) a[p] = *reinterpret_cast<const bf16x8 *>(&t.p[p][at]);
+}
+
+// The A operand of dims 32 d .. + 31 over rows row0 .. + 15, for a B operand whose eight numbers in half h are those of rows
+// 4 h .. + 3 and 8 + 4 h .. + 3: a product's result as it lies in a lane.
+template <int P>
+__device__ __forceinline__ void dims_operand(const Tile<P> &t, int row0, int d, int lane, bf16x8 (&a)[P]) {
+    typedef __attribute__((address_space(3))) s16x4 *lds4;
+    const int at = (row0 + 4 * (lane >> 5) + (lane & 15) / 4) * kPitch + 32 * d + (lane & 16) + 4 * (lane & 3);
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(&t.p[p][at]));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(&t.p[p][at + 8 * kPitch]));
+        a[p] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+}
+
+__device__ __forceinline__ float other_half(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+
+// ---- random numbers ----
+
+// Philox4x32 (Salmon, Moraes, Dror and Shaw, "Parallel random numbers: as easy as 1, 2, 3", SC 2011) with seven rounds, the
+// fewest that pass their whole test suite.
+__device__ __forceinline__ u32x4 philox(unsigned c0, unsigned c1, unsigned c2, unsigned c3, unsigned long long seed) {
+    unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
+#pragma unroll
+    for (int round = 0; round < 7; ++round) {
+        const unsigned long long a = (unsigned long long)c0 * 0xD2511F53u, b = (unsigned long long)c2 * 0xCD9E8D57u;
+        c0 = (unsigned)(b >> 32) ^ c1 ^ k0;
+        c1 = (unsigned)b;
+        c2 = (unsigned)(a >> 32) ^ c3 ^ k1;
+        c3 = (unsigned)a;
+        k0 += 0x9E3779B9u, k1 += 0xBB67AE85u;
+    }
+    return u32x4{c0, c1, c2, c3};
+}
+
+// Whether number j of a call's eight 16-bit ones is kept; `line` is dropped << 16.
+__device__ __forceinline__ bool kept16(const u32x4 &w, int j, unsigned line) {
+    return (j & 1 ? w[j >> 1] : w[j >> 1] << 16) >= line;
+}
+
+// ---- lengths and masks ----
+
+__device__ __forceinline__ int length_of(const unsigned *lengths, int e, int rows) {
+    return lengths ? (int)min(lengths[e], (unsigned)rows) : rows;
+}
+
+// Bit r: key 64 word + r is attended; `rows` is the estimator's length.
+__device__ __forceinline__ unsigned long long attended(const unsigned long long *keep, int words, int e, int word, int rows) {
+    const int left = rows - word * 64;
+    if (left <= 0) return 0;
+    unsigned long long m = keep ? keep[(long long)e * words + word] : ~0ull;
+    if (left < 64) m &= (1ull << left) - 1;
+    return m;
+}
+
+struct Args {
+    const void *q, *k, *v;
+    long long qs[3], ks[3], vs[3];
+    const unsigned *q_lengths, *lengths;
+    const unsigned long long *keep;
+    int heads, kv_heads, pairs, q_rows, rows, words;
+    float scale, c;  // c = scale log2(e)
+    const unsigned long long *seed;
+    unsigned site, line;
+    float w;
+    // forward
+    void *out;
+    long long os[3];
+    float *stats, *lse;
+    // backward
+    const void *dout;
+    void *dq, *dk, *dv;
+    long long gs[3], dqs[3], dks[3], dvs[3];
+    f32x4 *record;
+    // plans
+    int q_tiles, q_splits, q_chunk;     // units of 128 queries; a split's key tiles
+    int k_tiles, k_splits, k_chunk;     // units of 128 keys; a split's query tiles
+    int q_blocks;                       // workgroups on queries, before those on keys
+    float *q_part, *k_part;
+};
+
+__device__ __forceinline__ long long at(const long long *s, int e, int h, int row) {
+    return e * s[0] + h * s[1] + (long long)row * s[2];
+}
+
+// A tile's numbers on their way to LDS: NT threads load 64 x 64, eight adjacent ones at a time.
+template <int EL, int NT>
+struct Staged {
+    static constexpr int N = 512 / NT;
+    Raw<EL> r[N];
+
+    // Rows past `rows` are read from the last.
+    __device__ __forceinline__ void load(const void *base, const long long *s, int e, int h, int row0, int rows) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int u = threadIdx.x + i * NT;
+            r[i] = load8<EL>(base, at(s, e, h, min(row0 + u / 8, rows - 1)) + 8 * (u % 8));
+        }
+    }
+    // Rows whose bit is not set become zeros, whatever they hold. `factor`: null, or one for each row.
+    __device__ __forceinline__ void store(Tile<parts_of(EL)> &t, unsigned long long some, const float *factor) const {
+        constexpr int P = parts_of(EL);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int u = threadIdx.x + i * NT, row = u / 8;
+            bf16x8 b[P];
+            if (EL != kTrainBF16 && factor) {
+                float x[8];
+                to_floats<EL>(r[i], x);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] *= factor[row];
+                split8<P>(x, b);
+            } else {
+                split_raw<EL>(r[i], b);
+            }
+            const bool in = some >> row & 1;
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                u32x4 w = __builtin_bit_cast(u32x4, b[p]);
+                if (!in) w = u32x4{0, 0, 0, 0};
+                *reinterpret_cast<u32x4 *>(&t.p[p][row * kPitch + 8 * (u % 8)]) = w;
+            }
+        }
+    }
+};
+
+// The B operand of a lane's own row: dims 16 c + 8 h .. + 7; zeros where !in.
+template <int EL>
+__device__ __forceinline__ void own_row(const void *base, long long row, bool in, int lane, bf16x8 (&b)[4][parts_of(EL)]) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        Raw<EL> r{};
+        if (in) r = load8<EL>(base, row + 16 * c + 8 * (lane >> 5));
+        split_raw<EL>(r, b[c]);
+    }
+}
+
+// ---- forward ----
+
+// 32 WQ queries to a workgroup, 32 to a wave; keys and values pass through LDS in tiles of 64, and where WK is 2 a wave
+// takes 32 of each. S^T = K Q^T leaves a query's scores in one lane (and its other half), in the order in which the next
+// product takes them.
+template <int EL, int WQ, int WK>
+__global__ __launch_bounds__(64 * WQ * WK, 2) void train_forward_kernel(const Args a) {
+    constexpr int P = parts_of(EL), NT = 64 * WQ * WK, NS = 2 / WK;
+    __shared__ Tile<P> kt, vt;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wq = wave % WQ, wk = wave / WQ, half = lane >> 5;
+    const unsigned unit = blockIdx.x / (unsigned)a.pairs;
+    const int pair = blockIdx.x % (unsigned)a.pairs, tile = unit % (unsigned)a.q_tiles, split = unit / (unsigned)a.q_tiles;
+    const int e = pair / a.heads, h = pair % a.heads, hk = h / (a.heads / a.kv_heads);
+    const int q_len = length_of(a.q_lengths, e, a.q_rows), len = length_of(a.lengths, e, a.rows);
+    if (tile * 32 * WQ >= q_len) return;
+    const int query = tile * 32 * WQ + 32 * wq + (lane & 31);
+    const bool mine = query < q_len;
+    bf16x8 qb[4][P];
+    own_row<EL>(a.q, at(a.qs, e, h, query), mine, lane, qb);
+
+    f32x16 o[2] = {};
+    float r = -INFINITY, sum = 0.f;
+    const unsigned long long seed = a.line ? *a.seed : 0;
+    const int end = min((split + 1) * a.q_chunk, (int)((len + 63) / 64));
+    auto next = [&](int t, unsigned long long &m) {
+        for (m = 0; t < end && !(m = attended(a.keep, a.words, e, t, len)); ++t) {}
+        return t;
+    };
+    Staged<EL, NT> ks, vs;
+    unsigned long long some;
+    int t = next(split * a.q_chunk, some);
+    if (t < end) ks.load(a.k, a.ks, e, hk, t * 64, len), vs.load(a.v, a.vs, e, hk, t * 64, len);
+    while (t < end) {
+        __syncthreads();
+        ks.store(kt, some, nullptr);
+        vs.store(vt, some, nullptr);
+        __syncthreads();
+        unsigned long long following;
+        const int n = next(t + 1, following);
+        if (n < end) ks.load(a.k, a.ks, e, hk, n * 64, len), vs.load(a.v, a.vs, e, hk, n * 64, len);
+
+        f32x16 s[NS] = {};
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int b = 0; b < NS; ++b) {
+                bf16x8 x[P];
+                rows_operand<P>(kt, 32 * (WK == 1 ? b : wk), c, lane, x);
+                mma<P>(s[b], x, qb[c]);
+            }
+        float top = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < NS; ++b) {
+            const unsigned bits = (unsigned)(some >> (32 * (WK == 1 ? b : wk) + 4 * half));
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if (some != ~0ull) s[b][i] = bits >> (8 * (i / 4) + i % 4) & 1 ? s[b][i] : -INFINITY;
+                top = fmaxf(top, s[b][i]);
+            }
+        }
+        // A scale is positive: the largest score is that of the largest product.
+        top = fmaxf(top, other_half(top));
+        const float upto = fmaxf(r, ceilf(top * a.c));
+        if (__any(upto > r)) {
+            const float f = r == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(r - upto);
+            sum *= f;
+#pragma unroll
+            for (int d = 0; d < 2; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= f;
+            r = upto;
+        }
+        const float ref = r == -INFINITY ? 0.f : r;
+#pragma unroll
+        for (int b = 0; b < NS; ++b) {
+            const int sub = WK == 1 ? b : wk;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], a.c, -ref));
+                sum += s[b][i];
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                if (a.line) {
+                    const u32x4 z = philox(2 * (4 * t + 2 * sub + c) + half, query, pair, a.site, seed);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) s[b][8 * c + j] = kept16(z, j, a.line) ? s[b][8 * c + j] : 0.f;
+                }
+                float p[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) p[j] = s[b][8 * c + j];
+                bf16x8 pb[P];
+                split8<P>(p, pb);
+#pragma unroll
+                for (int d = 0; d < 2; ++d) {
+                    bf16x8 x[P];
+                    dims_operand<P>(vt, 32 * sub + 16 * c, d, lane, x);
+                    mma<P>(o[d], x, pb);
+                }
+            }
+        }
+        t = n, some = following;
+    }
+    sum += other_half(sum);
+    if constexpr (WK == 2) {
+        // The second wave's half of the keys joins the first's.
+        struct Half {
+            float o[32][64], r[64], sum[64];
+        };
+        static_assert(sizeof(Half) <= sizeof(Tile<P>));
+        Half *join = reinterpret_cast<Half *>(&kt);
+        __syncthreads();
+        if (wk == 1) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) join->o[i][lane] = o[i / 16][i % 16];
+            join->r[lane] = r, join->sum[lane] = sum;
+        }
+        __syncthreads();
+        if (wk == 1) return;
+        const float upto = fmaxf(r, join->r[lane]), ref = upto == -INFINITY ? 0.f : upto;
+        const float f = __builtin_amdgcn_exp2f(r - ref), g = __builtin_amdgcn_exp2f(join->r[lane] - ref);
+        r = upto, sum = sum * f + join->sum[lane] * g;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i / 16][i % 16] = o[i / 16][i % 16] * f + join->o[i][lane] * g;
+    }
+    if (!mine) return;
+    const long long row = (long long)pair * a.q_rows + query;
+    if (a.q_splits > 1) {
+        float *part = a.q_part + ((long long)split * a.pairs * a.q_rows + row) * 64;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const f32x16 &x = o[i / 4];
+            const int j = 4 * (i % 4);
+            *reinterpret_cast<f32x4 *>(part + 32 * (i / 4) + 2 * j + 4 * half) = f32x4{x[j], x[j + 1], x[j + 2], x[j + 3]};
+        }
+        if (!half) {
+            float *m = a.q_part + (long long)a.q_splits * a.pairs * a.q_rows * 64 + ((long long)split * a.pairs * a.q_rows + row) * 2;
+            *reinterpret_cast<f32x2 *>(m) = f32x2{r, sum};
+        }
+        return;
+    }
+    const float f = sum == 0.f ? 0.f : a.w / sum;
+    const long long to = at(a.os, e, h, query);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const f32x16 &x = o[i / 4];
+        const int j = 4 * (i % 4);
+        store4<EL>(a.out, to + 32 * (i / 4) + 2 * j + 4 * half, f32x4{x[j] * f, x[j + 1] * f, x[j + 2] * f, x[j + 3] * f});
+    }
+    if (!half) {
+        const float ref = r == -INFINITY ? 0.f : r;
+        if (a.stats) *reinterpret_cast<f32x2 *>(a.stats + 2 * row) = f32x2{ref, sum};
+        if (a.lse) a.lse[row] = kLn2 * (ref + __builtin_amdgcn_logf(sum));
+    }
+}
+
+// Joins the splits of a query: sixteen lanes to a row.
+template <int EL>
+__global__ __launch_bounds__(256) void train_merge_kernel(const Args a) {
+    const long long rows = (long long)a.pairs * a.q_rows;
+    const long long row = (long long)blockIdx.x * 16 + threadIdx.x / 16;
+    if (row >= rows) return;
+    const int pair = (int)(row / a.q_rows), query = (int)(row % a.q_rows), e = pair / a.heads, lane = threadIdx.x & 15;
+    if (query >= length_of(a.q_lengths, e, a.q_rows)) return;
+    const float *m = a.q_part + (long long)a.q_splits * rows * 64;
+    float r = -INFINITY;
+    for (int s = 0; s < a.q_splits; ++s) r = fmaxf(r, m[(s * rows + row) * 2]);
+    const float ref = r == -INFINITY ? 0.f : r;
+    float sum = 0.f;
+    f32x4 o = {};
+    for (int s = 0; s < a.q_splits; ++s) {
+        const f32x2 x = *reinterpret_cast<const f32x2 *>(m + (s * rows + row) * 2);
+        const float f = __builtin_amdgcn_exp2f(x[0] - ref);
+        sum += x[1] * f;
+        o += *reinterpret_cast<const f32x4 *>(a.q_part + (s * rows + row) * 64 + 4 * lane) * f;
+    }
+    const float f = sum == 0.f ? 0.f : a.w / sum;
+    store4<EL>(a.out, at(a.os, e, pair % a.heads, query) + 4 * lane, o * f);
+    if (!lane) {
+        if (a.stats) *reinterpret_cast<f32x2 *>(a.stats + 2 * row) = f32x2{ref, sum};
+        if (a.lse) a.lse[row] = kLn2 * (ref + __builtin_amdgcn_logf(sum));
+    }
+}
+
+// ---- backward ----
+
+// What the backward pass needs of each query: {r, 1 / s, delta}; r is +inf (all weights 0) for one that attends to nothing
+// or lies past the length. Sixteen lanes to a row.
+template <int EL>
+__global__ __launch_bounds__(256) void train_record_kernel(const Args a) {
+    const long long rows = (long long)a.pairs * a.q_rows;
+    const long long row = (long long)blockIdx.x * 16 + threadIdx.x / 16;
+    if (row >= rows) return;
+    const int pair = (int)(row / a.q_rows), query = (int)(row % a.q_rows), lane = threadIdx.x & 15;
+    const int e = pair / a.heads, h = pair % a.heads;
+    f32x4 record = {INFINITY, 0.f, 0.f, 0.f};
+    const f32x2 x = *reinterpret_cast<const f32x2 *>(a.stats + 2 * row);
+    if (query < length_of(a.q_lengths, e, a.q_rows) && x[1] != 0.f) {
+        const f32x4 o = load4<EL>(a.out, at(a.os, e, h, query) + 4 * lane);
+        const f32x4 g = load4<EL>(a.dout, at(a.gs, e, h, query) + 4 * lane);
+        float d = o[0] * g[0] + o[1] * g[1] + o[2] * g[2] + o[3] * g[3];
+#pragma unroll
+        for (int i = 8; i; i >>= 1) d += __shfl_xor(d, i, 16);
+        record = f32x4{x[0], 1.f / x[1], d, 0.f};
+    }
+    if (!lane) a.record[row] = record;
+}
+
+template <int P>
+struct Streamed {
+    Tile<P> x, y;
+    alignas(16) float r[kTile], inv[kTile], delta[kTile];
+};
+
+// The gradient of 32 queries a wave: dS^T = K Q^T, V dout^T, then K^T dS, over a split's key tiles.
+template <int EL>
+__device__ __forceinline__ void queries_backward(const Args &a, Streamed<parts_of(EL)> &lds, unsigned block) {
+    constexpr int P = parts_of(EL);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const unsigned unit = block / (unsigned)a.pairs;
+    const int pair = block % (unsigned)a.pairs, tile = unit % (unsigned)a.q_tiles, split = unit / (unsigned)a.q_tiles;
+    const int e = pair / a.heads, h = pair % a.heads, hk = h / (a.heads / a.kv_heads);
+    const int q_len = length_of(a.q_lengths, e, a.q_rows), len = length_of(a.lengths, e, a.rows);
+    if (tile * 128 >= q_len) return;
+    const int query = tile * 128 + 32 * wave + (lane & 31);
+    const bool mine = query < q_len;
+    const long long row = (long long)pair * a.q_rows + query;
+    f32x4 record = {INFINITY, 0.f, 0.f, 0.f};
+    if (mine) record = a.record[row];
+    const bool some_row = record[0] != INFINITY;
+    bf16x8 qb[4][P], gb[4][P];
+    own_row<EL>(a.q, at(a.qs, e, h, query), some_row, lane, qb);
+    own_row<EL>(a.dout, at(a.gs, e, h, query), some_row, lane, gb);
+
+    f32x16 o[2] = {};
+    const unsigned long long seed = a.line ? *a.seed : 0;
+    const int end = min((split + 1) * a.q_chunk, (int)((len + 63) / 64));
+    auto next = [&](int t, unsigned long long &m) {
+        for (m = 0; t < end && !(m = attended(a.keep, a.words, e, t, len)); ++t) {}
+        return t;
+    };
+    Staged<EL, 256> ks, vs;
+    unsigned long long some;
+    int t = next(split * a.q_chunk, some);
+    if (t < end) ks.load(a.k, a.ks, e, hk, t * 64, len), vs.load(a.v, a.vs, e, hk, t * 64, len);
+    while (t < end) {
+        __syncthreads();
+        ks.store(lds.x, some, nullptr);
+        vs.store(lds.y, some, nullptr);
+        __syncthreads();
+        unsigned long long following;
+        const int n = next(t + 1, following);
+        if (n < end) ks.load(a.k, a.ks, e, hk, n * 64, len), vs.load(a.v, a.vs, e, hk, n * 64, len);
+#pragma unroll 1
+        for (int b = 0; b < 2; ++b) {
+            f32x16 s = {}, dp = {};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                bf16x8 x[P];
+                rows_operand<P>(lds.x, 32 * b, c, lane, x);
+                mma<P>(s, x, qb[c]);
+                rows_operand<P>(lds.y, 32 * b, c, lane, x);
+                mma<P>(dp, x, gb[c]);
+            }
+            const unsigned bits = (unsigned)(some >> (32 * b + 4 * half));
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                u32x4 z;
+                if (a.line) z = philox(2 * (4 * t + 2 * b + c) + half, query, pair, a.site, seed);
+                float ds[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int i = 8 * c + j;
+                    float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, -record[0]));
+                    if (some != ~0ull) p = bits >> (8 * (i / 4) + i % 4) & 1 ? p : 0.f;
+                    float g = dp[i];
+                    if (a.line) g = kept16(z, j, a.line) ? g : 0.f;
+                    ds[j] = p * __builtin_fmaf(g, a.w, -record[2]);
+                }
+                bf16x8 db[P];
+                split8<P>(ds, db);
+#pragma unroll
+                for (int d = 0; d < 2; ++d) {
+                    bf16x8 x[P];
+                    dims_operand<P>(lds.x, 32 * b + 16 * c, d, lane, x);
+                    mma<P>(o[d], x, db);
+                }
+            }
+        }
+        t = n, some = following;
+    }
+    if (!mine) return;
+    const float f = a.scale * record[1];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const f32x16 &x = o[i / 4];
+        const int j = 4 * (i % 4), dim = 32 * (i / 4) + 2 * j + 4 * half;
+        const f32x4 y = {x[j] * f, x[j + 1] * f, x[j + 2] * f, x[j + 3] * f};
+        if (a.q_splits > 1)
+            *reinterpret_cast<f32x4 *>(a.q_part + ((long long)split * a.pairs * a.q_rows + row) * 64 + dim) = y;
+        else
+            store4<EL>(a.dq, at(a.dqs, e, h, query) + dim, y);
+    }
+}
+
+// Lane l (and l + 32) of the result: bit i of key l's word is whether query i of a wave's 32 keeps its weight of that key.
+// Each lane draws its query's numbers as the other passes do; a comparison's bits over the wave are then a key's word.
+__device__ __forceinline__ unsigned kept_words(unsigned cell, int query, int pair, unsigned site, unsigned line,
+                                               unsigned long long seed, int half) {
+    unsigned mine = 0;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        const u32x4 z = philox(cell + 2 * c + half, query, pair, site, seed);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const unsigned long long word = __ballot(kept16(z, j, line));
+            const int key = 16 * c + 8 * (j / 4) + j % 4;  // of the lower half's cell; the upper half's is 4 further
+            mine = irx_writelane((unsigned)word, key, mine);
+            mine = irx_writelane((unsigned)(word >> 32), key + 4, mine);
+        }
+    }
+    const auto r = __builtin_amdgcn_permlane32_swap(mine, mine, false, false);
+    return half ? r[0] : mine;
+}
+
+// The gradients of 32 keys a wave: S = Q K^T, dout V^T, then dout^T P and Q^T dS, over a split's query tiles of every head
+// that shares the keys.
+template <int EL>
+__device__ __forceinline__ void keys_backward(const Args &a, Streamed<parts_of(EL)> &lds, unsigned block) {
+    constexpr int P = parts_of(EL);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int group = a.heads / a.kv_heads, owners = a.pairs / group;
+    const unsigned unit = block / (unsigned)owners;
+    const int owner = block % (unsigned)owners, tile = unit % (unsigned)a.k_tiles, split = unit / (unsigned)a.k_tiles;
+    const int e = owner / a.kv_heads, hk = owner % a.kv_heads;
+    const int q_len = length_of(a.q_lengths, e, a.q_rows), len = length_of(a.lengths, e, a.rows);
+    if (tile * 128 >= len) return;
+    const int key = tile * 128 + 32 * wave + (lane & 31);
+    const unsigned long long here[2] = {attended(a.keep, a.words, e, 2 * tile, len), attended(a.keep, a.words, e, 2 * tile + 1, len)};
+    const bool in = here[wave / 2] >> (32 * (wave & 1) + (lane & 31)) & 1;
+    bf16x8 kb[4][P], vb[4][P];
+    own_row<EL>(a.k, at(a.ks, e, hk, key), in, lane, kb);
+    own_row<EL>(a.v, at(a.vs, e, hk, key), in, lane, vb);
+
+    f32x16 dk[2] = {}, dv[2] = {};
+    const unsigned long long seed = a.line ? *a.seed : 0;
+    // Query tiles that hold a query, of all heads of the group in turn.
+    const int q_tiles = (q_len + kTile - 1) / kTile;
+    const int end = here[0] | here[1] ? min((split + 1) * a.k_chunk, group * q_tiles) : 0;
+    int u = split * a.k_chunk;
+    Staged<EL, 256> qs, gs;
+    f32x4 record = {};
+    auto load = [&](int i) {
+        const int h = hk * group + i / q_tiles, row0 = i % q_tiles * kTile;
+        qs.load(a.q, a.qs, e, h, row0, q_len);
+        gs.load(a.dout, a.gs, e, h, row0, q_len);
+        if (threadIdx.x < kTile) {
+            record = f32x4{INFINITY, 0.f, 0.f, 0.f};
+            if (row0 + (int)threadIdx.x < q_len)
+                record = a.record[(long long)(e * a.heads + h) * a.q_rows + row0 + threadIdx.x];
+        }
+    };
+    if (u < end) load(u);
+    for (; u < end; ++u) {
+        const int h = hk * group + u / q_tiles, row0 = u % q_tiles * kTile;
+        __syncthreads();
+        if (threadIdx.x < kTile) {
+            lds.r[threadIdx.x] = record[0];
+            lds.inv[threadIdx.x] = record[1];
+            lds.delta[threadIdx.x] = EL == kTrainBF16 ? record[2] : record[2] * record[1];
+        }
+        __syncthreads();
+        {
+            unsigned long long some = __ballot(lds.r[lane] != INFINITY);
+            qs.store(lds.x, some, nullptr);
+            // 1 / s goes with dout where its parts are made; BF16's are not touched, and the weights take it.
+            gs.store(lds.y, some, EL == kTrainBF16 ? nullptr : lds.inv);
+        }
+        __syncthreads();
+        if (u + 1 < end) load(u + 1);
+#pragma unroll 1
+        for (int b = 0; b < 2; ++b) {
+            f32x16 s = {}, dp = {};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                bf16x8 x[P];
+                rows_operand<P>(lds.x, 32 * b, c, lane, x);
+                mma<P>(s, x, kb[c]);
+                rows_operand<P>(lds.y, 32 * b, c, lane, x);
+                mma<P>(dp, x, vb[c]);
+            }
+            unsigned kept = ~0u;
+            if (a.line)
+                kept = kept_words(2 * (tile * 8 + 2 * wave), row0 + 32 * b + (lane & 31), e * a.heads + h, a.site, a.line, seed, half) >> (4 * half);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float p[8], ds[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int i = 8 * c + j, q = 32 * b + 8 * (i / 4) + 4 * half + i % 4;
+                    p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, -lds.r[q]));
+                    if constexpr (EL == kTrainBF16) p[j] *= lds.inv[q];
+                    const bool z = kept >> (8 * (i / 4) + i % 4) & 1;
+                    ds[j] = p[j] * __builtin_fmaf(a.line && !z ? 0.f : dp[i], a.w, -lds.delta[q]);
+                    if (a.line) p[j] = z ? p[j] : 0.f;
+                }
+                bf16x8 x[P], pb[P];
+                split8<P>(p, pb);
+#pragma unroll
+                for (int d = 0; d < 2; ++d) {
+                    dims_operand<P>(lds.y, 32 * b + 16 * c, d, lane, x);
+                    mma<P>(dv[d], x, pb);
+                }
+                split8<P>(ds, pb);
+#pragma unroll
+                for (int d = 0; d < 2; ++d) {
+                    dims_operand<P>(lds.x, 32 * b + 16 * c, d, lane, x);
+                    mma<P>(dk[d], x, pb);
+                }
+            }
+        }
+    }
+    if (key >= len) return;
+    // A key that is not attended to has no gradient, whatever its lane summed.
+    const float fk = in ? a.scale : 0.f, fv = in ? a.w : 0.f;
+    const long long row = (long long)owner * a.rows + key, plane = (long long)owners * a.rows * 64;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const f32x16 &x = dk[i / 4], &y = dv[i / 4];
+        const int j = 4 * (i % 4), dim = 32 * (i / 4) + 2 * j + 4 * half;
+        f32x4 gk = {x[j] * fk, x[j + 1] * fk, x[j + 2] * fk, x[j + 3] * fk};
+        f32x4 gv = {y[j] * fv, y[j + 1] * fv, y[j + 2] * fv, y[j + 3] * fv};
+        if (!in) gk = gv = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (a.k_splits > 1) {
+            float *part = a.k_part + 2 * split * plane + row * 64 + dim;
+            *reinterpret_cast<f32x4 *>(part) = gk;
+            *reinterpret_cast<f32x4 *>(part + plane) = gv;
+        } else {
+            store4<EL>(a.dk, at(a.dks, e, hk, key) + dim, gk);
+            store4<EL>(a.dv, at(a.dvs, e, hk, key) + dim, gv);
+        }
+    }
+}
+
+template <int EL>
+__global__ __launch_bounds__(256, 2) void train_backward_kernel(const Args a) {
+    __shared__ Streamed<parts_of(EL)> lds;
+    if (blockIdx.x < (unsigned)a.q_blocks)
+        queries_backward<EL>(a, lds, blockIdx.x);
+    else
+        keys_backward<EL>(a, lds, blockIdx.x - a.q_blocks);
+}
+
+// Sums the splits' parts, in order. Rows of dq, then of dk, then of dv; sixteen lanes to a row.
+template <int EL>
+__global__ __launch_bounds__(256) void train_sum_kernel(const Args a) {
+    const long long q_rows = a.q_splits > 1 ? (long long)a.pairs * a.q_rows : 0;
+    const long long k_rows = a.k_splits > 1 ? (long long)(a.pairs / (a.heads / a.kv_heads)) * a.rows : 0;
+    long long row = (long long)blockIdx.x * 16 + threadIdx.x / 16;
+    const int lane = threadIdx.x & 15;
+    const float *part;
+    long long step;
+    int splits;
+    void *to;
+    long long offset;
+    if (row < q_rows) {
+        const int pair = (int)(row / a.q_rows), query = (int)(row % a.q_rows), e = pair / a.heads;
+        if (query >= length_of(a.q_lengths, e, a.q_rows)) return;
+        part = a.q_part + row * 64, step = q_rows * 64, splits = a.q_splits;
+        to = a.dq, offset = at(a.dqs, e, pair % a.heads, query);
+    } else {
+        row -= q_rows;
+        if (row >= 2 * k_rows) return;
+        const bool values = row >= k_rows;
+        if (values) row -= k_rows;
+        const int owner = (int)(row / a.rows), key = (int)(row % a.rows), e = owner / a.kv_heads, hk = owner % a.kv_heads;
+        if (key >= length_of(a.lengths, e, a.rows)) return;
+        part = a.k_part + (values ? k_rows * 64 : 0) + row * 64, step = 2 * k_rows * 64, splits = a.k_splits;
+        to = values ? a.dv : a.dk, offset = values ? at(a.dvs, e, hk, key) : at(a.dks, e, hk, key);
+    }
+    f32x4 sum = {};
+    for (int s = 0; s < splits; ++s) sum += *reinterpret_cast<const f32x4 *>(part + s * step + 4 * lane);
+    store4<EL>(to, offset + 4 * lane, sum);
+}
+
+// ---- dropout ----
+
+struct DropArgs {
+    const void *x, *residual;
+    void *out;
+    long long xs, rs, os;
+    long long groups;  // of eight columns, in all
+    int per_row, width;
+    const unsigned long long *seed;
+    unsigned site, line;
+    float w;
+};
+
+// Eight adjacent numbers of a row to a thread.
+template <int EL>
+__global__ __launch_bounds__(256) void train_dropout_kernel(const DropArgs a) {
+    const long long g = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (g >= a.groups) return;
+    const unsigned row = (unsigned)g / (unsigned)a.per_row, col = (unsigned)g % (unsigned)a.per_row;
+    const int left = min(8, a.width - 8 * (int)col);
+    const long long xi = row * a.xs + 8ll * col, ri = row * a.rs + 8ll * col, oi = row * a.os + 8ll * col;
+    float x[8], y[8] = {};
+    typedef std::conditional_t<EL == kTrainF32, float, std::conditional_t<EL == kTrainF16, _Float16, __bf16>> T;
+    if (left == 8) {
+        to_floats<EL>(load8<EL>(a.x, xi), x);
+        if (a.residual) to_floats<EL>(load8<EL>(a.residual, ri), y);
+    } else {
+        for (int j = 0; j < 8; ++j) {
+            x[j] = j < left ? (float)static_cast<const T *>(a.x)[xi + j] : 0.f;
+            if (a.residual && j < left) y[j] = (float)static_cast<const T *>(a.residual)[ri + j];
+        }
+    }
+    if (a.line) {
+        const u32x4 z = philox(col, row, ~0u, a.site, *a.seed);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = kept16(z, j, a.line) ? x[j] * a.w : 0.f;
+    }
+    if (a.residual)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] += y[j];
+    if (left == 8) {
+        store4<EL>(a.out, oi, f32x4{x[0], x[1], x[2], x[3]});
+        store4<EL>(a.out, oi + 4, f32x4{x[4], x[5], x[6], x[7]});
+    } else {
+        for (int j = 0; j < left; ++j) static_cast<T *>(a.out)[oi + j] = (T)x[j];
+    }
+}
+
+// ---- plans ----
+
+struct Plan {
+    int q_tiles, q_splits, q_chunk, k_tiles, k_splits, k_chunk;
+    bool few;  // forward: 32 queries to a workgroup
+    size_t record, q_part, k_part;  // bytes
+    double blocks;
+};
+
+int splits_of(double length, double target, long long tiles) {
+    const long long most = std::max(1ll, tiles / 4);  // a split walks four tiles at least
+    return (int)std::min<long long>(std::max(1ll, std::llround(length / target)), std::min(most, 256ll));
+}
+
+Plan plan(const TrainShape &s, int element, bool backward, int compute_units) {
+    Plan p{};
+    const long long pairs = (long long)s.estimators * s.heads, owners = (long long)s.estimators * s.kv_heads;
+    const long long words = (s.rows + 63) / 64, q_words = (s.q_rows + 63) / 64, group = s.heads / s.kv_heads;
+    const double slots = 2.0 * compute_units;
+    p.few = !backward && s.q_rows <= 32;
+    p.q_tiles = (int)ceil_div(s.q_rows, p.few ? 32 : 128);
+    p.k_tiles = (int)ceil_div(s.rows, 128);
+    if (backward) {
+        // A tile of keys costs a unit of queries three products, a tile of queries a unit of keys four. No workgroup walks
+        // further than its share of all the work.
+        const double all = 3.0 * pairs * p.q_tiles * words + 4.0 * owners * p.k_tiles * group * q_words;
+        const double share = std::max(all / slots, 12.0);
+        p.q_splits = splits_of(3.0 * words, share, words);
+        p.k_splits = splits_of(4.0 * group * q_words, share, group * q_words);
+    } else {
+        p.q_splits = splits_of((double)words, std::max(pairs * p.q_tiles * words / slots, 4.0), words);
+        p.k_splits = 1;
+    }
+    p.q_chunk = (int)ceil_div(words, p.q_splits);
+    p.q_splits = (int)ceil_div(words, p.q_chunk);
+    p.k_chunk = (int)ceil_div(group * q_words, p.k_splits);
+    p.k_splits = (int)ceil_div(group * q_words, p.k_chunk);
+    const size_t rows = (size_t)pairs * s.q_rows;
+    p.record = backward ? rows * 16 : 0;
+    p.q_part = p.q_splits > 1 ? (size_t)p.q_splits * rows * (backward ? 256 : 264) : 0;
+    p.k_part = p.k_splits > 1 ? (size_t)p.k_splits * owners * s.rows * 512 : 0;
+    p.blocks = (double)pairs * p.q_tiles * p.q_splits + (backward ? (double)owners * p.k_tiles * p.k_splits : 0.0);
+    return p;
+}
+
+size_t round16(size_t n) { return (n + 15) & ~(size_t)15; }
+
+Args common(const TrainInputs &a, const Plan &p) {
+    Args k{};
+    const TrainShape &s = a.shape;
+    k.q = a.q, k.k = a.k, k.v = a.v;
+    std::copy_n(a.qs, 3, k.qs), std::copy_n(a.ks, 3, k.ks), std::copy_n(a.vs, 3, k.vs);
+    k.q_lengths = a.q_lengths, k.lengths = a.lengths, k.keep = a.keep;
+    k.heads = s.heads, k.kv_heads = s.kv_heads, k.pairs = s.estimators * s.heads, k.q_rows = s.q_rows, k.rows = s.rows;
+    k.words = (int)ceil_div(s.rows, 64);
+    k.scale = a.scale, k.c = a.scale * kLog2e;
+    k.seed = a.drop.seed, k.site = a.drop.site, k.line = a.drop.dropped << 16;
+    k.w = 65536.f / (float)(65536u - a.drop.dropped);
+    k.q_tiles = p.q_tiles, k.q_splits = p.q_splits, k.q_chunk = p.q_chunk;
+    k.k_tiles = p.k_tiles, k.k_splits = p.k_splits, k.k_chunk = p.k_chunk;
+    return k;
+}
+
+template <int EL>
+void forward(const TrainInputs &a, const TrainForward &f, const Plan &p, hipStream_t stream) {
+    Args k = common(a, p);
+    k.out = f.out, k.stats = f.stats, k.lse = f.lse, k.q_part = static_cast<float *>(f.workspace);
+    std::copy_n(f.os, 3, k.os);
+    const dim3 grid((unsigned)p.blocks);
+    {
+        KernelTimer timer(kFamIcl, stream, 256.0 * k.pairs * k.q_rows * k.rows, 0.0);
+        if (p.few)
+            hipLaunchKernelGGL((train_forward_kernel<EL, 1, 2>), grid, dim3(128), 0, stream, k);
+        else
+            hipLaunchKernelGGL((train_forward_kernel<EL, 4, 1>), grid, dim3(256), 0, stream, k);
+        IRX_HIP(hipGetLastError());
+    }
+    if (p.q_splits > 1) {
+        KernelTimer timer(kFamIclMerge, stream, 0.0, (double)p.q_part);
+        hipLaunchKernelGGL(train_merge_kernel<EL>, dim3(ceil_div((size_t)k.pairs * k.q_rows, 16)), dim3(256), 0, stream, k);
+        IRX_HIP(hipGetLastError());
+    }
+}
+
+template <int EL>
+void backward(const TrainInputs &a, const TrainBackward &b, const Plan &p, hipStream_t stream) {
+    Args k = common(a, p);
+    k.out = const_cast<void *>(b.out), k.stats = const_cast<float *>(b.stats), k.dout = b.dout;
+    k.dq = b.dq, k.dk = b.dk, k.dv = b.dv;
+    std::copy_n(b.os, 3, k.os), std::copy_n(b.gs, 3, k.gs);
+    std::copy_n(b.dqs, 3, k.dqs), std::copy_n(b.dks, 3, k.dks), std::copy_n(b.dvs, 3, k.dvs);
+    char *space = static_cast<char *>(b.workspace);
+    k.record = reinterpret_cast<f32x4 *>(space);
+    k.q_part = reinterpret_cast<float *>(space + round16(p.record));
+    k.k_part = reinterpret_cast<float *>(space + round16(p.record) + round16(p.q_part));
+    const size_t rows = (size_t)k.pairs * k.q_rows, owned = (size_t)a.shape.estimators * a.shape.kv_heads * k.rows;
+    {
+        KernelTimer timer(kFamGlue, stream, 0.0, rows * (EL == kTrainF32 ? 512.0 : 256.0));
+        hipLaunchKernelGGL(train_record_kernel<EL>, dim3(ceil_div(rows, 16)), dim3(256), 0, stream, k);
+        IRX_HIP(hipGetLastError());
+    }
+    k.q_blocks = b.dq ? (int)((size_t)k.pairs * p.q_tiles * p.q_splits) : 0;
+    const size_t k_blocks = b.dk ? (size_t)a.shape.estimators * a.shape.kv_heads * p.k_tiles * p.k_splits : 0;
+    {
+        KernelTimer timer(kFamIcl, stream, 640.0 * rows * k.rows, 0.0);
+        hipLaunchKernelGGL(train_backward_kernel<EL>, dim3((unsigned)(k.q_blocks + k_blocks)), dim3(256), 0, stream, k);
+        IRX_HIP(hipGetLastError());
+    }
+    if (!b.dq) k.q_splits = 1;
+    if (!b.dk) k.k_splits = 1;
+    const size_t sums = (k.q_splits > 1 ? rows : 0) + (k.k_splits > 1 ? 2 * owned : 0);
+    if (sums) {
+        KernelTimer timer(kFamIclMerge, stream, 0.0, (double)(p.q_part + p.k_part));
+        hipLaunchKernelGGL(train_sum_kernel<EL>, dim3(ceil_div(sums, 16)), dim3(256), 0, stream, k);
+        IRX_HIP(hipGetLastError());
+    }
+}
+
+}  // namespace
+
+size_t train_workspace(const TrainShape &s, int element, bool backward, int compute_units) {
+    const Plan p = plan(s, element, backward, compute_units);
+    return round16(p.record) + round16(p.q_part) + round16(p.k_part);
+}
+
+bool train_fits(const TrainShape &s, int element, bool backward, int compute_units) {
+    // 256 work-items to a workgroup, less than 2^32 in a launch.
+    const double rows = (double)s.estimators * std::max((double)s.heads * s.q_rows, 2.0 * s.kv_heads * s.rows);
+    return plan(s, element, backward, compute_units).blocks < 16777216.0 && rows < 134217728.0;
+}
+
+void train_attention(const TrainInputs &a, const TrainForward &f, int compute_units, hipStream_t stream) {
+    const Plan p = plan(a.shape, a.element, false, compute_units);
+    if (a.element == kTrainF32)
+        forward<kTrainF32>(a, f, p, stream);
+    else if (a.element == kTrainF16)
+        forward<kTrainF16>(a, f, p, stream);
+    else
+        forward<kTrainBF16>(a, f, p, stream);
+}
+
+void train_backward(const TrainInputs &a, const TrainBackward &b, int compute_units, hipStream_t stream) {
+    const Plan p = plan(a.shape, a.element, true, compute_units);
+    if (a.element == kTrainF32)
+        backward<kTrainF32>(a, b, p, stream);
+    else if (a.element == kTrainF16)
+        backward<kTrainF16>(a, b, p, stream);
+    else
+        backward<kTrainBF16>(a, b, p, stream);
+}
+
+void train_dropout(const TrainRows &a, hipStream_t stream) {
+    DropArgs k{};
+    k.x = a.x, k.residual = a.residual, k.out = a.out, k.xs = a.xs, k.rs = a.rs, k.os = a.os;
+    k.width = (int)a.width, k.per_row = (int)ceil_div(a.width, 8), k.groups = (long long)a.rows * k.per_row;
+    k.seed = a.drop.seed, k.site = a.drop.site, k.line = a.drop.dropped << 16;
+    k.w = 65536.f / (float)(65536u - a.drop.dropped);
+    const dim3 grid(ceil_div((size_t)k.groups, 256));
+    KernelTimer timer(kFamGlue, stream, 0.0, (double)a.rows * a.width * (a.element == kTrainF32 ? 4 : 2) * (a.residual ? 3 : 2));
+    if (a.element == kTrainF32)
+        hipLaunchKernelGGL(train_dropout_kernel<kTrainF32>, grid, dim3(256), 0, stream, k);
+    else if (a.element == kTrainF16)
+        hipLaunchKernelGGL(train_dropout_kernel<kTrainF16>, grid, dim3(256), 0, stream, k);
+    else
+        hipLaunchKernelGGL(train_dropout_kernel<kTrainBF16>, grid, dim3(256), 0, stream, k);
+    IRX_HIP(hipGetLastError());
+}
+
+}  // namespace irx

@@ -59,7 +59,7 @@ class KernelStats(ctypes.Structure):
                 ("bytes", ctypes.c_double), ("busy_milliseconds", ctypes.c_double)]
 
 
-ELEMENT_F32, ELEMENT_F16 = 0, 1
+ELEMENT_F32, ELEMENT_F16, ELEMENT_BF16 = 0, 1, 2
 
 
 class Icl4Shape(ctypes.Structure):
@@ -78,6 +78,33 @@ class Icl4Rows(ctypes.Structure):
 class Icl4Queries(ctypes.Structure):
     _fields_ = [("shape", Icl4Shape), ("query_rows", _sz), ("element", ctypes.c_int), ("q", ctypes.c_void_p),
                 ("q_strides", Strides), ("lengths", ctypes.c_void_p), ("keep", ctypes.c_void_p)]
+
+
+class TrainShape(ctypes.Structure):
+    _fields_ = [("estimators", _sz), ("heads", _sz), ("kv_heads", _sz), ("query_rows", _sz), ("rows", _sz)]
+
+
+class TrainDrop(ctypes.Structure):
+    _fields_ = [("seed", ctypes.c_void_p), ("site", ctypes.c_uint32), ("dropped", ctypes.c_uint32)]
+
+
+class TrainInputs(ctypes.Structure):
+    _fields_ = [("shape", TrainShape), ("element", ctypes.c_int), ("scale", ctypes.c_float), ("q", ctypes.c_void_p),
+                ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("q_strides", Strides), ("k_strides", Strides),
+                ("v_strides", Strides), ("query_lengths", ctypes.c_void_p), ("lengths", ctypes.c_void_p),
+                ("keep", ctypes.c_void_p), ("drop", TrainDrop)]
+
+
+class TrainGradients(ctypes.Structure):
+    _fields_ = [("out", ctypes.c_void_p), ("stats", ctypes.c_void_p), ("dout", ctypes.c_void_p),
+                ("out_strides", Strides), ("dout_strides", Strides), ("dq", ctypes.c_void_p), ("dk", ctypes.c_void_p),
+                ("dv", ctypes.c_void_p), ("dq_strides", Strides), ("dk_strides", Strides), ("dv_strides", Strides)]
+
+
+class TrainRows(ctypes.Structure):
+    _fields_ = [("rows", _sz), ("width", _sz), ("element", ctypes.c_int), ("x", ctypes.c_void_p),
+                ("residual", ctypes.c_void_p), ("out", ctypes.c_void_p), ("x_stride", _sz), ("residual_stride", _sz),
+                ("out_stride", _sz), ("drop", TrainDrop)]
 
 
 # Every entry point include/ironicl_hip.h declares, with its ctypes signature.
@@ -141,6 +168,13 @@ SIGNATURES = {
     "irx_icl4_attention": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_float,
                                           ctypes.c_void_p, _sz, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                           ctypes.c_void_p, _sz, ctypes.c_void_p]),
+    # The training calls, likewise (training.py).
+    "irx_train_workspace_bytes": (_sz, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int]),
+    "irx_train_attention": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                           ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, _sz, ctypes.c_void_p]),
+    "irx_train_attention_backward": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                                    _sz, ctypes.c_void_p]),
+    "irx_train_dropout": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
     "irx_test_icl_attention_precision": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, _CF, _CF, _CF, _sz, _sz,
                                                         _sz, _F]),
     "irx_test_encode_icl8": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, _sz, _sz,
