@@ -201,9 +201,9 @@ __device__ __forceinline__ u32x4 philox(unsigned c0, unsigned c1, unsigned c2, u
 #pragma unroll
     for (int round = 0; round < 7; ++round) {
         const unsigned long long a = (unsigned long long)c0 * 0xD2511F53u, b = (unsigned long long)c2 * 0xCD9E8D57u;
-        c0 = (unsigned)(b >> 32) ^ c1 ^ k0;
+        c0 = __builtin_amdgcn_bitop3_b32((unsigned)(b >> 32), c1, k0, 0x96);  // the three's exclusive or
         c1 = (unsigned)b;
-        c2 = (unsigned)(a >> 32) ^ c3 ^ k1;
+        c2 = __builtin_amdgcn_bitop3_b32((unsigned)(a >> 32), c3, k1, 0x96);
         c3 = (unsigned)a;
         k0 += 0x9E3779B9u, k1 += 0xBB67AE85u;
     }
@@ -228,6 +228,13 @@ __device__ __forceinline__ unsigned long long attended(const unsigned long long 
     unsigned long long m = keep ? keep[(long long)e * words + word] : ~0ull;
     if (left < 64) m &= (1ull << left) - 1;
     return m;
+}
+
+// Scores of keys row0 .. + 31 of a tile that are not attended become -inf.
+__device__ __forceinline__ void leave_out(f32x16 &s, unsigned long long some, int row0, int half) {
+    const unsigned bits = (unsigned)(some >> (row0 + 4 * half));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = bits >> (8 * (i / 4) + i % 4) & 1 ? s[i] : -INFINITY;
 }
 
 struct Args {
@@ -317,10 +324,14 @@ __device__ __forceinline__ void own_row(const void *base, long long row, bool in
 // 32 WQ queries to a workgroup, 32 to a wave; keys and values pass through LDS in tiles of 64, and where WK is 2 a wave
 // takes 32 of each. S^T = K Q^T leaves a query's scores in one lane (and its other half), in the order in which the next
 // product takes them.
-template <int EL, int WQ, int WK>
-__global__ __launch_bounds__(64 * WQ * WK, 2) void train_forward_kernel(const Args a) {
+constexpr int forward_waves(int element, int wq, int wk) {  // of a SIMD: what registers and LDS leave room for
+    return element == kTrainBF16 ? 4 : element == kTrainF16 ? 2 : wq * wk == 4 ? 2 : 1;
+}
+template <int EL, int WQ, int WK, bool DROP>
+__global__ __launch_bounds__(64 * WQ * WK, forward_waves(EL, WQ, WK)) void train_forward_kernel(const Args a) {
     constexpr int P = parts_of(EL), NT = 64 * WQ * WK, NS = 2 / WK;
-    __shared__ Tile<P> kt, vt;
+    __shared__ Tile<P> tiles[2];
+    Tile<P> &kt = tiles[0], &vt = tiles[1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wq = wave % WQ, wk = wave / WQ, half = lane >> 5;
     const unsigned unit = blockIdx.x / (unsigned)a.pairs;
     const int pair = blockIdx.x % (unsigned)a.pairs, tile = unit % (unsigned)a.q_tiles, split = unit / (unsigned)a.q_tiles;
@@ -334,7 +345,7 @@ __global__ __launch_bounds__(64 * WQ * WK, 2) void train_forward_kernel(const Ar
 
     f32x16 o[2] = {};
     float r = -INFINITY, sum = 0.f;
-    const unsigned long long seed = a.line ? *a.seed : 0;
+    const unsigned long long seed = DROP ? *a.seed : 0;
     const int end = min((split + 1) * a.q_chunk, (int)((len + 63) / 64));
     auto next = [&](int t, unsigned long long &m) {
         for (m = 0; t < end && !(m = attended(a.keep, a.words, e, t, len)); ++t) {}
@@ -343,16 +354,7 @@ __global__ __launch_bounds__(64 * WQ * WK, 2) void train_forward_kernel(const Ar
     Staged<EL, NT> ks, vs;
     unsigned long long some;
     int t = next(split * a.q_chunk, some);
-    if (t < end) ks.load(a.k, a.ks, e, hk, t * 64, len), vs.load(a.v, a.vs, e, hk, t * 64, len);
-    while (t < end) {
-        __syncthreads();
-        ks.store(kt, some, nullptr);
-        vs.store(vt, some, nullptr);
-        __syncthreads();
-        unsigned long long following;
-        const int n = next(t + 1, following);
-        if (n < end) ks.load(a.k, a.ks, e, hk, n * 64, len), vs.load(a.v, a.vs, e, hk, n * 64, len);
-
+    auto work = [&] {
         f32x16 s[NS] = {};
 #pragma unroll
         for (int c = 0; c < 4; ++c)
@@ -362,16 +364,14 @@ __global__ __launch_bounds__(64 * WQ * WK, 2) void train_forward_kernel(const Ar
                 rows_operand<P>(kt, 32 * (WK == 1 ? b : wk), c, lane, x);
                 mma<P>(s[b], x, qb[c]);
             }
+        if (some != ~0ull)
+#pragma unroll
+            for (int b = 0; b < NS; ++b) leave_out(s[b], some, 32 * (WK == 1 ? b : wk), half);
         float top = -INFINITY;
 #pragma unroll
-        for (int b = 0; b < NS; ++b) {
-            const unsigned bits = (unsigned)(some >> (32 * (WK == 1 ? b : wk) + 4 * half));
+        for (int b = 0; b < NS; ++b)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                if (some != ~0ull) s[b][i] = bits >> (8 * (i / 4) + i % 4) & 1 ? s[b][i] : -INFINITY;
-                top = fmaxf(top, s[b][i]);
-            }
-        }
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
         // A scale is positive: the largest score is that of the largest product.
         top = fmaxf(top, other_half(top));
         const float upto = fmaxf(r, ceilf(top * a.c));
@@ -388,21 +388,23 @@ __global__ __launch_bounds__(64 * WQ * WK, 2) void train_forward_kernel(const Ar
 #pragma unroll
         for (int b = 0; b < NS; ++b) {
             const int sub = WK == 1 ? b : wk;
+            float part = 0.f;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 s[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], a.c, -ref));
-                sum += s[b][i];
+                part += s[b][i];
             }
+            sum += part;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                if (a.line) {
-                    const u32x4 z = philox(2 * (4 * t + 2 * sub + c) + half, query, pair, a.site, seed);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) s[b][8 * c + j] = kept16(z, j, a.line) ? s[b][8 * c + j] : 0.f;
-                }
                 float p[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) p[j] = s[b][8 * c + j];
+                if constexpr (DROP) {
+                    const u32x4 z = philox(2 * (4 * t + 2 * sub + c) + half, query, pair, a.site, seed);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) p[j] = kept16(z, j, a.line) ? p[j] : 0.f;
+                }
                 bf16x8 pb[P];
                 split8<P>(p, pb);
 #pragma unroll
@@ -413,6 +415,17 @@ __global__ __launch_bounds__(64 * WQ * WK, 2) void train_forward_kernel(const Ar
                 }
             }
         }
+    };
+    if (t < end) ks.load(a.k, a.ks, e, hk, t * 64, len), vs.load(a.v, a.vs, e, hk, t * 64, len);
+    while (t < end) {
+        __syncthreads();
+        ks.store(kt, some, nullptr);
+        vs.store(vt, some, nullptr);
+        __syncthreads();
+        unsigned long long following;
+        const int n = next(t + 1, following);
+        if (n < end) ks.load(a.k, a.ks, e, hk, n * 64, len), vs.load(a.v, a.vs, e, hk, n * 64, len);
+        work();
         t = n, some = following;
     }
     sum += other_half(sum);
@@ -421,8 +434,8 @@ __global__ __launch_bounds__(64 * WQ * WK, 2) void train_forward_kernel(const Ar
         struct Half {
             float o[32][64], r[64], sum[64];
         };
-        static_assert(sizeof(Half) <= sizeof(Tile<P>));
-        Half *join = reinterpret_cast<Half *>(&kt);
+        static_assert(WQ * sizeof(Half) <= sizeof(tiles));
+        Half *join = reinterpret_cast<Half *>(tiles) + wq;
         __syncthreads();
         if (wk == 1) {
 #pragma unroll
@@ -468,26 +481,45 @@ __global__ __launch_bounds__(64 * WQ * WK, 2) void train_forward_kernel(const Ar
     }
 }
 
-// Joins the splits of a query: sixteen lanes to a row.
-template <int EL>
+// Joins the splits of a query: sixteen lanes to a row's numbers, and W groups of them to its splits.
+template <int EL, int W>
 __global__ __launch_bounds__(256) void train_merge_kernel(const Args a) {
     const long long rows = (long long)a.pairs * a.q_rows;
-    const long long row = (long long)blockIdx.x * 16 + threadIdx.x / 16;
-    if (row >= rows) return;
-    const int pair = (int)(row / a.q_rows), query = (int)(row % a.q_rows), e = pair / a.heads, lane = threadIdx.x & 15;
-    if (query >= length_of(a.q_lengths, e, a.q_rows)) return;
+    const int lane = threadIdx.x & 15, group = threadIdx.x / 16 % W;
+    const long long row = (long long)blockIdx.x * (16 / W) + threadIdx.x / (16 * W);
+    __shared__ float joined[W > 1 ? 16 : 1][16][4];
+    bool some = row < rows;
+    const int pair = some ? (int)(row / a.q_rows) : 0, query = some ? (int)(row % a.q_rows) : 0, e = pair / a.heads;
+    some = some && query < length_of(a.q_lengths, e, a.q_rows);
     const float *m = a.q_part + (long long)a.q_splits * rows * 64;
-    float r = -INFINITY;
-    for (int s = 0; s < a.q_splits; ++s) r = fmaxf(r, m[(s * rows + row) * 2]);
-    const float ref = r == -INFINITY ? 0.f : r;
-    float sum = 0.f;
+    float r = -INFINITY, ref = 0.f, sum = 0.f;
     f32x4 o = {};
-    for (int s = 0; s < a.q_splits; ++s) {
-        const f32x2 x = *reinterpret_cast<const f32x2 *>(m + (s * rows + row) * 2);
-        const float f = __builtin_amdgcn_exp2f(x[0] - ref);
-        sum += x[1] * f;
-        o += *reinterpret_cast<const f32x4 *>(a.q_part + (s * rows + row) * 64 + 4 * lane) * f;
+    if (some) {
+        // Every group takes every split's statistics: the same reference and sum in all.
+        for (int s = lane; s < a.q_splits; s += 16) r = fmaxf(r, m[(s * rows + row) * 2]);
+#pragma unroll
+        for (int i = 8; i; i >>= 1) r = fmaxf(r, __shfl_xor(r, i, 16));
+        ref = r == -INFINITY ? 0.f : r;
+        for (int s = lane; s < a.q_splits; s += 16) {
+            const f32x2 x = *reinterpret_cast<const f32x2 *>(m + (s * rows + row) * 2);
+            sum += x[1] * __builtin_amdgcn_exp2f(x[0] - ref);
+        }
+#pragma unroll
+        for (int i = 8; i; i >>= 1) sum += __shfl_xor(sum, i, 16);
+#pragma unroll 4
+        for (int s = group; s < a.q_splits; s += W) {
+            const float f = __builtin_amdgcn_exp2f(m[(s * rows + row) * 2] - ref);
+            o += *reinterpret_cast<const f32x4 *>(a.q_part + (s * rows + row) * 64 + 4 * lane) * f;
+        }
     }
+    if constexpr (W > 1) {
+        *reinterpret_cast<f32x4 *>(joined[threadIdx.x / 16][lane]) = o;
+        __syncthreads();
+        if (group) return;
+#pragma unroll
+        for (int i = 1; i < W; ++i) o += *reinterpret_cast<const f32x4 *>(joined[threadIdx.x / 16 + i][lane]);
+    }
+    if (!some) return;
     const float f = sum == 0.f ? 0.f : a.w / sum;
     store4<EL>(a.out, at(a.os, e, pair % a.heads, query) + 4 * lane, o * f);
     if (!lane) {
@@ -527,7 +559,7 @@ struct Streamed {
 };
 
 // The gradient of 32 queries a wave: dS^T = K Q^T, V dout^T, then K^T dS, over a split's key tiles.
-template <int EL>
+template <int EL, bool DROP>
 __device__ __forceinline__ void queries_backward(const Args &a, Streamed<parts_of(EL)> &lds, unsigned block) {
     constexpr int P = parts_of(EL);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
@@ -547,7 +579,7 @@ __device__ __forceinline__ void queries_backward(const Args &a, Streamed<parts_o
     own_row<EL>(a.dout, at(a.gs, e, h, query), some_row, lane, gb);
 
     f32x16 o[2] = {};
-    const unsigned long long seed = a.line ? *a.seed : 0;
+    const unsigned long long seed = DROP ? *a.seed : 0;
     const int end = min((split + 1) * a.q_chunk, (int)((len + 63) / 64));
     auto next = [&](int t, unsigned long long &m) {
         for (m = 0; t < end && !(m = attended(a.keep, a.words, e, t, len)); ++t) {}
@@ -576,20 +608,20 @@ __device__ __forceinline__ void queries_backward(const Args &a, Streamed<parts_o
                 rows_operand<P>(lds.y, 32 * b, c, lane, x);
                 mma<P>(dp, x, gb[c]);
             }
-            const unsigned bits = (unsigned)(some >> (32 * b + 4 * half));
+            if (some != ~0ull) leave_out(s, some, 32 * b, half);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 u32x4 z;
-                if (a.line) z = philox(2 * (4 * t + 2 * b + c) + half, query, pair, a.site, seed);
+                if constexpr (DROP) z = philox(2 * (4 * t + 2 * b + c) + half, query, pair, a.site, seed);
                 float ds[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int i = 8 * c + j;
-                    float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, -record[0]));
-                    if (some != ~0ull) p = bits >> (8 * (i / 4) + i % 4) & 1 ? p : 0.f;
-                    float g = dp[i];
-                    if (a.line) g = kept16(z, j, a.line) ? g : 0.f;
-                    ds[j] = p * __builtin_fmaf(g, a.w, -record[2]);
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, -record[0]));
+                    if constexpr (DROP)
+                        ds[j] = p * __builtin_fmaf(kept16(z, j, a.line) ? dp[i] : 0.f, a.w, -record[2]);
+                    else
+                        ds[j] = p * (dp[i] - record[2]);
                 }
                 bf16x8 db[P];
                 split8<P>(ds, db);
@@ -639,7 +671,7 @@ __device__ __forceinline__ unsigned kept_words(unsigned cell, int query, int pai
 
 // The gradients of 32 keys a wave: S = Q K^T, dout V^T, then dout^T P and Q^T dS, over a split's query tiles of every head
 // that shares the keys.
-template <int EL>
+template <int EL, bool DROP>
 __device__ __forceinline__ void keys_backward(const Args &a, Streamed<parts_of(EL)> &lds, unsigned block) {
     constexpr int P = parts_of(EL);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
@@ -657,7 +689,7 @@ __device__ __forceinline__ void keys_backward(const Args &a, Streamed<parts_of(E
     own_row<EL>(a.v, at(a.vs, e, hk, key), in, lane, vb);
 
     f32x16 dk[2] = {}, dv[2] = {};
-    const unsigned long long seed = a.line ? *a.seed : 0;
+    const unsigned long long seed = DROP ? *a.seed : 0;
     // Query tiles that hold a query, of all heads of the group in turn.
     const int q_tiles = (q_len + kTile - 1) / kTile;
     const int end = here[0] | here[1] ? min((split + 1) * a.k_chunk, group * q_tiles) : 0;
@@ -704,7 +736,7 @@ __device__ __forceinline__ void keys_backward(const Args &a, Streamed<parts_of(E
                 mma<P>(dp, x, vb[c]);
             }
             unsigned kept = ~0u;
-            if (a.line)
+            if constexpr (DROP)
                 kept = kept_words(2 * (tile * 8 + 2 * wave), row0 + 32 * b + (lane & 31), e * a.heads + h, a.site, a.line, seed, half) >> (4 * half);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -714,9 +746,13 @@ __device__ __forceinline__ void keys_backward(const Args &a, Streamed<parts_of(E
                     const int i = 8 * c + j, q = 32 * b + 8 * (i / 4) + 4 * half + i % 4;
                     p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, -lds.r[q]));
                     if constexpr (EL == kTrainBF16) p[j] *= lds.inv[q];
-                    const bool z = kept >> (8 * (i / 4) + i % 4) & 1;
-                    ds[j] = p[j] * __builtin_fmaf(a.line && !z ? 0.f : dp[i], a.w, -lds.delta[q]);
-                    if (a.line) p[j] = z ? p[j] : 0.f;
+                    if constexpr (DROP) {
+                        const bool z = kept >> (8 * (i / 4) + i % 4) & 1;
+                        ds[j] = p[j] * __builtin_fmaf(z ? dp[i] : 0.f, a.w, -lds.delta[q]);
+                        p[j] = z ? p[j] : 0.f;
+                    } else {
+                        ds[j] = p[j] * (dp[i] - lds.delta[q]);
+                    }
                 }
                 bf16x8 x[P], pb[P];
                 split8<P>(p, pb);
@@ -756,13 +792,13 @@ __device__ __forceinline__ void keys_backward(const Args &a, Streamed<parts_of(E
     }
 }
 
-template <int EL>
+template <int EL, bool DROP>
 __global__ __launch_bounds__(256, 2) void train_backward_kernel(const Args a) {
     __shared__ Streamed<parts_of(EL)> lds;
     if (blockIdx.x < (unsigned)a.q_blocks)
-        queries_backward<EL>(a, lds, blockIdx.x);
+        queries_backward<EL, DROP>(a, lds, blockIdx.x);
     else
-        keys_backward<EL>(a, lds, blockIdx.x - a.q_blocks);
+        keys_backward<EL, DROP>(a, lds, blockIdx.x - a.q_blocks);
 }
 
 // Sums the splits' parts, in order. Rows of dq, then of dk, then of dv; sixteen lanes to a row.
@@ -849,14 +885,13 @@ __global__ __launch_bounds__(256) void train_dropout_kernel(const DropArgs a) {
 
 struct Plan {
     int q_tiles, q_splits, q_chunk, k_tiles, k_splits, k_chunk;
-    bool few;  // forward: 32 queries to a workgroup
+    int q_unit;  // queries of a workgroup
     size_t record, q_part, k_part;  // bytes
     double blocks;
 };
 
 int splits_of(double length, double target, long long tiles) {
-    const long long most = std::max(1ll, tiles / 4);  // a split walks four tiles at least
-    return (int)std::min<long long>(std::max(1ll, std::llround(length / target)), std::min(most, 256ll));
+    return (int)std::min<long long>(std::max(1ll, std::llround(length / target)), std::min(tiles, 64ll));
 }
 
 Plan plan(const TrainShape &s, int element, bool backward, int compute_units) {
@@ -864,18 +899,18 @@ Plan plan(const TrainShape &s, int element, bool backward, int compute_units) {
     const long long pairs = (long long)s.estimators * s.heads, owners = (long long)s.estimators * s.kv_heads;
     const long long words = (s.rows + 63) / 64, q_words = (s.q_rows + 63) / 64, group = s.heads / s.kv_heads;
     const double slots = 2.0 * compute_units;
-    p.few = !backward && s.q_rows <= 32;
-    p.q_tiles = (int)ceil_div(s.q_rows, p.few ? 32 : 128);
+    p.q_unit = backward || s.q_rows > 64 ? 128 : s.q_rows > 32 ? 64 : 32;
+    p.q_tiles = (int)ceil_div(s.q_rows, p.q_unit);
     p.k_tiles = (int)ceil_div(s.rows, 128);
     if (backward) {
         // A tile of keys costs a unit of queries three products, a tile of queries a unit of keys four. No workgroup walks
         // further than its share of all the work.
         const double all = 3.0 * pairs * p.q_tiles * words + 4.0 * owners * p.k_tiles * group * q_words;
-        const double share = std::max(all / slots, 12.0);
+        const double share = std::max(all / slots, 3.0);
         p.q_splits = splits_of(3.0 * words, share, words);
         p.k_splits = splits_of(4.0 * group * q_words, share, group * q_words);
     } else {
-        p.q_splits = splits_of((double)words, std::max(pairs * p.q_tiles * words / slots, 4.0), words);
+        p.q_splits = splits_of((double)words, std::max(pairs * p.q_tiles * words / slots, 1.0), words);
         p.k_splits = 1;
     }
     p.q_chunk = (int)ceil_div(words, p.q_splits);
@@ -916,15 +951,28 @@ void forward(const TrainInputs &a, const TrainForward &f, const Plan &p, hipStre
     const dim3 grid((unsigned)p.blocks);
     {
         KernelTimer timer(kFamIcl, stream, 256.0 * k.pairs * k.q_rows * k.rows, 0.0);
-        if (p.few)
-            hipLaunchKernelGGL((train_forward_kernel<EL, 1, 2>), grid, dim3(128), 0, stream, k);
+        auto launch = [&]<bool DROP>() {
+            if (p.q_unit == 32)
+                hipLaunchKernelGGL((train_forward_kernel<EL, 1, 2, DROP>), grid, dim3(128), 0, stream, k);
+            else if (p.q_unit == 64)
+                hipLaunchKernelGGL((train_forward_kernel<EL, 2, 2, DROP>), grid, dim3(256), 0, stream, k);
+            else
+                hipLaunchKernelGGL((train_forward_kernel<EL, 4, 1, DROP>), grid, dim3(256), 0, stream, k);
+        };
+        if (k.line)
+            launch.template operator()<true>();
         else
-            hipLaunchKernelGGL((train_forward_kernel<EL, 4, 1>), grid, dim3(256), 0, stream, k);
+            launch.template operator()<false>();
         IRX_HIP(hipGetLastError());
     }
     if (p.q_splits > 1) {
         KernelTimer timer(kFamIclMerge, stream, 0.0, (double)p.q_part);
-        hipLaunchKernelGGL(train_merge_kernel<EL>, dim3(ceil_div((size_t)k.pairs * k.q_rows, 16)), dim3(256), 0, stream, k);
+        // A group of sixteen lanes to two splits or so: one after another they wait for memory each time.
+        const size_t rows = (size_t)k.pairs * k.q_rows;
+        if (p.q_splits > 8)
+            hipLaunchKernelGGL((train_merge_kernel<EL, 16>), dim3((unsigned)rows), dim3(256), 0, stream, k);
+        else
+            hipLaunchKernelGGL((train_merge_kernel<EL, 4>), dim3(ceil_div(rows, 4)), dim3(256), 0, stream, k);
         IRX_HIP(hipGetLastError());
     }
 }
@@ -950,7 +998,11 @@ void backward(const TrainInputs &a, const TrainBackward &b, const Plan &p, hipSt
     const size_t k_blocks = b.dk ? (size_t)a.shape.estimators * a.shape.kv_heads * p.k_tiles * p.k_splits : 0;
     {
         KernelTimer timer(kFamIcl, stream, 640.0 * rows * k.rows, 0.0);
-        hipLaunchKernelGGL(train_backward_kernel<EL>, dim3((unsigned)(k.q_blocks + k_blocks)), dim3(256), 0, stream, k);
+        const dim3 grid((unsigned)(k.q_blocks + k_blocks));
+        if (k.line)
+            hipLaunchKernelGGL((train_backward_kernel<EL, true>), grid, dim3(256), 0, stream, k);
+        else
+            hipLaunchKernelGGL((train_backward_kernel<EL, false>), grid, dim3(256), 0, stream, k);
         IRX_HIP(hipGetLastError());
     }
     if (!b.dq) k.q_splits = 1;
