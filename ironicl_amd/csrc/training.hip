@@ -10,11 +10,17 @@
 // reference comes to it by an exact power of two. (One FP32 logarithm r + log2 s in place of the two
 // would put 2^-24 of itself into every weight of its row: 1e-5 at scores of 300.)
 //
-// Products run on the BF16 matrix cores with FP32 sums. BF16 operands are taken as they are; FP16 ones are
-// held as two BF16 parts (8 + 3 of 11 bits, exact) in three products, FP32 ones as three (8 + 8 + 8 of 24)
-// in six: lo.hi and hi.lo down to 2^-16 of hi.hi, what is left out is below 2^-23 of it (2^-17 with two
-// parts). BF16 has FP32's exponents, so gradients of any size need no scale. The probabilities and dS are
-// rounded to as many parts: BF16's eight bits, 2^-17, 2^-25.
+// Products run on the 16-bit matrix cores with FP32 sums: BF16 and FP16 operands as they are, FP32 ones as
+// pairs of FP16 values, three products (pair8; half the matrix cores' work of six products of three BF16 parts,
+// with which 512 queries over 50,000 keys took 293 us and their gradients 1,019). Pairs keep 2^-23 of a number of
+// [2^-14, 2^15] and 2^-25 of a smaller one, so FP32 operands and weights come to that range by powers of two:
+//   - a lane's own row (of q, or of k and v) by its own;
+//   - a streamed tile's rows by one power each for the tile's keys and its values (or queries and dout), the
+//     largest number's. Rows 2^14 smaller than the largest go in a turn of their own over the same tile, so
+//     that every row keeps 2^-24 of itself at least, whatever stands beside it;
+//   - weights and dS by a lane's power, raised as larger terms come, its sums with it: what is rounded is below
+//     2^-38 of the sum's largest term. FP16 operands' weights and dS, single values, take that too.
+// BF16 has FP32's exponents; weights and dS are rounded to its eight bits and take no power.
 #include "common.hpp"
 
 #include <algorithm>
@@ -38,7 +44,13 @@ constexpr int kTile = 64;   // rows of a streamed tile
 constexpr int kPitch = 72;  // BF16 numbers from one row of a tile to the next: 36 banks, so 16 rows' 16 bytes meet no bank twice
 constexpr float kLn2 = 0.69314718055994530942f;
 
-constexpr int parts_of(int element) { return element == kTrainF32 ? 3 : element == kTrainF16 ? 2 : 1; }
+constexpr int parts_of(int element) { return element == kTrainF32 ? 2 : 1; }
+constexpr bool scaled(int element) { return element == kTrainF32; }   // operands come by powers of two
+constexpr bool ranged(int element) { return element != kTrainBF16; }  // weights and dS do
+template <int EL>
+using V8 = std::conditional_t<EL == kTrainBF16, bf16x8, half8>;
+constexpr int kTop = 15;     // scaled numbers are below 2^15
+constexpr int kSpread = 14;  // rows of a turn: exponents within 14 of the largest
 
 // ---- elements ----
 
@@ -83,36 +95,51 @@ __device__ __forceinline__ unsigned bf16_pair(float a, float b) {
     return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{a, b}), bf16x2));
 }
 
-// Eight numbers as P BF16 parts: each the rounded rest of those before.
-template <int P>
-__device__ __forceinline__ void split8(const float *x, bf16x8 (&out)[P]) {
-    u32x4 w[P];
+// Eight numbers as an operand's parts.
+template <int EL>
+__device__ __forceinline__ void operand8(const float *x, V8<EL> (&out)[parts_of(EL)]) {
+    if constexpr (EL == kTrainF32) {
+        pair8(x, out[0], out[1]);
+    } else {
+        u32x4 w;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        float a = x[2 * i], b = x[2 * i + 1];
-#pragma unroll
-        for (int p = 0; p < P; ++p) {
-            w[p][i] = bf16_pair(a, b);
-            if (p + 1 < P) {
-                a -= __uint_as_float(w[p][i] << 16);
-                b -= __uint_as_float(w[p][i] & 0xffff0000u);
-            }
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (EL == kTrainF16)
+                w[i] = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{x[2 * i], x[2 * i + 1]}), half2v));
+            else
+                w[i] = bf16_pair(x[2 * i], x[2 * i + 1]);
         }
+        out[0] = __builtin_bit_cast(V8<EL>, w);
     }
-#pragma unroll
-    for (int p = 0; p < P; ++p) out[p] = __builtin_bit_cast(bf16x8, w[p]);
 }
 
+// Eight numbers as they lie in memory, FP32 ones times `scale`.
 template <int EL>
-__device__ __forceinline__ void split_raw(const Raw<EL> &r, bf16x8 (&out)[parts_of(EL)]) {
-    if constexpr (EL == kTrainBF16) {
-        out[0] = __builtin_bit_cast(bf16x8, r.w[0]);
-    } else {
+__device__ __forceinline__ void raw_operand(const Raw<EL> &r, float scale, V8<EL> (&out)[parts_of(EL)]) {
+    if constexpr (EL == kTrainF32) {
         float x[8];
         to_floats<EL>(r, x);
-        split8<parts_of(EL)>(x, out);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] *= scale;
+        operand8<EL>(x, out);
+    } else {
+        out[0] = __builtin_bit_cast(V8<EL>, r.w[0]);
     }
 }
+
+// The largest size of eight FP32 numbers.
+__device__ __forceinline__ float largest8(const Raw<kTrainF32> &r) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(__uint_as_float(r.w[i / 4][i % 4])));
+    return m;
+}
+
+// A number's exponent field, held to 16 (2^-111) so that the powers below are normal.
+__device__ __forceinline__ int field_of(float m) { return max(16, (int)(__float_as_uint(m) >> 23 & 255)); }
+// x times scale_of(f) is below 2^15 where x has the exponent field f; 2^down(f) takes it back.
+__device__ __forceinline__ int down(int f) { return f - 126 - kTop; }
+__device__ __forceinline__ float scale_of(int f) { return __uint_as_float((unsigned)(127 - down(f)) << 23); }
 
 // Four numbers rounded to the element type and stored.
 template <int EL>
@@ -149,41 +176,45 @@ __device__ __forceinline__ f32x4 load4(const void *base, long long at) {
 
 // ---- products ----
 
-// acc += A B on parts, the small terms first.
-template <int P>
-__device__ __forceinline__ void mma(f32x16 &acc, const bf16x8 (&a)[P], const bf16x8 (&b)[P]) {
-#pragma unroll
-    for (int order = P - 1; order >= 0; --order)
-#pragma unroll
-        for (int i = 0; i <= order; ++i)
-            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[order - i], b[i], acc, 0, 0, 0);
+// acc += A B, of pairs the small terms first.
+template <int EL>
+__device__ __forceinline__ void mma(f32x16 &acc, const V8<EL> (&a)[parts_of(EL)], const V8<EL> (&b)[parts_of(EL)]) {
+    if constexpr (EL == kTrainF32) {
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], b[0], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[1], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[0], acc, 0, 0, 0);
+    } else if constexpr (EL == kTrainF16) {
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[0], acc, 0, 0, 0);
+    } else {
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[0], acc, 0, 0, 0);
+    }
 }
 
-// A tile in LDS: P planes of 64 rows of 64 BF16 numbers.
-template <int P>
+// A tile in LDS: a plane of 64 rows of 64 16-bit numbers for each part.
+template <int EL>
 struct Tile {
-    alignas(16) __bf16 p[P][kTile * kPitch];
+    alignas(16) unsigned short p[parts_of(EL)][kTile * kPitch];
 };
 
 // The A operand of rows `row0` .. + 31, dims 16 c .. + 15: lane (row l % 32, half h) holds dims 16 c + 8 h .. + 7.
-template <int P>
-__device__ __forceinline__ void rows_operand(const Tile<P> &t, int row0, int c, int lane, bf16x8 (&a)[P]) {
+template <int EL>
+__device__ __forceinline__ void rows_operand(const Tile<EL> &t, int row0, int c, int lane, V8<EL> (&a)[parts_of(EL)]) {
     const int at = (row0 + (lane & 31)) * kPitch + 16 * c + 8 * (lane >> 5);
 #pragma unroll
-    for (int p = 0; p < P; ++p) a[p] = *reinterpret_cast<const bf16x8 *>(&t.p[p][at]);
+    for (int p = 0; p < parts_of(EL); ++p) a[p] = __builtin_bit_cast(V8<EL>, *reinterpret_cast<const u32x4 *>(&t.p[p][at]));
 }
 
 // The A operand of dims 32 d .. + 31 over rows row0 .. + 15, for a B operand whose eight numbers in half h are those of rows
 // 4 h .. + 3 and 8 + 4 h .. + 3: a product's result as it lies in a lane.
-template <int P>
-__device__ __forceinline__ void dims_operand(const Tile<P> &t, int row0, int d, int lane, bf16x8 (&a)[P]) {
+template <int EL>
+__device__ __forceinline__ void dims_operand(const Tile<EL> &t, int row0, int d, int lane, V8<EL> (&a)[parts_of(EL)]) {
     typedef __attribute__((address_space(3))) s16x4 *lds4;
     const int at = (row0 + 4 * (lane >> 5) + (lane & 15) / 4) * kPitch + 32 * d + (lane & 16) + 4 * (lane & 3);
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
+    for (int p = 0; p < parts_of(EL); ++p) {
         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(&t.p[p][at]));
         const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(&t.p[p][at + 8 * kPitch]));
-        a[p] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        a[p] = __builtin_bit_cast(V8<EL>, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     }
 }
 
@@ -267,6 +298,20 @@ __device__ __forceinline__ long long at(const long long *s, int e, int h, int ro
     return e * s[0] + h * s[1] + (long long)row * s[2];
 }
 
+// x 2^by (x > 0), held to FP32's normal numbers: a factor of 0 or of infinity would make NaN of what is left out or 0.
+__device__ __forceinline__ float times_power(float x, int by) {
+    return fminf(fmaxf(__builtin_ldexpf(x, by), 0x1p-126f), 0x1p127f);
+}
+
+// The largest of eight adjacent lanes' values.
+__device__ __forceinline__ float largest_of_8_lanes(float m) {
+    auto step = [&](int moved) { m = fmaxf(m, __int_as_float(moved)); };
+    step(__builtin_amdgcn_mov_dpp(__float_as_int(m), 0xB1, 15, 15, true));   // lane ^ 1
+    step(__builtin_amdgcn_mov_dpp(__float_as_int(m), 0x4E, 15, 15, true));   // lane ^ 2
+    step(__builtin_amdgcn_mov_dpp(__float_as_int(m), 0x141, 15, 15, true));  // lane ^ 7
+    return m;
+}
+
 // A tile's numbers on their way to LDS: NT threads load 64 x 64, eight adjacent ones at a time.
 template <int EL, int NT>
 struct Staged {
@@ -281,25 +326,32 @@ struct Staged {
             r[i] = load8<EL>(base, at(s, e, h, min(row0 + u / 8, rows - 1)) + 8 * (u % 8));
         }
     }
-    // Rows whose bit is not set become zeros, whatever they hold. `factor`: null, or one for each row.
-    __device__ __forceinline__ void store(Tile<parts_of(EL)> &t, unsigned long long some, const float *factor) const {
-        constexpr int P = parts_of(EL);
+    // FP32: rows times what stands for them in `factor`.
+    __device__ __forceinline__ void times(const float (&factor)[N]) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) r[i].w[j / 4][j % 4] = __float_as_uint(__uint_as_float(r[i].w[j / 4][j % 4]) * factor[i]);
+    }
+    // FP32: every row's largest number's exponent field, 0 for zeros.
+    __device__ __forceinline__ void fields(int *to) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int u = threadIdx.x + i * NT;
+            const float m = largest_of_8_lanes(largest8(r[i]));
+            if (u % 8 == 0) to[u / 8] = (int)(__float_as_uint(m) >> 23);
+        }
+    }
+    // Rows whose bit is not set become zeros, whatever they hold.
+    __device__ __forceinline__ void store(Tile<EL> &t, unsigned long long some, float scale) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int u = threadIdx.x + i * NT, row = u / 8;
-            bf16x8 b[P];
-            if (EL != kTrainBF16 && factor) {
-                float x[8];
-                to_floats<EL>(r[i], x);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] *= factor[row];
-                split8<P>(x, b);
-            } else {
-                split_raw<EL>(r[i], b);
-            }
+            V8<EL> b[parts_of(EL)];
+            raw_operand<EL>(r[i], scale, b);
             const bool in = some >> row & 1;
 #pragma unroll
-            for (int p = 0; p < P; ++p) {
+            for (int p = 0; p < parts_of(EL); ++p) {
                 u32x4 w = __builtin_bit_cast(u32x4, b[p]);
                 if (!in) w = u32x4{0, 0, 0, 0};
                 *reinterpret_cast<u32x4 *>(&t.p[p][row * kPitch + 8 * (u % 8)]) = w;
@@ -308,30 +360,83 @@ struct Staged {
     }
 };
 
-// The B operand of a lane's own row: dims 16 c + 8 h .. + 7; zeros where !in.
-template <int EL>
-__device__ __forceinline__ void own_row(const void *base, long long row, bool in, int lane, bf16x8 (&b)[4][parts_of(EL)]) {
+__device__ __forceinline__ int wave_max_int(int v) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        Raw<EL> r{};
-        if (in) r = load8<EL>(base, row + 16 * c + 8 * (lane >> 5));
-        split_raw<EL>(r, b[c]);
-    }
+    for (int i = 32; i; i >>= 1) v = max(v, __shfl_xor(v, i, 64));
+    return v;
 }
+
+// The rows of `todo` that a turn takes, and the exponent fields for x and y: those within 2^14 of the largest x (rows of
+// zeros go with any), and of them those within 2^14 of the largest y. It takes one row at least.
+struct Turn {
+    unsigned long long some;
+    int x, y;
+};
+__device__ __forceinline__ Turn turn_of(unsigned long long todo, const int *fx, const int *fy, int lane) {
+    const bool mine = todo >> lane & 1;
+    const int x = mine ? fx[lane] : 0, y = fy[lane];
+    const int most_x = wave_max_int(x);
+    bool in = mine && (x == 0 || x >= most_x - kSpread);
+    const int most_y = wave_max_int(in ? y : 0);
+    in = in && (y == 0 || y >= most_y - kSpread);
+    return {__ballot(in), __builtin_amdgcn_readfirstlane(max(16, most_x)), __builtin_amdgcn_readfirstlane(max(16, most_y))};
+}
+
+// The B operand of a lane's own row: dims 16 c + 8 h .. + 7; zeros where !in. FP32: returns the row's exponent field.
+template <int EL>
+__device__ __forceinline__ int own_row(const void *base, long long row, bool in, int lane, V8<EL> (&b)[4][parts_of(EL)]) {
+    Raw<EL> r[4] = {};
+    if (in)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) r[c] = load8<EL>(base, row + 16 * c + 8 * (lane >> 5));
+    int field = 127;
+    float scale = 1.f;
+    if constexpr (scaled(EL)) {
+        float m = 0.f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) m = fmaxf(m, largest8(r[c]));
+        field = field_of(fmaxf(m, other_half(m)));
+        scale = scale_of(field);
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) raw_operand<EL>(r[c], scale, b[c]);
+    return field;
+}
+
+// FP32 and FP16: weights or dS of 32 rows brought below 2^15 by a lane's power 2^-k, k raised where they need it, and what a
+// lane has summed under the former one with it. `row`: the power that the streamed rows of the product came by.
+__device__ __forceinline__ void bring(f32x16 &x, float most, int row, int &k, f32x16 (&sums)[2]) {
+    if (__any(__builtin_ldexpf(most, row - k) >= 32768.f)) {
+        // A factor of two to spare, so that a slightly larger term does not raise it again.
+        const int raised = max(k, row + (int)(__float_as_uint(most) >> 23) - 126 - (kTop - 1));
+        const int by = max(k - raised, -300);
+#pragma unroll
+        for (int d = 0; d < 2; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sums[d][i] = __builtin_ldexpf(sums[d][i], by);
+        k = raised;
+    }
+    const int by = row - k;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = __builtin_ldexpf(x[i], by);
+}
+constexpr int kNone = -1000;  // a lane's power before its first term
 
 // ---- forward ----
 
 // 32 WQ queries to a workgroup, 32 to a wave; keys and values pass through LDS in tiles of 64, and where WK is 2 a wave
 // takes 32 of each. S^T = K Q^T leaves a query's scores in one lane (and its other half), in the order in which the next
 // product takes them.
-constexpr int forward_waves(int element, int wq, int wk) {  // of a SIMD: what registers and LDS leave room for
-    return element == kTrainBF16 ? 4 : element == kTrainF16 ? 2 : wq * wk == 4 ? 2 : 1;
+constexpr int forward_waves(int element, int wq, int wk) {  // of a SIMD: what registers leave room for
+    return element == kTrainBF16 ? 4 : element == kTrainF16 ? 3 : wq * wk == 4 ? 2 : 1;
 }
 template <int EL, int WQ, int WK, bool DROP>
 __global__ __launch_bounds__(64 * WQ * WK, forward_waves(EL, WQ, WK)) void train_forward_kernel(const Args a) {
     constexpr int P = parts_of(EL), NT = 64 * WQ * WK, NS = 2 / WK;
-    __shared__ Tile<P> tiles[2];
-    Tile<P> &kt = tiles[0], &vt = tiles[1];
+    constexpr float TOP = ranged(EL) ? kTop - 1 : 0;  // weights are brought below 2^TOP
+    __shared__ Tile<EL> tiles[2];
+    __shared__ int fields[2][scaled(EL) ? kTile : 1];
+    Tile<EL> &kt = tiles[0], &vt = tiles[1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wq = wave % WQ, wk = wave / WQ, half = lane >> 5;
     const unsigned unit = blockIdx.x / (unsigned)a.pairs;
     const int pair = blockIdx.x % (unsigned)a.pairs, tile = unit % (unsigned)a.q_tiles, split = unit / (unsigned)a.q_tiles;
@@ -340,11 +445,14 @@ __global__ __launch_bounds__(64 * WQ * WK, forward_waves(EL, WQ, WK)) void train
     if (tile * 32 * WQ >= q_len) return;
     const int query = tile * 32 * WQ + 32 * wq + (lane & 31);
     const bool mine = query < q_len;
-    bf16x8 qb[4][P];
-    own_row<EL>(a.q, at(a.qs, e, h, query), mine, lane, qb);
+    V8<EL> qb[4][P];
+    const int q_down = down(own_row<EL>(a.q, at(a.qs, e, h, query), mine, lane, qb));
 
+    // o holds sum 2^(x - k) v: with FP32 a value's tile comes by 2^-v_down, its weights by 2^v_down, and k follows the largest
+    // of x + v_down, apart from the sum's reference r. With 16-bit elements k is r - TOP.
     f32x16 o[2] = {};
-    float r = -INFINITY, sum = 0.f;
+    float r = -INFINITY, k = -INFINITY, sum = 0.f;
+    int most_v = 0;
     const unsigned long long seed = DROP ? *a.seed : 0;
     const int end = min((split + 1) * a.q_chunk, (int)((len + 63) / 64));
     auto next = [&](int t, unsigned long long &m) {
@@ -352,17 +460,49 @@ __global__ __launch_bounds__(64 * WQ * WK, forward_waves(EL, WQ, WK)) void train
         return t;
     };
     Staged<EL, NT> ks, vs;
-    unsigned long long some;
-    int t = next(split * a.q_chunk, some);
-    auto work = [&] {
+    unsigned long long todo, following = 0;
+    int t = next(split * a.q_chunk, todo);
+    auto load = [&](int tile) {
+        ks.load(a.k, a.ks, e, hk, tile * 64, len);
+        vs.load(a.v, a.vs, e, hk, tile * 64, len);
+    };
+    if (t < end) load(t);
+    bool fresh = true;
+    while (t < end) {
+        Turn turn = {todo, 0, 0};
+        if (scaled(EL) && fresh) {
+            if constexpr (scaled(EL)) ks.fields(fields[0]), vs.fields(fields[1]);
+        }
+        __syncthreads();
+        if constexpr (scaled(EL)) {
+            turn = turn_of(todo, fields[0], fields[1], lane);
+            // Values 2^40 smaller than the largest so far stay that small: their weights must not leave FP32's range.
+            turn.y = max(turn.y, most_v - 40);
+            most_v = max(most_v, turn.y);
+        }
+        const unsigned long long some = turn.some;
+        const int v_down = scaled(EL) ? down(turn.y) : 0;
+        const float c = scaled(EL) ? times_power(a.c, down(turn.x) + q_down) : a.c;
+        ks.store(kt, some, scaled(EL) ? scale_of(turn.x) : 1.f);
+        vs.store(vt, some, scaled(EL) ? scale_of(turn.y) : 1.f);
+        __syncthreads();
+        todo &= ~some;
+        const int at_tile = t;
+        fresh = !todo;
+        if (fresh) {
+            t = next(t + 1, following);
+            if (t < end) load(t);
+            todo = following;
+        }
+
         f32x16 s[NS] = {};
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int b = 0; b < NS; ++b) {
-                bf16x8 x[P];
-                rows_operand<P>(kt, 32 * (WK == 1 ? b : wk), c, lane, x);
-                mma<P>(s[b], x, qb[c]);
+                V8<EL> x[P];
+                rows_operand<EL>(kt, 32 * (WK == 1 ? b : wk), c, lane, x);
+                mma<EL>(s[b], x, qb[c]);
             }
         if (some != ~0ull)
 #pragma unroll
@@ -373,62 +513,67 @@ __global__ __launch_bounds__(64 * WQ * WK, forward_waves(EL, WQ, WK)) void train
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
         // A scale is positive: the largest score is that of the largest product.
-        top = fmaxf(top, other_half(top));
-        const float upto = fmaxf(r, ceilf(top * a.c));
-        if (__any(upto > r)) {
-            const float f = r == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(r - upto);
-            sum *= f;
+        top = ceilf(fmaxf(top, other_half(top)) * c);
+        const float upto = fmaxf(k, top + (float)v_down - TOP);
+        if (__any(upto > k)) {
+            const float f = k == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(k - upto);
+            if constexpr (!scaled(EL)) sum *= f;
 #pragma unroll
             for (int d = 0; d < 2; ++d)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[d][i] *= f;
-            r = upto;
+            k = upto;
         }
-        const float ref = r == -INFINITY ? 0.f : r;
+        const float from = (float)v_down - (k == -INFINITY ? 0.f : k);
+        float part = 0.f;
 #pragma unroll
         for (int b = 0; b < NS; ++b) {
             const int sub = WK == 1 ? b : wk;
-            float part = 0.f;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], a.c, -ref));
+                s[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], c, from));
                 part += s[b][i];
             }
-            sum += part;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 float p[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) p[j] = s[b][8 * c + j];
                 if constexpr (DROP) {
-                    const u32x4 z = philox(2 * (4 * t + 2 * sub + c) + half, query, pair, a.site, seed);
+                    const u32x4 z = philox(2 * (4 * at_tile + 2 * sub + c) + half, query, pair, a.site, seed);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) p[j] = kept16(z, j, a.line) ? p[j] : 0.f;
                 }
-                bf16x8 pb[P];
-                split8<P>(p, pb);
+                V8<EL> pb[P];
+                operand8<EL>(p, pb);
 #pragma unroll
                 for (int d = 0; d < 2; ++d) {
-                    bf16x8 x[P];
-                    dims_operand<P>(vt, 32 * sub + 16 * c, d, lane, x);
-                    mma<P>(o[d], x, pb);
+                    V8<EL> x[P];
+                    dims_operand<EL>(vt, 32 * sub + 16 * c, d, lane, x);
+                    mma<EL>(o[d], x, pb);
                 }
             }
         }
-    };
-    if (t < end) ks.load(a.k, a.ks, e, hk, t * 64, len), vs.load(a.v, a.vs, e, hk, t * 64, len);
-    while (t < end) {
-        __syncthreads();
-        ks.store(kt, some, nullptr);
-        vs.store(vt, some, nullptr);
-        __syncthreads();
-        unsigned long long following;
-        const int n = next(t + 1, following);
-        if (n < end) ks.load(a.k, a.ks, e, hk, n * 64, len), vs.load(a.v, a.vs, e, hk, n * 64, len);
-        work();
-        t = n, some = following;
+        if constexpr (scaled(EL)) {
+            const float upto = fmaxf(r, top), ref = upto == -INFINITY ? 0.f : upto;
+            sum = sum * (r == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(r - ref)) + part * __builtin_amdgcn_exp2f(-from - ref);
+            r = upto;
+        } else {
+            sum += part;
+        }
     }
     sum += other_half(sum);
+    if constexpr (scaled(EL)) {
+        const int by = sum == 0.f ? 0 : (int)(k - r);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i / 16][i % 16] = __builtin_ldexpf(o[i / 16][i % 16], by);
+    } else if constexpr (TOP != 0) {
+        r = k + TOP, sum = __builtin_ldexpf(sum, (int)-TOP);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i / 16][i % 16] = __builtin_ldexpf(o[i / 16][i % 16], (int)-TOP);
+    } else {
+        r = k;
+    }
     if constexpr (WK == 2) {
         // The second wave's half of the keys joins the first's.
         struct Half {
@@ -552,15 +697,17 @@ __global__ __launch_bounds__(256) void train_record_kernel(const Args a) {
     if (!lane) a.record[row] = record;
 }
 
-template <int P>
+template <int EL>
 struct Streamed {
-    Tile<P> x, y;
+    Tile<EL> x, y;
     alignas(16) float r[kTile], inv[kTile], delta[kTile];
+    float coming[kTile];                        // the next tile's r
+    int fields[2][scaled(EL) ? kTile : 1];  // the next tile's exponents
 };
 
-// The gradient of 32 queries a wave: dS^T = K Q^T, V dout^T, then K^T dS, over a split's key tiles.
+// The gradient of 32 queries a wave: S^T = K Q^T, V dout^T, then K^T dS, over a split's key tiles.
 template <int EL, bool DROP>
-__device__ __forceinline__ void queries_backward(const Args &a, Streamed<parts_of(EL)> &lds, unsigned block) {
+__device__ __forceinline__ void queries_backward(const Args &a, Streamed<EL> &lds, unsigned block) {
     constexpr int P = parts_of(EL);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const unsigned unit = block / (unsigned)a.pairs;
@@ -574,11 +721,12 @@ __device__ __forceinline__ void queries_backward(const Args &a, Streamed<parts_o
     f32x4 record = {INFINITY, 0.f, 0.f, 0.f};
     if (mine) record = a.record[row];
     const bool some_row = record[0] != INFINITY;
-    bf16x8 qb[4][P], gb[4][P];
-    own_row<EL>(a.q, at(a.qs, e, h, query), some_row, lane, qb);
-    own_row<EL>(a.dout, at(a.gs, e, h, query), some_row, lane, gb);
+    V8<EL> qb[4][P], gb[4][P];
+    const int q_down = down(own_row<EL>(a.q, at(a.qs, e, h, query), some_row, lane, qb));
+    const int g_down = down(own_row<EL>(a.dout, at(a.gs, e, h, query), some_row, lane, gb));
 
     f32x16 o[2] = {};
+    int power = kNone;
     const unsigned long long seed = DROP ? *a.seed : 0;
     const int end = min((split + 1) * a.q_chunk, (int)((len + 63) / 64));
     auto next = [&](int t, unsigned long long &m) {
@@ -586,54 +734,79 @@ __device__ __forceinline__ void queries_backward(const Args &a, Streamed<parts_o
         return t;
     };
     Staged<EL, 256> ks, vs;
-    unsigned long long some;
-    int t = next(split * a.q_chunk, some);
-    if (t < end) ks.load(a.k, a.ks, e, hk, t * 64, len), vs.load(a.v, a.vs, e, hk, t * 64, len);
+    unsigned long long todo, following = 0;
+    int t = next(split * a.q_chunk, todo);
+    auto load = [&](int tile) {
+        ks.load(a.k, a.ks, e, hk, tile * 64, len);
+        vs.load(a.v, a.vs, e, hk, tile * 64, len);
+    };
+    if (t < end) load(t);
+    bool fresh = true;
     while (t < end) {
+        Turn turn = {todo, 0, 0};
+        if constexpr (scaled(EL))
+            if (fresh) ks.fields(lds.fields[0]), vs.fields(lds.fields[1]);
         __syncthreads();
-        ks.store(lds.x, some, nullptr);
-        vs.store(lds.y, some, nullptr);
+        if constexpr (scaled(EL)) turn = turn_of(todo, lds.fields[0], lds.fields[1], lane);
+        const unsigned long long some = turn.some;
+        const int k_down = scaled(EL) ? down(turn.x) : 0;
+        const float c = scaled(EL) ? times_power(a.c, k_down + q_down) : a.c;
+        const float w = scaled(EL) ? times_power(a.w, down(turn.y) + g_down) : a.w;
+        ks.store(lds.x, some, scaled(EL) ? scale_of(turn.x) : 1.f);
+        vs.store(lds.y, some, scaled(EL) ? scale_of(turn.y) : 1.f);
         __syncthreads();
-        unsigned long long following;
-        const int n = next(t + 1, following);
-        if (n < end) ks.load(a.k, a.ks, e, hk, n * 64, len), vs.load(a.v, a.vs, e, hk, n * 64, len);
+        todo &= ~some;
+        const int at_tile = t;
+        fresh = !todo;
+        if (fresh) {
+            t = next(t + 1, following);
+            if (t < end) load(t);
+            todo = following;
+        }
 #pragma unroll 1
         for (int b = 0; b < 2; ++b) {
             f32x16 s = {}, dp = {};
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                bf16x8 x[P];
-                rows_operand<P>(lds.x, 32 * b, c, lane, x);
-                mma<P>(s, x, qb[c]);
-                rows_operand<P>(lds.y, 32 * b, c, lane, x);
-                mma<P>(dp, x, gb[c]);
+                V8<EL> x[P];
+                rows_operand<EL>(lds.x, 32 * b, c, lane, x);
+                mma<EL>(s, x, qb[c]);
+                rows_operand<EL>(lds.y, 32 * b, c, lane, x);
+                mma<EL>(dp, x, gb[c]);
             }
             if (some != ~0ull) leave_out(s, some, 32 * b, half);
+            float most = 0.f;
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
+            for (int cc = 0; cc < 2; ++cc) {
                 u32x4 z;
-                if constexpr (DROP) z = philox(2 * (4 * t + 2 * b + c) + half, query, pair, a.site, seed);
-                float ds[8];
+                if constexpr (DROP) z = philox(2 * (4 * at_tile + 2 * b + cc) + half, query, pair, a.site, seed);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const int i = 8 * c + j;
-                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, -record[0]));
-                    if constexpr (DROP)
-                        ds[j] = p * __builtin_fmaf(kept16(z, j, a.line) ? dp[i] : 0.f, a.w, -record[2]);
+                    const int i = 8 * cc + j;
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -record[0]));
+                    if constexpr (DROP || scaled(EL))
+                        s[i] = p * __builtin_fmaf(!DROP || kept16(z, j, a.line) ? dp[i] : 0.f, w, -record[2]);
                     else
-                        ds[j] = p * (dp[i] - record[2]);
+                        s[i] = p * (dp[i] - record[2]);
+                    if constexpr (ranged(EL)) most = fmaxf(most, fabsf(s[i]));
                 }
-                bf16x8 db[P];
-                split8<P>(ds, db);
+            }
+            if constexpr (ranged(EL)) bring(s, fmaxf(most, other_half(most)), k_down, power, o);
+#pragma unroll
+            for (int cc = 0; cc < 2; ++cc) {
+                float ds[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) ds[j] = s[8 * cc + j];
+                V8<EL> db[P];
+                operand8<EL>(ds, db);
 #pragma unroll
                 for (int d = 0; d < 2; ++d) {
-                    bf16x8 x[P];
-                    dims_operand<P>(lds.x, 32 * b + 16 * c, d, lane, x);
-                    mma<P>(o[d], x, db);
+                    V8<EL> x[P];
+                    dims_operand<EL>(lds.x, 32 * b + 16 * cc, d, lane, x);
+                    mma<EL>(o[d], x, db);
                 }
             }
         }
-        t = n, some = following;
     }
     if (!mine) return;
     const float f = a.scale * record[1];
@@ -641,7 +814,9 @@ __device__ __forceinline__ void queries_backward(const Args &a, Streamed<parts_o
     for (int i = 0; i < 8; ++i) {
         const f32x16 &x = o[i / 4];
         const int j = 4 * (i % 4), dim = 32 * (i / 4) + 2 * j + 4 * half;
-        const f32x4 y = {x[j] * f, x[j + 1] * f, x[j + 2] * f, x[j + 3] * f};
+        f32x4 y = {x[j], x[j + 1], x[j + 2], x[j + 3]};
+#pragma unroll
+        for (int n = 0; n < 4; ++n) y[n] = ranged(EL) ? __builtin_ldexpf(y[n] * f, power) : y[n] * f;
         if (a.q_splits > 1)
             *reinterpret_cast<f32x4 *>(a.q_part + ((long long)split * a.pairs * a.q_rows + row) * 64 + dim) = y;
         else
@@ -672,8 +847,9 @@ __device__ __forceinline__ unsigned kept_words(unsigned cell, int query, int pai
 // The gradients of 32 keys a wave: S = Q K^T, dout V^T, then dout^T P and Q^T dS, over a split's query tiles of every head
 // that shares the keys.
 template <int EL, bool DROP>
-__device__ __forceinline__ void keys_backward(const Args &a, Streamed<parts_of(EL)> &lds, unsigned block) {
+__device__ __forceinline__ void keys_backward(const Args &a, Streamed<EL> &lds, unsigned block) {
     constexpr int P = parts_of(EL);
+    typedef Staged<EL, 256> Rows;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int group = a.heads / a.kv_heads, owners = a.pairs / group;
     const unsigned unit = block / (unsigned)owners;
@@ -684,102 +860,136 @@ __device__ __forceinline__ void keys_backward(const Args &a, Streamed<parts_of(E
     const int key = tile * 128 + 32 * wave + (lane & 31);
     const unsigned long long here[2] = {attended(a.keep, a.words, e, 2 * tile, len), attended(a.keep, a.words, e, 2 * tile + 1, len)};
     const bool in = here[wave / 2] >> (32 * (wave & 1) + (lane & 31)) & 1;
-    bf16x8 kb[4][P], vb[4][P];
-    own_row<EL>(a.k, at(a.ks, e, hk, key), in, lane, kb);
-    own_row<EL>(a.v, at(a.vs, e, hk, key), in, lane, vb);
+    V8<EL> kb[4][P], vb[4][P];
+    const int k_down = down(own_row<EL>(a.k, at(a.ks, e, hk, key), in, lane, kb));
+    const int v_down = down(own_row<EL>(a.v, at(a.vs, e, hk, key), in, lane, vb));
 
     f32x16 dk[2] = {}, dv[2] = {};
+    int dk_power = kNone, dv_power = kNone;
     const unsigned long long seed = DROP ? *a.seed : 0;
     // Query tiles that hold a query, of all heads of the group in turn.
     const int q_tiles = (q_len + kTile - 1) / kTile;
     const int end = here[0] | here[1] ? min((split + 1) * a.k_chunk, group * q_tiles) : 0;
     int u = split * a.k_chunk;
-    Staged<EL, 256> qs, gs;
-    f32x4 record = {};
+    Rows qs, gs;
+    float r[Rows::N], inv[Rows::N], delta[Rows::N];
     auto load = [&](int i) {
         const int h = hk * group + i / q_tiles, row0 = i % q_tiles * kTile;
         qs.load(a.q, a.qs, e, h, row0, q_len);
         gs.load(a.dout, a.gs, e, h, row0, q_len);
-        if (threadIdx.x < kTile) {
-            record = f32x4{INFINITY, 0.f, 0.f, 0.f};
-            if (row0 + (int)threadIdx.x < q_len)
-                record = a.record[(long long)(e * a.heads + h) * a.q_rows + row0 + threadIdx.x];
+#pragma unroll
+        for (int n = 0; n < Rows::N; ++n) {
+            const int row = row0 + threadIdx.x / 8 + 32 * n;
+            f32x4 x = {INFINITY, 0.f, 0.f, 0.f};
+            if (row < q_len) x = a.record[(long long)(e * a.heads + h) * a.q_rows + row];
+            r[n] = x[0], inv[n] = x[1], delta[n] = x[2];
         }
     };
     if (u < end) load(u);
-    for (; u < end; ++u) {
+    unsigned long long todo = 0;
+    while (u < end) {
         const int h = hk * group + u / q_tiles, row0 = u % q_tiles * kTile;
-        __syncthreads();
-        if (threadIdx.x < kTile) {
-            lds.r[threadIdx.x] = record[0];
-            lds.inv[threadIdx.x] = record[1];
-            lds.delta[threadIdx.x] = EL == kTrainBF16 ? record[2] : record[2] * record[1];
+        const bool fresh = !todo;
+        if (fresh) {
+            // 1 / s goes with FP32's dout, whose parts are made here; 16-bit elements are not touched, their weights take it.
+            if constexpr (scaled(EL)) {
+                gs.times(inv);
+                qs.fields(lds.fields[0]), gs.fields(lds.fields[1]);
+            }
+            if (threadIdx.x % 8 == 0)
+#pragma unroll
+                for (int n = 0; n < Rows::N; ++n) lds.coming[threadIdx.x / 8 + 32 * n] = r[n];
         }
         __syncthreads();
-        {
-            unsigned long long some = __ballot(lds.r[lane] != INFINITY);
-            qs.store(lds.x, some, nullptr);
-            // 1 / s goes with dout where its parts are made; BF16's are not touched, and the weights take it.
-            gs.store(lds.y, some, EL == kTrainBF16 ? nullptr : lds.inv);
-        }
+        if (fresh) todo = __ballot(lds.coming[lane] != INFINITY);
+        Turn turn = {todo, 0, 0};
+        if constexpr (scaled(EL)) turn = turn_of(todo, lds.fields[0], lds.fields[1], lane);
+        const unsigned long long some = turn.some;
+        const int q_down = scaled(EL) ? down(turn.x) : 0, g_down = scaled(EL) ? down(turn.y) : 0;
+        const float c = scaled(EL) ? times_power(a.c, q_down + k_down) : a.c;
+        const float w = scaled(EL) ? times_power(a.w, g_down + v_down) : a.w;
+        qs.store(lds.x, some, scaled(EL) ? scale_of(turn.x) : 1.f);
+        gs.store(lds.y, some, scaled(EL) ? scale_of(turn.y) : 1.f);
+        if (threadIdx.x % 8 == 0)
+#pragma unroll
+            for (int n = 0; n < Rows::N; ++n) {
+                const int row = threadIdx.x / 8 + 32 * n;
+                lds.r[row] = some >> row & 1 ? r[n] : INFINITY;
+                lds.inv[row] = inv[n];
+                lds.delta[row] = scaled(EL) ? delta[n] * inv[n] : delta[n];
+            }
         __syncthreads();
-        if (u + 1 < end) load(u + 1);
+        todo &= ~some;
+        if (!todo) {
+            ++u;
+            if (u < end) load(u);
+        }
 #pragma unroll 1
         for (int b = 0; b < 2; ++b) {
             f32x16 s = {}, dp = {};
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                bf16x8 x[P];
-                rows_operand<P>(lds.x, 32 * b, c, lane, x);
-                mma<P>(s, x, kb[c]);
-                rows_operand<P>(lds.y, 32 * b, c, lane, x);
-                mma<P>(dp, x, vb[c]);
+            for (int n = 0; n < 4; ++n) {
+                V8<EL> x[P];
+                rows_operand<EL>(lds.x, 32 * b, n, lane, x);
+                mma<EL>(s, x, kb[n]);
+                rows_operand<EL>(lds.y, 32 * b, n, lane, x);
+                mma<EL>(dp, x, vb[n]);
             }
             unsigned kept = ~0u;
             if constexpr (DROP)
                 kept = kept_words(2 * (tile * 8 + 2 * wave), row0 + 32 * b + (lane & 31), e * a.heads + h, a.site, a.line, seed, half) >> (4 * half);
+            float most_p = 0.f, most_ds = 0.f;
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
+            for (int i = 0; i < 16; ++i) {
+                const int q = 32 * b + 8 * (i / 4) + 4 * half + i % 4;
+                float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -lds.r[q]));
+                if constexpr (!scaled(EL)) p *= lds.inv[q];
+                const bool z = !DROP || (kept >> (8 * (i / 4) + i % 4) & 1);
+                if constexpr (DROP || scaled(EL))
+                    dp[i] = p * __builtin_fmaf(z ? dp[i] : 0.f, w, -lds.delta[q]);
+                else
+                    dp[i] = p * (dp[i] - lds.delta[q]);
+                s[i] = z ? p : 0.f;
+                if constexpr (ranged(EL)) most_p = fmaxf(most_p, s[i]), most_ds = fmaxf(most_ds, fabsf(dp[i]));
+            }
+            if constexpr (ranged(EL)) {
+                bring(s, fmaxf(most_p, other_half(most_p)), g_down, dv_power, dv);
+                bring(dp, fmaxf(most_ds, other_half(most_ds)), q_down, dk_power, dk);
+            }
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
                 float p[8], ds[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int i = 8 * c + j, q = 32 * b + 8 * (i / 4) + 4 * half + i % 4;
-                    p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, -lds.r[q]));
-                    if constexpr (EL == kTrainBF16) p[j] *= lds.inv[q];
-                    if constexpr (DROP) {
-                        const bool z = kept >> (8 * (i / 4) + i % 4) & 1;
-                        ds[j] = p[j] * __builtin_fmaf(z ? dp[i] : 0.f, a.w, -lds.delta[q]);
-                        p[j] = z ? p[j] : 0.f;
-                    } else {
-                        ds[j] = p[j] * (dp[i] - lds.delta[q]);
-                    }
-                }
-                bf16x8 x[P], pb[P];
-                split8<P>(p, pb);
+                for (int j = 0; j < 8; ++j) p[j] = s[8 * n + j], ds[j] = dp[8 * n + j];
+                V8<EL> x[P], pb[P];
+                operand8<EL>(p, pb);
 #pragma unroll
                 for (int d = 0; d < 2; ++d) {
-                    dims_operand<P>(lds.y, 32 * b + 16 * c, d, lane, x);
-                    mma<P>(dv[d], x, pb);
+                    dims_operand<EL>(lds.y, 32 * b + 16 * n, d, lane, x);
+                    mma<EL>(dv[d], x, pb);
                 }
-                split8<P>(ds, pb);
+                operand8<EL>(ds, pb);
 #pragma unroll
                 for (int d = 0; d < 2; ++d) {
-                    dims_operand<P>(lds.x, 32 * b + 16 * c, d, lane, x);
-                    mma<P>(dk[d], x, pb);
+                    dims_operand<EL>(lds.x, 32 * b + 16 * n, d, lane, x);
+                    mma<EL>(dk[d], x, pb);
                 }
             }
         }
     }
     if (key >= len) return;
     // A key that is not attended to has no gradient, whatever its lane summed.
-    const float fk = in ? a.scale : 0.f, fv = in ? a.w : 0.f;
     const long long row = (long long)owner * a.rows + key, plane = (long long)owners * a.rows * 64;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const f32x16 &x = dk[i / 4], &y = dv[i / 4];
         const int j = 4 * (i % 4), dim = 32 * (i / 4) + 2 * j + 4 * half;
-        f32x4 gk = {x[j] * fk, x[j + 1] * fk, x[j + 2] * fk, x[j + 3] * fk};
-        f32x4 gv = {y[j] * fv, y[j + 1] * fv, y[j + 2] * fv, y[j + 3] * fv};
+        f32x4 gk = {x[j], x[j + 1], x[j + 2], x[j + 3]}, gv = {y[j], y[j + 1], y[j + 2], y[j + 3]};
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            gk[n] = ranged(EL) ? __builtin_ldexpf(gk[n] * a.scale, dk_power) : gk[n] * a.scale;
+            gv[n] = ranged(EL) ? __builtin_ldexpf(gv[n] * a.w, dv_power) : gv[n] * a.w;
+        }
         if (!in) gk = gv = f32x4{0.f, 0.f, 0.f, 0.f};
         if (a.k_splits > 1) {
             float *part = a.k_part + 2 * split * plane + row * 64 + dim;
@@ -794,7 +1004,7 @@ __device__ __forceinline__ void keys_backward(const Args &a, Streamed<parts_of(E
 
 template <int EL, bool DROP>
 __global__ __launch_bounds__(256, 2) void train_backward_kernel(const Args a) {
-    __shared__ Streamed<parts_of(EL)> lds;
+    __shared__ Streamed<EL> lds;
     if (blockIdx.x < (unsigned)a.q_blocks)
         queries_backward<EL, DROP>(a, lds, blockIdx.x);
     else

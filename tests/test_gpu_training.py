@@ -2,18 +2,24 @@
 within bounds worked out beforehand.
 
 Bounds, relative to the sums of magnitudes that the oracle takes beside each result. A score is a sum of 64 products. FP32
-operands are three BF16 parts, exact, whose products below 2^-8 2^-16 twice are left out: 2^-23; FP16 ones are two, exact,
-without the product of the two lower: 2^-16; BF16 ones are whole. Their FP32 sums are off by 2^-18 at most (24 additions of
-sums inside the matrix cores), the scale by less. So with A the largest sum of |scale q k| the score is off by ds <= (2^-17,
-2^-15, 2^-17) A for (FP32, FP16, BF16), and a weight by 2 ds, relative. FP32 sums over N rows (16 in one addition) are off by
-N 2^-27, weights and dS by their rounding to parts, rp = (2^-22, 2^-15, 2^-8: half a step of 24, 16 and 8 bits, and for the
-two lower parts' product 2^-16), an exponential by 2^-22. An output's own rounding is half a step, h = (2^-24, 2^-11, 2^-8).
+operands are pairs of FP16 values: a half step of a half step, 2^-22, each, and the product of the two lower, 2^-22, left
+out; 16-bit operands are whole. Their FP32 sums are off by 2^-18 at most (24 additions of sums inside the matrix cores), the
+scale by less. So with A the largest sum of |scale q k| the score is off by ds <= 2^-17 A, and a weight by 2 ds, relative.
+FP32 sums over N rows (16 in one addition) are off by N 2^-27, weights and dS by their rounding, with the left-out product
+and the other operand's: rp = (2^-20, 2^-11, 2^-8: half a step of 16-bit types) for (FP32, FP16, BF16), an exponential by
+2^-22. An output's own rounding is half a step, h = (2^-24, 2^-11, 2^-8).
 
   out:  out_abs (2 ds + rp + N 2^-26 + 2^-20) + h |out|
-  dv:   dv_abs (2 ds + rp + e + Q 2^-26 + 2^-20) + h |dv|, e = 2^-22, 2^-15, 0: dout's parts
+  dv:   dv_abs (2 ds + rp + Q 2^-26 + 2^-20) + h |dv|
   dS:   its dP is a product like a score's, 2^-18 + rp of its magnitude; its delta is off by what out is, and by 2^-20 of
         its own magnitude: dS_abs (2 ds + rp + 2^-17 + [out's bound and h])
   dq:   dq_abs ([dS's] + rp + N 2^-26 + 2^-20) + h |dq|; dk the same with Q.
+
+FP16 values below 2^-14 are off by 2^-25. FP32's and FP16's weights (and dS) come by a power with which the largest of them
+times its tile's power is 2^13 at least, and FP32's rows by one with which the largest number of the tile's turn is 2^14 at
+least, its other rows within 2^14 of it: every term may miss 2^-37 (2^-25 2^15 / 2^13 / 2^14) of the largest factor times
+its turn's largest number, which is at most 2^14 that row's own, and at most the largest of all. A row's own small numbers
+miss 2^-25 / 2^14 of the turn's largest: as much again. And values 2^40 below the largest of their context keep 2^-79 of it.
 
 FP16 results below its normal numbers round by 2^-25. A key's sums take every head of its group: Q stands for all of them."""
 
@@ -27,9 +33,8 @@ from ironicl_amd import hip, hipmem, training
 
 pytestmark = pytest.mark.gpu
 HALF = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
-PARTS = {"f32": 2.0 ** -22, "f16": 2.0 ** -15, "bf16": 2.0 ** -8}
-SCORE = {"f32": 2.0 ** -17, "f16": 2.0 ** -15, "bf16": 2.0 ** -17}
-OPERAND = {"f32": 2.0 ** -22, "f16": 2.0 ** -15, "bf16": 0.0}
+PARTS = {"f32": 2.0 ** -20, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+SCORE = 2.0 ** -17
 # Weights below 2^-126 are taken as 0, and parts of products' operands below that: a result of 2^15 terms with operands up to
 # 2^11 misses 2^-126 2^15 2^11 at most.
 TINY = {"f32": 2.0 ** -100, "f16": 2.0 ** -25, "bf16": 2.0 ** -100}
@@ -156,10 +161,11 @@ class Case:
         out, lse, stats, dq, dk, dv = got
         n, group = self.shape[4], self.shape[1] // self.shape[2]
         m = self.shape[3] * group
-        ds = SCORE[el] * want.magnitude.max(initial=0.0)
+        ds = SCORE * want.magnitude.max(initial=0.0)
         rows = want.inside[:, None, :, None] & np.ones(out.shape, bool)
         held = want.held[:, None, :, None] & np.ones(dk.shape, bool)
-        within(out, want.out, want.out_abs * (2 * ds + PARTS[el] + n * 2.0 ** -26 + 2.0 ** -20), rows, el, "out")
+        within(out, want.out, want.out_abs * (2 * ds + PARTS[el] + n * 2.0 ** -26 + 2.0 ** -20)
+               + floor(want.out_term, n, el) + n * 2.0 ** -79 * np.abs(self.v.values[np.isfinite(self.v.values)]).max(), rows, el, "out")
         empty = np.isneginf(want.lse)
         inside = want.inside[:, None, :] & np.ones(lse.shape, bool)
         assert np.array_equal(np.isneginf(lse) & inside, empty & inside), "queries that attend to nothing"
@@ -176,10 +182,10 @@ class Case:
         forward = 2 * ds + PARTS[el] + n * 2.0 ** -26 + 2.0 ** -20
         score = 2 * ds + PARTS[el] + 2.0 ** -17 + forward + HALF[el] + 2.0 ** -20
         if queries:
-            within(dq, want.dq, want.dq_abs * (score + PARTS[el] + n * 2.0 ** -26 + 2.0 ** -20), rows, el, "dq")
+            within(dq, want.dq, want.dq_abs * (score + PARTS[el] + n * 2.0 ** -26 + 2.0 ** -20) + floor(want.dq_term, n, el), rows, el, "dq")
         if keys:
-            within(dk, want.dk, want.dk_abs * (score + PARTS[el] + m * 2.0 ** -26 + 2.0 ** -20), held, el, "dk")
-            within(dv, want.dv, want.dv_abs * (2 * ds + PARTS[el] + OPERAND[el] + m * 2.0 ** -26 + 2.0 ** -20), held, el, "dv")
+            within(dk, want.dk, want.dk_abs * (score + PARTS[el] + m * 2.0 ** -26 + 2.0 ** -20) + floor(want.dk_term, m, el), held, el, "dk")
+            within(dv, want.dv, want.dv_abs * (2 * ds + PARTS[el] + m * 2.0 ** -26 + 2.0 ** -20) + floor(want.dv_term, m, el), held, el, "dv")
             masked = held & ~want.attended[:, None, :, None]
             assert np.all(dk[masked] == 0) and np.all(dv[masked] == 0), "gradients of rows that are not attended"
 
@@ -192,6 +198,11 @@ def within(got, want, bound, written, element, name):
     off = np.abs(got - want)[bad]
     where = np.argwhere(bad)[:4].tolist()
     assert not bad.any(), f"{name}: {bad.sum()} of {bad.size} past the bound, by {np.max(off - bound[bad]):.3e}, at {where}"
+
+
+def floor(term, count, element):
+    """What `count` terms may miss: see above."""
+    return 0.0 if element == "bf16" else 2 * count * 2.0 ** -37 * np.minimum(term[0] * 2.0 ** 14, term[1])
 
 
 def random_keep(e, n, seed):
@@ -275,12 +286,12 @@ def test_large_scores(device, element, size):
     # log2(e) scale is rounded to 2^-25, and its product with a score to 2^-24 of itself.
     ds = 2.0 ** -23 * want.magnitude.max()
     n = 300
-    for name, have, exact, size_of in (("out", got[0], want.out, want.out_abs), ("dv", got[5], want.dv, want.dv_abs)):
-        within(have, exact, size_of * (4 * ds + 2 * PARTS[element] + OPERAND[element] + n * 2.0 ** -26 + 2.0 ** -20),
-               np.ones(have.shape, bool), element, name)
     rest = 6 * ds + 4 * PARTS[element] + HALF[element] + n * 2.0 ** -25 + 2.0 ** -16
-    within(got[3], want.dq, want.dq_abs * rest, np.ones(got[3].shape, bool), element, "dq")
-    within(got[4], want.dk, want.dk_abs * rest, np.ones(got[4].shape, bool), element, "dk")
+    weights = 4 * ds + 2 * PARTS[element] + n * 2.0 ** -26 + 2.0 ** -20
+    for name, have, exact, bound, term, count in (
+            ("out", got[0], want.out, want.out_abs * weights, want.out_term, n), ("dq", got[3], want.dq, want.dq_abs * rest, want.dq_term, n),
+            ("dk", got[4], want.dk, want.dk_abs * rest, want.dk_term, 40), ("dv", got[5], want.dv, want.dv_abs * weights, want.dv_term, 40)):
+        within(have, exact, bound + floor(term, count, element), np.ones(have.shape, bool), element, name)
 
 
 @pytest.mark.parametrize("exponent", [-90, -40, 40, 90])
@@ -298,6 +309,39 @@ def test_fp32_gradients_of_any_size(device, exponent):
             assert np.all(np.abs(x * 2.0 ** exponent - y) <= size * 2.0 ** (exponent - 18) + 130 * 8 * 2.0 ** -126)
         else:
             np.testing.assert_array_equal(x * 2.0 ** exponent, y)
+
+
+def spread(shape, seed, low, high):
+    """Normal numbers, every row times a power of two of its own."""
+    x = normal(shape, seed)
+    return x * 2.0 ** np.random.default_rng(seed + 99).integers(low, high + 1, shape[:3])[..., None]
+
+
+@pytest.mark.parametrize("element", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("which", ["values", "gradients", "scores", "all", "zeros", "channel"])
+def test_rows_of_very_different_sizes(device, which, element):
+    """Rows side by side whose sizes span up to 60 binades (FP16's own range for FP16), rows of zeros, and one channel that
+    outweighs the others: every result is within the same bounds of its own terms' sizes."""
+    e, h, g, m, n = 2, 2, 1, 90, 300
+    wide = (-30, 30) if element != "f16" else (-6, 6)
+    q, k, v, dout = normal((e, h, m, 64), 1), normal((e, g, n, 64), 2), normal((e, g, n, 64), 3), normal((e, h, m, 64), 4)
+    if which in ("values", "all"):
+        v = spread(v.shape, 5, *wide)
+    if which in ("gradients", "all"):
+        dout = spread(dout.shape, 6, *wide)
+    if which in ("scores", "all"):
+        q, k = spread(q.shape, 7, wide[0] // 2, 1), spread(k.shape, 8, wide[0] // 2, 1)
+    if which == "zeros":
+        for x in (q, k, v, dout):
+            x[:, :, ::3] = 0.0
+        k[:, :, 64:128], v[:, :, 64:128], v[1], dout[:, :, 64:] = 0.0, 0.0, 0.0, 0.0
+    if which == "channel":
+        k[..., 5] *= 50.0
+        v[..., 9] *= 300.0
+        dout[..., 11] *= 1000.0
+    for dropped in (0, 9000):
+        case = Case(device, e, h, g, m, n, element, "tokens", dropped=dropped, q=q, k=k, v=v, dout=dout, keep=random_keep(e, n, 3))
+        case.check(case.run())
 
 
 @pytest.mark.parametrize("element", ["f32", "bf16"])

@@ -51,6 +51,12 @@ def bits(keep):
     return np.packbits(padded, axis=-1, bitorder="little").view(np.uint64)[..., 0]
 
 
+def terms(factor, rows):
+    """[2, results, 1] of factors [results, terms] and rows [terms, 64]."""
+    largest = np.abs(rows).max(-1)
+    return np.stack(((factor * largest).max(-1), factor.max(-1) * largest.max()))[..., None]
+
+
 class Attention:
     """float64 results and, for error bounds, sums of magnitudes of every output. Inputs [E, H, Q, 64] and [E, G, N, 64]."""
 
@@ -64,6 +70,10 @@ class Attention:
         self.magnitude, self.out_abs = np.zeros((e, h, m)), np.zeros(q.shape)
         self.dq, self.dq_abs = np.zeros(q.shape), np.zeros(q.shape)
         self.dk, self.dv, self.dk_abs, self.dv_abs = (np.zeros(k.shape) for _ in range(4))
+        # The largest |factor| times its row's largest number among a result's terms, and the largest factor times the largest
+        # number of all rows.
+        self.out_term, self.dq_term = np.zeros((2, e, h, m, 1)), np.zeros((2, e, h, m, 1))
+        self.dk_term, self.dv_term = np.zeros((2, e, g, n, 1)), np.zeros((2, e, g, n, 1))
         self.inside = np.arange(m) < (np.full(e, m) if q_lengths is None else np.minimum(q_lengths, m))[:, None]
         self.held = np.arange(n) < (np.full(e, n) if lengths is None else np.minimum(lengths, n))[:, None]
         self.attended = self.held if keep is None else self.held & keep
@@ -87,6 +97,7 @@ class Attention:
                 self.magnitude[i, j, queries] = size.max(-1)
                 self.out[i, j, queries] = (p * z) @ vv
                 self.out_abs[i, j, queries] = (p * z) @ np.abs(vv)
+                self.out_term[:, i, j, queries] = terms(p * w, vv)
                 if dout is None:
                     continue
                 d = dout[i, j, queries].astype(np.float64)
@@ -97,6 +108,9 @@ class Attention:
                 self.dq[i, j, queries] = ds @ kk * scale
                 self.dq_abs[i, j, queries] = ds_abs @ np.abs(kk) * scale
                 self.dk[i, j // (h // g), rows] += ds.T @ qq * scale
+                self.dq_term[:, i, j, queries] = terms(ds_abs, kk) * scale
+                for into, factor, of in ((self.dk_term, ds_abs * scale, qq), (self.dv_term, p * w, d)):
+                    into[:, i, j // (h // g), rows] = np.maximum(into[:, i, j // (h // g), rows], terms(factor.T, of))
                 self.dk_abs[i, j // (h // g), rows] += ds_abs.T @ np.abs(qq) * scale
                 self.dv[i, j // (h // g), rows] += (p * z).T @ d
                 self.dv_abs[i, j // (h // g), rows] += (p * z).T @ np.abs(d)
