@@ -41,7 +41,6 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kTile = 64;   // rows of a streamed tile
-constexpr int kPitch = 72;  // BF16 numbers from one row of a tile to the next: 36 banks, so 16 rows' 16 bytes meet no bank twice
 constexpr float kLn2 = 0.69314718055994530942f;
 
 constexpr int parts_of(int element) { return element == kTrainF32 ? 2 : 1; }
@@ -93,6 +92,14 @@ __device__ __forceinline__ void to_floats(const Raw<EL> &r, float *x) {
 // Two numbers rounded to BF16 (nearest, ties to even), the first in the lower half.
 __device__ __forceinline__ unsigned bf16_pair(float a, float b) {
     return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{a, b}), bf16x2));
+}
+
+// A number as three BF16 parts, each the rounded rest of those before: 24 bits.
+__device__ __forceinline__ u32x2 bf16_parts(float x) {
+    const unsigned a = bf16_pair(x, 0.f);
+    const float y = x - __uint_as_float(a << 16);
+    const unsigned b = bf16_pair(y, 0.f);
+    return {a | b << 16, bf16_pair(y - __uint_as_float(b << 16), 0.f)};
 }
 
 // Eight numbers as an operand's parts.
@@ -190,16 +197,31 @@ __device__ __forceinline__ void mma(f32x16 &acc, const V8<EL> (&a)[parts_of(EL)]
     }
 }
 
-// A tile in LDS: a plane of 64 rows of 64 16-bit numbers for each part.
+// A tile in LDS: for each part a plane of 64 rows of 64 16-bit numbers, so that loads can go straight there. The 64 banks hold
+// two rows; number d of row r lies in the row's 16 bytes (d / 8) ^ swizzle(r). Sixteen rows' 16 bytes of the same dims, as a
+// rows operand takes them at once, meet no bank twice, and nor do four rows' 64 bytes, as a dims operand does.
 template <int EL>
 struct Tile {
-    alignas(16) unsigned short p[parts_of(EL)][kTile * kPitch];
+    alignas(16) unsigned short p[parts_of(EL)][kTile * 64];
+};
+__device__ __forceinline__ int swizzle(int row) { return (row & 2) * 2 | (row >> 2 & 3); }
+__device__ __forceinline__ int swizzled(int row, int chunk) { return row * 64 + 8 * (chunk ^ swizzle(row)); }
+
+// Where a lane's operands of row 0 and dim 0 begin; a row is 64 on, dims 16 c (of rows) and 32 d (of dims) are exclusive ors.
+struct Lanes {
+    int rows, dims, dims8;  // dims8: eight rows on
+    __device__ __forceinline__ explicit Lanes(int lane) {
+        const int row = 4 * (lane >> 5) + (lane & 15) / 4, chunk = (lane & 16) / 8 + (lane & 3) / 2;
+        rows = swizzled(lane & 31, lane >> 5);
+        dims = swizzled(row, chunk) + 4 * (lane & 1);
+        dims8 = swizzled(row + 8, chunk) + 4 * (lane & 1);
+    }
 };
 
 // The A operand of rows `row0` .. + 31, dims 16 c .. + 15: lane (row l % 32, half h) holds dims 16 c + 8 h .. + 7.
 template <int EL>
-__device__ __forceinline__ void rows_operand(const Tile<EL> &t, int row0, int c, int lane, V8<EL> (&a)[parts_of(EL)]) {
-    const int at = (row0 + (lane & 31)) * kPitch + 16 * c + 8 * (lane >> 5);
+__device__ __forceinline__ void rows_operand(const Tile<EL> &t, int row0, int c, const Lanes &l, V8<EL> (&a)[parts_of(EL)]) {
+    const int at = row0 * 64 + (l.rows ^ 16 * c);
 #pragma unroll
     for (int p = 0; p < parts_of(EL); ++p) a[p] = __builtin_bit_cast(V8<EL>, *reinterpret_cast<const u32x4 *>(&t.p[p][at]));
 }
@@ -207,13 +229,13 @@ __device__ __forceinline__ void rows_operand(const Tile<EL> &t, int row0, int c,
 // The A operand of dims 32 d .. + 31 over rows row0 .. + 15, for a B operand whose eight numbers in half h are those of rows
 // 4 h .. + 3 and 8 + 4 h .. + 3: a product's result as it lies in a lane.
 template <int EL>
-__device__ __forceinline__ void dims_operand(const Tile<EL> &t, int row0, int d, int lane, V8<EL> (&a)[parts_of(EL)]) {
+__device__ __forceinline__ void dims_operand(const Tile<EL> &t, int row0, int d, const Lanes &l, V8<EL> (&a)[parts_of(EL)]) {
     typedef __attribute__((address_space(3))) s16x4 *lds4;
-    const int at = (row0 + 4 * (lane >> 5) + (lane & 15) / 4) * kPitch + 32 * d + (lane & 16) + 4 * (lane & 3);
+    const int at = row0 * 64 + (l.dims ^ 32 * d), at8 = row0 * 64 + (l.dims8 ^ 32 * d);
 #pragma unroll
     for (int p = 0; p < parts_of(EL); ++p) {
         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(&t.p[p][at]));
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(&t.p[p][at + 8 * kPitch]));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(&t.p[p][at8]));
         a[p] = __builtin_bit_cast(V8<EL>, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     }
 }
@@ -312,7 +334,29 @@ __device__ __forceinline__ float largest_of_8_lanes(float m) {
     return m;
 }
 
-// A tile's numbers on their way to LDS: NT threads load 64 x 64, eight adjacent ones at a time.
+// 16-bit elements: a tile of rows row0 .. + 63 straight to LDS, a wave's instruction to eight rows. Rows past `rows` are read
+// from the last.
+template <int EL, int NT>
+__device__ __forceinline__ void load_tile(Tile<EL> &t, const void *base, const long long *s, int e, int h, int row0, int rows) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+    for (int i = 0; i < 512 / NT; ++i) {
+        const int first = 8 * (wave + i * (NT / 64)), row = first + lane / 8;
+        const unsigned short *from = static_cast<const unsigned short *>(base) + at(s, e, h, min(row0 + row, rows - 1)) + 8 * ((lane & 7) ^ swizzle(row));
+        __builtin_amdgcn_global_load_lds(from, (__attribute__((address_space(3))) void *)&t.p[0][first * 64], 16, 0, 0);
+    }
+}
+// Rows whose bit is not set become zeros, whatever they hold.
+template <int EL, int NT>
+__device__ __forceinline__ void clear_rows(Tile<EL> &t, unsigned long long some) {
+#pragma unroll
+    for (int i = 0; i < 512 / NT; ++i) {
+        const int u = threadIdx.x + i * NT;
+        if (!(some >> u / 8 & 1)) *reinterpret_cast<u32x4 *>(&t.p[0][8 * u]) = u32x4{0, 0, 0, 0};
+    }
+}
+
+// FP32: a tile's numbers on their way to LDS. NT threads load 64 x 64, eight adjacent ones at a time.
 template <int EL, int NT>
 struct Staged {
     static constexpr int N = 512 / NT;
@@ -354,7 +398,7 @@ struct Staged {
             for (int p = 0; p < parts_of(EL); ++p) {
                 u32x4 w = __builtin_bit_cast(u32x4, b[p]);
                 if (!in) w = u32x4{0, 0, 0, 0};
-                *reinterpret_cast<u32x4 *>(&t.p[p][row * kPitch + 8 * (u % 8)]) = w;
+                *reinterpret_cast<u32x4 *>(&t.p[p][swizzled(row, u % 8)]) = w;
             }
         }
     }
@@ -428,15 +472,14 @@ constexpr int kNone = -1000;  // a lane's power before its first term
 // takes 32 of each. S^T = K Q^T leaves a query's scores in one lane (and its other half), in the order in which the next
 // product takes them.
 constexpr int forward_waves(int element, int wq, int wk) {  // of a SIMD: what registers leave room for
-    return element == kTrainBF16 ? 4 : element == kTrainF16 ? 3 : wq * wk == 4 ? 2 : 1;
+    return element == kTrainF32 ? 2 : wq * wk == 4 ? 4 : 2;
 }
 template <int EL, int WQ, int WK, bool DROP>
 __global__ __launch_bounds__(64 * WQ * WK, forward_waves(EL, WQ, WK)) void train_forward_kernel(const Args a) {
     constexpr int P = parts_of(EL), NT = 64 * WQ * WK, NS = 2 / WK;
     constexpr float TOP = ranged(EL) ? kTop - 1 : 0;  // weights are brought below 2^TOP
-    __shared__ Tile<EL> tiles[2];
+    __shared__ Tile<EL> tiles[scaled(EL) ? 1 : 2][2];  // 16-bit: the next tile's while one is worked on
     __shared__ int fields[2][scaled(EL) ? kTile : 1];
-    Tile<EL> &kt = tiles[0], &vt = tiles[1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wq = wave % WQ, wk = wave / WQ, half = lane >> 5;
     const unsigned unit = blockIdx.x / (unsigned)a.pairs;
     const int pair = blockIdx.x % (unsigned)a.pairs, tile = unit % (unsigned)a.q_tiles, split = unit / (unsigned)a.q_tiles;
@@ -459,49 +502,17 @@ __global__ __launch_bounds__(64 * WQ * WK, forward_waves(EL, WQ, WK)) void train
         for (m = 0; t < end && !(m = attended(a.keep, a.words, e, t, len)); ++t) {}
         return t;
     };
-    Staged<EL, NT> ks, vs;
-    unsigned long long todo, following = 0;
-    int t = next(split * a.q_chunk, todo);
-    auto load = [&](int tile) {
-        ks.load(a.k, a.ks, e, hk, tile * 64, len);
-        vs.load(a.v, a.vs, e, hk, tile * 64, len);
-    };
-    if (t < end) load(t);
-    bool fresh = true;
-    while (t < end) {
-        Turn turn = {todo, 0, 0};
-        if (scaled(EL) && fresh) {
-            if constexpr (scaled(EL)) ks.fields(fields[0]), vs.fields(fields[1]);
-        }
-        __syncthreads();
-        if constexpr (scaled(EL)) {
-            turn = turn_of(todo, fields[0], fields[1], lane);
-            // Values 2^40 smaller than the largest so far stay that small: their weights must not leave FP32's range.
-            turn.y = max(turn.y, most_v - 40);
-            most_v = max(most_v, turn.y);
-        }
-        const unsigned long long some = turn.some;
-        const int v_down = scaled(EL) ? down(turn.y) : 0;
-        const float c = scaled(EL) ? times_power(a.c, down(turn.x) + q_down) : a.c;
-        ks.store(kt, some, scaled(EL) ? scale_of(turn.x) : 1.f);
-        vs.store(vt, some, scaled(EL) ? scale_of(turn.y) : 1.f);
-        __syncthreads();
-        todo &= ~some;
-        const int at_tile = t;
-        fresh = !todo;
-        if (fresh) {
-            t = next(t + 1, following);
-            if (t < end) load(t);
-            todo = following;
-        }
-
+    const Lanes lanes(lane);
+    // One turn: rows `some` of tile t, its keys by 2^-k_down and its values by 2^-v_down.
+    auto work = [&](const Tile<EL> &kt, const Tile<EL> &vt, int t, unsigned long long some, int k_down, int v_down) {
+        const float c = scaled(EL) ? times_power(a.c, k_down + q_down) : a.c;
         f32x16 s[NS] = {};
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int b = 0; b < NS; ++b) {
                 V8<EL> x[P];
-                rows_operand<EL>(kt, 32 * (WK == 1 ? b : wk), c, lane, x);
+                rows_operand<EL>(kt, 32 * (WK == 1 ? b : wk), c, lanes, x);
                 mma<EL>(s[b], x, qb[c]);
             }
         if (some != ~0ull)
@@ -540,7 +551,7 @@ __global__ __launch_bounds__(64 * WQ * WK, forward_waves(EL, WQ, WK)) void train
 #pragma unroll
                 for (int j = 0; j < 8; ++j) p[j] = s[b][8 * c + j];
                 if constexpr (DROP) {
-                    const u32x4 z = philox(2 * (4 * at_tile + 2 * sub + c) + half, query, pair, a.site, seed);
+                    const u32x4 z = philox(2 * (4 * t + 2 * sub + c) + half, query, pair, a.site, seed);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) p[j] = kept16(z, j, a.line) ? p[j] : 0.f;
                 }
@@ -549,7 +560,7 @@ __global__ __launch_bounds__(64 * WQ * WK, forward_waves(EL, WQ, WK)) void train
 #pragma unroll
                 for (int d = 0; d < 2; ++d) {
                     V8<EL> x[P];
-                    dims_operand<EL>(vt, 32 * sub + 16 * c, d, lane, x);
+                    dims_operand<EL>(vt, 32 * sub + 16 * c, d, lanes, x);
                     mma<EL>(o[d], x, pb);
                 }
             }
@@ -560,6 +571,54 @@ __global__ __launch_bounds__(64 * WQ * WK, forward_waves(EL, WQ, WK)) void train
             r = upto;
         } else {
             sum += part;
+        }
+    };
+    unsigned long long todo, following = 0;
+    int t = next(split * a.q_chunk, todo);
+    if constexpr (scaled(EL)) {
+        Staged<EL, NT> ks, vs;
+        auto load = [&](int tile) {
+            ks.load(a.k, a.ks, e, hk, tile * 64, len);
+            vs.load(a.v, a.vs, e, hk, tile * 64, len);
+        };
+        if (t < end) load(t);
+        bool fresh = true;
+        while (t < end) {
+            if (fresh) ks.fields(fields[0]), vs.fields(fields[1]);
+            __syncthreads();
+            Turn turn = turn_of(todo, fields[0], fields[1], lane);
+            // Values 2^40 smaller than the largest so far stay that small: their weights must not leave FP32's range.
+            turn.y = max(turn.y, most_v - 40);
+            most_v = max(most_v, turn.y);
+            ks.store(tiles[0][0], turn.some, scale_of(turn.x));
+            vs.store(tiles[0][1], turn.some, scale_of(turn.y));
+            __syncthreads();
+            todo &= ~turn.some;
+            const int at_tile = t;
+            fresh = !todo;
+            if (fresh) {
+                t = next(t + 1, following);
+                if (t < end) load(t);
+                todo = following;
+            }
+            work(tiles[0][0], tiles[0][1], at_tile, turn.some, down(turn.x), down(turn.y));
+        }
+    } else {
+        auto load = [&](int tile, int to) {
+            load_tile<EL, NT>(tiles[to][0], a.k, a.ks, e, hk, tile * 64, len);
+            load_tile<EL, NT>(tiles[to][1], a.v, a.vs, e, hk, tile * 64, len);
+        };
+        if (t < end) load(t, 0);
+        for (int now = 0; t < end; now ^= 1) {
+            __syncthreads();  // the tile has come, and the other is read
+            if (todo != ~0ull) {
+                clear_rows<EL, NT>(tiles[now][0], todo), clear_rows<EL, NT>(tiles[now][1], todo);
+                __syncthreads();
+            }
+            const int n = next(t + 1, following);
+            if (n < end) load(n, now ^ 1);
+            work(tiles[now][0], tiles[now][1], t, todo, 0, 0);
+            t = n, todo = following;
         }
     }
     sum += other_half(sum);
@@ -675,8 +734,8 @@ __global__ __launch_bounds__(256) void train_merge_kernel(const Args a) {
 
 // ---- backward ----
 
-// What the backward pass needs of each query: {r, 1 / s, delta}; r is +inf (all weights 0) for one that attends to nothing
-// or lies past the length. Sixteen lanes to a row.
+// What the backward pass needs of each query: {r, 1 / s, delta, r + log2 s}; r is +inf (all weights 0) for one that attends to
+// nothing or lies past the length. Sixteen lanes to a row.
 template <int EL>
 __global__ __launch_bounds__(256) void train_record_kernel(const Args a) {
     const long long rows = (long long)a.pairs * a.q_rows;
@@ -692,17 +751,19 @@ __global__ __launch_bounds__(256) void train_record_kernel(const Args a) {
         float d = o[0] * g[0] + o[1] * g[1] + o[2] * g[2] + o[3] * g[3];
 #pragma unroll
         for (int i = 8; i; i >>= 1) d += __shfl_xor(d, i, 16);
-        record = f32x4{x[0], 1.f / x[1], d, 0.f};
+        record = f32x4{x[0], 1.f / x[1], d, x[0] + __builtin_amdgcn_logf(x[1])};
     }
     if (!lane) a.record[row] = record;
 }
 
 template <int EL>
 struct Streamed {
-    Tile<EL> x, y;
-    alignas(16) float r[kTile], inv[kTile], delta[kTile];
-    float coming[kTile];                        // the next tile's r
-    int fields[2][scaled(EL) ? kTile : 1];  // the next tile's exponents
+    static constexpr int N = scaled(EL) ? 1 : 2;
+    Tile<EL> x[N], y[N];
+    alignas(16) float r[N][kTile], delta[N][kTile];
+    alignas(16) u32x4 more[N][scaled(EL) ? 1 : kTile];  // 16-bit: what each row's scores and dP take besides
+    float coming[scaled(EL) ? kTile : 1];               // the next tile's r
+    int fields[2][scaled(EL) ? kTile : 1];  // and exponents
 };
 
 // The gradient of 32 queries a wave: S^T = K Q^T, V dout^T, then K^T dS, over a split's key tiles.
@@ -733,45 +794,19 @@ __device__ __forceinline__ void queries_backward(const Args &a, Streamed<EL> &ld
         for (m = 0; t < end && !(m = attended(a.keep, a.words, e, t, len)); ++t) {}
         return t;
     };
-    Staged<EL, 256> ks, vs;
-    unsigned long long todo, following = 0;
-    int t = next(split * a.q_chunk, todo);
-    auto load = [&](int tile) {
-        ks.load(a.k, a.ks, e, hk, tile * 64, len);
-        vs.load(a.v, a.vs, e, hk, tile * 64, len);
-    };
-    if (t < end) load(t);
-    bool fresh = true;
-    while (t < end) {
-        Turn turn = {todo, 0, 0};
-        if constexpr (scaled(EL))
-            if (fresh) ks.fields(lds.fields[0]), vs.fields(lds.fields[1]);
-        __syncthreads();
-        if constexpr (scaled(EL)) turn = turn_of(todo, lds.fields[0], lds.fields[1], lane);
-        const unsigned long long some = turn.some;
-        const int k_down = scaled(EL) ? down(turn.x) : 0;
+    const Lanes lanes(lane);
+    auto work = [&](const Tile<EL> &kt, const Tile<EL> &vt, int t, unsigned long long some, int k_down, int v_down) {
         const float c = scaled(EL) ? times_power(a.c, k_down + q_down) : a.c;
-        const float w = scaled(EL) ? times_power(a.w, down(turn.y) + g_down) : a.w;
-        ks.store(lds.x, some, scaled(EL) ? scale_of(turn.x) : 1.f);
-        vs.store(lds.y, some, scaled(EL) ? scale_of(turn.y) : 1.f);
-        __syncthreads();
-        todo &= ~some;
-        const int at_tile = t;
-        fresh = !todo;
-        if (fresh) {
-            t = next(t + 1, following);
-            if (t < end) load(t);
-            todo = following;
-        }
+        const float w = scaled(EL) ? times_power(a.w, v_down + g_down) : a.w;
 #pragma unroll 1
         for (int b = 0; b < 2; ++b) {
             f32x16 s = {}, dp = {};
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 V8<EL> x[P];
-                rows_operand<EL>(lds.x, 32 * b, c, lane, x);
+                rows_operand<EL>(kt, 32 * b, c, lanes, x);
                 mma<EL>(s, x, qb[c]);
-                rows_operand<EL>(lds.y, 32 * b, c, lane, x);
+                rows_operand<EL>(vt, 32 * b, c, lanes, x);
                 mma<EL>(dp, x, gb[c]);
             }
             if (some != ~0ull) leave_out(s, some, 32 * b, half);
@@ -779,7 +814,7 @@ __device__ __forceinline__ void queries_backward(const Args &a, Streamed<EL> &ld
 #pragma unroll
             for (int cc = 0; cc < 2; ++cc) {
                 u32x4 z;
-                if constexpr (DROP) z = philox(2 * (4 * at_tile + 2 * b + cc) + half, query, pair, a.site, seed);
+                if constexpr (DROP) z = philox(2 * (4 * t + 2 * b + cc) + half, query, pair, a.site, seed);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int i = 8 * cc + j;
@@ -802,10 +837,55 @@ __device__ __forceinline__ void queries_backward(const Args &a, Streamed<EL> &ld
 #pragma unroll
                 for (int d = 0; d < 2; ++d) {
                     V8<EL> x[P];
-                    dims_operand<EL>(lds.x, 32 * b + 16 * cc, d, lane, x);
+                    dims_operand<EL>(kt, 32 * b + 16 * cc, d, lanes, x);
                     mma<EL>(o[d], x, db);
                 }
             }
+        }
+    };
+    unsigned long long todo, following = 0;
+    int t = next(split * a.q_chunk, todo);
+    if constexpr (scaled(EL)) {
+        Staged<EL, 256> ks, vs;
+        auto load = [&](int tile) {
+            ks.load(a.k, a.ks, e, hk, tile * 64, len);
+            vs.load(a.v, a.vs, e, hk, tile * 64, len);
+        };
+        if (t < end) load(t);
+        bool fresh = true;
+        while (t < end) {
+            if (fresh) ks.fields(lds.fields[0]), vs.fields(lds.fields[1]);
+            __syncthreads();
+            const Turn turn = turn_of(todo, lds.fields[0], lds.fields[1], lane);
+            ks.store(lds.x[0], turn.some, scale_of(turn.x));
+            vs.store(lds.y[0], turn.some, scale_of(turn.y));
+            __syncthreads();
+            todo &= ~turn.some;
+            const int at_tile = t;
+            fresh = !todo;
+            if (fresh) {
+                t = next(t + 1, following);
+                if (t < end) load(t);
+                todo = following;
+            }
+            work(lds.x[0], lds.y[0], at_tile, turn.some, down(turn.x), down(turn.y));
+        }
+    } else {
+        auto load = [&](int tile, int to) {
+            load_tile<EL, 256>(lds.x[to], a.k, a.ks, e, hk, tile * 64, len);
+            load_tile<EL, 256>(lds.y[to], a.v, a.vs, e, hk, tile * 64, len);
+        };
+        if (t < end) load(t, 0);
+        for (int now = 0; t < end; now ^= 1) {
+            __syncthreads();  // the tile has come, and the other is read
+            if (todo != ~0ull) {
+                clear_rows<EL, 256>(lds.x[now], todo), clear_rows<EL, 256>(lds.y[now], todo);
+                __syncthreads();
+            }
+            const int n = next(t + 1, following);
+            if (n < end) load(n, now ^ 1);
+            work(lds.x[now], lds.y[now], t, todo, 0, 0);
+            t = n, todo = following;
         }
     }
     if (!mine) return;
@@ -871,68 +951,32 @@ __device__ __forceinline__ void keys_backward(const Args &a, Streamed<EL> &lds, 
     const int q_tiles = (q_len + kTile - 1) / kTile;
     const int end = here[0] | here[1] ? min((split + 1) * a.k_chunk, group * q_tiles) : 0;
     int u = split * a.k_chunk;
-    Rows qs, gs;
-    float r[Rows::N], inv[Rows::N], delta[Rows::N];
-    auto load = [&](int i) {
-        const int h = hk * group + i / q_tiles, row0 = i % q_tiles * kTile;
-        qs.load(a.q, a.qs, e, h, row0, q_len);
-        gs.load(a.dout, a.gs, e, h, row0, q_len);
+    const Lanes lanes(lane);
+    // One turn: queries of the tile at row0 of head h. FP32's r and delta stand beside them. With 16-bit elements one more
+    // product of BF16 parts adds -(r + log2 s) / c to the scores (24 bits of it) and, without dropout, -delta to dP: read from
+    // LDS for every element, the three take as much of its time as the tiles' operands.
+    bf16x8 ones[2] = {};
+    if (!half)
 #pragma unroll
-        for (int n = 0; n < Rows::N; ++n) {
-            const int row = row0 + threadIdx.x / 8 + 32 * n;
-            f32x4 x = {INFINITY, 0.f, 0.f, 0.f};
-            if (row < q_len) x = a.record[(long long)(e * a.heads + h) * a.q_rows + row];
-            r[n] = x[0], inv[n] = x[1], delta[n] = x[2];
-        }
-    };
-    if (u < end) load(u);
-    unsigned long long todo = 0;
-    while (u < end) {
-        const int h = hk * group + u / q_tiles, row0 = u % q_tiles * kTile;
-        const bool fresh = !todo;
-        if (fresh) {
-            // 1 / s goes with FP32's dout, whose parts are made here; 16-bit elements are not touched, their weights take it.
-            if constexpr (scaled(EL)) {
-                gs.times(inv);
-                qs.fields(lds.fields[0]), gs.fields(lds.fields[1]);
-            }
-            if (threadIdx.x % 8 == 0)
-#pragma unroll
-                for (int n = 0; n < Rows::N; ++n) lds.coming[threadIdx.x / 8 + 32 * n] = r[n];
-        }
-        __syncthreads();
-        if (fresh) todo = __ballot(lds.coming[lane] != INFINITY);
-        Turn turn = {todo, 0, 0};
-        if constexpr (scaled(EL)) turn = turn_of(todo, lds.fields[0], lds.fields[1], lane);
-        const unsigned long long some = turn.some;
-        const int q_down = scaled(EL) ? down(turn.x) : 0, g_down = scaled(EL) ? down(turn.y) : 0;
+        for (int n = 0; n < 3; ++n) ones[0][n] = ones[1][3 + n] = (__bf16)1.f;
+    auto work = [&](const Tile<EL> &qt, const Tile<EL> &gt, const float *r, const u32x4 *more, const float *delta, int h, int row0,
+                    int q_down, int g_down) {
         const float c = scaled(EL) ? times_power(a.c, q_down + k_down) : a.c;
         const float w = scaled(EL) ? times_power(a.w, g_down + v_down) : a.w;
-        qs.store(lds.x, some, scaled(EL) ? scale_of(turn.x) : 1.f);
-        gs.store(lds.y, some, scaled(EL) ? scale_of(turn.y) : 1.f);
-        if (threadIdx.x % 8 == 0)
-#pragma unroll
-            for (int n = 0; n < Rows::N; ++n) {
-                const int row = threadIdx.x / 8 + 32 * n;
-                lds.r[row] = some >> row & 1 ? r[n] : INFINITY;
-                lds.inv[row] = inv[n];
-                lds.delta[row] = scaled(EL) ? delta[n] * inv[n] : delta[n];
-            }
-        __syncthreads();
-        todo &= ~some;
-        if (!todo) {
-            ++u;
-            if (u < end) load(u);
-        }
 #pragma unroll 1
         for (int b = 0; b < 2; ++b) {
             f32x16 s = {}, dp = {};
+            if constexpr (!scaled(EL)) {
+                const bf16x8 x = __builtin_bit_cast(bf16x8, more[32 * b + (lane & 31)]);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, ones[0], s, 0, 0, 0);
+                if constexpr (!DROP) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, ones[1], dp, 0, 0, 0);
+            }
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
                 V8<EL> x[P];
-                rows_operand<EL>(lds.x, 32 * b, n, lane, x);
+                rows_operand<EL>(qt, 32 * b, n, lanes, x);
                 mma<EL>(s, x, kb[n]);
-                rows_operand<EL>(lds.y, 32 * b, n, lane, x);
+                rows_operand<EL>(gt, 32 * b, n, lanes, x);
                 mma<EL>(dp, x, vb[n]);
             }
             unsigned kept = ~0u;
@@ -942,13 +986,12 @@ __device__ __forceinline__ void keys_backward(const Args &a, Streamed<EL> &lds, 
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int q = 32 * b + 8 * (i / 4) + 4 * half + i % 4;
-                float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -lds.r[q]));
-                if constexpr (!scaled(EL)) p *= lds.inv[q];
+                const float p = __builtin_amdgcn_exp2f(scaled(EL) ? __builtin_fmaf(s[i], c, -r[q]) : s[i] * c);
                 const bool z = !DROP || (kept >> (8 * (i / 4) + i % 4) & 1);
                 if constexpr (DROP || scaled(EL))
-                    dp[i] = p * __builtin_fmaf(z ? dp[i] : 0.f, w, -lds.delta[q]);
+                    dp[i] = p * __builtin_fmaf(z ? dp[i] : 0.f, w, -delta[q]);
                 else
-                    dp[i] = p * (dp[i] - lds.delta[q]);
+                    dp[i] *= p;
                 s[i] = z ? p : 0.f;
                 if constexpr (ranged(EL)) most_p = fmaxf(most_p, s[i]), most_ds = fmaxf(most_ds, fabsf(dp[i]));
             }
@@ -965,16 +1008,96 @@ __device__ __forceinline__ void keys_backward(const Args &a, Streamed<EL> &lds, 
                 operand8<EL>(p, pb);
 #pragma unroll
                 for (int d = 0; d < 2; ++d) {
-                    dims_operand<EL>(lds.y, 32 * b + 16 * n, d, lane, x);
+                    dims_operand<EL>(gt, 32 * b + 16 * n, d, lanes, x);
                     mma<EL>(dv[d], x, pb);
                 }
                 operand8<EL>(ds, pb);
 #pragma unroll
                 for (int d = 0; d < 2; ++d) {
-                    dims_operand<EL>(lds.x, 32 * b + 16 * n, d, lane, x);
+                    dims_operand<EL>(qt, 32 * b + 16 * n, d, lanes, x);
                     mma<EL>(dk[d], x, pb);
                 }
             }
+        }
+    };
+    auto record = [&](int i, int row) {
+        const int h = hk * group + i / q_tiles, query = i % q_tiles * kTile + row;
+        f32x4 x = {INFINITY, 0.f, 0.f, 0.f};
+        if (query < q_len) x = a.record[(long long)(e * a.heads + h) * a.q_rows + query];
+        return x;
+    };
+    if constexpr (scaled(EL)) {
+        Rows qs, gs;
+        float r[Rows::N], inv[Rows::N], delta[Rows::N];
+        auto load = [&](int i) {
+            const int h = hk * group + i / q_tiles, row0 = i % q_tiles * kTile;
+            qs.load(a.q, a.qs, e, h, row0, q_len);
+            gs.load(a.dout, a.gs, e, h, row0, q_len);
+#pragma unroll
+            for (int n = 0; n < Rows::N; ++n) {
+                const f32x4 x = record(i, threadIdx.x / 8 + 32 * n);
+                r[n] = x[0], inv[n] = x[1], delta[n] = x[2];
+            }
+        };
+        if (u < end) load(u);
+        unsigned long long todo = 0;
+        while (u < end) {
+            const int h = hk * group + u / q_tiles, row0 = u % q_tiles * kTile;
+            const bool fresh = !todo;
+            if (fresh) {
+                gs.times(inv);  // 1 / s goes with dout, whose parts are made here
+                qs.fields(lds.fields[0]), gs.fields(lds.fields[1]);
+                if (threadIdx.x % 8 == 0)
+#pragma unroll
+                    for (int n = 0; n < Rows::N; ++n) lds.coming[threadIdx.x / 8 + 32 * n] = r[n];
+            }
+            __syncthreads();
+            if (fresh) todo = __ballot(lds.coming[lane] != INFINITY);
+            const Turn turn = turn_of(todo, lds.fields[0], lds.fields[1], lane);
+            qs.store(lds.x[0], turn.some, scale_of(turn.x));
+            gs.store(lds.y[0], turn.some, scale_of(turn.y));
+            if (threadIdx.x % 8 == 0)
+#pragma unroll
+                for (int n = 0; n < Rows::N; ++n) {
+                    const int row = threadIdx.x / 8 + 32 * n;
+                    lds.r[0][row] = turn.some >> row & 1 ? r[n] : INFINITY;
+                    lds.delta[0][row] = delta[n] * inv[n];
+                }
+            __syncthreads();
+            todo &= ~turn.some;
+            if (!todo) {
+                ++u;
+                if (u < end) load(u);
+            }
+            work(lds.x[0], lds.y[0], lds.r[0], nullptr, lds.delta[0], h, row0, down(turn.x), down(turn.y));
+        }
+    } else {
+        const float inverse = -1.f / a.c;
+        f32x4 coming = {};
+        auto load = [&](int i, int to) {
+            const int h = hk * group + i / q_tiles, row0 = i % q_tiles * kTile;
+            load_tile<EL, 256>(lds.x[to], a.q, a.qs, e, h, row0, q_len);
+            load_tile<EL, 256>(lds.y[to], a.dout, a.gs, e, h, row0, q_len);
+            if (threadIdx.x < kTile) coming = record(i, threadIdx.x);
+        };
+        if (u < end) load(u, 0);
+        for (int now = 0; u < end; ++u, now ^= 1) {
+            if (threadIdx.x < kTile) {
+                lds.r[now][threadIdx.x] = coming[0];
+                lds.delta[now][threadIdx.x] = coming[2];
+                // A row without weights has a score that leaves none.
+                const bool none = coming[0] == INFINITY;
+                const u32x2 x = bf16_parts(none ? -0x1p120f : coming[3] * inverse), y = bf16_parts(-coming[2]);
+                lds.more[now][threadIdx.x] = u32x4{x[0], x[1] | y[0] << 16, y[0] >> 16 | y[1] << 16, 0};
+            }
+            __syncthreads();  // the tile has come, and the other is read
+            const unsigned long long some = __ballot(lds.r[now][lane] != INFINITY);
+            if (some != ~0ull) {
+                clear_rows<EL, 256>(lds.x[now], some), clear_rows<EL, 256>(lds.y[now], some);
+                __syncthreads();
+            }
+            if (u + 1 < end) load(u + 1, now ^ 1);
+            work(lds.x[now], lds.y[now], nullptr, lds.more[now], lds.delta[now], hk * group + u / q_tiles, u % q_tiles * kTile, 0, 0);
         }
     }
     if (key >= len) return;
@@ -1003,7 +1126,7 @@ __device__ __forceinline__ void keys_backward(const Args &a, Streamed<EL> &lds, 
 }
 
 template <int EL, bool DROP>
-__global__ __launch_bounds__(256, 2) void train_backward_kernel(const Args a) {
+__global__ __launch_bounds__(256, EL == kTrainF32 || DROP ? 2 : 3) void train_backward_kernel(const Args a) {
     __shared__ Streamed<EL> lds;
     if (blockIdx.x < (unsigned)a.q_blocks)
         queries_backward<EL, DROP>(a, lds, blockIdx.x);
