@@ -102,11 +102,33 @@ __device__ __forceinline__ u32x2 bf16_parts(float x) {
     return {a | b << 16, bf16_pair(y - __uint_as_float(b << 16), 0.f)};
 }
 
+// Eight FP32 numbers, times a power of two where SCALED, as pairs of FP16 values, the second the rounded rest of the first:
+// each rest one mixed multiplication and addition (with an opaque -1 in place of a subtraction), the first's conversion kept
+// from being made again for it.
+template <bool SCALED>
+__device__ __forceinline__ void pairs8(const float *x, float scale, half8 (&out)[2]) {
+    u32x4 h, l;
+    float minus = -1.f;
+    asm("" : "+s"(minus));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float a = x[2 * i], b = x[2 * i + 1];
+        unsigned w = __builtin_bit_cast(unsigned, __builtin_convertvector((SCALED ? f32x2{a * scale, b * scale} : f32x2{a, b}), half2v));
+        asm("" : "+v"(w));
+        const half2v hi = __builtin_bit_cast(half2v, w);
+        half2v lo;
+        lo[0] = (_Float16)(SCALED ? __builtin_fmaf(a, scale, -(float)hi[0]) : __builtin_fmaf((float)hi[0], minus, a));
+        lo[1] = (_Float16)(SCALED ? __builtin_fmaf(b, scale, -(float)hi[1]) : __builtin_fmaf((float)hi[1], minus, b));
+        h[i] = w, l[i] = __builtin_bit_cast(unsigned, lo);
+    }
+    out[0] = __builtin_bit_cast(half8, h), out[1] = __builtin_bit_cast(half8, l);
+}
+
 // Eight numbers as an operand's parts.
 template <int EL>
 __device__ __forceinline__ void operand8(const float *x, V8<EL> (&out)[parts_of(EL)]) {
     if constexpr (EL == kTrainF32) {
-        pair8(x, out[0], out[1]);
+        pairs8<false>(x, 1.f, out);
     } else {
         u32x4 w;
 #pragma unroll
@@ -126,9 +148,7 @@ __device__ __forceinline__ void raw_operand(const Raw<EL> &r, float scale, V8<EL
     if constexpr (EL == kTrainF32) {
         float x[8];
         to_floats<EL>(r, x);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] *= scale;
-        operand8<EL>(x, out);
+        pairs8<true>(x, scale, out);
     } else {
         out[0] = __builtin_bit_cast(V8<EL>, r.w[0]);
     }
@@ -388,12 +408,19 @@ struct Staged {
     }
     // Rows whose bit is not set become zeros, whatever they hold.
     __device__ __forceinline__ void store(Tile<EL> &t, unsigned long long some, float scale) const {
+        if (some == ~0ull)
+            put<true>(t, some, scale);
+        else
+            put<false>(t, some, scale);
+    }
+    template <bool ALL>
+    __device__ __forceinline__ void put(Tile<EL> &t, unsigned long long some, float scale) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int u = threadIdx.x + i * NT, row = u / 8;
             V8<EL> b[parts_of(EL)];
             raw_operand<EL>(r[i], scale, b);
-            const bool in = some >> row & 1;
+            const bool in = ALL || (some >> row & 1);
 #pragma unroll
             for (int p = 0; p < parts_of(EL); ++p) {
                 u32x4 w = __builtin_bit_cast(u32x4, b[p]);
@@ -404,10 +431,16 @@ struct Staged {
     }
 };
 
+// A wave's largest value, in every lane. (Through LDS, as shuffles go, six steps cost a tile more than its softmax.)
 __device__ __forceinline__ int wave_max_int(int v) {
-#pragma unroll
-    for (int i = 32; i; i >>= 1) v = max(v, __shfl_xor(v, i, 64));
-    return v;
+    v = max(v, __builtin_amdgcn_mov_dpp(v, 0xB1, 15, 15, true));   // lane ^ 1
+    v = max(v, __builtin_amdgcn_mov_dpp(v, 0x4E, 15, 15, true));   // lane ^ 2
+    v = max(v, __builtin_amdgcn_mov_dpp(v, 0x141, 15, 15, true));  // lane ^ 7
+    v = max(v, __builtin_amdgcn_mov_dpp(v, 0x140, 15, 15, true));  // lane ^ 15
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max((int)a[0], (int)a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max((int)b[0], (int)b[1]);
 }
 
 // The rows of `todo` that a turn takes, and the exponent fields for x and y: those within 2^14 of the largest x (rows of
