@@ -185,6 +185,16 @@ __device__ __forceinline__ void store4(void *base, long long at, f32x4 x) {
 }
 
 template <int EL>
+__device__ __forceinline__ void store1(void *base, long long at, float x) {
+    if constexpr (EL == kTrainF32)
+        static_cast<float *>(base)[at] = x;
+    else if constexpr (EL == kTrainF16)
+        static_cast<_Float16 *>(base)[at] = (_Float16)x;
+    else
+        static_cast<unsigned short *>(base)[at] = (unsigned short)bf16_pair(x, 0.f);
+}
+
+template <int EL>
 __device__ __forceinline__ f32x4 load4(const void *base, long long at) {
     if constexpr (EL == kTrainF32) {
         return *reinterpret_cast<const f32x4 *>(static_cast<const float *>(base) + at);
@@ -715,6 +725,168 @@ __global__ __launch_bounds__(64 * WQ * WK, forward_waves(EL, WQ, WK)) void train
         const float ref = r == -INFINITY ? 0.f : r;
         if (a.stats) *reinterpret_cast<f32x2 *>(a.stats + 2 * row) = f32x2{ref, sum};
         if (a.lse) a.lse[row] = kLn2 * (ref + __builtin_amdgcn_logf(sum));
+    }
+}
+
+// One to four rows (queries of the heads that share a key head) against their keys, for which the matrix cores' 32 columns
+// stand empty and reading keys and values is all there is: FP32 sums, LK lanes to a key (16 bytes each), eight keys of one
+// call of random numbers to a group of lanes, a wave's 64 keys (FP32: 32) in flight at once.
+template <int EL, int NQ, bool DROP>
+__global__ __launch_bounds__(256) void train_rows_kernel(const Args a) {
+    constexpr int D = EL == kTrainF32 ? 4 : 8, LK = 64 / D, GROUPS = 64 / LK;  // dims of a lane; groups of a wave
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane / LK, dim = D * (lane % LK);
+    const int share = a.heads / a.kv_heads, owners = a.pairs / share;
+    const int owner = blockIdx.x % (unsigned)owners, split = blockIdx.x / (unsigned)owners;
+    const int e = owner / a.kv_heads, hk = owner % a.kv_heads;
+    const int q_len = length_of(a.q_lengths, e, a.q_rows), len = length_of(a.lengths, e, a.rows);
+    if (!q_len) return;
+    auto place = [&](int n, int &h, int &query) {
+        n = min(n, share * a.q_rows - 1);
+        h = hk * share + n / a.q_rows, query = n % a.q_rows;
+    };
+    float q[NQ][D], o[NQ][D] = {}, r[NQ], sum[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        int h, query;
+        place(n, h, query);
+        r[n] = -INFINITY, sum[n] = 0.f;
+#pragma unroll
+        for (int j = 0; j < D; j += 4) {
+            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+            if (query < q_len) x = load4<EL>(a.q, at(a.qs, e, h, query) + dim + j);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q[n][j + i] = x[i];
+        }
+    }
+    const unsigned long long seed = DROP ? *a.seed : 0;
+    const int end = min((split + 1) * a.q_chunk, (int)((len + 63) / 64));
+    for (int t = split * a.q_chunk + wave; t < end; t += 4) {
+        const unsigned long long some = attended(a.keep, a.words, e, t, len);
+        if (!some) continue;
+#pragma unroll 1
+        for (int first = 0; first < 64; first += 8 * GROUPS) {
+            // The group's cell: keys 16 (cell / 2) + 4 (cell % 2) + 0..3 and 8..11 of the tile.
+            const int cell = first / 8 + group, base = 16 * (cell / 2) + 4 * (cell % 2);
+            u32x4 k[8], v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int row = min(t * 64 + base + 8 * (j / 4) + j % 4, len - 1);
+                const int bytes = EL == kTrainF32 ? 4 : 2;
+                k[j] = *reinterpret_cast<const u32x4 *>(static_cast<const char *>(a.k) + (at(a.ks, e, hk, row) + dim) * bytes);
+                v[j] = *reinterpret_cast<const u32x4 *>(static_cast<const char *>(a.v) + (at(a.vs, e, hk, row) + dim) * bytes);
+            }
+            const unsigned bits = (unsigned)(some >> base);
+            if (some != ~0ull)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (!(bits >> (8 * (j / 4) + j % 4) & 1)) k[j] = v[j] = u32x4{0, 0, 0, 0};
+            auto numbers = [](const u32x4 &w, float *x) {
+                Raw<EL> raw;
+                if constexpr (EL == kTrainF32) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(w[i]);
+                } else {
+                    raw.w[0] = w;
+                    to_floats<EL>(raw, x);
+                }
+            };
+            float x[NQ][8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float kk[D];
+                numbers(k[j], kk);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+                    float d = 0.f;
+#pragma unroll
+                    for (int i = 0; i < D; ++i) d = __builtin_fmaf(q[n][i], kk[i], d);
+                    auto step = [&](int moved) { d += __int_as_float(moved); };
+                    step(__builtin_amdgcn_mov_dpp(__float_as_int(d), 0xB1, 15, 15, true));
+                    step(__builtin_amdgcn_mov_dpp(__float_as_int(d), 0x4E, 15, 15, true));
+                    step(__builtin_amdgcn_mov_dpp(__float_as_int(d), 0x141, 15, 15, true));
+                    if constexpr (LK == 16) step(__builtin_amdgcn_mov_dpp(__float_as_int(d), 0x140, 15, 15, true));
+                    x[n][j] = d * a.c;
+                }
+            }
+            if (some != ~0ull)
+#pragma unroll
+                for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[n][j] = bits >> (8 * (j / 4) + j % 4) & 1 ? x[n][j] : -INFINITY;
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                float top = x[n][0];
+#pragma unroll
+                for (int j = 1; j < 8; ++j) top = fmaxf(top, x[n][j]);
+                const float upto = fmaxf(r[n], ceilf(top));
+                if (__any(upto > r[n])) {
+                    const float f = r[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(r[n] - upto);
+                    sum[n] *= f;
+#pragma unroll
+                    for (int i = 0; i < D; ++i) o[n][i] *= f;
+                    r[n] = upto;
+                }
+                const float ref = r[n] == -INFINITY ? 0.f : r[n];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    x[n][j] = __builtin_amdgcn_exp2f(x[n][j] - ref);
+                    sum[n] += x[n][j];
+                }
+                if constexpr (DROP) {
+                    int h, query;
+                    place(n, h, query);
+                    const u32x4 z = philox(8 * t + cell, query, e * a.heads + h, a.site, seed);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[n][j] = kept16(z, j, a.line) ? x[n][j] : 0.f;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float vv[D];
+                numbers(v[j], vv);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                    for (int i = 0; i < D; ++i) o[n][i] = __builtin_fmaf(x[n][j], vv[i], o[n][i]);
+            }
+        }
+    }
+    // The groups of the workgroup's waves: each leaves its sums, and a wave joins a row's.
+    __shared__ float left_o[NQ][4 * GROUPS][64], left_r[NQ][4 * GROUPS], left_sum[NQ][4 * GROUPS];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+#pragma unroll
+        for (int i = 0; i < D; ++i) left_o[n][wave * GROUPS + group][dim + i] = o[n][i];
+        if (lane % LK == 0) left_r[n][wave * GROUPS + group] = r[n], left_sum[n][wave * GROUPS + group] = sum[n];
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int n = wave; n < min(NQ, share * a.q_rows); n += 4) {
+        int h, query;
+        place(n, h, query);
+        if (query >= q_len) continue;
+        float top = -INFINITY, total = 0.f, out = 0.f;
+#pragma unroll
+        for (int g = 0; g < 4 * GROUPS; ++g) top = fmaxf(top, left_r[n][g]);
+        const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int g = 0; g < 4 * GROUPS; ++g) {
+            const float f = __builtin_amdgcn_exp2f(left_r[n][g] - ref);
+            total += left_sum[n][g] * f;
+            out += left_o[n][g][lane] * f;
+        }
+        const long long row = (long long)(e * a.heads + h) * a.q_rows + query;
+        if (a.q_splits > 1) {
+            a.q_part[((long long)split * a.pairs * a.q_rows + row) * 64 + lane] = out;
+            float *m = a.q_part + (long long)a.q_splits * a.pairs * a.q_rows * 64 + ((long long)split * a.pairs * a.q_rows + row) * 2;
+            if (!lane) *reinterpret_cast<f32x2 *>(m) = f32x2{top, total};
+            continue;
+        }
+        store1<EL>(a.out, at(a.os, e, h, query) + lane, total == 0.f ? 0.f : out * (a.w / total));
+        if (!lane) {
+            if (a.stats) *reinterpret_cast<f32x2 *>(a.stats + 2 * row) = f32x2{ref, total};
+            if (a.lse) a.lse[row] = kLn2 * (ref + __builtin_amdgcn_logf(total));
+        }
     }
 }
 
@@ -1257,15 +1429,23 @@ struct Plan {
 };
 
 int splits_of(double length, double target, long long tiles) {
-    return (int)std::min<long long>(std::max(1ll, std::llround(length / target)), std::min(tiles, 64ll));
+    return (int)std::min<long long>(std::max(1ll, std::llround(length / target)), std::min(tiles, 128ll));
 }
 
 Plan plan(const TrainShape &s, int element, bool backward, int compute_units) {
     Plan p{};
     const long long pairs = (long long)s.estimators * s.heads, owners = (long long)s.estimators * s.kv_heads;
     const long long words = (s.rows + 63) / 64, q_words = (s.q_rows + 63) / 64, group = s.heads / s.kv_heads;
-    const double slots = 2.0 * compute_units;
+    const double slots = (backward || element == kTrainF32 ? 2.0 : 4.0) * compute_units;
     p.q_unit = backward || s.q_rows > 64 ? 128 : s.q_rows > 32 ? 64 : 32;
+    // Few rows go one key at a time. Over 50,000 rows, in us, so and by the matrix cores: 8 FP32 heads of 1 / 2 / 4 / 8
+    // queries 37.6 / 39.2 / 41.2 / 53.8 and 55 to 56; of 2 key heads, 1 / 2 queries (4 / 8 rows) 21.1 / 27.7 and 55; BF16, 8
+    // heads of 1 / 2 / 4 queries 24.6 / 26.5 / 30.3 and 25.1 / 25.4 / 25.9, of 2 key heads, 1 / 2 queries 16.4 / 23.2 and 25;
+    // over 1,000, 8 FP32 heads of 1 / 2 / 4 / 8 8.2 / 9.1 / 10.6 / 14.8 and 10.0 to 10.3, BF16 of 2 key heads, 1 query 10.2
+    // and 7.9.
+    const long long few = group * s.q_rows;
+    const bool shared = group > 1 && s.rows >= 8192, single = element == kTrainF32;
+    if (!backward && (few == 1 || (few <= 4 && (single || shared)) || (few <= 8 && single && shared))) p.q_unit = (int)few;
     p.q_tiles = (int)ceil_div(s.q_rows, p.q_unit);
     p.k_tiles = (int)ceil_div(s.rows, 128);
     if (backward) {
@@ -1275,6 +1455,10 @@ Plan plan(const TrainShape &s, int element, bool backward, int compute_units) {
         const double share = std::max(all / slots, 3.0);
         p.q_splits = splits_of(3.0 * words, share, words);
         p.k_splits = splits_of(4.0 * group * q_words, share, group * q_words);
+    } else if (p.q_unit <= 8) {
+        // A wave takes a tile at a time.
+        p.q_splits = splits_of((double)words, std::max(owners * words / (2.0 * compute_units), 4.0), words);
+        p.k_splits = 1;
     } else {
         p.q_splits = splits_of((double)words, std::max(pairs * p.q_tiles * words / slots, 1.0), words);
         p.k_splits = 1;
@@ -1287,7 +1471,7 @@ Plan plan(const TrainShape &s, int element, bool backward, int compute_units) {
     p.record = backward ? rows * 16 : 0;
     p.q_part = p.q_splits > 1 ? (size_t)p.q_splits * rows * (backward ? 256 : 264) : 0;
     p.k_part = p.k_splits > 1 ? (size_t)p.k_splits * owners * s.rows * 512 : 0;
-    p.blocks = (double)pairs * p.q_tiles * p.q_splits + (backward ? (double)owners * p.k_tiles * p.k_splits : 0.0);
+    p.blocks = (double)(p.q_unit <= 8 ? owners : pairs * p.q_tiles) * p.q_splits + (backward ? (double)owners * p.k_tiles * p.k_splits : 0.0);
     return p;
 }
 
@@ -1318,7 +1502,15 @@ void forward(const TrainInputs &a, const TrainForward &f, const Plan &p, hipStre
     {
         KernelTimer timer(kFamIcl, stream, 256.0 * k.pairs * k.q_rows * k.rows, 0.0);
         auto launch = [&]<bool DROP>() {
-            if (p.q_unit == 32)
+            if (p.q_unit == 1)
+                hipLaunchKernelGGL((train_rows_kernel<EL, 1, DROP>), grid, dim3(256), 0, stream, k);
+            else if (p.q_unit == 2)
+                hipLaunchKernelGGL((train_rows_kernel<EL, 2, DROP>), grid, dim3(256), 0, stream, k);
+            else if (p.q_unit <= 4)
+                hipLaunchKernelGGL((train_rows_kernel<EL, 4, DROP>), grid, dim3(256), 0, stream, k);
+            else if (EL == kTrainF32 && p.q_unit <= 8)
+                hipLaunchKernelGGL((train_rows_kernel<kTrainF32, 8, DROP>), grid, dim3(256), 0, stream, k);
+            else if (p.q_unit == 32)
                 hipLaunchKernelGGL((train_forward_kernel<EL, 1, 2, DROP>), grid, dim3(128), 0, stream, k);
             else if (p.q_unit == 64)
                 hipLaunchKernelGGL((train_forward_kernel<EL, 2, 2, DROP>), grid, dim3(256), 0, stream, k);
