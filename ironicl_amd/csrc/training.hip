@@ -278,11 +278,13 @@ __device__ __forceinline__ float other_half(float x) {
 // ---- random numbers ----
 
 // Philox4x32 (Salmon, Moraes, Dror and Shaw, "Parallel random numbers: as easy as 1, 2, 3", SC 2011) with seven rounds, the
-// fewest that pass their whole test suite.
+// fewest that pass their whole test suite. FLIP: an exclusive or with every word, half of it in what the last round adds.
+template <unsigned FLIP = 0>
 __device__ __forceinline__ u32x4 philox(unsigned c0, unsigned c1, unsigned c2, unsigned c3, unsigned long long seed) {
     unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
 #pragma unroll
     for (int round = 0; round < 7; ++round) {
+        if (round == 6) k0 ^= FLIP, k1 ^= FLIP;
         const unsigned long long a = (unsigned long long)c0 * 0xD2511F53u, b = (unsigned long long)c2 * 0xCD9E8D57u;
         c0 = __builtin_amdgcn_bitop3_b32((unsigned)(b >> 32), c1, k0, 0x96);  // the three's exclusive or
         c1 = (unsigned)b;
@@ -290,12 +292,30 @@ __device__ __forceinline__ u32x4 philox(unsigned c0, unsigned c1, unsigned c2, u
         c3 = (unsigned)a;
         k0 += 0x9E3779B9u, k1 += 0xBB67AE85u;
     }
-    return u32x4{c0, c1, c2, c3};
+    return u32x4{c0, c1 ^ FLIP, c2, c3 ^ FLIP};
 }
 
 // Whether number j of a call's eight 16-bit ones is kept; `line` is dropped << 16.
 __device__ __forceinline__ bool kept16(const u32x4 &w, int j, unsigned line) {
     return (j & 1 ? w[j >> 1] : w[j >> 1] << 16) >= line;
+}
+
+// Eight 16-bit numbers without those that a call drops, its words with every value's highest bit flipped. The 16-bit values are compared two at a time, as signed ones: a
+// saturated difference's sign, over the half, is the mask (3.5 instructions a pair, with comparisons and selections 5).
+constexpr unsigned kFlip = 0x80008000u;
+template <int EL>
+__device__ __forceinline__ V8<EL> drop8(V8<EL> x, const u32x4 &z, unsigned line) {
+    typedef short s16x2 __attribute__((ext_vector_type(2)));
+    u32x4 w = __builtin_bit_cast(u32x4, x);
+    const s16x2 at = __builtin_bit_cast(s16x2, (line | line >> 16) ^ kFlip);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const unsigned values = z[i];
+        const s16x2 below = __builtin_elementwise_sub_sat(__builtin_bit_cast(s16x2, values), at) >> 15;
+        const unsigned lost = __builtin_bit_cast(unsigned, below);
+        w[i] &= ~lost;
+    }
+    return __builtin_bit_cast(V8<EL>, w);
 }
 
 // ---- lengths and masks ----
@@ -593,13 +613,14 @@ __global__ __launch_bounds__(64 * WQ * WK, forward_waves(EL, WQ, WK)) void train
                 float p[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) p[j] = s[b][8 * c + j];
-                if constexpr (DROP) {
-                    const u32x4 z = philox(2 * (4 * t + 2 * sub + c) + half, query, pair, a.site, seed);
+                u32x4 z;
+                if constexpr (DROP) z = philox<scaled(EL) ? 0 : kFlip>(2 * (4 * t + 2 * sub + c) + half, query, pair, a.site, seed);
+                if constexpr (DROP && scaled(EL))
 #pragma unroll
                     for (int j = 0; j < 8; ++j) p[j] = kept16(z, j, a.line) ? p[j] : 0.f;
-                }
                 V8<EL> pb[P];
                 operand8<EL>(p, pb);
+                if constexpr (DROP && !scaled(EL)) pb[0] = drop8<EL>(pb[0], z, a.line);
 #pragma unroll
                 for (int d = 0; d < 2; ++d) {
                     V8<EL> x[P];
@@ -897,8 +918,9 @@ __global__ __launch_bounds__(256) void train_merge_kernel(const Args a) {
     const int lane = threadIdx.x & 15, group = threadIdx.x / 16 % W;
     const long long row = (long long)blockIdx.x * (16 / W) + threadIdx.x / (16 * W);
     __shared__ float joined[W > 1 ? 16 : 1][16][4];
-    bool some = row < rows;
-    const int pair = some ? (int)(row / a.q_rows) : 0, query = some ? (int)(row % a.q_rows) : 0, e = pair / a.heads;
+    bool some = row < rows;  // fewer than 2^27 of them
+    const int pair = some ? (int)((unsigned)row / (unsigned)a.q_rows) : 0, e = pair / a.heads;
+    const int query = some ? (int)((unsigned)row % (unsigned)a.q_rows) : 0;
     some = some && query < length_of(a.q_lengths, e, a.q_rows);
     const float *m = a.q_part + (long long)a.q_splits * rows * 64;
     float r = -INFINITY, ref = 0.f, sum = 0.f;
@@ -1529,8 +1551,10 @@ void forward(const TrainInputs &a, const TrainForward &f, const Plan &p, hipStre
         const size_t rows = (size_t)k.pairs * k.q_rows;
         if (p.q_splits > 8)
             hipLaunchKernelGGL((train_merge_kernel<EL, 16>), dim3((unsigned)rows), dim3(256), 0, stream, k);
-        else
+        else if (p.q_splits > 4)
             hipLaunchKernelGGL((train_merge_kernel<EL, 4>), dim3(ceil_div(rows, 4)), dim3(256), 0, stream, k);
+        else
+            hipLaunchKernelGGL((train_merge_kernel<EL, 1>), dim3(ceil_div(rows, 16)), dim3(256), 0, stream, k);
         IRX_HIP(hipGetLastError());
     }
 }
