@@ -535,7 +535,7 @@ constexpr int kNone = -1000;  // a lane's power before its first term
 // takes 32 of each. S^T = K Q^T leaves a query's scores in one lane (and its other half), in the order in which the next
 // product takes them.
 constexpr int forward_waves(int element, int wq, int wk) {  // of a SIMD: what registers leave room for
-    return element == kTrainF32 ? 2 : wq * wk == 4 ? 4 : 2;
+    return element == kTrainF32 ? 2 : wq * wk;
 }
 template <int EL, int WQ, int WK, bool DROP>
 __global__ __launch_bounds__(64 * WQ * WK, forward_waves(EL, WQ, WK)) void train_forward_kernel(const Args a) {
@@ -1214,12 +1214,22 @@ __device__ __forceinline__ void keys_backward(const Args &a, Streamed<EL> &lds, 
             for (int i = 0; i < 16; ++i) {
                 const int q = 32 * b + 8 * (i / 4) + 4 * half + i % 4;
                 const float p = __builtin_amdgcn_exp2f(scaled(EL) ? __builtin_fmaf(s[i], c, -r[q]) : s[i] * c);
-                const bool z = !DROP || (kept >> (8 * (i / 4) + i % 4) & 1);
+                s[i] = p;
+                if constexpr (DROP && scaled(EL)) {
+                    const bool z = kept >> (8 * (i / 4) + i % 4) & 1;
+                    dp[i] = z ? dp[i] : 0.f;
+                    s[i] = z ? p : 0.f;
+                } else if constexpr (DROP) {
+                    // A bit as a mask of the whole number: an instruction less; FP32's kernel has no registers left for it (195 us
+                    // in place of 163 for the gradients of four tables of 1,024 rows).
+                    const int z = __builtin_amdgcn_sbfe((int)kept, 8 * (i / 4) + i % 4, 1);
+                    dp[i] = __int_as_float(__float_as_int(dp[i]) & z);
+                    s[i] = __int_as_float(__float_as_int(p) & z);
+                }
                 if constexpr (DROP || scaled(EL))
-                    dp[i] = p * __builtin_fmaf(z ? dp[i] : 0.f, w, -delta[q]);
+                    dp[i] = p * __builtin_fmaf(dp[i], w, -delta[q]);
                 else
                     dp[i] *= p;
-                s[i] = z ? p : 0.f;
                 if constexpr (ranged(EL)) most_p = fmaxf(most_p, s[i]), most_ds = fmaxf(most_ds, fabsf(dp[i]));
             }
             if constexpr (ranged(EL)) {
@@ -1474,7 +1484,7 @@ Plan plan(const TrainShape &s, int element, bool backward, int compute_units) {
         // A tile of keys costs a unit of queries three products, a tile of queries a unit of keys four. No workgroup walks
         // further than its share of all the work.
         const double all = 3.0 * pairs * p.q_tiles * words + 4.0 * owners * p.k_tiles * group * q_words;
-        const double share = std::max(all / slots, 3.0);
+        const double share = std::max(all / slots, 6.0);
         p.q_splits = splits_of(3.0 * words, share, words);
         p.k_splits = splits_of(4.0 * group * q_words, share, group * q_words);
     } else if (p.q_unit <= 8) {
