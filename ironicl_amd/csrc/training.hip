@@ -1469,13 +1469,15 @@ Plan plan(const TrainShape &s, int element, bool backward, bool uneven, int comp
     Plan p{};
     const long long pairs = (long long)s.estimators * s.heads, owners = (long long)s.estimators * s.kv_heads;
     const long long words = (s.rows + 63) / 64, q_words = (s.q_rows + 63) / 64, group = s.heads / s.kv_heads;
-    const double slots = (backward || element == kTrainF32 ? 2.0 : 4.0) * compute_units;
     p.q_unit = backward || s.q_rows > 64 ? 128 : s.q_rows > 32 ? 64 : 32;
-    // Few rows go one key at a time. Over 50,000 rows, in us, so and by the matrix cores: 8 FP32 heads of 1 / 2 / 4 / 8
-    // queries 37.6 / 39.2 / 41.2 / 53.8 and 55 to 56; of 2 key heads, 1 / 2 queries (4 / 8 rows) 21.1 / 27.7 and 55; BF16, 8
-    // heads of 1 / 2 / 4 queries 24.6 / 26.5 / 30.3 and 25.1 / 25.4 / 25.9, of 2 key heads, 1 / 2 queries 16.4 / 23.2 and 25;
-    // over 1,000, 8 FP32 heads of 1 / 2 / 4 / 8 8.2 / 9.1 / 10.6 / 14.8 and 10.0 to 10.3, BF16 of 2 key heads, 1 query 10.2
-    // and 7.9.
+    // Workgroups that a launch should have at once: what registers leave room for on the compute units (with two of 128 threads
+    // on each, 32 FP32 queries over 50,000 rows took 59 us in place of 47).
+    const double slots = (backward || (element == kTrainF32 && p.q_unit > 32) ? 2.0 : 4.0) * compute_units;
+    // Few rows go one key at a time where that is faster. In us, so and by the matrix cores, over 50,000 rows: 8 FP32 heads
+    // of 1 / 2 / 4 / 8 queries 37.9 / 40.1 / 42.8 / 53.1 and 44.6 / 45.4 / 45.2 / 45.8; 8 over 2 key heads, of 1 / 2 queries
+    // 21.0 / 27.6 and 45; 8 BF16 heads of 1 / 2 / 4 queries 24.4 / 27.0 / 30.1 and 26.1 / 26.3 / 26.8, over 2 key heads, of 1
+    // query 16.7 and 26.3. Over 1,000: 8 FP32 heads of 1 / 2 / 4 / 8 queries 7.7 / 8.9 / 10.8 / 14.8 and 10.0 to 10.3, over 2
+    // key heads, of 2 queries 14.2 and 10.1; BF16, of 1 query 9.9 and 7.9.
     const long long few = group * s.q_rows;
     const bool shared = group > 1 && s.rows >= 8192, single = element == kTrainF32;
     if (!backward && (few == 1 || (few <= 4 && (single || shared)) || (few <= 8 && single && shared))) p.q_unit = (int)few;
