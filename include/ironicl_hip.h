@@ -541,11 +541,13 @@ size_t irx_train_workspace_bytes(irx_device *device, const irx_train_shape *shap
  * query that attends to none. stats, when not NULL, [E, heads, query_rows, 2] FP32,
  * 8-byte aligned: what the backward pass needs, a whole number r and s = the sum of 2^(log2(e) scale q k - r)
  * (0 and 0 where there is none).
- * Inputs that are read must be finite, at most 2^127, and scale q and the scores
- * within FP32's range. What is rounded: FP32 operands of a product to 24 bits
- * (products of the lowest parts, below 2^-23, left out), FP16's operands of weights
- * to 16, BF16's to 8; sums and statistics are FP32. Weights below 2^-126, and parts
- * of operands below that, may be taken as 0. */
+ * Inputs that are read must be finite, scale q k at most 2^20 in size and q k within
+ * FP32's range. What is rounded: FP32's operands of a product to 22 bits, weights and
+ * dS too, or to 2^-38 of the largest number beside them (of their row, and of those of
+ * its 64 neighbours that are within 2^14 of it; weights and dS: of the largest for
+ * their query or key) where that is more; 16-bit operands not at all, weights and dS to
+ * one value of the type (FP16's to 2^-38 of the largest where that is more); sums and
+ * statistics are FP32. Weights below 2^-126 are taken as 0. */
 int irx_train_attention(irx_device *device, const irx_train_inputs *inputs, void *out, const irx_strides *out_strides,
                         float *stats, float *lse, void *workspace, size_t workspace_bytes, void *stream);
 /* The gradients of q, k and v from the output's. Probabilities are computed anew
