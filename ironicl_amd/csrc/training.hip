@@ -1493,7 +1493,7 @@ Plan plan(const TrainShape &s, int element, bool backward, bool uneven, int comp
         p.k_splits = splits_of(4.0 * group * q_words, share, group * q_words);
     } else if (p.q_unit <= 8) {
         // A wave takes a tile at a time.
-        p.q_splits = splits_of((double)words, std::max(owners * words / (2.0 * compute_units), 4.0), words);
+        p.q_splits = splits_of((double)words, std::max((double)owners * words / compute_units, 4.0), words);
         p.k_splits = 1;
     } else {
         p.q_splits = splits_of((double)words, std::max(pairs * p.q_tiles * words / slots, 1.0), words);
