@@ -559,7 +559,7 @@ int irx_train_attention_backward(irx_device *device, const irx_train_inputs *inp
 /* out = residual + w D(x), rounded once; with residual NULL, w D(x), which is also
  * the gradient of x from that of out. Rows start `stride` elements apart (multiples of
  * 16 bytes, as the pointers are; at least the width, where there is more than one
- * row). out may be x or residual, at its stride. 1 to 2^31 - 1 columns, rows with less
+ * row). out may be x or residual, with that one's stride. 1 to 2^31 - 1 columns, rows with less
  * than 2^31 groups of 8 columns in all. */
 typedef struct irx_train_rows {
     size_t rows;

@@ -2492,6 +2492,8 @@ int irx_train_dropout(irx_device *device, const irx_train_rows *rows, void *stre
                 fail(IRX_INVALID_ARGUMENT, "strides must be multiples of 16 bytes, the width at least, and within range");
             *to[i] = (long long)strides[i];
         }
+        if ((r.out == r.x && a.os != a.xs) || (r.out == r.residual && a.os != a.rs))
+            fail(IRX_INVALID_ARGUMENT, "an input that is the output has its stride");
         icl4_device(device);
         CurrentDevice here(device);
         train_dropout(a, static_cast<hipStream_t>(stream));

@@ -96,6 +96,9 @@ def test_dropout_is_checked():
     refused("multiples of 16 bytes", call, 4, 12, Q, Q, element="f16")
     refused("within range", call, 4, 8, Q, Q, out_stride=1 << 40)
     refused("dropout needs a seed", call, 4, 8, Q, Q, dropped=1)
+    refused("an input that is the output", call, 4, 8, Q, Q, x_stride=16)
+    refused("an input that is the output", call, 4, 8, Q, Q + 64, residual=Q + 64, out_stride=16)
+    refused("needs a device", call, 4, 8, Q, Q + 64, residual=Q, x_stride=16)
     refused("needs a device", call, 1, 13, Q, Q)
     refused("needs a device", call, 4, 12, Q, Q, residual=Q, seed=Q, dropped=65535)
     with pytest.raises(ValueError, match="element must be one of"):
