@@ -382,6 +382,80 @@ def test_the_same_call_gives_the_same_bits(device, element):
         np.testing.assert_array_equal(x, y)
 
 
+@pytest.mark.parametrize("dropped", [0, 6554])
+@pytest.mark.parametrize("element", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("number", [np.inf, -np.inf, np.nan])
+def test_gradients_that_are_not_finite(device, number, element, dropped):
+    """One such number of the output's gradient: it shows in its query's gradient and in every key's, as a step that scales
+    its loss looks for, and other queries' stay: FP32's and FP16's powers may differ, by which 200 terms miss 2^-37 each."""
+    e, h, m, n = 1, 2, 70, 200
+    first = Case(device, e, h, h, m, n, element, dropped=dropped)
+    clean = first.run()
+    dout = first.dout.values.copy()
+    dout[0, 1, 41, 7] = number
+    got = Case(device, e, h, h, m, n, element, dropped=dropped, dout=dout).run()
+    dq, dk, dv = got[3:]
+    assert not np.isfinite(dq[0, 1, 41]).any()
+    assert not np.isfinite(dk[0, 1]).any() and not np.isfinite(dv[0, 1, :, 7]).any()
+    assert np.isfinite(dk[0, 0]).all() and np.isfinite(dv[0, 0]).all()
+    dq[0, 1, 41] = clean[3][0, 1, 41]
+    assert np.all(np.abs(dq - clean[3]) <= 2 * HALF[element] * np.abs(dq) + 2.0 ** -20 * np.abs(dq).max())
+    for x, y in zip(got[:3], clean[:3]):
+        np.testing.assert_array_equal(x, y)
+
+
+@pytest.mark.parametrize("element", ["f32", "bf16"])
+def test_two_calls_at_once(device, element):
+    """On two streams, with a workspace each: the results of one after the other."""
+    cases = [Case(device, 1, 4, 2, 200, 6000, element, dropped=6554), Case(device, 2, 4, 4, 33, 1500, element)]
+    alone = [case.run() for case in cases]
+    rt = hipmem.runtime()
+    streams = [ctypes.c_void_p(), ctypes.c_void_p()]
+    for s in streams:
+        assert rt.hipStreamCreate(ctypes.byref(s)) == 0
+    for _ in range(4):
+        for call in ("forward", "backward"):
+            for case, s in zip(cases, streams):
+                getattr(case, call)(s.value)
+    hipmem.synchronize()
+    for case, want in zip(cases, alone):
+        for x, y in zip(case.results(), want):
+            np.testing.assert_array_equal(x, y)
+    for s in streams:
+        assert rt.hipStreamDestroy(s) == 0
+
+
+def test_the_most_pairs(device):
+    """65,535 estimators of one head, of two queries and three rows."""
+    rng = np.random.default_rng(0)
+    e = 65535
+    lengths, keep = rng.integers(0, 4, e), rng.random((e, 3)) < 0.7
+    case = Case(device, e, 1, 1, 2, 3, "f32", "heads", rng.integers(0, 3, e), lengths, keep, 9000)
+    case.check(case.run())
+
+
+def test_the_most_rows(device):
+    """2^24 rows of keys that are 0: every weight is the same, and values of row number mod 16 have whole sums."""
+    n, e, h, m = 1 << 24, 1, 1, 3
+    shape = (e, h, h, m, n)
+    k = put(np.zeros(n * 64, np.uint16))
+    v = put(np.tile(np.repeat(np.arange(16, dtype=np.float16), 64).view(np.uint16), n // 16))
+    q = put(encode(normal((e, h, m, 64), 1), "f16"))
+    out, stats, lse = put(np.zeros((m, 64), np.float16)), put(np.zeros((m, 2), np.float32)), put(np.zeros(m, np.float32))
+    training.attention(device, shape, q, k, v, out, element="f16", stats=stats, lse=lse, **workspace(device, shape, "f16", False))
+    dout = put(np.full((m, 64), 16.0, np.float16))
+    dq = put(np.full((m, 64), 1, np.float16))
+    dk, dv = hipmem.DeviceArray((n * 64,), np.uint16), hipmem.DeviceArray((n * 64,), np.uint16)
+    training.attention_backward(device, shape, q, k, v, out, stats, dout, dq=dq, dk=dk, dv=dv, element="f16",
+                                **workspace(device, shape, "f16", True))
+    hipmem.synchronize()
+    assert np.all(out.to_host() == 7.5) and np.all(stats.to_host() == [0, n])
+    np.testing.assert_allclose(lse.to_host(), np.log(n), rtol=2.0 ** -22)
+    assert np.all(dq.to_host() == 0)  # the keys are 0
+    # 3 * 16 / 2^24 for every number of dv.
+    assert np.all(dv.to_host().view(np.float16) == np.float16(48.0 / n))
+
+
 def test_shared_inputs_have_gradients_of_their_own(device):
     """Keys and values with strides of 0 over heads and estimators."""
     k, v = normal((1, 1, 150, 64), 1), normal((1, 1, 150, 64), 2)
