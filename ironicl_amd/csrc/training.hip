@@ -300,8 +300,9 @@ __device__ __forceinline__ bool kept16(const u32x4 &w, int j, unsigned line) {
     return (j & 1 ? w[j >> 1] : w[j >> 1] << 16) >= line;
 }
 
-// Eight 16-bit numbers without those that a call drops, its words with every value's highest bit flipped. The 16-bit values are compared two at a time, as signed ones: a
-// saturated difference's sign, over the half, is the mask (3.5 instructions a pair, with comparisons and selections 5).
+// Eight 16-bit numbers without those that a call drops. `z` holds its words with every value's highest bit flipped, so that
+// two values at a time are compared as signed ones: a saturated difference's sign, over the half, is the mask (3.5
+// instructions a pair, with comparisons and selections 5).
 constexpr unsigned kFlip = 0x80008000u;
 template <int EL>
 __device__ __forceinline__ V8<EL> drop8(V8<EL> x, const u32x4 &z, unsigned line) {
@@ -360,9 +361,9 @@ struct Args {
     long long gs[3], dqs[3], dks[3], dvs[3];
     f32x4 *record;
     // plans
-    int q_tiles, q_splits, q_chunk;     // units of 128 queries; a split's key tiles
-    int k_tiles, k_splits, k_chunk;     // units of 128 keys; a split's query tiles
-    int q_blocks;                       // workgroups on queries, before those on keys
+    int q_tiles, q_splits, q_chunk;  // units of queries; a split's key tiles
+    int k_tiles, k_splits, k_chunk;  // units of 128 keys; a split's query tiles
+    int q_blocks;                    // workgroups on queries, before those on keys
     float *q_part, *k_part;
 };
 
@@ -392,10 +393,12 @@ __device__ __forceinline__ void load_tile(Tile<EL> &t, const void *base, const l
 #pragma unroll
     for (int i = 0; i < 512 / NT; ++i) {
         const int first = 8 * (wave + i * (NT / 64)), row = first + lane / 8;
-        const unsigned short *from = static_cast<const unsigned short *>(base) + at(s, e, h, min(row0 + row, rows - 1)) + 8 * ((lane & 7) ^ swizzle(row));
+        const long long place = at(s, e, h, min(row0 + row, rows - 1)) + 8 * ((lane & 7) ^ swizzle(row));
+        const unsigned short *from = static_cast<const unsigned short *>(base) + place;
         __builtin_amdgcn_global_load_lds(from, (__attribute__((address_space(3))) void *)&t.p[0][first * 64], 16, 0, 0);
     }
 }
+
 // Rows whose bit is not set become zeros, whatever they hold.
 template <int EL, int NT>
 __device__ __forceinline__ void clear_rows(Tile<EL> &t, unsigned long long some) {
@@ -533,7 +536,13 @@ constexpr int kNone = -1000;  // a lane's power before its first term
 
 // 32 WQ queries to a workgroup, 32 to a wave; keys and values pass through LDS in tiles of 64, and where WK is 2 a wave
 // takes 32 of each. S^T = K Q^T leaves a query's scores in one lane (and its other half), in the order in which the next
-// product takes them.
+// product takes them. FP32 tiles are loaded into registers while the last is worked on and become pairs on their way to LDS;
+// 16-bit ones go straight to LDS, the next tile's while one is worked on (so done, with two barriers a tile in place of one,
+// FP32's took as long).
+// 512 FP32 queries over 50,000 rows of 8 heads: 204 us, 257 TFLOP/s, the matrix cores 36% busy and the vector unit 54%; with
+// two waves a SIMD they overlap little (a wave alone issues a vector instruction every seven cycles), and a third wave's
+// registers are not there. 10,007 BF16 rows over themselves with dropout: 411 us, the vector unit 78% busy, half of it
+// with random numbers.
 constexpr int forward_waves(int element, int wq, int wk) {  // of a SIMD: what registers leave room for
     return element == kTrainF32 ? 2 : wq * wk;
 }
@@ -749,9 +758,10 @@ __global__ __launch_bounds__(64 * WQ * WK, forward_waves(EL, WQ, WK)) void train
     }
 }
 
-// One to four rows (queries of the heads that share a key head) against their keys, for which the matrix cores' 32 columns
+// One to eight rows (queries of the heads that share a key head) against their keys, for which the matrix cores' 32 columns
 // stand empty and reading keys and values is all there is: FP32 sums, LK lanes to a key (16 bytes each), eight keys of one
-// call of random numbers to a group of lanes, a wave's 64 keys (FP32: 32) in flight at once.
+// call of random numbers to a group of lanes, a wave's 64 keys (FP32: 32) in flight at once. One query of 8 FP32 heads over
+// 50,000 rows: 31 us, 6.6 TB/s, and 5 for the joining of 32 splits.
 template <int EL, int NQ, bool DROP>
 __global__ __launch_bounds__(256) void train_rows_kernel(const Args a) {
     constexpr int D = EL == kTrainF32 ? 4 : 8, LK = 64 / D, GROUPS = 64 / LK;  // dims of a lane; groups of a wave
@@ -911,7 +921,8 @@ __global__ __launch_bounds__(256) void train_rows_kernel(const Args a) {
     }
 }
 
-// Joins the splits of a query: sixteen lanes to a row's numbers, and W groups of them to its splits.
+// Joins the splits of a query: sixteen lanes to a row's numbers, and W groups of them to its splits (one group after another
+// waits for memory each time: 64 splits of 8 rows took 27 us by one group and 5 by sixteen).
 template <int EL, int W>
 __global__ __launch_bounds__(256) void train_merge_kernel(const Args a) {
     const long long rows = (long long)a.pairs * a.q_rows;
@@ -960,6 +971,14 @@ __global__ __launch_bounds__(256) void train_merge_kernel(const Args a) {
 }
 
 // ---- backward ----
+
+// The two sides of the backward pass are workgroups of one launch, which fill its end for each other (two launches: 987 us
+// in place of 868 for 10,007 BF16 rows). Both compute the scores and dP: seven products in place of five. Five would take
+// either atomic additions to dq, whose order changes results, or dq's part of every 128 keys through memory, written and
+// read (10,007 rows: 1.6 GB each way, 0.6 ms; the two products take 0.2).
+// 10,007 BF16 rows: 780 to 814 us, 630 TFLOP/s counted as five products, 880 as seven; the matrix cores 46% busy, the vector
+// unit 54%. 512 FP32 queries over 50,000 rows: 656 us, 200 (three FP16 products each: 840 as seven); 40% and 52%. Two
+// masked tables of 12,345 rows, FP16 with dropout: 260; 16% and 52%, random numbers and selections.
 
 // What the backward pass needs of each query: {r, 1 / s, delta, r + log2 s}; r is +inf (all weights 0) for one that attends to
 // nothing or lies past the length. Sixteen lanes to a row.
@@ -1208,7 +1227,8 @@ __device__ __forceinline__ void keys_backward(const Args &a, Streamed<EL> &lds, 
             }
             unsigned kept = ~0u;
             if constexpr (DROP)
-                kept = kept_words(2 * (tile * 8 + 2 * wave), row0 + 32 * b + (lane & 31), e * a.heads + h, a.site, a.line, seed, half) >> (4 * half);
+                kept = kept_words(16 * tile + 4 * wave, row0 + 32 * b + (lane & 31), e * a.heads + h, a.site, a.line, seed, half) >>
+                       (4 * half);
             float most_p = 0.f, most_ds = 0.f;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -1371,7 +1391,7 @@ __global__ __launch_bounds__(256, EL == kTrainF32 || DROP ? 2 : 3) void train_ba
         keys_backward<EL, DROP>(a, lds, blockIdx.x - a.q_blocks);
 }
 
-// Sums the splits' parts, in order. Rows of dq, then of dk, then of dv; sixteen lanes to a row.
+// Sums the splits' parts, in order, so that results hang on nothing else. Rows of dq, then of dk, then of dv; sixteen lanes to a row.
 template <int EL>
 __global__ __launch_bounds__(256) void train_sum_kernel(const Args a) {
     const long long q_rows = a.q_splits > 1 ? (long long)a.pairs * a.q_rows : 0;
@@ -1416,7 +1436,8 @@ struct DropArgs {
     float w;
 };
 
-// Eight adjacent numbers of a row to a thread.
+// Eight adjacent numbers of a row, one call of random numbers, to a thread; bound by memory: 200,000 x 1,024 FP32 numbers 278
+// us, 5.9 TB/s.
 template <int EL>
 __global__ __launch_bounds__(256) void train_dropout_kernel(const DropArgs a) {
     const long long g = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -1507,7 +1528,8 @@ Plan plan(const TrainShape &s, int element, bool backward, bool uneven, int comp
     p.record = backward ? rows * 16 : 0;
     p.q_part = p.q_splits > 1 ? (size_t)p.q_splits * rows * (backward ? 256 : 264) : 0;
     p.k_part = p.k_splits > 1 ? (size_t)p.k_splits * owners * s.rows * 512 : 0;
-    p.blocks = (double)(p.q_unit <= 8 ? owners : pairs * p.q_tiles) * p.q_splits + (backward ? (double)owners * p.k_tiles * p.k_splits : 0.0);
+    p.blocks = (double)(p.q_unit <= 8 ? owners : pairs * p.q_tiles) * p.q_splits;
+    if (backward) p.blocks += (double)owners * p.k_tiles * p.k_splits;
     return p;
 }
 
@@ -1625,8 +1647,9 @@ size_t train_workspace(const TrainShape &s, int element, bool backward, int comp
 bool train_fits(const TrainShape &s, int element, bool backward, int compute_units) {
     // 256 work-items to a workgroup, less than 2^32 in a launch.
     const double rows = (double)s.estimators * std::max((double)s.heads * s.q_rows, 2.0 * s.kv_heads * s.rows);
-    const double blocks = std::max(plan(s, element, backward, false, compute_units).blocks, plan(s, element, backward, true, compute_units).blocks);
-    return blocks < 16777216.0 && rows < 134217728.0;
+    for (const bool uneven : {false, true})
+        if (plan(s, element, backward, uneven, compute_units).blocks >= 16777216.0) return false;
+    return rows < 134217728.0;
 }
 
 void train_attention(const TrainInputs &a, const TrainForward &f, int compute_units, hipStream_t stream) {
