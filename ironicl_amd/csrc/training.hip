@@ -365,6 +365,7 @@ struct Args {
     int k_tiles, k_splits, k_chunk;  // units of 128 keys; a split's query tiles
     int q_blocks;                    // workgroups on queries, before those on keys
     float *q_part, *k_part;
+    int keys_last;  // 1: the keys' side walks further
 };
 
 __device__ __forceinline__ long long at(const long long *s, int e, int h, int row) {
@@ -1385,6 +1386,8 @@ __device__ __forceinline__ void keys_backward(const Args &a, Streamed<EL> &lds, 
 template <int EL, bool DROP>
 __global__ __launch_bounds__(256, EL == kTrainF32 || DROP ? 2 : 3) void train_backward_kernel(const Args a) {
     __shared__ Streamed<EL> lds;
+    // The side that walks further goes ahead of the other where both have instructions to issue.
+    if ((blockIdx.x < (unsigned)a.q_blocks) != a.keys_last) __builtin_amdgcn_s_setprio(1);
     if (blockIdx.x < (unsigned)a.q_blocks)
         queries_backward<EL, DROP>(a, lds, blockIdx.x);
     else
@@ -1485,6 +1488,29 @@ int splits_of(double length, double target, long long tiles) {
     return (int)std::min<long long>(std::max(1ll, std::llround(length / target)), std::min(tiles, 128ll));
 }
 
+// Splits of `units` 128-query units over `words` key tiles: as many as take the least time, of those with which the launch is
+// 1, 2, .. 16 workgroups to a compute unit. A workgroup's tile takes so many us beside 0, 1, .. others on its compute unit,
+// and so does the last, partly filled round (10,007 FP32 queries over as many rows in 1 / 2 / 3 / 4 / 5 splits: 959, 802, 822,
+// 792, 829 us; 1,024 over 1,024: 49, 33, 29, 26, 26, in 16 splits 41; four tables of 1,024 BF16 rows: 24, 31, 32, 33, 33). Joining
+// writes and reads every split's sums.
+int splits_of_rounds(double units, int words, double rows, bool single, int compute_units) {
+    static constexpr double kTileUs[2][4] = {{1.0, 1.6, 2.1, 2.7}, {2.45, 3.83, 0.0, 0.0}};
+    const int most = single ? 2 : 4;
+    const double *us = kTileUs[single];
+    double best = INFINITY;
+    int splits = 1;
+    for (int m = 0, last = 0; m <= 16; ++m) {
+        const int s = std::min((int)std::max(m * compute_units / units, 1.0), std::min(words, 128));
+        if (s == last) continue;
+        last = s;
+        const double tiles = (words + s - 1) / s, blocks = units * s / compute_units, rounds = std::floor(blocks / most);
+        const int left = (int)std::ceil(blocks - most * rounds);
+        const double time = tiles * (rounds * us[most - 1] + (left ? us[left - 1] : 0.0)) + (s > 1 ? 2.5 + rows * s * 528 / 6e6 : 0.0);
+        if (time < best) best = time, splits = s;
+    }
+    return splits;
+}
+
 // `uneven`: estimators' lengths or masks are given, which only the device knows.
 Plan plan(const TrainShape &s, int element, bool backward, bool uneven, int compute_units) {
     Plan p{};
@@ -1517,7 +1543,9 @@ Plan plan(const TrainShape &s, int element, bool backward, bool uneven, int comp
         p.q_splits = splits_of((double)words, std::max((double)owners * words / compute_units, 4.0), words);
         p.k_splits = 1;
     } else {
-        p.q_splits = splits_of((double)words, std::max(pairs * p.q_tiles * words / slots, 1.0), words);
+        p.q_splits = p.q_unit == 128
+                         ? splits_of_rounds((double)pairs * p.q_tiles, (int)words, (double)pairs * s.q_rows, single, compute_units)
+                         : splits_of((double)words, std::max(pairs * p.q_tiles * words / slots, 1.0), words);
         p.k_splits = 1;
     }
     p.q_chunk = (int)ceil_div(words, p.q_splits);
@@ -1612,6 +1640,7 @@ void backward(const TrainInputs &a, const TrainBackward &b, const Plan &p, hipSt
         hipLaunchKernelGGL(train_record_kernel<EL>, dim3(ceil_div(rows, 16)), dim3(256), 0, stream, k);
         IRX_HIP(hipGetLastError());
     }
+    k.keys_last = 4 * p.k_chunk > 3 * p.q_chunk;
     k.q_blocks = b.dq ? (int)((size_t)k.pairs * p.q_tiles * p.q_splits) : 0;
     const size_t k_blocks = b.dk ? (size_t)a.shape.estimators * a.shape.kv_heads * p.k_tiles * p.k_splits : 0;
     {
