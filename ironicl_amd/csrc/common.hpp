@@ -546,9 +546,8 @@ struct TrainRows {
     long long xs, rs, os;
     TrainDrop drop;
 };
-size_t train_workspace(const TrainShape &s, int element, bool backward, int compute_units);
-// Whether a call's launches hold it.
-bool train_fits(const TrainShape &s, int element, bool backward, int compute_units);
+// Whether a call's launches hold it, and the bytes of workspace that it takes.
+bool train_needs(const TrainShape &s, int element, bool backward, int compute_units, size_t *workspace);
 void train_attention(const TrainInputs &a, const TrainForward &f, int compute_units, hipStream_t stream);
 void train_backward(const TrainInputs &a, const TrainBackward &b, int compute_units, hipStream_t stream);
 void train_dropout(const TrainRows &a, hipStream_t stream);

@@ -2421,8 +2421,8 @@ int irx_icl4_attention(irx_device *device, const irx_icl4_queries *queries, cons
 size_t irx_train_workspace_bytes(irx_device *device, const irx_train_shape *shape, int element, int backward) {
     if (!device || !train_shape_ok(shape) || element < IRX_ELEMENT_F32 || element > IRX_ELEMENT_BF16) return 0;
     const TrainShape s = train_shape(*shape);
-    if (!train_fits(s, element, backward, device->compute_units)) return 0;
-    return train_workspace(s, element, backward, device->compute_units);
+    size_t bytes;
+    return train_needs(s, element, backward, device->compute_units, &bytes) ? bytes : 0;
 }
 
 int irx_train_attention(irx_device *device, const irx_train_inputs *inputs, void *out, const irx_strides *out_strides,
@@ -2437,8 +2437,9 @@ int irx_train_attention(irx_device *device, const irx_train_inputs *inputs, void
         icl4_aligned(stats, 8, "stats");
         icl4_aligned(lse, 4, "lse");
         icl4_device(device);
-        if (!train_fits(a.shape, a.element, false, device->compute_units)) fail(IRX_INVALID_ARGUMENT, "too many rows for one call");
-        icl4_workspace(workspace, workspace_bytes, train_workspace(a.shape, a.element, false, device->compute_units));
+        size_t needed;
+        if (!train_needs(a.shape, a.element, false, device->compute_units, &needed)) fail(IRX_INVALID_ARGUMENT, "too many rows for one call");
+        icl4_workspace(workspace, workspace_bytes, needed);
         CurrentDevice here(device);
         train_attention(a, f, device->compute_units, static_cast<hipStream_t>(stream));
     });
@@ -2466,8 +2467,9 @@ int irx_train_attention_backward(irx_device *device, const irx_train_inputs *inp
             train_tensor(s, s.kv_heads, s.rows, a.element, g.dv, "the values' gradient", g.dv_strides, b.dvs, true);
         }
         icl4_device(device);
-        if (!train_fits(a.shape, a.element, true, device->compute_units)) fail(IRX_INVALID_ARGUMENT, "too many rows for one call");
-        icl4_workspace(workspace, workspace_bytes, train_workspace(a.shape, a.element, true, device->compute_units));
+        size_t needed;
+        if (!train_needs(a.shape, a.element, true, device->compute_units, &needed)) fail(IRX_INVALID_ARGUMENT, "too many rows for one call");
+        icl4_workspace(workspace, workspace_bytes, needed);
         CurrentDevice here(device);
         train_backward(a, b, device->compute_units, static_cast<hipStream_t>(stream));
     });

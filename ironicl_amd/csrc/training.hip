@@ -1511,8 +1511,71 @@ int splits_of_rounds(double units, int words, double rows, bool single, int comp
     return splits;
 }
 
-// `uneven`: estimators' lengths or masks are given, which only the device knows.
-Plan plan(const TrainShape &s, int element, bool backward, bool uneven, int compute_units) {
+// What a compute unit takes for `first` workgroups that each take a and then `second` of b (the last of either may be a part
+// of one), `most` of them at once, where us[0], us[1], .. pass for a unit of that with none, one, .. beside it.
+double us_of_workgroups(double first, double a, double second, double b, int most, const double *us) {
+    double left[3], time = 0.0;
+    for (int n = 0;;) {
+        for (; n < most && (first > 0.0 || second > 0.0); ++n) {
+            double &of = first > 0.0 ? first : second;
+            left[n] = (&of == &first ? a : b) * std::min(of, 1.0);
+            of -= 1.0;
+        }
+        if (!n) return time;
+        const double least = *std::min_element(left, left + n);
+        time += least * us[n - 1];
+        int kept = 0;
+        for (int i = 0; i < n; ++i)
+            if (left[i] - least > 1e-9) left[kept++] = left[i] - least;
+        n = kept;
+    }
+}
+
+// What a tile of keys costs 128 queries and a tile of queries 128 keys, and a workgroup's start.
+constexpr double kQueriesCost = 3.0, kKeysCost = 5.5, kStartCost = 1.2;
+
+// The backward pass' splits: as many as take the least time, of those with which the launch has 1, 2, 3 or 4 workgroups of as
+// many products to a compute unit; more only where that saves a fortieth. The costs are fitted to 64 shapes with ten choices
+// each, of which these are 1% from the best on average and 9% at most (in us, with as many as let no workgroup walk further than
+// half a compute unit's share, and these: 3,000 FP32 queries over as many rows 272 and 244, 5,000 FP16 with dropout 421 and 337,
+// four tables of 300 FP16 rows 29 and 23).
+void backward_splits(Plan &p, double pairs, double owners, int words, int q_words, const TrainShape &s, int element, bool drop,
+                     int compute_units) {
+    static constexpr double kUs[2][2][3] = {{{0.39, 0.52, 0.87}, {0.74, 1.0, 0.0}}, {{1.05, 1.43, 0.0}, {1.85, 2.5, 0.0}}};
+    const bool single = element == kTrainF32;
+    const int most = single || drop ? 2 : 3;
+    const double *us = kUs[single][drop], q_units = pairs * p.q_tiles, k_units = owners * p.k_tiles;
+    const double all = 3.0 * q_units * words + 4.0 * k_units * q_words;  // products
+    double best = INFINITY;
+    // Where there are many workgroups anyway, no one walks further than half a compute unit's share.
+    const bool many = q_units + k_units > 20.0 * compute_units;
+    for (int m = many ? 2 : 0; m <= (many ? 2 : 4); ++m) {
+        const double share = m ? all / (m * compute_units) : INFINITY;
+        const int q_chunk = (int)ceil_div(words, splits_of(3.0 * words, share, words));
+        const int k_chunk = (int)ceil_div(q_words, splits_of(4.0 * q_words, share, q_words));
+        const int q_splits = (int)ceil_div(words, q_chunk), k_splits = (int)ceil_div(q_words, k_chunk);
+        const double q_blocks = q_units * q_splits / compute_units, k_blocks = k_units * k_splits / compute_units;
+        const double blocks = q_blocks + k_blocks;
+        if (many) {
+            p.q_splits = q_splits, p.k_splits = k_splits;
+            break;
+        }
+        const double q_cost = kQueriesCost * q_chunk + kStartCost, k_cost = kKeysCost * k_chunk + kStartCost;
+        // The compute unit with the most to do has as many as it can of those that take longer; the others level out where they
+        // are many.
+        const double longer = std::ceil(k_cost >= q_cost ? k_blocks : q_blocks), rest = std::max(blocks - longer, 0.0);
+        const double others = rest > 2.0 ? rest : std::ceil(rest);
+        const double q_jobs = k_cost >= q_cost ? others : longer, k_jobs = k_cost >= q_cost ? longer : others;
+        double sums = q_splits > 1 ? pairs * s.q_rows * q_splits * 512.0 : 0.0;
+        if (k_splits > 1) sums += owners * s.rows * k_splits * 1024.0;
+        double time = us_of_workgroups(q_jobs, q_cost, k_jobs, k_cost, most, us);
+        if (sums > 0.0) time += 3.0 + sums / 4.3e6;
+        if (time < 0.978 * best) best = time, p.q_splits = q_splits, p.k_splits = k_splits;
+    }
+}
+
+// `uneven`: estimators' lengths or masks are given, which only the device knows. `drop`: weights are dropped.
+Plan plan(const TrainShape &s, int element, bool backward, bool uneven, bool drop, int compute_units) {
     Plan p{};
     const long long pairs = (long long)s.estimators * s.heads, owners = (long long)s.estimators * s.kv_heads;
     const long long words = (s.rows + 63) / 64, q_words = (s.q_rows + 63) / 64, group = s.heads / s.kv_heads;
@@ -1531,13 +1594,16 @@ Plan plan(const TrainShape &s, int element, bool backward, bool uneven, int comp
     p.q_tiles = (int)ceil_div(s.q_rows, p.q_unit);
     p.k_tiles = (int)ceil_div(s.rows, 128);
     if (backward) {
-        // A tile of keys costs a unit of queries three products, a tile of queries a unit of keys four. No workgroup walks
-        // further than its share of all the work, or, where some find little to do, a third of that (two masked tables of 12,345
-        // rows, FP16: 320 us with the share, 272 with a third; four even tables of 1,024 rows, FP32: 163 and 190).
-        const double all = 3.0 * pairs * p.q_tiles * words + 4.0 * owners * p.k_tiles * group * q_words;
-        const double share = std::max(all / (uneven ? 3.0 * slots : slots), 6.0);
-        p.q_splits = splits_of(3.0 * words, share, words);
-        p.k_splits = splits_of(4.0 * group * q_words, share, group * q_words);
+        if (uneven) {
+            // No workgroup walks further than a third of a compute unit's share, for some find little to do (two masked tables of
+            // 12,345 rows, FP16: 320 us with the share, 272 with a third).
+            const double all = 3.0 * pairs * p.q_tiles * words + 4.0 * owners * p.k_tiles * group * q_words;
+            const double share = std::max(all / (3.0 * slots), 6.0);
+            p.q_splits = splits_of(3.0 * words, share, words);
+            p.k_splits = splits_of(4.0 * group * q_words, share, group * q_words);
+        } else {
+            backward_splits(p, (double)pairs, (double)owners, (int)words, (int)(group * q_words), s, element, drop, compute_units);
+        }
     } else if (p.q_unit <= 8) {
         // A wave takes a tile at a time.
         p.q_splits = splits_of((double)words, std::max((double)owners * words / compute_units, 4.0), words);
@@ -1640,7 +1706,7 @@ void backward(const TrainInputs &a, const TrainBackward &b, const Plan &p, hipSt
         hipLaunchKernelGGL(train_record_kernel<EL>, dim3(ceil_div(rows, 16)), dim3(256), 0, stream, k);
         IRX_HIP(hipGetLastError());
     }
-    k.keys_last = 4 * p.k_chunk > 3 * p.q_chunk;
+    k.keys_last = kKeysCost * p.k_chunk > kQueriesCost * p.q_chunk;
     k.q_blocks = b.dq ? (int)((size_t)k.pairs * p.q_tiles * p.q_splits) : 0;
     const size_t k_blocks = b.dk ? (size_t)a.shape.estimators * a.shape.kv_heads * p.k_tiles * p.k_splits : 0;
     {
@@ -1664,25 +1730,21 @@ void backward(const TrainInputs &a, const TrainBackward &b, const Plan &p, hipSt
 
 }  // namespace
 
-size_t train_workspace(const TrainShape &s, int element, bool backward, int compute_units) {
-    size_t most = 0;
-    for (const bool uneven : {false, true}) {
-        const Plan p = plan(s, element, backward, uneven, compute_units);
-        most = std::max(most, round16(p.record) + round16(p.q_part) + round16(p.k_part));
-    }
-    return most;
-}
-
-bool train_fits(const TrainShape &s, int element, bool backward, int compute_units) {
+bool train_needs(const TrainShape &s, int element, bool backward, int compute_units, size_t *workspace) {
     // 256 work-items to a workgroup, less than 2^32 in a launch.
-    const double rows = (double)s.estimators * std::max((double)s.heads * s.q_rows, 2.0 * s.kv_heads * s.rows);
-    for (const bool uneven : {false, true})
-        if (plan(s, element, backward, uneven, compute_units).blocks >= 16777216.0) return false;
-    return rows < 134217728.0;
+    *workspace = 0;
+    if ((double)s.estimators * std::max((double)s.heads * s.q_rows, 2.0 * s.kv_heads * s.rows) >= 134217728.0) return false;
+    // The workspace serves every plan of the shape: with lengths or masks, and else without dropout and with it.
+    for (int i = 0; i < (backward ? 3 : 1); ++i) {
+        const Plan p = plan(s, element, backward, i == 1, i == 2, compute_units);
+        if (p.blocks >= 16777216.0) return false;
+        *workspace = std::max(*workspace, round16(p.record) + round16(p.q_part) + round16(p.k_part));
+    }
+    return true;
 }
 
 void train_attention(const TrainInputs &a, const TrainForward &f, int compute_units, hipStream_t stream) {
-    const Plan p = plan(a.shape, a.element, false, false, compute_units);
+    const Plan p = plan(a.shape, a.element, false, false, false, compute_units);
     if (a.element == kTrainF32)
         forward<kTrainF32>(a, f, p, stream);
     else if (a.element == kTrainF16)
@@ -1692,7 +1754,7 @@ void train_attention(const TrainInputs &a, const TrainForward &f, int compute_un
 }
 
 void train_backward(const TrainInputs &a, const TrainBackward &b, int compute_units, hipStream_t stream) {
-    const Plan p = plan(a.shape, a.element, true, a.q_lengths || a.lengths || a.keep, compute_units);
+    const Plan p = plan(a.shape, a.element, true, a.q_lengths || a.lengths || a.keep, a.drop.dropped, compute_units);
     if (a.element == kTrainF32)
         backward<kTrainF32>(a, b, p, stream);
     else if (a.element == kTrainF16)
