@@ -1538,23 +1538,27 @@ constexpr double kQueriesCost = 3.0, kKeysCost = 5.5, kStartCost = 1.2;
 // many products to a compute unit; more only where that saves a fortieth. The costs are fitted to 64 shapes with ten choices
 // each, of which these are 1% from the best on average and 9% at most (in us, with as many as let no workgroup walk further than
 // half a compute unit's share, and these: 3,000 FP32 queries over as many rows 272 and 244, 5,000 FP16 with dropout 421 and 337,
-// four tables of 300 FP16 rows 29 and 23).
-void backward_splits(Plan &p, double pairs, double owners, int words, int q_words, const TrainShape &s, int element, bool drop,
-                     int compute_units) {
+// four tables of 300 FP16 rows 29 and 23). Where only the device knows how much there is to do, as if half the workgroups had
+// nothing, the others everything (for ten masked shapes 5% from the best on average and 16% at most; with a third of a share as
+// the longest walk 14% and 37%: four tables of 1,024 FP32 rows with dropout 154 us, so 143, of BF16 rows without 61 and 47).
+void backward_splits(Plan &p, double pairs, double owners, int words, int q_words, const TrainShape &s, int element, bool uneven,
+                     bool drop, int compute_units) {
     static constexpr double kUs[2][2][3] = {{{0.39, 0.52, 0.87}, {0.74, 1.0, 0.0}}, {{1.05, 1.43, 0.0}, {1.85, 2.5, 0.0}}};
     const bool single = element == kTrainF32;
     const int most = single || drop ? 2 : 3;
     const double *us = kUs[single][drop], q_units = pairs * p.q_tiles, k_units = owners * p.k_tiles;
     const double all = 3.0 * q_units * words + 4.0 * k_units * q_words;  // products
     double best = INFINITY;
+    const double full = uneven ? 0.5 : 1.0;
+    const int last = uneven ? 8 : 4;
     // Where there are many workgroups anyway, no one walks further than half a compute unit's share.
     const bool many = q_units + k_units > 20.0 * compute_units;
-    for (int m = many ? 2 : 0; m <= (many ? 2 : 4); ++m) {
+    for (int m = many ? last / 2 : 0; m <= last; ++m) {
         const double share = m ? all / (m * compute_units) : INFINITY;
         const int q_chunk = (int)ceil_div(words, splits_of(3.0 * words, share, words));
         const int k_chunk = (int)ceil_div(q_words, splits_of(4.0 * q_words, share, q_words));
         const int q_splits = (int)ceil_div(words, q_chunk), k_splits = (int)ceil_div(q_words, k_chunk);
-        const double q_blocks = q_units * q_splits / compute_units, k_blocks = k_units * k_splits / compute_units;
+        const double q_blocks = full * q_units * q_splits / compute_units, k_blocks = full * k_units * k_splits / compute_units;
         const double blocks = q_blocks + k_blocks;
         if (many) {
             p.q_splits = q_splits, p.k_splits = k_splits;
@@ -1569,7 +1573,7 @@ void backward_splits(Plan &p, double pairs, double owners, int words, int q_word
         double sums = q_splits > 1 ? pairs * s.q_rows * q_splits * 512.0 : 0.0;
         if (k_splits > 1) sums += owners * s.rows * k_splits * 1024.0;
         double time = us_of_workgroups(q_jobs, q_cost, k_jobs, k_cost, most, us);
-        if (sums > 0.0) time += 3.0 + sums / 4.3e6;
+        if (sums > 0.0) time += 3.0 + full * sums / 4.3e6;
         if (time < 0.978 * best) best = time, p.q_splits = q_splits, p.k_splits = k_splits;
     }
 }
@@ -1582,7 +1586,7 @@ Plan plan(const TrainShape &s, int element, bool backward, bool uneven, bool dro
     p.q_unit = backward || s.q_rows > 64 ? 128 : s.q_rows > 32 ? 64 : 32;
     // Workgroups that a launch should have at once: what registers leave room for on the compute units (with two of 128 threads
     // on each, 32 FP32 queries over 50,000 rows took 59 us in place of 47).
-    const double slots = (backward || (element == kTrainF32 && p.q_unit > 32) ? 2.0 : 4.0) * compute_units;
+    const double slots = (element == kTrainF32 && p.q_unit > 32 ? 2.0 : 4.0) * compute_units;
     // Few rows go one key at a time where that is faster. In us, so and by the matrix cores, over 50,000 rows: 8 FP32 heads
     // of 1 / 2 / 4 / 8 queries 37.9 / 40.1 / 42.8 / 53.1 and 44.6 / 45.4 / 45.2 / 45.8; 8 over 2 key heads, of 1 / 2 queries
     // 21.0 / 27.6 and 45; 8 BF16 heads of 1 / 2 / 4 queries 24.4 / 27.0 / 30.1 and 26.1 / 26.3 / 26.8, over 2 key heads, of 1
@@ -1594,16 +1598,8 @@ Plan plan(const TrainShape &s, int element, bool backward, bool uneven, bool dro
     p.q_tiles = (int)ceil_div(s.q_rows, p.q_unit);
     p.k_tiles = (int)ceil_div(s.rows, 128);
     if (backward) {
-        if (uneven) {
-            // No workgroup walks further than a third of a compute unit's share, for some find little to do (two masked tables of
-            // 12,345 rows, FP16: 320 us with the share, 272 with a third).
-            const double all = 3.0 * pairs * p.q_tiles * words + 4.0 * owners * p.k_tiles * group * q_words;
-            const double share = std::max(all / (3.0 * slots), 6.0);
-            p.q_splits = splits_of(3.0 * words, share, words);
-            p.k_splits = splits_of(4.0 * group * q_words, share, group * q_words);
-        } else {
-            backward_splits(p, (double)pairs, (double)owners, (int)words, (int)(group * q_words), s, element, drop, compute_units);
-        }
+        backward_splits(p, (double)pairs, (double)owners, (int)words, (int)(group * q_words), s, element, uneven, drop,
+                        compute_units);
     } else if (p.q_unit <= 8) {
         // A wave takes a tile at a time.
         p.q_splits = splits_of((double)words, std::max((double)owners * words / compute_units, 4.0), words);
@@ -1734,9 +1730,9 @@ bool train_needs(const TrainShape &s, int element, bool backward, int compute_un
     // 256 work-items to a workgroup, less than 2^32 in a launch.
     *workspace = 0;
     if ((double)s.estimators * std::max((double)s.heads * s.q_rows, 2.0 * s.kv_heads * s.rows) >= 134217728.0) return false;
-    // The workspace serves every plan of the shape: with lengths or masks, and else without dropout and with it.
-    for (int i = 0; i < (backward ? 3 : 1); ++i) {
-        const Plan p = plan(s, element, backward, i == 1, i == 2, compute_units);
+    // The workspace serves every plan of the shape: with lengths or masks and without, with dropout and without.
+    for (int i = 0; i < (backward ? 4 : 1); ++i) {
+        const Plan p = plan(s, element, backward, i & 1, i & 2, compute_units);
         if (p.blocks >= 16777216.0) return false;
         *workspace = std::max(*workspace, round16(p.record) + round16(p.q_part) + round16(p.k_part));
     }
