@@ -1492,8 +1492,10 @@ int splits_of(double length, double target, long long tiles) {
 // 1, 2, .. 16 workgroups to a compute unit. A workgroup's tile takes so many us beside 0, 1, .. others on its compute unit,
 // and so does the last, partly filled round (10,007 FP32 queries over as many rows in 1 / 2 / 3 / 4 / 5 splits: 959, 802, 822,
 // 792, 829 us; 1,024 over 1,024: 49, 33, 29, 26, 26, in 16 splits 41; four tables of 1,024 BF16 rows: 24, 31, 32, 33, 33). Joining
-// writes and reads every split's sums.
-int splits_of_rounds(double units, int words, double rows, bool single, int compute_units) {
+// writes and reads every split's sums. Where only the device knows how much there is to do, the sum of two times: as if every
+// workgroup had everything, and as if half of them had nothing (512 FP32 queries over four masked tables of 20,000 rows: 260 us
+// by the first alone, 234 so; of twelve masked shapes 3% and 6% from the best on average).
+int splits_of_rounds(double units, int words, double rows, bool single, bool uneven, int compute_units) {
     static constexpr double kTileUs[2][4] = {{1.0, 1.6, 2.1, 2.7}, {2.45, 3.83, 0.0, 0.0}};
     const int most = single ? 2 : 4;
     const double *us = kTileUs[single];
@@ -1503,9 +1505,15 @@ int splits_of_rounds(double units, int words, double rows, bool single, int comp
         const int s = std::min((int)std::max(m * compute_units / units, 1.0), std::min(words, 128));
         if (s == last) continue;
         last = s;
-        const double tiles = (words + s - 1) / s, blocks = units * s / compute_units, rounds = std::floor(blocks / most);
-        const int left = (int)std::ceil(blocks - most * rounds);
-        const double time = tiles * (rounds * us[most - 1] + (left ? us[left - 1] : 0.0)) + (s > 1 ? 2.5 + rows * s * 528 / 6e6 : 0.0);
+        const double tiles = (words + s - 1) / s;
+        double time = 0.0;
+        for (const double full : {1.0, 0.5}) {
+            const double blocks = full * units * s / compute_units, rounds = std::floor(blocks / most);
+            const int left = (int)std::ceil(blocks - most * rounds);
+            time += tiles * (rounds * us[most - 1] + (left ? us[left - 1] : 0.0));
+            if (s > 1) time += 2.5 + full * rows * s * 528 / 6e6;
+            if (!uneven) break;
+        }
         if (time < best) best = time, splits = s;
     }
     return splits;
@@ -1606,7 +1614,7 @@ Plan plan(const TrainShape &s, int element, bool backward, bool uneven, bool dro
         p.k_splits = 1;
     } else {
         p.q_splits = p.q_unit == 128
-                         ? splits_of_rounds((double)pairs * p.q_tiles, (int)words, (double)pairs * s.q_rows, single, compute_units)
+                         ? splits_of_rounds((double)pairs * p.q_tiles, (int)words, (double)pairs * s.q_rows, single, uneven, compute_units)
                          : splits_of((double)words, std::max(pairs * p.q_tiles * words / slots, 1.0), words);
         p.k_splits = 1;
     }
@@ -1731,7 +1739,7 @@ bool train_needs(const TrainShape &s, int element, bool backward, int compute_un
     *workspace = 0;
     if ((double)s.estimators * std::max((double)s.heads * s.q_rows, 2.0 * s.kv_heads * s.rows) >= 134217728.0) return false;
     // The workspace serves every plan of the shape: with lengths or masks and without, with dropout and without.
-    for (int i = 0; i < (backward ? 4 : 1); ++i) {
+    for (int i = 0; i < (backward ? 4 : 2); ++i) {
         const Plan p = plan(s, element, backward, i & 1, i & 2, compute_units);
         if (p.blocks >= 16777216.0) return false;
         *workspace = std::max(*workspace, round16(p.record) + round16(p.q_part) + round16(p.k_part));
@@ -1740,7 +1748,7 @@ bool train_needs(const TrainShape &s, int element, bool backward, int compute_un
 }
 
 void train_attention(const TrainInputs &a, const TrainForward &f, int compute_units, hipStream_t stream) {
-    const Plan p = plan(a.shape, a.element, false, false, false, compute_units);
+    const Plan p = plan(a.shape, a.element, false, a.q_lengths || a.lengths || a.keep, false, compute_units);
     if (a.element == kTrainF32)
         forward<kTrainF32>(a, f, p, stream);
     else if (a.element == kTrainF16)
