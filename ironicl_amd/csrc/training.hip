@@ -542,7 +542,7 @@ constexpr int kNone = -1000;  // a lane's power before its first term
 // FP32's took as long).
 // 512 FP32 queries over 50,000 rows of 8 heads: 204 us, 257 TFLOP/s, the matrix cores 36% busy and the vector unit 54%; with
 // two waves a SIMD they overlap little (a wave alone issues a vector instruction every seven cycles), and a third wave's
-// registers are not there. 10,007 BF16 rows over themselves with dropout: 411 us, the vector unit 78% busy, half of it
+// registers are not there. 10,007 BF16 rows over themselves with dropout: 365 us, the vector unit 78% busy, half of it
 // with random numbers.
 constexpr int forward_waves(int element, int wq, int wk) {  // of a SIMD: what registers leave room for
     return element == kTrainF32 ? 2 : wq * wk;
@@ -973,13 +973,13 @@ __global__ __launch_bounds__(256) void train_merge_kernel(const Args a) {
 
 // ---- backward ----
 
-// The two sides of the backward pass are workgroups of one launch, which fill its end for each other (two launches: 987 us
-// in place of 868 for 10,007 BF16 rows). Both compute the scores and dP: seven products in place of five. Five would take
+// The two sides of the backward pass are workgroups of one launch, which fill its end for each other (two launches: 988 us
+// in place of 858 for 10,007 BF16 rows). Both compute the scores and dP: seven products in place of five. Five would take
 // either atomic additions to dq, whose order changes results, or dq's part of every 128 keys through memory, written and
 // read (10,007 rows: 1.6 GB each way, 0.6 ms; the two products take 0.2).
-// 10,007 BF16 rows: 780 to 814 us, 630 TFLOP/s counted as five products, 880 as seven; the matrix cores 46% busy, the vector
+// 10,007 BF16 rows: 765 to 814 us, 630 TFLOP/s counted as five products, 880 as seven; the matrix cores 46% busy, the vector
 // unit 54%. 512 FP32 queries over 50,000 rows: 656 us, 200 (three FP16 products each: 840 as seven); 40% and 52%. Two
-// masked tables of 12,345 rows, FP16 with dropout: 260; 16% and 52%, random numbers and selections.
+// masked tables of 12,345 rows, FP16 with dropout: 216 to 255; 16% and 52%, random numbers and selections.
 
 // What the backward pass needs of each query: {r, 1 / s, delta, r + log2 s}; r is +inf (all weights 0) for one that attends to
 // nothing or lies past the length. Sixteen lanes to a row.
@@ -1042,11 +1042,15 @@ __device__ __forceinline__ void queries_backward(const Args &a, Streamed<EL> &ld
         return t;
     };
     const Lanes lanes(lane);
+    // A wave without a query has nothing to do but load (8 FP32 queries over 50,000 rows: 178 us where it worked on, 166).
+    const bool idle = __builtin_amdgcn_readfirstlane(tile * 128 + 32 * wave) >= q_len;
     auto work = [&](const Tile<EL> &kt, const Tile<EL> &vt, int t, unsigned long long some, int k_down, int v_down) {
+        if (idle) return;
         const float c = scaled(EL) ? times_power(a.c, k_down + q_down) : a.c;
         const float w = scaled(EL) ? times_power(a.w, v_down + g_down) : a.w;
 #pragma unroll 1
         for (int b = 0; b < 2; ++b) {
+            if (!(unsigned)(some >> 32 * b)) continue;
             f32x16 s = {}, dp = {};
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
@@ -1207,11 +1211,12 @@ __device__ __forceinline__ void keys_backward(const Args &a, Streamed<EL> &lds, 
 #pragma unroll
         for (int n = 0; n < 3; ++n) ones[0][n] = ones[1][3 + n] = (__bf16)1.f;
     auto work = [&](const Tile<EL> &qt, const Tile<EL> &gt, const float *r, const u32x4 *more, const float *delta, int h, int row0,
-                    int q_down, int g_down) {
+                    unsigned long long some, int q_down, int g_down) {
         const float c = scaled(EL) ? times_power(a.c, q_down + k_down) : a.c;
         const float w = scaled(EL) ? times_power(a.w, g_down + v_down) : a.w;
 #pragma unroll 1
         for (int b = 0; b < 2; ++b) {
+            if (!(unsigned)(some >> 32 * b)) continue;  // 24 FP32 queries over 50,000 rows, dropout: 223 us without, 214
             f32x16 s = {}, dp = {};
             if constexpr (!scaled(EL)) {
                 const bf16x8 x = __builtin_bit_cast(bf16x8, more[32 * b + (lane & 31)]);
@@ -1327,7 +1332,7 @@ __device__ __forceinline__ void keys_backward(const Args &a, Streamed<EL> &lds, 
                 ++u;
                 if (u < end) load(u);
             }
-            work(lds.x[0], lds.y[0], lds.r[0], nullptr, lds.delta[0], h, row0, down(turn.x), down(turn.y));
+            work(lds.x[0], lds.y[0], lds.r[0], nullptr, lds.delta[0], h, row0, turn.some, down(turn.x), down(turn.y));
         }
     } else {
         const float inverse = -1.f / a.c;
@@ -1355,7 +1360,7 @@ __device__ __forceinline__ void keys_backward(const Args &a, Streamed<EL> &lds, 
                 __syncthreads();
             }
             if (u + 1 < end) load(u + 1, now ^ 1);
-            work(lds.x[now], lds.y[now], nullptr, lds.more[now], lds.delta[now], hk * group + u / q_tiles, u % q_tiles * kTile, 0, 0);
+            work(lds.x[now], lds.y[now], nullptr, lds.more[now], lds.delta[now], hk * group + u / q_tiles, u % q_tiles * kTile, some, 0, 0);
         }
     }
     if (key >= len) return;
