@@ -552,8 +552,8 @@ int irx_train_attention(irx_device *device, const irx_train_inputs *inputs, void
                         float *stats, float *lse, void *workspace, size_t workspace_bytes, void *stream);
 /* The gradients of q, k and v from the output's. Probabilities are computed anew
  * from stats. dout's numbers are below 2^126 in size, and its products with v and the output within
- * FP32's range; one that is not finite leaves its query's gradient, and those of all keys that it attends to,
- * not finite. */
+ * FP32's range (dP, dS and dout / s below 2^-126 may be taken as 0); one that is not finite leaves its query's gradient,
+ * and those of all keys that it attends to, not finite. */
 int irx_train_attention_backward(irx_device *device, const irx_train_inputs *inputs,
                                  const irx_train_gradients *gradients, void *workspace, size_t workspace_bytes,
                                  void *stream);

@@ -372,7 +372,8 @@ __device__ __forceinline__ long long at(const long long *s, int e, int h, int ro
     return e * s[0] + h * s[1] + (long long)row * s[2];
 }
 
-// x 2^by (x > 0), held to FP32's normal numbers: a factor of 0 or of infinity would make NaN of what is left out or 0.
+// x 2^by (x > 0), held to FP32's normal numbers: a factor of 0 or of infinity would make NaN of scores that are left out or 0.
+// Where the power would be a smaller one, scores are below 2^-90. dP, of which any size counts, takes its power by itself.
 __device__ __forceinline__ float times_power(float x, int by) {
     return fminf(fmaxf(__builtin_ldexpf(x, by), 0x1p-126f), 0x1p127f);
 }
@@ -1047,7 +1048,6 @@ __device__ __forceinline__ void queries_backward(const Args &a, Streamed<EL> &ld
     auto work = [&](const Tile<EL> &kt, const Tile<EL> &vt, int t, unsigned long long some, int k_down, int v_down) {
         if (idle) return;
         const float c = scaled(EL) ? times_power(a.c, k_down + q_down) : a.c;
-        const float w = scaled(EL) ? times_power(a.w, v_down + g_down) : a.w;
 #pragma unroll 1
         for (int b = 0; b < 2; ++b) {
             if (!(unsigned)(some >> 32 * b)) continue;
@@ -1060,6 +1060,9 @@ __device__ __forceinline__ void queries_backward(const Args &a, Streamed<EL> &ld
                 rows_operand<EL>(vt, 32 * b, c, lanes, x);
                 mma<EL>(dp, x, gb[c]);
             }
+            if constexpr (scaled(EL))
+#pragma unroll
+                for (int i = 0; i < 16; ++i) dp[i] = __builtin_ldexpf(dp[i], v_down + g_down);
             if (some != ~0ull) leave_out(s, some, 32 * b, half);
             float most = 0.f;
 #pragma unroll
@@ -1071,7 +1074,7 @@ __device__ __forceinline__ void queries_backward(const Args &a, Streamed<EL> &ld
                     const int i = 8 * cc + j;
                     const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -record[0]));
                     if constexpr (DROP || scaled(EL))
-                        s[i] = p * __builtin_fmaf(!DROP || kept16(z, j, a.line) ? dp[i] : 0.f, w, -record[2]);
+                        s[i] = p * __builtin_fmaf(!DROP || kept16(z, j, a.line) ? dp[i] : 0.f, a.w, -record[2]);
                     else
                         s[i] = p * (dp[i] - record[2]);
                     if constexpr (ranged(EL)) most = fmaxf(most, fabsf(s[i]));
@@ -1213,7 +1216,6 @@ __device__ __forceinline__ void keys_backward(const Args &a, Streamed<EL> &lds, 
     auto work = [&](const Tile<EL> &qt, const Tile<EL> &gt, const float *r, const u32x4 *more, const float *delta, int h, int row0,
                     unsigned long long some, int q_down, int g_down) {
         const float c = scaled(EL) ? times_power(a.c, q_down + k_down) : a.c;
-        const float w = scaled(EL) ? times_power(a.w, g_down + v_down) : a.w;
 #pragma unroll 1
         for (int b = 0; b < 2; ++b) {
             if (!(unsigned)(some >> 32 * b)) continue;  // 24 FP32 queries over 50,000 rows, dropout: 223 us without, 214
@@ -1231,6 +1233,12 @@ __device__ __forceinline__ void keys_backward(const Args &a, Streamed<EL> &lds, 
                 rows_operand<EL>(gt, 32 * b, n, lanes, x);
                 mma<EL>(dp, x, vb[n]);
             }
+            // The power by itself: as part of w it would have to stay a normal number, for which dout of 2^-100 is too small. (Only
+            // where some lane needs it so: 512 FP32 queries over 50,000 rows 631 us in place of 636, but registers spill with
+            // dropout, and four tables of 1,024 rows take 149 in place of 137.)
+            if constexpr (scaled(EL))
+#pragma unroll
+                for (int i = 0; i < 16; ++i) dp[i] = __builtin_ldexpf(dp[i], g_down + v_down);
             unsigned kept = ~0u;
             if constexpr (DROP)
                 kept = kept_words(16 * tile + 4 * wave, row0 + 32 * b + (lane & 31), e * a.heads + h, a.site, a.line, seed, half) >>
@@ -1253,7 +1261,7 @@ __device__ __forceinline__ void keys_backward(const Args &a, Streamed<EL> &lds, 
                     s[i] = __int_as_float(__float_as_int(p) & z);
                 }
                 if constexpr (DROP || scaled(EL))
-                    dp[i] = p * __builtin_fmaf(dp[i], w, -delta[q]);
+                    dp[i] = p * __builtin_fmaf(dp[i], a.w, -delta[q]);
                 else
                     dp[i] *= p;
                 if constexpr (ranged(EL)) most_p = fmaxf(most_p, s[i]), most_ds = fmaxf(most_ds, fabsf(dp[i]));

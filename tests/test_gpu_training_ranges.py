@@ -1,0 +1,64 @@
+"""The training calls at the ends of their ranges, against float64 (training_np.py) within the bounds that
+test_gpu_training.py works out: numbers far below 1, and far above it beside others; only what a test adds to them stands there."""
+
+import numpy as np
+import pytest
+
+import training_np
+from ironicl_amd import hip
+from test_gpu_training import HALF, PARTS, Case, floor, normal, within
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def device():
+    return hip.Device(0)
+
+
+def bounds(case, want, ds, key_ds=None):
+    """Bounds of out, dq, dk and dv where every score is off by ds (in the keys' sums by key_ds)."""
+    el, (_, h, g, m, n) = case.element, case.shape
+    m *= h // g
+    key_ds = ds if key_ds is None else key_ds
+    forward = 2 * ds + PARTS[el] + n * 2.0 ** -26 + 2.0 ** -20
+    gradient = 2 * PARTS[el] + 2.0 ** -17 + forward + HALF[el] + 2.0 ** -19
+    return (want.out_abs * forward + floor(want.out_term, n, el),
+            want.dq_abs * (gradient + 2 * ds + n * 2.0 ** -26) + floor(want.dq_term, n, el),
+            want.dk_abs * (gradient + 2 * key_ds + m * 2.0 ** -26) + floor(want.dk_term, m, el),
+            want.dv_abs * (2 * key_ds + PARTS[el] + m * 2.0 ** -26 + 2.0 ** -20) + floor(want.dv_term, m, el))
+
+
+def compare(case, got, want, ds, key_ds=None):
+    exact = (want.out, want.dq, want.dk, want.dv)
+    for name, have, x, bound in zip(("out", "dq", "dk", "dv"), [got[0]] + got[3:], exact, bounds(case, want, ds, key_ds)):
+        within(have, x, bound, np.ones(have.shape, bool), case.element, name)
+
+
+@pytest.mark.parametrize("dropped", [0, 3000])
+@pytest.mark.parametrize("values,gradients", [(0, -100), (0, -108), (-50, -55), (-55, -50), (40, -108)])
+def test_fp32_gradients_of_small_products(device, values, gradients, dropped):
+    """dout and v by powers of two: dq and dk by their product, dv by dout's, though dP is far below 1. Each of 130 terms may
+    miss 2^-126 times an operand up to 8, and a sum that misses one may round the other way once in each of its additions,
+    fewer than 64, by 2^-24 of a sum of magnitudes."""
+    dout, v = normal((1, 2, 70, 64), 3), normal((1, 2, 130, 64), 2)
+    a = Case(device, 1, 2, 2, 70, 130, dropped=dropped, seed=4, dout=dout, v=v)
+    b = Case(device, 1, 2, 2, 70, 130, dropped=dropped, seed=4, dout=a.dout.values * 2.0 ** gradients, v=a.v.values * 2.0 ** values)
+    want, first, second = a.oracle(), a.run(), b.run()
+    np.testing.assert_array_equal(first[0] * 2.0 ** values, second[0])
+    for name, x, y, by, size in zip(("dq", "dk", "dv"), first[3:], second[3:], (values + gradients,) * 2 + (gradients,),
+                                    (want.dq_abs, want.dk_abs, want.dv_abs)):
+        off = np.abs(x * 2.0 ** by - y) - (size * 2.0 ** (by - 18) + 130 * 8 * 2.0 ** -126)
+        assert off.max() <= 0, f"{name} past the bound by {off.max():.3e}"
+
+
+def test_fp32_gradients_of_large_rows(device):
+    """Rows of v whose largest number meets a zero of dout: dP is within FP32's range though its row times dout's is not."""
+    rng = np.random.default_rng(5)
+    v, dout = np.zeros((1, 2, 200, 64)), np.zeros((1, 2, 40, 64))
+    v[..., 0] = 2.0 ** 120 * rng.choice([-1.0, 1.0], (1, 2, 200))
+    v[..., 1] = 2.0 ** 85 * rng.choice([-1.0, 1.0], (1, 2, 200))
+    dout[..., 1] = 2.0 ** 40 * rng.choice([-1.0, 1.0], (1, 2, 40))
+    case = Case(device, 1, 2, 2, 40, 200, v=v, dout=dout)
+    got, want = case.run(), case.oracle()
+    compare(case, got, want, 2.0 ** -17 * want.magnitude.max())
