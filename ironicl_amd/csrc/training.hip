@@ -566,10 +566,11 @@ __global__ __launch_bounds__(64 * WQ * WK, forward_waves(EL, WQ, WK)) void train
     const int q_down = down(own_row<EL>(a.q, at(a.qs, e, h, query), mine, lane, qb));
 
     // o holds sum 2^(x - k) v: with FP32 a value's tile comes by 2^-v_down, its weights by 2^v_down, and k follows the largest
-    // of x + v_down, apart from the sum's reference r. With 16-bit elements k is r - TOP.
+    // of x + v_down, apart from the sum's reference r. With 16-bit elements k is r - TOP. FP32's sum is that of the same
+    // weights, taken back to r, but where earlier values outweigh a tile's by so much (2^60) that weights of its order fall
+    // out of FP32's range beside them: there it has exponentials of its own.
     f32x16 o[2] = {};
     float r = -INFINITY, k = -INFINITY, sum = 0.f;
-    int most_v = 0;
     const unsigned long long seed = DROP ? *a.seed : 0;
     const int end = min((split + 1) * a.q_chunk, (int)((len + 63) / 64));
     auto next = [&](int t, unsigned long long &m) {
@@ -610,7 +611,14 @@ __global__ __launch_bounds__(64 * WQ * WK, forward_waves(EL, WQ, WK)) void train
             k = upto;
         }
         const float from = (float)v_down - (k == -INFINITY ? 0.f : k);
-        float part = 0.f;
+        float part = 0.f, own = 0.f;
+        const float most = fmaxf(r, top), ref = most == -INFINITY ? 0.f : most;
+        const bool apart = scaled(EL) && __any(-from - ref > 60.f);
+        if (apart)
+#pragma unroll
+            for (int b = 0; b < NS; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) own += __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], c, -ref));
 #pragma unroll
         for (int b = 0; b < NS; ++b) {
             const int sub = WK == 1 ? b : wk;
@@ -641,9 +649,9 @@ __global__ __launch_bounds__(64 * WQ * WK, forward_waves(EL, WQ, WK)) void train
             }
         }
         if constexpr (scaled(EL)) {
-            const float upto = fmaxf(r, top), ref = upto == -INFINITY ? 0.f : upto;
-            sum = sum * (r == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(r - ref)) + part * __builtin_amdgcn_exp2f(-from - ref);
-            r = upto;
+            const float here = apart ? own : part * __builtin_amdgcn_exp2f(-from - ref);
+            sum = sum * (r == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(r - ref)) + here;
+            r = most;
         } else {
             sum += part;
         }
@@ -661,10 +669,7 @@ __global__ __launch_bounds__(64 * WQ * WK, forward_waves(EL, WQ, WK)) void train
         while (t < end) {
             if (fresh) ks.fields(fields[0]), vs.fields(fields[1]);
             __syncthreads();
-            Turn turn = turn_of(todo, fields[0], fields[1], lane);
-            // Values 2^40 smaller than the largest so far stay that small: their weights must not leave FP32's range.
-            turn.y = max(turn.y, most_v - 40);
-            most_v = max(most_v, turn.y);
+            const Turn turn = turn_of(todo, fields[0], fields[1], lane);
             ks.store(tiles[0][0], turn.some, scale_of(turn.x));
             vs.store(tiles[0][1], turn.some, scale_of(turn.y));
             __syncthreads();

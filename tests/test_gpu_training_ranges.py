@@ -62,3 +62,27 @@ def test_fp32_gradients_of_large_rows(device):
     case = Case(device, 1, 2, 2, 40, 200, v=v, dout=dout)
     got, want = case.run(), case.oracle()
     compare(case, got, want, 2.0 ** -17 * want.magnitude.max())
+
+
+@pytest.mark.parametrize("at", [0, 20, 299])
+@pytest.mark.parametrize("queries", [9, 40, 130])
+@pytest.mark.parametrize("element", ["f32", "bf16"])
+@pytest.mark.parametrize("size,score", [(60, -1000), (80, -1000), (120, -1000), (80, -62), (120, -40), (126, -12)])
+def test_small_values_beside_a_large_one(device, size, score, element, queries, at):
+    """One value of 2^size whose score lies far below the others': of no weight, of as much as the others have together, or of
+    so much more that they hardly show, but in the sums of weights. It is in the first tile, beside them, or in the last."""
+    e, h, n = 1, 2, 300
+    q, k, v = normal((e, h, queries, 64), 1, 1.3), normal((e, h, n, 64), 2, 1.1), normal((e, h, n, 64), 3)
+    q[..., 0], k[..., 0] = 8.0, 0.0
+    k[:, :, at] = 0.0
+    k[:, :, at, 0], v[:, :, at, 5] = score, 2.0 ** size
+    dout = normal(q.shape, 4, 2.0 ** -6)
+    case = Case(device, e, h, h, queries, n, element, q=q, k=k, v=v, dout=dout)
+    got, want = case.run(), case.oracle()
+    # Its score is a whole number; at no weight, the others' alone count.
+    keep = np.arange(n) != at
+    others = training_np.Attention(case.q.values, case.k.values, case.v.values, keep=keep[None])
+    ds = 2.0 ** -17 * (others.magnitude.max() + (-score if score > -1000 else 0))
+    compare(case, got, want, ds)
+    off = np.abs(got[1] - want.lse) - (2 * ds + n * 2.0 ** -26 + 2.0 ** -21 * np.abs(want.lse) + 1e-6)
+    assert off.max() <= 0
