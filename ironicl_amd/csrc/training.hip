@@ -987,7 +987,7 @@ __global__ __launch_bounds__(256) void train_merge_kernel(const Args a) {
 // unit 54%. 512 FP32 queries over 50,000 rows: 656 us, 200 (three FP16 products each: 840 as seven); 40% and 52%. Two
 // masked tables of 12,345 rows, FP16 with dropout: 216 to 255; 16% and 52%, random numbers and selections.
 
-// What the backward pass needs of each query: {r, 1 / s, delta, r + log2 s}; r is +inf (all weights 0) for one that attends to
+// What the backward pass needs of each query: {r, 1 / s, delta, log2 s}; r is +inf (all weights 0) for one that attends to
 // nothing or lies past the length. Sixteen lanes to a row.
 template <int EL>
 __global__ __launch_bounds__(256) void train_record_kernel(const Args a) {
@@ -1004,7 +1004,7 @@ __global__ __launch_bounds__(256) void train_record_kernel(const Args a) {
         float d = o[0] * g[0] + o[1] * g[1] + o[2] * g[2] + o[3] * g[3];
 #pragma unroll
         for (int i = 8; i; i >>= 1) d += __shfl_xor(d, i, 16);
-        record = f32x4{x[0], 1.f / x[1], d, x[0] + __builtin_amdgcn_logf(x[1])};
+        record = f32x4{x[0], 1.f / x[1], d, __builtin_amdgcn_logf(x[1])};
     }
     if (!lane) a.record[row] = record;
 }
@@ -1014,6 +1014,7 @@ struct Streamed {
     static constexpr int N = scaled(EL) ? 1 : 2;
     Tile<EL> x[N], y[N];
     alignas(16) float r[N][kTile], delta[N][kTile];
+    alignas(16) float logs[scaled(EL) ? 1 : N][kTile];      // 16-bit: log2 s
     alignas(16) u32x4 more[N][scaled(EL) ? 1 : kTile];  // 16-bit: what each row's scores and dP take besides
     float coming[scaled(EL) ? kTile : 1];               // the next tile's r
     int fields[2][scaled(EL) ? kTile : 1];  // and exponents
@@ -1183,6 +1184,8 @@ __device__ __forceinline__ unsigned kept_words(unsigned cell, int query, int pai
     return half ? r[0] : mine;
 }
 
+constexpr float kNear = 128.f;
+
 // The gradients of 32 keys a wave: S = Q K^T, dout V^T, then dout^T P and Q^T dS, over a split's query tiles of every head
 // that shares the keys.
 template <int EL, bool DROP>
@@ -1213,21 +1216,24 @@ __device__ __forceinline__ void keys_backward(const Args &a, Streamed<EL> &lds, 
     const Lanes lanes(lane);
     // One turn: queries of the tile at row0 of head h. FP32's r and delta stand beside them. With 16-bit elements one more
     // product of BF16 parts adds -(r + log2 s) / c to the scores (24 bits of it) and, without dropout, -delta to dP: read from
-    // LDS for every element, the three take as much of its time as the tiles' operands.
+    // LDS for every element, the three take as much of its time as the tiles' operands. Where a reference is past kNear,
+    // 2^-24 of it, several times over, would show beside the weights' own rounding (2^-12 for FP16): such a tile's are read,
+    // r taken from the score in one multiplication and addition and log2 s after it (for every tile so: the gradients of 10,007
+    // BF16 rows 902 us in place of 806).
     bf16x8 ones[2] = {};
     if (!half)
 #pragma unroll
         for (int n = 0; n < 3; ++n) ones[0][n] = ones[1][3 + n] = (__bf16)1.f;
-    auto work = [&](const Tile<EL> &qt, const Tile<EL> &gt, const float *r, const u32x4 *more, const float *delta, int h, int row0,
-                    unsigned long long some, int q_down, int g_down) {
-        const float c = scaled(EL) ? times_power(a.c, q_down + k_down) : a.c;
+    auto work = [&](const Tile<EL> &qt, const Tile<EL> &gt, const float *r, const float *logs, const u32x4 *more, const float *delta,
+                    int h, int row0, unsigned long long some, bool near, int q_down, int g_down) {
+        const float c = scaled(EL) ? times_power(a.c, q_down + k_down) : near ? a.c : 1.f;
 #pragma unroll 1
         for (int b = 0; b < 2; ++b) {
             if (!(unsigned)(some >> 32 * b)) continue;  // 24 FP32 queries over 50,000 rows, dropout: 223 us without, 214
             f32x16 s = {}, dp = {};
             if constexpr (!scaled(EL)) {
                 const bf16x8 x = __builtin_bit_cast(bf16x8, more[32 * b + (lane & 31)]);
-                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, ones[0], s, 0, 0, 0);
+                if (near) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, ones[0], s, 0, 0, 0);
                 if constexpr (!DROP) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, ones[1], dp, 0, 0, 0);
             }
 #pragma unroll
@@ -1238,6 +1244,15 @@ __device__ __forceinline__ void keys_backward(const Args &a, Streamed<EL> &lds, 
                 rows_operand<EL>(gt, 32 * b, n, lanes, x);
                 mma<EL>(dp, x, vb[n]);
             }
+            if (!scaled(EL) && !near)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const int q = 32 * b + 2 * i + 4 * half;
+                    const f32x4 ref = *reinterpret_cast<const f32x4 *>(r + q), log = *reinterpret_cast<const f32x4 *>(logs + q);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[i + j] = __builtin_fmaf(s[i + j], a.c, -ref[j]) - log[j];
+                    __builtin_amdgcn_sched_barrier(0);  // all sixteen's at once cost registers: spills, and 839 us in place of 806
+                }
             // The power by itself: as part of w it would have to stay a normal number, for which dout of 2^-100 is too small. (Only
             // where some lane needs it so: 512 FP32 queries over 50,000 rows 631 us in place of 636, but registers spill with
             // dropout, and four tables of 1,024 rows take 149 in place of 137.)
@@ -1345,7 +1360,7 @@ __device__ __forceinline__ void keys_backward(const Args &a, Streamed<EL> &lds, 
                 ++u;
                 if (u < end) load(u);
             }
-            work(lds.x[0], lds.y[0], lds.r[0], nullptr, lds.delta[0], h, row0, turn.some, down(turn.x), down(turn.y));
+            work(lds.x[0], lds.y[0], lds.r[0], nullptr, nullptr, lds.delta[0], h, row0, turn.some, true, down(turn.x), down(turn.y));
         }
     } else {
         const float inverse = -1.f / a.c;
@@ -1361,19 +1376,23 @@ __device__ __forceinline__ void keys_backward(const Args &a, Streamed<EL> &lds, 
             if (threadIdx.x < kTile) {
                 lds.r[now][threadIdx.x] = coming[0];
                 lds.delta[now][threadIdx.x] = coming[2];
+                lds.logs[now][threadIdx.x] = coming[3];
                 // A row without weights has a score that leaves none.
                 const bool none = coming[0] == INFINITY;
-                const u32x2 x = bf16_parts(none ? -0x1p120f : coming[3] * inverse), y = bf16_parts(-coming[2]);
+                const u32x2 x = bf16_parts(none ? -0x1p120f : (coming[0] + coming[3]) * inverse), y = bf16_parts(-coming[2]);
                 lds.more[now][threadIdx.x] = u32x4{x[0], x[1] | y[0] << 16, y[0] >> 16 | y[1] << 16, 0};
             }
             __syncthreads();  // the tile has come, and the other is read
-            const unsigned long long some = __ballot(lds.r[now][lane] != INFINITY);
+            const float of_lane = lds.r[now][lane];
+            const unsigned long long some = __ballot(of_lane != INFINITY);
+            const bool near = !__any(of_lane != INFINITY && !(fabsf(of_lane) <= kNear));
             if (some != ~0ull) {
                 clear_rows<EL, 256>(lds.x[now], some), clear_rows<EL, 256>(lds.y[now], some);
                 __syncthreads();
             }
             if (u + 1 < end) load(u + 1, now ^ 1);
-            work(lds.x[now], lds.y[now], nullptr, lds.more[now], lds.delta[now], hk * group + u / q_tiles, u % q_tiles * kTile, some, 0, 0);
+            work(lds.x[now], lds.y[now], lds.r[now], lds.logs[now], lds.more[now], lds.delta[now], hk * group + u / q_tiles,
+                 u % q_tiles * kTile, some, near, 0, 0);
         }
     }
     if (key >= len) return;

@@ -86,3 +86,26 @@ def test_small_values_beside_a_large_one(device, size, score, element, queries, 
     compare(case, got, want, ds)
     off = np.abs(got[1] - want.lse) - (2 * ds + n * 2.0 ** -26 + 2.0 ** -21 * np.abs(want.lse) + 1e-6)
     assert off.max() <= 0
+
+
+@pytest.mark.parametrize("dropped", [0, 9000])
+@pytest.mark.parametrize("element", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("queries", [40, 200])
+@pytest.mark.parametrize("size", [2.0 ** 5, 2.0 ** 8, 2.0 ** 13, 2.0 ** 20])
+def test_scores_that_are_whole_at_any_size(device, size, queries, element, dropped):
+    """Products of queries and keys are whole numbers below 2^24, and their sums in any order: scores differ by a few either
+    way at sizes up to 2^20. log2(e) scale is off by 2^-24 of itself, and so are differences of scores; a score's distance
+    from its reference (24 at most, where its weight counts) is rounded once, to 2^-24 of it: 2^-19 in all, with a step to
+    spare. In the sums of 16-bit types' keys, references below 2^7 stand as one number with their sums' logarithms: 16
+    roundings of it at most, 2^-13."""
+    e, h, n = 1, 2, 300
+    rng = np.random.default_rng(int(size))
+    q, k = (rng.integers(-2, 3, (e, h, rows, 64)).astype(float) for rows in (queries, n))
+    q[..., 0] = 2.0 ** 12 * rng.choice([-1.0, 1.0], (e, h, queries))
+    k[..., 0] = size * 2.0 ** -9 * rng.choice([-1.0, 1.0], (e, h, n))
+    case = Case(device, e, h, h, queries, n, element, q=q, k=k, scale=2.0 ** -3, dropped=dropped)
+    got, want = case.run(), case.oracle()
+    assert want.lse.min() > size - 20
+    few = element != "f32" and size < 2.0 ** 6
+    compare(case, got, want, 2.0 ** -19, 2.0 ** -13 if few else None)
+    assert np.all(np.abs(got[1] - want.lse) <= 2.0 ** -22 * np.abs(want.lse) + n * 2.0 ** -26 + 2.0 ** -18)
