@@ -843,7 +843,7 @@ __global__ __launch_bounds__(256) void train_rows_kernel(const Args a) {
                     step(__builtin_amdgcn_mov_dpp(__float_as_int(d), 0x4E, 15, 15, true));
                     step(__builtin_amdgcn_mov_dpp(__float_as_int(d), 0x141, 15, 15, true));
                     if constexpr (LK == 16) step(__builtin_amdgcn_mov_dpp(__float_as_int(d), 0x140, 15, 15, true));
-                    x[n][j] = d * a.c;
+                    x[n][j] = d;
                 }
             }
             if (some != ~0ull)
@@ -856,7 +856,8 @@ __global__ __launch_bounds__(256) void train_rows_kernel(const Args a) {
                 float top = x[n][0];
 #pragma unroll
                 for (int j = 1; j < 8; ++j) top = fmaxf(top, x[n][j]);
-                const float upto = fmaxf(r[n], ceilf(top));
+                // A scale is positive: the largest score is that of the largest product.
+                const float upto = fmaxf(r[n], ceilf(top * a.c));
                 if (__any(upto > r[n])) {
                     const float f = r[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(r[n] - upto);
                     sum[n] *= f;
@@ -867,7 +868,7 @@ __global__ __launch_bounds__(256) void train_rows_kernel(const Args a) {
                 const float ref = r[n] == -INFINITY ? 0.f : r[n];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    x[n][j] = __builtin_amdgcn_exp2f(x[n][j] - ref);
+                    x[n][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[n][j], a.c, -ref));
                     sum[n] += x[n][j];
                 }
                 if constexpr (DROP) {

@@ -90,7 +90,7 @@ def test_small_values_beside_a_large_one(device, size, score, element, queries, 
 
 @pytest.mark.parametrize("dropped", [0, 9000])
 @pytest.mark.parametrize("element", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("queries", [40, 200])
+@pytest.mark.parametrize("queries", [1, 3, 40, 200])
 @pytest.mark.parametrize("size", [2.0 ** 5, 2.0 ** 8, 2.0 ** 13, 2.0 ** 20])
 def test_scores_that_are_whole_at_any_size(device, size, queries, element, dropped):
     """Products of queries and keys are whole numbers below 2^24, and their sums in any order: scores differ by a few either
