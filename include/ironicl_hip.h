@@ -558,8 +558,8 @@ int irx_train_attention_backward(irx_device *device, const irx_train_inputs *inp
                                  const irx_train_gradients *gradients, void *workspace, size_t workspace_bytes,
                                  void *stream);
 
-/* out = residual + w D(x), rounded once; with residual NULL, w D(x), which is also
- * the gradient of x from that of out. Rows start `stride` elements apart (multiples of
+/* out = residual + w D(x) as one FP32 multiplication and addition, rounded to the type;
+ * with residual NULL, w D(x), which is also the gradient of x from that of out. Rows start `stride` elements apart (multiples of
  * 16 bytes, as the pointers are; at least the width, where there is more than one
  * row). out may be x or residual, with that one's stride. 1 to 2^31 - 1 columns, rows with less
  * than 2^31 groups of 8 columns in all. */

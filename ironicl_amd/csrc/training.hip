@@ -1500,11 +1500,11 @@ __global__ __launch_bounds__(256) void train_dropout_kernel(const DropArgs a) {
     if (a.line) {
         const u32x4 z = philox(col, row, ~0u, a.site, *a.seed);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = kept16(z, j, a.line) ? x[j] * a.w : 0.f;
+        for (int j = 0; j < 8; ++j) x[j] = kept16(z, j, a.line) ? x[j] : 0.f;
     }
-    if (a.residual)
+    // One rounding to FP32; without a residual zeros keep their signs.
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] += y[j];
+    for (int j = 0; j < 8; ++j) x[j] = a.residual ? __builtin_fmaf(x[j], a.w, y[j]) : x[j] * a.w;
     if (left == 8) {
         store4<EL>(a.out, oi, f32x4{x[0], x[1], x[2], x[3]});
         store4<EL>(a.out, oi + 4, f32x4{x[4], x[5], x[6], x[7]});

@@ -5,8 +5,8 @@ import numpy as np
 import pytest
 
 import training_np
-from ironicl_amd import hip
-from test_gpu_training import HALF, PARTS, Case, floor, normal, within
+from ironicl_amd import hip, hipmem, training
+from test_gpu_training import HALF, PARTS, SEED, Case, decode, encode, floor, normal, put, within
 
 pytestmark = pytest.mark.gpu
 
@@ -109,3 +109,23 @@ def test_scores_that_are_whole_at_any_size(device, size, queries, element, dropp
     few = element != "f32" and size < 2.0 ** 6
     compare(case, got, want, 2.0 ** -19, 2.0 ** -13 if few else None)
     assert np.all(np.abs(got[1] - want.lse) <= 2.0 ** -22 * np.abs(want.lse) + n * 2.0 ** -26 + 2.0 ** -18)
+
+
+@pytest.mark.parametrize("element", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dropped", [0, 1, 6554, 40001, 65535])
+def test_dropout_is_one_multiplication_and_addition(device, dropped, element):
+    """x w + residual, rounded once to FP32 and then to the type. x and residual are multiples of 2^-3 and 2^-10 below 2^4,
+    so that float64 holds the products with w's 24 bits, and the sums, whole."""
+    rng = np.random.default_rng(dropped)
+    rows, width = 300, 136
+    x = rng.integers(-127, 128, (rows, width)) * 2.0 ** -3
+    residual = rng.integers(-127, 128, (rows, width)) * 2.0 ** -10
+    seed, out = put(np.array([SEED], np.uint64)), put(encode(np.zeros((rows, width)), element))
+    w = float(np.float32(65536.0) / np.float32(65536 - dropped))
+    term = x * w * training_np.kept_numbers(SEED, 7, dropped, rows, width)
+    for second in (None, residual):
+        training.dropout(device, rows, width, put(encode(x, element)), out, element=element,
+                         residual=None if second is None else put(encode(second, element)), seed=seed, site=7, dropped=dropped)
+        hipmem.synchronize()
+        want = encode((term + (0.0 if second is None else second)).astype(np.float32), element)
+        np.testing.assert_array_equal(decode(out.to_host(), element), decode(want, element))
