@@ -401,6 +401,10 @@ __device__ __forceinline__ void load_tile(Tile<EL> &t, const void *base, const l
     }
 }
 
+// A wave's loads to LDS have arrived: vmcnt(0); expcnt and lgkmcnt left at their maxima (no wait). What other waves loaded has
+// arrived after the barrier that follows.
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+
 // Rows whose bit is not set become zeros, whatever they hold.
 template <int EL, int NT>
 __device__ __forceinline__ void clear_rows(Tile<EL> &t, unsigned long long some) {
@@ -539,8 +543,9 @@ constexpr int kNone = -1000;  // a lane's power before its first term
 // 32 WQ queries to a workgroup, 32 to a wave; keys and values pass through LDS in tiles of 64, and where WK is 2 a wave
 // takes 32 of each. S^T = K Q^T leaves a query's scores in one lane (and its other half), in the order in which the next
 // product takes them. FP32 tiles are loaded into registers while the last is worked on and become pairs on their way to LDS;
-// 16-bit ones go straight to LDS, the next tile's while one is worked on (so done, with two barriers a tile in place of one,
-// FP32's took as long).
+// 16-bit ones go straight to LDS, the next tile's while one's scores and softmax are worked on: the compiler, which cannot tell
+// the two buffers apart, has the transposed reads of one wait for the loads to the other. (With two buffers and two barriers
+// a tile in place of one, FP32's took as long.)
 // 512 FP32 queries over 50,000 rows of 8 heads: 204 us, 257 TFLOP/s, the matrix cores 36% busy and the vector unit 54%; with
 // two waves a SIMD they overlap little (a wave alone issues a vector instruction every seven cycles), and a third wave's
 // registers are not there. 10,007 BF16 rows over themselves with dropout: 365 us, the vector unit 78% busy, half of it
@@ -690,6 +695,7 @@ __global__ __launch_bounds__(64 * WQ * WK, forward_waves(EL, WQ, WK)) void train
         };
         if (t < end) load(t, 0);
         for (int now = 0; t < end; now ^= 1) {
+            wait_loads();
             __syncthreads();  // the tile has come, and the other is read
             if (todo != ~0ull) {
                 clear_rows<EL, NT>(tiles[now][0], todo), clear_rows<EL, NT>(tiles[now][1], todo);
@@ -1138,6 +1144,7 @@ __device__ __forceinline__ void queries_backward(const Args &a, Streamed<EL> &ld
         };
         if (t < end) load(t, 0);
         for (int now = 0; t < end; now ^= 1) {
+            wait_loads();
             __syncthreads();  // the tile has come, and the other is read
             if (todo != ~0ull) {
                 clear_rows<EL, 256>(lds.x[now], todo), clear_rows<EL, 256>(lds.y[now], todo);
@@ -1383,6 +1390,7 @@ __device__ __forceinline__ void keys_backward(const Args &a, Streamed<EL> &lds, 
                 const u32x2 x = bf16_parts(none ? -0x1p120f : (coming[0] + coming[3]) * inverse), y = bf16_parts(-coming[2]);
                 lds.more[now][threadIdx.x] = u32x4{x[0], x[1] | y[0] << 16, y[0] >> 16 | y[1] << 16, 0};
             }
+            wait_loads();
             __syncthreads();  // the tile has come, and the other is read
             const float of_lane = lds.r[now][lane];
             const unsigned long long some = __ballot(of_lane != INFINITY);
