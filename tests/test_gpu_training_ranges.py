@@ -129,3 +129,22 @@ def test_dropout_is_one_multiplication_and_addition(device, dropped, element):
         hipmem.synchronize()
         want = encode((term + (0.0 if second is None else second)).astype(np.float32), element)
         np.testing.assert_array_equal(decode(out.to_host(), element), decode(want, element))
+
+
+@pytest.mark.parametrize("queries", [1, 8, 40, 200])
+def test_fp32_products_keep_their_lower_halves(device, queries):
+    """Numbers whose bits past the eleventh all point one way: a product of a lower with an upper half that went missing
+    would show in every score, weight and gradient at once (64 terms of 2^-12, one sign)."""
+    def numbers(shape, seed):
+        rng = np.random.default_rng(seed)
+        # 1 to 2 in steps of 2^-10, and half a step more: the half step is the lower half.
+        return 1.0 + (rng.integers(0, 1024, shape) + 0.5) * 2.0 ** -10 - 2.0 ** -22
+
+    e, h, n = 1, 2, 300
+    signs = [np.random.default_rng(i).choice([-1.0, 1.0], (e, h, rows, 1)) for i, rows in ((9, n), (10, queries))]
+    case = Case(device, e, h, h, queries, n, q=numbers((e, h, queries, 64), 1), k=numbers((e, h, n, 64), 2) * signs[0],
+                v=numbers((e, h, n, 64), 3), dout=numbers((e, h, queries, 64), 4) * signs[1], scale=2.0 ** -7)
+    got, want = case.run(), case.oracle()
+    compare(case, got, want, 2.0 ** -17 * want.magnitude.max())
+    # A score is |scale q k| <= 2: two lower halves' product left out and two rounded, 2^-22 each, and sums of 2^-18 of it.
+    assert np.all(np.abs(got[1] - want.lse) <= 2.0 ** -16 + n * 2.0 ** -26)
