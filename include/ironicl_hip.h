@@ -545,9 +545,11 @@ size_t irx_train_workspace_bytes(irx_device *device, const irx_train_shape *shap
  * FP32's range. What is rounded: FP32's operands of a product to 22 bits, weights and
  * dS too, or to 2^-38 of the largest number beside them (of their row, and of those of
  * its 64 neighbours that are within 2^14 of it; weights and dS: of the largest for
- * their query or key) where that is more; 16-bit operands not at all, weights and dS to
- * one value of the type (FP16's to 2^-38 of the largest where that is more); sums and
- * statistics are FP32. Weights below 2^-126 are taken as 0. */
+ * their query or key, each times the largest number of the rows beside it) where that is
+ * more; 16-bit operands not at all, weights and dS to one value of the type (FP16's to
+ * 2^-38 of the largest where that is more), and the weights of keys' and values' gradients
+ * may be off by 2^-13 besides; scores, sums and statistics are FP32. Weights below 2^-126
+ * are taken as 0. */
 int irx_train_attention(irx_device *device, const irx_train_inputs *inputs, void *out, const irx_strides *out_strides,
                         float *stats, float *lse, void *workspace, size_t workspace_bytes, void *stream);
 /* The gradients of q, k and v from the output's. Probabilities are computed anew

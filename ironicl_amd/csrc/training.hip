@@ -546,10 +546,11 @@ constexpr int kNone = -1000;  // a lane's power before its first term
 // 16-bit ones go straight to LDS, the next tile's while one's scores and softmax are worked on: the compiler, which cannot tell
 // the two buffers apart, has the transposed reads of one wait for the loads to the other. (With two buffers and two barriers
 // a tile in place of one, FP32's took as long.)
-// 512 FP32 queries over 50,000 rows of 8 heads: 204 us, 257 TFLOP/s, the matrix cores 36% busy and the vector unit 54%; with
-// two waves a SIMD they overlap little (a wave alone issues a vector instruction every seven cycles), and a third wave's
-// registers are not there. 10,007 BF16 rows over themselves with dropout: 365 us, the vector unit 78% busy, half of it
-// with random numbers.
+// 512 FP32 queries over 50,000 rows of 8 heads: 200 to 218 us, 250 TFLOP/s, the matrix cores 36% busy and the vector unit 55%;
+// with two waves a SIMD they overlap little (a wave alone issues a vector instruction every seven cycles), and a third wave's
+// registers are not there. (icl_attention_kernel, eight waves to a workgroup with products and softmax opposite each other,
+// takes 165 for the same products.) 10,007 BF16 rows over themselves with dropout: 361 to 401 us, the vector unit 79% busy,
+// half of it with random numbers.
 constexpr int forward_waves(int element, int wq, int wk) {  // of a SIMD: what registers leave room for
     return element == kTrainF32 ? 2 : wq * wk;
 }
@@ -990,9 +991,10 @@ __global__ __launch_bounds__(256) void train_merge_kernel(const Args a) {
 // in place of 858 for 10,007 BF16 rows). Both compute the scores and dP: seven products in place of five. Five would take
 // either atomic additions to dq, whose order changes results, or dq's part of every 128 keys through memory, written and
 // read (10,007 rows: 1.6 GB each way, 0.6 ms; the two products take 0.2).
-// 10,007 BF16 rows: 765 to 814 us, 630 TFLOP/s counted as five products, 880 as seven; the matrix cores 46% busy, the vector
-// unit 54%. 512 FP32 queries over 50,000 rows: 656 us, 200 (three FP16 products each: 840 as seven); 40% and 52%. Two
-// masked tables of 12,345 rows, FP16 with dropout: 216 to 255; 16% and 52%, random numbers and selections.
+// 10,007 BF16 rows: 771 to 814 us, 630 TFLOP/s counted as five products, 880 as seven; the matrix cores 44% busy, the vector
+// unit 55%. 512 FP32 queries over 50,000 rows: 613 to 667 us, 205 (three FP16 products each: 860 as seven); 38% and 53%. Two
+// masked tables of 12,345 rows, FP16 with dropout: 210 to 265; 15% and 50%. Four tables of 1,024 FP32 rows with dropout: 139
+// to 148; 26% and 47%, with 104 bytes a lane spilled.
 
 // What the backward pass needs of each query: {r, 1 / s, delta, log2 s}; r is +inf (all weights 0) for one that attends to
 // nothing or lies past the length. Sixteen lanes to a row.
@@ -1536,8 +1538,8 @@ int splits_of(double length, double target, long long tiles) {
 
 // Splits of `units` 128-query units over `words` key tiles: as many as take the least time, of those with which the launch is
 // 1, 2, .. 16 workgroups to a compute unit. A workgroup's tile takes so many us beside 0, 1, .. others on its compute unit,
-// and so does the last, partly filled round (10,007 FP32 queries over as many rows in 1 / 2 / 3 / 4 / 5 splits: 959, 802, 822,
-// 792, 829 us; 1,024 over 1,024: 49, 33, 29, 26, 26, in 16 splits 41; four tables of 1,024 BF16 rows: 24, 31, 32, 33, 33). Joining
+// and so does the last, partly filled round (10,007 FP32 queries over as many rows in 1 / 2 / 3 / 4 / 5 splits: 883, 748, 774,
+// 746, 781 us; 1,024 over 1,024: 49, 33, 29, 26, 26, in 16 splits 41; four tables of 1,024 BF16 rows: 24, 31, 32, 33, 33). Joining
 // writes and reads every split's sums. Where only the device knows how much there is to do, the sum of two times: as if every
 // workgroup had everything, and as if half of them had nothing (512 FP32 queries over four masked tables of 20,000 rows: 260 us
 // by the first alone, 234 so; of twelve masked shapes 3% and 6% from the best on average).
