@@ -1023,7 +1023,7 @@ struct Streamed {
     static constexpr int N = scaled(EL) ? 1 : 2;
     Tile<EL> x[N], y[N];
     alignas(16) float r[N][kTile], delta[N][kTile];
-    alignas(16) float logs[scaled(EL) ? 1 : N][kTile];      // 16-bit: log2 s
+    alignas(16) float logs[scaled(EL) ? 1 : N][kTile];  // 16-bit: log2 s
     alignas(16) u32x4 more[N][scaled(EL) ? 1 : kTile];  // 16-bit: what each row's scores and dP take besides
     float coming[scaled(EL) ? kTile : 1];               // the next tile's r
     int fields[2][scaled(EL) ? kTile : 1];  // and exponents
@@ -1194,7 +1194,7 @@ __device__ __forceinline__ unsigned kept_words(unsigned cell, int query, int pai
     return half ? r[0] : mine;
 }
 
-constexpr float kNear = 128.f;
+constexpr float kNear = 128.f;  // references up to here stand as one number with their sums' logarithms (keys_backward)
 
 // The gradients of 32 keys a wave: S = Q K^T, dout V^T, then dout^T P and Q^T dS, over a split's query tiles of every head
 // that shares the keys.
@@ -1227,7 +1227,7 @@ __device__ __forceinline__ void keys_backward(const Args &a, Streamed<EL> &lds, 
     // One turn: queries of the tile at row0 of head h. FP32's r and delta stand beside them. With 16-bit elements one more
     // product of BF16 parts adds -(r + log2 s) / c to the scores (24 bits of it) and, without dropout, -delta to dP: read from
     // LDS for every element, the three take as much of its time as the tiles' operands. Where a reference is past kNear,
-    // 2^-24 of it, several times over, would show beside the weights' own rounding (2^-12 for FP16): such a tile's are read,
+    // 2^-24 of it, several times over, would show beside the weights' own rounding (2^-11 for FP16): such a tile's are read,
     // r taken from the score in one multiplication and addition and log2 s after it (for every tile so: the gradients of 10,007
     // BF16 rows 902 us in place of 806).
     bf16x8 ones[2] = {};
