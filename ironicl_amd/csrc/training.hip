@@ -993,7 +993,7 @@ __global__ __launch_bounds__(256) void train_merge_kernel(const Args a) {
 // read (10,007 rows: 1.6 GB each way, 0.6 ms; the two products take 0.2).
 // 10,007 BF16 rows: 771 to 814 us, 630 TFLOP/s counted as five products, 880 as seven; the matrix cores 44% busy, the vector
 // unit 55%. 512 FP32 queries over 50,000 rows: 613 to 667 us, 205 (three FP16 products each: 860 as seven); 38% and 53%. Two
-// masked tables of 12,345 rows, FP16 with dropout: 210 to 265; 15% and 50%. Four tables of 1,024 FP32 rows with dropout: 139
+// masked tables of 12,345 rows, FP16 with dropout: 197 to 265; 15% and 50%. Four tables of 1,024 FP32 rows with dropout: 139
 // to 148; 26% and 47%, with 104 bytes a lane spilled.
 
 // What the backward pass needs of each query: {r, 1 / s, delta, log2 s}; r is +inf (all weights 0) for one that attends to
